@@ -115,6 +115,20 @@ tg_status tg_step_staged(tg_runtime* rt, int slot, float* loss);
 tg_status tg_run(tg_runtime* rt, int n, const char* const* names, const void* const* data,
                  const int64_t* nbytes, void* out, int64_t out_bytes);
 
+/* Forward-only dispatch within device memory. No counterpart in the reference: it is for
+ * callers whose tensors stay on the GPU (a key/value cache, a gradient, a recurrent state).
+ * The user inputs are read where they are and the graph's outputs, in their order, written
+ * to dev_out; all of them whole allocations or parts of them on the runtime's device,
+ * aligned to 16 bytes, no output overlapping anything else. The work is enqueued on
+ * `stream` (a hipStream_t; NULL: the default stream) and the call returns without waiting:
+ * inputs and outputs must stay as they are until the stream has passed it. Calls on one
+ * runtime and its siblings run one after another, whatever their streams; every other entry
+ * point waits for them first. A stream under graph capture is refused (the runtime's
+ * intermediate buffers would be shared with every later call). */
+tg_status tg_run_device(tg_runtime* rt, int n, const char* const* names, const void* const* dev_data,
+                        const int64_t* nbytes, int n_out, void* const* dev_out, const int64_t* out_bytes,
+                        void* stream);
+
 /* Activation captures of the last step/run (src/runtime.ts:26-75). */
 int tg_capture_count(const tg_runtime* rt);
 const char* tg_capture_name(const tg_runtime* rt, int i);

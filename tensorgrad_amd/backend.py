@@ -27,6 +27,7 @@ EXPORTED = (
     'tg_set_lr', 'tg_describe', 'tg_plan', 'tg_profile_nodes', 'tg_profile_kernels', 'tg_time_replays', 'tg_time_kinds',
     'tg_state_count', 'tg_state_name', 'tg_state_numel', 'tg_download_state', 'tg_upload_state',
     'tg_save_checkpoint', 'tg_load_checkpoint', 'tg_check_checkpoint', 'tg_safetensors_index', 'tg_step_noalloc',
+    'tg_run_device',
 )
 
 
@@ -76,6 +77,8 @@ def lib():
     L.tg_step_device.argtypes = L.tg_step.argtypes
     L.tg_step_noalloc.argtypes = L.tg_step.argtypes
     L.tg_run.argtypes = [vp, ctypes.c_int, c_char_pp, ctypes.POINTER(vp), i64p, vp, ctypes.c_int64]
+    L.tg_run_device.argtypes = [vp, ctypes.c_int, c_char_pp, ctypes.POINTER(vp), i64p, ctypes.c_int, ctypes.POINTER(vp),
+                                i64p, vp]
     L.tg_stage_batch.argtypes = [vp, ctypes.c_int, ctypes.c_int, c_char_pp, ctypes.POINTER(vp), i64p]
     L.tg_step_staged.argtypes = [vp, ctypes.c_int, ctypes.POINTER(ctypes.c_float)]
     L.tg_capture_count.argtypes = [vp]
@@ -237,6 +240,14 @@ class NativeRuntime:
         out = np.empty(out_shape, out_dtype)
         _check(lib().tg_run(self._h, n, names, ptrs, sizes, out.ctypes.data, out.nbytes))
         return out
+
+    def run_device(self, names: Sequence[str], dev_ptrs: Sequence[int], nbytes: Sequence[int], out_ptrs: Sequence[int],
+                   out_nbytes: Sequence[int], stream: int = 0) -> None:
+        """tg_run_device: a forward pass from device memory to device memory on `stream` (a hipStream_t as an int), without
+        waiting for it."""
+        n, m = len(names), len(out_ptrs)
+        _check(lib().tg_run_device(self._h, n, _names(names), (ctypes.c_void_p * n)(*dev_ptrs), (ctypes.c_int64 * n)(*nbytes),
+                                   m, (ctypes.c_void_p * m)(*out_ptrs), (ctypes.c_int64 * m)(*out_nbytes), stream))
 
     def state_names(self) -> List[str]:
         L = lib()

@@ -15,7 +15,7 @@ from __future__ import annotations
 import random
 from collections import OrderedDict
 from dataclasses import dataclass, field
-from typing import Callable, Dict, Optional
+from typing import Callable, Dict, Optional, Sequence
 
 import numpy as np
 
@@ -77,6 +77,32 @@ def _guarded(body, cls):
         return cls('failed', error=e)
 
 
+def _on_device(name: str, x, dtype: str, size: int):
+    """(address, bytes) of a device tensor: contiguous, of the given dtype and element count. Any object with torch's
+    data_ptr / numel / is_contiguous / dtype will do."""
+    if not hasattr(x, 'data_ptr'):
+        raise TypeError(f'run_device: {name} must be a tensor in device memory, got {type(x).__name__}')
+    want = 'torch.float32' if dtype == 'f32' else 'torch.int32'
+    if str(x.dtype) != want:
+        raise TypeError(f'run_device: {name}: expected {want}, got {x.dtype}')
+    if x.numel() != size:
+        raise ValueError(f'run_device: {name}: expected {size} elements, got {x.numel()}')
+    if not x.is_contiguous():
+        raise ValueError(f'run_device: {name} must be contiguous')
+    return x.data_ptr(), 4 * size
+
+
+def _run_device(rt: NativeRuntime, ir: TrainingIR, inputs, outputs, stream: int):
+    g = ir.graph
+    decls = {op['name']: g.tensors[op['out']] for op in g.ops if op['kind'] == 'tensor_input' and op['name'] in inputs}
+    given = [_on_device(f"input '{n}'", inputs[n], t.dtype, t.size) for n, t in decls.items()]
+    outs = [g.tensors[t] for t in g.outputs]
+    if len(outputs) != len(outs):
+        raise ValueError(f'run_device: the graph has {len(outs)} outputs, got {len(outputs)}')
+    to = [_on_device(f'output {i}', x, t.dtype, t.size) for i, (x, t) in enumerate(zip(outputs, outs))]
+    rt.run_device(list(decls), [p for p, _ in given], [n for _, n in given], [p for p, _ in to], [n for _, n in to], stream)
+
+
 def _capture_meta(ir: TrainingIR):
     g = ir.graph
     return {name: (g.tensors[tid].shape, _DT[g.tensors[tid].dtype]) for name, tid in g.captures.items()}
@@ -130,6 +156,20 @@ class CompiledForward:
             rt, ir, shape, dt, meta = self._sibling(inputs)
             out = rt.run(inputs, shape, dt)
             return RunResult('completed', output=out, captures=_read_captures(rt, meta))
+        return _guarded(body, RunResult)
+
+    def run_device(self, inputs: Dict, outputs: Sequence, stream: int = 0) -> RunResult:
+        """`run` within device memory, for tensors that stay on the GPU (no reference counterpart): reads `inputs` (tensors
+        in device memory, by name) and writes the graph's outputs, all that the forward returned, into `outputs`; result
+        `output` is `outputs`. The work is enqueued on `stream` (a hipStream_t as an int; 0: the default stream) and the call
+        returns without waiting for it. Calls on one executor run one after another, also from several streams. A stream
+        under graph capture is refused."""
+        def body():
+            if not self.parent._rt.alive:
+                raise AbortError('run aborted: graph destroyed')
+            rt, ir = self._sibling(inputs)[:2]
+            _run_device(rt, ir, inputs, outputs, stream)
+            return RunResult('completed', output=outputs)
         return _guarded(body, RunResult)
 
     def graph_for(self, inputs) -> TrainingIR:
@@ -322,6 +362,20 @@ class CompiledForwardExecutor:
             return RunResult('completed', output=out, captures=_read_captures(rt, meta))
         return _guarded(body, RunResult)
 
+    def run_device(self, inputs: Dict, outputs: Sequence, stream: int = 0) -> RunResult:
+        """`run` within device memory, for tensors that stay on the GPU (no reference counterpart): reads `inputs` (tensors
+        in device memory, by name) and writes the graph's outputs, all that the forward returned, into `outputs`; result
+        `output` is `outputs`. The work is enqueued on `stream` (a hipStream_t as an int; 0: the default stream) and the call
+        returns without waiting for it. Calls on one executor run one after another, also from several streams. A stream
+        under graph capture is refused."""
+        def body():
+            if self._destroyed:
+                raise AbortError('run aborted: executor destroyed')
+            rt, ir = self._sibling(inputs)[:2]
+            _run_device(rt, ir, inputs, outputs, stream)
+            return RunResult('completed', output=outputs)
+        return _guarded(body, RunResult)
+
     def graph_for(self, inputs) -> TrainingIR:
         return self._sibling(inputs)[1]
 
@@ -371,7 +425,7 @@ def _resolve_decls(decls, inputs: Dict[str, np.ndarray]) -> Dict:
         for d in shape:
             if d is not None:
                 concrete *= d
-        n = np.asarray(inputs[name]).size
+        n = inputs[name].numel() if hasattr(inputs[name], 'numel') else np.asarray(inputs[name]).size
         if n % concrete != 0:
             raise ValueError(f"run: input '{name}' length {n} is not divisible by {concrete}")
         dim = n // concrete

@@ -43,6 +43,7 @@
 #include "jit.h"
 #include "kernels.h"
 #include "safetensors.hpp"
+#include "sequence.h"
 
 // Device scratch of the scratch-only step (tg_step_noalloc): split-K partials, reduction
 // partials, the embedding-gradient sort and the launch-completion counters of one step
@@ -196,6 +197,7 @@ struct Node {
   std::string detail;  // fused groups: member op kinds in program order
   std::string tile;    // products: the kernel that runs them
   bool ws = false;     // bind() reads cur_ws_ / cur_counters_ (rebound for the scratch-only step)
+  bool direct = false; // bind() only reads addresses: run_device binds it to the caller's tensors
   bool partials = false;   // reads column partials another launch of the step writes (in no tensor of `reads`)
   std::function<void(hipStream_t)> launch;   // bound after allocation
   std::function<std::function<void(hipStream_t)>()> bind;
@@ -218,6 +220,9 @@ class Runtime {
   float step(int n, const char* const* names, const void* const* data, const int64_t* nbytes, bool device);
   float step_noalloc(int n, const char* const* names, const void* const* data, const int64_t* nbytes);
   void run(int n, const char* const* names, const void* const* data, const int64_t* nbytes, void* out, int64_t out_bytes);
+  void run_device(int n, const char* const* names, const void* const* data, const int64_t* nbytes, int n_out,
+                  void* const* out, const int64_t* out_bytes, hipStream_t st);
+  void settle();
   void get_capture(const std::string& name, void* out, int64_t nbytes);
   void reset_optimizer();
   void set_lr(const char* json);
@@ -313,6 +318,18 @@ class Runtime {
   std::map<std::string, std::pair<void*, size_t>> table_cache_;   // dev_table copies by key
   const void* dev_table(const std::string& key, const void* data, size_t bytes);
   std::vector<int> state_roots_;
+
+  // Calls that return before their work is done (run_device): a family of runtimes, which share parameters, keeps the event
+  // of its last one. A later one waits for it on its own stream, every other entry point on the host.
+  struct Pending {
+    std::mutex mu;
+    hipEvent_t done = nullptr;
+    bool any = false;
+    ~Pending() { if (done) hipEventDestroy(done); }
+  };
+  std::shared_ptr<Pending> pending_;
+  int device_ = 0;
+  std::vector<std::vector<size_t>> touched_by_;   // per root: nodes that read or write it (made at the first run_device)
 
   // the captured step: [0] user inputs already in the input region, [1] fetched from pinned host memory
   hipGraph_t graph_[2] = {nullptr, nullptr};
@@ -492,6 +509,18 @@ class Runtime {
                     int64_t& bdiv, int64_t& s0, int64_t& s1, int64_t& sr, int64_t& sc, bool transposeOk) const;
   void add_node(Node n) { nodes_.push_back(std::move(n)); }
   void lower_op(int i);
+  // Sequence operators: an op and its siblings (results of the same inputs) run as one node.
+  bool same_fields(int i, int j, std::initializer_list<const char*> names) const;
+  int opt_fld(int op, const char* f) const { const tgj::Value& v = O(op).at(f); return v.null() ? -1 : v.i32(); }
+  tgk::Rows rows_of(int t, const char* what) const;
+  void expect(bool ok, int op, const char* what) const;
+  void mask_fields(int i, Node& n, tgk::AttendDesc& a) const;
+  std::function<tgk::AttendDesc()> attend_binder(int i, const tgk::AttendDesc& d);
+  void lower_attend(int i);
+  void lower_attend_grad(int i);
+  void lower_rope(int i);
+  void lower_scan(int i);
+  void lower_scan_grad(int i);
 
   // GEMMs whose results only the fused optimizer reads (weight gradients) and that would
   // split K run together just before it: one grouped launch per operand-layout kind, with
@@ -629,6 +658,8 @@ Runtime::Runtime(const char* json, Runtime* par, bool plan_only) : parent(par) {
   compute_views();
   lower();
   if (!plan_only) hip_check(hipStreamCreateWithFlags(&stream_, hipStreamNonBlocking), "hipStreamCreate");
+  if (!plan_only) hip_check(hipGetDevice(&device_), "hipGetDevice");
+  pending_ = par ? par->pending_ : std::make_shared<Pending>();
   split_init_nodes();
   allocate();
   bind_all();   // in plan-only mode this still runs every launch's host-side bounds proof
@@ -673,6 +704,7 @@ void Runtime::read_document() {
 }
 
 Runtime::~Runtime() {
+  try { settle(); } catch (...) {}
   for (hipGraphExec_t g : graph_exec_) if (g) hipGraphExecDestroy(g);
   for (hipGraph_t g : graph_) if (g) hipGraphDestroy(g);
   if (stream_) { hipStreamSynchronize(stream_); hipStreamDestroy(stream_); }
@@ -698,6 +730,14 @@ static std::vector<int> op_inputs(const tgj::Value& op) {
       {"conv2d", {"input", "weight"}}, {"conv2d_input_grad", {"weight", "dy"}},
       {"conv2d_weight_grad", {"input", "dy"}}, {"max_pool_2d", {"input"}},
       {"max_pool_2d_grad", {"input", "dy"}},
+      {"attention", {"q", "k", "v", "documents", "prefix", "lengths"}},
+      {"attention_lse", {"q", "k", "v", "documents", "prefix", "lengths"}},
+      {"attention_grad_q", {"q", "k", "v", "y", "lse", "dy", "documents", "prefix", "lengths"}},
+      {"attention_grad_k", {"q", "k", "v", "y", "lse", "dy", "documents", "prefix", "lengths"}},
+      {"attention_grad_v", {"q", "k", "v", "y", "lse", "dy", "documents", "prefix", "lengths"}},
+      {"rope_axes", {"a", "positions"}}, {"linear_recurrence", {"a", "x", "h0"}},
+      {"linear_recurrence_grad_a", {"a", "h", "dh", "h0"}}, {"linear_recurrence_grad_x", {"a", "h", "dh", "h0"}},
+      {"linear_recurrence_grad_h0", {"a", "h", "dh", "h0"}},
       {"param_input", {}}, {"tensor_input", {}}, {"state_input", {}}, {"arange", {}},
       {"const_scalar", {}}, {"const_fill", {}},
   };
@@ -894,6 +934,8 @@ void Runtime::compute_views() {
       if (k == "add" || k == "sub" || k == "mul" || k == "div" || k == "min" || k == "max" || k == "less" ||
           k == "greater" || k == "broadcast_to")
         continue;   // strided element-wise kernels
+      if ((k.compare(0, 9, "attention") == 0 || k == "rope_axes") && v.dims.size() == 4 && v.strides[3] == 1)
+        continue;   // [B, heads, T, D] rows through strides
       return true;
     }
     for (int o : outputs_) if (o == t) return true;
@@ -3645,6 +3687,326 @@ bool Runtime::ready_now(int t) const {
   return false;
 }
 
+// ---- sequence operators ----------------------------------------------------------------------
+
+static bool same_value(const tgj::Value& x, const tgj::Value& y) {
+  if (x.kind != y.kind || x.items.size() != y.items.size()) return false;
+  for (size_t i = 0; i < x.items.size(); ++i) if (!same_value(x.items[i], y.items[i])) return false;
+  return x.boolean == y.boolean && x.number == y.number && x.string == y.string;
+}
+
+bool Runtime::same_fields(int i, int j, std::initializer_list<const char*> names) const {
+  for (const char* f : names) if (!same_value(O(i).at(f), O(j).at(f))) return false;
+  return true;
+}
+
+void Runtime::expect(bool ok, int op, const char* what) const {
+  if (!ok) throw Error(TG_INVALID_ARGUMENT, "IR: " + kinds_[op] + ": " + what);
+}
+
+// A rank-4 tensor as rows, its reach checked against its allocation.
+tgk::Rows Runtime::rows_of(int t, const char* what) const {
+  const View& v = view_[t];
+  if (v.dims.size() != 4 || (v.strides[3] != 1 && v.dims[3] != 1)) throw Error(TG_INTERNAL, std::string(what) + ": not rows");
+  check_span(what, T_[v.root].numel, 0, v.dims.data(), v.strides.data(), 4);
+  return {(float*)dptr(t), v.strides[0], v.strides[1], v.strides[2]};
+}
+
+// Shapes, masks and constants of an attention op, checked; reads q, k, v and the masks.
+void Runtime::mask_fields(int i, Node& n, tgk::AttendDesc& a) const {
+  const tgj::Value& op = O(i);
+  const int q = fld(i, "q"), k = fld(i, "k"), v = fld(i, "v");
+  for (int t : {q, k, v}) {
+    expect(T_[t].dt == F32 && T_[t].shape.size() == 4 && T_[t].numel > 0, i, "q, k and v must be f32 of rank 4");
+    n.reads.push_back(root(t));
+  }
+  const Dims &qs = T_[q].shape, &ks = T_[k].shape, &vs = T_[v].shape;
+  expect(ks[0] == qs[0] && vs[0] == qs[0] && ks[3] == qs[3] && ks[1] == vs[1] && ks[2] == vs[2] && qs[1] % ks[1] == 0, i,
+         "q, k and v do not fit each other");
+  expect(qs[3] <= tgk::kAttendMaxHead && vs[3] <= tgk::kAttendMaxHead, i, "head size above 128");
+  const int64_t lim = int64_t(1) << 31;
+  expect(qs[0] * qs[1] * qs[2] < lim && ks[0] * ks[1] * ks[2] < lim, i, "2^31 or more rows");
+  a.B = (int)qs[0]; a.H = (int)qs[1]; a.Tq = (int)qs[2]; a.D = (int)qs[3];
+  a.Hk = (int)ks[1]; a.Tk = (int)ks[2]; a.Dv = (int)vs[3];
+  a.causal = op.at("causal").boolean;
+  const double scale = op.at("scale").num(), cap = op.at("softcap").null() ? 0 : op.at("softcap").num();
+  expect(scale > 0 && std::isfinite(scale) && cap >= 0 && std::isfinite(cap), i, "scale and softcap must be positive");
+  a.scale = (float)scale;
+  a.cap = (float)cap;
+  const int doc = opt_fld(i, "documents"), pre = opt_fld(i, "prefix"), len = opt_fld(i, "lengths");
+  a.positional = a.causal || doc >= 0 || !op.at("slopes").null();
+  expect(!a.positional || a.Tq <= a.Tk, i, "more queries than positions");
+  expect(op.at("slopes").null() || (int64_t)op.at("slopes").items.size() == a.H, i, "one slope per query head");
+  const std::pair<int, Dims> masks[] = {{doc, {a.B, a.Tk}}, {pre, {a.B}}, {len, {a.B}}};
+  for (const auto& m : masks)
+    if (m.first >= 0) {
+      expect(T_[m.first].dt == I32 && T_[m.first].shape == m.second && view_[m.first].contiguous(), i,
+             "documents must be i32 [B, Tk], prefix and lengths i32 [B]");
+      n.reads.push_back(root(m.first));
+    }
+}
+
+// The descriptor with the addresses of the moment it is called (at bind).
+std::function<tgk::AttendDesc()> Runtime::attend_binder(int i, const tgk::AttendDesc& d) {
+  const int q = fld(i, "q"), k = fld(i, "k"), v = fld(i, "v");
+  const int doc = opt_fld(i, "documents"), pre = opt_fld(i, "prefix"), len = opt_fld(i, "lengths");
+  std::vector<float> slopes;
+  if (!O(i).at("slopes").null()) for (const auto& x : O(i).at("slopes").items) slopes.push_back((float)x.num());
+  return [=]() {
+    tgk::AttendDesc a = d;
+    a.q = rows_of(q, "attention q");
+    a.k = rows_of(k, "attention k");
+    a.v = rows_of(v, "attention v");
+    a.documents = doc >= 0 ? (const int32_t*)dptr(doc) : nullptr;
+    a.prefix = pre >= 0 ? (const int32_t*)dptr(pre) : nullptr;
+    a.lengths = len >= 0 ? (const int32_t*)dptr(len) : nullptr;
+    a.slopes = nullptr;
+    if (!slopes.empty() && !plan_only_)
+      a.slopes = (const float*)dev_table("slopes " + std::to_string(i), slopes.data(), slopes.size() * sizeof(float));
+    return a;
+  };
+}
+
+#define TG_MASKED "q", "k", "v", "documents", "prefix", "lengths", "causal", "scale", "softcap", "slopes"
+
+// attention and attention_lse of the same inputs: one node, whichever comes first in the graph.
+void Runtime::lower_attend(int i) {
+  Node n;
+  n.kind = "attend";
+  n.op = i;
+  n.direct = true;
+  n.detail = kinds_[i];
+  tgk::AttendDesc d{};
+  mask_fields(i, n, d);
+  int y = -1, lse = -1;
+  auto take = [&](int j) { (kinds_[j] == "attention" ? y : lse) = O(j).at("out").i32(); };
+  take(i);
+  for (int j = i + 1; j < (int)ops_.size(); ++j)
+    if ((kinds_[j] == "attention" ? y : kinds_[j] == "attention_lse" ? lse : 0) < 0 && !gemm_done_[j] &&
+        same_fields(i, j, {TG_MASKED})) {
+      take(j);
+      gemm_done_[j] = 1;
+      n.detail += "," + kinds_[j];
+    }
+  if (y >= 0) {
+    expect(T_[y].shape == Dims({d.B, d.H, d.Tq, d.Dv}) && T_[y].dt == F32, i, "bad output shape");
+    n.writes.push_back(root(y));
+  }
+  if (lse >= 0) {
+    expect(T_[lse].shape == Dims({d.B, d.H, d.Tq}) && T_[lse].dt == F32, i, "bad output shape");
+    n.writes.push_back(root(lse));
+  }
+  n.shape = shape_str(T_[fld(i, "q")].shape) + "x" + shape_str(T_[fld(i, "k")].shape);
+  n.flops = 2.0 * d.B * d.H * (double)d.Tq * d.Tk * (d.D + d.Dv);
+  n.bytes = 4.0 * (T_[fld(i, "q")].numel + T_[fld(i, "k")].numel + T_[fld(i, "v")].numel + (y >= 0 ? T_[y].numel : 0));
+  const int64_t ws = tgk::attend_workspace_bytes(d);
+  workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
+  n.ws = ws > 0;
+  auto desc = attend_binder(i, d);
+  n.bind = [=]() -> std::function<void(hipStream_t)> {
+    tgk::AttendDesc a = desc();
+    if (y >= 0) a.y = rows_of(y, "attention y");
+    a.lse = lse >= 0 ? (float*)dptr(lse) : nullptr;
+    void* w = cur_ws_;
+    return [=](hipStream_t st) { tgk::attend(a, w, st); };
+  };
+  add_node(std::move(n));
+}
+
+// The gradients of one attention: one node for those of dq, dk, dv that the graph has.
+void Runtime::lower_attend_grad(int i) {
+  Node n;
+  n.kind = "attend_grad";
+  n.op = i;
+  n.direct = true;
+  tgk::AttendGradDesc g{};
+  mask_fields(i, n, g.a);
+  const tgk::AttendDesc& d = g.a;
+  const int y = fld(i, "y"), lse = fld(i, "lse"), dy = fld(i, "dy");
+  const Dims ys = {d.B, d.H, d.Tq, d.Dv};
+  expect(T_[y].shape == ys && T_[dy].shape == ys && T_[lse].shape == Dims({d.B, d.H, d.Tq}) && T_[y].dt == F32 &&
+             T_[dy].dt == F32 && T_[lse].dt == F32 && view_[lse].contiguous(), i, "y, dy or lse do not fit");
+  for (int t : {y, lse, dy}) n.reads.push_back(root(t));
+  int out[3] = {-1, -1, -1};
+  for (int j = i; j < (int)ops_.size(); ++j) {
+    if (kinds_[j].compare(0, 15, "attention_grad_") != 0 || gemm_done_[j]) continue;
+    if (j != i && !same_fields(i, j, {TG_MASKED, "y", "lse", "dy"})) continue;
+    const int which = kinds_[j].back() == 'q' ? 0 : kinds_[j].back() == 'k' ? 1 : 2;
+    if (out[which] >= 0) continue;
+    out[which] = O(j).at("out").i32();
+    expect(T_[out[which]].shape == T_[fld(j, which == 0 ? "q" : which == 1 ? "k" : "v")].shape && T_[out[which]].dt == F32, j,
+           "bad output shape");
+    gemm_done_[j] = 1;
+    n.writes.push_back(root(out[which]));
+    n.detail += (n.detail.empty() ? "" : ",") + kinds_[j];
+  }
+  n.shape = shape_str(T_[fld(i, "q")].shape) + "x" + shape_str(T_[fld(i, "k")].shape);
+  n.flops = 2.0 * d.B * d.H * (double)d.Tq * d.Tk * (3.0 * d.D + 2.0 * d.Dv);
+  n.bytes = 4.0 * (2.0 * T_[fld(i, "q")].numel + 2.0 * T_[fld(i, "k")].numel + 2.0 * T_[fld(i, "v")].numel + 2.0 * prod(ys));
+  const int dq = out[0], dk = out[1], dv = out[2];
+  // presence decides the workspace; the addresses follow at bind
+  g.dq.p = dq >= 0 ? (float*)16 : nullptr;
+  g.dk.p = dk >= 0 ? (float*)16 : nullptr;
+  g.dv.p = dv >= 0 ? (float*)16 : nullptr;
+  const int64_t ws = tgk::attend_grad_workspace_bytes(g);
+  workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
+  n.ws = ws > 0;
+  auto desc = attend_binder(i, g.a);
+  n.bind = [=]() -> std::function<void(hipStream_t)> {
+    tgk::AttendGradDesc b{};
+    b.a = desc();
+    b.a.y = rows_of(y, "attention y");
+    b.a.lse = (float*)dptr(lse);
+    b.dy = rows_of(dy, "attention dy");
+    if (dq >= 0) b.dq = rows_of(dq, "attention dq");
+    if (dk >= 0) b.dk = rows_of(dk, "attention dk");
+    if (dv >= 0) b.dv = rows_of(dv, "attention dv");
+    void* w = cur_ws_;
+    return [=](hipStream_t st) { tgk::attend_grad(b, w, st); };
+  };
+  add_node(std::move(n));
+}
+
+// Rotations by the same positions whose inputs are there: one node.
+void Runtime::lower_rope(int i) {
+  const tgj::Value& op = O(i);
+  const int pos = fld(i, "positions");
+  const Dims xs = T_[fld(i, "a")].shape;
+  expect(xs.size() == 4 && T_[fld(i, "a")].numel > 0, i, "the input must have rank 4");
+  const double base = op.at("base").num();
+  const bool per_axis = op.at("perAxis").boolean;
+  std::vector<int64_t> sizes;
+  int64_t half = 0;
+  for (const auto& x : op.at("sections").items) {
+    sizes.push_back(x.i64());
+    expect(sizes.back() > 0, i, "sections must be positive");
+    half += sizes.back();
+  }
+  expect(half > 0 && 2 * half <= xs[3] && base > 0 && std::isfinite(base), i, "bad sections or base");
+  expect(T_[pos].dt == I32 && T_[pos].shape == Dims({(int64_t)sizes.size(), xs[0], xs[2]}) && view_[pos].contiguous(), i,
+         "positions must be i32 [axes, B, T]");
+  expect(xs[0] * xs[2] * xs[3] < (int64_t(1) << 31), i, "too large");
+  std::vector<tgk::RopePair> pairs;
+  for (size_t a = 0; a < sizes.size(); ++a)
+    for (int64_t p = 0; p < sizes[a]; ++p) {
+      const double e = per_axis ? (double)p / sizes[a] : (double)pairs.size() / half;
+      pairs.push_back({std::pow(base, -e), (int32_t)a, 0});
+    }
+  Node n;
+  n.kind = "rope";
+  n.op = i;
+  n.direct = true;
+  n.reads.push_back(root(pos));
+  std::vector<int> members;
+  double total = 0;
+  for (int j = i; j < (int)ops_.size() && (int)members.size() < tgk::kRopeMax; ++j) {
+    if (kinds_[j] != "rope_axes" || gemm_done_[j]) continue;
+    const int x = fld(j, "a"), out = O(j).at("out").i32();
+    if (j != i && (!same_fields(i, j, {"positions", "sections", "base", "perAxis"}) || !ready_now(x))) continue;
+    const Dims& js = T_[x].shape;
+    expect(T_[x].dt == F32 && js.size() == 4 && js[0] == xs[0] && js[2] == xs[2] && js[3] == xs[3] && T_[x].numel > 0 &&
+               T_[out].shape == js && T_[out].dt == F32, j, "tensors turned by the same positions must agree in shape");
+    members.push_back(j);
+    gemm_done_[j] = 1;
+    n.reads.push_back(root(x));
+    n.writes.push_back(root(out));
+    n.detail += (n.detail.empty() ? "" : ",") + kinds_[j];
+    total += T_[x].numel;
+  }
+  n.shape = shape_str(xs) + " x" + std::to_string(members.size());
+  n.flops = 3.0 * total;
+  n.bytes = 8.0 * total + 4.0 * T_[pos].numel;
+  const std::string key = "rope " + std::to_string(i);
+  n.bind = [=]() -> std::function<void(hipStream_t)> {
+    tgk::RopeDesc r{};
+    r.B = (int)xs[0]; r.T = (int)xs[2]; r.D = (int)xs[3]; r.half = (int)half; r.n = (int)members.size();
+    r.positions = (const int32_t*)dptr(pos);
+    if (!plan_only_) r.pairs = (const tgk::RopePair*)dev_table(key, pairs.data(), pairs.size() * sizeof(tgk::RopePair));
+    for (int m = 0; m < r.n; ++m) {
+      const int x = fld(members[m], "a"), out = O(members[m]).at("out").i32();
+      r.x[m] = rows_of(x, "rope input");
+      r.y[m] = rows_of(out, "rope output");
+      r.heads[m] = (int)T_[x].shape[1];
+      r.inverse[m] = O(members[m]).at("inverse").boolean;
+    }
+    return [=](hipStream_t st) { tgk::rope(r, st); };
+  };
+  add_node(std::move(n));
+}
+
+void Runtime::lower_scan(int i) {
+  const int a = fld(i, "a"), x = fld(i, "x"), h0 = opt_fld(i, "h0"), h = O(i).at("out").i32();
+  const Dims s = T_[a].shape;
+  expect(s.size() == 3 && T_[a].numel > 0 && T_[x].shape == s && T_[h].shape == s && T_[a].dt == F32 && T_[x].dt == F32 &&
+             T_[h].dt == F32 && (h0 < 0 || (T_[h0].shape == Dims({s[0], s[2]}) && T_[h0].dt == F32)), i,
+         "a and x must be f32 [B, T, C], h0 f32 [B, C]");
+  Node n;
+  n.kind = "scan";
+  n.op = i;
+  n.direct = true;
+  n.shape = shape_str(s);
+  for (int t : {a, x, h0}) if (t >= 0) {
+    if (!view_[t].contiguous()) throw Error(TG_INTERNAL, "linear_recurrence needs contiguous operands");
+    n.reads.push_back(root(t));
+  }
+  n.writes.push_back(root(h));
+  n.flops = 2.0 * T_[a].numel;
+  n.bytes = 12.0 * T_[a].numel;
+  const int64_t ws = tgk::scan_workspace_bytes(s[0], s[1], s[2]);
+  workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
+  n.ws = ws > 0;
+  n.bind = [=]() -> std::function<void(hipStream_t)> {
+    tgk::ScanDesc d{s[0], s[1], s[2], (const float*)dptr(a), (const float*)dptr(x), h0 >= 0 ? (const float*)dptr(h0) : nullptr,
+                    (float*)dptr(h)};
+    void* w = cur_ws_;
+    return [=](hipStream_t st) { tgk::scan(d, w, st); };
+  };
+  add_node(std::move(n));
+}
+
+void Runtime::lower_scan_grad(int i) {
+  const int a = fld(i, "a"), h = fld(i, "h"), dh = fld(i, "dh"), h0 = opt_fld(i, "h0");
+  const Dims s = T_[a].shape;
+  expect(s.size() == 3 && T_[a].numel > 0 && T_[h].shape == s && T_[dh].shape == s && T_[a].dt == F32 && T_[h].dt == F32 &&
+             T_[dh].dt == F32 && (h0 < 0 || (T_[h0].shape == Dims({s[0], s[2]}) && T_[h0].dt == F32)), i,
+         "a, h and dh must be f32 [B, T, C], h0 f32 [B, C]");
+  Node n;
+  n.kind = "scan_grad";
+  n.op = i;
+  n.direct = true;
+  n.shape = shape_str(s);
+  for (int t : {a, h, dh, h0}) if (t >= 0) {
+    if (!view_[t].contiguous()) throw Error(TG_INTERNAL, "linear_recurrence gradient needs contiguous operands");
+    n.reads.push_back(root(t));
+  }
+  int out[3] = {-1, -1, -1};
+  for (int j = i; j < (int)ops_.size(); ++j) {
+    if (kinds_[j].compare(0, 23, "linear_recurrence_grad_") != 0 || gemm_done_[j]) continue;
+    if (j != i && !same_fields(i, j, {"a", "h", "dh", "h0"})) continue;
+    const int which = kinds_[j].back() == 'a' ? 0 : kinds_[j].back() == 'x' ? 1 : 2;
+    if (out[which] >= 0) continue;
+    out[which] = O(j).at("out").i32();
+    expect(T_[out[which]].shape == (which == 2 ? Dims({s[0], s[2]}) : s) && T_[out[which]].dt == F32, j, "bad output shape");
+    gemm_done_[j] = 1;
+    n.writes.push_back(root(out[which]));
+    n.detail += (n.detail.empty() ? "" : ",") + kinds_[j];
+  }
+  const int da = out[0], dx = out[1], dh0 = out[2];
+  n.flops = 3.0 * T_[a].numel;
+  n.bytes = 4.0 * T_[a].numel * (3 + (da >= 0) + (dx >= 0));
+  const int64_t ws = tgk::scan_workspace_bytes(s[0], s[1], s[2]);
+  workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
+  n.ws = ws > 0;
+  n.bind = [=]() -> std::function<void(hipStream_t)> {
+    auto in = [&](int t) { return t >= 0 ? (const float*)dptr(t) : nullptr; };
+    auto to = [&](int t) { return t >= 0 ? (float*)dptr(t) : nullptr; };
+    tgk::ScanGradDesc d{s[0], s[1], s[2], in(a), in(h), in(dh), in(h0), to(da), to(dx), to(dh0)};
+    void* w = cur_ws_;
+    return [=](hipStream_t st) { tgk::scan_grad(d, w, st); };
+  };
+  add_node(std::move(n));
+}
+
 void Runtime::lower_op(int i) {
   const std::string& k = kinds_[i];
   const tgj::Value& op = O(i);
@@ -4323,6 +4685,21 @@ void Runtime::lower_op(int i) {
       const float* pd = (const float*)dptr(dy);
       return [=](hipStream_t st) { tgk::max_pool_grad(px, pd, po, p, st, relu); };
     };
+  } else if (k == "attention" || k == "attention_lse") {
+    lower_attend(i);
+    return;
+  } else if (k.compare(0, 15, "attention_grad_") == 0) {
+    lower_attend_grad(i);
+    return;
+  } else if (k == "rope_axes") {
+    lower_rope(i);
+    return;
+  } else if (k == "linear_recurrence") {
+    lower_scan(i);
+    return;
+  } else if (k.compare(0, 23, "linear_recurrence_grad_") == 0) {
+    lower_scan_grad(i);
+    return;
   } else if (k == "adam_update_m" || k == "adam_update_v" || k == "adam_update_p") {
     throw Error(TG_INTERNAL, "adam op outside the fused update");
   } else {
@@ -4774,6 +5151,148 @@ void Runtime::run(int n, const char* const* names, const void* const* data, cons
   if (!view_[o].contiguous()) throw Error(TG_INTERNAL, "run: output is not contiguous");
   hip_check(hipMemcpyAsync(out, dptr(o), (size_t)out_bytes, hipMemcpyDeviceToHost, stream_), "hipMemcpyAsync(D2H)");
   hip_check(hipStreamSynchronize(stream_), "hipStreamSynchronize");
+}
+
+// Waits on the host for the family's last run_device.
+void Runtime::settle() {
+  if (!pending_) return;
+  std::lock_guard<std::mutex> g(pending_->mu);
+  if (!pending_->any) return;
+  pending_->any = false;
+  hip_check(hipEventSynchronize(pending_->done), "hipEventSynchronize");
+}
+
+// One forward pass on the caller's stream, from and to the caller's device memory. Nodes that can take any addresses
+// (direct) are bound to the caller's tensors for this call; the others run on the runtime's own buffers, with copies on the
+// same stream before and after. Returns without waiting.
+void Runtime::run_device(int n, const char* const* names, const void* const* data, const int64_t* nbytes, int n_out,
+                         void* const* out, const int64_t* out_bytes, hipStream_t st) {
+  if (opt_cfg_) throw Error(TG_INVALID_ARGUMENT, "run_device: a training graph (use step)");
+  int dev = 0;
+  hip_check(hipGetDevice(&dev), "hipGetDevice");
+  struct Current {   // the runtime's device for the call's duration
+    int back = -1;
+    ~Current() { if (back >= 0) hipSetDevice(back); }
+  } current;
+  if (dev != device_) {
+    hip_check(hipSetDevice(device_), "hipSetDevice");
+    current.back = dev;
+  }
+  if (st) {
+    int of = device_;
+    hip_check(hipStreamGetDevice(st, &of), "hipStreamGetDevice");
+    if (of != device_) throw Error(TG_INVALID_ARGUMENT, "run_device: the stream belongs to another device");
+  }
+  // A capture would record the runtime's intermediate buffers, which every other call on it uses too.
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(st, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone) {
+    (void)hipGetLastError();
+    throw Error(TG_INVALID_ARGUMENT, "run_device: the stream is being captured into a graph");
+  }
+  struct Span { const char* lo; const char* hi; bool write; std::string name; };
+  std::vector<Span> spans;
+  auto span = [&](const void* p, int64_t bytes, int64_t want, bool write, const std::string& name) {
+    if (bytes != want)
+      throw Error(TG_INVALID_ARGUMENT, name + ": expected " + std::to_string(want) + " bytes, got " + std::to_string(bytes));
+    hipPointerAttribute_t at{};
+    hipDeviceptr_t base = nullptr;
+    size_t size = 0;
+    if (!p || hipPointerGetAttributes(&at, p) != hipSuccess || at.type != hipMemoryTypeDevice || at.device != device_ ||
+        hipMemGetAddressRange(&base, &size, const_cast<void*>(p)) != hipSuccess ||
+        (const char*)p + bytes > (const char*)base + size) {
+      (void)hipGetLastError();
+      throw Error(TG_INVALID_ARGUMENT, name + ": not " + std::to_string(bytes) + " bytes of this device's memory");
+    }
+    if ((uintptr_t)p % 16) throw Error(TG_INVALID_ARGUMENT, name + ": must be aligned to 16 bytes");
+    spans.push_back({(const char*)p, (const char*)p + bytes, write, name});
+  };
+  std::map<int, const void*> given;
+  for (int i = 0; i < n; ++i) {
+    auto it = input_tid_.find(names[i]);
+    if (it == input_tid_.end() || input_offset_[it->second] >= user_bytes_) continue;   // as in upload_inputs
+    if (!given.emplace(it->second, data[i]).second) throw Error(TG_INVALID_ARGUMENT, std::string("input '") + names[i] + "' given twice");
+    span(data[i], nbytes[i], T_[it->second].numel * 4, false, std::string("input '") + names[i] + "'");
+  }
+  for (auto& kv : input_tid_)
+    if (input_offset_[kv.second] < user_bytes_ && !given.count(kv.second))
+      throw Error(TG_INVALID_ARGUMENT, "missing input '" + kv.first + "'");
+  if (n_out != (int)outputs_.size())
+    throw Error(TG_INVALID_ARGUMENT, "run_device: the graph has " + std::to_string(outputs_.size()) + " outputs, got " + std::to_string(n_out));
+  for (int o = 0; o < n_out; ++o) span(out[o], out_bytes[o], T_[outputs_[o]].numel * 4, true, "output " + std::to_string(o));
+  for (size_t x = 0; x < spans.size(); ++x)
+    for (size_t y = 0; y < x; ++y)
+      if ((spans[x].write || spans[y].write) && spans[x].lo < spans[y].hi && spans[y].lo < spans[x].hi)
+        throw Error(TG_INVALID_ARGUMENT, "run_device: " + spans[y].name + " and " + spans[x].name + " overlap");
+
+  if (touched_by_.empty()) {
+    touched_by_.resize(T_.size());
+    for (size_t i = 0; i < nodes_.size(); ++i) {
+      std::set<int> roots(nodes_[i].reads.begin(), nodes_[i].reads.end());
+      roots.insert(nodes_[i].writes.begin(), nodes_[i].writes.end());
+      for (int r : roots) touched_by_[r].push_back(i);
+    }
+  }
+  auto all_direct = [&](int r) {
+    for (size_t i : touched_by_[r]) if (!nodes_[i].direct) return false;
+    return true;
+  };
+  // The family's earlier calls use the same buffers (this runtime's) or parameters: wait for them on the stream. The seed
+  // goes through pinned memory that the last call may still read: wait on the host.
+  std::unique_lock<std::mutex> lock(pending_->mu);
+  if (!pending_->done) hip_check(hipEventCreateWithFlags(&pending_->done, hipEventDisableTiming), "hipEventCreate");
+  if (pending_->any) {
+    if (uses_prng_) hip_check(hipEventSynchronize(pending_->done), "hipEventSynchronize");
+    else hip_check(hipStreamWaitEvent(st, pending_->done, 0), "hipStreamWaitEvent");
+  }
+  advance_scalars(false);
+
+  std::vector<std::pair<int, void*>> saved;   // root -> its own address, put back below
+  std::set<size_t> rebind;
+  auto point = [&](int r, const void* p) {
+    saved.emplace_back(r, ptr_[r]);
+    ptr_[r] = const_cast<void*>(p);
+    rebind.insert(touched_by_[r].begin(), touched_by_[r].end());
+  };
+  auto put_back = [&] { for (auto it = saved.rbegin(); it != saved.rend(); ++it) ptr_[it->first] = it->second; };
+  std::vector<std::pair<int, int>> copies;    // output index, tensor
+  try {
+    std::set<int> pinned;                     // roots that must keep their own storage
+    for (auto& c : captures_) pinned.insert(root(c.second));
+    for (auto& w : copy_writebacks_) pinned.insert(root(w.first));
+    for (auto& g : given) {
+      if (all_direct(g.first) && !pinned.count(g.first)) point(g.first, g.second);
+      else tgk::copy_words(ptr_[g.first], g.second, T_[g.first].numel * 4, st);
+    }
+    for (int o = 0; o < n_out; ++o) {
+      const int t = outputs_[o], r = root(t);
+      if (!view_[t].contiguous()) throw Error(TG_INTERNAL, "run_device: output is not contiguous");
+      const bool made = !init_roots_.count(r) && !is_leaf(T_[r].src) && T_[r].numel == T_[t].numel;
+      if (made && all_direct(r) && pinned.insert(r).second) point(r, out[o]);
+      else copies.emplace_back(o, t);
+    }
+    if (uses_prng_)
+      tgk::copy_words(input_region_ + user_bytes_, staging_ + user_bytes_, (int64_t)(input_region_bytes_ - user_bytes_), st);
+    cur_ws_ = workspace_;
+    cur_counters_ = counters_;
+    for (size_t i = 0; i < nodes_.size(); ++i) {
+      if (rebind.count(i)) nodes_[i].bind()(st);
+      else nodes_[i].launch(st);
+    }
+    apply_copy_writebacks(st);
+    for (auto& c : copies) tgk::copy_words(out[c.first], dptr(c.second), out_bytes[c.first], st);
+    hip_check(hipGetLastError(), "run_device launch");
+  } catch (...) {
+    put_back();
+    cur_ws_ = nullptr;
+    cur_counters_ = nullptr;
+    if (hipEventRecord(pending_->done, st) == hipSuccess) pending_->any = true;
+    throw;
+  }
+  put_back();
+  cur_ws_ = nullptr;
+  cur_counters_ = nullptr;
+  hip_check(hipEventRecord(pending_->done, st), "hipEventRecord");
+  pending_->any = true;
 }
 
 void Runtime::get_capture(const std::string& name, void* out, int64_t nbytes) {
@@ -5234,10 +5753,14 @@ void tg_destroy(tg_runtime* h) {
   destroy_rec(h);
 }
 
-#define TG_ENTER(h)                                                       \
+// Enters a call on h; the host first waits for work that an earlier tg_run_device of the family left running.
+#define TG_ENTER_RUNNING(h)                                               \
   if (!live(h)) { tg::g_error = "graph destroyed"; return TG_ABORTED; } \
   std::lock_guard<std::mutex> lk_((h)->mu);                               \
   if (!(h)->rt) { tg::g_error = "graph destroyed"; return TG_ABORTED; }
+#define TG_ENTER(h)                                                       \
+  TG_ENTER_RUNNING(h)                                                     \
+  if (tg_status s_ = guarded([&] { (h)->rt->settle(); })) return s_;
 
 int tg_param_count(const tg_runtime* h) {
   return if_live(h, 0, [](const tg::Runtime& r) { return (int)r.param_names.size(); });
@@ -5296,6 +5819,18 @@ tg_status tg_run(tg_runtime* h, int n, const char* const* names, const void* con
                  void* out, int64_t out_bytes) {
   TG_ENTER(h);
   return guarded([&] { h->rt->run(n, names, data, nbytes, out, out_bytes); });
+}
+
+tg_status tg_run_device(tg_runtime* h, int n, const char* const* names, const void* const* dev_data, const int64_t* nbytes,
+                        int n_out, void* const* dev_out, const int64_t* out_bytes, void* stream) {
+  TG_ENTER_RUNNING(h);
+  if (n < 0 || n_out < 0 || (n && (!names || !dev_data || !nbytes)) || (n_out && (!dev_out || !out_bytes))) {
+    tg::g_error = "null argument";
+    return TG_INVALID_ARGUMENT;
+  }
+  return guarded([&] {
+    h->rt->run_device(n, names, dev_data, nbytes, n_out, dev_out, out_bytes, static_cast<hipStream_t>(stream));
+  });
 }
 
 int tg_capture_count(const tg_runtime* h) {

@@ -253,6 +253,21 @@ def _adjoint(op: dict, oc: Tensor, graph: Graph, cot: Dict[int, Tensor]) -> None
         x = T(op['input'])
         acc(op['input'], O.max_pool2d_grad(x, oc, op['kH'], op['kW'], op['strideH'], op['strideW'],
                                            op['padH'], op['padW']))
+    elif k == 'attention':
+        opt = lambda n: None if op[n] is None else T(op[n])  # noqa: E731
+        grads = O.attention_grad(T(op['q']), T(op['k']), T(op['v']), T(op['out']), oc, op['causal'], op['scale'],
+                                 op['softcap'], op['slopes'], opt('documents'), opt('prefix'), opt('lengths'))
+        for n, c in zip('qkv', grads):
+            acc(op[n], c)
+    elif k == 'rope_axes':
+        acc(op['a'], O._rope_axes(oc, T(op['positions']), op['sections'], op['base'], op['perAxis'], not op['inverse']))
+    elif k == 'linear_recurrence':
+        h0 = None if op['h0'] is None else T(op['h0'])
+        grads = O.linear_recurrence_grad(T(op['a']), T(op['out']), oc, h0)
+        for n, c in zip(('a', 'x', 'h0'), grads):
+            acc(op[n], c)
+    elif k == 'attention_lse' or k.startswith(('attention_grad_', 'linear_recurrence_grad_')):
+        raise ValueError(f"autograd: cannot differentiate through {k} (it's a backward op)")
     elif k in ('conv2d_input_grad', 'conv2d_weight_grad', 'max_pool_2d_grad', 'scatter_axis'):
         raise ValueError(f"autograd: cannot differentiate through {k} (it's a backward op)")
     elif k == 'relu_grad':

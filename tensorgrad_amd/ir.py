@@ -100,6 +100,24 @@ _INPUT_FIELDS.update({
 
 OP_KINDS = tuple(_INPUT_FIELDS.keys())
 
+# Kinds of this framework that the reference's union does not have: sequence operators with
+# their gradients. Masks and initial states are optional inputs (None where absent).
+_MASKS = ('documents', 'prefix', 'lengths')
+_EXTENSIONS: Dict[str, Tuple[str, ...]] = {
+    'attention': ('q', 'k', 'v') + _MASKS,
+    'attention_lse': ('q', 'k', 'v') + _MASKS,
+    'attention_grad_q': ('q', 'k', 'v', 'y', 'lse', 'dy') + _MASKS,
+    'attention_grad_k': ('q', 'k', 'v', 'y', 'lse', 'dy') + _MASKS,
+    'attention_grad_v': ('q', 'k', 'v', 'y', 'lse', 'dy') + _MASKS,
+    'rope_axes': ('a', 'positions'),
+    'linear_recurrence': ('a', 'x', 'h0'),
+    'linear_recurrence_grad_a': ('a', 'h', 'dh', 'h0'),
+    'linear_recurrence_grad_x': ('a', 'h', 'dh', 'h0'),
+    'linear_recurrence_grad_h0': ('a', 'h', 'dh', 'h0'),
+}
+_INPUT_FIELDS.update(_EXTENSIONS)
+EXTENSION_KINDS = tuple(_EXTENSIONS)
+
 
 def input_fields(kind: str) -> Tuple[str, ...]:
     try:
@@ -110,7 +128,8 @@ def input_fields(kind: str) -> Tuple[str, ...]:
 
 def remap_op_inputs(op: dict, f: Callable[[int], int]) -> dict:
     """Copy of `op` with every input tensor id passed through `f` (ir.ts:356-395).
-    `decayShrinkTensor` may be None (literal decayShrink) and is then left alone."""
+    `decayShrinkTensor` may be None (literal decayShrink), as may an extension's optional
+    inputs; they are then left alone."""
     out = dict(op)
     for name in input_fields(op['kind']):
         v = op[name]

@@ -542,6 +542,146 @@ def rope(q: Tensor, k: Tensor, base: float = 10000) -> Tuple[Tensor, Tensor]:
     return apply_rot(q), apply_rot(k)
 
 
+# ---- Sequence operators (no reference counterpart) ---------------------------------------------------
+
+ATTENTION_MAX_HEAD = 128   # the kernels' tiles hold whole heads
+
+
+def _finite(x) -> bool:
+    return _num(x) and math.isfinite(x)
+
+
+def _attention_fields(site: str, q: Tensor, k: Tensor, v: Tensor, causal, scale, softcap, slopes, documents, prefix,
+                      lengths) -> dict:
+    for name, t in (('q', q), ('k', k), ('v', v)):
+        if t.dtype != 'f32':
+            raise ShapeError(f'{site}: {name} must be f32, got {t.dtype}', site)
+        if len(t.shape) != 4:
+            raise ShapeError(f'{site}: {name} must be [batch, heads, length, head size], got {S.show(t.shape)}', site)
+    B, H, Tq, D = q.shape
+    _, Hk, Tk, Dv = v.shape
+    if min(B, H, Tq, D, Hk, Tk, Dv) < 1:
+        raise ShapeError(f'{site}: empty operand', site)
+    if k.shape != (B, Hk, Tk, D) or v.shape[0] != B:
+        raise ShapeError(f'{site}: q {S.show(q.shape)}, k {S.show(k.shape)} and v {S.show(v.shape)} must agree in batch, '
+                         'q and k in head size, k and v in heads and length', site)
+    if H % Hk != 0:
+        raise ShapeError(f'{site}: {H} query heads cannot share {Hk} key heads evenly', site)
+    if D > ATTENTION_MAX_HEAD or Dv > ATTENTION_MAX_HEAD:
+        raise ShapeError(f'{site}: head sizes above {ATTENTION_MAX_HEAD} are not supported, got {D} and {Dv}', site)
+    positional = causal or slopes is not None or documents is not None
+    if positional and Tq > Tk:
+        raise ShapeError(f'{site}: {Tq} queries are not the last of {Tk} positions', site)
+    if scale is None:
+        scale = 1 / math.sqrt(D)
+    if not _finite(scale) or scale <= 0:
+        raise ShapeError(f'{site}: scale must be positive, got {scale}', site)
+    if softcap is not None and (not _finite(softcap) or softcap <= 0):
+        raise ShapeError(f'{site}: softcap must be positive, got {softcap}', site)
+    if slopes is not None:
+        slopes = [float(x) for x in slopes] if all(_finite(x) for x in slopes) else None
+        if slopes is None or len(slopes) != H:
+            raise ShapeError(f'{site}: slopes must be {H} finite numbers, one per query head', site)
+    if prefix is not None and not causal:
+        raise ShapeError(f'{site}: a prefix needs a causal mask', site)
+    for name, t, shape in (('documents', documents, (B, Tk)), ('prefix', prefix, (B,)), ('lengths', lengths, (B,))):
+        if t is not None and (t.dtype != 'i32' or t.shape != shape):
+            raise ShapeError(f'{site}: {name} must be i32 {S.show(shape)}, got {t.dtype} {S.show(t.shape)}', site)
+    ids = {n: None if t is None else t.id for n, t in (('documents', documents), ('prefix', prefix), ('lengths', lengths))}
+    return {'q': q.id, 'k': k.id, 'v': v.id, **ids, 'causal': bool(causal), 'scale': scale, 'softcap': softcap, 'slopes': slopes}
+
+
+def attention(q: Tensor, k: Tensor, v: Tensor, causal: bool = True, scale: Optional[float] = None,
+              softcap: Optional[float] = None, slopes: Optional[Sequence[float]] = None, documents: Optional[Tensor] = None,
+              prefix: Optional[Tensor] = None, lengths: Optional[Tensor] = None) -> Tensor:
+    """Attention of q [B, H, Tq, D] over k [B, Hk, Tk, D], v [B, Hk, Tk, Dv] -> [B, H, Tq, Dv]. Query head h reads key head
+    h // (H / Hk). With x = scale q.k (scale: 1 / sqrt(D)), the score of key j for a query at position p is
+
+        softcap tanh(x / softcap) - slopes[h] |p - j|        (each part where it is given)
+
+    `lengths` i32 [B]: only the first lengths[b] keys are there (clamped to 0..Tk; without it all Tk). The queries are the
+    last Tq of those positions, so one new token against a filled cache is Tq = 1. `causal` hides keys after p, except those
+    below `prefix` i32 [B], which every query sees. `documents` i32 [B, Tk]: a query sees the keys of its own document (that
+    at its position); negative ids are padding, which sees and is seen by nothing. A query that sees no key (or, where
+    positions matter, lies before position 0) gives zeros and takes and gives no gradient. What a mask hides has no
+    influence, whatever its values (infinities and NaN included)."""
+    f = _attention_fields('attention', q, k, v, causal, scale, softcap, slopes, documents, prefix, lengths)
+    return add_op(current_graph(), 'attention', (*q.shape[:3], v.shape[3]), 'f32', 'attention', f)
+
+
+def attention_grad(q: Tensor, k: Tensor, v: Tensor, y: Tensor, dy: Tensor, causal: bool = True, scale: Optional[float] = None,
+                   softcap: Optional[float] = None, slopes: Optional[Sequence[float]] = None,
+                   documents: Optional[Tensor] = None, prefix: Optional[Tensor] = None,
+                   lengths: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dq, dk, dv) of y = attention(q, k, v, ...) for the gradient dy of y; the other arguments as given there."""
+    site = 'attentionGrad'
+    f = _attention_fields(site, q, k, v, causal, scale, softcap, slopes, documents, prefix, lengths)
+    shape = (*q.shape[:3], v.shape[3])
+    for name, t in (('y', y), ('dy', dy)):
+        if t.dtype != 'f32' or t.shape != shape:
+            raise ShapeError(f'{site}: {name} must be f32 {S.show(shape)}, got {t.dtype} {S.show(t.shape)}', site)
+    g = current_graph()
+    lse = add_op(g, 'attention_lse', q.shape[:3], 'f32', site, f)
+    f = dict(f, y=y.id, lse=lse.id, dy=dy.id)
+    return tuple(add_op(g, f'attention_grad_{n}', t.shape, 'f32', site, f) for n, t in (('q', q), ('k', k), ('v', v)))
+
+
+def rope_axes(q: Tensor, k: Tensor, positions: Tensor, sections: Sequence[int], base: float = 10000, per_axis: bool = False,
+              inverse: bool = False) -> Tuple[Tensor, Tensor]:
+    """Rotary embedding by positions of several axes (time, height, width; one axis: given positions), rotate-half
+    convention as `rope`. q [B, H, T, D], k [B, Hk, T, D], positions i32 [A, B, T]; `sections` gives each axis its number of
+    pairs, laid end to end: with half = sum(sections), pair p is (x[p], x[p + half]), features from 2 half on pass
+    unchanged. A pair of axis a turns by positions[a] * base^(-p / half), with `per_axis` by
+    positions[a] * base^(-(p - first pair of a) / sections[a]). `inverse` turns back (the gradient)."""
+    site = 'ropeAxes'
+    for name, t in (('q', q), ('k', k)):
+        if t.dtype != 'f32' or len(t.shape) != 4 or min(t.shape) < 1:
+            raise ShapeError(f'{site}: {name} must be f32 [batch, heads, length, head size], got {t.dtype} {S.show(t.shape)}', site)
+    B, _, T, D = q.shape
+    if (k.shape[0], k.shape[2], k.shape[3]) != (B, T, D):
+        raise ShapeError(f'{site}: q {S.show(q.shape)} and k {S.show(k.shape)} must agree in batch, length and head size', site)
+    sections = list(sections)
+    if not sections or not all(isinstance(n, int) and not isinstance(n, bool) and n > 0 for n in sections) or 2 * sum(sections) > D:
+        raise ShapeError(f'{site}: sections must be positive pair counts of at most {D // 2} in all, got {sections}', site)
+    if positions.dtype != 'i32' or positions.shape != (len(sections), B, T):
+        raise ShapeError(f'{site}: positions must be i32 {S.show((len(sections), B, T))}, got {positions.dtype} '
+                         f'{S.show(positions.shape)}', site)
+    if not _finite(base) or base <= 0:
+        raise ShapeError(f'{site}: base must be positive, got {base}', site)
+    return tuple(_rope_axes(x, positions, sections, base, bool(per_axis), bool(inverse)) for x in (q, k))
+
+
+def _rope_axes(x: Tensor, positions: Tensor, sections, base, per_axis: bool, inverse: bool) -> Tensor:
+    return add_op(current_graph(), 'rope_axes', x.shape, 'f32', 'ropeAxes', {
+        'a': x.id, 'positions': positions.id, 'sections': list(sections), 'base': base, 'perAxis': per_axis, 'inverse': inverse})
+
+
+def _recurrence_check(site: str, a: Tensor, h0: Optional[Tensor], **others: Tensor) -> None:
+    for name, t in (('a', a), *others.items()):
+        if t.dtype != 'f32' or len(t.shape) != 3 or min(t.shape) < 1 or t.shape != a.shape:
+            raise ShapeError(f'{site}: {name} must be f32 [batch, length, channels] like a {S.show(a.shape)}, got {t.dtype} '
+                             f'{S.show(t.shape)}', site)
+    if h0 is not None and (h0.dtype != 'f32' or h0.shape != (a.shape[0], a.shape[2])):
+        raise ShapeError(f'{site}: h0 must be f32 [batch, channels] for a {S.show(a.shape)}, got {h0.dtype} {S.show(h0.shape)}', site)
+
+
+def linear_recurrence(a: Tensor, x: Tensor, h0: Optional[Tensor] = None) -> Tensor:
+    """Gated linear recurrence h[:, t] = a[:, t] h[:, t-1] + x[:, t] over [B, T, C], each channel by itself, from h0 [B, C]
+    (zeros without it). A gate of 0 starts afresh (the first position of a packed document)."""
+    _recurrence_check('linearRecurrence', a, h0, x=x)
+    return add_op(current_graph(), 'linear_recurrence', a.shape, 'f32', 'linearRecurrence',
+                  {'a': a.id, 'x': x.id, 'h0': None if h0 is None else h0.id})
+
+
+def linear_recurrence_grad(a: Tensor, h: Tensor, dh: Tensor, h0: Optional[Tensor] = None) -> Tuple[Tensor, ...]:
+    """(da, dx), with h0 (da, dx, dh0), of h = linear_recurrence(a, x, h0) for the gradient dh of h."""
+    site = 'linearRecurrenceGrad'
+    _recurrence_check(site, a, h0, h=h, dh=dh)
+    f = {'a': a.id, 'h': h.id, 'dh': dh.id, 'h0': None if h0 is None else h0.id}
+    outs = (('a', a.shape), ('x', a.shape)) + ((('h0', h0.shape),) if h0 is not None else ())
+    return tuple(add_op(current_graph(), f'linear_recurrence_grad_{n}', s, 'f32', site, f) for n, s in outs)
+
+
 # ---- Broadcast / constants / comparisons (ops.ts:943-1008) -----------------------------------------
 
 def broadcast_to(a: Tensor, target: Sequence[int]) -> Tensor:

@@ -1,0 +1,515 @@
+"""The sequence operators on the GPU against 64 bits, at the sizes and masks where they can go wrong."""
+import numpy as np
+import pytest
+import torch
+
+import _sequence as R
+from tensorgrad_amd import backend, nn
+from tensorgrad_amd import ir as IR
+from tensorgrad_amd import ops as O
+from tensorgrad_amd.compile import compile as tg_compile
+from tensorgrad_amd.compile import compile_forward
+from tensorgrad_amd.module import Module
+
+pytestmark = pytest.mark.gpu
+
+
+def rng(*key):
+    return np.random.default_rng(list(key))
+
+
+def f32(a):
+    return np.ascontiguousarray(a, np.float32)
+
+
+def forward(fn, arrays, decl=None, stream=0):
+    """The outputs of a traced forward, run in device memory."""
+    decl = decl or {n: {'shape': list(a.shape), 'dtype': 'i32' if a.dtype == np.int32 else 'f32'} for n, a in arrays.items()}
+    ex = compile_forward(Module(), lambda m, i: fn(i), decl, seed=0)
+    g = ex.graph_for(arrays).graph
+    dev = {n: torch.from_numpy(a).cuda() for n, a in arrays.items()}
+    outs = [torch.full(g.tensors[t].shape, float('nan'), device='cuda') for t in g.outputs]
+    torch.cuda.synchronize()
+    r = ex.run_device(dev, outs, stream)
+    if r.error is not None:
+        raise r.error
+    torch.cuda.synchronize()
+    got = [o.cpu().numpy() for o in outs]
+    ex.destroy()
+    return got
+
+
+def attend(q, k, v, dy=None, how=None, masks=None):
+    """{'y', ...} of the package for numpy inputs."""
+    how, masks = how or {}, masks or {}
+    arrays = dict(q=q, k=k, v=v, **masks, **({} if dy is None else {'dy': dy}))
+
+    def fn(i):
+        m = {n: i[n] for n in masks}
+        y = O.attention(i['q'], i['k'], i['v'], **how, **m)
+        return [y] if dy is None else [y, *O.attention_grad(i['q'], i['k'], i['v'], y, i['dy'], **how, **m)]
+    return dict(zip(('y', 'dq', 'dk', 'dv'), forward(fn, arrays)))
+
+
+def check_attention(q, k, v, dy, how, masks, what=''):
+    want, tol = R.attention(q, k, v, dy, **how, **masks)
+    got = attend(q, k, v, dy, how, masks)
+    for n in want:
+        R.check(got[n], want[n], tol[n], f'{what} {n}')
+    return got
+
+
+def qkv(B, H, Hk, Tq, Tk, D, Dv, seed, size=1.0):
+    r = rng(B, H, Tq, Tk, D, Dv, seed)
+    return (f32(size * r.standard_normal((B, H, Tq, D))), f32(r.standard_normal((B, Hk, Tk, D))),
+            f32(r.standard_normal((B, Hk, Tk, Dv))), f32(r.standard_normal((B, H, Tq, Dv))))
+
+
+SHAPES = [  # B, H, Hk, Tq, Tk, D, Dv
+    (1, 1, 1, 1, 1, 1, 1), (2, 2, 1, 2, 3, 5, 7), (2, 4, 2, 16, 16, 16, 16), (1, 2, 2, 31, 33, 32, 32), (1, 3, 1, 65, 97, 40, 24),
+    (1, 2, 1, 129, 129, 64, 64), (1, 2, 1, 100, 260, 96, 96), (1, 4, 1, 70, 130, 128, 128), (2, 1, 1, 64, 64, 127, 1),
+    (1, 7, 1, 3, 300, 80, 80), (3, 2, 2, 1, 517, 64, 64), (1, 16, 2, 1, 1030, 128, 128), (1, 2, 2, 8, 640, 17, 64),
+]
+
+
+@pytest.mark.parametrize('shape', SHAPES)
+@pytest.mark.parametrize('how', [dict(), dict(causal=False), dict(softcap=3.0, scale=0.3), dict(slopes=True), dict(softcap=20.0, slopes=True)],
+                         ids=['causal', 'full', 'cap', 'slopes', 'cap+slopes'])
+def test_attention_shapes_and_scores(shape, how):
+    B, H, Hk, Tq, Tk, D, Dv = shape
+    how = dict(how)
+    if how.get('slopes'):
+        how['slopes'] = [2.0 ** (-i - 1) for i in range(H)]
+    check_attention(*qkv(*shape, 1, 2.0), how, {}, str(shape))
+
+
+@pytest.mark.parametrize('shape', [(2, 3, 5, 7), (3, 2, 40, 64), (2, 2, 100, 32), (2, 2, 260, 128)])
+@pytest.mark.parametrize('kind', ['documents', 'scattered', 'padding', 'prefix', 'lengths', 'all', 'nothing'])
+def test_attention_masks(shape, kind):
+    B, H, T, D = shape
+    q, k, v, dy = qkv(B, H, 1, T, T, D, D, 2)
+    r = rng(T, D, 7)
+    how, masks = {}, {}
+    if kind in ('documents', 'all'):
+        masks['documents'] = np.sort(r.integers(0, 4, (B, T), dtype=np.int32), 1)
+    if kind == 'scattered':                              # ids in any order, without a causal mask
+        masks['documents'] = r.integers(-1, 3, (B, T), dtype=np.int32)
+        how['causal'] = False
+    if kind in ('padding', 'all'):
+        d = masks.setdefault('documents', np.zeros((B, T), np.int32))
+        d[0, T - T // 3:] = -1
+        d[1, :T // 3] = -5
+    if kind in ('prefix', 'all'):
+        masks['prefix'] = np.array([T // 2, 0, T + 9][:B], np.int32)
+    if kind in ('lengths', 'all'):                       # fewer places than queries: the first ones lie before position 0
+        masks['lengths'] = np.array([T, T // 2, 0][:B], np.int32)
+    if kind == 'nothing':
+        masks['documents'] = np.full((B, T), -1, np.int32)
+    got = check_attention(q, k, v, dy, how, masks, kind)
+    if kind == 'nothing':
+        assert not any(np.any(x) for x in got.values())
+
+
+@pytest.mark.parametrize('Tq,Tk', [(1, 1), (1, 31), (1, 700), (5, 700), (33, 700), (128, 1000)])
+@pytest.mark.parametrize('causal', [True, False])
+def test_attention_over_a_part_filled_cache(Tq, Tk, causal):
+    """Lengths from none to beyond the cache (clamped); what lies behind them is garbage."""
+    q, k, v, dy = qkv(5, 4, 2, Tq, Tk, 64, 64, 3)
+    n = np.array([0, 1, Tk // 2, Tk, Tk + 1000], np.int32)
+    for b in range(5):
+        k[b, :, min(n[b], Tk):], v[b, :, min(n[b], Tk):] = np.nan, np.inf
+    check_attention(q, k, v, dy, dict(causal=causal), dict(lengths=n), f'{Tq}x{Tk}')
+    check_attention(q, k, v, None, dict(causal=causal), dict(lengths=n), f'{Tq}x{Tk} forward')
+
+
+@pytest.mark.parametrize('bad', [np.nan, np.inf, -np.inf, 3.4e38])
+@pytest.mark.parametrize('what', ['padding', 'document', 'future', 'padded query'])
+def test_masked_garbage_stays_out(bad, what):
+    B, H, T, D = 1, 2, 90, 32
+    q, k, v, dy = qkv(B, H, 1, T, T, D, D, 4)
+    doc = np.repeat(np.array([[0, 1, 2]], np.int32), 30, 1)
+    masks, how = dict(documents=doc), {}
+    if what == 'padding':
+        doc[:, 60:] = -1
+        k[:, :, 60:], v[:, :, 60:] = bad, bad
+    elif what == 'document':                             # a whole document of it: its own rows may be anything
+        k[:, :, 30:60], v[:, :, 30:60] = bad, bad
+        want, tol = R.attention(q, k, v, **masks)
+        got = attend(q, k, v, None, how, masks)['y']
+        rows = np.r_[0:30, 60:90]
+        R.check(got[:, :, rows], want['y'][:, :, rows], tol['y'][:, :, rows], what)
+        return
+    elif what == 'future':                               # seen by the last query alone
+        masks = {}
+        k[:, :, -1], v[:, :, -1] = bad, bad
+        want, tol = R.attention(q, k, v)
+        got = attend(q, k, v)['y']
+        R.check(got[:, :, :-1], want['y'][:, :, :-1], tol['y'][:, :, :-1], what)
+        return
+    else:
+        doc[:, 60:] = -1
+        q[:, :, 60:], dy[:, :, 60:] = bad, bad
+        k[:, :, 60:], v[:, :, 60:] = bad, bad
+    got = check_attention(q, k, v, dy, how, masks, what)
+    assert not np.any(got['y'][:, :, 60:]) and not np.any(got['dq'][:, :, 60:])
+    assert not np.any(got['dk'][:, :, 60:]) and not np.any(got['dv'][:, :, 60:])
+
+
+def test_visible_infinities_reach_the_result():
+    q, k, v, _ = qkv(1, 1, 1, 40, 40, 32, 32, 5)
+    v[0, 0, 3, 2] = np.inf
+    v[0, 0, 20, 5] = np.nan
+    y = attend(q, k, v)['y'][0, 0]
+    assert np.all(y[3:, 2] == np.inf) and np.all(np.isfinite(y[:3])) and np.all(np.isfinite(y[:, 3]))
+    assert np.all(np.isnan(y[20:, 5])) and np.all(np.isfinite(y[:20, 5]))
+
+
+@pytest.mark.parametrize('size', [1e-6, 1e-3, 1e3])
+def test_attention_keeps_small_and_large_values(size):
+    """Scores stay moderate (the scale undoes the size); values and gradients carry it."""
+    q, k, v, dy = qkv(1, 2, 1, 70, 70, 64, 64, 6)
+    check_attention(f32(q * size), f32(k * size), f32(v * size), f32(dy / size), dict(scale=0.125 / size ** 2), {}, str(size))
+
+
+def test_columns_of_very_different_size():
+    q, k, v, dy = qkv(1, 1, 1, 80, 80, 32, 32, 8)
+    v[..., 0] *= 4000
+    k[..., 1] *= 300
+    q[..., 1] /= 300
+    check_attention(q, k, v, dy, {}, {})
+
+
+def test_large_scores_do_not_overflow():
+    q, k, v, dy = qkv(1, 2, 1, 40, 40, 16, 16, 9)
+    check_attention(f32(60 * q), f32(10 * k), v, dy, {}, {}, 'plain')
+    check_attention(f32(60 * q), f32(10 * k), v, dy, dict(softcap=5.0), {}, 'cap')
+
+
+def test_attention_gradient_against_differences():
+    """Directional differences of the package's own forward, in steps where f32 resolves them: with values of size 1, a
+    difference over 2 h at h = 2^-6 is off by h^2 times the third derivative (some 1e-3 here) and 2^-24 / h of rounding."""
+    r = rng(11)
+    q, k, v, dy = qkv(1, 2, 1, 24, 24, 16, 16, 10)
+    how = dict(softcap=4.0, slopes=[0.25, 0.125])
+    got = attend(q, k, v, dy, how)
+    for name, x in (('dq', q), ('dk', k), ('dv', v)):
+        u = f32(r.standard_normal(x.shape) / np.sqrt(x.size))
+        h = 2.0 ** -6
+        sides = []
+        for s in (1, -1):
+            args = dict(q=q, k=k, v=v)
+            args[name[1]] = f32(x + s * h * u)
+            sides.append((attend(args['q'], args['k'], args['v'], None, how)['y'].astype(np.float64) * dy).sum())
+        diff = (sides[0] - sides[1]) / (2 * h)
+        assert abs(diff - (got[name].astype(np.float64) * u).sum()) <= 1e-3 * np.abs(got[name] * u).sum() + 1e-3
+
+
+def test_attention_is_deterministic():
+    q, k, v, dy = qkv(2, 4, 2, 300, 300, 64, 64, 12)
+    a, b = attend(q, k, v, dy), attend(q, k, v, dy)
+    assert all(np.array_equal(a[n], b[n]) for n in a)
+
+
+# ---- rotary positions -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize('B,H,Hk,T,D,sections', [
+    (1, 1, 1, 1, 2, [1]), (2, 3, 1, 7, 10, [2, 1, 2]), (2, 4, 2, 33, 64, [8, 12, 12]), (1, 2, 2, 130, 96, [8, 8]),
+    (3, 1, 1, 5, 7, [1, 1]), (1, 2, 1, 64, 128, [16, 24, 24]), (33, 16, 4, 1, 80, [40]), (1, 2, 2, 9, 6, [1, 1, 1])])
+@pytest.mark.parametrize('per_axis', [False, True])
+@pytest.mark.parametrize('inverse', [False, True])
+def test_rope_axes(B, H, Hk, T, D, sections, per_axis, inverse):
+    r = rng(T, D, len(sections))
+    q, k = f32(r.standard_normal((B, H, T, D))), f32(r.standard_normal((B, Hk, T, D)))
+    pos = r.integers(-50, 2000000, (len(sections), B, T), dtype=np.int32)
+    pos.flat[:2] = [0, 2 ** 31 - 1][:pos.size]
+    got = forward(lambda i: list(O.rope_axes(i['q'], i['k'], i['p'], sections, 5000.0, per_axis, inverse)), dict(q=q, k=k, p=pos))
+    for g, x in zip(got, (q, k)):
+        want, tol = R.rope_axes(x, pos, sections, 5000.0, per_axis, inverse)
+        R.check(g, want, tol)
+
+
+def test_rope_axes_passes_infinities_of_other_pairs():
+    q = f32(rng(1).standard_normal((1, 1, 3, 8)))
+    q[0, 0, 1, 6] = np.inf
+    y = forward(lambda i: list(O.rope_axes(i['q'], i['q'], i['p'], [2])), dict(q=q, p=np.arange(3, dtype=np.int32).reshape(1, 1, 3)))[0]
+    assert y[0, 0, 1, 6] == np.inf and np.isfinite(np.delete(y.ravel(), 14)).all()
+
+
+# ---- recurrence ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('B,T,C', [(1, 1, 1), (2, 2, 3), (3, 17, 64), (2, 63, 65), (1, 128, 256), (2, 257, 33), (1, 1000, 7), (4, 515, 130),
+                                   (1, 4097, 12), (300, 3, 5)])
+@pytest.mark.parametrize('start', [False, True])
+def test_recurrence(B, T, C, start):
+    r = rng(B, T, C)
+    a = f32(1 / (1 + np.exp(-r.standard_normal((B, T, C)) - 3)))
+    a[:, T // 2:T // 2 + 1] = 0                          # a fresh start half way
+    x, dh, h0 = (f32(r.standard_normal(s)) for s in ((B, T, C), (B, T, C), (B, C)))
+    ins = dict(a=a, x=x, dh=dh, **(dict(h0=h0) if start else {}))
+
+    def fn(i):
+        h = O.linear_recurrence(i['a'], i['x'], i.get('h0'))
+        return [h, *O.linear_recurrence_grad(i['a'], h, i['dh'], i.get('h0'))]
+    got = dict(zip(('h', 'da', 'dx', 'dh0'), forward(fn, ins)))
+    want, tol = R.recurrence(a, x, h0 if start else None, dh)
+    for n in want:
+        R.check(got[n], want[n], tol[n], n)
+
+
+def test_recurrence_gates_of_any_sign_and_size():
+    """Gates beyond 1 grow, negative ones alternate; a zero gate forgets what came before (by its product: only finite
+    values)."""
+    r = rng(21)
+    a = f32(r.uniform(-1.1, 1.1, (2, 300, 40)))
+    x, dh = f32(r.standard_normal(a.shape)), f32(r.standard_normal(a.shape))
+
+    def fn(i):
+        h = O.linear_recurrence(i['a'], i['x'])
+        return [h, *O.linear_recurrence_grad(i['a'], h, i['dh'])]
+    got = dict(zip(('h', 'da', 'dx'), forward(fn, dict(a=a, x=x, dh=dh))))
+    want, tol = R.recurrence(a, x, None, dh)
+    for n in want:
+        R.check(got[n], want[n], tol[n], n)
+
+
+def test_recurrence_does_not_look_ahead_or_across():
+    r = rng(22)
+    a, x = f32(r.uniform(0.5, 1, (3, 700, 20))), f32(r.standard_normal((3, 700, 20)))
+    clean = forward(lambda i: [O.linear_recurrence(i['a'], i['x'])], dict(a=a, x=x))[0]
+    a[1, 400:], x[1, 400:] = np.nan, np.inf
+    got = forward(lambda i: [O.linear_recurrence(i['a'], i['x'])], dict(a=a, x=x))[0]
+    assert np.array_equal(got[[0, 2]], clean[[0, 2]]) and np.array_equal(got[1, :400], clean[1, :400])
+    assert np.isnan(got[1, 400:]).all()
+
+
+# ---- together, as a model uses them ------------------------------------------------------------------
+
+VOCAB, DIM, HEADS, KV = 29, 32, 4, 2
+
+
+class Mixed(Module):
+    """An attention layer with turned positions and a recurrent layer over a packed batch."""
+
+    def __init__(self):
+        self.emb = nn.Embedding(VOCAB, DIM)
+        self.q, self.k, self.v, self.o = (nn.Linear(DIM, n, bias=False) for n in (DIM, DIM * KV // HEADS, DIM * KV // HEADS, DIM))
+        self.gate, self.val = nn.Linear(DIM, DIM), nn.Linear(DIM, DIM)
+        self.head = nn.Linear(DIM, VOCAB)
+
+
+def mixed_logits(p, i):
+    x = p.emb.fwd(i['tokens'])
+    q, k, v = (O.split_heads(m.fwd(x), n) for m, n in ((p.q, HEADS), (p.k, KV), (p.v, KV)))
+    q, k = O.rope_axes(q, k, i['positions'], [2, 2])
+    y = O.attention(q, k, v, softcap=8.0, slopes=[0.5, 0.25, 0.125, 0.0625], documents=i['documents'], prefix=i['prefix'])
+    x = O.add(x, p.o.fwd(O.merge_heads(y)))
+    a = O.mul(O.sigmoid(p.gate.fwd(x)), O.reshape(i['keep'], [*i['keep'].shape, 1]))
+    x = O.add(x, O.linear_recurrence(a, O.tanh(p.val.fwd(x))))
+    return p.head.fwd(x)
+
+
+def mixed_batch(B, T, seed):
+    r = rng(B, T, seed)
+    doc = np.sort(r.integers(0, 3, (B, T), dtype=np.int32), 1)
+    doc[:, T - 2:] = -1
+    fresh = np.concatenate([np.ones((B, 1), bool), doc[:, 1:] != doc[:, :-1]], 1)
+    at = np.arange(T) - np.maximum.accumulate(np.where(fresh, np.arange(T), 0), 1)
+    return {'tokens': r.integers(0, VOCAB, (B, T), dtype=np.int32), 'targets': r.integers(0, VOCAB, (B, T), dtype=np.int32),
+            'documents': doc, 'positions': np.ascontiguousarray(np.stack([at, at // 3]).astype(np.int32)),
+            'prefix': r.integers(0, T // 2, B, dtype=np.int32), 'keep': f32(~fresh)}
+
+
+def mixed_torch(w, i, B, T):
+    """The same loss in f64 torch, for autograd."""
+    t = {n: torch.from_numpy(a) for n, a in i.items()}
+    x = w['emb.W'][t['tokens'].long()]
+    heads = lambda n, h: (x @ w[n + '.W']).reshape(B, T, h, -1).transpose(1, 2)  # noqa: E731
+    q, k, v = heads('q', HEADS), heads('k', KV), heads('v', KV)
+    freq = 10000.0 ** -(torch.arange(4, dtype=torch.float64) / 4)
+    ang = t['positions'].double()[[0, 0, 1, 1]].permute(1, 2, 0) * freq
+    c, s = torch.cos(ang)[:, None], torch.sin(ang)[:, None]
+    turn = lambda z: torch.cat([z[..., :4] * c - z[..., 4:] * s, z[..., 4:] * c + z[..., :4] * s], -1)  # noqa: E731
+    q, k = turn(q), turn(k).repeat_interleave(HEADS // KV, 1)
+    sc = q @ k.transpose(-1, -2) / 8 ** 0.5
+    j = torch.arange(T)
+    sc = 8 * torch.tanh(sc / 8) - torch.tensor([0.5, 0.25, 0.125, 0.0625]).double()[:, None, None] * (j[:, None] - j).abs()
+    d = t['documents']
+    ok = ((j <= j[:, None]) | (j < t['prefix'][:, None, None])) & (d[:, :, None] == d[:, None, :]) & (d[:, None, :] >= 0)
+    ok = ok[:, None]
+    P = torch.softmax(sc.masked_fill(~ok, -1e300), -1).masked_fill(~ok, 0)
+    y = (P @ v.repeat_interleave(HEADS // KV, 1)).transpose(1, 2).reshape(B, T, DIM)
+    x = x + y @ w['o.W']
+    a = torch.sigmoid(x @ w['gate.W'] + w['gate.b']) * t['keep'].double()[..., None]
+    z = torch.tanh(x @ w['val.W'] + w['val.b'])
+    h, hs = torch.zeros(B, DIM).double(), []
+    for n in range(T):
+        h = a[:, n] * h + z[:, n]
+        hs.append(h)
+    x = x + torch.stack(hs, 1)
+    logits = x @ w['head.W'] + w['head.b']
+    return torch.nn.functional.cross_entropy(logits.reshape(-1, VOCAB), t['targets'].long().reshape(-1)), logits
+
+
+@pytest.mark.parametrize('B,T', [(2, 12), (3, 65)])
+def test_model_of_them_trains_as_in_64_bits(B, T):
+    """One SGD step at rate 1 from known weights: what the weights moved by is the gradient. Chains of some ten f32 operations
+    and sums over B T positions: 2e-5 of each gradient's norm is about 300 roundings."""
+    batch = mixed_batch(B, T, 1)
+    decl = {n: {'shape': list(a.shape), 'dtype': 'i32' if a.dtype == np.int32 else 'f32'} for n, a in batch.items()}
+    t = tg_compile(Mixed(), lambda p, i: nn.cross_entropy(mixed_logits(p, i), i['targets']), decl, {'kind': 'sgd', 'lr': 1.0}, seed=3)
+    before = t.download_params()
+    shapes = t.ir.param_shapes()
+    r = t.step(batch)
+    assert r.kind == 'completed', r.error
+    after = t.download_params()
+    w = {n: torch.from_numpy(a.reshape(shapes[n])).double().requires_grad_(True) for n, a in before.items()}
+    loss, logits = mixed_torch(w, batch, B, T)
+    assert abs(r.loss - float(loss)) <= 1e-5 * abs(float(loss))
+    grads = dict(zip(w, torch.autograd.grad(loss, list(w.values()))))
+    for n, g in grads.items():
+        moved = (before[n].astype(np.float64) - after[n]).reshape(shapes[n])
+        # the difference of two f32 weights carries their own rounding
+        slack = 2e-5 * np.linalg.norm(g) + 2 * R.U * np.linalg.norm(before[n])
+        assert np.linalg.norm(moved - g.numpy()) <= slack, n
+    kinds = [n['kind'] for n in t._rt.describe()['nodes']]
+    assert [kinds.count(k) for k in ('attend', 'attend_grad', 'rope', 'scan', 'scan_grad')] == [1, 1, 2, 1, 1]
+    # the trained weights in a forward graph, from host arrays and in device memory
+    f = t.attach(lambda p, i: mixed_logits(p, i), {n: d for n, d in decl.items() if n != 'targets'})
+    out = f.run(batch).output
+    w2 = {n: torch.from_numpy(a.reshape(shapes[n])).double() for n, a in after.items()}
+    want = mixed_torch(w2, batch, B, T)[1].numpy()
+    assert np.linalg.norm(out - want) <= 1e-5 * np.linalg.norm(want)
+    dev = {n: torch.from_numpy(a).cuda() for n, a in batch.items()}
+    got = torch.empty(out.shape, device='cuda')
+    torch.cuda.synchronize()
+    assert f.run_device(dev, [got]).error is None
+    torch.cuda.synchronize()
+    assert np.array_equal(got.cpu().numpy(), out)
+    t.destroy()
+
+
+# ---- device-resident calls -----------------------------------------------------------------------------
+
+def _scan_executor(B=2, T=100, C=64):
+    d = {'a': [B, T, C], 'x': [B, T, C]}
+    ex = compile_forward(Module(), lambda m, i: [O.linear_recurrence(i['a'], i['x']), O.mul(i['a'], 2.0), O.reshape(i['x'], [B * T, C])], d, seed=0)
+    r = rng(31)
+    ins = {n: torch.from_numpy(f32(r.uniform(0.2, 1, s))).cuda() for n, s in d.items()}
+    outs = [torch.empty(B, T, C, device='cuda'), torch.empty(B, T, C, device='cuda'), torch.empty(B * T, C, device='cuda')]
+    torch.cuda.synchronize()
+    return ex, ins, outs
+
+
+def test_run_device_writes_every_output():
+    """A recurrence bound to the caller's tensors beside a fused group (run on the runtime's own buffers) and an output that
+    is a view of an input."""
+    ex, ins, outs = _scan_executor()
+    host = ex.run({n: t.cpu().numpy() for n, t in ins.items()}).output
+    for _ in range(3):
+        for o in outs:
+            o.fill_(float('nan'))
+        torch.cuda.synchronize()
+        r = ex.run_device(ins, outs)
+        assert r.error is None
+        torch.cuda.synchronize()
+        assert np.array_equal(outs[0].cpu().numpy(), host)
+        assert torch.equal(outs[1], ins['a'] * 2) and torch.equal(outs[2], ins['x'].reshape(outs[2].shape))
+    ex.destroy()
+
+
+def test_run_device_follows_the_stream():
+    """Producer, call and consumer on one stream, then on several, without the host waiting between."""
+    ex, ins, outs = _scan_executor(4, 1000, 256)
+    want = ex.run({n: t.cpu().numpy() for n, t in ins.items()}).output
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    keep = []
+    for turn in range(6):
+        s = streams[turn % 3]
+        with torch.cuda.stream(s):
+            scaled = {n: t * 2 for n, t in ins.items()}
+            scaled['a'] = scaled['a'] / 2
+            o = [torch.empty_like(x) for x in outs]
+            assert ex.run_device(scaled, o, s.cuda_stream).error is None
+            keep.append((scaled, o, o[0] / 2))
+    torch.cuda.synchronize()
+    for _, _, half in keep:                             # doubling and halving are exact
+        assert np.array_equal(half.cpu().numpy(), want)
+    host = ex.run({n: t.cpu().numpy() for n, t in ins.items()}).output      # the host path waits for them
+    assert np.array_equal(host, want)
+    ex.destroy()
+
+
+def test_run_device_refusals():
+    ex, ins, outs = _scan_executor()
+    bad = [
+        (dict(ins, a=ins['a'].cpu()), outs, "input 'a': not"),
+        (dict(ins, a=ins['a'][:1]), outs, 'elements'),
+        (dict(ins, a=ins['a'].double()), outs, 'float32'),
+        (dict(ins, a=ins['a'].transpose(0, 1).contiguous().transpose(0, 1)), outs, 'contiguous'),
+        ({'a': ins['a']}, outs, 'missing input'),
+        (ins, outs[:2], '3 outputs'),
+        (ins, [ins['a'], outs[1], outs[2]], 'overlap'),
+        (ins, [outs[0], outs[0], outs[2]], 'overlap'),
+        (dict(ins, a=torch.empty(2 * 100 * 64 + 1, device='cuda')[1:]), outs, 'aligned'),
+        (dict(ins, a=np.zeros((2, 100, 64), np.float32)), outs, 'device memory'),
+    ]
+    for i, o, what in bad:
+        r = ex.run_device(i, o)
+        assert r.kind == 'failed' and what in str(r.error), (what, r.error)
+    n = 2 * 100 * 64 * 4
+    with pytest.raises(backend.BackendError, match='expected'):
+        ex._owner[0].run_device(['a', 'x'], [ins['a'].data_ptr(), ins['x'].data_ptr()], [n, n - 4], [o.data_ptr() for o in outs], [n] * 3)
+    s = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        graph.capture_begin(capture_error_mode='relaxed')
+        r = ex.run_device(ins, outs, s.cuda_stream)
+        graph.capture_end()
+    assert r.kind == 'failed' and 'captured' in str(r.error)
+    torch.cuda.synchronize()
+    assert ex.run_device(ins, outs).kind == 'completed'
+    ex.destroy()
+    assert ex.run_device(ins, outs).kind == 'aborted'
+
+
+def test_run_device_with_random_numbers_and_parameters():
+    """Dropout takes a new seed each call, parameters may be replaced between calls; both as `run` does."""
+    class M(Module):
+        def __init__(self):
+            self.l = nn.Linear(8, 8)
+    fwd = lambda m, i: O.dropout(m.l.fwd(i['x']), 0.5)  # noqa: E731
+    x = f32(rng(41).standard_normal((16, 8)))
+    host, dev = (compile_forward(M(), fwd, {'x': [16, 8]}, seed=1) for _ in range(2))
+    p = {n: f32(rng(42).standard_normal(a.shape)) for n, a in host.download_params().items()}
+    out = [torch.empty(16, 8, device='cuda') for _ in range(4)]
+    xd = torch.from_numpy(x).cuda()
+    torch.cuda.synchronize()
+    for turn in range(4):
+        if turn == 2:
+            host.upload_params(p)
+            dev.upload_params(p)
+        want = host.run({'x': x}).output
+        assert dev.run_device({'x': xd}, [out[turn]]).error is None
+        torch.cuda.synchronize()
+        assert np.array_equal(out[turn].cpu().numpy(), want)
+    host.destroy()
+    dev.destroy()
+
+
+def test_parametric_length_and_host_run():
+    """One executor over growing caches: a graph per length, the same results as from host arrays."""
+    ex = compile_forward(Module(), lambda m, i: O.attention(i['q'], i['k'], i['v'], lengths=i['n']),
+                         {'q': [2, 4, 1, 32], 'k': [2, 2, None, 32], 'v': [2, 2, None, 32], 'n': {'shape': [2], 'dtype': 'i32'}}, seed=0)
+    for T in (1, 40, 300):
+        q, k, v, _ = qkv(2, 4, 2, 1, T, 32, 32, 51)
+        n = np.array([T, (T + 1) // 2], np.int32)
+        host = ex.run(dict(q=q, k=k, v=v, n=n)).output
+        want, tol = R.attention(q, k, v, lengths=n)
+        R.check(host, want['y'], tol['y'])
+        out = torch.empty(2, 4, 1, 32, device='cuda')
+        dev = {m: torch.from_numpy(a).cuda() for m, a in dict(q=q, k=k, v=v, n=n).items()}
+        torch.cuda.synchronize()
+        assert ex.run_device(dev, [out]).error is None
+        torch.cuda.synchronize()
+        assert np.array_equal(out.cpu().numpy(), host)
+    ex.destroy()
