@@ -17,7 +17,7 @@ struct Rows {
 struct AttendDesc {
   int B, H, Hk, Tq, Tk, D, Dv;
   Rows q, k, v, y;
-  float* lse;                // [B, H, Tq]: log of the sum of exp(score); +inf for a row that sees nothing, so that exp(s - lse) = 0
+  float* lse;                // [B, H, Tq]: log2 of the sum of exp(score); +inf for a row that sees nothing (its exp2(s - lse) is 0)
   const int32_t* documents;  // [B, Tk] or null
   const int32_t* prefix;     // [B] or null
   const int32_t* lengths;    // [B] or null
