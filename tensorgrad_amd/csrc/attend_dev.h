@@ -106,16 +106,12 @@ __device__ __forceinline__ Sight sight(const AttendDesc& a, int b) {
   s.positional = a.positional;
   return s;
 }
-// Key j < Tk for a query at position p of document d.
-__device__ __forceinline__ bool sees(const Sight& s, int p, int d, int j) {
-  bool ok = j < s.n && !(s.positional && p < 0) && !(s.causal && j > p && j >= s.prefix);
-  if (s.doc && ok) {
-    const int dj = s.doc[j];
-    ok = dj == d && dj >= 0;
-  }
-  return ok;
+// A query at position p sees the keys below this, of its document.
+__device__ __forceinline__ int sees_below(const Sight& s, int p) {
+  if (s.positional && p < 0) return 0;
+  return s.causal ? min(s.n, max(p + 1, s.prefix)) : s.n;
 }
-__device__ __forceinline__ int doc_at(const Sight& s, int p) { return s.doc && p >= 0 ? s.doc[p] : -1; }
+__device__ __forceinline__ int doc_at(const Sight& s, int p) { return s.doc && p >= 0 ? s.doc[p] : -1; }   // negative: sees nothing
 
 // Rows [lo, hi] of positions against keys [j0, j0 + 32): does any pair see, do all.
 struct Span {
@@ -157,10 +153,20 @@ __device__ __forceinline__ RowMap row_map(const Rows& x, int b, int head, const 
   return {x.p + b * x.b + head * x.h, x.h, x.t, group};
 }
 
-// B fragments of 32 rows (lane l: row l % 32), each row with its own power of two; returns its exponent. wide: rows are
-// 16-byte aligned and n a multiple of 8.
+// An exponent that bounds a 2-norm: values of at most `top`, whose squares relative to it sum to sq.
+__device__ __forceinline__ int norm_exponent(float top, float sq) {
+  return top > 0 ? exponent(top) + 1 + (exponent(sq) + 2) / 2 : -126;
+}
+__device__ __forceinline__ float finite_abs(float x) {
+  x = fabsf(x);
+  return x < INFINITY ? x : 0.0f;
+}
+
+// B fragments of 32 rows (lane l: row l % 32), each row with its own power of two; returns its exponent, and in *norm a bound
+// on its 2-norm. wide: rows are 16-byte aligned and n a multiple of 8.
 template <int KC>
-__device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bool wide, half8 (&hi)[KC], half8 (&lo)[KC]) {
+__device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bool wide, half8 (&hi)[KC], half8 (&lo)[KC],
+                                         int* norm = nullptr) {
   const int h = (threadIdx.x >> 5) & 1;
   float x[KC][8];
 #pragma unroll
@@ -183,11 +189,20 @@ __device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bo
 #pragma unroll
   for (int c = 0; c < KC; ++c)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float z = fabsf(x[c][i]);
-      m = fmaxf(m, z < INFINITY ? z : 0.0f);   // of the finite ones; the others stay what they are
-    }
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(x[c][i]));   // the others stay what they are
   m = halves_max(m);
+  if (norm) {
+    float sq = 0;
+    const float inv = m > 0 ? 1.0f / fmaxf(m, 1e-37f) : 0.0f;
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float z = finite_abs(x[c][i]) * inv;
+        sq = fmaf(z, z, sq);
+      }
+    *norm = norm_exponent(m, halves_sum(sq));
+  }
   const int e = m > 0 ? min(14 - exponent(m), 126) : 0;
   const float s = pow2(e);
 #pragma unroll
@@ -217,17 +232,41 @@ __device__ __forceinline__ void plain_scores(f32x16& s, RowOf row_of, int rows, 
     for (int r = 0; r < 16; ++r) s[r] = r == q ? x : s[r];
   }
 }
-// acc (columns: lanes, rows: features) += sum over the tile's rows j of row(j) * w[j] * c, rows of weight 0 left out.
+// Sums over several tiles in one accumulator: the weights (f16 parts of x 2^e) times a tile packed at 2^t are in units of
+// 2^-(e + t), which must be the accumulator's 2^-c. A lane's c only falls, when a tile's largest weight `big` would pass
+// 2^14: what comes later and is smaller is rounded like the largest of the sum (2^-37 of it), what was hidden has weight 0
+// and counts for nothing. c starts at kUnset, the accumulator at 0. Returns e; *change: the accumulator's factor.
+constexpr int kUnset = 1000;
+__device__ __forceinline__ int fit_unit(int& c, float big, int t, float* change) {
+  int e = c - t;
+  if (big > 0 && e > 14 - exponent(big)) {
+    e = min(12 - exponent(big), 110);
+    *change *= __builtin_amdgcn_ldexpf(1.0f, e + t - c);   // 0 where acc no longer counts
+    c = e + t;
+  }
+  return e;
+}
+template <int DB>
+__device__ __forceinline__ void rescale(f32x16 (&acc)[DB], float change) {
+  if (!__any(change != 1)) return;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int q = 0; q < 16; ++q) acc[d][q] *= change;
+}
+// acc (columns: lanes, rows: features) += sum over the tile's rows j of row(j) * w[j] in f32, rows of weight 0 left out. The
+// values go in as they are, so acc leaves its unit for the sum, and returns to it unless they are too large for it.
 template <int DB, class RowOf>
-__device__ __forceinline__ void plain_accumulate(f32x16 (&acc)[DB], const f32x16& w, float c, RowOf row_of, int rows, int n) {
+__device__ __forceinline__ void plain_accumulate(f32x16 (&acc)[DB], int& c, const f32x16& w, RowOf row_of, int rows, int n) {
   const int lane = threadIdx.x & 63, h = lane >> 5;
+  rescale<DB>(acc, __builtin_amdgcn_ldexpf(1.0f, c == kUnset ? 0 : -c));
 #pragma unroll 1
   for (int j = 0; j < min(rows, kTile); ++j) {
     const int at = 4 * (j / 8) + j % 4;
     float x = 0;
 #pragma unroll
     for (int r = 0; r < 16; ++r) x = r == at ? w[r] : x;
-    x = __shfl(x, (lane & 31) + 32 * ((j / 4) & 1)) * c;
+    x = __shfl(x, (lane & 31) + 32 * ((j / 4) & 1));
     const float* a = row_of(j);
 #pragma unroll
     for (int b = 0; b < DB; ++b)
@@ -237,6 +276,56 @@ __device__ __forceinline__ void plain_accumulate(f32x16 (&acc)[DB], const f32x16
         if (d < n && x != 0) acc[b][r] = fmaf(x, a[d], acc[b][r]);
       }
   }
+  float m = 0;
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) m = fmaxf(m, finite_abs(acc[b][r]));
+  m = halves_max(m);
+  if (m > 0) c = min(min(c == kUnset ? 26 - exponent(m) : c, 110 - exponent(m)), 120);
+  rescale<DB>(acc, pow2(c == kUnset ? 0 : c));
+}
+
+// acc += A fragments (feature blocks x two k steps, from fragment f0 of L) times the split of x * scale
+template <int DB>
+__device__ __forceinline__ void accumulate(f32x16 (&acc)[DB], const f32x16& x, float scale, const _Float16* L, int f0) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    float z[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) z[q] = x[8 * ks + q] * scale;
+    half8 bh, bl;
+    split8(z, bh, bl);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const half8 ah = *(const half8*)(L + (f0 + (d * 2 + ks) * 2) * kFrag + lane * 8);
+      const half8 al = *(const half8*)(L + (f0 + (d * 2 + ks) * 2 + 1) * kFrag + lane * 8);
+      acc[d] = mfma(al, bh, acc[d]);
+      acc[d] = mfma(ah, bl, acc[d]);
+      acc[d] = mfma(ah, bh, acc[d]);
+    }
+  }
+}
+// A fragments (KC k steps, from fragment f0 of L) times B fragments
+template <int KC>
+__device__ __forceinline__ f32x16 scores(const _Float16* L, int f0, const half8 (&bh)[KC], const half8 (&bl)[KC]) {
+  const int lane = threadIdx.x & 63;
+  f32x16 x = {};
+#pragma unroll
+  for (int c = 0; c < KC; ++c) {
+    const half8 ah = *(const half8*)(L + (f0 + 2 * c) * kFrag + lane * 8), al = *(const half8*)(L + (f0 + 2 * c + 1) * kFrag + lane * 8);
+    x = mfma(al, bh[c], x);
+    x = mfma(ah, bl[c], x);
+    x = mfma(ah, bh[c], x);
+  }
+  return x;
+}
+__device__ __forceinline__ float largest(const f32x16& x) {   // magnitude, over a row's two lane halves
+  float m = 0;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) m = fmaxf(m, fabsf(x[q]));
+  return halves_max(m);
 }
 
 // Blocks of one slab (batch entry and key head) on one XCD, whose L2 then holds its packed tiles: hardware deals block ids
@@ -256,11 +345,12 @@ struct PackJob {
   int n, G, rows, tiles;           // features; heads that share a key head; rows = positions * G; tiles
   _Float16 *rowf, *colf;           // [slab][tile][2 KC][512], [slab][tile][4 DB][512], or null
   TileInfo* info;                  // [slab][tile]
-  const int32_t* documents;        // of the rows [B, rows], or null
-  // of the gradient dy: y's rows for its dot products, and the row values of a tile (see RowInfo), else null
+  bool query;                      // rows are queries: their documents are those at their positions
+  // of the gradient dy: y's rows for its dot products, and what the key blocks need of each row, else null
   Rows y;
-  float* rowinfo;                  // [slab][tile][4][32]: lse, dot(dy, y), position, slope
+  float* rowinfo;                  // [slab][tile][kRowInfo][32]
 };
+enum { RI_LSE, RI_DOT, RI_POS, RI_SLOPE, RI_BELOW, RI_DOC, kRowInfo = 8 };   // dot(dy, y); sees keys below; ints as bits
 // The attention's operands as packed for one pass, in the workspace.
 struct Packs {
   int n;

@@ -43,9 +43,8 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const float z = fabsf(u[q]);
-      odd |= !(z < INFINITY);
-      m = fmaxf(m, z < INFINITY ? z : 0.0f);
+      odd |= !(fabsf(u[q]) < INFINITY);
+      m = fmaxf(m, finite_abs(u[q]));
       v[4 * c + q] = u[q];
     }
     *(f32x4*)(x + row * LD + d) = u;
@@ -66,29 +65,32 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
   const float inv = m > 0 ? 1.0f / fmaxf(m, 1e-37f) : 0.0f;
 #pragma unroll
   for (int q = 0; q < DP / 8; ++q) {
-    const float z = fabsf(v[q]) * inv;
-    sq = fmaf(z < INFINITY ? z : 0.0f, z < INFINITY ? z : 0.0f, sq);
+    const float z = finite_abs(v[q]) * inv;
+    sq = fmaf(z, z, sq);
   }
 #pragma unroll
   for (int o = 1; o < 8; o *= 2) sq += __shfl_xor(sq, o);
   if (sub == 0) {
+    const Sight s = sight(p.a, b);
+    const int pos = j.query ? s.first + i : r;
     top[row] = odd ? INFINITY : m;
-    norm[row] = m > 0 ? exponent(m) + 1 + (exponent(sq) + 2) / 2 : -1000;
-    doc[row] = j.documents && in ? j.documents[(int64_t)b * j.rows + r] : -1;
+    norm[row] = norm_exponent(m, sq);
+    doc[row] = in ? doc_at(s, pos) : -1;
     if (j.rowinfo) {
       const AttendDesc& a = p.a;
       const int h = hk * j.G + g;
-      float* o = j.rowinfo + ((int64_t)slab * j.tiles + tile) * (4 * kTile) + row;
-      const int n = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
-      o[0] = in ? a.lse[((int64_t)b * a.H + h) * a.Tq + i] : INFINITY;
-      o[kTile] = in ? dot : 0.0f;
-      o[2 * kTile] = __int_as_float(n - a.Tq + i);
-      o[3 * kTile] = in && a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+      float* o = j.rowinfo + ((int64_t)slab * j.tiles + tile) * (kRowInfo * kTile) + row;
+      o[RI_LSE * kTile] = in ? a.lse[((int64_t)b * a.H + h) * a.Tq + i] : INFINITY;
+      o[RI_DOT * kTile] = in ? dot : 0.0f;
+      o[RI_POS * kTile] = __int_as_float(pos);
+      o[RI_SLOPE * kTile] = in && a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+      o[RI_BELOW * kTile] = __int_as_float(in ? sees_below(s, pos) : 0);
+      o[RI_DOC * kTile] = __int_as_float(doc[row]);
     }
   }
   __syncthreads();
   float hi = 0, lo = INFINITY;
-  int nm = -1000, dmin = INT32_MAX, dmax = INT32_MIN;
+  int nm = -126, dmin = INT32_MAX, dmax = INT32_MIN;
   bool bad = false, same = true;
   for (int q = 0; q < kTile; ++q) {
     const float t = top[q];
@@ -172,7 +174,7 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   const int row0 = blk * 128 + w * kTile, r = row0 + l;
   const bool valid = r < A.M;
   const int i = (int)fastdiv((uint32_t)min(r, A.M - 1), A.group), g = min(r, A.M - 1) - i * G, head = hk * G + g;
-  const int p = s.first + i, doc = doc_at(s, p);
+  const int p = s.first + i, doc = doc_at(s, p), below = sees_below(s, p);
   const float* qrow = a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t;
   half8 qh[KC], ql[KC];
   const int qe = load_rows<KC>(qrow, valid, a.D, A.wide, qh, ql);
@@ -247,7 +249,7 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
 #pragma unroll
   for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
   float m = kNone, sum = 0;        // running maximum (log2) and this lane half's sum
-  int ce = 0;                      // acc is in units of 2^-ce
+  int ce = kUnset;                 // acc is in units of 2^-ce
   if (t0 < t1) fetch(t0, 0);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, j0 = t * kTile;
@@ -257,7 +259,6 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
     const TileInfo kt = ki[t], vt = vi[t];
     if (!any_seen(s, me, kt, j0)) continue;
     const _Float16* L = lds[buf];
-    auto frag = [&](int f) { return *(const half8*)(L + f * kFrag + lane * 8); };
     // scores, transposed: register r of this lane is key j0 + 8 (r / 4) + 4 h + r % 4
     f32x16 x = {};
     float unit;
@@ -266,13 +267,7 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
       plain_scores(x, [&](int j) { return k + j * a.k.t; }, a.Tk - j0, qrow, valid, a.D);
       unit = a.scale;
     } else {
-#pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const half8 kh = frag(2 * c), kl = frag(2 * c + 1);
-        x = mfma(kl, qh[c], x);
-        x = mfma(kh, ql[c], x);
-        x = mfma(kh, qh[c], x);
-      }
+      x = scores<KC>(L, 0, qh, ql);
       unit = a.scale * pow2(-qe) * (1.0f / kt.scale);
     }
     float f = 1;                   // exponent of 2 = f x (plain) or x (RICH)
@@ -293,18 +288,22 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
       f = unit * kLog2e;
     }
     if (!all_seen(s, me, kt, j0)) {
+      if (s.doc) {
+        int dj[16];
 #pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        const int j = j0 + 8 * (q / 4) + 4 * h + q % 4;
-        x[q] = j < a.Tk && sees(s, p, doc, j) ? x[q] : kNone;
+        for (int q = 0; q < 16; ++q) dj[q] = s.doc[min(j0 + 8 * (q / 4) + 4 * h + q % 4, a.Tk - 1)];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) x[q] = dj[q] == doc && doc >= 0 ? x[q] : kNone;
       }
+#pragma unroll
+      for (int q = 0; q < 16; ++q) x[q] = j0 + 8 * (q / 4) + 4 * h + q % 4 < below ? x[q] : kNone;
     }
     float top = x[0];
 #pragma unroll
     for (int q = 1; q < 16; ++q) top = fmaxf(top, x[q]);
     top = halves_max(top) * f;
     // The maximum moves only when it grows by more than 2^8 (or from nothing), so that most tiles leave acc alone: weights
-    // then reach 2^8 instead of 1, and their f16 parts at most 2^15.
+    // then reach 2^8 instead of 1.
     float keep = 1;
     if (top > m + 8 || (m == kNone && top > kNone)) {
       keep = __builtin_amdgcn_exp2f(m - top);
@@ -318,50 +317,29 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
 #pragma unroll
     for (int q = 0; q < 16; ++q) part += x[q];
     sum += part;
-    // acc's unit: 2^pe times the tile's scale, pe in 3..7 so that the weights' f16 parts stay within 2^15; it is kept from
-    // tile to tile while that holds
-    int pe = ce - exponent(vt.scale);
     float change = keep;
-    if (!vt.irregular && (pe < 3 || pe > 7)) {
-      const int want = 5 + exponent(vt.scale);
-      change *= pow2(want - ce);
-      ce = want;
-      pe = 5;
-    }
-    if (__any(change != 1)) {
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int q = 0; q < 16; ++q) acc[d][q] *= change;
-    }
     if (vt.irregular) {
       const float* v = a.v.p + b * a.v.b + hk * a.v.h + (int64_t)j0 * a.v.t;
-      plain_accumulate<DB>(acc, x, pow2(ce), [&](int j) { return v + j * a.v.t; }, a.Tk - j0, a.Dv);
+      rescale<DB>(acc, change);
+      plain_accumulate<DB>(acc, ce, x, [&](int j) { return v + j * a.v.t; }, a.Tk - j0, a.Dv);
       continue;
     }
-    const float ps = pow2(pe);
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      float z[8];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) z[q] = x[8 * ks + q] * ps;
-      half8 ph, pl;
-      split8(z, ph, pl);
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const half8 vh = frag(2 * KC + (d * 2 + ks) * 2), vl = frag(2 * KC + (d * 2 + ks) * 2 + 1);
-        acc[d] = mfma(vl, ph, acc[d]);
-        acc[d] = mfma(vh, pl, acc[d]);
-        acc[d] = mfma(vh, ph, acc[d]);
-      }
+    // what acc held has shrunk by `keep`: so may its unit
+    if (keep < 1 && ce != kUnset) {
+      const int shrunk = keep > 0 ? min(-exponent(keep) - 1, 100) : 0;
+      change *= pow2(shrunk);
+      ce += shrunk;
     }
+    const int e = fit_unit(ce, __builtin_amdgcn_exp2f(top - off), exponent(vt.scale), &change);
+    rescale<DB>(acc, change);
+    accumulate<DB>(acc, x, pow2(e), L, 2 * KC);
   }
 
   sum = halves_sum(sum);
   if (!valid) return;
   const bool none = sum == 0;      // not m: a visible NaN leaves no maximum
   const float lse = none ? (A.splits > 1 ? kNone : INFINITY) : m + __builtin_amdgcn_logf(sum);
-  const float out = none ? 0.0f : 1.0f / sum, unit = pow2(-ce);
+  const float out = none ? 0.0f : 1.0f / sum;
   float* y;
   if (A.splits > 1) {
     const int64_t at = ((int64_t)split * a.B * a.Hk + slab) * A.M + r;
@@ -380,7 +358,7 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
       const int at = 32 * d + 8 * q + 4 * h;
       f32x4 v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : acc[d][4 * q + e] * unit * out;
+      for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : __builtin_amdgcn_ldexpf(acc[d][4 * q + e], -ce) * out;
       if (wide) {
         if (at < a.Dv) *(f32x4*)(y + at) = v;
       } else {
@@ -423,13 +401,14 @@ __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
     }
   };
   float q[R][E], acc[R][E], m[R], sum[R];
-  int p[R], doc[R];
+  int p[R], doc[R], below[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int rr = min(r, A.M - 1), i = rr / G, head = hk * G + rr % G;
     load(a.q.p + b * a.q.b + head * a.q.h + i * a.q.t, a.D, q[r]);
     p[r] = s.first + i;
     doc[r] = doc_at(s, p[r]);
+    below[r] = sees_below(s, p[r]);
     m[r] = kNone;
     sum[r] = 0;
 #pragma unroll
@@ -474,7 +453,7 @@ __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
       if (a.cap > 0) x = a.cap * tanh_of(x / a.cap);
       if (a.slopes) x -= a.slopes[hk * G + min(r, A.M - 1) % G] * fabsf((float)(p[r] - j));
       x *= kLog2e;
-      if (!all && !sees(s, p[r], doc[r], j)) continue;
+      if (!all && (j >= below[r] || (s.doc && (doc[r] < 0 || s.doc[j] != doc[r])))) continue;
       if (x > m[r] + 8 || m[r] == kNone) {
         const float top = __builtin_isfinite(x) ? x : m[r] == kNone ? 0.0f : m[r];   // an infinite score shows in the weight
         const float keep = __builtin_amdgcn_exp2f(m[r] - top);
@@ -652,8 +631,8 @@ void attend(const AttendDesc& a, void* work, hipStream_t st) {
     k.Hk = a.Hk;
     k.wide = wide;
     k.a = a;
-    k.job[0] = {a.k, a.D, 1, a.Tk, p.tiles, (_Float16*)(w + p.kf), nullptr, (TileInfo*)(w + p.ki), a.documents, {}, nullptr};
-    k.job[1] = {a.v, a.Dv, 1, a.Tk, p.tiles, nullptr, (_Float16*)(w + p.vf), (TileInfo*)(w + p.vi), nullptr, {}, nullptr};
+    k.job[0] = {a.k, a.D, 1, a.Tk, p.tiles, (_Float16*)(w + p.kf), nullptr, (TileInfo*)(w + p.ki), false, {}, nullptr};
+    k.job[1] = {a.v, a.Dv, 1, a.Tk, p.tiles, nullptr, (_Float16*)(w + p.vf), (TileInfo*)(w + p.vi), false, {}, nullptr};
     attend_pack(k, p.DP, st);
     const TilesArgs t{a, (_Float16*)(w + p.kf), (_Float16*)(w + p.vf), (TileInfo*)(w + p.ki), (TileInfo*)(w + p.vi),
                       make_fastdiv(p.G), p.M, p.blocks, p.splits, wide, part, plse};

@@ -3,10 +3,13 @@
 Bounds count roundings in units U = 2^-24, half a step of f32. A product of two values may be taken from operands split
 into two 11-bit parts with the product of the low parts left out: each operand then keeps 22 bits (2^-22 = 4 U off at most)
 and the lost product is another 4 U, 12 U in all. A sum of n terms in f32 is off by about sqrt(n) U of its terms' absolute
-sum; 4 sqrt(n) U is allowed. A value's own last roundings (exp, log, tanh, a division) are 2 to 4 U each."""
+sum; 4 sqrt(n) U is allowed. A value's own last roundings (exp, log, tanh, a division) are 2 to 4 U each. A probability
+below 2^-126, the smallest normal f32, may count as zero (the hardware's exp2 gives no subnormals): each pair may be off by
+TINY = 2^-126, whatever its relative bound says."""
 import numpy as np
 
 U = 2.0 ** -24
+TINY = 2.0 ** -126
 
 
 def seen_mask(B, Tq, Tk, causal, slopes, documents, prefix, lengths):
@@ -72,7 +75,7 @@ def _attention(q, k, v, dy, causal, scale, softcap, slopes, documents, prefix, l
             vis = lambda w, z: np.stack([(w[i][m[i], None] * z[m[i]]).sum(0) for i in range(w.shape[0])])  # noqa: E731
             y = vis(P, V)
             out['y'][b, h] = y
-            tol['y'][b, h] = R * vis(P, np.abs(V))
+            tol['y'][b, h] = R * vis(P, np.abs(V)) + TINY * vis(m, np.abs(V))
             if dy is None:
                 continue
             G = pick(rows[:, None], dy[b, h])
@@ -82,7 +85,7 @@ def _attention(q, k, v, dy, causal, scale, softcap, slopes, documents, prefix, l
             ds = pick(m, P * (dP - Di) * fac)
             e_dp = (pick(m, (12 + 4 * np.sqrt(Dv)) * U * norm(G)[:, None] * norm(V)[None])
                     + ((np.abs(G) * tol['y'][b, h]).sum(1) + 4 * np.sqrt(Dv) * U * norm(G) * norm(y))[:, None])
-            e_ds = pick(m, P * ((R + 8 * U) * np.abs(dP - Di) * fac + e_dp * fac
+            e_ds = pick(m, TINY * np.abs(dP - Di) * fac + P * ((R + 8 * U) * np.abs(dP - Di) * fac + e_dp * fac
                                 + (np.abs(dP - Di) * (4 * U + 2 * np.abs(t) * (e_s / softcap if softcap else 0)))))
             out['dq'][b, h] = scale * vis(ds, K)
             tol['dq'][b, h] = scale * (vis(e_ds, np.abs(K)) + (16 + 4 * np.sqrt(Tk)) * U * vis(np.abs(ds), np.abs(K)))
@@ -92,7 +95,7 @@ def _attention(q, k, v, dy, causal, scale, softcap, slopes, documents, prefix, l
             out['dk'][b, h // g] += scale * visT(ds, Q)
             tol['dk'][b, h // g] += scale * (visT(e_ds, np.abs(Q)) + n * visT(np.abs(ds), np.abs(Q)))
             out['dv'][b, h // g] += visT(P, G)
-            tol['dv'][b, h // g] += (R.max() + n) * visT(P, np.abs(G))
+            tol['dv'][b, h // g] += (R.max() + n) * visT(P, np.abs(G)) + TINY * visT(m, np.abs(G))
     return out, tol
 
 
