@@ -1,81 +1,280 @@
 // Rotary positions of several axes and the gated linear recurrence for gfx950.
+#include <algorithm>
+
 #include "kernels.h"
 #include "sequence.h"
 
 namespace tgk {
 namespace {
 
-// A thread turns one pair of one row (b, t) in every head of every tensor.
-__global__ __launch_bounds__(256) void rope_pairs(RopeDesc r) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int units = r.D - r.half;            // pairs, then features that pass
-  if (id >= (int64_t)r.B * r.T * units) return;
-  const int u = (int)(id % units);
-  const int t = (int)(id / units % r.T), b = (int)(id / units / r.T);
+// ---- rotary positions ------------------------------------------------------------------------------
+//
+// Bound by memory: every value is read once and written once. A thread finds the angle of one pair of one row (b, t) and
+// turns that pair in `each` heads, all tensors' heads counted through, so that the angle costs little. Few rows: fewer heads
+// a thread, so that there are threads for the whole card.
+
+// cos and sin of position * freq. The product is taken in 64 bits and brought to r in [-pi/4, pi/4] by the nearest multiple
+// of pi/2 (in two parts, 2^-106 in all), where the Taylor series to r^9 and r^10 are off by less than 2^-28.
+__device__ __forceinline__ void angle(int position, double freq, float& c, float& s) {
+  const double x = (double)position * freq, n = rint(x * 0.63661977236758134308);
+  const float r = (float)fma(-n, 6.123233995736766e-17, fma(-n, 1.5707963267948966, x));
+  const float q = r * r;
+  const float sr = fmaf(r * q, fmaf(q, fmaf(q, fmaf(q, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), r);
+  const float cr = fmaf(q, fmaf(q, fmaf(q, fmaf(q, fmaf(q, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
+  const int k = (int)((long long)n & 3);
+  c = k & 1 ? sr : cr;
+  s = k & 1 ? cr : sr;
+  if (k == 1 || k == 2) c = -c;
+  if (k >= 2) s = -s;
+}
+
+struct RopeArgs {
+  RopeDesc d;
+  FastDiv units, T;
+  int total, each;                 // heads of all tensors; heads a thread
+};
+__global__ __launch_bounds__(256) void rope_pairs(RopeArgs R) {
+  const RopeDesc& r = R.d;
+  const uint32_t id = blockIdx.x * 256 + threadIdx.x, row = fastdiv(id, R.units), u = id - row * R.units.d;
+  if (row >= (uint32_t)(r.B * r.T)) return;
+  const int b = fastdiv(row, R.T), t = row - b * R.T.d;
+  const bool turn = (int)u < r.half;         // a pair, else a feature that passes
   float c = 1, s = 0;
-  const bool turn = u < r.half;
   if (turn) {
     const RopePair p = r.pairs[u];
-    double sd, cd;
-    sincos((double)r.positions[((int64_t)p.axis * r.B + b) * r.T + t] * p.freq, &sd, &cd);
-    c = (float)cd;
-    s = (float)sd;
+    angle(r.positions[((int64_t)p.axis * r.B + b) * r.T + t], p.freq, c, s);
   }
-  for (int i = 0; i < r.n; ++i) {
+  const int from = blockIdx.y * R.each, to = min(from + R.each, R.total);
+  int first = 0;                             // heads before this tensor
+  for (int i = 0; i < r.n; first += r.heads[i], ++i) {
+    const int h0 = max(from - first, 0), h1 = min(to - first, r.heads[i]);
     const float sg = r.inverse[i] ? -s : s;
-    for (int h = 0; h < r.heads[i]; ++h) {
-      const float* x = r.x[i].p + b * r.x[i].b + h * r.x[i].h + t * r.x[i].t;
-      float* y = r.y[i].p + b * r.y[i].b + h * r.y[i].h + t * r.y[i].t;
-      if (turn) {
-        const float x1 = x[u], x2 = x[u + r.half];
-        y[u] = x1 * c - x2 * sg;
-        y[u + r.half] = x2 * c + x1 * sg;
-      } else {
-        y[u + r.half] = x[u + r.half];
+    const float* x = r.x[i].p + b * r.x[i].b + t * r.x[i].t;
+    float* y = r.y[i].p + b * r.y[i].b + t * r.y[i].t;
+    for (int h = h0; h < h1; h += 4) {
+      float x1[4], x2[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float* xh = x + min(h + e, h1 - 1) * r.x[i].h;
+        x1[e] = turn ? xh[u] : 0.0f;
+        x2[e] = xh[u + r.half];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (h + e >= h1) break;
+        float* yh = y + (h + e) * r.y[i].h;
+        if (turn) yh[u] = x1[e] * c - x2[e] * sg;
+        yh[u + r.half] = turn ? x2[e] * c + x1[e] * sg : x2[e];
       }
     }
   }
 }
 
-__global__ __launch_bounds__(64) void scan_channels(ScanDesc s) {
-  const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x, b = blockIdx.y;
-  if (c >= s.C) return;
-  float h = s.h0 ? s.h0[b * s.C + c] : 0;
-  for (int64_t t = 0; t < s.T; ++t) {
-    const int64_t at = (b * s.T + t) * s.C + c;
-    h = fmaf(s.a[at], h, s.x[at]);
-    s.h[at] = h;
+// ---- gated linear recurrence -----------------------------------------------------------------------
+//
+// Bound by memory: a and x are read once and h written once (a, h, dh read, da, dx written). Channels alone do not fill the
+// card, so time is cut into chunks, and a chunk keeps its values in registers while it waits for what comes in:
+//  * a block holds 64 channels x 4 S steps, S steps a wavefront, a channel a lane. Each wavefront folds its steps into
+//    (A, H), h_out = A h_in + H; the block joins its four and publishes its own pair;
+//  * what comes in is joined from the pairs of the chunks before, in a fixed order whatever the timing (so results repeat bit
+//    for bit): first those of whole groups of kGroup chunks, which the last block of each group joins and publishes, then
+//    those of its own group;
+//  * then the steps are run again from registers, now with the true state, and stored.
+// A pair is one 64-bit word, stored and loaded whole at device scope; all ones mean "not there yet". A block takes its place
+// from a counter as it starts, and waits only for blocks of lower places: those are running, and publish their own pair
+// before they wait for anything, a group's pair after waiting for lower places only. So every wait ends.
+
+typedef unsigned long long word;
+constexpr int kGroup = 8;
+constexpr word kEmpty = ~0ull;
+
+__device__ __forceinline__ word look(const word* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float gates(word v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float value(word v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ void publish(word* at, float A, float H) {
+  word v = (word)__float_as_uint(H) << 32 | __float_as_uint(A);
+  if (v == kEmpty) v = kEmpty - 1;             // a NaN either way
+  __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// (A, H) followed by n pairs, `step` words apart, in order. Loads go out together; what is not there yet is asked for again.
+__device__ __forceinline__ void follow(float& A, float& H, const word* at, int64_t step, int n) {
+  for (int k0 = 0; k0 < n; k0 += kGroup) {
+    word v[kGroup];
+#pragma unroll
+    for (int k = 0; k < kGroup; ++k) v[k] = look(at + min(k0 + k, n - 1) * step);
+#pragma unroll
+    for (int k = 0; k < kGroup; ++k) {
+      if (k0 + k >= n) break;
+      while (v[k] == kEmpty) {
+        __builtin_amdgcn_s_sleep(2);
+        v[k] = look(at + (k0 + k) * step);
+      }
+      H = fmaf(gates(v[k]), H, value(v[k]));
+      A *= gates(v[k]);
+    }
   }
 }
 
-__global__ __launch_bounds__(64) void scan_grad_channels(ScanGradDesc s) {
-  const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x, b = blockIdx.y;
-  if (c >= s.C) return;
-  float carry = 0;
-  for (int64_t t = s.T - 1; t >= 0; --t) {
-    const int64_t at = (b * s.T + t) * s.C + c;
-    const float g = s.dh[at] + carry;
-    const float before = t > 0 ? s.h[at - s.C] : s.h0 ? s.h0[b * s.C + c] : 0;
-    if (s.da) s.da[at] = g * before;
-    if (s.dx) s.dx[at] = g;
-    carry = s.a[at] * g;
+struct ScanPlan {
+  int S, chunks, cblocks;          // steps a wavefront; chunks of 4 S steps; blocks of 64 channels over all batch entries
+  int64_t words;                   // pairs: of the chunks, then of the groups, [.][cblocks * 64]; then the place counter
+};
+ScanPlan scan_plan(int64_t B, int64_t T, int64_t C) {
+  ScanPlan p{};
+  p.cblocks = (int)(B * ((C + 63) / 64));
+  p.S = 32;
+  while (p.S > 4 && (T <= 2 * p.S || p.cblocks * ((T + 4 * p.S - 1) / (4 * p.S)) < 1024)) p.S /= 2;
+  p.chunks = (int)((T + 4 * p.S - 1) / (4 * p.S));
+  p.words = p.chunks > 1 ? (int64_t)(p.chunks + p.chunks / kGroup) * p.cblocks * 64 + 1 : 0;
+  return p;
+}
+
+__global__ __launch_bounds__(256) void scan_clear(word* w, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) w[i] = i == n - 1 ? 0 : kEmpty;   // the last word is the place counter
+}
+
+// Forward and backward in one form: step u = 0, 1, .. is t = u or t = T - 1 - u, state = gate * state + in. Backward the
+// state g[t + 1] comes in to step t through its gate a[t + 1].
+struct ScanArgs {
+  int64_t T, C;
+  int chunks, cblocks, per;        // per: channel blocks of a batch entry
+  const float *a, *in, *h0, *h;    // h: backward
+  float *out, *da, *dh0;           // out: h, or dx; each may be null backward
+  word* words;
+};
+
+template <int S, bool BACK>
+__global__ __launch_bounds__(256) void scan_chunks(ScanArgs s) {
+  __shared__ float fold[4][2][64], came[64];
+  __shared__ unsigned place;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int64_t row = (int64_t)s.cblocks * 64;
+  unsigned id = blockIdx.x;
+  if (s.chunks > 1) {
+    if (tid == 0) place = atomicAdd((unsigned*)(s.words + (s.chunks + s.chunks / kGroup) * row), 1u);
+    __syncthreads();
+    id = place;
   }
-  if (s.dh0) s.dh0[b * s.C + c] = carry;
+  const int chunk = id / s.cblocks, cb = id % s.cblocks, b = cb / s.per;
+  const int64_t c = (int64_t)(cb % s.per) * 64 + lane, cc = min(c, s.C - 1);
+  const int64_t u0 = ((int64_t)chunk * 4 + w) * S, base = (int64_t)b * s.T * s.C + cc;
+  const float h0 = s.h0 ? s.h0[(int64_t)b * s.C + cc] : 0.0f;
+  float g[S], x[S], before[BACK ? S : 1];
+#pragma unroll
+  for (int k = 0; k < S; ++k) {    // past the end: any value that is there, put right below
+    const int64_t u = min(u0 + k, s.T - 1), t = BACK ? s.T - 1 - u : u;
+    x[k] = s.in[base + t * s.C];
+    g[k] = s.a[base + (BACK ? min(t + 1, s.T - 1) : t) * s.C];
+    if (BACK) before[k] = s.da ? s.h[base + max(t - 1, (int64_t)0) * s.C] : 0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < S; ++k) {    // there the state goes on as it is
+    const int64_t u = u0 + k;
+    if (BACK && u == 0) g[k] = 0;  // nothing comes in to the last step
+    if (BACK && u == s.T - 1) before[k] = h0;
+    if (u >= s.T) {
+      x[k] = 0;
+      g[k] = 1;
+    }
+  }
+  float A = 1, H = 0;
+#pragma unroll
+  for (int k = 0; k < S; ++k) {
+    H = fmaf(g[k], H, x[k]);
+    A *= g[k];
+  }
+  fold[w][0][lane] = A;
+  fold[w][1][lane] = H;
+  __syncthreads();
+  float state = BACK ? 0.0f : h0;
+  if (s.chunks > 1) {
+    if (w == 0) {
+      word* pairs = s.words + (int64_t)cb * 64 + lane;
+      word* groups = pairs + s.chunks * row;
+      const int group = chunk / kGroup, in_group = chunk % kGroup;
+      float a4 = 1, h4 = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        h4 = fmaf(fold[k][0][lane], h4, fold[k][1][lane]);
+        a4 *= fold[k][0][lane];
+      }
+      publish(pairs + chunk * row, a4, h4);
+      float ga = 1, gh = 0, skip = 1;
+      follow(ga, gh, pairs + (int64_t)group * kGroup * row, row, in_group);      // the group's chunks before this one
+      if (in_group == kGroup - 1) publish(groups + group * row, ga * a4, fmaf(a4, gh, h4));
+      follow(skip, state, groups, row, group);
+      came[lane] = fmaf(ga, state, gh);
+    }
+    __syncthreads();
+    state = came[lane];
+  }
+  for (int k = 0; k < w; ++k) state = fmaf(fold[k][0][lane], state, fold[k][1][lane]);
+  if (c >= s.C) return;
+#pragma unroll
+  for (int k = 0; k < S; ++k) {
+    const int64_t u = u0 + k, t = BACK ? s.T - 1 - u : u;
+    if (u >= s.T) break;
+    state = fmaf(g[k], state, x[k]);
+    if (!BACK || s.out) s.out[base + t * s.C] = state;
+    if (BACK && s.da) s.da[base + t * s.C] = state * before[k];
+  }
+  if (BACK && s.dh0 && u0 < s.T && u0 + S >= s.T) s.dh0[(int64_t)b * s.C + c] = state * s.a[base];
 }
 
 }  // namespace
 
 void rope(const RopeDesc& r, hipStream_t st) {
-  const int64_t n = (int64_t)r.B * r.T * (r.D - r.half);
-  klaunch(rope_pairs, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, r);
+  RopeArgs R{r, make_fastdiv((uint32_t)(r.D - r.half)), make_fastdiv((uint32_t)r.T), 0, 0};
+  for (int i = 0; i < r.n; ++i) R.total += r.heads[i];
+  const int64_t threads = (int64_t)r.B * r.T * (r.D - r.half);
+  // 2^19 threads fill the card (256 CUs of 32 wavefronts); beyond, a thread takes all heads
+  R.each = (int)std::min<int64_t>(R.total, std::max<int64_t>(1, threads * R.total >> 19));
+  klaunch(rope_pairs, dim3((unsigned)((threads + 255) / 256), (unsigned)((R.total + R.each - 1) / R.each)), dim3(256), 0, st, R);
 }
 
-int64_t scan_workspace_bytes(int64_t, int64_t, int64_t) { return 0; }
-void scan(const ScanDesc& s, void*, hipStream_t st) {
-  klaunch(scan_channels, dim3((unsigned)((s.C + 63) / 64), (unsigned)s.B), dim3(64), 0, st, s);
+int64_t scan_workspace_bytes(int64_t B, int64_t T, int64_t C) { return scan_plan(B, T, C).words * 8; }
+
+namespace {
+template <bool BACK>
+void run_scan(ScanArgs s, int64_t B, void* work, hipStream_t st) {
+  const ScanPlan p = scan_plan(B, s.T, s.C);
+  s.chunks = p.chunks;
+  s.cblocks = p.cblocks;
+  s.per = (int)((s.C + 63) / 64);
+  s.words = (word*)work;
+  if (p.words) klaunch(scan_clear, dim3((unsigned)((p.words + 255) / 256)), dim3(256), 0, st, s.words, p.words);
+  const dim3 grid((unsigned)((int64_t)p.chunks * p.cblocks));
+  if (p.S == 32) klaunch(scan_chunks<32, BACK>, grid, dim3(256), 0, st, s);
+  else if (p.S == 16) klaunch(scan_chunks<16, BACK>, grid, dim3(256), 0, st, s);
+  else if (p.S == 8) klaunch(scan_chunks<8, BACK>, grid, dim3(256), 0, st, s);
+  else klaunch(scan_chunks<4, BACK>, grid, dim3(256), 0, st, s);
 }
-void scan_grad(const ScanGradDesc& s, void*, hipStream_t st) {
-  klaunch(scan_grad_channels, dim3((unsigned)((s.C + 63) / 64), (unsigned)s.B), dim3(64), 0, st, s);
+}  // namespace
+
+void scan(const ScanDesc& d, void* work, hipStream_t st) {
+  ScanArgs s{};
+  s.T = d.T;
+  s.C = d.C;
+  s.a = d.a;
+  s.in = d.x;
+  s.h0 = d.h0;
+  s.out = d.h;
+  run_scan<false>(s, d.B, work, st);
+}
+
+void scan_grad(const ScanGradDesc& d, void* work, hipStream_t st) {
+  ScanArgs s{};
+  s.T = d.T;
+  s.C = d.C;
+  s.a = d.a;
+  s.in = d.dh;
+  s.h0 = d.h0;
+  s.h = d.h;
+  s.out = d.dx;
+  s.da = d.da;
+  s.dh0 = d.dh0;
+  run_scan<true>(s, d.B, work, st);
 }
 
 }  // namespace tgk

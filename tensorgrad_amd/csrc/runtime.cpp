@@ -3952,6 +3952,7 @@ void Runtime::lower_scan(int i) {
   n.writes.push_back(root(h));
   n.flops = 2.0 * T_[a].numel;
   n.bytes = 12.0 * T_[a].numel;
+  expect(s[0] * ((s[2] + 63) / 64) * ((s[1] + 15) / 16) < (int64_t(1) << 31), i, "too large");
   const int64_t ws = tgk::scan_workspace_bytes(s[0], s[1], s[2]);
   workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
   n.ws = ws > 0;
@@ -3994,6 +3995,7 @@ void Runtime::lower_scan_grad(int i) {
   const int da = out[0], dx = out[1], dh0 = out[2];
   n.flops = 3.0 * T_[a].numel;
   n.bytes = 4.0 * T_[a].numel * (3 + (da >= 0) + (dx >= 0));
+  expect(s[0] * ((s[2] + 63) / 64) * ((s[1] + 15) / 16) < (int64_t(1) << 31), i, "too large");
   const int64_t ws = tgk::scan_workspace_bytes(s[0], s[1], s[2]);
   workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
   n.ws = ws > 0;
