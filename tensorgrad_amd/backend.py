@@ -176,6 +176,7 @@ class NativeRuntime:
             _check(lib().tg_runtime_create_sibling(parent._h, ir_json.encode(), ctypes.byref(h)))
         self._h = h
         self.parent = parent
+        self._last_names = None   # run_device: (names, their C array)
         n = lib().tg_param_count(h)
         self.param_names: List[str] = [lib().tg_param_name(h, i).decode() for i in range(n)]
         self.param_numel: Dict[str, int] = {self.param_names[i]: lib().tg_param_numel(h, i) for i in range(n)}
@@ -246,8 +247,11 @@ class NativeRuntime:
         """tg_run_device: a forward pass from device memory to device memory on `stream` (a hipStream_t as an int), without
         waiting for it."""
         n, m = len(names), len(out_ptrs)
-        _check(lib().tg_run_device(self._h, n, _names(names), (ctypes.c_void_p * n)(*dev_ptrs), (ctypes.c_int64 * n)(*nbytes),
-                                   m, (ctypes.c_void_p * m)(*out_ptrs), (ctypes.c_int64 * m)(*out_nbytes), stream))
+        if self._last_names is None or self._last_names[0] != tuple(names):
+            self._last_names = (tuple(names), _names(names))
+        _check(lib().tg_run_device(self._h, n, self._last_names[1], (ctypes.c_void_p * n)(*dev_ptrs),
+                                   (ctypes.c_int64 * n)(*nbytes), m, (ctypes.c_void_p * m)(*out_ptrs),
+                                   (ctypes.c_int64 * m)(*out_nbytes), stream))
 
     def state_names(self) -> List[str]:
         L = lib()

@@ -22,6 +22,7 @@ import numpy as np
 from .backend import AbortError, NativeRuntime
 from .build_ir import TrainingIR, build_forward_ir, build_training_ir, normalize_decl
 from .module import Module
+from .ops import PRNG_SEED_INPUT
 
 _DT = {'f32': np.float32, 'i32': np.int32, 'bool': np.int32}
 
@@ -77,30 +78,56 @@ def _guarded(body, cls):
         return cls('failed', error=e)
 
 
-def _on_device(name: str, x, dtype: str, size: int):
-    """(address, bytes) of a device tensor: contiguous, of the given dtype and element count. Any object with torch's
+_TORCH_DT: Dict = {}   # dtype object -> 'f32' / 'i32', by its name
+
+
+def _on_device(what: str, x, dtype: str, size: int) -> int:
+    """Address of a device tensor, checked: contiguous, of the given dtype and element count. Any object with torch's
     data_ptr / numel / is_contiguous / dtype will do."""
-    if not hasattr(x, 'data_ptr'):
-        raise TypeError(f'run_device: {name} must be a tensor in device memory, got {type(x).__name__}')
-    want = 'torch.float32' if dtype == 'f32' else 'torch.int32'
-    if str(x.dtype) != want:
-        raise TypeError(f'run_device: {name}: expected {want}, got {x.dtype}')
-    if x.numel() != size:
-        raise ValueError(f'run_device: {name}: expected {size} elements, got {x.numel()}')
-    if not x.is_contiguous():
-        raise ValueError(f'run_device: {name} must be contiguous')
-    return x.data_ptr(), 4 * size
+    try:
+        dt, n, whole, p = x.dtype, x.numel(), x.is_contiguous(), x.data_ptr()
+    except AttributeError:
+        raise TypeError(f'run_device: {what} must be a tensor in device memory, got {type(x).__name__}') from None
+    if dt not in _TORCH_DT:
+        _TORCH_DT[dt] = {'torch.float32': 'f32', 'torch.int32': 'i32'}.get(str(dt))
+    if _TORCH_DT[dt] != dtype:
+        raise TypeError(f"run_device: {what}: expected {'float32' if dtype == 'f32' else 'int32'}, got {dt}")
+    if n != size:
+        raise ValueError(f'run_device: {what}: expected {size} elements, got {n}')
+    if not whole:
+        raise ValueError(f'run_device: {what} must be contiguous')
+    return p
 
 
-def _run_device(rt: NativeRuntime, ir: TrainingIR, inputs, outputs, stream: int):
-    g = ir.graph
-    decls = {op['name']: g.tensors[op['out']] for op in g.ops if op['kind'] == 'tensor_input' and op['name'] in inputs}
-    given = [_on_device(f"input '{n}'", inputs[n], t.dtype, t.size) for n, t in decls.items()]
-    outs = [g.tensors[t] for t in g.outputs]
-    if len(outputs) != len(outs):
-        raise ValueError(f'run_device: the graph has {len(outs)} outputs, got {len(outputs)}')
-    to = [_on_device(f'output {i}', x, t.dtype, t.size) for i, (x, t) in enumerate(zip(outputs, outs))]
-    rt.run_device(list(decls), [p for p, _ in given], [n for _, n in given], [p for p, _ in to], [n for _, n in to], stream)
+class _DeviceCall:
+    """What run_device passes for one graph: its inputs and outputs in order, with their sizes."""
+
+    def __init__(self, ir: TrainingIR):
+        g = ir.graph
+        dt = lambda t: 'f32' if t.dtype == 'f32' else 'i32'  # noqa: E731
+        self.inputs = [(op['name'], f"input '{op['name']}'", dt(g.tensors[op['out']]), g.tensors[op['out']].size)
+                       for op in g.ops if op['kind'] == 'tensor_input' and op['name'] != PRNG_SEED_INPUT]
+        self.outputs = [(f'output {i}', dt(g.tensors[t]), g.tensors[t].size) for i, t in enumerate(g.outputs)]
+        self.names = tuple(n for n, _, _, _ in self.inputs)
+        self.in_bytes = tuple(4 * n for _, _, _, n in self.inputs)
+        self.out_bytes = tuple(4 * n for _, _, n in self.outputs)
+
+    def __call__(self, rt: NativeRuntime, inputs, outputs, stream: int) -> None:
+        for n in self.names:
+            if n not in inputs:
+                raise ValueError(f"run_device: missing input '{n}'")
+        if len(outputs) != len(self.outputs):
+            raise ValueError(f'run_device: the graph has {len(self.outputs)} outputs, got {len(outputs)}')
+        given = [_on_device(what, inputs[n], dt, size) for n, what, dt, size in self.inputs]
+        to = [_on_device(what, x, dt, size) for x, (what, dt, size) in zip(outputs, self.outputs)]
+        rt.run_device(self.names, given, self.in_bytes, to, self.out_bytes, stream)
+
+
+def _run_device(ir: TrainingIR, rt: NativeRuntime, inputs, outputs, stream: int) -> None:
+    call = ir.__dict__.get('_device_call')
+    if call is None:
+        call = ir._device_call = _DeviceCall(ir)
+    call(rt, inputs, outputs, stream)
 
 
 def _capture_meta(ir: TrainingIR):
@@ -162,13 +189,13 @@ class CompiledForward:
         """`run` within device memory, for tensors that stay on the GPU (no reference counterpart): reads `inputs` (tensors
         in device memory, by name) and writes the graph's outputs, all that the forward returned, into `outputs`; result
         `output` is `outputs`. The work is enqueued on `stream` (a hipStream_t as an int; 0: the default stream) and the call
-        returns without waiting for it. Calls on one executor run one after another, also from several streams. A stream
-        under graph capture is refused."""
+        returns without waiting for it. Calls on one executor run one after another, also from several streams; a stream must
+        stay until a later call on another one, a host call or `destroy`. A stream under graph capture is refused."""
         def body():
             if not self.parent._rt.alive:
                 raise AbortError('run aborted: graph destroyed')
             rt, ir = self._sibling(inputs)[:2]
-            _run_device(rt, ir, inputs, outputs, stream)
+            _run_device(ir, rt, inputs, outputs, stream)
             return RunResult('completed', output=outputs)
         return _guarded(body, RunResult)
 
@@ -308,7 +335,8 @@ class CompiledForwardExecutor:
         meta = {k: {'shape': [1 if d is None else d for d in s], 'dtype': dt} for k, (s, dt) in self.decls.items()}
         ir = build_forward_ir(self.model, self.forward, meta)
         self._param_names = ir.param_names
-        if all(d is not None for s, _ in self.decls.values() for d in s):
+        self._fixed = all(d is not None for s, _ in self.decls.values() for d in s)
+        if self._fixed:
             self._create_owner(meta, ir)
 
     @property
@@ -336,6 +364,8 @@ class CompiledForwardExecutor:
         return self._owner
 
     def _sibling(self, inputs):
+        if self._fixed and self._owner is not None:
+            return self._owner
         resolved = _resolve_decls(self.decls, inputs)
         key = _shape_key(resolved)
         if self._owner is None:
@@ -366,13 +396,13 @@ class CompiledForwardExecutor:
         """`run` within device memory, for tensors that stay on the GPU (no reference counterpart): reads `inputs` (tensors
         in device memory, by name) and writes the graph's outputs, all that the forward returned, into `outputs`; result
         `output` is `outputs`. The work is enqueued on `stream` (a hipStream_t as an int; 0: the default stream) and the call
-        returns without waiting for it. Calls on one executor run one after another, also from several streams. A stream
-        under graph capture is refused."""
+        returns without waiting for it. Calls on one executor run one after another, also from several streams; a stream must
+        stay until a later call on another one, a host call or `destroy`. A stream under graph capture is refused."""
         def body():
             if self._destroyed:
                 raise AbortError('run aborted: executor destroyed')
             rt, ir = self._sibling(inputs)[:2]
-            _run_device(rt, ir, inputs, outputs, stream)
+            _run_device(ir, rt, inputs, outputs, stream)
             return RunResult('completed', output=outputs)
         return _guarded(body, RunResult)
 

@@ -89,21 +89,19 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
     }
   }
   __syncthreads();
-  float hi = 0, lo = INFINITY;
-  int nm = -126, dmin = INT32_MAX, dmax = INT32_MIN;
-  bool bad = false, same = true;
-  for (int q = 0; q < kTile; ++q) {
-    const float t = top[q];
-    bad |= !(t < INFINITY);
-    hi = fmaxf(hi, t);
-    if (t > 0) lo = fminf(lo, t);
-    nm = max(nm, norm[q]);
-    if (doc[q] >= 0) {
-      dmin = min(dmin, doc[q]);
-      dmax = max(dmax, doc[q]);
-    }
-    same = same && doc[q] >= 0 && doc[q] == doc[0];
+  const int lane = tid & 63, w = tid >> 6, h = lane >> 5, l = lane & 31;
+  float hi = top[l], lo = hi > 0 ? hi : INFINITY;
+  int nm = norm[l], dmin = doc[l] >= 0 ? doc[l] : INT32_MAX, dmax = doc[l] >= 0 ? doc[l] : INT32_MIN;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    hi = fmaxf(hi, __shfl_xor(hi, o));
+    lo = fminf(lo, __shfl_xor(lo, o));
+    nm = max(nm, __shfl_xor(nm, o));
+    dmin = min(dmin, __shfl_xor(dmin, o));
+    dmax = max(dmax, __shfl_xor(dmax, o));
   }
+  bool bad = !(hi < INFINITY);
+  const bool same = dmin == dmax && !__any(doc[l] < 0);
   bad |= lo * 1048576.0f < hi;
   const float scale = bad || hi == 0 ? 1.0f : pow2(min(14 - exponent(hi), 126));
   const int64_t slot = (int64_t)slab * j.tiles + tile;
@@ -118,7 +116,6 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
     j.info[slot] = t;
   }
   if (bad) return;
-  const int lane = tid & 63, w = tid >> 6, h = lane >> 5, l = lane & 31;
   if (j.rowf)
     for (int c = w; c < KC; c += 4) {
       float z[8];
@@ -552,7 +549,7 @@ Plan plan(const AttendDesc& a) {
   p.M = p.G * a.Tq;
   p.slabs = a.B * a.Hk;
   p.tiles = (a.Tk + kTile - 1) / kTile;
-  p.few = p.M <= few_rows(p.DP);
+  p.few = p.M <= few_rows(p.DP) && (p.M <= 2 || a.Tk >= 32 * p.M);
   if (p.few) {
     p.blocks = 1;
     const int64_t want = (2048 + p.slabs - 1) / p.slabs, most = (a.Tk + 127) / 128;

@@ -123,7 +123,7 @@ ScanPlan scan_plan(int64_t B, int64_t T, int64_t C) {
   ScanPlan p{};
   p.cblocks = (int)(B * ((C + 63) / 64));
   p.S = 32;
-  while (p.S > 4 && (T <= 2 * p.S || p.cblocks * ((T + 4 * p.S - 1) / (4 * p.S)) < 1024)) p.S /= 2;
+  while (p.S > 4 && (T <= 2 * p.S || p.cblocks * ((T + 4 * p.S - 1) / (4 * p.S)) < 256)) p.S /= 2;
   p.chunks = (int)((T + 4 * p.S - 1) / (4 * p.S));
   p.words = p.chunks > 1 ? (int64_t)(p.chunks + p.chunks / kGroup) * p.cblocks * 64 + 1 : 0;
   return p;

@@ -319,13 +319,15 @@ class Runtime {
   const void* dev_table(const std::string& key, const void* data, size_t bytes);
   std::vector<int> state_roots_;
 
-  // Calls that return before their work is done (run_device): a family of runtimes, which share parameters, keeps the event
-  // of its last one. A later one waits for it on its own stream, every other entry point on the host.
+  // Calls that return before their work is done (run_device): a family of runtimes, which share parameters, keeps the
+  // stream of its last one. A later one on another stream waits for it there, every other entry point on the host. (An event
+  // recorded after every call would say the same, for 4 us of the stream's time.)
   struct Pending {
     std::mutex mu;
-    hipEvent_t done = nullptr;
     bool any = false;
-    ~Pending() { if (done) hipEventDestroy(done); }
+    hipStream_t stream = nullptr;
+    hipEvent_t passed = nullptr;
+    ~Pending() { if (passed) hipEventDestroy(passed); }
   };
   std::shared_ptr<Pending> pending_;
   int device_ = 0;
@@ -481,6 +483,7 @@ class Runtime {
   void split_init_nodes();
   void launch_all(hipStream_t st);
   void upload_inputs(int n, const char* const* names, const void* const* data, const int64_t* nbytes, bool device);
+  void need_staging();
   void advance_scalars(bool optimizer);
   void launch_step(hipStream_t st, bool host);
  public:
@@ -4872,8 +4875,7 @@ void Runtime::allocate() {
     return;
   }
   hip_check(hipMalloc(&input_region_, input_region_bytes_), "hipMalloc(inputs)");
-  hip_check(hipHostMalloc(&staging_, input_region_bytes_, hipHostMallocDefault), "hipHostMalloc");
-  memset(staging_, 0, input_region_bytes_);
+  if (opt_cfg_) need_staging();   // a forward graph's calls may all stay within device memory: at its first host call
   for (int t : input_roots) ptr_[t] = input_region_ + input_offset_[t];
   hip_check(hipHostMalloc(&loss_host_, 256, hipHostMallocDefault), "hipHostMalloc");
   if (workspace_bytes_) hip_check(hipMalloc(&workspace_, (workspace_bytes_ + 255) & ~(size_t)255), "hipMalloc(workspace)");
@@ -5040,7 +5042,14 @@ void Runtime::ensure_graph(bool host) {
   hip_check(hipGraphInstantiate(&graph_exec_[host], graph_[host], nullptr, nullptr, 0), "hipGraphInstantiate");
 }
 
+void Runtime::need_staging() {
+  if (staging_) return;
+  hip_check(hipHostMalloc(&staging_, input_region_bytes_, hipHostMallocDefault), "hipHostMalloc");
+  memset(staging_, 0, input_region_bytes_);
+}
+
 void Runtime::advance_scalars(bool optimizer) {
+  if (uses_prng_) need_staging();
   // Per-step scalars (src/worker.ts:187-214), written into the host mirror of the tail of
   // the input region. The worker bumps t and the seed counter before the runtime checks
   // the inputs (src/worker.ts:225, :249), so a rejected call still consumes both.
@@ -5085,6 +5094,7 @@ void Runtime::upload_inputs(int n, const char* const* names, const void* const* 
   for (auto& kv : input_tid_)
     if (input_offset_[kv.second] < user_bytes_ && !given.count(kv.second))
       throw Error(TG_INVALID_ARGUMENT, "missing input '" + kv.first + "'");
+  if (!device) need_staging();
   for (auto& g : given) {
     int t = g.first, i = g.second;
     if (device)
@@ -5161,7 +5171,9 @@ void Runtime::settle() {
   std::lock_guard<std::mutex> g(pending_->mu);
   if (!pending_->any) return;
   pending_->any = false;
-  hip_check(hipEventSynchronize(pending_->done), "hipEventSynchronize");
+  if (hipStreamSynchronize(pending_->stream) == hipSuccess) return;
+  (void)hipGetLastError();   // a stream that is gone
+  hip_check(hipDeviceSynchronize(), "hipDeviceSynchronize");
 }
 
 // One forward pass on the caller's stream, from and to the caller's device memory. Nodes that can take any addresses
@@ -5241,11 +5253,19 @@ void Runtime::run_device(int n, const char* const* names, const void* const* dat
   // The family's earlier calls use the same buffers (this runtime's) or parameters: wait for them on the stream. The seed
   // goes through pinned memory that the last call may still read: wait on the host.
   std::unique_lock<std::mutex> lock(pending_->mu);
-  if (!pending_->done) hip_check(hipEventCreateWithFlags(&pending_->done, hipEventDisableTiming), "hipEventCreate");
-  if (pending_->any) {
-    if (uses_prng_) hip_check(hipEventSynchronize(pending_->done), "hipEventSynchronize");
-    else hip_check(hipStreamWaitEvent(st, pending_->done, 0), "hipStreamWaitEvent");
+  if (pending_->any && (uses_prng_ || pending_->stream != st)) {
+    if (!pending_->passed) hip_check(hipEventCreateWithFlags(&pending_->passed, hipEventDisableTiming), "hipEventCreate");
+    if (uses_prng_ || hipEventRecord(pending_->passed, pending_->stream) != hipSuccess ||
+        hipStreamWaitEvent(st, pending_->passed, 0) != hipSuccess) {
+      (void)hipGetLastError();
+      if (hipStreamSynchronize(pending_->stream) != hipSuccess) {
+        (void)hipGetLastError();
+        hip_check(hipDeviceSynchronize(), "hipDeviceSynchronize");
+      }
+    }
   }
+  pending_->any = true;
+  pending_->stream = st;
   advance_scalars(false);
 
   std::vector<std::pair<int, void*>> saved;   // root -> its own address, put back below
@@ -5287,14 +5307,11 @@ void Runtime::run_device(int n, const char* const* names, const void* const* dat
     put_back();
     cur_ws_ = nullptr;
     cur_counters_ = nullptr;
-    if (hipEventRecord(pending_->done, st) == hipSuccess) pending_->any = true;
     throw;
   }
   put_back();
   cur_ws_ = nullptr;
   cur_counters_ = nullptr;
-  hip_check(hipEventRecord(pending_->done, st), "hipEventRecord");
-  pending_->any = true;
 }
 
 void Runtime::get_capture(const std::string& name, void* out, int64_t nbytes) {
