@@ -29,15 +29,16 @@ constexpr int kFrag = 512;         // halves of a fragment (1 KiB)
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kNone = -INFINITY;
 
-// What the kernels need to know of a packed tile. irregular: it holds infinities, NaN or rows whose largest values differ
-// by more than 2^20, so that one scale cannot serve it: it is multiplied in f32, value by value.
+// What the kernels need to know of a packed tile. One power of two serves all its rows, that of the largest, unless they
+// differ by more than 2^12 (uneven): then every row has its own, and what was multiplied by it takes the row's `rel`, the
+// tile's over the row's, afterwards. So a row keeps its precision whatever its neighbours are. odd: infinities, NaN or rows
+// 2^90 apart: blocks that walk such a tile run in plain f32.
 struct TileInfo {
-  float scale;                     // power of two on the packed values
-  int norm;                        // 2^norm bounds the rows' 2-norms
-  int irregular;
+  float scale, inv;                // power of two on the largest row's values, and its inverse
+  int uneven, odd;
   int dmin, dmax;                  // documents of its rows (>= 0 ones; none: dmin > dmax)
   int same;                        // all rows have one document
-  int pad[2];
+  int pad;
 };
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
@@ -78,16 +79,34 @@ __device__ __forceinline__ float halves_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// tanh, to a few units of its own last place: an odd rational form (continued fraction to x^5) where 1 - e^-2x would
-// cancel, else that. The rational form is off by less than 2^-25 of the value up to 0.625.
+// tanh. Up to kFlat by an odd polynomial (least squares in the relative error: 0.16 * 2^-24 off, 1.4 with f32's roundings);
+// above by 1 - e^-2x, which does not cancel there.
+constexpr float kFlat = 0.625f;
+__device__ __forceinline__ float tanh_flat(float x) {
+  const float q = x * x;
+  const float r = fmaf(q, fmaf(q, fmaf(q, fmaf(q, -0.00570404f, 0.02063786f), -0.05373916f), 0.13331432f), -0.33333281f);
+  return fmaf(x * q, r, x);
+}
 __device__ __forceinline__ float tanh_of(float x) {
-  const float z = fabsf(x), q = x * x;
-  const float e = __builtin_amdgcn_exp2f(-2 * kLog2e * z);
-  const bool small = z < 0.625f;
-  const float num = small ? z * fmaf(q, fmaf(q, 1.0f, 105.0f), 945.0f) : 1 - e;
-  const float den = small ? fmaf(q, fmaf(q, 15.0f, 420.0f), 945.0f) : 1 + e;
-  const float r = __builtin_amdgcn_rcpf(den);
-  return copysignf(num * r, x);
+  const float z = fabsf(x), e = __builtin_amdgcn_exp2f(-2 * kLog2e * z);
+  const float far = copysignf((1 - e) * __builtin_amdgcn_rcpf(1 + e), x);
+  return z < kFlat ? tanh_flat(x) : far;
+}
+// x = tanh(x u), all 16; the polynomial alone where no lane needs more
+__device__ __forceinline__ void tanh_all(f32x16& x, float u) {
+  float m = 0;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    x[q] *= u;
+    m = fmaxf(m, fabsf(x[q]));
+  }
+  if (__any(m >= kFlat)) {
+#pragma unroll
+    for (int q = 0; q < 16; ++q) x[q] = tanh_of(x[q]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 16; ++q) x[q] = tanh_flat(x[q]);
+  }
 }
 
 // What the queries of one batch entry see, wave-uniform.
@@ -139,34 +158,15 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
 
-// Row r of tile-ordered rows: r = i G + g is position i of the g-th query head that shares the key head (keys: G = 1).
-struct RowMap {
-  const float* p;                  // of (b, first head)
-  int64_t h, t;
-  FastDiv group;
-  __device__ __forceinline__ const float* row(int r) const {
-    const uint32_t i = fastdiv((uint32_t)r, group), g = (uint32_t)r - i * group.d;
-    return p + g * h + i * t;
-  }
-};
-__device__ __forceinline__ RowMap row_map(const Rows& x, int b, int head, const FastDiv& group) {
-  return {x.p + b * x.b + head * x.h, x.h, x.t, group};
-}
-
-// An exponent that bounds a 2-norm: values of at most `top`, whose squares relative to it sum to sq.
-__device__ __forceinline__ int norm_exponent(float top, float sq) {
-  return top > 0 ? exponent(top) + 1 + (exponent(sq) + 2) / 2 : -126;
-}
 __device__ __forceinline__ float finite_abs(float x) {
   x = fabsf(x);
   return x < INFINITY ? x : 0.0f;
 }
 
-// B fragments of 32 rows (lane l: row l % 32), each row with its own power of two; returns its exponent, and in *norm a bound
-// on its 2-norm. wide: rows are 16-byte aligned and n a multiple of 8.
+// B fragments of 32 rows (lane l: row l % 32), each row with its own power of two; returns its exponent. wide: rows are
+// 16-byte aligned and n a multiple of 8.
 template <int KC>
-__device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bool wide, half8 (&hi)[KC], half8 (&lo)[KC],
-                                         int* norm = nullptr) {
+__device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bool wide, half8 (&hi)[KC], half8 (&lo)[KC]) {
   const int h = (threadIdx.x >> 5) & 1;
   float x[KC][8];
 #pragma unroll
@@ -191,18 +191,6 @@ __device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bo
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(x[c][i]));   // the others stay what they are
   m = halves_max(m);
-  if (norm) {
-    float sq = 0;
-    const float inv = m > 0 ? 1.0f / fmaxf(m, 1e-37f) : 0.0f;
-#pragma unroll
-    for (int c = 0; c < KC; ++c)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float z = finite_abs(x[c][i]) * inv;
-        sq = fmaf(z, z, sq);
-      }
-    *norm = norm_exponent(m, halves_sum(sq));
-  }
   const int e = m > 0 ? min(14 - exponent(m), 126) : 0;
   const float s = pow2(e);
 #pragma unroll
@@ -214,24 +202,6 @@ __device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bo
   return e;
 }
 
-// Products in f32, value by value, for tiles that one scale cannot serve (rare, so small code rather than fast).
-// s[r] = row(8 (r / 4) + 4 h + r % 4 of the tile) . mine, for n features.
-template <class RowOf>
-__device__ __forceinline__ void plain_scores(f32x16& s, RowOf row_of, int rows, const float* mine, bool valid, int n) {
-  const int h = (threadIdx.x >> 5) & 1;
-#pragma unroll 1
-  for (int q = 0; q < 16; ++q) {
-    const int j = 8 * (q / 4) + 4 * h + q % 4;
-    float x = 0;
-    if (valid && j < rows) {
-      const float* a = row_of(j);
-#pragma unroll 1
-      for (int d = 0; d < n; ++d) x = fmaf(a[d], mine[d], x);
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = r == q ? x : s[r];
-  }
-}
 // Sums over several tiles in one accumulator: the weights (f16 parts of x 2^e) times a tile packed at 2^t are in units of
 // 2^-(e + t), which must be the accumulator's 2^-c. A lane's c only falls, when a tile's largest weight `big` would pass
 // 2^14: what comes later and is smaller is rounded like the largest of the sum (2^-37 of it), what was hidden has weight 0
@@ -254,78 +224,172 @@ __device__ __forceinline__ void rescale(f32x16 (&acc)[DB], float change) {
 #pragma unroll
     for (int q = 0; q < 16; ++q) acc[d][q] *= change;
 }
-// acc (columns: lanes, rows: features) += sum over the tile's rows j of row(j) * w[j] in f32, rows of weight 0 left out. The
-// values go in as they are, so acc leaves its unit for the sum, and returns to it unless they are too large for it.
-template <int DB, class RowOf>
-__device__ __forceinline__ void plain_accumulate(f32x16 (&acc)[DB], int& c, const f32x16& w, RowOf row_of, int rows, int n) {
-  const int lane = threadIdx.x & 63, h = lane >> 5;
-  rescale<DB>(acc, __builtin_amdgcn_ldexpf(1.0f, c == kUnset ? 0 : -c));
-#pragma unroll 1
-  for (int j = 0; j < min(rows, kTile); ++j) {
-    const int at = 4 * (j / 8) + j % 4;
-    float x = 0;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) x = r == at ? w[r] : x;
-    x = __shfl(x, (lane & 31) + 32 * ((j / 4) & 1));
-    const float* a = row_of(j);
-#pragma unroll
-    for (int b = 0; b < DB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int d = 32 * b + 8 * (r / 4) + 4 * h + r % 4;
-        if (d < n && x != 0) acc[b][r] = fmaf(x, a[d], acc[b][r]);
-      }
-  }
-  float m = 0;
-#pragma unroll
-  for (int b = 0; b < DB; ++b)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) m = fmaxf(m, finite_abs(acc[b][r]));
-  m = halves_max(m);
-  if (m > 0) c = min(min(c == kUnset ? 26 - exponent(m) : c, 110 - exponent(m)), 120);
-  rescale<DB>(acc, pow2(c == kUnset ? 0 : c));
-}
-
-// acc += A fragments (feature blocks x two k steps, from fragment f0 of L) times the split of x * scale
+__device__ __forceinline__ half8 frag(const _Float16* L, int f) { return *(const half8*)(L + f * kFrag + (threadIdx.x & 63) * 8); }
+// acc += A fragments (feature blocks x two k steps, from fragment f0 of L) times the split of x * scale. Fragments are read
+// one step ahead of the products that take them; products of different accumulators alternate.
 template <int DB>
 __device__ __forceinline__ void accumulate(f32x16 (&acc)[DB], const f32x16& x, float scale, const _Float16* L, int f0) {
-  const int lane = threadIdx.x & 63;
+  half8 ah[2][DB], al[2][DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) {
+    ah[0][d] = frag(L, f0 + d * 4);
+    al[0][d] = frag(L, f0 + d * 4 + 1);
+  }
+  half8 bh[2], bl[2];
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
     float z[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) z[q] = x[8 * ks + q] * scale;
-    half8 bh, bl;
-    split8(z, bh, bl);
+    split8(z, bh[ks], bl[ks]);
+  }
 #pragma unroll
-    for (int d = 0; d < DB; ++d) {
-      const half8 ah = *(const half8*)(L + (f0 + (d * 2 + ks) * 2) * kFrag + lane * 8);
-      const half8 al = *(const half8*)(L + (f0 + (d * 2 + ks) * 2 + 1) * kFrag + lane * 8);
-      acc[d] = mfma(al, bh, acc[d]);
-      acc[d] = mfma(ah, bl, acc[d]);
-      acc[d] = mfma(ah, bh, acc[d]);
-    }
+  for (int ks = 0; ks < 2; ++ks) {
+    if (ks == 0)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        ah[1][d] = frag(L, f0 + d * 4 + 2);
+        al[1][d] = frag(L, f0 + d * 4 + 3);
+      }
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d] = mfma(al[ks][d], bh[ks], acc[d]);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d] = mfma(ah[ks][d], bl[ks], acc[d]);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d] = mfma(ah[ks][d], bh[ks], acc[d]);
   }
 }
-// A fragments (KC k steps, from fragment f0 of L) times B fragments
+// A fragments (KC k steps, from fragment f0 of L) times B fragments; two accumulators take turns.
 template <int KC>
 __device__ __forceinline__ f32x16 scores(const _Float16* L, int f0, const half8 (&bh)[KC], const half8 (&bl)[KC]) {
-  const int lane = threadIdx.x & 63;
-  f32x16 x = {};
+  f32x16 x = {}, y = {};
+  half8 ah[2], al[2];
+  ah[0] = frag(L, f0);
+  al[0] = frag(L, f0 + 1);
 #pragma unroll
   for (int c = 0; c < KC; ++c) {
-    const half8 ah = *(const half8*)(L + (f0 + 2 * c) * kFrag + lane * 8), al = *(const half8*)(L + (f0 + 2 * c + 1) * kFrag + lane * 8);
-    x = mfma(al, bh[c], x);
-    x = mfma(ah, bl[c], x);
-    x = mfma(ah, bh[c], x);
+    if (c + 1 < KC) {
+      ah[(c + 1) & 1] = frag(L, f0 + 2 * c + 2);
+      al[(c + 1) & 1] = frag(L, f0 + 2 * c + 3);
+    }
+    y = mfma(al[c & 1], bh[c], y);
+    x = mfma(ah[c & 1], bh[c], x);
+    y = mfma(ah[c & 1], bl[c], y);
   }
+#pragma unroll
+  for (int q = 0; q < 16; ++q) x[q] += y[q];
   return x;
+}
+// x[q] *= rel of the tile's row 8 (q / 4) + 4 h + q % 4
+__device__ __forceinline__ void per_row(f32x16& x, const float* rel) {
+  const int h = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int q4 = 0; q4 < 4; ++q4) {
+    const f32x4 r = *(const f32x4*)(rel + 8 * q4 + 4 * h);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * q4 + e] *= r[e];
+  }
 }
 __device__ __forceinline__ float largest(const f32x16& x) {   // magnitude, over a row's two lane halves
   float m = 0;
 #pragma unroll
   for (int q = 0; q < 16; ++q) m = fmaxf(m, fabsf(x[q]));
   return halves_max(m);
+}
+
+// This lane's column of acc (features), in units of 2^-c, to a row in memory.
+template <int DB>
+__device__ __forceinline__ void store_row(float* row, const f32x16 (&acc)[DB], int c, float scale, int n, bool wide) {
+  const int h = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int at = 32 * d + 8 * q + 4 * h;
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_ldexpf(acc[d][4 * q + e], -c) * scale;
+      if (wide) {
+        if (at < n) *(f32x4*)(row + at) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (at + e < n) row[at + e] = v[e];
+      }
+    }
+}
+
+// First and one past the last of the tiles [t0, t1) whose documents meet [lo, hi] (all of them without documents); odd: one
+// of those is. By the whole block.
+struct Range {
+  int t0, t1;
+  bool odd;
+};
+__device__ __forceinline__ Range tile_range(const Sight& s, int t0, int t1, const TileInfo* docs, const TileInfo* x, const TileInfo* y,
+                                            int dmin, int dmax, int (&buf)[5]) {
+  const int tid = threadIdx.x;
+  if (tid < 5) buf[tid] = tid == 0 || tid == 2 ? INT32_MAX : tid == 4 ? 0 : INT32_MIN;
+  __syncthreads();
+  if ((tid & 63) == 0 && s.doc) {
+    atomicMin(&buf[0], dmin);
+    atomicMax(&buf[1], dmax);
+  }
+  __syncthreads();
+  const int lo = buf[0], hi = buf[1];
+  int first = INT32_MAX, end = INT32_MIN, odd = 0;
+  for (int t = t0 + tid; t < t1; t += 256) {
+    if (s.doc && !(docs[t].dmin <= hi && lo <= docs[t].dmax)) continue;
+    first = min(first, t);
+    end = max(end, t + 1);
+    odd |= x[t].odd | y[t].odd;
+  }
+  if (first != INT32_MAX) {
+    atomicMin(&buf[2], first);
+    atomicMax(&buf[3], end);
+    if (odd) atomicOr(&buf[4], 1);
+  }
+  __syncthreads();
+  Range r;
+  r.t0 = __builtin_amdgcn_readfirstlane(buf[2]);
+  r.t1 = __builtin_amdgcn_readfirstlane(buf[3]);
+  r.odd = __builtin_amdgcn_readfirstlane(buf[4]) != 0;
+  if (r.t0 >= r.t1) r.t0 = r.t1 = 0;
+  return r;
+}
+
+// ---- plain f32, for blocks that walk an odd tile: a wavefront takes one row at a time, a lane a pair ----
+
+struct PlainPair {
+  float score, slack;              // log2; 1 - tanh^2
+};
+__device__ __forceinline__ float plain_dot(const float* x, const float* y, int n) {
+  float s = 0;
+#pragma unroll 1
+  for (int d = 0; d < n; ++d) s = fmaf(x[d], y[d], s);
+  return s;
+}
+__device__ __forceinline__ PlainPair plain_score(const AttendDesc& a, float dot, float slope, int far) {
+  PlainPair r;
+  float x = dot * a.scale, t = 0;
+  if (a.cap > 0) {
+    t = tanh_of(x / a.cap);
+    x = a.cap * t;
+  }
+  r.score = (x * kLog2e) - slope * fabsf((float)far);
+  r.slack = fmaf(-t, t, 1.0f);
+  return r;
+}
+// acc[e] += w of each lane k times rows(k)[64 e + lane], lanes of weight 0 left out
+template <class RowOf>
+__device__ __forceinline__ void plain_add(float (&acc)[2], float w, RowOf row_of, int n) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (int k = 0; k < 64; ++k) {
+    const float x = __shfl(w, k);
+    if (x == 0) continue;
+    const float* r = row_of(k);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) if (64 * e + lane < n) acc[e] = fmaf(x, r[64 * e + lane], acc[e]);
+  }
 }
 
 // Blocks of one slab (batch entry and key head) on one XCD, whose L2 then holds its packed tiles: hardware deals block ids
@@ -345,12 +409,15 @@ struct PackJob {
   int n, G, rows, tiles;           // features; heads that share a key head; rows = positions * G; tiles
   _Float16 *rowf, *colf;           // [slab][tile][2 KC][512], [slab][tile][4 DB][512], or null
   TileInfo* info;                  // [slab][tile]
-  bool query;                      // rows are queries: their documents are those at their positions
-  // of the gradient dy: y's rows for its dot products, and what the key blocks need of each row, else null
-  Rows y;
-  float* rowinfo;                  // [slab][tile][kRowInfo][32]
+  bool query;                      // rows are queries, else keys
+  float* side;                     // [slab][tile][kSide][32]: what a block needs of each row of the tile, see below
+  int rel;                         // where this operand's rel goes
+  bool ids;                        // this job also writes the rows' documents and the rest
+  Rows y;                          // of the gradient dy (ids of queries): y's rows for its dot products
 };
-enum { RI_LSE, RI_DOT, RI_POS, RI_SLOPE, RI_BELOW, RI_DOC, kRowInfo = 8 };   // dot(dy, y); sees keys below; ints as bits
+// Rows of a side block, 32 values each (integers as bits), 1 KiB in all: of queries and of keys.
+enum { QS_LSE, QS_DOT, QS_POS, QS_SLOPE, QS_BELOW, QS_DOC, QS_RELQ, QS_RELG, kSide = 8 };   // dot(dy, y); sees keys below
+enum { KS_DOC, KS_RELK, KS_RELV };
 // The attention's operands as packed for one pass, in the workspace.
 struct Packs {
   int n;

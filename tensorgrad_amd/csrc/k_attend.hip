@@ -14,23 +14,26 @@ namespace {
 
 // ---- packing -------------------------------------------------------------------------------------
 
-// A block packs one tile of 32 rows: reads them once, finds the tile's scale, writes its fragments.
+// A block packs one tile of 32 rows: reads them once, finds their scales, writes its fragments. Rows that see nothing and
+// are seen by nothing are packed as zeros, whatever they hold.
 template <int DP>
 __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
   constexpr int KC = DP / 16, DB = DP / 32, LD = DP + 4;
   __shared__ float x[kTile * LD];
-  __shared__ float top[kTile];
-  __shared__ int norm[kTile], doc[kTile];
+  __shared__ float top[kTile], own[kTile];
+  __shared__ int doc[kTile];
   const PackJob j = p.job[blockIdx.z];
   const int tile = blockIdx.x, slab = blockIdx.y, b = slab / p.Hk, hk = slab % p.Hk;
   if (tile >= j.tiles) return;
+  const Sight s = sight(p.a, b);
   const int tid = threadIdx.x, row = tid / 8, sub = tid % 8, r = tile * kTile + row;
-  const bool in = r < j.rows;
-  const int i = r / j.G, g = r - i * j.G;
+  const int i = r / j.G, g = r - i * j.G, pos = j.query ? s.first + i : r;
+  const int id = r < j.rows ? doc_at(s, pos) : -1;
+  const bool in = r < j.rows && (!s.doc || id >= 0) && (j.query ? !s.positional || pos >= 0 : pos < s.n);
   const int64_t at = b * j.x.b + (int64_t)(hk * j.G + g) * j.x.h + (int64_t)i * j.x.t;
+  const bool dots = j.ids && j.query;
   float m = 0, dot = 0;
   bool odd = false;
-  float v[DP / 8];
 #pragma unroll
   for (int c = 0; c < DB; ++c) {
     const int d = 4 * (sub + 8 * c);
@@ -45,10 +48,9 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
     for (int q = 0; q < 4; ++q) {
       odd |= !(fabsf(u[q]) < INFINITY);
       m = fmaxf(m, finite_abs(u[q]));
-      v[4 * c + q] = u[q];
     }
     *(f32x4*)(x + row * LD + d) = u;
-    if (j.rowinfo && in) {
+    if (dots && in) {
       const int64_t ay = b * j.y.b + (int64_t)(hk * j.G + g) * j.y.h + (int64_t)i * j.y.t;
 #pragma unroll
       for (int q = 0; q < 4; ++q) if (d + q < j.n) dot = fmaf(u[q], j.y.p[ay + d + q], dot);
@@ -60,83 +62,71 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
     dot += __shfl_xor(dot, o);
     odd = __shfl_xor((int)odd, o) || odd;
   }
-  // the 2-norm, from values relative to the largest so that nothing overflows: 2^norm >= it
-  float sq = 0;
-  const float inv = m > 0 ? 1.0f / fmaxf(m, 1e-37f) : 0.0f;
-#pragma unroll
-  for (int q = 0; q < DP / 8; ++q) {
-    const float z = finite_abs(v[q]) * inv;
-    sq = fmaf(z, z, sq);
-  }
-#pragma unroll
-  for (int o = 1; o < 8; o *= 2) sq += __shfl_xor(sq, o);
+  float* side = j.side + ((int64_t)slab * j.tiles + tile) * (kSide * kTile);
   if (sub == 0) {
-    const Sight s = sight(p.a, b);
-    const int pos = j.query ? s.first + i : r;
     top[row] = odd ? INFINITY : m;
-    norm[row] = norm_exponent(m, sq);
-    doc[row] = in ? doc_at(s, pos) : -1;
-    if (j.rowinfo) {
+    doc[row] = id;
+    if (dots) {
       const AttendDesc& a = p.a;
       const int h = hk * j.G + g;
-      float* o = j.rowinfo + ((int64_t)slab * j.tiles + tile) * (kRowInfo * kTile) + row;
-      o[RI_LSE * kTile] = in ? a.lse[((int64_t)b * a.H + h) * a.Tq + i] : INFINITY;
-      o[RI_DOT * kTile] = in ? dot : 0.0f;
-      o[RI_POS * kTile] = __int_as_float(pos);
-      o[RI_SLOPE * kTile] = in && a.slopes ? a.slopes[h] * kLog2e : 0.0f;
-      o[RI_BELOW * kTile] = __int_as_float(in ? sees_below(s, pos) : 0);
-      o[RI_DOC * kTile] = __int_as_float(doc[row]);
+      side[QS_LSE * kTile + row] = in ? a.lse[((int64_t)b * a.H + h) * a.Tq + i] : INFINITY;
+      side[QS_DOT * kTile + row] = in ? dot : 0.0f;
+      side[QS_POS * kTile + row] = __int_as_float(pos);
+      side[QS_SLOPE * kTile + row] = in && a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+      side[QS_BELOW * kTile + row] = __int_as_float(in ? sees_below(s, pos) : 0);
+      side[QS_DOC * kTile + row] = __int_as_float(id);
+    } else if (j.ids) {
+      side[KS_DOC * kTile + row] = __int_as_float(id);
     }
   }
   __syncthreads();
   const int lane = tid & 63, w = tid >> 6, h = lane >> 5, l = lane & 31;
-  float hi = top[l], lo = hi > 0 ? hi : INFINITY;
-  int nm = norm[l], dmin = doc[l] >= 0 ? doc[l] : INT32_MAX, dmax = doc[l] >= 0 ? doc[l] : INT32_MIN;
+  const float mine = top[l];
+  float hi = mine, lo = mine > 0 ? mine : INFINITY;
+  int dmin = doc[l] >= 0 ? doc[l] : INT32_MAX, dmax = doc[l] >= 0 ? doc[l] : INT32_MIN;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
     hi = fmaxf(hi, __shfl_xor(hi, o));
     lo = fminf(lo, __shfl_xor(lo, o));
-    nm = max(nm, __shfl_xor(nm, o));
     dmin = min(dmin, __shfl_xor(dmin, o));
     dmax = max(dmax, __shfl_xor(dmax, o));
   }
-  bool bad = !(hi < INFINITY);
-  const bool same = dmin == dmax && !__any(doc[l] < 0);
-  bad |= lo * 1048576.0f < hi;
-  const float scale = bad || hi == 0 ? 1.0f : pow2(min(14 - exponent(hi), 126));
+  const bool bad = !(hi < INFINITY) || (hi > 0 && exponent(hi) - exponent(lo) > 90);
+  const bool uneven = !bad && hi > 0 && exponent(hi) - exponent(lo) > 12, same = dmin == dmax && !__any(doc[l] < 0);
+  const int e = bad || hi == 0 ? 0 : min(14 - exponent(hi), 126);
   const int64_t slot = (int64_t)slab * j.tiles + tile;
-  if (tid == 0) {
-    TileInfo t{};
-    t.scale = scale;
-    t.norm = nm;
-    t.irregular = bad;
-    t.dmin = dmin;
-    t.dmax = dmax;
-    t.same = same;
-    j.info[slot] = t;
+  if (tid == 0) j.info[slot] = {pow2(e), pow2(-e), uneven, bad, dmin, dmax, same, 0};
+  if (tid < kTile) {
+    const int mye = uneven && mine > 0 ? min(14 - exponent(mine), 126) : e;
+    own[l] = pow2(mye);
+    side[j.rel * kTile + l] = pow2(e - mye);
   }
   if (bad) return;
+  __syncthreads();
   if (j.rowf)
     for (int c = w; c < KC; c += 4) {
       float z[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) z[q] = x[l * LD + 16 * c + 8 * h + q] * scale;
-      half8 a, e;
-      split8(z, a, e);
+      for (int q = 0; q < 8; ++q) z[q] = x[l * LD + 16 * c + 8 * h + q] * own[l];
+      half8 a, f;
+      split8(z, a, f);
       half8* o = (half8*)(j.rowf + (slot * KC + c) * 2 * kFrag) + lane;
       o[0] = a;
-      o[kFrag / 8] = e;
+      o[kFrag / 8] = f;
     }
   if (j.colf)
     for (int c = w; c < 2 * DB; c += 4) {   // feature block c / 2, k step c % 2
       float z[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) z[q] = x[(16 * (c % 2) + 8 * (q / 4) + 4 * h + q % 4) * LD + 32 * (c / 2) + l] * scale;
-      half8 a, e;
-      split8(z, a, e);
+      for (int q = 0; q < 8; ++q) {
+        const int k = 16 * (c % 2) + 8 * (q / 4) + 4 * h + q % 4;
+        z[q] = x[k * LD + 32 * (c / 2) + l] * own[k];
+      }
+      half8 a, f;
+      split8(z, a, f);
       half8* o = (half8*)(j.colf + (slot * 2 * DB + c) * 2 * kFrag) + lane;
       o[0] = a;
-      o[kFrag / 8] = e;
+      o[kFrag / 8] = f;
     }
 }
 
@@ -146,17 +136,72 @@ struct TilesArgs {
   AttendDesc a;
   const _Float16 *kf, *vf;         // k's row fragments, v's column fragments
   const TileInfo *ki, *vi;
+  const float* side;
   FastDiv group;                   // G
   int M, blocks, splits;           // rows of a slab, row blocks, parts of the key axis
   bool wide;
   float *part, *plse;              // parts: [split][slab][M][Dv], [split][slab][M]
 };
 
+// Where a row's result goes, and its lse.
+__device__ __forceinline__ float* result_row(const TilesArgs& A, int split, int slab, int b, int head, int r, int i, float lse, bool none,
+                                             bool writes) {
+  const AttendDesc& a = A.a;
+  if (A.splits > 1) {
+    const int64_t at = ((int64_t)split * a.B * a.Hk + slab) * A.M + r;
+    if (writes) A.plse[at] = none ? kNone : lse;
+    return A.part + at * a.Dv;
+  }
+  if (writes && a.lse) a.lse[((int64_t)b * a.H + head) * a.Tq + i] = none ? INFINITY : lse;
+  return a.y.p ? a.y.p + b * a.y.b + head * a.y.h + (int64_t)i * a.y.t : nullptr;
+}
+
+// A wavefront's rows [row0, row0 + 32) over keys [j0, j1) in plain f32.
+__device__ __forceinline__ void plain_rows(const TilesArgs& A, const Sight& s, int split, int slab, int b, int hk, int row0, int j0, int j1) {
+  const AttendDesc& a = A.a;
+  const int lane = threadIdx.x & 63, G = (int)A.group.d;
+  const float* k = a.k.p + b * a.k.b + hk * a.k.h;
+  const float* v = a.v.p + b * a.v.b + hk * a.v.h;
+#pragma unroll 1
+  for (int r = row0; r < min(row0 + kTile, A.M); ++r) {
+    const int i = r / G, head = hk * G + r % G, p = s.first + i, doc = doc_at(s, p), end = min(j1, sees_below(s, p));
+    const float* q = a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t;
+    const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+    auto shown = [&](int j) { return j < end && (!s.doc || (doc >= 0 && s.doc[j] == doc)); };
+    auto score = [&](int j) { return plain_score(a, plain_dot(k + j * a.k.t, q, a.D), slope, p - j).score; };
+    float m = kNone;
+    bool any = false;
+#pragma unroll 1
+    for (int j = j0 + lane; j < end; j += 64)
+      if (shown(j)) {
+        m = fmaxf(m, score(j));
+        any = true;
+      }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
+    const bool none = !__any(any);
+    if (m == kNone) m = 0;         // NaN alone, or minus infinities
+    float sum = 0, acc[2] = {0, 0};
+#pragma unroll 1
+    for (int c = j0; c < end; c += 64) {
+      const int j = c + lane;
+      const float w = shown(j) ? __builtin_amdgcn_exp2f(score(j) - m) : 0.0f;
+      sum += w;
+      plain_add(acc, w, [&](int z) { return v + min(c + z, a.Tk - 1) * a.v.t; }, a.Dv);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
+    float* y = result_row(A, split, slab, b, head, r, i, m + __builtin_amdgcn_logf(sum), none, lane == 0);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) if (y && 64 * e + lane < a.Dv) y[64 * e + lane] = none ? 0.0f : acc[e] / sum;
+  }
+}
+
 template <int DP, bool RICH>       // RICH: capped scores or slopes
 __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
-  constexpr int KC = DP / 16, DB = DP / 32, NF = 2 * KC + 4 * DB;
-  __shared__ __align__(16) _Float16 lds[2][NF * kFrag];
-  __shared__ int range[4];
+  constexpr int KC = DP / 16, DB = DP / 32, F_V = 2 * KC, F_SIDE = F_V + 4 * DB, NF = F_SIDE + 1;
+  __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
+  __shared__ int range[5];
   const AttendDesc& a = A.a;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
   const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
@@ -172,10 +217,6 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   const bool valid = r < A.M;
   const int i = (int)fastdiv((uint32_t)min(r, A.M - 1), A.group), g = min(r, A.M - 1) - i * G, head = hk * G + g;
   const int p = s.first + i, doc = doc_at(s, p), below = sees_below(s, p);
-  const float* qrow = a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t;
-  half8 qh[KC], ql[KC];
-  const int qe = load_rows<KC>(qrow, valid, a.D, A.wide, qh, ql);
-  const float slope = RICH && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
 
   // the wavefront's rows, and the block's key tiles
   Span me;
@@ -199,46 +240,34 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   int t0 = 0, t1 = s.n;
   if (s.causal) t1 = min(t1, max(last + 1, s.prefix));
   if (s.positional && last < 0) t1 = 0;
-  t1 = (t1 + kTile - 1) / kTile;
-  if (s.doc) {
-    if (tid < 4) range[tid] = tid & 1 ? INT32_MIN : INT32_MAX;
-    __syncthreads();
-    if (lane == 0) {
-      atomicMin(&range[0], me.dmin);
-      atomicMax(&range[1], me.dmax);
-    }
-    __syncthreads();
-    const int lo = range[0], hi = range[1];
-    int first = INT32_MAX, end = INT32_MIN;
-    for (int t = tid; t < t1; t += 256)
-      if (ki[t].dmin <= hi && lo <= ki[t].dmax) {
-        first = min(first, t);
-        end = max(end, t + 1);
-      }
-    atomicMin(&range[2], first);
-    atomicMax(&range[3], end);
-    __syncthreads();
-    t0 = range[2];
-    t1 = range[3];
-    if (t0 >= t1) t0 = t1 = 0;
-  }
+  const Range range_ = tile_range(s, 0, (t1 + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax, range);
+  t0 = range_.t0;
+  t1 = range_.t1;
   if (A.splits > 1) {
     const int n = t1 - t0, each = (n + A.splits - 1) / A.splits;
     t0 = min(t0 + split * each, t1);
     t1 = min(t0 + each, t1);
   }
-  t0 = __builtin_amdgcn_readfirstlane(t0);
-  t1 = __builtin_amdgcn_readfirstlane(t1);
+  if (range_.odd) {
+    plain_rows(A, s, split, slab, b, hk, row0, t0 * kTile, t1 * kTile);
+    return;
+  }
 
-  const _Float16* kf = A.kf + (int64_t)slab * tiles * (2 * KC * kFrag);
-  const _Float16* vf = A.vf + (int64_t)slab * tiles * (4 * DB * kFrag);
+  const float* qrow = a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t;
+  half8 qh[KC], ql[KC];
+  const int qe = load_rows<KC>(qrow, valid, a.D, A.wide, qh, ql);
+  const float slope = RICH && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+  const int64_t tile0 = (int64_t)slab * tiles;
   const uint32_t base = lds_address(lds), lane16 = lane * 16;
   auto fetch = [&](int t, int buf) {
 #pragma unroll
-    for (int f = 0; f < NF / 4; ++f) {
+    for (int f = 0; f < (NF + 3) / 4; ++f) {
       const int q = f * 4 + w;
-      const _Float16* src = q < 2 * KC ? kf + ((int64_t)t * (2 * KC) + q) * kFrag : vf + ((int64_t)t * (4 * DB) + q - 2 * KC) * kFrag;
-      frag_to_lds(src, base + (buf * NF + q) * (kFrag * 2), lane16);
+      const _Float16* src;
+      if (q < F_V) src = A.kf + ((tile0 + t) * (2 * KC) + q) * kFrag;
+      else if (q < F_SIDE) src = A.vf + ((tile0 + t) * (4 * DB) + q - F_V) * kFrag;
+      else src = (const _Float16*)(A.side + (tile0 + t) * (kSide * kTile));
+      if (q < NF) frag_to_lds(src, base + (buf * NF + q) * (kFrag * 2), lane16);
     }
   };
 
@@ -247,50 +276,49 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
   float m = kNone, sum = 0;        // running maximum (log2) and this lane half's sum
   int ce = kUnset;                 // acc is in units of 2^-ce
-  if (t0 < t1) fetch(t0, 0);
+  TileInfo kn = {}, vn = {};
+  if (t0 < t1) {
+    fetch(t0, 0);
+    kn = ki[t0];
+    vn = vi[t0];
+  }
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, j0 = t * kTile;
     loads_done();
     __syncthreads();
-    if (t + 1 < t1) fetch(t + 1, buf ^ 1);
-    const TileInfo kt = ki[t], vt = vi[t];
-    if (!any_seen(s, me, kt, j0)) continue;
-    const _Float16* L = lds[buf];
-    // scores, transposed: register r of this lane is key j0 + 8 (r / 4) + 4 h + r % 4
-    f32x16 x = {};
-    float unit;
-    if (kt.irregular) {
-      const float* k = a.k.p + b * a.k.b + hk * a.k.h + (int64_t)j0 * a.k.t;
-      plain_scores(x, [&](int j) { return k + j * a.k.t; }, a.Tk - j0, qrow, valid, a.D);
-      unit = a.scale;
-    } else {
-      x = scores<KC>(L, 0, qh, ql);
-      unit = a.scale * pow2(-qe) * (1.0f / kt.scale);
+    const TileInfo kt = kn, vt = vn;
+    if (t + 1 < t1) {
+      fetch(t + 1, buf ^ 1);
+      kn = ki[t + 1];
+      vn = vi[t + 1];
     }
-    float f = 1;                   // exponent of 2 = f x (plain) or x (RICH)
+    if (!any_seen(s, me, kt, j0)) continue;
+    const _Float16* L = lds + buf * (NF * kFrag);
+    const float* side = (const float*)(L + F_SIDE * kFrag);
+    // scores, transposed: register r of this lane is key j0 + 8 (r / 4) + 4 h + r % 4
+    f32x16 x = scores<KC>(L, 0, qh, ql);
+    if (kt.uneven) per_row(x, side + KS_RELK * kTile);
+    const float unit = a.scale * pow2(-qe) * kt.inv;
+    float f = unit * kLog2e;       // the score is f x, in log2
     if (RICH) {
       if (a.cap > 0) {
-        const float u = unit / a.cap, c = a.cap * kLog2e;
-#pragma unroll
-        for (int q = 0; q < 16; ++q) x[q] = c * tanh_of(x[q] * u);
-      } else {
-        const float u = unit * kLog2e;
-#pragma unroll
-        for (int q = 0; q < 16; ++q) x[q] *= u;
+        tanh_all(x, unit / a.cap);
+        f = a.cap * kLog2e;
       }
-      if (a.slopes)
+      if (a.slopes) {
 #pragma unroll
-        for (int q = 0; q < 16; ++q) x[q] -= slope * fabsf((float)(p - (j0 + 8 * (q / 4) + 4 * h + q % 4)));
-    } else {
-      f = unit * kLog2e;
+        for (int q = 0; q < 16; ++q) x[q] = x[q] * f - slope * fabsf((float)(p - (j0 + 8 * (q / 4) + 4 * h + q % 4)));
+        f = 1;
+      }
     }
     if (!all_seen(s, me, kt, j0)) {
       if (s.doc) {
-        int dj[16];
 #pragma unroll
-        for (int q = 0; q < 16; ++q) dj[q] = s.doc[min(j0 + 8 * (q / 4) + 4 * h + q % 4, a.Tk - 1)];
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const f32x4 dj = *(const f32x4*)(side + KS_DOC * kTile + 8 * q4 + 4 * h);
 #pragma unroll
-        for (int q = 0; q < 16; ++q) x[q] = dj[q] == doc && doc >= 0 ? x[q] : kNone;
+          for (int e = 0; e < 4; ++e) x[4 * q4 + e] = __float_as_int(dj[e]) == doc && doc >= 0 ? x[4 * q4 + e] : kNone;
+        }
       }
 #pragma unroll
       for (int q = 0; q < 16; ++q) x[q] = j0 + 8 * (q / 4) + 4 * h + q % 4 < below ? x[q] : kNone;
@@ -301,11 +329,17 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
     top = halves_max(top) * f;
     // The maximum moves only when it grows by more than 2^8 (or from nothing), so that most tiles leave acc alone: weights
     // then reach 2^8 instead of 1.
-    float keep = 1;
+    float change = 1;
     if (top > m + 8 || (m == kNone && top > kNone)) {
-      keep = __builtin_amdgcn_exp2f(m - top);
+      const float keep = __builtin_amdgcn_exp2f(m - top);
       m = top;
       sum *= keep;
+      change = keep;
+      if (ce != kUnset) {          // what acc held has shrunk: so may its unit
+        const int shrunk = keep > 0 ? min(-exponent(keep) - 1, 100) : 0;
+        change *= pow2(shrunk);
+        ce += shrunk;
+      }
     }
     const float off = m == kNone ? 0.0f : m;
 #pragma unroll
@@ -314,55 +348,22 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
 #pragma unroll
     for (int q = 0; q < 16; ++q) part += x[q];
     sum += part;
-    float change = keep;
-    if (vt.irregular) {
-      const float* v = a.v.p + b * a.v.b + hk * a.v.h + (int64_t)j0 * a.v.t;
-      rescale<DB>(acc, change);
-      plain_accumulate<DB>(acc, ce, x, [&](int j) { return v + j * a.v.t; }, a.Tk - j0, a.Dv);
-      continue;
+    float big = __builtin_amdgcn_exp2f(top - off);
+    if (vt.uneven) {
+      per_row(x, side + KS_RELV * kTile);
+      big = largest(x);
     }
-    // what acc held has shrunk by `keep`: so may its unit
-    if (keep < 1 && ce != kUnset) {
-      const int shrunk = keep > 0 ? min(-exponent(keep) - 1, 100) : 0;
-      change *= pow2(shrunk);
-      ce += shrunk;
-    }
-    const int e = fit_unit(ce, __builtin_amdgcn_exp2f(top - off), exponent(vt.scale), &change);
+    const int e = fit_unit(ce, big, exponent(vt.scale), &change);
     rescale<DB>(acc, change);
-    accumulate<DB>(acc, x, pow2(e), L, 2 * KC);
+    accumulate<DB>(acc, x, pow2(e), L, F_V);
   }
 
   sum = halves_sum(sum);
   if (!valid) return;
   const bool none = sum == 0;      // not m: a visible NaN leaves no maximum
-  const float lse = none ? (A.splits > 1 ? kNone : INFINITY) : m + __builtin_amdgcn_logf(sum);
   const float out = none ? 0.0f : 1.0f / sum;
-  float* y;
-  if (A.splits > 1) {
-    const int64_t at = ((int64_t)split * a.B * a.Hk + slab) * A.M + r;
-    if (h == 0) A.plse[at] = lse;
-    y = A.part + at * a.Dv;
-  } else {
-    if (h == 0 && a.lse) a.lse[((int64_t)b * a.H + head) * a.Tq + i] = lse;
-    y = a.y.p + b * a.y.b + head * a.y.h + (int64_t)i * a.y.t;
-    if (!a.y.p) return;
-  }
-  const bool wide = A.splits > 1 ? a.Dv % 4 == 0 : A.wide;
-#pragma unroll
-  for (int d = 0; d < DB; ++d)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int at = 32 * d + 8 * q + 4 * h;
-      f32x4 v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : __builtin_amdgcn_ldexpf(acc[d][4 * q + e], -ce) * out;
-      if (wide) {
-        if (at < a.Dv) *(f32x4*)(y + at) = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) if (at + e < a.Dv) y[at + e] = v[e];
-      }
-    }
+  float* y = result_row(A, split, slab, b, head, r, i, m + __builtin_amdgcn_logf(sum), none, h == 0);
+  if (y) store_row<DB>(y, acc, ce, out, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide);
 }
 
 // ---- few rows --------------------------------------------------------------------------------------
@@ -531,7 +532,7 @@ __global__ __launch_bounds__(128) void attend_join(JoinArgs A) {
 struct Plan {
   int DP, M, G, tiles, blocks, splits, slabs;
   bool few;
-  int64_t kf, vf, ki, vi, part, plse, bytes;   // byte offsets into the workspace
+  int64_t kf, vf, ki, vi, side, part, plse, bytes;   // byte offsets into the workspace
 };
 constexpr int64_t kAlign = 256;
 inline int64_t take(int64_t& at, int64_t bytes) {
@@ -566,6 +567,7 @@ Plan plan(const AttendDesc& a) {
     p.vf = take(at, frag);
     p.ki = take(at, (int64_t)p.slabs * p.tiles * sizeof(TileInfo));
     p.vi = take(at, (int64_t)p.slabs * p.tiles * sizeof(TileInfo));
+    p.side = take(at, (int64_t)p.slabs * p.tiles * kSide * kTile * 4);
   }
   if (p.splits > 1) {
     p.part = take(at, (int64_t)p.splits * p.slabs * p.M * a.Dv * 4);
@@ -628,10 +630,11 @@ void attend(const AttendDesc& a, void* work, hipStream_t st) {
     k.Hk = a.Hk;
     k.wide = wide;
     k.a = a;
-    k.job[0] = {a.k, a.D, 1, a.Tk, p.tiles, (_Float16*)(w + p.kf), nullptr, (TileInfo*)(w + p.ki), false, {}, nullptr};
-    k.job[1] = {a.v, a.Dv, 1, a.Tk, p.tiles, nullptr, (_Float16*)(w + p.vf), (TileInfo*)(w + p.vi), false, {}, nullptr};
+    float* side = (float*)(w + p.side);
+    k.job[0] = {a.k, a.D, 1, a.Tk, p.tiles, (_Float16*)(w + p.kf), nullptr, (TileInfo*)(w + p.ki), false, side, KS_RELK, true, {}};
+    k.job[1] = {a.v, a.Dv, 1, a.Tk, p.tiles, nullptr, (_Float16*)(w + p.vf), (TileInfo*)(w + p.vi), false, side, KS_RELV, false, {}};
     attend_pack(k, p.DP, st);
-    const TilesArgs t{a, (_Float16*)(w + p.kf), (_Float16*)(w + p.vf), (TileInfo*)(w + p.ki), (TileInfo*)(w + p.vi),
+    const TilesArgs t{a, (_Float16*)(w + p.kf), (_Float16*)(w + p.vf), (TileInfo*)(w + p.ki), (TileInfo*)(w + p.vi), side,
                       make_fastdiv(p.G), p.M, p.blocks, p.splits, wide, part, plse};
     const int64_t grid = (int64_t)p.slabs * p.blocks * p.splits;
     if (p.DP == 32) run_tiles<32>(t, grid, st);

@@ -15,41 +15,70 @@ struct GradArgs {
   AttendGradDesc g;
   const _Float16 *qr, *qc, *gr, *gc, *kr, *kc, *vr;   // row / column fragments of q, dy, k, v
   const TileInfo *qi, *gi, *ki, *vi;
-  const float* rowinfo;
+  const float *qside, *kside;
   FastDiv group;
   int M, qtiles, ktiles, blocks, splits;
   bool wide;
   float *pk, *pv;                                     // parts of dk, dv: [split][slab][Tk][D or Dv]
 };
 
-// This lane's column of acc (features), in units of 2^-c, to a row in memory.
-template <int DB>
-__device__ __forceinline__ void store_row(float* row, const f32x16 (&acc)[DB], int c, float scale, int n, bool wide) {
-  const int h = (threadIdx.x >> 5) & 1;
-#pragma unroll
-  for (int d = 0; d < DB; ++d)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int at = 32 * d + 8 * q + 4 * h;
-      f32x4 v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_ldexpf(acc[d][4 * q + e], -c) * scale;
-      if (wide) {
-        if (at < n) *(f32x4*)(row + at) = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) if (at + e < n) row[at + e] = v[e];
-      }
-    }
+// ---- dk, dv --------------------------------------------------------------------------------------
+
+// Where dk and dv of key j go.
+__device__ __forceinline__ float* dk_row(const GradArgs& A, int split, int slab, int b, int hk, int j) {
+  if (!A.g.dk.p) return nullptr;
+  if (A.splits > 1) return A.pk + (((int64_t)split * A.g.a.B * A.g.a.Hk + slab) * A.g.a.Tk + j) * A.g.a.D;
+  return A.g.dk.p + b * A.g.dk.b + hk * A.g.dk.h + (int64_t)j * A.g.dk.t;
+}
+__device__ __forceinline__ float* dv_row(const GradArgs& A, int split, int slab, int b, int hk, int j) {
+  if (!A.g.dv.p) return nullptr;
+  if (A.splits > 1) return A.pv + (((int64_t)split * A.g.a.B * A.g.a.Hk + slab) * A.g.a.Tk + j) * A.g.a.Dv;
+  return A.g.dv.p + b * A.g.dv.b + hk * A.g.dv.h + (int64_t)j * A.g.dv.t;
 }
 
-// ---- dk, dv --------------------------------------------------------------------------------------
+// A wavefront's keys [j0, j0 + 32) over query rows [r0, r1) in plain f32.
+__device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, int split, int slab, int b, int hk, int j0, int r0, int r1) {
+  const AttendDesc& a = A.g.a;
+  const int lane = threadIdx.x & 63, G = (int)A.group.d;
+  r1 = min(r1, A.M);
+  auto row = [&](const Rows& x, int r) { return x.p + b * x.b + (hk * G + r % G) * x.h + (int64_t)(r / G) * x.t; };
+#pragma unroll 1
+  for (int j = j0; j < min(j0 + kTile, a.Tk); ++j) {
+    const float* k = a.k.p + b * a.k.b + hk * a.k.h + (int64_t)j * a.k.t;
+    const float* v = a.v.p + b * a.v.b + hk * a.v.h + (int64_t)j * a.v.t;
+    const int doc = s.doc ? s.doc[j] : 0;
+    float dk[2] = {0, 0}, dv[2] = {0, 0};
+#pragma unroll 1
+    for (int c = r0; c < r1; c += 64) {
+      const int r = c + lane;
+      float p = 0, ds = 0;
+      if (r < r1) {
+        const float* side = A.qside + ((int64_t)slab * A.qtiles + r / kTile) * (kSide * kTile) + r % kTile;
+        if (j < __float_as_int(side[QS_BELOW * kTile]) && (!s.doc || (doc >= 0 && __float_as_int(side[QS_DOC * kTile]) == doc))) {
+          const PlainPair z = plain_score(a, plain_dot(row(a.q, r), k, a.D), side[QS_SLOPE * kTile], __float_as_int(side[QS_POS * kTile]) - j);
+          p = __builtin_amdgcn_exp2f(z.score - side[QS_LSE * kTile]);
+          ds = p * (plain_dot(row(A.g.dy, r), v, a.Dv) - side[QS_DOT * kTile]) * z.slack;
+        }
+      }
+      plain_add(dv, p, [&](int z) { return row(A.g.dy, min(c + z, A.M - 1)); }, a.Dv);
+      plain_add(dk, ds, [&](int z) { return row(a.q, min(c + z, A.M - 1)); }, a.D);
+    }
+    float* ok = dk_row(A, split, slab, b, hk, j);
+    float* ov = dv_row(A, split, slab, b, hk, j);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (ok && 64 * e + lane < a.D) ok[64 * e + lane] = dk[e] * a.scale;
+      if (ov && 64 * e + lane < a.Dv) ov[64 * e + lane] = dv[e];
+    }
+  }
+}
 
 template <int DP, bool RICH>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs A) {
   constexpr int KC = DP / 16, DB = DP / 32;
-  constexpr int F_GR = 2 * KC, F_QC = 4 * KC, F_GC = F_QC + 4 * DB, F_INFO = F_GC + 4 * DB, NF = F_INFO + 1;
+  constexpr int F_GR = 2 * KC, F_QC = 4 * KC, F_GC = F_QC + 4 * DB, F_SIDE = F_GC + 4 * DB, NF = F_SIDE + 1;
   __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
+  __shared__ int range[5];
   const AttendDesc& a = A.g.a;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
   const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
@@ -57,58 +86,38 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
   const int slab = id / per, split = id % per % A.splits, blk = id % per / A.splits;   // the first keys are seen by most
   const int b = slab / a.Hk, hk = slab % a.Hk;
   const Sight s = sight(a, b);
-  const int j0 = blk * 128 + w * kTile, j = j0 + l, kt = min(j0 / kTile, A.ktiles - 1);
+  const int j0 = blk * 128 + w * kTile, j = j0 + l;
   const bool valid = j < a.Tk;
-  const float* krow = a.k.p + b * a.k.b + hk * a.k.h + (int64_t)min(j, a.Tk - 1) * a.k.t;
-  const float* vrow = a.v.p + b * a.v.b + hk * a.v.h + (int64_t)min(j, a.Tk - 1) * a.v.t;
-  half8 kh[KC], kl[KC], vh[KC], vl[KC];
-  int vnorm;
-  const int ke = load_rows<KC>(krow, valid, a.D, A.wide, kh, kl);
-  const int ve = load_rows<KC>(vrow, valid, a.Dv, A.wide, vh, vl, &vnorm);
   const int doc = s.doc && valid ? s.doc[j] : -1;
-  const TileInfo mine = A.ki[(int64_t)slab * A.ktiles + kt];
+  TileInfo mine = A.ki[(int64_t)slab * A.ktiles + min(j0 / kTile, A.ktiles - 1)];
+  if (j0 >= a.Tk) {
+    mine.dmin = INT32_MAX;
+    mine.dmax = INT32_MIN;
+  }
 
   // the query tiles that see any of the block's keys: from its first key's position on, unless a prefix shows it to all
   const TileInfo* qi = A.qi + (int64_t)slab * A.qtiles;
   const TileInfo* gi = A.gi + (int64_t)slab * A.qtiles;
   const int k0 = blk * 128;
-  int t0 = 0, t1 = A.qtiles;
-  if (k0 >= s.n) t1 = 0;
   int64_t i0 = 0;                  // first position index that sees anything here
   if (s.causal && k0 >= s.prefix) i0 = (int64_t)k0 - s.first;
   if (s.positional) i0 = max(i0, (int64_t)-s.first);
-  t0 = (int)min(max(i0, (int64_t)0) * A.group.d / kTile, (int64_t)t1);
-  if (s.doc) {
-    __shared__ int range[4];
-    if (tid < 4) range[tid] = tid & 1 ? INT32_MIN : INT32_MAX;
-    __syncthreads();
-    if (lane == 0 && j0 < a.Tk) {
-      atomicMin(&range[0], mine.dmin);
-      atomicMax(&range[1], mine.dmax);
-    }
-    __syncthreads();
-    const int lo = range[0], hi = range[1];
-    int first = INT32_MAX, end = INT32_MIN;
-    for (int t = t0 + tid; t < t1; t += 256)
-      if (gi[t].dmin <= hi && lo <= gi[t].dmax) {
-        first = min(first, t);
-        end = max(end, t + 1);
-      }
-    atomicMin(&range[2], first);
-    atomicMax(&range[3], end);
-    __syncthreads();
-    t0 = range[2];
-    t1 = range[3];
-    if (t0 >= t1) t0 = t1 = 0;
-  }
+  const int from = (int)min(max(i0, (int64_t)0) * A.group.d / kTile, (int64_t)A.qtiles);
+  const Range range_ = tile_range(s, from, k0 < s.n ? A.qtiles : 0, gi, qi, gi, mine.dmin, mine.dmax, range);
+  int t0 = range_.t0, t1 = range_.t1;
   if (A.splits > 1) {
-    const int n = max(t1 - t0, 0), each = (n + A.splits - 1) / A.splits;
+    const int n = t1 - t0, each = (n + A.splits - 1) / A.splits;
     t0 = min(t0 + split * each, t1);
     t1 = min(t0 + each, t1);
   }
-  t0 = __builtin_amdgcn_readfirstlane(t0);
-  t1 = __builtin_amdgcn_readfirstlane(t1);
+  if (range_.odd) {
+    plain_keys(A, s, split, slab, b, hk, j0, t0 * kTile, t1 * kTile);
+    return;
+  }
 
+  half8 kh[KC], kl[KC], vh[KC], vl[KC];
+  const int ke = load_rows<KC>(a.k.p + b * a.k.b + hk * a.k.h + (int64_t)min(j, a.Tk - 1) * a.k.t, valid, a.D, A.wide, kh, kl);
+  const int ve = load_rows<KC>(a.v.p + b * a.v.b + hk * a.v.h + (int64_t)min(j, a.Tk - 1) * a.v.t, valid, a.Dv, A.wide, vh, vl);
   const int64_t tile0 = (int64_t)slab * A.qtiles;
   const uint32_t base = lds_address(lds), lane16 = lane * 16;
   auto fetch = [&](int t, int buf) {
@@ -119,8 +128,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
       if (q < F_GR) src = A.qr + ((tile0 + t) * (2 * KC) + q) * kFrag;
       else if (q < F_QC) src = A.gr + ((tile0 + t) * (2 * KC) + q - F_GR) * kFrag;
       else if (q < F_GC) src = A.qc + ((tile0 + t) * (4 * DB) + q - F_QC) * kFrag;
-      else if (q < F_INFO) src = A.gc + ((tile0 + t) * (4 * DB) + q - F_GC) * kFrag;
-      else src = (const _Float16*)(A.rowinfo + (tile0 + t) * (kRowInfo * kTile));
+      else if (q < F_SIDE) src = A.gc + ((tile0 + t) * (4 * DB) + q - F_GC) * kFrag;
+      else src = (const _Float16*)(A.qside + (tile0 + t) * (kSide * kTile));
       if (q < NF) frag_to_lds(src, base + (buf * NF + q) * (kFrag * 2), lane16);
     }
   };
@@ -129,14 +138,22 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
 #pragma unroll
   for (int d = 0; d < DB; ++d) dk[d] = dv[d] = f32x16{};
   int ck = kUnset, cv = kUnset;
-  const RowMap qmap = row_map(a.q, b, hk * (int)A.group.d, A.group), gmap = row_map(A.g.dy, b, hk * (int)A.group.d, A.group);
-  if (t0 < t1) fetch(t0, 0);
+  TileInfo qn = {}, gn = {};
+  if (t0 < t1) {
+    fetch(t0, 0);
+    qn = qi[t0];
+    gn = gi[t0];
+  }
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, r0 = t * kTile;
     loads_done();
     __syncthreads();
-    if (t + 1 < t1) fetch(t + 1, buf ^ 1);
-    const TileInfo qt = qi[t], gt = gi[t];
+    const TileInfo qt = qn, gt = gn;
+    if (t + 1 < t1) {
+      fetch(t + 1, buf ^ 1);
+      qn = qi[t + 1];
+      gn = gi[t + 1];
+    }
     Span rows;
     rows.pmin = s.first + (int)fastdiv((uint32_t)r0, A.group);
     rows.pmax = s.first + (int)fastdiv((uint32_t)min(r0 + kTile - 1, A.M - 1), A.group);
@@ -144,67 +161,42 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
     rows.dmax = gt.dmax;
     rows.same = gt.same;
     if (j0 >= a.Tk || !any_seen(s, rows, mine, j0)) continue;
-    const _Float16* L = lds + buf * NF * kFrag;
-    const float* info = (const float*)(L + F_INFO * kFrag);
-    const bool odd = qt.irregular || gt.irregular;
-    const int left = A.M - r0;
+    const _Float16* L = lds + buf * (NF * kFrag);
+    const float* side = (const float*)(L + F_SIDE * kFrag);
     // register r: row r0 + 8 (r / 4) + 4 h + r % 4
-    f32x16 x, y;
-    float unit, yunit;
-    if (odd) {
-      plain_scores(x, [&](int i) { return qmap.row(r0 + i); }, left, krow, valid, a.D);
-      plain_scores(y, [&](int i) { return gmap.row(r0 + i); }, left, vrow, valid, a.Dv);
-      unit = a.scale;
-      yunit = 1;
-    } else {
-      x = scores<KC>(L, 0, kh, kl);
-      y = scores<KC>(L, F_GR, vh, vl);
-      unit = a.scale * pow2(-ke) * (1.0f / qt.scale);
-      yunit = pow2(-ve) * (1.0f / gt.scale);
-    }
-    f32x16 slack;                  // 1 - tanh^2
-    if (RICH) {
-      if (a.cap > 0) {
-        const float u = unit / a.cap, c = a.cap * kLog2e;
+    f32x16 x = scores<KC>(L, 0, kh, kl), y = scores<KC>(L, F_GR, vh, vl), slack;
+    if (qt.uneven) per_row(x, side + QS_RELQ * kTile);
+    if (gt.uneven) per_row(y, side + QS_RELG * kTile);
+    const float unit = a.scale * pow2(-ke) * qt.inv, yunit = pow2(-ve) * gt.inv;
+    float f = unit * kLog2e;
+    if (RICH && a.cap > 0) {
+      tanh_all(x, unit / a.cap);
+      f = a.cap * kLog2e;
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const float th = tanh_of(x[q] * u);
-          slack[q] = fmaf(-th, th, 1.0f);
-          x[q] = c * th;
-        }
-      } else {
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          x[q] *= unit * kLog2e;
-          slack[q] = 1;
-        }
-      }
+      for (int q = 0; q < 16; ++q) slack[q] = fmaf(-x[q], x[q], 1.0f);   // 1 - tanh^2
     }
-    const float f = RICH ? 1.0f : unit * kLog2e;
-    const bool all = left >= kTile && all_seen(s, rows, mine, j0);
+    const bool all = A.M - r0 >= kTile && all_seen(s, rows, mine, j0);
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) {
       const int at = 8 * q4 + 4 * h;
-      const f32x4 lse = *(const f32x4*)(info + RI_LSE * kTile + at), dot = *(const f32x4*)(info + RI_DOT * kTile + at);
-      f32x4 pos, slope, below, rdoc;
+      const f32x4 lse = *(const f32x4*)(side + QS_LSE * kTile + at), dot = *(const f32x4*)(side + QS_DOT * kTile + at);
+      f32x4 off = lse;
       if (RICH && a.slopes) {
-        pos = *(const f32x4*)(info + RI_POS * kTile + at);
-        slope = *(const f32x4*)(info + RI_SLOPE * kTile + at);
+        const f32x4 pos = *(const f32x4*)(side + QS_POS * kTile + at), slope = *(const f32x4*)(side + QS_SLOPE * kTile + at);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * q4 + e] -= slope[e] * fabsf((float)(__float_as_int(pos[e]) - j));
+        for (int e = 0; e < 4; ++e) off[e] = fmaf(slope[e], fabsf((float)(__float_as_int(pos[e]) - j)), lse[e]);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int q = 4 * q4 + e;
-        const float p = __builtin_amdgcn_exp2f(fmaf(x[q], f, -lse[e]));
+        const float p = __builtin_amdgcn_exp2f(fmaf(x[q], f, -off[e]));
         float ds = p * fmaf(y[q], yunit, -dot[e]);
-        if (RICH) ds *= slack[q];
+        if (RICH && a.cap > 0) ds *= slack[q];
         x[q] = p;
         y[q] = ds;
       }
       if (!all) {
-        below = *(const f32x4*)(info + RI_BELOW * kTile + at);
-        rdoc = *(const f32x4*)(info + RI_DOC * kTile + at);
+        const f32x4 below = *(const f32x4*)(side + QS_BELOW * kTile + at), rdoc = *(const f32x4*)(side + QS_DOC * kTile + at);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const bool ok = j < __float_as_int(below[e]) && (!s.doc || (doc >= 0 && __float_as_int(rdoc[e]) == doc));
@@ -213,15 +205,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
         }
       }
     }
-    if (odd) {
-      plain_accumulate<DB>(dv, cv, x, [&](int i) { return gmap.row(r0 + i); }, left, a.Dv);
-      plain_accumulate<DB>(dk, ck, y, [&](int i) { return qmap.row(r0 + i); }, left, a.D);
-      continue;
-    }
+    if (gt.uneven) per_row(x, side + QS_RELG * kTile);
     float change = 1;
     int e = fit_unit(cv, largest(x), exponent(gt.scale), &change);
     rescale<DB>(dv, change);
     accumulate<DB>(dv, x, pow2(e), L, F_GC);
+    if (qt.uneven) per_row(y, side + QS_RELQ * kTile);
     change = 1;
     e = fit_unit(ck, largest(y), exponent(qt.scale), &change);
     rescale<DB>(dk, change);
@@ -229,16 +218,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
   }
 
   if (!valid) return;
-  const bool parts = A.splits > 1;
-  const int64_t at = ((int64_t)split * a.B * a.Hk + slab) * a.Tk + j;
-  if (A.g.dk.p) {
-    float* o = parts ? A.pk + at * a.D : A.g.dk.p + b * A.g.dk.b + hk * A.g.dk.h + (int64_t)j * A.g.dk.t;
-    store_row<DB>(o, dk, ck, a.scale, a.D, parts ? a.D % 4 == 0 : A.wide);
-  }
-  if (A.g.dv.p) {
-    float* o = parts ? A.pv + at * a.Dv : A.g.dv.p + b * A.g.dv.b + hk * A.g.dv.h + (int64_t)j * A.g.dv.t;
-    store_row<DB>(o, dv, cv, 1.0f, a.Dv, parts ? a.Dv % 4 == 0 : A.wide);
-  }
+  float* ok = dk_row(A, split, slab, b, hk, j);
+  float* ov = dv_row(A, split, slab, b, hk, j);
+  if (ok) store_row<DB>(ok, dk, ck, a.scale, a.D, A.splits > 1 ? a.D % 4 == 0 : A.wide);
+  if (ov) store_row<DB>(ov, dv, cv, 1.0f, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide);
 }
 
 // The parts of dk and dv in order.
@@ -260,11 +243,43 @@ __global__ __launch_bounds__(256) void attend_grad_join(GradArgs A) {
 
 // ---- dq --------------------------------------------------------------------------------------------
 
+// A wavefront's rows [row0, row0 + 32) over keys [j0, j1) in plain f32.
+__device__ __forceinline__ void plain_dq(const GradArgs& A, const Sight& s, int slab, int b, int hk, int row0, int j0, int j1) {
+  const AttendDesc& a = A.g.a;
+  const int lane = threadIdx.x & 63, G = (int)A.group.d;
+  const float* k = a.k.p + b * a.k.b + hk * a.k.h;
+  const float* v = a.v.p + b * a.v.b + hk * a.v.h;
+#pragma unroll 1
+  for (int r = row0; r < min(row0 + kTile, A.M); ++r) {
+    const int i = r / G, head = hk * G + r % G;
+    const float* q = a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t;
+    const float* dy = A.g.dy.p + b * A.g.dy.b + head * A.g.dy.h + (int64_t)i * A.g.dy.t;
+    const float* side = A.qside + ((int64_t)slab * A.qtiles + r / kTile) * (kSide * kTile) + r % kTile;
+    const int p = __float_as_int(side[QS_POS * kTile]), doc = __float_as_int(side[QS_DOC * kTile]);
+    const int end = min(j1, __float_as_int(side[QS_BELOW * kTile]));
+    float dq[2] = {0, 0};
+#pragma unroll 1
+    for (int c = j0; c < end; c += 64) {
+      const int j = c + lane;
+      float ds = 0;
+      if (j < end && (!s.doc || (doc >= 0 && s.doc[j] == doc))) {
+        const PlainPair z = plain_score(a, plain_dot(k + j * a.k.t, q, a.D), side[QS_SLOPE * kTile], p - j);
+        ds = __builtin_amdgcn_exp2f(z.score - side[QS_LSE * kTile]) * (plain_dot(v + j * a.v.t, dy, a.Dv) - side[QS_DOT * kTile]) * z.slack;
+      }
+      plain_add(dq, ds, [&](int z) { return k + min(c + z, a.Tk - 1) * a.k.t; }, a.D);
+    }
+    float* o = A.g.dq.p + b * A.g.dq.b + head * A.g.dq.h + (int64_t)i * A.g.dq.t;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) if (64 * e + lane < a.D) o[64 * e + lane] = dq[e] * a.scale;
+  }
+}
+
 template <int DP, bool RICH>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs A) {
   constexpr int KC = DP / 16, DB = DP / 32;
-  constexpr int F_V = 2 * KC, F_KC = 4 * KC, NF = F_KC + 4 * DB;
+  constexpr int F_V = 2 * KC, F_KC = 4 * KC, F_SIDE = F_KC + 4 * DB, NF = F_SIDE + 1;
   __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
+  __shared__ int range[5];
   const AttendDesc& a = A.g.a;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
   const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
@@ -276,67 +291,46 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
   const bool valid = r < A.M;
   const int i = (int)fastdiv((uint32_t)rr, A.group), g = rr - i * G, head = hk * G + g;
   const int p = s.first + i, doc = doc_at(s, p), below = sees_below(s, p);
-  const float* qrow = a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t;
-  const float* grow = A.g.dy.p + b * A.g.dy.b + head * A.g.dy.h + (int64_t)i * A.g.dy.t;
-  half8 qh[KC], ql[KC], gh[KC], gl[KC];
-  const int qe = load_rows<KC>(qrow, valid, a.D, A.wide, qh, ql);
-  const int ge = load_rows<KC>(grow, valid, a.Dv, A.wide, gh, gl);
-  const float slope = RICH && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
   const int qt = min(row0 / kTile, A.qtiles - 1);
-  const float* info = A.rowinfo + ((int64_t)slab * A.qtiles + qt) * (kRowInfo * kTile) + l;
-  const float lse = info[RI_LSE * kTile], dot = info[RI_DOT * kTile];
-  const TileInfo mine = A.gi[(int64_t)slab * A.qtiles + qt];
+  const float* mine = A.qside + ((int64_t)slab * A.qtiles + qt) * (kSide * kTile) + l;
+  const float lse = mine[QS_LSE * kTile], dot = mine[QS_DOT * kTile];
+  const TileInfo gt = A.gi[(int64_t)slab * A.qtiles + qt];
   Span me;
   me.pmin = s.first + (int)fastdiv((uint32_t)min(row0, A.M - 1), A.group);
   me.pmax = s.first + (int)fastdiv((uint32_t)min(row0 + kTile - 1, A.M - 1), A.group);
-  me.dmin = mine.dmin;
-  me.dmax = mine.dmax;
-  me.same = mine.same;
+  me.dmin = row0 < A.M ? gt.dmin : INT32_MAX;
+  me.dmax = row0 < A.M ? gt.dmax : INT32_MIN;
+  me.same = gt.same;
 
   const TileInfo* ki = A.ki + (int64_t)slab * A.ktiles;
   const TileInfo* vi = A.vi + (int64_t)slab * A.ktiles;
   const int last = s.first + (int)fastdiv((uint32_t)min(blk * 128 + 127, A.M - 1), A.group);
-  int t0 = 0, t1 = s.n;
-  if (s.causal) t1 = min(t1, max(last + 1, s.prefix));
-  if (s.positional && last < 0) t1 = 0;
-  t1 = (t1 + kTile - 1) / kTile;
-  if (s.doc) {
-    __shared__ int range[4];
-    if (tid < 4) range[tid] = tid & 1 ? INT32_MIN : INT32_MAX;
-    __syncthreads();
-    if (lane == 0 && row0 < A.M) {
-      atomicMin(&range[0], me.dmin);
-      atomicMax(&range[1], me.dmax);
-    }
-    __syncthreads();
-    const int lo = range[0], hi = range[1];
-    int first = INT32_MAX, end = INT32_MIN;
-    for (int t = tid; t < t1; t += 256)
-      if (ki[t].dmin <= hi && lo <= ki[t].dmax) {
-        first = min(first, t);
-        end = max(end, t + 1);
-      }
-    atomicMin(&range[2], first);
-    atomicMax(&range[3], end);
-    __syncthreads();
-    t0 = range[2];
-    t1 = range[3];
-    if (t0 >= t1) t0 = t1 = 0;
+  int end = s.n;
+  if (s.causal) end = min(end, max(last + 1, s.prefix));
+  if (s.positional && last < 0) end = 0;
+  const Range range_ = tile_range(s, 0, (end + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax, range);
+  const int t0 = range_.t0, t1 = range_.t1;
+  if (range_.odd) {
+    plain_dq(A, s, slab, b, hk, row0, t0 * kTile, t1 * kTile);
+    return;
   }
-  t0 = __builtin_amdgcn_readfirstlane(t0);
-  t1 = __builtin_amdgcn_readfirstlane(t1);
 
+  half8 qh[KC], ql[KC], gh[KC], gl[KC];
+  const int qe = load_rows<KC>(a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t, valid, a.D, A.wide, qh, ql);
+  const int ge = load_rows<KC>(A.g.dy.p + b * A.g.dy.b + head * A.g.dy.h + (int64_t)i * A.g.dy.t, valid, a.Dv, A.wide, gh, gl);
+  const float slope = RICH && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
   const int64_t tile0 = (int64_t)slab * A.ktiles;
   const uint32_t base = lds_address(lds), lane16 = lane * 16;
   auto fetch = [&](int t, int buf) {
 #pragma unroll
-    for (int f = 0; f < NF / 4; ++f) {
+    for (int f = 0; f < (NF + 3) / 4; ++f) {
       const int q = f * 4 + w;
       const _Float16* src;
       if (q < F_V) src = A.kr + ((tile0 + t) * (2 * KC) + q) * kFrag;
       else if (q < F_KC) src = A.vr + ((tile0 + t) * (2 * KC) + q - F_V) * kFrag;
-      else src = A.kc + ((tile0 + t) * (4 * DB) + q - F_KC) * kFrag;
-      frag_to_lds(src, base + (buf * NF + q) * (kFrag * 2), lane16);
+      else if (q < F_SIDE) src = A.kc + ((tile0 + t) * (4 * DB) + q - F_KC) * kFrag;
+      else src = (const _Float16*)(A.kside + (tile0 + t) * (kSide * kTile));
+      if (q < NF) frag_to_lds(src, base + (buf * NF + q) * (kFrag * 2), lane16);
     }
   };
 
@@ -344,62 +338,52 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
 #pragma unroll
   for (int d = 0; d < DB; ++d) dq[d] = f32x16{};
   int cq = kUnset;
-  if (t0 < t1) fetch(t0, 0);
+  TileInfo kn = {}, vn = {};
+  if (t0 < t1) {
+    fetch(t0, 0);
+    kn = ki[t0];
+    vn = vi[t0];
+  }
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, j0 = t * kTile;
     loads_done();
     __syncthreads();
-    if (t + 1 < t1) fetch(t + 1, buf ^ 1);
-    const TileInfo kt = ki[t], vt = vi[t];
-    if (!any_seen(s, me, kt, j0)) continue;
-    const _Float16* L = lds + buf * NF * kFrag;
-    const bool odd = kt.irregular || vt.irregular;
-    const float* k = a.k.p + b * a.k.b + hk * a.k.h + (int64_t)j0 * a.k.t;
-    const float* v = a.v.p + b * a.v.b + hk * a.v.h + (int64_t)j0 * a.v.t;
-    f32x16 x, y;
-    float unit, yunit;
-    if (odd) {
-      plain_scores(x, [&](int j) { return k + j * a.k.t; }, a.Tk - j0, qrow, valid, a.D);
-      plain_scores(y, [&](int j) { return v + j * a.v.t; }, a.Tk - j0, grow, valid, a.Dv);
-      unit = a.scale;
-      yunit = 1;
-    } else {
-      x = scores<KC>(L, 0, qh, ql);
-      y = scores<KC>(L, F_V, gh, gl);
-      unit = a.scale * pow2(-qe) * (1.0f / kt.scale);
-      yunit = pow2(-ge) * (1.0f / vt.scale);
+    const TileInfo kt = kn, vt = vn;
+    if (t + 1 < t1) {
+      fetch(t + 1, buf ^ 1);
+      kn = ki[t + 1];
+      vn = vi[t + 1];
     }
-    const bool all = all_seen(s, me, kt, j0);
-    const float u = RICH && a.cap > 0 ? unit / a.cap : unit * kLog2e, c = a.cap * kLog2e;
+    if (!any_seen(s, me, kt, j0)) continue;
+    const _Float16* L = lds + buf * (NF * kFrag);
+    const float* side = (const float*)(L + F_SIDE * kFrag);
+    f32x16 x = scores<KC>(L, 0, qh, ql), y = scores<KC>(L, F_V, gh, gl);
+    if (kt.uneven) per_row(x, side + KS_RELK * kTile);
+    if (vt.uneven) per_row(y, side + KS_RELV * kTile);
+    const float unit = a.scale * pow2(-qe) * kt.inv, yunit = pow2(-ge) * vt.inv;
+    const bool cap = RICH && a.cap > 0;
+    if (cap) tanh_all(x, unit / a.cap);
+    const float f = (cap ? a.cap : unit) * kLog2e;
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
-      const int j = j0 + 8 * (q / 4) + 4 * h + q % 4;
-      float z = x[q] * u, slack = 1;
-      if (RICH && a.cap > 0) {
-        z = tanh_of(z);
-        slack = fmaf(-z, z, 1.0f);
-        z *= c;
-      }
-      if (RICH && a.slopes) z -= slope * fabsf((float)(p - j));
-      const float w = __builtin_amdgcn_exp2f(RICH ? z - lse : fmaf(x[q], u, -lse));
-      y[q] = w * fmaf(y[q], yunit, -dot);
-      if (RICH) y[q] *= slack;
+      float off = lse;
+      if (RICH && a.slopes) off = fmaf(slope, fabsf((float)(p - (j0 + 8 * (q / 4) + 4 * h + q % 4))), lse);
+      y[q] = __builtin_amdgcn_exp2f(fmaf(x[q], f, -off)) * fmaf(y[q], yunit, -dot);
+      if (cap) y[q] *= fmaf(-x[q], x[q], 1.0f);
     }
-    if (!all) {
+    if (!all_seen(s, me, kt, j0)) {
       if (s.doc) {
-        int dj[16];
 #pragma unroll
-        for (int q = 0; q < 16; ++q) dj[q] = s.doc[min(j0 + 8 * (q / 4) + 4 * h + q % 4, a.Tk - 1)];
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const f32x4 dj = *(const f32x4*)(side + KS_DOC * kTile + 8 * q4 + 4 * h);
 #pragma unroll
-        for (int q = 0; q < 16; ++q) y[q] = dj[q] == doc && doc >= 0 ? y[q] : 0.0f;
+          for (int e = 0; e < 4; ++e) y[4 * q4 + e] = __float_as_int(dj[e]) == doc && doc >= 0 ? y[4 * q4 + e] : 0.0f;
+        }
       }
 #pragma unroll
       for (int q = 0; q < 16; ++q) y[q] = j0 + 8 * (q / 4) + 4 * h + q % 4 < below ? y[q] : 0.0f;
     }
-    if (odd) {
-      plain_accumulate<DB>(dq, cq, y, [&](int j) { return k + j * a.k.t; }, a.Tk - j0, a.D);
-      continue;
-    }
+    if (kt.uneven) per_row(y, side + KS_RELK * kTile);
     float change = 1;
     const int e = fit_unit(cq, largest(y), exponent(kt.scale), &change);
     rescale<DB>(dq, change);
@@ -413,7 +397,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
 
 struct GradPlan {
   int DP, M, G, qtiles, ktiles, blocks, splits, slabs;
-  int64_t qr, qc, gr, gc, kr, kc, vr, qi, gi, ki, vi, rowinfo, pk, pv, bytes;
+  int64_t qr, qc, gr, gc, kr, kc, vr, qi, gi, ki, vi, qside, kside, pk, pv, bytes;
 };
 GradPlan grad_plan(const AttendGradDesc& g) {
   const AttendDesc& a = g.a;
@@ -445,7 +429,8 @@ GradPlan grad_plan(const AttendGradDesc& g) {
   p.gi = take(q * sizeof(TileInfo));
   p.ki = take(k * sizeof(TileInfo));
   p.vi = take(k * sizeof(TileInfo));
-  p.rowinfo = take(q * kRowInfo * kTile * 4);
+  p.qside = take(q * kSide * kTile * 4);
+  p.kside = take(k * kSide * kTile * 4);
   if (p.splits > 1) {
     p.pk = take((int64_t)p.splits * p.slabs * a.Tk * a.D * 4);
     p.pv = take((int64_t)p.splits * p.slabs * a.Tk * a.Dv * 4);
@@ -485,13 +470,14 @@ void attend_grad(const AttendGradDesc& g, void* work, hipStream_t st) {
   k.Hk = a.Hk;
   k.wide = wide;
   k.a = a;
-  k.job[0] = {a.q, a.D, p.G, p.M, p.qtiles, half(p.qr), half(p.qc), info(p.qi), true, {}, nullptr};
-  k.job[1] = {g.dy, a.Dv, p.G, p.M, p.qtiles, half(p.gr), half(p.gc), info(p.gi), true, a.y, (float*)(w + p.rowinfo)};
-  k.job[2] = {a.k, a.D, 1, a.Tk, p.ktiles, half(p.kr), half(p.kc), info(p.ki), false, {}, nullptr};
-  k.job[3] = {a.v, a.Dv, 1, a.Tk, p.ktiles, half(p.vr), nullptr, info(p.vi), false, {}, nullptr};
+  float *qs = (float*)(w + p.qside), *ks = (float*)(w + p.kside);
+  k.job[0] = {a.q, a.D, p.G, p.M, p.qtiles, half(p.qr), half(p.qc), info(p.qi), true, qs, QS_RELQ, false, {}};
+  k.job[1] = {g.dy, a.Dv, p.G, p.M, p.qtiles, half(p.gr), half(p.gc), info(p.gi), true, qs, QS_RELG, true, a.y};
+  k.job[2] = {a.k, a.D, 1, a.Tk, p.ktiles, half(p.kr), half(p.kc), info(p.ki), false, ks, KS_RELK, true, {}};
+  k.job[3] = {a.v, a.Dv, 1, a.Tk, p.ktiles, half(p.vr), nullptr, info(p.vi), false, ks, KS_RELV, false, {}};
   attend_pack(k, p.DP, st);
   const GradArgs A{g, half(p.qr), half(p.qc), half(p.gr), half(p.gc), half(p.kr), half(p.kc), half(p.vr),
-                   info(p.qi), info(p.gi), info(p.ki), info(p.vi), (const float*)(w + p.rowinfo), make_fastdiv(p.G), p.M, p.qtiles,
+                   info(p.qi), info(p.gi), info(p.ki), info(p.vi), qs, ks, make_fastdiv(p.G), p.M, p.qtiles,
                    p.ktiles, p.blocks, p.splits, wide, (float*)(w + p.pk), (float*)(w + p.pv)};
   if (p.DP == 32) run_grad<32>(A, p.slabs, st);
   else if (p.DP == 64) run_grad<64>(A, p.slabs, st);
