@@ -148,10 +148,15 @@ __device__ __forceinline__ bool all_seen(const Sight& s, const Span& q, const Ti
   return !s.doc || (k.same && q.same && k.dmin == q.dmin);
 }
 
-// 1 KiB fragments from memory straight into LDS: lane l's 16 bytes land at base + 16 l. In inline assembly, so that the
-// compiler does not drain every load before the next LDS read; the kernels wait (vmcnt) and meet (barrier) themselves.
-__device__ __forceinline__ void frag_to_lds(const _Float16* src, uint32_t lds, uint32_t lane16) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane16), "s"(src), "{m0}"(lds));
+// Fragments from memory straight into LDS (lane l's 16 bytes land at base + 16 l), N of 1 KiB by four wavefronts, wavefront
+// w's at src and lds + 1024 w; N is a multiple of 4. In inline assembly, so that the compiler does not drain every load
+// before the next LDS read; the kernels wait (vmcnt) and meet (barrier) themselves.
+template <int N>
+__device__ __forceinline__ void frags_to_lds(const char* src, uint32_t lds, uint32_t lane16) {
+  static_assert(N % 4 == 0, "whole rounds of four wavefronts");
+#pragma unroll
+  for (int f = 0; f < N / 4; ++f)
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane16), "s"(src + f * 4096), "{m0}"(lds + f * 4096));
 }
 __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ uint32_t lds_address(const void* p) {

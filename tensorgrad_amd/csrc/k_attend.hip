@@ -258,17 +258,18 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   const int qe = load_rows<KC>(qrow, valid, a.D, A.wide, qh, ql);
   const float slope = RICH && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
   const int64_t tile0 = (int64_t)slab * tiles;
-  const uint32_t base = lds_address(lds), lane16 = lane * 16;
-  auto fetch = [&](int t, int buf) {
-#pragma unroll
-    for (int f = 0; f < (NF + 3) / 4; ++f) {
-      const int q = f * 4 + w;
-      const _Float16* src;
-      if (q < F_V) src = A.kf + ((tile0 + t) * (2 * KC) + q) * kFrag;
-      else if (q < F_SIDE) src = A.vf + ((tile0 + t) * (4 * DB) + q - F_V) * kFrag;
-      else src = (const _Float16*)(A.side + (tile0 + t) * (kSide * kTile));
-      if (q < NF) frag_to_lds(src, base + (buf * NF + q) * (kFrag * 2), lane16);
-    }
+  const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
+  const char* kf = (const char*)(A.kf + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
+  const char* vf = (const char*)(A.vf + (tile0 + t0) * (4 * DB * kFrag)) + w * 1024;
+  const char* side_p = (const char*)(A.side + (tile0 + t0) * (kSide * kTile));
+  auto fetch = [&](int buf) {    // the next tile
+    const uint32_t to = base + buf * (NF * 1024);
+    frags_to_lds<2 * KC>(kf, to, lane16);
+    kf += 2 * KC * 1024;
+    frags_to_lds<4 * DB>(vf, to + F_V * 1024, lane16);
+    vf += 4 * DB * 1024;
+    if (w == 0) frags_to_lds<4>(side_p, to + F_SIDE * 1024, lane16);
+    side_p += kSide * kTile * 4;
   };
 
   f32x16 acc[DB];
@@ -276,9 +277,10 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
   float m = kNone, sum = 0;        // running maximum (log2) and this lane half's sum
   int ce = kUnset;                 // acc is in units of 2^-ce
+  const float icap = RICH && a.cap > 0 ? 1.0f / a.cap : 0.0f;
   TileInfo kn = {}, vn = {};
   if (t0 < t1) {
-    fetch(t0, 0);
+    fetch(0);
     kn = ki[t0];
     vn = vi[t0];
   }
@@ -288,7 +290,7 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
     __syncthreads();
     const TileInfo kt = kn, vt = vn;
     if (t + 1 < t1) {
-      fetch(t + 1, buf ^ 1);
+      fetch(buf ^ 1);
       kn = ki[t + 1];
       vn = vi[t + 1];
     }
@@ -302,7 +304,7 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
     float f = unit * kLog2e;       // the score is f x, in log2
     if (RICH) {
       if (a.cap > 0) {
-        tanh_all(x, unit / a.cap);
+        tanh_all(x, unit * icap);
         f = a.cap * kLog2e;
       }
       if (a.slopes) {

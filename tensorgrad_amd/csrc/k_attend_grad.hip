@@ -119,28 +119,34 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
   const int ke = load_rows<KC>(a.k.p + b * a.k.b + hk * a.k.h + (int64_t)min(j, a.Tk - 1) * a.k.t, valid, a.D, A.wide, kh, kl);
   const int ve = load_rows<KC>(a.v.p + b * a.v.b + hk * a.v.h + (int64_t)min(j, a.Tk - 1) * a.v.t, valid, a.Dv, A.wide, vh, vl);
   const int64_t tile0 = (int64_t)slab * A.qtiles;
-  const uint32_t base = lds_address(lds), lane16 = lane * 16;
-  auto fetch = [&](int t, int buf) {
-#pragma unroll
-    for (int f = 0; f < (NF + 3) / 4; ++f) {
-      const int q = f * 4 + w;
-      const _Float16* src;
-      if (q < F_GR) src = A.qr + ((tile0 + t) * (2 * KC) + q) * kFrag;
-      else if (q < F_QC) src = A.gr + ((tile0 + t) * (2 * KC) + q - F_GR) * kFrag;
-      else if (q < F_GC) src = A.qc + ((tile0 + t) * (4 * DB) + q - F_QC) * kFrag;
-      else if (q < F_SIDE) src = A.gc + ((tile0 + t) * (4 * DB) + q - F_GC) * kFrag;
-      else src = (const _Float16*)(A.qside + (tile0 + t) * (kSide * kTile));
-      if (q < NF) frag_to_lds(src, base + (buf * NF + q) * (kFrag * 2), lane16);
-    }
+  const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
+  const char* qr = (const char*)(A.qr + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
+  const char* gr = (const char*)(A.gr + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
+  const char* qc = (const char*)(A.qc + (tile0 + t0) * (4 * DB * kFrag)) + w * 1024;
+  const char* gc = (const char*)(A.gc + (tile0 + t0) * (4 * DB * kFrag)) + w * 1024;
+  const char* side_p = (const char*)(A.qside + (tile0 + t0) * (kSide * kTile));
+  auto fetch = [&](int buf) {    // the next tile
+    const uint32_t to = base + buf * (NF * 1024);
+    frags_to_lds<2 * KC>(qr, to, lane16);
+    qr += 2 * KC * 1024;
+    frags_to_lds<2 * KC>(gr, to + F_GR * 1024, lane16);
+    gr += 2 * KC * 1024;
+    frags_to_lds<4 * DB>(qc, to + F_QC * 1024, lane16);
+    qc += 4 * DB * 1024;
+    frags_to_lds<4 * DB>(gc, to + F_GC * 1024, lane16);
+    gc += 4 * DB * 1024;
+    if (w == 0) frags_to_lds<4>(side_p, to + F_SIDE * 1024, lane16);
+    side_p += kSide * kTile * 4;
   };
 
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dk[d] = dv[d] = f32x16{};
   int ck = kUnset, cv = kUnset;
+  const float icap = RICH && a.cap > 0 ? 1.0f / a.cap : 0.0f;
   TileInfo qn = {}, gn = {};
   if (t0 < t1) {
-    fetch(t0, 0);
+    fetch(0);
     qn = qi[t0];
     gn = gi[t0];
   }
@@ -150,7 +156,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
     __syncthreads();
     const TileInfo qt = qn, gt = gn;
     if (t + 1 < t1) {
-      fetch(t + 1, buf ^ 1);
+      fetch(buf ^ 1);
       qn = qi[t + 1];
       gn = gi[t + 1];
     }
@@ -170,7 +176,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
     const float unit = a.scale * pow2(-ke) * qt.inv, yunit = pow2(-ve) * gt.inv;
     float f = unit * kLog2e;
     if (RICH && a.cap > 0) {
-      tanh_all(x, unit / a.cap);
+      tanh_all(x, unit * icap);
       f = a.cap * kLog2e;
 #pragma unroll
       for (int q = 0; q < 16; ++q) slack[q] = fmaf(-x[q], x[q], 1.0f);   // 1 - tanh^2
@@ -320,27 +326,31 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
   const int ge = load_rows<KC>(A.g.dy.p + b * A.g.dy.b + head * A.g.dy.h + (int64_t)i * A.g.dy.t, valid, a.Dv, A.wide, gh, gl);
   const float slope = RICH && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
   const int64_t tile0 = (int64_t)slab * A.ktiles;
-  const uint32_t base = lds_address(lds), lane16 = lane * 16;
-  auto fetch = [&](int t, int buf) {
-#pragma unroll
-    for (int f = 0; f < (NF + 3) / 4; ++f) {
-      const int q = f * 4 + w;
-      const _Float16* src;
-      if (q < F_V) src = A.kr + ((tile0 + t) * (2 * KC) + q) * kFrag;
-      else if (q < F_KC) src = A.vr + ((tile0 + t) * (2 * KC) + q - F_V) * kFrag;
-      else if (q < F_SIDE) src = A.kc + ((tile0 + t) * (4 * DB) + q - F_KC) * kFrag;
-      else src = (const _Float16*)(A.kside + (tile0 + t) * (kSide * kTile));
-      if (q < NF) frag_to_lds(src, base + (buf * NF + q) * (kFrag * 2), lane16);
-    }
+  const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
+  const char* kr = (const char*)(A.kr + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
+  const char* vr = (const char*)(A.vr + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
+  const char* kc = (const char*)(A.kc + (tile0 + t0) * (4 * DB * kFrag)) + w * 1024;
+  const char* side_p = (const char*)(A.kside + (tile0 + t0) * (kSide * kTile));
+  auto fetch = [&](int buf) {    // the next tile
+    const uint32_t to = base + buf * (NF * 1024);
+    frags_to_lds<2 * KC>(kr, to, lane16);
+    kr += 2 * KC * 1024;
+    frags_to_lds<2 * KC>(vr, to + F_V * 1024, lane16);
+    vr += 2 * KC * 1024;
+    frags_to_lds<4 * DB>(kc, to + F_KC * 1024, lane16);
+    kc += 4 * DB * 1024;
+    if (w == 0) frags_to_lds<4>(side_p, to + F_SIDE * 1024, lane16);
+    side_p += kSide * kTile * 4;
   };
 
   f32x16 dq[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dq[d] = f32x16{};
   int cq = kUnset;
+  const float icap = RICH && a.cap > 0 ? 1.0f / a.cap : 0.0f;
   TileInfo kn = {}, vn = {};
   if (t0 < t1) {
-    fetch(t0, 0);
+    fetch(0);
     kn = ki[t0];
     vn = vi[t0];
   }
@@ -350,7 +360,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
     __syncthreads();
     const TileInfo kt = kn, vt = vn;
     if (t + 1 < t1) {
-      fetch(t + 1, buf ^ 1);
+      fetch(buf ^ 1);
       kn = ki[t + 1];
       vn = vi[t + 1];
     }
@@ -362,7 +372,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
     if (vt.uneven) per_row(y, side + KS_RELV * kTile);
     const float unit = a.scale * pow2(-qe) * kt.inv, yunit = pow2(-ge) * vt.inv;
     const bool cap = RICH && a.cap > 0;
-    if (cap) tanh_all(x, unit / a.cap);
+    if (cap) tanh_all(x, unit * icap);
     const float f = (cap ? a.cap : unit) * kLog2e;
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
