@@ -41,6 +41,13 @@ struct TileInfo {
   int pad;
 };
 
+// What a block needs of each row of a tile it walks, 32 values each (integers as bits), 2 KiB that come with the fragments
+// into LDS: of queries and of keys. Row S_INFO: the TileInfo of the first operand (q, k) and eight words on the second's (dy,
+// v). From LDS, because a load from memory inside the loop would wait for the next tile's fragments, which are ahead of it.
+enum { QS_LSE, QS_DOT, QS_POS, QS_SLOPE, QS_BELOW, QS_DOC, QS_RELQ, QS_RELG, S_INFO, kSide = 16 };   // dot(dy, y); sees keys below
+enum { KS_DOC, KS_RELK, KS_RELV };
+constexpr int kSideFrags = kSide * kTile * 4 / 1024;
+
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 __device__ __forceinline__ int exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 255) - 127; }   // floor(log2 |x|)
 
@@ -285,6 +292,40 @@ __device__ __forceinline__ f32x16 scores(const _Float16* L, int f0, const half8 
   for (int q = 0; q < 16; ++q) x[q] += y[q];
   return x;
 }
+// Both products of a gradient's pair, step by step in turn: four accumulators, and twice the products between a fragment's
+// read and its use. For head sizes above 64, where a SIMD has one wavefront to keep it busy.
+template <int KC>
+__device__ __forceinline__ void scores2(const _Float16* L, int f0, const half8 (&bh)[KC], const half8 (&bl)[KC], f32x16& x, int f1,
+                                        const half8 (&ch)[KC], const half8 (&cl)[KC], f32x16& y) {
+  f32x16 x0 = {}, x1 = {}, y0 = {}, y1 = {};
+  half8 a[2][4];
+  auto read = [&](int c) {
+    a[c & 1][0] = frag(L, f0 + 2 * c);
+    a[c & 1][1] = frag(L, f0 + 2 * c + 1);
+    a[c & 1][2] = frag(L, f1 + 2 * c);
+    a[c & 1][3] = frag(L, f1 + 2 * c + 1);
+  };
+  read(0);
+  __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+  for (int c = 0; c < KC; ++c) {
+    if (c + 1 < KC) read(c + 1);
+    const half8* f = a[c & 1];
+    x1 = mfma(f[1], bh[c], x1);
+    y1 = mfma(f[3], ch[c], y1);
+    x0 = mfma(f[0], bh[c], x0);
+    y0 = mfma(f[2], ch[c], y0);
+    x1 = mfma(f[0], bl[c], x1);
+    y1 = mfma(f[2], cl[c], y1);
+    if (c + 1 < KC) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);   // the next step's reads, then this step's products
+    __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
+  }
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    x[q] = x0[q] + x1[q];
+    y[q] = y0[q] + y1[q];
+  }
+}
 // x[q] *= rel of the tile's row 8 (q / 4) + 4 h + q % 4
 __device__ __forceinline__ void per_row(f32x16& x, const float* rel) {
   const int h = (threadIdx.x >> 5) & 1;
@@ -323,6 +364,12 @@ __device__ __forceinline__ void store_row(float* row, const f32x16 (&acc)[DB], i
     }
 }
 
+// Operand x's (0 or 1) TileInfo from a side block, wave-uniform.
+__device__ __forceinline__ TileInfo side_info(const float* side, int x) {
+  const int* p = (const int*)(side + S_INFO * kTile + 8 * x);
+  auto u = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  return {__int_as_float(u(p[0])), __int_as_float(u(p[1])), u(p[2]), u(p[3]), u(p[4]), u(p[5]), u(p[6]), 0};
+}
 // First and one past the last of the tiles [t0, t1) whose documents meet [lo, hi] (all of them without documents); odd: one
 // of those is. By the whole block.
 struct Range {
@@ -417,12 +464,10 @@ struct PackJob {
   bool query;                      // rows are queries, else keys
   float* side;                     // [slab][tile][kSide][32]: what a block needs of each row of the tile, see below
   int rel;                         // where this operand's rel goes
+  bool second;                     // and its info
   bool ids;                        // this job also writes the rows' documents and the rest
   Rows y;                          // of the gradient dy (ids of queries): y's rows for its dot products
 };
-// Rows of a side block, 32 values each (integers as bits), 1 KiB in all: of queries and of keys.
-enum { QS_LSE, QS_DOT, QS_POS, QS_SLOPE, QS_BELOW, QS_DOC, QS_RELQ, QS_RELG, kSide = 8 };   // dot(dy, y); sees keys below
-enum { KS_DOC, KS_RELK, KS_RELV };
 // The attention's operands as packed for one pass, in the workspace.
 struct Packs {
   int n;

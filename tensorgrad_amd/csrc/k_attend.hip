@@ -95,7 +95,11 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
   const bool uneven = !bad && hi > 0 && exponent(hi) - exponent(lo) > 12, same = dmin == dmax && !__any(doc[l] < 0);
   const int e = bad || hi == 0 ? 0 : min(14 - exponent(hi), 126);
   const int64_t slot = (int64_t)slab * j.tiles + tile;
-  if (tid == 0) j.info[slot] = {pow2(e), pow2(-e), uneven, bad, dmin, dmax, same, 0};
+  if (tid == 0) {
+    const TileInfo t = {pow2(e), pow2(-e), uneven, bad, dmin, dmax, same, 0};
+    j.info[slot] = t;
+    *(TileInfo*)(side + S_INFO * kTile + 8 * j.second) = t;
+  }
   if (tid < kTile) {
     const int mye = uneven && mine > 0 ? min(14 - exponent(mine), 126) : e;
     own[l] = pow2(mye);
@@ -199,7 +203,7 @@ __device__ __forceinline__ void plain_rows(const TilesArgs& A, const Sight& s, i
 
 template <int DP, bool RICH>       // RICH: capped scores or slopes
 __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
-  constexpr int KC = DP / 16, DB = DP / 32, F_V = 2 * KC, F_SIDE = F_V + 4 * DB, NF = F_SIDE + 1;
+  constexpr int KC = DP / 16, DB = DP / 32, F_V = 2 * KC, F_SIDE = F_V + 4 * DB, NF = F_SIDE + kSideFrags;
   __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
   __shared__ int range[5];
   const AttendDesc& a = A.a;
@@ -261,14 +265,14 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
   const char* kf = (const char*)(A.kf + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
   const char* vf = (const char*)(A.vf + (tile0 + t0) * (4 * DB * kFrag)) + w * 1024;
-  const char* side_p = (const char*)(A.side + (tile0 + t0) * (kSide * kTile));
+  const char* side_p = (const char*)(A.side + (tile0 + t0) * (kSide * kTile)) + w * 1024;
   auto fetch = [&](int buf) {    // the next tile
     const uint32_t to = base + buf * (NF * 1024);
     frags_to_lds<2 * KC>(kf, to, lane16);
     kf += 2 * KC * 1024;
     frags_to_lds<4 * DB>(vf, to + F_V * 1024, lane16);
     vf += 4 * DB * 1024;
-    if (w == 0) frags_to_lds<4>(side_p, to + F_SIDE * 1024, lane16);
+    if (w < kSideFrags) frags_to_lds<4>(side_p, to + F_SIDE * 1024, lane16);
     side_p += kSide * kTile * 4;
   };
 
@@ -278,25 +282,16 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   float m = kNone, sum = 0;        // running maximum (log2) and this lane half's sum
   int ce = kUnset;                 // acc is in units of 2^-ce
   const float icap = RICH && a.cap > 0 ? 1.0f / a.cap : 0.0f;
-  TileInfo kn = {}, vn = {};
-  if (t0 < t1) {
-    fetch(0);
-    kn = ki[t0];
-    vn = vi[t0];
-  }
+  if (t0 < t1) fetch(0);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, j0 = t * kTile;
     loads_done();
     __syncthreads();
-    const TileInfo kt = kn, vt = vn;
-    if (t + 1 < t1) {
-      fetch(buf ^ 1);
-      kn = ki[t + 1];
-      vn = vi[t + 1];
-    }
-    if (!any_seen(s, me, kt, j0)) continue;
+    if (t + 1 < t1) fetch(buf ^ 1);
     const _Float16* L = lds + buf * (NF * kFrag);
     const float* side = (const float*)(L + F_SIDE * kFrag);
+    const TileInfo kt = side_info(side, 0), vt = side_info(side, 1);
+    if (!any_seen(s, me, kt, j0)) continue;
     // scores, transposed: register r of this lane is key j0 + 8 (r / 4) + 4 h + r % 4
     f32x16 x = scores<KC>(L, 0, qh, ql);
     if (kt.uneven) per_row(x, side + KS_RELK * kTile);
@@ -633,8 +628,8 @@ void attend(const AttendDesc& a, void* work, hipStream_t st) {
     k.wide = wide;
     k.a = a;
     float* side = (float*)(w + p.side);
-    k.job[0] = {a.k, a.D, 1, a.Tk, p.tiles, (_Float16*)(w + p.kf), nullptr, (TileInfo*)(w + p.ki), false, side, KS_RELK, true, {}};
-    k.job[1] = {a.v, a.Dv, 1, a.Tk, p.tiles, nullptr, (_Float16*)(w + p.vf), (TileInfo*)(w + p.vi), false, side, KS_RELV, false, {}};
+    k.job[0] = {a.k, a.D, 1, a.Tk, p.tiles, (_Float16*)(w + p.kf), nullptr, (TileInfo*)(w + p.ki), false, side, KS_RELK, false, true, {}};
+    k.job[1] = {a.v, a.Dv, 1, a.Tk, p.tiles, nullptr, (_Float16*)(w + p.vf), (TileInfo*)(w + p.vi), false, side, KS_RELV, true, false, {}};
     attend_pack(k, p.DP, st);
     const TilesArgs t{a, (_Float16*)(w + p.kf), (_Float16*)(w + p.vf), (TileInfo*)(w + p.ki), (TileInfo*)(w + p.vi), side,
                       make_fastdiv(p.G), p.M, p.blocks, p.splits, wide, part, plse};

@@ -76,7 +76,7 @@ __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, in
 template <int DP, bool RICH>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs A) {
   constexpr int KC = DP / 16, DB = DP / 32;
-  constexpr int F_GR = 2 * KC, F_QC = 4 * KC, F_GC = F_QC + 4 * DB, F_SIDE = F_GC + 4 * DB, NF = F_SIDE + 1;
+  constexpr int F_GR = 2 * KC, F_QC = 4 * KC, F_GC = F_QC + 4 * DB, F_SIDE = F_GC + 4 * DB, NF = F_SIDE + kSideFrags;
   __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
   __shared__ int range[5];
   const AttendDesc& a = A.g.a;
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
   const char* gr = (const char*)(A.gr + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
   const char* qc = (const char*)(A.qc + (tile0 + t0) * (4 * DB * kFrag)) + w * 1024;
   const char* gc = (const char*)(A.gc + (tile0 + t0) * (4 * DB * kFrag)) + w * 1024;
-  const char* side_p = (const char*)(A.qside + (tile0 + t0) * (kSide * kTile));
+  const char* side_p = (const char*)(A.qside + (tile0 + t0) * (kSide * kTile)) + w * 1024;
   auto fetch = [&](int buf) {    // the next tile
     const uint32_t to = base + buf * (NF * 1024);
     frags_to_lds<2 * KC>(qr, to, lane16);
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
     qc += 4 * DB * 1024;
     frags_to_lds<4 * DB>(gc, to + F_GC * 1024, lane16);
     gc += 4 * DB * 1024;
-    if (w == 0) frags_to_lds<4>(side_p, to + F_SIDE * 1024, lane16);
+    if (w < kSideFrags) frags_to_lds<4>(side_p, to + F_SIDE * 1024, lane16);
     side_p += kSide * kTile * 4;
   };
 
@@ -144,22 +144,15 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
   for (int d = 0; d < DB; ++d) dk[d] = dv[d] = f32x16{};
   int ck = kUnset, cv = kUnset;
   const float icap = RICH && a.cap > 0 ? 1.0f / a.cap : 0.0f;
-  TileInfo qn = {}, gn = {};
-  if (t0 < t1) {
-    fetch(0);
-    qn = qi[t0];
-    gn = gi[t0];
-  }
+  if (t0 < t1) fetch(0);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, r0 = t * kTile;
     loads_done();
     __syncthreads();
-    const TileInfo qt = qn, gt = gn;
-    if (t + 1 < t1) {
-      fetch(buf ^ 1);
-      qn = qi[t + 1];
-      gn = gi[t + 1];
-    }
+    if (t + 1 < t1) fetch(buf ^ 1);
+    const _Float16* L = lds + buf * (NF * kFrag);
+    const float* side = (const float*)(L + F_SIDE * kFrag);
+    const TileInfo qt = side_info(side, 0), gt = side_info(side, 1);
     Span rows;
     rows.pmin = s.first + (int)fastdiv((uint32_t)r0, A.group);
     rows.pmax = s.first + (int)fastdiv((uint32_t)min(r0 + kTile - 1, A.M - 1), A.group);
@@ -167,10 +160,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
     rows.dmax = gt.dmax;
     rows.same = gt.same;
     if (j0 >= a.Tk || !any_seen(s, rows, mine, j0)) continue;
-    const _Float16* L = lds + buf * (NF * kFrag);
-    const float* side = (const float*)(L + F_SIDE * kFrag);
     // register r: row r0 + 8 (r / 4) + 4 h + r % 4
-    f32x16 x = scores<KC>(L, 0, kh, kl), y = scores<KC>(L, F_GR, vh, vl), slack;
+    f32x16 x, y, slack;
+    if constexpr (DP > 64) {
+      scores2<KC>(L, 0, kh, kl, x, F_GR, vh, vl, y);
+    } else {
+      x = scores<KC>(L, 0, kh, kl);
+      y = scores<KC>(L, F_GR, vh, vl);
+    }
     if (qt.uneven) per_row(x, side + QS_RELQ * kTile);
     if (gt.uneven) per_row(y, side + QS_RELG * kTile);
     const float unit = a.scale * pow2(-ke) * qt.inv, yunit = pow2(-ve) * gt.inv;
@@ -283,7 +280,7 @@ __device__ __forceinline__ void plain_dq(const GradArgs& A, const Sight& s, int 
 template <int DP, bool RICH>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs A) {
   constexpr int KC = DP / 16, DB = DP / 32;
-  constexpr int F_V = 2 * KC, F_KC = 4 * KC, F_SIDE = F_KC + 4 * DB, NF = F_SIDE + 1;
+  constexpr int F_V = 2 * KC, F_KC = 4 * KC, F_SIDE = F_KC + 4 * DB, NF = F_SIDE + kSideFrags;
   __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
   __shared__ int range[5];
   const AttendDesc& a = A.g.a;
@@ -330,7 +327,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
   const char* kr = (const char*)(A.kr + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
   const char* vr = (const char*)(A.vr + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
   const char* kc = (const char*)(A.kc + (tile0 + t0) * (4 * DB * kFrag)) + w * 1024;
-  const char* side_p = (const char*)(A.kside + (tile0 + t0) * (kSide * kTile));
+  const char* side_p = (const char*)(A.kside + (tile0 + t0) * (kSide * kTile)) + w * 1024;
   auto fetch = [&](int buf) {    // the next tile
     const uint32_t to = base + buf * (NF * 1024);
     frags_to_lds<2 * KC>(kr, to, lane16);
@@ -339,7 +336,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
     vr += 2 * KC * 1024;
     frags_to_lds<4 * DB>(kc, to + F_KC * 1024, lane16);
     kc += 4 * DB * 1024;
-    if (w == 0) frags_to_lds<4>(side_p, to + F_SIDE * 1024, lane16);
+    if (w < kSideFrags) frags_to_lds<4>(side_p, to + F_SIDE * 1024, lane16);
     side_p += kSide * kTile * 4;
   };
 
@@ -348,26 +345,23 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
   for (int d = 0; d < DB; ++d) dq[d] = f32x16{};
   int cq = kUnset;
   const float icap = RICH && a.cap > 0 ? 1.0f / a.cap : 0.0f;
-  TileInfo kn = {}, vn = {};
-  if (t0 < t1) {
-    fetch(0);
-    kn = ki[t0];
-    vn = vi[t0];
-  }
+  if (t0 < t1) fetch(0);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, j0 = t * kTile;
     loads_done();
     __syncthreads();
-    const TileInfo kt = kn, vt = vn;
-    if (t + 1 < t1) {
-      fetch(buf ^ 1);
-      kn = ki[t + 1];
-      vn = vi[t + 1];
-    }
-    if (!any_seen(s, me, kt, j0)) continue;
+    if (t + 1 < t1) fetch(buf ^ 1);
     const _Float16* L = lds + buf * (NF * kFrag);
     const float* side = (const float*)(L + F_SIDE * kFrag);
-    f32x16 x = scores<KC>(L, 0, qh, ql), y = scores<KC>(L, F_V, gh, gl);
+    const TileInfo kt = side_info(side, 0), vt = side_info(side, 1);
+    if (!any_seen(s, me, kt, j0)) continue;
+    f32x16 x, y;
+    if constexpr (DP > 64) {
+      scores2<KC>(L, 0, qh, ql, x, F_V, gh, gl, y);
+    } else {
+      x = scores<KC>(L, 0, qh, ql);
+      y = scores<KC>(L, F_V, gh, gl);
+    }
     if (kt.uneven) per_row(x, side + KS_RELK * kTile);
     if (vt.uneven) per_row(y, side + KS_RELV * kTile);
     const float unit = a.scale * pow2(-qe) * kt.inv, yunit = pow2(-ge) * vt.inv;
@@ -481,10 +475,10 @@ void attend_grad(const AttendGradDesc& g, void* work, hipStream_t st) {
   k.wide = wide;
   k.a = a;
   float *qs = (float*)(w + p.qside), *ks = (float*)(w + p.kside);
-  k.job[0] = {a.q, a.D, p.G, p.M, p.qtiles, half(p.qr), half(p.qc), info(p.qi), true, qs, QS_RELQ, false, {}};
-  k.job[1] = {g.dy, a.Dv, p.G, p.M, p.qtiles, half(p.gr), half(p.gc), info(p.gi), true, qs, QS_RELG, true, a.y};
-  k.job[2] = {a.k, a.D, 1, a.Tk, p.ktiles, half(p.kr), half(p.kc), info(p.ki), false, ks, KS_RELK, true, {}};
-  k.job[3] = {a.v, a.Dv, 1, a.Tk, p.ktiles, half(p.vr), nullptr, info(p.vi), false, ks, KS_RELV, false, {}};
+  k.job[0] = {a.q, a.D, p.G, p.M, p.qtiles, half(p.qr), half(p.qc), info(p.qi), true, qs, QS_RELQ, false, false, {}};
+  k.job[1] = {g.dy, a.Dv, p.G, p.M, p.qtiles, half(p.gr), half(p.gc), info(p.gi), true, qs, QS_RELG, true, true, a.y};
+  k.job[2] = {a.k, a.D, 1, a.Tk, p.ktiles, half(p.kr), half(p.kc), info(p.ki), false, ks, KS_RELK, false, true, {}};
+  k.job[3] = {a.v, a.Dv, 1, a.Tk, p.ktiles, half(p.vr), nullptr, info(p.vi), false, ks, KS_RELV, true, false, {}};
   attend_pack(k, p.DP, st);
   const GradArgs A{g, half(p.qr), half(p.qc), half(p.gr), half(p.gc), half(p.kr), half(p.kc), half(p.vr),
                    info(p.qi), info(p.gi), info(p.ki), info(p.vi), qs, ks, make_fastdiv(p.G), p.M, p.qtiles,
