@@ -237,16 +237,20 @@ __device__ __forceinline__ void rescale(f32x16 (&acc)[DB], float change) {
     for (int q = 0; q < 16; ++q) acc[d][q] *= change;
 }
 __device__ __forceinline__ half8 frag(const _Float16* L, int f) { return *(const half8*)(L + f * kFrag + (threadIdx.x & 63) * 8); }
-// acc += A fragments (feature blocks x two k steps, from fragment f0 of L) times the split of x * scale. Fragments are read
-// one step ahead of the products that take them; products of different accumulators alternate.
+// acc += A fragments (feature blocks x two k steps, from fragment f0 of L) times the split of x * scale, two of them a step;
+// a step's fragments are read while the step before is multiplied.
 template <int DB>
 __device__ __forceinline__ void accumulate(f32x16 (&acc)[DB], const f32x16& x, float scale, const _Float16* L, int f0) {
-  half8 ah[2][DB], al[2][DB];
+  half8 a[2][4];
+  auto read = [&](int i) {         // of fragments 2 i and 2 i + 1: feature block u % DB, k step u / DB
 #pragma unroll
-  for (int d = 0; d < DB; ++d) {
-    ah[0][d] = frag(L, f0 + d * 4);
-    al[0][d] = frag(L, f0 + d * 4 + 1);
-  }
+    for (int e = 0; e < 2; ++e) {
+      const int u = 2 * i + e, f = f0 + u % DB * 4 + u / DB * 2;
+      a[i & 1][2 * e] = frag(L, f);
+      a[i & 1][2 * e + 1] = frag(L, f + 1);
+    }
+  };
+  read(0);
   half8 bh[2], bl[2];
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
@@ -256,19 +260,16 @@ __device__ __forceinline__ void accumulate(f32x16 (&acc)[DB], const f32x16& x, f
     split8(z, bh[ks], bl[ks]);
   }
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
-    if (ks == 0)
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        ah[1][d] = frag(L, f0 + d * 4 + 2);
-        al[1][d] = frag(L, f0 + d * 4 + 3);
-      }
-#pragma unroll
-    for (int d = 0; d < DB; ++d) acc[d] = mfma(al[ks][d], bh[ks], acc[d]);
-#pragma unroll
-    for (int d = 0; d < DB; ++d) acc[d] = mfma(ah[ks][d], bl[ks], acc[d]);
-#pragma unroll
-    for (int d = 0; d < DB; ++d) acc[d] = mfma(ah[ks][d], bh[ks], acc[d]);
+  for (int i = 0; i < DB; ++i) {
+    if (i + 1 < DB) read(i + 1);
+    const int d0 = 2 * i % DB, k0 = 2 * i / DB, d1 = (2 * i + 1) % DB, k1 = (2 * i + 1) / DB;
+    const half8* f = a[i & 1];
+    acc[d0] = mfma(f[1], bh[k0], acc[d0]);
+    acc[d1] = mfma(f[3], bh[k1], acc[d1]);
+    acc[d0] = mfma(f[0], bl[k0], acc[d0]);
+    acc[d1] = mfma(f[2], bl[k1], acc[d1]);
+    acc[d0] = mfma(f[0], bh[k0], acc[d0]);
+    acc[d1] = mfma(f[2], bh[k1], acc[d1]);
   }
 }
 // A fragments (KC k steps, from fragment f0 of L) times B fragments; two accumulators take turns.
@@ -444,13 +445,22 @@ __device__ __forceinline__ void plain_add(float (&acc)[2], float w, RowOf row_of
   }
 }
 
-// Blocks of one slab (batch entry and key head) on one XCD, whose L2 then holds its packed tiles: hardware deals block ids
-// to the 8 XCDs in turn.
-__device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t total) {
-  const uint32_t per = total / 8;
-  return id < per * 8 ? (id % 8) * per + id / 8 : id;
+// A block's slab (batch entry and key head) and its item of the slab's, in the order that blocks start. Hardware deals block
+// ids to the 8 XCDs in turn; a slab stays on one XCD (or 2, 4, 8 of them where there are fewer slabs), whose L2 then holds
+// its packed tiles, and every XCD gets long and short items alike.
+__device__ __forceinline__ void place(uint32_t id, uint32_t slabs, int& slab, int& item) {
+  const uint32_t x = id % 8, k = id / 8;
+  if (slabs % 8 == 0) {
+    slab = x + 8 * (k % (slabs / 8));
+    item = k / (slabs / 8);
+  } else if (8 % slabs == 0) {
+    slab = x % slabs;
+    item = k * (8 / slabs) + x / slabs;
+  } else {
+    slab = id % slabs;
+    item = id / slabs;
+  }
 }
-
 }  // namespace
 
 // ---- packing -----------------------------------------------------------------------------------
@@ -477,6 +487,10 @@ struct Packs {
   AttendDesc a;
 };
 void attend_pack(const Packs& p, int DP, hipStream_t st);
+// Blocks for `items` of each slab: those of place() beyond the last item end at once.
+inline unsigned place_grid(int64_t slabs, int64_t items) {
+  return (unsigned)(slabs % 8 != 0 && 8 % slabs == 0 ? (items + 8 / slabs - 1) / (8 / slabs) * 8 : slabs * items);
+}
 inline int attend_dp(const AttendDesc& a) { return (max(a.D, a.Dv) + 31) / 32 * 32; }
 inline bool attend_wide(const Rows& x, int n) {
   return ((uintptr_t)x.p & 15) == 0 && x.b % 4 == 0 && x.h % 4 == 0 && x.t % 4 == 0 && n % 8 == 0;

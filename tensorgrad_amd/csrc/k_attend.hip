@@ -208,10 +208,14 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   __shared__ int range[5];
   const AttendDesc& a = A.a;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
-  const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
-  const uint32_t per = (uint32_t)A.blocks * A.splits;
-  const int slab = id / per, split = id % per % A.splits;
-  const int blk = A.blocks - 1 - (int)(id % per / A.splits);       // the last rows see the most keys: first
+  int slab, item;
+  place(blockIdx.x, a.B * a.Hk, slab, item);
+  if (item >= A.blocks * A.splits) return;
+  // The last rows see the most keys: first. Where all blocks run at once, two on a CU, the second half goes the other way, so
+  // that a CU's two are a long and a short one.
+  const int all = A.blocks * A.splits, half = all / 2;
+  if (gridDim.x <= 512 && item >= half) item = all - 1 - (item - half);
+  const int split = item % A.splits, blk = A.blocks - 1 - item / A.splits;
   const int b = slab / a.Hk, hk = slab % a.Hk, G = (int)A.group.d;
   const Sight s = sight(a, b);
   const int tiles = (a.Tk + kTile - 1) / kTile;
@@ -575,9 +579,9 @@ Plan plan(const AttendDesc& a) {
 }
 
 template <int DP>
-void run_tiles(const TilesArgs& t, int64_t grid, hipStream_t st) {
-  if (t.a.cap > 0 || t.a.slopes) klaunch(attend_tiles<DP, true>, dim3((unsigned)grid), dim3(256), 0, st, t);
-  else klaunch(attend_tiles<DP, false>, dim3((unsigned)grid), dim3(256), 0, st, t);
+void run_tiles(const TilesArgs& t, unsigned grid, hipStream_t st) {
+  if (t.a.cap > 0 || t.a.slopes) klaunch(attend_tiles<DP, true>, dim3(grid), dim3(256), 0, st, t);
+  else klaunch(attend_tiles<DP, false>, dim3(grid), dim3(256), 0, st, t);
 }
 template <int E, int R>
 void run_few(const FewArgs& f, bool wide, int slabs, hipStream_t st) {
@@ -633,7 +637,7 @@ void attend(const AttendDesc& a, void* work, hipStream_t st) {
     attend_pack(k, p.DP, st);
     const TilesArgs t{a, (_Float16*)(w + p.kf), (_Float16*)(w + p.vf), (TileInfo*)(w + p.ki), (TileInfo*)(w + p.vi), side,
                       make_fastdiv(p.G), p.M, p.blocks, p.splits, wide, part, plse};
-    const int64_t grid = (int64_t)p.slabs * p.blocks * p.splits;
+    const unsigned grid = place_grid(p.slabs, (int64_t)p.blocks * p.splits);
     if (p.DP == 32) run_tiles<32>(t, grid, st);
     else if (p.DP == 64) run_tiles<64>(t, grid, st);
     else if (p.DP == 96) run_tiles<96>(t, grid, st);

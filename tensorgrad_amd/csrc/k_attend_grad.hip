@@ -24,6 +24,18 @@ struct GradArgs {
 
 // ---- dk, dv --------------------------------------------------------------------------------------
 
+// Query tiles [from, to) of part `split` that the masks by position let see any of the keys [k0, k0 + 128): parts are equal
+// stretches of the rows. False: none, which the join finds again and does not read.
+__device__ __forceinline__ bool part_rows(const GradArgs& A, const Sight& s, int k0, int split, int& from, int& to) {
+  int64_t i0 = 0;                  // first position index that sees any: a prefix shows its keys to all
+  if (s.causal && k0 >= s.prefix) i0 = (int64_t)k0 - s.first;
+  if (s.positional) i0 = max(i0, (int64_t)-s.first);
+  const int each = (A.qtiles + A.splits - 1) / A.splits;
+  from = max((int)min(max(i0, (int64_t)0) * A.group.d / kTile, (int64_t)A.qtiles), split * each);
+  to = k0 < s.n ? min((split + 1) * each, A.qtiles) : 0;
+  return from < to || A.splits == 1;
+}
+
 // Where dk and dv of key j go.
 __device__ __forceinline__ float* dk_row(const GradArgs& A, int split, int slab, int b, int hk, int j) {
   if (!A.g.dk.p) return nullptr;
@@ -81,9 +93,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
   __shared__ int range[5];
   const AttendDesc& a = A.g.a;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
-  const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
-  const uint32_t per = (uint32_t)A.blocks * A.splits;
-  const int slab = id / per, split = id % per % A.splits, blk = id % per / A.splits;   // the first keys are seen by most
+  int slab, item;
+  place(blockIdx.x, a.B * a.Hk, slab, item);
+  if (item >= A.blocks * A.splits) return;
+  const int split = A.splits - 1 - item / A.blocks, blk = item % A.blocks;   // blocks that start together walk the same rows
   const int b = slab / a.Hk, hk = slab % a.Hk;
   const Sight s = sight(a, b);
   const int j0 = blk * 128 + w * kTile, j = j0 + l;
@@ -99,17 +112,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
   const TileInfo* qi = A.qi + (int64_t)slab * A.qtiles;
   const TileInfo* gi = A.gi + (int64_t)slab * A.qtiles;
   const int k0 = blk * 128;
-  int64_t i0 = 0;                  // first position index that sees anything here
-  if (s.causal && k0 >= s.prefix) i0 = (int64_t)k0 - s.first;
-  if (s.positional) i0 = max(i0, (int64_t)-s.first);
-  const int from = (int)min(max(i0, (int64_t)0) * A.group.d / kTile, (int64_t)A.qtiles);
-  const Range range_ = tile_range(s, from, k0 < s.n ? A.qtiles : 0, gi, qi, gi, mine.dmin, mine.dmax, range);
-  int t0 = range_.t0, t1 = range_.t1;
-  if (A.splits > 1) {
-    const int n = t1 - t0, each = (n + A.splits - 1) / A.splits;
-    t0 = min(t0 + split * each, t1);
-    t1 = min(t0 + each, t1);
-  }
+  int from, to;
+  if (!part_rows(A, s, k0, split, from, to)) return;   // nothing, and the join knows
+  const Range range_ = tile_range(s, from, to, gi, qi, gi, mine.dmin, mine.dmax, range);
+  const int t0 = range_.t0, t1 = range_.t1;
   if (range_.odd) {
     plain_keys(A, s, split, slab, b, hk, j0, t0 * kTile, t1 * kTile);
     return;
@@ -237,10 +243,14 @@ __global__ __launch_bounds__(256) void attend_grad_join(GradArgs A) {
   if (!o.p) return;
   const int64_t all = (int64_t)a.B * a.Hk * a.Tk * n, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= all) return;
-  float x = 0;
-  for (int z = 0; z < A.splits; ++z) x += part[at + z * all];
   const int64_t row = at / n;
   const int d = (int)(at - row * n), j = (int)(row % a.Tk), slab = (int)(row / a.Tk);
+  const Sight s = sight(a, slab / a.Hk);
+  float x = 0;
+  for (int z = 0; z < A.splits; ++z) {
+    int from, to;
+    if (part_rows(A, s, j / 128 * 128, z, from, to)) x += part[at + z * all];
+  }
   o.p[slab / a.Hk * o.b + slab % a.Hk * o.h + (int64_t)j * o.t + d] = x;
 }
 
@@ -285,9 +295,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
   __shared__ int range[5];
   const AttendDesc& a = A.g.a;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
-  const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
   const int rblocks = (A.M + 127) / 128;
-  const int slab = id / rblocks, blk = rblocks - 1 - (int)(id % rblocks);
+  int slab, item;
+  place(blockIdx.x, a.B * a.Hk, slab, item);
+  if (item >= rblocks) return;
+  const int blk = rblocks - 1 - item;
   const int b = slab / a.Hk, hk = slab % a.Hk, G = (int)A.group.d;
   const Sight s = sight(a, b);
   const int row0 = blk * 128 + w * kTile, r = row0 + l, rr = min(r, A.M - 1);
@@ -414,7 +426,8 @@ GradPlan grad_plan(const AttendGradDesc& g) {
   p.ktiles = (a.Tk + kTile - 1) / kTile;
   p.blocks = (a.Tk + 127) / 128;
   const int64_t have = (int64_t)p.slabs * p.blocks;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / have, p.qtiles / 8));
+  const int lim = getenv("KV_LIM") ? atoi(getenv("KV_LIM")) : 1024;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((lim + have - 1) / have, p.qtiles / 8));
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t b = at;
@@ -447,9 +460,9 @@ template <int DP, bool RICH>
 void run_grad(const GradArgs& A, int slabs, hipStream_t st) {
   const AttendGradDesc& g = A.g;
   if (g.dk.p || g.dv.p)
-    klaunch(attend_grad_kv<DP, RICH>, dim3((unsigned)(slabs * A.blocks * A.splits)), dim3(256), 0, st, A);
+    klaunch(attend_grad_kv<DP, RICH>, dim3(place_grid(slabs, (int64_t)A.blocks * A.splits)), dim3(256), 0, st, A);
   if (g.dq.p)
-    klaunch(attend_grad_q<DP, RICH>, dim3((unsigned)(slabs * ((A.M + 127) / 128))), dim3(256), 0, st, A);
+    klaunch(attend_grad_q<DP, RICH>, dim3(place_grid(slabs, (A.M + 127) / 128)), dim3(256), 0, st, A);
 }
 template <int DP>
 void run_grad(const GradArgs& A, int slabs, hipStream_t st) {
