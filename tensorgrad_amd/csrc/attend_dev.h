@@ -293,6 +293,28 @@ __device__ __forceinline__ f32x16 scores(const _Float16* L, int f0, const half8 
   for (int q = 0; q < 16; ++q) x[q] += y[q];
   return x;
 }
+// x = A fragments times B fragments, woven with work(0), .. work(N - 1), vector work of other data. A wavefront issues in
+// order: a product issued right behind another waits for the matrix unit, and everything after it waits too. With vector work
+// between the products both units run. The scheduler is held to the written order, step by step.
+template <int KC, int N, class Work>
+__device__ __forceinline__ void scores_woven(f32x16& x, const _Float16* L, int f0, const half8 (&bh)[KC], const half8 (&bl)[KC], Work work) {
+  half8 ah[2], al[2];
+  ah[0] = frag(L, f0);
+  al[0] = frag(L, f0 + 1);
+  x = f32x16{};
+#pragma unroll
+  for (int m = 0; m < 3 * KC; ++m) {
+    const int c = m / 3, k = m % 3;
+    if (k == 0 && c + 1 < KC) {
+      ah[(c + 1) & 1] = frag(L, f0 + 2 * c + 2);
+      al[(c + 1) & 1] = frag(L, f0 + 2 * c + 3);
+    }
+    x = mfma(k == 0 ? al[c & 1] : ah[c & 1], k == 1 ? bl[c] : bh[c], x);
+#pragma unroll
+    for (int i = N * m / (3 * KC); i < N * (m + 1) / (3 * KC); ++i) work(i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
 // Both products of a gradient's pair, step by step in turn: four accumulators, and twice the products between a fragment's
 // read and its use. For head sizes above 64, where a SIMD has one wavefront to keep it busy.
 template <int KC>

@@ -201,10 +201,10 @@ __device__ __forceinline__ void plain_rows(const TilesArgs& A, const Sight& s, i
   }
 }
 
-template <int DP, bool RICH>       // RICH: capped scores or slopes
-__global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
-  constexpr int KC = DP / 16, DB = DP / 32, F_V = 2 * KC, F_SIDE = F_V + 4 * DB, NF = F_SIDE + kSideFrags;
-  __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
+template <int DP, bool CAP, bool SLOPES>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 2) void attend_tiles(TilesArgs A) {
+  constexpr int KC = DP / 16, DB = DP / 32, NV = 4 * DB + kSideFrags;   // LDS: k, k, v and side, v and side
+  __shared__ __align__(16) _Float16 lds[(4 * KC + 2 * NV) * kFrag];
   __shared__ int range[5];
   const AttendDesc& a = A.a;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
@@ -264,19 +264,21 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   const float* qrow = a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t;
   half8 qh[KC], ql[KC];
   const int qe = load_rows<KC>(qrow, valid, a.D, A.wide, qh, ql);
-  const float slope = RICH && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+  const float slope = SLOPES ? a.slopes[head] * kLog2e : 0.0f;
   const int64_t tile0 = (int64_t)slab * tiles;
   const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
   const char* kf = (const char*)(A.kf + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
   const char* vf = (const char*)(A.vf + (tile0 + t0) * (4 * DB * kFrag)) + w * 1024;
   const char* side_p = (const char*)(A.side + (tile0 + t0) * (kSide * kTile)) + w * 1024;
-  auto fetch = [&](int buf) {    // the next tile
-    const uint32_t to = base + buf * (NF * 1024);
-    frags_to_lds<2 * KC>(kf, to, lane16);
+  auto fetch_k = [&](int buf) {    // the next tile of each
+    frags_to_lds<2 * KC>(kf, base + buf * (2 * KC * 1024), lane16);
     kf += 2 * KC * 1024;
-    frags_to_lds<4 * DB>(vf, to + F_V * 1024, lane16);
+  };
+  auto fetch_v = [&](int buf) {
+    const uint32_t to = base + (4 * KC + buf * NV) * 1024;
+    frags_to_lds<4 * DB>(vf, to, lane16);
     vf += 4 * DB * 1024;
-    if (w < kSideFrags) frags_to_lds<4>(side_p, to + F_SIDE * 1024, lane16);
+    if (w < kSideFrags) frags_to_lds<4>(side_p, to + 4 * DB * 1024, lane16);
     side_p += kSide * kTile * 4;
   };
 
@@ -285,34 +287,85 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
   float m = kNone, sum = 0;        // running maximum (log2) and this lane half's sum
   int ce = kUnset;                 // acc is in units of 2^-ce
-  const float icap = RICH && a.cap > 0 ? 1.0f / a.cap : 0.0f;
-  if (t0 < t1) fetch(0);
+  const float icap = CAP ? 1.0f / a.cap : 0.0f;
+  // A tile's scores are computed a tile ahead, while the weights of the tile before are: k runs a tile ahead of v.
+  f32x16 next = {};
+  if (t0 < t1) {
+    fetch_k(0);
+    fetch_v(0);
+    if (t0 + 1 < t1) fetch_k(1);
+    loads_done();
+    __syncthreads();
+    next = scores<KC>(lds, 0, qh, ql);
+  }
+  const float capped = CAP ? a.cap * kLog2e : 0.0f;
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, j0 = t * kTile;
     loads_done();
     __syncthreads();
-    if (t + 1 < t1) fetch(buf ^ 1);
-    const _Float16* L = lds + buf * (NF * kFrag);
-    const float* side = (const float*)(L + F_SIDE * kFrag);
+    if (t + 1 < t1) fetch_v(buf ^ 1);
+    if (t + 2 < t1) fetch_k(buf);
+    const _Float16 *K = lds + (buf ^ 1) * (2 * KC * kFrag), *V = lds + (4 * KC + buf * NV) * kFrag;
+    const float* side = (const float*)(V + 4 * DB * kFrag);
     const TileInfo kt = side_info(side, 0), vt = side_info(side, 1);
-    if (!any_seen(s, me, kt, j0)) continue;
-    // scores, transposed: register r of this lane is key j0 + 8 (r / 4) + 4 h + r % 4
-    f32x16 x = scores<KC>(L, 0, qh, ql);
-    if (kt.uneven) per_row(x, side + KS_RELK * kTile);
+    f32x16 x = next;               // transposed: register r of this lane is key j0 + 8 (r / 4) + 4 h + r % 4
+    if (!any_seen(s, me, kt, j0)) {
+      next = scores<KC>(K, 0, qh, ql);
+      continue;
+    }
     const float unit = a.scale * pow2(-qe) * kt.inv;
-    float f = unit * kLog2e;       // the score is f x, in log2
-    if (RICH) {
-      if (a.cap > 0) {
-        tanh_all(x, unit * icap);
-        f = a.cap * kLog2e;
+    float top = kNone, most = 0;
+    if (CAP)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) most = fmaxf(most, fabsf(x[q]));
+    const float u = CAP ? unit * icap : unit * kLog2e;
+    float change = 1, big;
+    auto grow = [&](float top) {   // the running maximum, and what acc and sum take for it
+      // It moves only when it grows by more than 2^8 (or from nothing), so that most tiles leave acc alone: weights then
+      // reach 2^8 instead of 1.
+      const bool up = top > m + 8 || (m == kNone && top > kNone);
+      const float to = up ? top : m, keep = up ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
+      m = to;
+      sum *= keep;
+      // what acc held has shrunk: so may its unit
+      const int shrunk = up && keep > 0 && ce != kUnset ? min(-exponent(keep) - 1, 100) : 0;
+      change = keep * pow2(shrunk);
+      ce += shrunk;
+    };
+    if (all_seen(s, me, kt, j0) && !kt.uneven && !vt.uneven && (!CAP || !__any(most * u >= kFlat))) {
+      // the common tile, without a branch: the next scores' products between the vector work
+      const float f = SLOPES ? 1.0f : CAP ? capped : u;
+      float part = 0;
+      scores_woven<KC, 32>(next, K, 0, qh, ql, [&](int i) {
+        const int q = i % 16;
+        if (i < 16) {              // scores, and their maximum
+          if (CAP) x[q] = tanh_flat(x[q] * u);
+          if (SLOPES) x[q] = x[q] * (CAP ? capped : u) - slope * fabsf((float)(p - (j0 + 8 * (q / 4) + 4 * h + q % 4)));
+          top = fmaxf(top, x[q]);
+        } else {
+          if (i == 16) {
+            top = halves_max(top) * f;
+            grow(top);
+          }
+          x[q] = __builtin_amdgcn_exp2f(fmaf(x[q], f, -m));
+          part += x[q];
+        }
+      });
+      sum += part;
+      big = __builtin_amdgcn_exp2f(top - m);
+    } else {
+      next = scores<KC>(K, 0, qh, ql);
+      if (kt.uneven) per_row(x, side + KS_RELK * kTile);
+      float f = u;                 // the score is f x, in log2
+      if (CAP) {
+        tanh_all(x, u);
+        f = capped;
       }
-      if (a.slopes) {
+      if (SLOPES) {
 #pragma unroll
         for (int q = 0; q < 16; ++q) x[q] = x[q] * f - slope * fabsf((float)(p - (j0 + 8 * (q / 4) + 4 * h + q % 4)));
         f = 1;
       }
-    }
-    if (!all_seen(s, me, kt, j0)) {
       if (s.doc) {
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
@@ -323,40 +376,27 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
       }
 #pragma unroll
       for (int q = 0; q < 16; ++q) x[q] = j0 + 8 * (q / 4) + 4 * h + q % 4 < below ? x[q] : kNone;
-    }
-    float top = x[0];
+      top = x[0];
 #pragma unroll
-    for (int q = 1; q < 16; ++q) top = fmaxf(top, x[q]);
-    top = halves_max(top) * f;
-    // The maximum moves only when it grows by more than 2^8 (or from nothing), so that most tiles leave acc alone: weights
-    // then reach 2^8 instead of 1.
-    float change = 1;
-    if (top > m + 8 || (m == kNone && top > kNone)) {
-      const float keep = __builtin_amdgcn_exp2f(m - top);
-      m = top;
-      sum *= keep;
-      change = keep;
-      if (ce != kUnset) {          // what acc held has shrunk: so may its unit
-        const int shrunk = keep > 0 ? min(-exponent(keep) - 1, 100) : 0;
-        change *= pow2(shrunk);
-        ce += shrunk;
+      for (int q = 1; q < 16; ++q) top = fmaxf(top, x[q]);
+      top = halves_max(top) * f;
+      grow(top);
+      const float off = m == kNone ? 0.0f : m;
+#pragma unroll
+      for (int q = 0; q < 16; ++q) x[q] = __builtin_amdgcn_exp2f(fmaf(x[q], f, -off));
+      float part = 0;
+#pragma unroll
+      for (int q = 0; q < 16; ++q) part += x[q];
+      sum += part;
+      big = __builtin_amdgcn_exp2f(top - off);
+      if (vt.uneven) {
+        per_row(x, side + KS_RELV * kTile);
+        big = largest(x);
       }
-    }
-    const float off = m == kNone ? 0.0f : m;
-#pragma unroll
-    for (int q = 0; q < 16; ++q) x[q] = __builtin_amdgcn_exp2f(fmaf(x[q], f, -off));
-    float part = 0;
-#pragma unroll
-    for (int q = 0; q < 16; ++q) part += x[q];
-    sum += part;
-    float big = __builtin_amdgcn_exp2f(top - off);
-    if (vt.uneven) {
-      per_row(x, side + KS_RELV * kTile);
-      big = largest(x);
     }
     const int e = fit_unit(ce, big, exponent(vt.scale), &change);
     rescale<DB>(acc, change);
-    accumulate<DB>(acc, x, pow2(e), L, F_V);
+    accumulate<DB>(acc, x, pow2(e), V, 0);
   }
 
   sum = halves_sum(sum);
@@ -580,8 +620,10 @@ Plan plan(const AttendDesc& a) {
 
 template <int DP>
 void run_tiles(const TilesArgs& t, unsigned grid, hipStream_t st) {
-  if (t.a.cap > 0 || t.a.slopes) klaunch(attend_tiles<DP, true>, dim3(grid), dim3(256), 0, st, t);
-  else klaunch(attend_tiles<DP, false>, dim3(grid), dim3(256), 0, st, t);
+  if (t.a.cap > 0 && t.a.slopes) klaunch(attend_tiles<DP, true, true>, dim3(grid), dim3(256), 0, st, t);
+  else if (t.a.cap > 0) klaunch(attend_tiles<DP, true, false>, dim3(grid), dim3(256), 0, st, t);
+  else if (t.a.slopes) klaunch(attend_tiles<DP, false, true>, dim3(grid), dim3(256), 0, st, t);
+  else klaunch(attend_tiles<DP, false, false>, dim3(grid), dim3(256), 0, st, t);
 }
 template <int E, int R>
 void run_few(const FewArgs& f, bool wide, int slabs, hipStream_t st) {
