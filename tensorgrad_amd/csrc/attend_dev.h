@@ -230,7 +230,7 @@ __device__ __forceinline__ int fit_unit(int& c, float big, int t, float* change)
 }
 template <int DB>
 __device__ __forceinline__ void rescale(f32x16 (&acc)[DB], float change) {
-  if (!__any(change != 1)) return;
+  if (__builtin_expect(!__any(change != 1), 1)) return;   // the hint keeps the moves for it out of the common path
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll

@@ -256,7 +256,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 2) void attend_tiles(TilesArgs 
     t0 = min(t0 + split * each, t1);
     t1 = min(t0 + each, t1);
   }
-  if (range_.odd) {
+  if (__builtin_expect(range_.odd, 0)) {
     plain_rows(A, s, split, slab, b, hk, row0, t0 * kTile, t1 * kTile);
     return;
   }
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 2) void attend_tiles(TilesArgs 
     const float* side = (const float*)(V + 4 * DB * kFrag);
     const TileInfo kt = side_info(side, 0), vt = side_info(side, 1);
     f32x16 x = next;               // transposed: register r of this lane is key j0 + 8 (r / 4) + 4 h + r % 4
-    if (!any_seen(s, me, kt, j0)) {
+    if (__builtin_expect(!any_seen(s, me, kt, j0), 0)) {
       next = scores<KC>(K, 0, qh, ql);
       continue;
     }
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 2) void attend_tiles(TilesArgs 
       change = keep * pow2(shrunk);
       ce += shrunk;
     };
-    if (all_seen(s, me, kt, j0) && !kt.uneven && !vt.uneven && (!CAP || !__any(most * u >= kFlat))) {
+    if (__builtin_expect(all_seen(s, me, kt, j0) && !kt.uneven && !vt.uneven && (!CAP || !__any(most * u >= kFlat)), 1)) {
       // the common tile, without a branch: the next scores' products between the vector work
       const float f = SLOPES ? 1.0f : CAP ? capped : u;
       float part = 0;

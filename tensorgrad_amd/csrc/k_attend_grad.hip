@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
   if (!part_rows(A, s, k0, split, from, to)) return;   // nothing, and the join knows
   const Range range_ = tile_range(s, from, to, gi, qi, gi, mine.dmin, mine.dmax, range);
   const int t0 = range_.t0, t1 = range_.t1;
-  if (range_.odd) {
+  if (__builtin_expect(range_.odd, 0)) {
     plain_keys(A, s, split, slab, b, hk, j0, t0 * kTile, t1 * kTile);
     return;
   }
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
     rows.dmin = gt.dmin;
     rows.dmax = gt.dmax;
     rows.same = gt.same;
-    if (j0 >= a.Tk || !any_seen(s, rows, mine, j0)) continue;
+    if (__builtin_expect(j0 >= a.Tk || !any_seen(s, rows, mine, j0), 0)) continue;
     // register r: row r0 + 8 (r / 4) + 4 h + r % 4
     f32x16 x, y, slack;
     if constexpr (DP > 64) {
@@ -174,8 +174,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
       x = scores<KC>(L, 0, kh, kl);
       y = scores<KC>(L, F_GR, vh, vl);
     }
-    if (qt.uneven) per_row(x, side + QS_RELQ * kTile);
-    if (gt.uneven) per_row(y, side + QS_RELG * kTile);
+    if (__builtin_expect(qt.uneven, 0)) per_row(x, side + QS_RELQ * kTile);
+    if (__builtin_expect(gt.uneven, 0)) per_row(y, side + QS_RELG * kTile);
     const float unit = a.scale * pow2(-ke) * qt.inv, yunit = pow2(-ve) * gt.inv;
     float f = unit * kLog2e;
     if (RICH && a.cap > 0) {
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
         x[q] = p;
         y[q] = ds;
       }
-      if (!all) {
+      if (__builtin_expect(!all, 0)) {
         const f32x4 below = *(const f32x4*)(side + QS_BELOW * kTile + at), rdoc = *(const f32x4*)(side + QS_DOC * kTile + at);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -214,12 +214,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
         }
       }
     }
-    if (gt.uneven) per_row(x, side + QS_RELG * kTile);
+    if (__builtin_expect(gt.uneven, 0)) per_row(x, side + QS_RELG * kTile);
     float change = 1;
     int e = fit_unit(cv, largest(x), exponent(gt.scale), &change);
     rescale<DB>(dv, change);
     accumulate<DB>(dv, x, pow2(e), L, F_GC);
-    if (qt.uneven) per_row(y, side + QS_RELQ * kTile);
+    if (__builtin_expect(qt.uneven, 0)) per_row(y, side + QS_RELQ * kTile);
     change = 1;
     e = fit_unit(ck, largest(y), exponent(qt.scale), &change);
     rescale<DB>(dk, change);
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
   if (s.positional && last < 0) end = 0;
   const Range range_ = tile_range(s, 0, (end + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax, range);
   const int t0 = range_.t0, t1 = range_.t1;
-  if (range_.odd) {
+  if (__builtin_expect(range_.odd, 0)) {
     plain_dq(A, s, slab, b, hk, row0, t0 * kTile, t1 * kTile);
     return;
   }
@@ -366,7 +366,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
     const _Float16* L = lds + buf * (NF * kFrag);
     const float* side = (const float*)(L + F_SIDE * kFrag);
     const TileInfo kt = side_info(side, 0), vt = side_info(side, 1);
-    if (!any_seen(s, me, kt, j0)) continue;
+    if (__builtin_expect(!any_seen(s, me, kt, j0), 0)) continue;
     f32x16 x, y;
     if constexpr (DP > 64) {
       scores2<KC>(L, 0, qh, ql, x, F_V, gh, gl, y);
@@ -374,8 +374,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
       x = scores<KC>(L, 0, qh, ql);
       y = scores<KC>(L, F_V, gh, gl);
     }
-    if (kt.uneven) per_row(x, side + KS_RELK * kTile);
-    if (vt.uneven) per_row(y, side + KS_RELV * kTile);
+    if (__builtin_expect(kt.uneven, 0)) per_row(x, side + KS_RELK * kTile);
+    if (__builtin_expect(vt.uneven, 0)) per_row(y, side + KS_RELV * kTile);
     const float unit = a.scale * pow2(-qe) * kt.inv, yunit = pow2(-ge) * vt.inv;
     const bool cap = RICH && a.cap > 0;
     if (cap) tanh_all(x, unit * icap);
@@ -387,7 +387,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
       y[q] = __builtin_amdgcn_exp2f(fmaf(x[q], f, -off)) * fmaf(y[q], yunit, -dot);
       if (cap) y[q] *= fmaf(-x[q], x[q], 1.0f);
     }
-    if (!all_seen(s, me, kt, j0)) {
+    if (__builtin_expect(!all_seen(s, me, kt, j0), 0)) {
       if (s.doc) {
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
 #pragma unroll
       for (int q = 0; q < 16; ++q) y[q] = j0 + 8 * (q / 4) + 4 * h + q % 4 < below ? y[q] : 0.0f;
     }
-    if (kt.uneven) per_row(y, side + KS_RELK * kTile);
+    if (__builtin_expect(kt.uneven, 0)) per_row(y, side + KS_RELK * kTile);
     float change = 1;
     const int e = fit_unit(cq, largest(y), exponent(kt.scale), &change);
     rescale<DB>(dq, change);
