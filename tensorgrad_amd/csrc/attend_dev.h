@@ -503,12 +503,12 @@ struct PackJob {
 // The attention's operands as packed for one pass, in the workspace.
 struct Packs {
   int n;
-  int Hk;
+  int Hk, tiles;                   // tiles: the most of any job
   bool wide;                       // every operand's rows are 16-byte aligned and whole 16-byte pieces
   PackJob job[4];
   AttendDesc a;
 };
-void attend_pack(const Packs& p, int DP, hipStream_t st);
+void attend_pack(Packs p, int DP, hipStream_t st);
 // Blocks for `items` of each slab: those of place() beyond the last item end at once.
 inline unsigned place_grid(int64_t slabs, int64_t items) {
   return (unsigned)(slabs % 8 != 0 && 8 % slabs == 0 ? (items + 8 / slabs - 1) / (8 / slabs) * 8 : slabs * items);

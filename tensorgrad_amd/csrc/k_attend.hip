@@ -1,12 +1,12 @@
 // Masked attention for gfx950: y = softmax(scores) v, one pass over the keys with a running maximum and sum, so that no
-// score reaches memory. Three kernels, by the number of query rows that share a key head (G query heads times Tq):
-//  * many rows: k and v are packed once into f16 hi / lo fragments (attend_pack), then blocks of 4 wavefronts with 32 rows
+// score reaches memory. Two ways, by the number of query rows that share a key head (G query heads times Tq):
+//  * many rows: k and v are packed once into f16 hi / lo fragments (pack_tiles), then blocks of 4 wavefronts with 32 rows
 //    each walk the visible key tiles (attend_tiles). Scores are computed transposed (keys x queries), so that a lane holds
 //    half the keys of ONE query: maximum and sum are lane arithmetic and one exchange between lane halves, and the
 //    probabilities are the next product's B fragment as they stand;
 //  * few rows (one new token against a cache): the keys are read once, in f32, by all heads that share them (attend_few);
 //    bound by memory, so split over the keys until the card is full.
-// Both split a long key axis when there are few rows, and join the parts (attend_join).
+// Both split a long key axis when there are few rows, and join the parts in their order (attend_join).
 #include "attend_dev.h"
 
 namespace tgk {
@@ -22,8 +22,8 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
   __shared__ float x[kTile * LD];
   __shared__ float top[kTile], own[kTile];
   __shared__ int doc[kTile];
-  const PackJob j = p.job[blockIdx.z];
-  const int tile = blockIdx.x, slab = blockIdx.y, b = slab / p.Hk, hk = slab % p.Hk;
+  const PackJob j = p.job[blockIdx.y];
+  const int tile = blockIdx.x % p.tiles, slab = blockIdx.x / p.tiles, b = slab / p.Hk, hk = slab % p.Hk;
   if (tile >= j.tiles) return;
   const Sight s = sight(p.a, b);
   const int tid = threadIdx.x, row = tid / 8, sub = tid % 8, r = tile * kTile + row;
@@ -202,7 +202,7 @@ __device__ __forceinline__ void plain_rows(const TilesArgs& A, const Sight& s, i
 }
 
 template <int DP, bool CAP, bool SLOPES>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 2) void attend_tiles(TilesArgs A) {
+__global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   constexpr int KC = DP / 16, DB = DP / 32, NV = 4 * DB + kSideFrags;   // LDS: k, k, v and side, v and side
   __shared__ __align__(16) _Float16 lds[(4 * KC + 2 * NV) * kFrag];
   __shared__ int range[5];
@@ -211,11 +211,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 2) void attend_tiles(TilesArgs 
   int slab, item;
   place(blockIdx.x, a.B * a.Hk, slab, item);
   if (item >= A.blocks * A.splits) return;
-  // The last rows see the most keys: first. Where all blocks run at once, two on a CU, the second half goes the other way, so
-  // that a CU's two are a long and a short one.
-  const int all = A.blocks * A.splits, half = all / 2;
-  if (gridDim.x <= 512 && item >= half) item = all - 1 - (item - half);
-  const int split = item % A.splits, blk = A.blocks - 1 - item / A.splits;
+  const int split = item % A.splits, blk = A.blocks - 1 - item / A.splits;   // the last rows see the most keys: first
   const int b = slab / a.Hk, hk = slab % a.Hk, G = (int)A.group.d;
   const Sight s = sight(a, b);
   const int tiles = (a.Tk + kTile - 1) / kTile;
@@ -411,7 +407,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 2) void attend_tiles(TilesArgs 
 
 struct FewArgs {
   AttendDesc a;
-  int M, splits;
+  int M, splits, each;             // keys of a part
   float *part, *plse;
 };
 
@@ -422,7 +418,7 @@ template <int E, int R, bool WIDE>
 __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
   const AttendDesc& a = A.a;
   const int tid = threadIdx.x, sub = tid & 7, grp = tid >> 3;
-  const int split = blockIdx.x, slab = blockIdx.y, b = slab / a.Hk, hk = slab % a.Hk, G = a.H / a.Hk;
+  const int split = blockIdx.x % A.splits, slab = blockIdx.x / A.splits, b = slab / a.Hk, hk = slab % a.Hk, G = a.H / a.Hk;
   const Sight s = sight(a, b);
   auto feature = [&](int e) { return WIDE ? 4 * (sub + 8 * (e / 4)) + e % 4 : sub + 8 * e; };
   auto load = [&](const float* row, int n, float (&x)[E]) {
@@ -457,8 +453,7 @@ __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
   int n = s.n;
   if (s.causal) n = min(n, max(pmax + 1, s.prefix));
   if (s.positional && pmax < 0) n = 0;
-  const int each = ((n + A.splits - 1) / A.splits + 31) / 32 * 32;
-  const int begin = min((int64_t)split * each, (int64_t)n), end = min(begin + each, n);
+  const int begin = min((int64_t)split * A.each, (int64_t)n), end = min((int64_t)begin + A.each, (int64_t)n);
   const float* k = a.k.p + b * a.k.b + hk * a.k.h;
   const float* v = a.v.p + b * a.v.b + hk * a.v.h;
   float kn[E], vn[E];
@@ -507,71 +502,129 @@ __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
       for (int e = 0; e < E; ++e) acc[r][e] = fmaf(w, vx[e], acc[r][e]);
     }
   }
-  // the block's 32 groups, row by row
-  __shared__ float sm[32], ss[32], sa[32][8 * E + 1];
-  for (int r = 0; r < min(R, A.M); ++r) {
-    float mr = 0, sr = 0;
+  // the eight groups of a wavefront, then the four wavefronts
 #pragma unroll
-    for (int z = 0; z < R; ++z) if (z == r) { mr = m[z]; sr = sum[z]; }
-    if (sub == 0) { sm[grp] = mr; ss[grp] = sr; }
+  for (int o = 8; o < 64; o *= 2)
 #pragma unroll
-    for (int z = 0; z < R; ++z)
-      if (z == r)
+    for (int r = 0; r < R; ++r) {
+      const float other = __shfl_xor(m[r], o), top = fmaxf(m[r], other);
+      const float here = top == kNone ? 0.0f : __builtin_amdgcn_exp2f(m[r] - top), there = top == kNone ? 0.0f : __builtin_amdgcn_exp2f(other - top);
+      m[r] = top;
+      sum[r] = fmaf(__shfl_xor(sum[r], o), there, sum[r] * here);
 #pragma unroll
-        for (int e = 0; e < E; ++e) sa[grp][feature(e)] = acc[z][e];
-    __syncthreads();
-    float top = kNone, all = 0;
-    for (int z = 0; z < 32; ++z) top = fmaxf(top, sm[z]);
-    const int i = r / G, head = hk * G + r % G;
-    if (top != kNone) for (int z = 0; z < 32; ++z) all += ss[z] * __builtin_amdgcn_exp2f(sm[z] - top);
-    if (tid < a.Dv) {
-      float o = 0;
-      if (top != kNone) {
-        for (int z = 0; z < 32; ++z) if (sm[z] != kNone) o = fmaf(sa[z][tid], __builtin_amdgcn_exp2f(sm[z] - top), o);
-        o /= all;
-      }
-      if (A.splits > 1) A.part[(((int64_t)split * a.B * a.Hk + slab) * A.M + r) * a.Dv + tid] = o;
-      else if (a.y.p) a.y.p[b * a.y.b + head * a.y.h + i * a.y.t + tid] = o;
+      for (int e = 0; e < E; ++e) acc[r][e] = fmaf(__shfl_xor(acc[r][e], o), there, acc[r][e] * here);
     }
-    if (tid == 0) {
+  __shared__ float sm[4][R], ss[4][R], sa[4][R][8 * E];
+  if (grp % 8 == 0) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (sub == 0) {
+        sm[grp / 8][r] = m[r];
+        ss[grp / 8][r] = sum[r];
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) sa[grp / 8][r][feature(e)] = acc[r][e];
+    }
+  }
+  __syncthreads();
+  for (int z = tid; z < min(R, A.M) * (8 * E); z += 256) {
+    const int r = z / (8 * E), d = z % (8 * E), i = r / G, head = hk * G + r % G;
+    float top = kNone, all = 0, o = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) top = fmaxf(top, sm[u][r]);
+    if (top != kNone) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float f = __builtin_amdgcn_exp2f(sm[u][r] - top);
+        all = fmaf(ss[u][r], f, all);
+        o = fmaf(sa[u][r][d], f, o);
+      }
+      o /= all;
+    }
+    const int64_t at = ((int64_t)split * a.B * a.Hk + slab) * A.M + r;
+    if (d < a.Dv) {
+      if (A.splits > 1) A.part[at * a.Dv + d] = o;
+      else if (a.y.p) a.y.p[b * a.y.b + head * a.y.h + i * a.y.t + d] = o;
+    }
+    if (d == 0) {
       const float lse = top == kNone ? kNone : top + __builtin_amdgcn_logf(all);
-      if (A.splits > 1) A.plse[((int64_t)split * a.B * a.Hk + slab) * A.M + r] = lse;
+      if (A.splits > 1) A.plse[at] = lse;
       else if (a.lse) a.lse[((int64_t)b * a.H + head) * a.Tq + i] = top == kNone ? INFINITY : lse;
     }
-    __syncthreads();
   }
 }
 
 // ---- joining the parts ---------------------------------------------------------------------------
+
+// One round of the card: 512 blocks of attend_few read 8 sequences of up to 16000 keys (4 heads of 128, 16 query heads) in
+// 66 us, 1024 in 74, 2048 in 83, and 256 leave compute units idle (89).
+constexpr int kMostParts = 512;
+constexpr int kJoinFew = 16;       // parts of a row that 32 threads join
 
 struct JoinArgs {
   AttendDesc a;
   int M, splits;
   const float *part, *plse;
 };
-__global__ __launch_bounds__(128) void attend_join(JoinArgs A) {
+// L threads join a row: its weights first, then every 32 threads an L / 32nd of the parts. 32 threads take a row with few
+// parts and a block one with many (a long cache read by one token).
+template <int L>
+__global__ __launch_bounds__(256) void attend_join(JoinArgs A) {
+  constexpr int W = L < 64 ? L : 64, P = L / 32, PER = 256 / L;
   const AttendDesc& a = A.a;
-  const int r = blockIdx.x, slab = blockIdx.y, b = slab / a.Hk, hk = slab % a.Hk, G = a.H / a.Hk;
-  const int i = r / G, head = hk * G + r % G, tid = threadIdx.x;
-  const int64_t at = (int64_t)slab * A.M + r, step = (int64_t)a.B * a.Hk * A.M;
-  float top = kNone, all = 0, o = 0;
-  for (int z = 0; z < A.splits; ++z) top = fmaxf(top, A.plse[at + z * step]);
-  if (top != kNone)
-    for (int z = 0; z < A.splits; ++z) {
-      const float e = A.plse[at + z * step];
-      if (e == kNone) continue;
-      const float w = __builtin_amdgcn_exp2f(e - top);
-      all += w;
-      if (tid < a.Dv) o = fmaf(w, A.part[(at + z * step) * a.Dv + tid], o);
+  __shared__ float weight[PER * (L == 256 ? kMostParts : kJoinFew)];
+  __shared__ f32x4 sums[P > 1 ? 256 : 1];
+  const int tid = threadIdx.x, own = tid / L, t = tid % L, unit = t % 32, d = 4 * unit;
+  const int64_t rows = (int64_t)a.B * a.Hk * A.M, row = (int64_t)blockIdx.x * PER + own, at = min(row, rows - 1);
+  const int r = (int)(at % A.M), slab = (int)(at / A.M), b = slab / a.Hk, hk = slab % a.Hk, G = a.H / a.Hk;
+  const int i = r / G, head = hk * G + r % G;
+  float top = kNone, all = 0;
+  for (int z = t % W; z < A.splits; z += W) top = fmaxf(top, A.plse[at + z * rows]);
+#pragma unroll
+  for (int o = 1; o < W; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+  for (int z = t % W; z < A.splits; z += W) {
+    const float e = A.plse[at + z * rows], w = e == kNone ? 0.0f : __builtin_amdgcn_exp2f(e - top);
+    if (t < W) weight[own * A.splits + z] = w;
+    all += w;
+  }
+#pragma unroll
+  for (int o = 1; o < W; o *= 2) all += __shfl_xor(all, o);
+  __syncthreads();
+  f32x4 x = {};
+  const float* part = A.part + at * a.Dv + d;
+#pragma unroll 4
+  for (int z = t / 32; z < A.splits; z += P) {
+    const float w = weight[own * A.splits + z];
+    f32x4 u = {};
+    if (a.Dv % 4 == 0) {
+      if (d < a.Dv) u = *(const f32x4*)(part + z * rows * a.Dv);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) if (d + q < a.Dv) u[q] = part[z * rows * a.Dv + q];
     }
-  if (a.y.p && tid < a.Dv) a.y.p[b * a.y.b + head * a.y.h + (int64_t)i * a.y.t + tid] = top == kNone ? 0.0f : o / all;
-  if (a.lse && tid == 0) a.lse[((int64_t)b * a.H + head) * a.Tq + i] = top == kNone ? INFINITY : top + __builtin_amdgcn_logf(all);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = fmaf(w, u[q], x[q]);
+  }
+  if constexpr (P > 1) {
+    sums[tid] = x;
+    __syncthreads();
+    if (tid >= 32) return;
+#pragma unroll
+    for (int z = 1; z < P; ++z) x += sums[32 * z + tid];
+  }
+  if (row >= rows) return;
+  if (a.y.p) {
+    float* y = a.y.p + b * a.y.b + head * a.y.h + (int64_t)i * a.y.t + d;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) if (d + q < a.Dv) y[q] = top == kNone ? 0.0f : x[q] / all;
+  }
+  if (a.lse && t == 0) a.lse[((int64_t)b * a.H + head) * a.Tq + i] = top == kNone ? INFINITY : top + __builtin_amdgcn_logf(all);
 }
 
 // ---- plans -----------------------------------------------------------------------------------------
 
 struct Plan {
-  int DP, M, G, tiles, blocks, splits, slabs;
+  int DP, M, G, tiles, blocks, splits, slabs, each;
   bool few;
   int64_t kf, vf, ki, vi, side, part, plse, bytes;   // byte offsets into the workspace
 };
@@ -594,12 +647,13 @@ Plan plan(const AttendDesc& a) {
   p.few = p.M <= few_rows(p.DP) && (p.M <= 2 || a.Tk >= 32 * p.M);
   if (p.few) {
     p.blocks = 1;
-    const int64_t want = (2048 + p.slabs - 1) / p.slabs, most = (a.Tk + 127) / 128;
-    p.splits = (int)std::max<int64_t>(1, std::min(want, most));
+    const int64_t want = std::max<int64_t>(1, kMostParts / p.slabs);
+    p.each = (int)std::max<int64_t>(128, ((a.Tk + want - 1) / want + 31) / 32 * 32);
+    p.splits = std::max(1, (a.Tk - 1) / p.each + 1);
   } else {
     p.blocks = (p.M + 127) / 128;
     const int64_t have = (int64_t)p.slabs * p.blocks;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / have, p.tiles / 8));
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kMostParts / have, p.tiles / 8));
   }
   int64_t at = 0;
   if (!p.few) {
@@ -627,8 +681,8 @@ void run_tiles(const TilesArgs& t, unsigned grid, hipStream_t st) {
 }
 template <int E, int R>
 void run_few(const FewArgs& f, bool wide, int slabs, hipStream_t st) {
-  if (wide) klaunch(attend_few<E, R, true>, dim3(f.splits, slabs), dim3(256), 0, st, f);
-  else klaunch(attend_few<E, R, false>, dim3(f.splits, slabs), dim3(256), 0, st, f);
+  if (wide) klaunch(attend_few<E, R, true>, dim3(f.splits * slabs), dim3(256), 0, st, f);
+  else klaunch(attend_few<E, R, false>, dim3(f.splits * slabs), dim3(256), 0, st, f);
 }
 template <int E>
 void run_few_rows(const FewArgs& f, bool wide, int slabs, hipStream_t st) {
@@ -643,10 +697,10 @@ void run_few_rows(const FewArgs& f, bool wide, int slabs, hipStream_t st) {
 
 }  // namespace
 
-void attend_pack(const Packs& p, int DP, hipStream_t st) {
-  int tiles = 0;
-  for (int i = 0; i < p.n; ++i) tiles = std::max(tiles, p.job[i].tiles);
-  const dim3 grid(tiles, p.a.B * p.Hk, p.n);
+void attend_pack(Packs p, int DP, hipStream_t st) {
+  p.tiles = 0;
+  for (int i = 0; i < p.n; ++i) p.tiles = std::max(p.tiles, p.job[i].tiles);
+  const dim3 grid((unsigned)p.tiles * p.a.B * p.Hk, p.n);
   if (DP == 32) klaunch(pack_tiles<32>, grid, dim3(256), 0, st, p);
   else if (DP == 64) klaunch(pack_tiles<64>, grid, dim3(256), 0, st, p);
   else if (DP == 96) klaunch(pack_tiles<96>, grid, dim3(256), 0, st, p);
@@ -662,7 +716,7 @@ void attend(const AttendDesc& a, void* work, hipStream_t st) {
   float* plse = p.splits > 1 ? (float*)(w + p.plse) : nullptr;
   const bool wide = attend_wide(a.q, a.D) && attend_wide(a.k, a.D) && attend_wide(a.v, a.Dv) && (!a.y.p || attend_wide(a.y, a.Dv));
   if (p.few) {
-    const FewArgs f{a, p.M, p.splits, part, plse};
+    const FewArgs f{a, p.M, p.splits, p.each, part, plse};
     if (p.DP == 32) run_few_rows<4>(f, wide, p.slabs, st);
     else if (p.DP == 64) run_few_rows<8>(f, wide, p.slabs, st);
     else if (p.DP == 96) run_few_rows<12>(f, wide, p.slabs, st);
@@ -685,7 +739,12 @@ void attend(const AttendDesc& a, void* work, hipStream_t st) {
     else if (p.DP == 96) run_tiles<96>(t, grid, st);
     else run_tiles<128>(t, grid, st);
   }
-  if (p.splits > 1) klaunch(attend_join, dim3(p.M, p.slabs), dim3(128), 0, st, JoinArgs{a, p.M, p.splits, part, plse});
+  if (p.splits > 1) {
+    const JoinArgs j{a, p.M, p.splits, part, plse};
+    const int64_t rows = (int64_t)p.slabs * p.M;
+    if (p.splits <= kJoinFew) klaunch(attend_join<32>, dim3((rows + 7) / 8), dim3(256), 0, st, j);
+    else klaunch(attend_join<256>, dim3(rows), dim3(256), 0, st, j);
+  }
 }
 
 }  // namespace tgk

@@ -49,6 +49,7 @@ __device__ __forceinline__ float* dv_row(const GradArgs& A, int split, int slab,
 }
 
 // A wavefront's keys [j0, j0 + 32) over query rows [r0, r1) in plain f32.
+template <int WHAT>
 __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, int split, int slab, int b, int hk, int j0, int r0, int r1) {
   const AttendDesc& a = A.g.a;
   const int lane = threadIdx.x & 63, G = (int)A.group.d;
@@ -72,23 +73,28 @@ __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, in
           ds = p * (plain_dot(row(A.g.dy, r), v, a.Dv) - side[QS_DOT * kTile]) * z.slack;
         }
       }
-      plain_add(dv, p, [&](int z) { return row(A.g.dy, min(c + z, A.M - 1)); }, a.Dv);
-      plain_add(dk, ds, [&](int z) { return row(a.q, min(c + z, A.M - 1)); }, a.D);
+      if (WHAT & 2) plain_add(dv, p, [&](int z) { return row(A.g.dy, min(c + z, A.M - 1)); }, a.Dv);
+      if (WHAT & 1) plain_add(dk, ds, [&](int z) { return row(a.q, min(c + z, A.M - 1)); }, a.D);
     }
     float* ok = dk_row(A, split, slab, b, hk, j);
     float* ov = dv_row(A, split, slab, b, hk, j);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      if (ok && 64 * e + lane < a.D) ok[64 * e + lane] = dk[e] * a.scale;
-      if (ov && 64 * e + lane < a.Dv) ov[64 * e + lane] = dv[e];
+      if (WHAT & 1 && ok && 64 * e + lane < a.D) ok[64 * e + lane] = dk[e] * a.scale;
+      if (WHAT & 2 && ov && 64 * e + lane < a.Dv) ov[64 * e + lane] = dv[e];
     }
   }
 }
 
-template <int DP, bool RICH>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs A) {
+// WHAT: 1 for dk, 2 for dv, 3 for both in one walk. Both take the registers of two wavefronts at head sizes above 96: there
+// each has a walk of its own (a quarter more products, but no spilled registers: 0.99 ms instead of 1.05 over 4096 causal
+// rows of 16 heads).
+template <int DP, bool RICH, int WHAT>
+__global__ __launch_bounds__(256, DP <= 64 || WHAT == 2 ? 2 : 1) void attend_grad_kv(GradArgs A) {
   constexpr int KC = DP / 16, DB = DP / 32;
-  constexpr int F_GR = 2 * KC, F_QC = 4 * KC, F_GC = F_QC + 4 * DB, F_SIDE = F_GC + 4 * DB, NF = F_SIDE + kSideFrags;
+  constexpr bool DK = WHAT & 1, DV = WHAT & 2;
+  constexpr int F_GR = 2 * KC, F_QC = F_GR + (DK ? 2 * KC : 0), F_GC = F_QC + (DK ? 4 * DB : 0), F_SIDE = F_GC + (DV ? 4 * DB : 0),
+                NF = F_SIDE + kSideFrags;
   __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
   __shared__ int range[5];
   const AttendDesc& a = A.g.a;
@@ -117,13 +123,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
   const Range range_ = tile_range(s, from, to, gi, qi, gi, mine.dmin, mine.dmax, range);
   const int t0 = range_.t0, t1 = range_.t1;
   if (__builtin_expect(range_.odd, 0)) {
-    plain_keys(A, s, split, slab, b, hk, j0, t0 * kTile, t1 * kTile);
+    plain_keys<WHAT>(A, s, split, slab, b, hk, j0, t0 * kTile, t1 * kTile);
     return;
   }
 
-  half8 kh[KC], kl[KC], vh[KC], vl[KC];
+  half8 kh[KC], kl[KC], vh[DK ? KC : 1], vl[DK ? KC : 1];
   const int ke = load_rows<KC>(a.k.p + b * a.k.b + hk * a.k.h + (int64_t)min(j, a.Tk - 1) * a.k.t, valid, a.D, A.wide, kh, kl);
-  const int ve = load_rows<KC>(a.v.p + b * a.v.b + hk * a.v.h + (int64_t)min(j, a.Tk - 1) * a.v.t, valid, a.Dv, A.wide, vh, vl);
+  int ve = 0;
+  if constexpr (DK) ve = load_rows<KC>(a.v.p + b * a.v.b + hk * a.v.h + (int64_t)min(j, a.Tk - 1) * a.v.t, valid, a.Dv, A.wide, vh, vl);
   const int64_t tile0 = (int64_t)slab * A.qtiles;
   const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
   const char* qr = (const char*)(A.qr + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
@@ -135,12 +142,16 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
     const uint32_t to = base + buf * (NF * 1024);
     frags_to_lds<2 * KC>(qr, to, lane16);
     qr += 2 * KC * 1024;
-    frags_to_lds<2 * KC>(gr, to + F_GR * 1024, lane16);
-    gr += 2 * KC * 1024;
-    frags_to_lds<4 * DB>(qc, to + F_QC * 1024, lane16);
-    qc += 4 * DB * 1024;
-    frags_to_lds<4 * DB>(gc, to + F_GC * 1024, lane16);
-    gc += 4 * DB * 1024;
+    if (DK) {
+      frags_to_lds<2 * KC>(gr, to + F_GR * 1024, lane16);
+      frags_to_lds<4 * DB>(qc, to + F_QC * 1024, lane16);
+      gr += 2 * KC * 1024;
+      qc += 4 * DB * 1024;
+    }
+    if (DV) {
+      frags_to_lds<4 * DB>(gc, to + F_GC * 1024, lane16);
+      gc += 4 * DB * 1024;
+    }
     if (w < kSideFrags) frags_to_lds<4>(side_p, to + F_SIDE * 1024, lane16);
     side_p += kSide * kTile * 4;
   };
@@ -167,22 +178,20 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
     rows.same = gt.same;
     if (__builtin_expect(j0 >= a.Tk || !any_seen(s, rows, mine, j0), 0)) continue;
     // register r: row r0 + 8 (r / 4) + 4 h + r % 4
-    f32x16 x, y, slack;
-    if constexpr (DP > 64) {
+    f32x16 x, y = {};
+    if constexpr (DK && DP > 64) {
       scores2<KC>(L, 0, kh, kl, x, F_GR, vh, vl, y);
     } else {
       x = scores<KC>(L, 0, kh, kl);
-      y = scores<KC>(L, F_GR, vh, vl);
+      if constexpr (DK) y = scores<KC>(L, F_GR, vh, vl);
     }
     if (__builtin_expect(qt.uneven, 0)) per_row(x, side + QS_RELQ * kTile);
-    if (__builtin_expect(gt.uneven, 0)) per_row(y, side + QS_RELG * kTile);
+    if (DK && __builtin_expect(gt.uneven, 0)) per_row(y, side + QS_RELG * kTile);
     const float unit = a.scale * pow2(-ke) * qt.inv, yunit = pow2(-ve) * gt.inv;
     float f = unit * kLog2e;
     if (RICH && a.cap > 0) {
       tanh_all(x, unit * icap);
       f = a.cap * kLog2e;
-#pragma unroll
-      for (int q = 0; q < 16; ++q) slack[q] = fmaf(-x[q], x[q], 1.0f);   // 1 - tanh^2
     }
     const bool all = A.M - r0 >= kTile && all_seen(s, rows, mine, j0);
 #pragma unroll
@@ -199,10 +208,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
       for (int e = 0; e < 4; ++e) {
         const int q = 4 * q4 + e;
         const float p = __builtin_amdgcn_exp2f(fmaf(x[q], f, -off[e]));
-        float ds = p * fmaf(y[q], yunit, -dot[e]);
-        if (RICH && a.cap > 0) ds *= slack[q];
+        if (DK) {
+          y[q] = p * fmaf(y[q], yunit, -dot[e]);
+          if (RICH && a.cap > 0) y[q] *= fmaf(-x[q], x[q], 1.0f);   // 1 - tanh^2
+        }
         x[q] = p;
-        y[q] = ds;
       }
       if (__builtin_expect(!all, 0)) {
         const f32x4 below = *(const f32x4*)(side + QS_BELOW * kTile + at), rdoc = *(const f32x4*)(side + QS_DOC * kTile + at);
@@ -214,44 +224,74 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_kv(GradArgs
         }
       }
     }
-    if (__builtin_expect(gt.uneven, 0)) per_row(x, side + QS_RELG * kTile);
-    float change = 1;
-    int e = fit_unit(cv, largest(x), exponent(gt.scale), &change);
-    rescale<DB>(dv, change);
-    accumulate<DB>(dv, x, pow2(e), L, F_GC);
-    if (__builtin_expect(qt.uneven, 0)) per_row(y, side + QS_RELQ * kTile);
-    change = 1;
-    e = fit_unit(ck, largest(y), exponent(qt.scale), &change);
-    rescale<DB>(dk, change);
-    accumulate<DB>(dk, y, pow2(e), L, F_QC);
+    if (DV) {
+      if (__builtin_expect(gt.uneven, 0)) per_row(x, side + QS_RELG * kTile);
+      float change = 1;
+      const int e = fit_unit(cv, largest(x), exponent(gt.scale), &change);
+      rescale<DB>(dv, change);
+      accumulate<DB>(dv, x, pow2(e), L, F_GC);
+    }
+    if (DK) {
+      if (__builtin_expect(qt.uneven, 0)) per_row(y, side + QS_RELQ * kTile);
+      float change = 1;
+      const int e = fit_unit(ck, largest(y), exponent(qt.scale), &change);
+      rescale<DB>(dk, change);
+      accumulate<DB>(dk, y, pow2(e), L, F_QC);
+    }
   }
 
   if (!valid) return;
   float* ok = dk_row(A, split, slab, b, hk, j);
   float* ov = dv_row(A, split, slab, b, hk, j);
-  if (ok) store_row<DB>(ok, dk, ck, a.scale, a.D, A.splits > 1 ? a.D % 4 == 0 : A.wide);
-  if (ov) store_row<DB>(ov, dv, cv, 1.0f, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide);
+  if (DK && ok) store_row<DB>(ok, dk, ck, a.scale, a.D, A.splits > 1 ? a.D % 4 == 0 : A.wide);
+  if (DV && ov) store_row<DB>(ov, dv, cv, 1.0f, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide);
 }
 
-// The parts of dk and dv in order.
+// The parts of dk and dv in order: a block takes 32 of the 128 keys that the parts were split for.
 __global__ __launch_bounds__(256) void attend_grad_join(GradArgs A) {
   const AttendDesc& a = A.g.a;
   const bool v = blockIdx.y;
   const int n = v ? a.Dv : a.D;
   const Rows& o = v ? A.g.dv : A.g.dk;
-  const float* part = v ? A.pv : A.pk;
   if (!o.p) return;
-  const int64_t all = (int64_t)a.B * a.Hk * a.Tk * n, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= all) return;
-  const int64_t row = at / n;
-  const int d = (int)(at - row * n), j = (int)(row % a.Tk), slab = (int)(row / a.Tk);
-  const Sight s = sight(a, slab / a.Hk);
-  float x = 0;
-  for (int z = 0; z < A.splits; ++z) {
+  const int rows = (a.Tk + 31) / 32, slab = (int)(blockIdx.x / (unsigned)rows), j0 = (int)(blockIdx.x % (unsigned)rows) * 32;
+  const int b = slab / a.Hk, hk = slab % a.Hk;
+  const Sight s = sight(a, b);
+  int first = A.splits, last = -1;   // parts that were written
+  for (int z = threadIdx.x & 63; z < A.splits; z += 64) {
     int from, to;
-    if (part_rows(A, s, j / 128 * 128, z, from, to)) x += part[at + z * all];
+    if (part_rows(A, s, j0 / 128 * 128, z, from, to)) {
+      first = min(first, z);
+      last = max(last, z);
+    }
   }
-  o.p[slab / a.Hk * o.b + slab % a.Hk * o.h + (int64_t)j * o.t + d] = x;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    first = min(first, __shfl_xor(first, o));
+    last = max(last, __shfl_xor(last, o));
+  }
+  const int64_t all = (int64_t)a.B * a.Hk * a.Tk * n;
+  const float* part = (v ? A.pv : A.pk) + ((int64_t)slab * a.Tk + j0) * n;
+  float* y = o.p + b * o.b + hk * o.h + (int64_t)j0 * o.t;
+  const int end = min(32, a.Tk - j0) * n;
+  const bool wide = n % 4 == 0, aligned = A.wide;
+  for (int e = 4 * threadIdx.x; e < end; e += 1024) {
+    f32x4 x = {};
+#pragma unroll 4
+    for (int z = first; z <= last; ++z) {
+      const float* from = part + z * all + e;
+      if (wide) x += *(const f32x4*)from;
+      else
+#pragma unroll
+        for (int q = 0; q < 4; ++q) if (e + q < end) x[q] += from[q];
+    }
+    if (wide && aligned) {
+      *(f32x4*)(y + (int64_t)(e / n) * o.t + e % n) = x;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) if (e + q < end) y[(int64_t)((e + q) / n) * o.t + (e + q) % n] = x[q];
+    }
+  }
 }
 
 // ---- dq --------------------------------------------------------------------------------------------
@@ -426,8 +466,9 @@ GradPlan grad_plan(const AttendGradDesc& g) {
   p.ktiles = (a.Tk + kTile - 1) / kTile;
   p.blocks = (a.Tk + 127) / 128;
   const int64_t have = (int64_t)p.slabs * p.blocks;
-  const int lim = getenv("KV_LIM") ? atoi(getenv("KV_LIM")) : 1024;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((lim + have - 1) / have, p.qtiles / 8));
+  // About 1024 blocks, two to four rounds of the card: 512 leave it to the longest (4096 causal rows of 4 slabs: 1.30 ms
+  // instead of 1.03), 2048 write and join twice the parts (58 us instead of 38).
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((1024 + have - 1) / have, p.qtiles / 8));
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t b = at;
@@ -459,8 +500,15 @@ GradPlan grad_plan(const AttendGradDesc& g) {
 template <int DP, bool RICH>
 void run_grad(const GradArgs& A, int slabs, hipStream_t st) {
   const AttendGradDesc& g = A.g;
-  if (g.dk.p || g.dv.p)
-    klaunch(attend_grad_kv<DP, RICH>, dim3(place_grid(slabs, (int64_t)A.blocks * A.splits)), dim3(256), 0, st, A);
+  const dim3 keys(place_grid(slabs, (int64_t)A.blocks * A.splits));
+  if constexpr (DP <= 96) {
+    if (g.dk.p && g.dv.p) klaunch(attend_grad_kv<DP, RICH, 3>, keys, dim3(256), 0, st, A);
+    else if (g.dk.p) klaunch(attend_grad_kv<DP, RICH, 1>, keys, dim3(256), 0, st, A);
+    else if (g.dv.p) klaunch(attend_grad_kv<DP, RICH, 2>, keys, dim3(256), 0, st, A);
+  } else {
+    if (g.dk.p) klaunch(attend_grad_kv<DP, RICH, 1>, keys, dim3(256), 0, st, A);
+    if (g.dv.p) klaunch(attend_grad_kv<DP, RICH, 2>, keys, dim3(256), 0, st, A);
+  }
   if (g.dq.p)
     klaunch(attend_grad_q<DP, RICH>, dim3(place_grid(slabs, (A.M + 127) / 128)), dim3(256), 0, st, A);
 }
@@ -500,10 +548,8 @@ void attend_grad(const AttendGradDesc& g, void* work, hipStream_t st) {
   else if (p.DP == 64) run_grad<64>(A, p.slabs, st);
   else if (p.DP == 96) run_grad<96>(A, p.slabs, st);
   else run_grad<128>(A, p.slabs, st);
-  if (p.splits > 1 && (g.dk.p || g.dv.p)) {
-    const int64_t most = (int64_t)a.B * a.Hk * a.Tk * std::max(a.D, a.Dv);
-    klaunch(attend_grad_join, dim3((unsigned)((most + 255) / 256), 2), dim3(256), 0, st, A);
-  }
+  if (p.splits > 1 && (g.dk.p || g.dv.p))
+    klaunch(attend_grad_join, dim3((unsigned)((int64_t)p.slabs * ((a.Tk + 31) / 32)), 2), dim3(256), 0, st, A);
 }
 
 }  // namespace tgk

@@ -229,7 +229,7 @@ void rope(const RopeDesc& r, hipStream_t st) {
   for (int i = 0; i < r.n; ++i) R.total += r.heads[i];
   const int64_t threads = (int64_t)r.B * r.T * (r.D - r.half);
   // 2^19 threads fill the card (256 CUs of 32 wavefronts); beyond, a thread takes all heads
-  R.each = (int)std::min<int64_t>(R.total, std::max<int64_t>(1, threads * R.total >> 19));
+  R.each = (int)std::min<int64_t>(R.total, std::max<int64_t>((R.total + 65534) / 65535, threads * R.total >> 19));
   klaunch(rope_pairs, dim3((unsigned)((threads + 255) / 256), (unsigned)((R.total + R.each - 1) / R.each)), dim3(256), 0, st, R);
 }
 

@@ -3727,8 +3727,9 @@ void Runtime::mask_fields(int i, Node& n, tgk::AttendDesc& a) const {
   expect(ks[0] == qs[0] && vs[0] == qs[0] && ks[3] == qs[3] && ks[1] == vs[1] && ks[2] == vs[2] && qs[1] % ks[1] == 0, i,
          "q, k and v do not fit each other");
   expect(qs[3] <= tgk::kAttendMaxHead && vs[3] <= tgk::kAttendMaxHead, i, "head size above 128");
-  const int64_t lim = int64_t(1) << 31;
-  expect(qs[0] * qs[1] * qs[2] < lim && ks[0] * ks[1] * ks[2] < lim, i, "2^31 or more rows");
+  // a launch has fewer than 2^32 threads, 256 of them for 32 rows of a key head
+  const int64_t rows = std::max(qs[1] / ks[1] * qs[2], ks[2]);
+  expect(rows < (int64_t(1) << 31) && qs[0] * ks[1] * ((rows + 31) / 32) < (int64_t(1) << 24), i, "too many rows");
   a.B = (int)qs[0]; a.H = (int)qs[1]; a.Tq = (int)qs[2]; a.D = (int)qs[3];
   a.Hk = (int)ks[1]; a.Tk = (int)ks[2]; a.Dv = (int)vs[3];
   a.causal = op.at("causal").boolean;
@@ -3955,7 +3956,7 @@ void Runtime::lower_scan(int i) {
   n.writes.push_back(root(h));
   n.flops = 2.0 * T_[a].numel;
   n.bytes = 12.0 * T_[a].numel;
-  expect(s[0] * ((s[2] + 63) / 64) * ((s[1] + 15) / 16) < (int64_t(1) << 31), i, "too large");
+  expect(s[0] * ((s[2] + 63) / 64) * ((s[1] + 15) / 16) < (int64_t(1) << 24), i, "too large");
   const int64_t ws = tgk::scan_workspace_bytes(s[0], s[1], s[2]);
   workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
   n.ws = ws > 0;
@@ -3998,7 +3999,7 @@ void Runtime::lower_scan_grad(int i) {
   const int da = out[0], dx = out[1], dh0 = out[2];
   n.flops = 3.0 * T_[a].numel;
   n.bytes = 4.0 * T_[a].numel * (3 + (da >= 0) + (dx >= 0));
-  expect(s[0] * ((s[2] + 63) / 64) * ((s[1] + 15) / 16) < (int64_t(1) << 31), i, "too large");
+  expect(s[0] * ((s[2] + 63) / 64) * ((s[1] + 15) / 16) < (int64_t(1) << 24), i, "too large");
   const int64_t ws = tgk::scan_workspace_bytes(s[0], s[1], s[2]);
   workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
   n.ws = ws > 0;
