@@ -80,9 +80,13 @@ __global__ __launch_bounds__(256) void rope_pairs(RopeArgs R) {
 //    for bit): first those of whole groups of kGroup chunks, which the last block of each group joins and publishes, then
 //    those of its own group;
 //  * then the steps are run again from registers, now with the true state, and stored.
+// Gates above 1 in magnitude can take a product A out of f32's range while no state is (h_in = 0, or a small gate later). A
+// block whose products leave [2^-100, 2^100] that way waits for the true state, runs its steps in order and publishes
+// (0, its state); a group whose product does, likewise. Where all gates are at most 1, A only shrinks, and what is lost below
+// 2^-126 is that part of h_in.
 // A pair is one 64-bit word, stored and loaded whole at device scope; all ones mean "not there yet". A block takes its place
 // from a counter as it starts, and waits only for blocks of lower places: those are running, and publish their own pair
-// before they wait for anything, a group's pair after waiting for lower places only. So every wait ends.
+// after waiting for lower places at most, a group's pair too. So every wait ends.
 
 typedef unsigned long long word;
 constexpr int kGroup = 8;
@@ -96,8 +100,19 @@ __device__ __forceinline__ void publish(word* at, float A, float H) {
   if (v == kEmpty) v = kEmpty - 1;             // a NaN either way
   __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// Whether a product of gates, seen factor by factor, can be used: it must not have left the range upwards, nor downwards
+// where a factor above 1 may have brought it back.
+struct Reach {
+  float most = 1, least = 1, gate = 0;
+  __device__ __forceinline__ void see(float A, float g) {
+    most = fmaxf(most, fabsf(A));
+    least = fminf(least, fabsf(A));
+    gate = fmaxf(gate, fabsf(g));
+  }
+  __device__ __forceinline__ bool out(float A) const { return A != A || (gate > 1 && (most > 0x1p100f || least < 0x1p-100f)); }
+};
 // (A, H) followed by n pairs, `step` words apart, in order. Loads go out together; what is not there yet is asked for again.
-__device__ __forceinline__ void follow(float& A, float& H, const word* at, int64_t step, int n) {
+__device__ __forceinline__ void follow(float& A, float& H, Reach& reach, const word* at, int64_t step, int n) {
   for (int k0 = 0; k0 < n; k0 += kGroup) {
     word v[kGroup];
 #pragma unroll
@@ -111,6 +126,7 @@ __device__ __forceinline__ void follow(float& A, float& H, const word* at, int64
       }
       H = fmaf(gates(v[k]), H, value(v[k]));
       A *= gates(v[k]);
+      reach.see(A, gates(v[k]));
     }
   }
 }
@@ -179,37 +195,81 @@ __global__ __launch_bounds__(256) void scan_chunks(ScanArgs s) {
     }
   }
   float A = 1, H = 0;
+  Reach own;
 #pragma unroll
   for (int k = 0; k < S; ++k) {
     H = fmaf(g[k], H, x[k]);
     A *= g[k];
+    own.see(A, g[k]);
   }
   fold[w][0][lane] = A;
   fold[w][1][lane] = H;
-  __syncthreads();
-  float state = BACK ? 0.0f : h0;
-  if (s.chunks > 1) {
-    if (w == 0) {
-      word* pairs = s.words + (int64_t)cb * 64 + lane;
-      word* groups = pairs + s.chunks * row;
-      const int group = chunk / kGroup, in_group = chunk % kGroup;
-      float a4 = 1, h4 = 0;
+  const bool apart = __syncthreads_or(own.out(A));   // the wavefronts' products cannot be used
+  word* pairs = s.words + (int64_t)cb * 64 + lane;
+  word* groups = pairs + s.chunks * row;
+  const int group = chunk / kGroup, in_group = chunk % kGroup;
+  const bool closes = in_group == kGroup - 1;
+  float state = BACK ? 0.0f : h0, skip = 1;
+  Reach none;
+  if (!apart) {
+    if (s.chunks > 1) {
+      if (w == 0) {
+        float a4 = 1, h4 = 0;
+        Reach reach;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        h4 = fmaf(fold[k][0][lane], h4, fold[k][1][lane]);
-        a4 *= fold[k][0][lane];
+        for (int k = 0; k < 4; ++k) {
+          const float f = fold[k][0][lane];
+          h4 = fmaf(f, h4, fold[k][1][lane]);
+          a4 *= f;
+          reach.see(a4, f);
+        }
+        const bool serial = __any(reach.out(a4));     // nor their product
+        if (!serial) publish(pairs + chunk * row, a4, h4);
+        float ga = 1, gh = 0;
+        follow(ga, gh, reach, pairs + (int64_t)group * kGroup * row, row, in_group);   // the group's chunks before this one
+        reach.see(ga * a4, a4);
+        const bool whole = !__any(reach.out(ga * a4));     // the group's product
+        if (whole && closes) publish(groups + group * row, ga * a4, fmaf(a4, gh, h4));
+        follow(skip, state, none, groups, row, group);
+        if (whole) state = fmaf(ga, state, gh);
+        else follow(skip, state, none, pairs + (int64_t)group * kGroup * row, row, in_group);
+        came[lane] = state;
+        if (!whole) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) state = fmaf(fold[k][0][lane], state, fold[k][1][lane]);
+          if (serial) publish(pairs + chunk * row, 0, state);
+          if (closes) publish(groups + group * row, 0, state);
+        }
       }
-      publish(pairs + chunk * row, a4, h4);
-      float ga = 1, gh = 0, skip = 1;
-      follow(ga, gh, pairs + (int64_t)group * kGroup * row, row, in_group);      // the group's chunks before this one
-      if (in_group == kGroup - 1) publish(groups + group * row, ga * a4, fmaf(a4, gh, h4));
-      follow(skip, state, groups, row, group);
-      came[lane] = fmaf(ga, state, gh);
+      __syncthreads();
+      state = came[lane];
+    }
+    for (int k = 0; k < w; ++k) state = fmaf(fold[k][0][lane], state, fold[k][1][lane]);
+  } else {
+    if (w == 0) {
+      if (s.chunks > 1) {
+        follow(skip, state, none, groups, row, group);
+        follow(skip, state, none, pairs + (int64_t)group * kGroup * row, row, in_group);
+      }
+      came[lane] = state;
+    }
+    float mine = 0;                // the state that comes to this wavefront
+    for (int k = 0; k < 4; ++k) {
+      __syncthreads();
+      if (w == k) {
+        float h = mine = came[lane];
+#pragma unroll
+        for (int e = 0; e < S; ++e) h = fmaf(g[e], h, x[e]);
+        came[lane] = h;
+      }
     }
     __syncthreads();
-    state = came[lane];
+    if (s.chunks > 1 && w == 0) {
+      publish(pairs + chunk * row, 0, came[lane]);
+      if (closes) publish(groups + group * row, 0, came[lane]);
+    }
+    state = mine;
   }
-  for (int k = 0; k < w; ++k) state = fmaf(fold[k][0][lane], state, fold[k][1][lane]);
   if (c >= s.C) return;
 #pragma unroll
   for (int k = 0; k < S; ++k) {

@@ -282,6 +282,56 @@ def test_recurrence_does_not_look_ahead_or_across():
     assert np.isnan(got[1, 400:]).all()
 
 
+def scan_and_gradients(a, x, dh, h0):
+    def fn(i):
+        h = O.linear_recurrence(i['a'], i['x'], i['h0'])
+        return [h, *O.linear_recurrence_grad(i['a'], h, i['dh'], i['h0'])]
+    return dict(zip(('h', 'da', 'dx', 'dh0'), forward(fn, dict(a=a, x=x, dh=dh, h0=h0))))
+
+
+@pytest.mark.parametrize('B,T,C,gate,live', [(1, 700, 5, 4, 40), (2, 900, 70, 1024, 6), (4, 2048, 256, 1.5, 100), (4, 2048, 256, 4, 40),
+                                             (1, 60, 3, 1024, 6)])
+def test_recurrence_products_of_gates_beyond_the_range_of_values(B, T, C, gate, live):
+    """Nothing comes in until the last `live` steps: every state is a finite number, though the gates' product is not. In the
+    gradient's direction, dh ends before the first steps."""
+    r = rng(23, T)
+    a = f32(np.full((B, T, C), gate))
+    a[:, :, ::2] *= -1
+    x, dh = (f32(r.standard_normal(a.shape)) for _ in range(2))
+    x[:, :-live] = 0
+    dh[:, live:] = 0
+    h0 = f32(np.zeros((B, C)))
+    got = scan_and_gradients(a, x, dh, h0)
+    want, tol = R.recurrence(a, x, h0, dh)
+    for n in want:
+        R.check(got[n], want[n], tol[n], n)
+
+
+def test_recurrence_that_fades_and_comes_back():
+    """The state falls by 2^112 and rises again, over and over, at borders that no chunk shares."""
+    r = rng(24)
+    a = f32(np.where(np.arange(1000) // 56 % 2 == 0, 0.25, 4.0)[None, :, None] * np.ones((2, 1, 70)))
+    dh, h0 = f32(r.standard_normal(a.shape)), f32(r.standard_normal((2, 70)))
+    got = scan_and_gradients(a, np.zeros_like(a), dh, h0)
+    want, tol = R.recurrence(a, np.zeros_like(a), h0, dh)
+    for n in want:
+        R.check(got[n], want[n], tol[n], n)
+
+
+def test_recurrence_gates_that_are_not_finite():
+    r = rng(25)
+    a, x = f32(r.uniform(0.5, 1, (1, 500, 70))), f32(r.standard_normal((1, 500, 70)))
+    a[0, 333, 3], a[0, 130, 66] = np.inf, np.nan
+    got = forward(lambda i: [O.linear_recurrence(i['a'], i['x'])], dict(a=a, x=x))[0]
+    with np.errstate(all='ignore'):
+        want, tol = R.recurrence(a, x)
+    assert np.isinf(got[0, 333:, 3]).all() and (np.sign(got[0, 333:, 3]) == np.sign(want['h'][0, 333:, 3])).all()
+    assert np.isnan(got[0, 130:, 66]).all()
+    fine = np.isfinite(want['h'])
+    assert (np.isfinite(got) == fine).all()
+    R.check(got[fine], want['h'][fine], tol['h'][fine], 'h')
+
+
 # ---- together, as a model uses them ------------------------------------------------------------------
 
 VOCAB, DIM, HEADS, KV = 29, 32, 4, 2
