@@ -1,4 +1,4 @@
-// Device code shared by the attention kernels (k_attend.hip, k_attend_grad.hip).
+// Device code shared by the attention kernels (k_attend.hip, k_attend_grad.hip, k_attend_small.hip).
 //
 // Products of f32 operands run on the f16 matrix instructions: a value times a power of two that puts its tile's (or row's)
 // largest at 2^14 is split as hi + lo of 11 bits each, and a b = hi hi + hi lo + lo hi, accumulated in f32. The product
@@ -514,6 +514,14 @@ inline unsigned place_grid(int64_t slabs, int64_t items) {
   return (unsigned)(slabs % 8 != 0 && 8 % slabs == 0 ? (items + 8 / slabs - 1) / (8 / slabs) * 8 : slabs * items);
 }
 inline int attend_dp(const AttendDesc& a) { return (max(a.D, a.Dv) + 31) / 32 * 32; }
+// Rows that k_attend_small.hip holds (query rows of a key head, and keys); 0: not for it.
+inline int attend_small_rows(const AttendDesc& a) {
+  const int64_t n = max((int64_t)(a.H / a.Hk) * a.Tq, (int64_t)a.Tk);
+  const int dp = attend_dp(a);
+  return n <= 32 && dp <= 64 ? 32 : n <= 64 && dp <= 32 ? 64 : 0;
+}
+void attend_small_forward(const AttendDesc& a, hipStream_t st);
+void attend_small_grad(const AttendGradDesc& g, hipStream_t st);
 inline bool attend_wide(const Rows& x, int n) {
   return ((uintptr_t)x.p & 15) == 0 && x.b % 4 == 0 && x.h % 4 == 0 && x.t % 4 == 0 && n % 8 == 0;
 }

@@ -6,7 +6,7 @@
 //    probabilities are the next product's B fragment as they stand;
 //  * few rows (one new token against a cache): the keys are read once, in f32, by all heads that share them (attend_few);
 //    bound by memory, so split over the keys until the card is full.
-// Both split a long key axis when there are few rows, and join the parts in their order (attend_join).
+// Both split a long key axis when there are few rows (attend_join). A few dozen positions in all: k_attend_small.hip.
 #include "attend_dev.h"
 
 namespace tgk {
@@ -707,9 +707,10 @@ void attend_pack(Packs p, int DP, hipStream_t st) {
   else klaunch(pack_tiles<128>, grid, dim3(256), 0, st, p);
 }
 
-int64_t attend_workspace_bytes(const AttendDesc& a) { return plan(a).bytes; }
+int64_t attend_workspace_bytes(const AttendDesc& a) { return attend_small_rows(a) ? 0 : plan(a).bytes; }
 
 void attend(const AttendDesc& a, void* work, hipStream_t st) {
+  if (attend_small_rows(a)) return attend_small_forward(a, st);
   const Plan p = plan(a);
   char* w = (char*)work;
   float* part = p.splits > 1 ? (float*)(w + p.part) : nullptr;

@@ -520,9 +520,10 @@ void run_grad(const GradArgs& A, int slabs, hipStream_t st) {
 
 }  // namespace
 
-int64_t attend_grad_workspace_bytes(const AttendGradDesc& g) { return grad_plan(g).bytes; }
+int64_t attend_grad_workspace_bytes(const AttendGradDesc& g) { return attend_small_rows(g.a) ? 0 : grad_plan(g).bytes; }
 
 void attend_grad(const AttendGradDesc& g, void* work, hipStream_t st) {
+  if (attend_small_rows(g.a)) return attend_small_grad(g, st);
   const GradPlan p = grad_plan(g);
   const AttendDesc& a = g.a;
   char* w = (char*)work;
