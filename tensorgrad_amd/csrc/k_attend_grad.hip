@@ -17,23 +17,33 @@ struct GradArgs {
   const TileInfo *qi, *gi, *ki, *vi;
   const float *qside, *kside;
   FastDiv group;
-  int M, qtiles, ktiles, blocks, splits;
+  int M, qtiles, ktiles, blocks, splits, qsplits;     // splits: parts of the query rows; qsplits: parts of the keys
   bool wide;
-  float *pk, *pv;                                     // parts of dk, dv: [split][slab][Tk][D or Dv]
+  float *pk, *pv, *pq;                                // parts: of dk, dv [split][slab][Tk][D or Dv], of dq [qsplit][slab][M][D]
+  int* parts;                                         // with documents: parts of dk and dv that were written, [slab][blocks]
 };
 
 // ---- dk, dv --------------------------------------------------------------------------------------
 
-// Query tiles [from, to) of part `split` that the masks by position let see any of the keys [k0, k0 + 128): parts are equal
-// stretches of the rows. False: none, which the join finds again and does not read.
-__device__ __forceinline__ bool part_rows(const GradArgs& A, const Sight& s, int k0, int split, int& from, int& to) {
+// Query tiles [from, to) that the masks by position let see any of the keys [k0, k0 + 128).
+__device__ __forceinline__ void seeing_tiles(const GradArgs& A, const Sight& s, int k0, int& from, int& to) {
   int64_t i0 = 0;                  // first position index that sees any: a prefix shows its keys to all
   if (s.causal && k0 >= s.prefix) i0 = (int64_t)k0 - s.first;
   if (s.positional) i0 = max(i0, (int64_t)-s.first);
+  from = (int)min(max(i0, (int64_t)0) * A.group.d / kTile, (int64_t)A.qtiles);
+  to = k0 < s.n ? A.qtiles : 0;
+}
+// Those of part `split`, equal stretches of all rows, so that blocks that run together walk the same ones. False: none, which
+// the join finds again and does not read. With documents the stretch that a key block's own see is short: there its tiles are
+// cut into equal parts, of 8 at least, when they are known (8 x 1000 positions, 2 key heads of 64, documents of 50: 53 us
+// instead of 81, of 170: 82 instead of 87; one document: 130 instead of 123).
+__device__ __forceinline__ bool part_rows(const GradArgs& A, const Sight& s, int k0, int split, int& from, int& to) {
+  seeing_tiles(A, s, k0, from, to);
+  if (A.splits == 1 || s.doc) return true;
   const int each = (A.qtiles + A.splits - 1) / A.splits;
-  from = max((int)min(max(i0, (int64_t)0) * A.group.d / kTile, (int64_t)A.qtiles), split * each);
-  to = k0 < s.n ? min((split + 1) * each, A.qtiles) : 0;
-  return from < to || A.splits == 1;
+  from = max(from, split * each);
+  to = min(to, (split + 1) * each);
+  return from < to;
 }
 
 // Where dk and dv of key j go.
@@ -121,7 +131,14 @@ __global__ __launch_bounds__(256, DP <= 64 || WHAT == 2 ? 2 : 1) void attend_gra
   int from, to;
   if (!part_rows(A, s, k0, split, from, to)) return;   // nothing, and the join knows
   const Range range_ = tile_range(s, from, to, gi, qi, gi, mine.dmin, mine.dmax, range);
-  const int t0 = range_.t0, t1 = range_.t1;
+  int t0 = range_.t0, t1 = range_.t1;
+  if (s.doc && A.splits > 1) {
+    const int each = max((t1 - t0 + A.splits - 1) / A.splits, 8);
+    if (split == 0 && tid == 0) A.parts[slab * A.blocks + blk] = each > 0 ? (t1 - t0 + each - 1) / each : 0;
+    t0 += split * each;
+    t1 = min(t0 + each, t1);
+    if (t0 >= t1) return;
+  }
   if (__builtin_expect(range_.odd, 0)) {
     plain_keys<WHAT>(A, s, split, slab, b, hk, j0, t0 * kTile, t1 * kTile);
     return;
@@ -247,33 +264,39 @@ __global__ __launch_bounds__(256, DP <= 64 || WHAT == 2 ? 2 : 1) void attend_gra
   if (DV && ov) store_row<DB>(ov, dv, cv, 1.0f, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide);
 }
 
-// The parts of dk and dv in order: a block takes 32 of the 128 keys that the parts were split for.
+// The parts of dk, dv and dq in order: a block takes 32 keys of the 128 that the parts were split for, or 32 query rows.
 __global__ __launch_bounds__(256) void attend_grad_join(GradArgs A) {
   const AttendDesc& a = A.g.a;
-  const bool v = blockIdx.y;
-  const int n = v ? a.Dv : a.D;
-  const Rows& o = v ? A.g.dv : A.g.dk;
-  if (!o.p) return;
-  const int rows = (a.Tk + 31) / 32, slab = (int)(blockIdx.x / (unsigned)rows), j0 = (int)(blockIdx.x % (unsigned)rows) * 32;
+  const int what = blockIdx.y, n = what == 1 ? a.Dv : a.D, G = what == 2 ? (int)A.group.d : 1, T = what == 2 ? A.M : a.Tk;
+  const Rows& o = what == 0 ? A.g.dk : what == 1 ? A.g.dv : A.g.dq;
+  if (!o.p || (what == 2 ? A.qsplits : A.splits) == 1) return;
+  const int tiles = max(A.ktiles, A.qtiles), slab = (int)(blockIdx.x / (unsigned)tiles), r0 = (int)(blockIdx.x % (unsigned)tiles) * kTile;
+  if (r0 >= T) return;
   const int b = slab / a.Hk, hk = slab % a.Hk;
   const Sight s = sight(a, b);
-  int first = A.splits, last = -1;   // parts that were written
-  for (int z = threadIdx.x & 63; z < A.splits; z += 64) {
-    int from, to;
-    if (part_rows(A, s, j0 / 128 * 128, z, from, to)) {
-      first = min(first, z);
-      last = max(last, z);
+  int first = 0, last = A.qsplits - 1;   // parts that were written
+  if (what < 2 && s.doc) {
+    last = A.parts[slab * A.blocks + r0 / 128] - 1;
+  } else if (what < 2) {
+    first = A.splits;
+    last = -1;
+    for (int z = threadIdx.x & 63; z < A.splits; z += 64) {
+      int from, to;
+      if (part_rows(A, s, r0 / 128 * 128, z, from, to)) {
+        first = min(first, z);
+        last = max(last, z);
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      first = min(first, __shfl_xor(first, o));
+      last = max(last, __shfl_xor(last, o));
     }
   }
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    first = min(first, __shfl_xor(first, o));
-    last = max(last, __shfl_xor(last, o));
-  }
-  const int64_t all = (int64_t)a.B * a.Hk * a.Tk * n;
-  const float* part = (v ? A.pv : A.pk) + ((int64_t)slab * a.Tk + j0) * n;
-  float* y = o.p + b * o.b + hk * o.h + (int64_t)j0 * o.t;
-  const int end = min(32, a.Tk - j0) * n;
+  const int64_t all = (int64_t)a.B * a.Hk * T * n;
+  const float* part = (what == 0 ? A.pk : what == 1 ? A.pv : A.pq) + ((int64_t)slab * T + r0) * n;
+  auto to = [&](int r) { return o.p + b * o.b + (hk * G + r % G) * o.h + (int64_t)(r / G) * o.t; };
+  const int end = min(kTile, T - r0) * n;
   const bool wide = n % 4 == 0, aligned = A.wide;
   for (int e = 4 * threadIdx.x; e < end; e += 1024) {
     f32x4 x = {};
@@ -286,18 +309,23 @@ __global__ __launch_bounds__(256) void attend_grad_join(GradArgs A) {
         for (int q = 0; q < 4; ++q) if (e + q < end) x[q] += from[q];
     }
     if (wide && aligned) {
-      *(f32x4*)(y + (int64_t)(e / n) * o.t + e % n) = x;
+      *(f32x4*)(to(r0 + e / n) + e % n) = x;
     } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) if (e + q < end) y[(int64_t)((e + q) / n) * o.t + (e + q) % n] = x[q];
+      for (int q = 0; q < 4; ++q) if (e + q < end) to(r0 + (e + q) / n)[(e + q) % n] = x[q];
     }
   }
 }
 
 // ---- dq --------------------------------------------------------------------------------------------
 
+// Where dq of row r of a slab goes.
+__device__ __forceinline__ float* dq_row(const GradArgs& A, int split, int slab, int b, int head, int r, int i) {
+  if (A.qsplits > 1) return A.pq + (((int64_t)split * A.g.a.B * A.g.a.Hk + slab) * A.M + r) * A.g.a.D;
+  return A.g.dq.p + b * A.g.dq.b + head * A.g.dq.h + (int64_t)i * A.g.dq.t;
+}
 // A wavefront's rows [row0, row0 + 32) over keys [j0, j1) in plain f32.
-__device__ __forceinline__ void plain_dq(const GradArgs& A, const Sight& s, int slab, int b, int hk, int row0, int j0, int j1) {
+__device__ __forceinline__ void plain_dq(const GradArgs& A, const Sight& s, int split, int slab, int b, int hk, int row0, int j0, int j1) {
   const AttendDesc& a = A.g.a;
   const int lane = threadIdx.x & 63, G = (int)A.group.d;
   const float* k = a.k.p + b * a.k.b + hk * a.k.h;
@@ -321,7 +349,7 @@ __device__ __forceinline__ void plain_dq(const GradArgs& A, const Sight& s, int 
       }
       plain_add(dq, ds, [&](int z) { return k + min(c + z, a.Tk - 1) * a.k.t; }, a.D);
     }
-    float* o = A.g.dq.p + b * A.g.dq.b + head * A.g.dq.h + (int64_t)i * A.g.dq.t;
+    float* o = dq_row(A, split, slab, b, head, r, i);
 #pragma unroll
     for (int e = 0; e < 2; ++e) if (64 * e + lane < a.D) o[64 * e + lane] = dq[e] * a.scale;
   }
@@ -338,8 +366,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
   const int rblocks = (A.M + 127) / 128;
   int slab, item;
   place(blockIdx.x, a.B * a.Hk, slab, item);
-  if (item >= rblocks) return;
-  const int blk = rblocks - 1 - item;
+  if (item >= rblocks * A.qsplits) return;
+  const int split = item % A.qsplits, blk = rblocks - 1 - item / A.qsplits;
   const int b = slab / a.Hk, hk = slab % a.Hk, G = (int)A.group.d;
   const Sight s = sight(a, b);
   const int row0 = blk * 128 + w * kTile, r = row0 + l, rr = min(r, A.M - 1);
@@ -364,9 +392,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
   if (s.causal) end = min(end, max(last + 1, s.prefix));
   if (s.positional && last < 0) end = 0;
   const Range range_ = tile_range(s, 0, (end + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax, range);
-  const int t0 = range_.t0, t1 = range_.t1;
+  int t0 = range_.t0, t1 = range_.t1;
+  if (A.qsplits > 1) {
+    const int each = (t1 - t0 + A.qsplits - 1) / A.qsplits;
+    t0 = min(t0 + split * each, t1);
+    t1 = min(t0 + each, t1);
+  }
   if (__builtin_expect(range_.odd, 0)) {
-    plain_dq(A, s, slab, b, hk, row0, t0 * kTile, t1 * kTile);
+    plain_dq(A, s, split, slab, b, hk, row0, t0 * kTile, t1 * kTile);
     return;
   }
 
@@ -446,14 +479,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attend_grad_q(GradArgs 
     accumulate<DB>(dq, y, pow2(e), L, F_KC);
   }
   if (valid)
-    store_row<DB>(A.g.dq.p + b * A.g.dq.b + head * A.g.dq.h + (int64_t)i * A.g.dq.t, dq, cq, a.scale, a.D, A.wide);
+    store_row<DB>(dq_row(A, split, slab, b, head, r, i), dq, cq, a.scale, a.D, A.qsplits > 1 ? a.D % 4 == 0 : A.wide);
 }
 
 // ---- plan --------------------------------------------------------------------------------------------
 
 struct GradPlan {
-  int DP, M, G, qtiles, ktiles, blocks, splits, slabs;
-  int64_t qr, qc, gr, gc, kr, kc, vr, qi, gi, ki, vi, qside, kside, pk, pv, bytes;
+  int DP, M, G, qtiles, ktiles, blocks, splits, qsplits, slabs;
+  int64_t qr, qc, gr, gc, kr, kc, vr, qi, gi, ki, vi, qside, kside, pk, pv, pq, parts, bytes;
 };
 GradPlan grad_plan(const AttendGradDesc& g) {
   const AttendDesc& a = g.a;
@@ -469,6 +502,8 @@ GradPlan grad_plan(const AttendGradDesc& g) {
   // About 1024 blocks, two to four rounds of the card: 512 leave it to the longest (4096 causal rows of 4 slabs: 1.30 ms
   // instead of 1.03), 2048 write and join twice the parts (58 us instead of 38).
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((1024 + have - 1) / have, p.qtiles / 8));
+  // dq: one round of the card (32 slabs of 777 rows, head size 96: 64 us and 4 more to join, instead of 73; in two rounds 73)
+  p.qsplits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / ((int64_t)p.slabs * ((p.M + 127) / 128)), p.ktiles / 8));
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t b = at;
@@ -492,7 +527,9 @@ GradPlan grad_plan(const AttendGradDesc& g) {
   if (p.splits > 1) {
     p.pk = take((int64_t)p.splits * p.slabs * a.Tk * a.D * 4);
     p.pv = take((int64_t)p.splits * p.slabs * a.Tk * a.Dv * 4);
+    p.parts = take(have * 4);
   }
+  if (p.qsplits > 1) p.pq = take((int64_t)p.qsplits * p.slabs * p.M * a.D * 4);
   p.bytes = at;
   return p;
 }
@@ -510,7 +547,7 @@ void run_grad(const GradArgs& A, int slabs, hipStream_t st) {
     if (g.dv.p) klaunch(attend_grad_kv<DP, RICH, 2>, keys, dim3(256), 0, st, A);
   }
   if (g.dq.p)
-    klaunch(attend_grad_q<DP, RICH>, dim3(place_grid(slabs, (A.M + 127) / 128)), dim3(256), 0, st, A);
+    klaunch(attend_grad_q<DP, RICH>, dim3(place_grid(slabs, (int64_t)((A.M + 127) / 128) * A.qsplits)), dim3(256), 0, st, A);
 }
 template <int DP>
 void run_grad(const GradArgs& A, int slabs, hipStream_t st) {
@@ -544,13 +581,14 @@ void attend_grad(const AttendGradDesc& g, void* work, hipStream_t st) {
   attend_pack(k, p.DP, st);
   const GradArgs A{g, half(p.qr), half(p.qc), half(p.gr), half(p.gc), half(p.kr), half(p.kc), half(p.vr),
                    info(p.qi), info(p.gi), info(p.ki), info(p.vi), qs, ks, make_fastdiv(p.G), p.M, p.qtiles,
-                   p.ktiles, p.blocks, p.splits, wide, (float*)(w + p.pk), (float*)(w + p.pv)};
+                   p.ktiles, p.blocks, p.splits, p.qsplits, wide, (float*)(w + p.pk), (float*)(w + p.pv), (float*)(w + p.pq),
+                   (int*)(w + p.parts)};
   if (p.DP == 32) run_grad<32>(A, p.slabs, st);
   else if (p.DP == 64) run_grad<64>(A, p.slabs, st);
   else if (p.DP == 96) run_grad<96>(A, p.slabs, st);
   else run_grad<128>(A, p.slabs, st);
-  if (p.splits > 1 && (g.dk.p || g.dv.p))
-    klaunch(attend_grad_join, dim3((unsigned)((int64_t)p.slabs * ((a.Tk + 31) / 32)), 2), dim3(256), 0, st, A);
+  if ((p.splits > 1 && (g.dk.p || g.dv.p)) || (p.qsplits > 1 && g.dq.p))
+    klaunch(attend_grad_join, dim3((unsigned)((int64_t)p.slabs * std::max(p.ktiles, p.qtiles)), 3), dim3(256), 0, st, A);
 }
 
 }  // namespace tgk
