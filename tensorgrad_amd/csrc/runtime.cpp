@@ -3734,13 +3734,16 @@ void Runtime::mask_fields(int i, Node& n, tgk::AttendDesc& a) const {
   a.Hk = (int)ks[1]; a.Tk = (int)ks[2]; a.Dv = (int)vs[3];
   a.causal = op.at("causal").boolean;
   const double scale = op.at("scale").num(), cap = op.at("softcap").null() ? 0 : op.at("softcap").num();
-  expect(scale > 0 && std::isfinite(scale) && cap >= 0 && std::isfinite(cap), i, "scale and softcap must be positive");
+  auto fits = [](double x) { return x >= 0x1p-60 && x <= 0x1p60; };
+  expect(fits(scale) && (op.at("softcap").null() || fits(cap)), i, "scale and softcap must be positive, between 2^-60 and 2^60");
   a.scale = (float)scale;
   a.cap = (float)cap;
   const int doc = opt_fld(i, "documents"), pre = opt_fld(i, "prefix"), len = opt_fld(i, "lengths");
   a.positional = a.causal || doc >= 0 || !op.at("slopes").null();
   expect(!a.positional || a.Tq <= a.Tk, i, "more queries than positions");
   expect(op.at("slopes").null() || (int64_t)op.at("slopes").items.size() == a.H, i, "one slope per query head");
+  if (!op.at("slopes").null())
+    for (const auto& x : op.at("slopes").items) expect(std::fabs(x.num()) <= 0x1p60, i, "slopes must be finite, of 2^60 at most");
   const std::pair<int, Dims> masks[] = {{doc, {a.B, a.Tk}}, {pre, {a.B}}, {len, {a.B}}};
   for (const auto& m : masks)
     if (m.first >= 0) {

@@ -545,6 +545,7 @@ def rope(q: Tensor, k: Tensor, base: float = 10000) -> Tuple[Tensor, Tensor]:
 # ---- Sequence operators (no reference counterpart) ---------------------------------------------------
 
 ATTENTION_MAX_HEAD = 128   # the kernels' tiles hold whole heads
+ATTENTION_RANGE = 2.0 ** 60   # of constants that the kernels multiply in f32
 
 
 def _finite(x) -> bool:
@@ -574,14 +575,13 @@ def _attention_fields(site: str, q: Tensor, k: Tensor, v: Tensor, causal, scale,
         raise ShapeError(f'{site}: {Tq} queries are not the last of {Tk} positions', site)
     if scale is None:
         scale = 1 / math.sqrt(D)
-    if not _finite(scale) or scale <= 0:
-        raise ShapeError(f'{site}: scale must be positive, got {scale}', site)
-    if softcap is not None and (not _finite(softcap) or softcap <= 0):
-        raise ShapeError(f'{site}: softcap must be positive, got {softcap}', site)
+    for name, x in (('scale', scale), ('softcap', softcap)):
+        if x is not None and (not _finite(x) or not 1 / ATTENTION_RANGE <= x <= ATTENTION_RANGE):
+            raise ShapeError(f'{site}: {name} must be positive, between 2^-60 and 2^60, got {x}', site)
     if slopes is not None:
-        slopes = [float(x) for x in slopes] if all(_finite(x) for x in slopes) else None
+        slopes = [float(x) for x in slopes] if all(_finite(x) and abs(x) <= ATTENTION_RANGE for x in slopes) else None
         if slopes is None or len(slopes) != H:
-            raise ShapeError(f'{site}: slopes must be {H} finite numbers, one per query head', site)
+            raise ShapeError(f'{site}: slopes must be {H} finite numbers, one per query head, of 2^60 at most', site)
     if prefix is not None and not causal:
         raise ShapeError(f'{site}: a prefix needs a causal mask', site)
     for name, t, shape in (('documents', documents, (B, Tk)), ('prefix', prefix, (B,)), ('lengths', lengths, (B,))):

@@ -210,6 +210,84 @@ def test_attention_is_deterministic():
     assert all(np.array_equal(a[n], b[n]) for n in a)
 
 
+@pytest.mark.parametrize('T,D', [(30, 16), (150, 64), (600, 128)])
+@pytest.mark.parametrize('what', ['q', 'k', 'v', 'dy', 'all'])
+def test_rows_of_very_different_size(T, D, what):
+    """Neighbouring rows apart by up to 2^24 (2^48 in the products): each keeps its own precision."""
+    x = dict(zip(('q', 'k', 'v', 'dy'), qkv(1, 2, 1, T, T, D, D, 13)))
+    r = rng(14, T)
+    for n in x if what == 'all' else (what,):
+        x[n] = f32(x[n] * 2.0 ** r.integers(-24, 1, (1, x[n].shape[1], T, 1)))
+    check_attention(*x.values(), dict(softcap=30.0), {}, what)
+
+
+@pytest.mark.parametrize('Tq,Tk,D', [(20, 5, 16), (130, 33, 64), (700, 300, 128), (3, 1, 8)])
+def test_more_queries_than_keys(Tq, Tk, D):
+    """Without positions; the second entry's keys are none."""
+    q, k, v, dy = qkv(3, 4, 2, Tq, Tk, D, D, 15)
+    check_attention(q, k, v, dy, dict(causal=False), {})
+    check_attention(q, k, v, dy, dict(causal=False, softcap=2.0), dict(lengths=np.array([Tk, 0, Tk // 2], np.int32)))
+
+
+@pytest.mark.parametrize('T,D,kind', [(1300, 40, 'documents'), (1100, 96, 'prefix'), (900, 128, 'all'), (1500, 16, 'one document')])
+def test_long_rows_in_parts(T, D, kind):
+    """Three query heads a key head and walks that are cut into parts, forward and backward; the same bits twice."""
+    q, k, v, dy = qkv(1, 3, 1, T, T, D, D, 16)
+    r, masks = rng(T, 17), {}
+    if kind in ('documents', 'all'):
+        masks['documents'] = np.sort(r.integers(0, 5, (1, T), dtype=np.int32), 1)
+        masks['documents'][:, T - 37:] = -1
+    if kind == 'one document':
+        masks['documents'] = np.zeros((1, T), np.int32)
+    if kind in ('prefix', 'all'):
+        masks['prefix'] = np.array([T // 3], np.int32)
+    if kind == 'all':
+        masks['lengths'] = np.array([T - 100], np.int32)
+    a = check_attention(q, k, v, dy, {}, masks, kind)
+    b = attend(q, k, v, dy, {}, masks)
+    assert all(np.array_equal(a[n], b[n]) for n in a)
+
+
+@pytest.mark.parametrize('bad', [np.nan, np.inf, 3.4e38])
+@pytest.mark.parametrize('T,D', [(48, 16), (600, 64), (600, 128)])
+def test_gradients_beside_a_document_of_garbage(bad, T, D):
+    """Of three documents the middle one is not finite: the gradients of the others are as without it."""
+    q, k, v, dy = qkv(1, 2, 1, T, T, D, D, 18)
+    doc = np.repeat(np.array([[0, 1, 2]], np.int32), T // 3, 1)
+    mid, rest = slice(T // 3, 2 * T // 3), np.r_[0:T // 3, 2 * T // 3:T]
+    want, tol = R.attention(q, k, v, dy, documents=doc)
+    for x in (q, k, v, dy):
+        x[:, :, mid] = bad
+    got = attend(q, k, v, dy, {}, dict(documents=doc))
+    for n in want:
+        R.check(got[n][:, :, rest], want[n][:, :, rest], tol[n][:, :, rest], n)
+
+
+@pytest.mark.parametrize('T,D', [(24, 16), (200, 64)])
+def test_one_tensor_in_every_place_and_gradients_asked_twice(T, D):
+    x, dy = f32(rng(19, T).standard_normal((2, 2, T, D))), f32(rng(20, T).standard_normal((2, 2, T, D)))
+
+    def fn(i):
+        y = O.attention(i['x'], i['x'], i['x'])
+        return [y, *O.attention_grad(i['x'], i['x'], i['x'], y, i['dy']), *O.attention_grad(i['x'], i['x'], i['x'], y, i['dy'])]
+    got = forward(fn, dict(x=x, dy=dy))
+    want, tol = R.attention(x, x, x, dy)
+    for n, g in zip(('y', 'dq', 'dk', 'dv', 'dq', 'dk', 'dv'), got):
+        R.check(g, want[n], tol[n], n)
+
+
+@pytest.mark.parametrize('T', [3, 70])
+def test_more_key_heads_than_a_grid_axis_holds(T):
+    """70000 key heads, forward: of a few positions, and one token against a longer cache."""
+    B, Tq = 70000, 3 if T == 3 else 1
+    q, k, v, dy = qkv(B, 1, 1, Tq, T, 4, 4, 21)
+    y = attend(q, k, v)['y']
+    pick = np.r_[0:20, 65530:65545, B - 20:B]
+    want, tol = R.attention(q[pick], k[pick], v[pick])
+    R.check(y[pick], want['y'], tol['y'])
+    assert np.isfinite(y).all()
+
+
 # ---- rotary positions -----------------------------------------------------------------------------
 
 @pytest.mark.parametrize('B,H,Hk,T,D,sections', [
@@ -226,6 +304,15 @@ def test_rope_axes(B, H, Hk, T, D, sections, per_axis, inverse):
     for g, x in zip(got, (q, k)):
         want, tol = R.rope_axes(x, pos, sections, 5000.0, per_axis, inverse)
         R.check(g, want, tol)
+
+
+def test_rope_axes_of_more_heads_than_a_grid_axis_holds():
+    r = rng(26)
+    q, k = f32(r.standard_normal((1, 200000, 1, 2))), f32(r.standard_normal((1, 1, 1, 2)))
+    pos = np.array([[[5]]], np.int32)
+    got = forward(lambda i: list(O.rope_axes(i['q'], i['k'], i['p'], [1])), dict(q=q, k=k, p=pos))
+    for g, x in zip(got, (q, k)):
+        R.check(g, *R.rope_axes(x, pos, [1]))
 
 
 def test_rope_axes_passes_infinities_of_other_pairs():
@@ -436,6 +523,29 @@ def test_model_of_them_trains_as_in_64_bits(B, T):
     torch.cuda.synchronize()
     assert np.array_equal(got.cpu().numpy(), out)
     t.destroy()
+
+
+def test_model_of_them_steps_alike_captured_and_launched(monkeypatch):
+    """Captured steps, replayed with eager work and waits between, against steps launched one by one: the same bits."""
+    B, T = 2, 150
+    batches = [mixed_batch(B, T, n) for n in range(5)]
+    decl = {n: {'shape': list(a.shape), 'dtype': 'i32' if a.dtype == np.int32 else 'f32'} for n, a in batches[0].items()}
+
+    def train(graph):
+        monkeypatch.setenv('TG_GRAPH', graph)
+        t = tg_compile(Mixed(), lambda p, i: nn.cross_entropy(mixed_logits(p, i), i['targets']), decl, {'kind': 'adam', 'lr': 0.01}, seed=4)
+        losses = []
+        for b in batches:
+            r = t.step(b)
+            assert r.kind == 'completed', r.error
+            losses.append(r.loss)
+            torch.randn(1 << 20, device='cuda').sum()
+            torch.cuda.synchronize()
+        w = t.download_params()
+        t.destroy()
+        return losses, w
+    (l0, w0), (l1, w1) = train('0'), train('1')
+    assert l0 == l1 and all(np.array_equal(w0[n], w1[n]) for n in w0)
 
 
 # ---- device-resident calls -----------------------------------------------------------------------------

@@ -49,6 +49,14 @@ def test_attention_refusals():
     trace_fn(lambda: O.attention(*base(Tq=5), causal=False))       # cross attention may have more queries than keys
 
 
+def test_attention_refuses_constants_beyond_f32():
+    for x in (1e-300, 1e-40, 1e30, 1e300):
+        refuses(lambda: O.attention(*base(), scale=x), 'scale')
+        refuses(lambda: O.attention(*base(), softcap=x), 'softcap')
+    refuses(lambda: O.attention(*base(), slopes=[1, 1, 1, -1e39]), 'slopes')
+    trace_fn(lambda: O.attention(*base(), scale=2.0 ** -60, softcap=2.0 ** 60, slopes=[0, -1, 1, 2.0 ** 60]))
+
+
 def test_rope_axes_refusals():
     q, k, p = (lambda: t('q', 2, 4, 3, 8)), (lambda: t('k', 2, 2, 3, 8)), (lambda n=2, dtype='i32': t('p', n, 2, 3, dtype=dtype))
     refuses(lambda: O.rope_axes(t('q', 2, 3, 8), k(), p(), [2, 2]), 'q must be')
