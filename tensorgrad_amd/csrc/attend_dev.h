@@ -10,6 +10,10 @@
 // register r holds row 8 (r / 4) + 4 (l / 32) + r % 4 of column l % 32. One fragment of a wavefront is 1 KiB. The scores'
 // registers 8 s .. 8 s + 7 are the B fragment of the next product's k step s as they stand, if that product's A fragments
 // take their k in the same order: rows 16 s + 4 h + 0..3 and 16 s + 8 + 4 h + 0..3 for lane half h.
+//
+// Of a 16 x 16 x 32 product: lane l holds row or column l % 16 and k = 8 g + 0..7, g = l / 16; result register r holds row
+// 4 g + r of column l % 16. Two such blocks of scores, rows 0..15 and 16..31, are the B fragment of one k step: rows
+// 4 g + 0..3 and 16 + 4 g + 0..3.
 #pragma once
 #include "kernels.h"
 #include "sequence.h"
@@ -75,6 +79,8 @@ __device__ __forceinline__ void split8(const float* x, half8& hi, half8& lo) {
 }
 
 __device__ __forceinline__ f32x16 mfma(half8 a, half8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 // Over lanes l and l ^ 32, which hold the two halves of a row.
 __device__ __forceinline__ float halves_max(float x) {
@@ -505,6 +511,7 @@ struct Packs {
   int n;
   int Hk, tiles;                   // tiles: the most of any job
   bool wide;                       // every operand's rows are 16-byte aligned and whole 16-byte pieces
+  bool narrow;                     // queries are packed for products of 16 columns
   PackJob job[4];
   AttendDesc a;
 };

@@ -107,11 +107,15 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
   }
   if (bad) return;
   __syncthreads();
+  const bool narrow = p.narrow && j.query;
+  const int g16 = lane >> 4, l16 = lane & 15;
   if (j.rowf)
     for (int c = w; c < KC; c += 4) {
+      // 16 features c of 32 rows; narrow: 32 features c / 2 of 16 rows
+      const int r = narrow ? 16 * (c % 2) + l16 : l, d = narrow ? 32 * (c / 2) + 8 * g16 : 16 * c + 8 * h;
       float z[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) z[q] = x[l * LD + 16 * c + 8 * h + q] * own[l];
+      for (int q = 0; q < 8; ++q) z[q] = x[r * LD + d + q] * own[r];
       half8 a, f;
       split8(z, a, f);
       half8* o = (half8*)(j.rowf + (slot * KC + c) * 2 * kFrag) + lane;
@@ -119,12 +123,13 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
       o[kFrag / 8] = f;
     }
   if (j.colf)
-    for (int c = w; c < 2 * DB; c += 4) {   // feature block c / 2, k step c % 2
+    for (int c = w; c < 2 * DB; c += 4) {   // feature block c / 2, k step c % 2; narrow: feature block c of 16
+      const int d = narrow ? 16 * c + l16 : 32 * (c / 2) + l;
       float z[8];
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        const int k = 16 * (c % 2) + 8 * (q / 4) + 4 * h + q % 4;
-        z[q] = x[k * LD + 32 * (c / 2) + l] * own[k];
+        const int k = narrow ? 16 * (q / 4) + 4 * g16 + q % 4 : 16 * (c % 2) + 8 * (q / 4) + 4 * h + q % 4;
+        z[q] = x[k * LD + d] * own[k];
       }
       half8 a, f;
       split8(z, a, f);

@@ -46,6 +46,15 @@ __device__ __forceinline__ bool part_rows(const GradArgs& A, const Sight& s, int
   return from < to;
 }
 
+__device__ __forceinline__ bool document_part(const GradArgs& A, const Sight& s, int split, int slab, int blk, int& t0, int& t1) {
+  if (!s.doc || A.splits == 1) return true;
+  const int each = max((t1 - t0 + A.splits - 1) / A.splits, 8);
+  if (split == 0 && threadIdx.x == 0) A.parts[slab * A.blocks + blk] = (t1 - t0 + each - 1) / each;
+  t0 += split * each;
+  t1 = min(t0 + each, t1);
+  return t0 < t1;
+}
+
 // Where dk and dv of key j go.
 __device__ __forceinline__ float* dk_row(const GradArgs& A, int split, int slab, int b, int hk, int j) {
   if (!A.g.dk.p) return nullptr;
@@ -58,15 +67,15 @@ __device__ __forceinline__ float* dv_row(const GradArgs& A, int split, int slab,
   return A.g.dv.p + b * A.g.dv.b + hk * A.g.dv.h + (int64_t)j * A.g.dv.t;
 }
 
-// A wavefront's keys [j0, j0 + 32) over query rows [r0, r1) in plain f32.
-template <int WHAT>
+// A wavefront's keys [j0, j0 + KEYS) over query rows [r0, r1) in plain f32.
+template <int WHAT, int KEYS>
 __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, int split, int slab, int b, int hk, int j0, int r0, int r1) {
   const AttendDesc& a = A.g.a;
   const int lane = threadIdx.x & 63, G = (int)A.group.d;
   r1 = min(r1, A.M);
   auto row = [&](const Rows& x, int r) { return x.p + b * x.b + (hk * G + r % G) * x.h + (int64_t)(r / G) * x.t; };
 #pragma unroll 1
-  for (int j = j0; j < min(j0 + kTile, a.Tk); ++j) {
+  for (int j = j0; j < min(j0 + KEYS, a.Tk); ++j) {
     const float* k = a.k.p + b * a.k.b + hk * a.k.h + (int64_t)j * a.k.t;
     const float* v = a.v.p + b * a.v.b + hk * a.v.h + (int64_t)j * a.v.t;
     const int doc = s.doc ? s.doc[j] : 0;
@@ -96,11 +105,9 @@ __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, in
   }
 }
 
-// WHAT: 1 for dk, 2 for dv, 3 for both in one walk. Both take the registers of two wavefronts at head sizes above 96: there
-// each has a walk of its own (a quarter more products, but no spilled registers: 0.99 ms instead of 1.05 over 4096 causal
-// rows of 16 heads).
+// WHAT: 1 for dk, 2 for dv, 3 for both in one walk. For head sizes up to 64.
 template <int DP, bool RICH, int WHAT>
-__global__ __launch_bounds__(256, DP <= 64 || WHAT == 2 ? 2 : 1) void attend_grad_kv(GradArgs A) {
+__global__ __launch_bounds__(256, 2) void attend_grad_kv(GradArgs A) {
   constexpr int KC = DP / 16, DB = DP / 32;
   constexpr bool DK = WHAT & 1, DV = WHAT & 2;
   constexpr int F_GR = 2 * KC, F_QC = F_GR + (DK ? 2 * KC : 0), F_GC = F_QC + (DK ? 4 * DB : 0), F_SIDE = F_GC + (DV ? 4 * DB : 0),
@@ -132,15 +139,9 @@ __global__ __launch_bounds__(256, DP <= 64 || WHAT == 2 ? 2 : 1) void attend_gra
   if (!part_rows(A, s, k0, split, from, to)) return;   // nothing, and the join knows
   const Range range_ = tile_range(s, from, to, gi, qi, gi, mine.dmin, mine.dmax, range);
   int t0 = range_.t0, t1 = range_.t1;
-  if (s.doc && A.splits > 1) {
-    const int each = max((t1 - t0 + A.splits - 1) / A.splits, 8);
-    if (split == 0 && tid == 0) A.parts[slab * A.blocks + blk] = each > 0 ? (t1 - t0 + each - 1) / each : 0;
-    t0 += split * each;
-    t1 = min(t0 + each, t1);
-    if (t0 >= t1) return;
-  }
+  if (!document_part(A, s, split, slab, blk, t0, t1)) return;
   if (__builtin_expect(range_.odd, 0)) {
-    plain_keys<WHAT>(A, s, split, slab, b, hk, j0, t0 * kTile, t1 * kTile);
+    plain_keys<WHAT, kTile>(A, s, split, slab, b, hk, j0, t0 * kTile, t1 * kTile);
     return;
   }
 
@@ -196,12 +197,8 @@ __global__ __launch_bounds__(256, DP <= 64 || WHAT == 2 ? 2 : 1) void attend_gra
     if (__builtin_expect(j0 >= a.Tk || !any_seen(s, rows, mine, j0), 0)) continue;
     // register r: row r0 + 8 (r / 4) + 4 h + r % 4
     f32x16 x, y = {};
-    if constexpr (DK && DP > 64) {
-      scores2<KC>(L, 0, kh, kl, x, F_GR, vh, vl, y);
-    } else {
-      x = scores<KC>(L, 0, kh, kl);
-      if constexpr (DK) y = scores<KC>(L, F_GR, vh, vl);
-    }
+    x = scores<KC>(L, 0, kh, kl);
+    if constexpr (DK) y = scores<KC>(L, F_GR, vh, vl);
     if (__builtin_expect(qt.uneven, 0)) per_row(x, side + QS_RELQ * kTile);
     if (DK && __builtin_expect(gt.uneven, 0)) per_row(y, side + QS_RELG * kTile);
     const float unit = a.scale * pow2(-ke) * qt.inv, yunit = pow2(-ve) * gt.inv;
@@ -262,6 +259,297 @@ __global__ __launch_bounds__(256, DP <= 64 || WHAT == 2 ? 2 : 1) void attend_gra
   float* ov = dv_row(A, split, slab, b, hk, j);
   if (DK && ok) store_row<DB>(ok, dk, ck, a.scale, a.D, A.splits > 1 ? a.D % 4 == 0 : A.wide);
   if (DV && ov) store_row<DB>(ov, dv, cv, 1.0f, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide);
+}
+
+// The same for head sizes above 64, where 32 keys with their k, v, dk and dv take all registers of a SIMD and its one wavefront
+// waits for every product: a wavefront keeps 16 keys and multiplies 16 x 16 x 32, two wavefronts a SIMD, 8 a block. The
+// fragments are read from LDS twice as often for it. Both gradients of
+// 4096 causal rows of 16 heads of 128: 690 us, where dk and dv by 32 keys took 638 and 350 in walks of their own; 32 slabs of
+// 777 rows, head size 96: 72 us instead of 88.
+__device__ __forceinline__ float groups_max(float x) {   // over lanes l % 16 + 0, 16, 32, 48
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+// B fragments of 16 rows (lane l: row l % 16), each row with its own power of two; returns its exponent.
+template <int N>
+__device__ __forceinline__ int load_rows16(const float* row, bool valid, int n, bool wide, half8 (&hi)[N], half8 (&lo)[N]) {
+  const int g = (threadIdx.x >> 4) & 3;
+  float x[N][8], m = 0;
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    const int d = 32 * c + 8 * g;
+    if (wide) {
+      f32x4 u = {}, w = {};
+      if (valid && d < n) {
+        u = *(const f32x4*)(row + d);
+        w = *(const f32x4*)(row + d + 4);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { x[c][i] = u[i]; x[c][4 + i] = w[i]; }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[c][i] = valid && d + i < n ? row[d + i] : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < N; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(x[c][i]));
+  m = groups_max(m);
+  const int e = m > 0 ? min(14 - exponent(m), 126) : 0;
+  const float s = pow2(e);
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[c][i] *= s;
+    split8(x[c], hi[c], lo[c]);
+  }
+  return e;
+}
+// N fragments by eight wavefronts, wavefront w's at src and lds + 1024 w.
+template <int N>
+__device__ __forceinline__ void frags_by_eight(const char* src, uint32_t lds, uint32_t lane16, int w) {
+#pragma unroll
+  for (int f = 0; f < N / 8; ++f) frags_to_lds<4>(src + f * 8192, lds + f * 8192, lane16);
+  if (N % 8 && w < N % 8) frags_to_lds<4>(src + N / 8 * 8192, lds + N / 8 * 8192, lane16);
+}
+// x = A fragments (N chunks of 32 features, two blocks of 16 rows each, from fragment f0) times B fragments.
+template <int N>
+__device__ __forceinline__ void scores16(const _Float16* L, int f0, const half8 (&bh)[N], const half8 (&bl)[N], float (&x)[8]) {
+  f32x4 z[2] = {};
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    half8 a[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = frag(L, f0 + 4 * c + i);
+    z[0] = mfma16(a[1], bh[c], z[0]);
+    z[1] = mfma16(a[3], bh[c], z[1]);
+    z[0] = mfma16(a[0], bl[c], z[0]);
+    z[1] = mfma16(a[2], bl[c], z[1]);
+    z[0] = mfma16(a[0], bh[c], z[0]);
+    z[1] = mfma16(a[2], bh[c], z[1]);
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) x[q] = z[q / 4][q % 4];
+}
+// acc += A fragments (N blocks of 16 features, from fragment f0) times the split of x * scale.
+template <int N>
+__device__ __forceinline__ void accumulate16(f32x4 (&acc)[N], const float (&x)[8], float scale, const _Float16* L, int f0) {
+  half8 bh, bl;
+  float z[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) z[q] = x[q] * scale;
+  split8(z, bh, bl);
+#pragma unroll
+  for (int d = 0; d < N; d += 2) {
+    half8 a[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = frag(L, f0 + 2 * d + i);
+    acc[d] = mfma16(a[1], bh, acc[d]);
+    acc[d + 1] = mfma16(a[3], bh, acc[d + 1]);
+    acc[d] = mfma16(a[0], bl, acc[d]);
+    acc[d + 1] = mfma16(a[2], bl, acc[d + 1]);
+    acc[d] = mfma16(a[0], bh, acc[d]);
+    acc[d + 1] = mfma16(a[2], bh, acc[d + 1]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void rescale16(f32x4 (&acc)[N], float change) {
+  if (__builtin_expect(!__any(change != 1), 1)) return;
+#pragma unroll
+  for (int d = 0; d < N; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[d][q] *= change;
+}
+__device__ __forceinline__ void per_row16(float (&x)[8], const float* rel, int g) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) x[q] *= rel[16 * (q / 4) + 4 * g + q % 4];
+}
+__device__ __forceinline__ float largest16(const float (&x)[8]) {
+  float m = 0;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) m = fmaxf(m, fabsf(x[q]));
+  return groups_max(m);
+}
+template <int N>
+__device__ __forceinline__ void store_row16(float* row, const f32x4 (&acc)[N], int c, float scale, int n, bool wide, int g) {
+#pragma unroll
+  for (int d = 0; d < N; ++d) {
+    const int at = 16 * d + 4 * g;
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_ldexpf(acc[d][e], -c) * scale;
+    if (wide) {
+      if (at < n) *(f32x4*)(row + at) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) if (at + e < n) row[at + e] = v[e];
+    }
+  }
+}
+
+template <int DP, bool RICH, int WHAT>
+__global__ __launch_bounds__(512) void attend_grad_kv16(GradArgs A) {
+  constexpr int N = DP / 32, F = 4 * N;                      // chunks of 32 features; fragments of an operand
+  constexpr bool DK = WHAT & 1, DV = WHAT & 2;
+  constexpr int F_GR = F, F_QC = F_GR + (DK ? F : 0), F_GC = F_QC + (DK ? F : 0), F_SIDE = F_GC + (DV ? F : 0), NF = F_SIDE + kSideFrags;
+  __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
+  __shared__ int range[5];
+  const AttendDesc& a = A.g.a;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15;
+  int slab, item;
+  place(blockIdx.x, a.B * a.Hk, slab, item);
+  if (item >= A.blocks * A.splits) return;
+  const int split = A.splits - 1 - item / A.blocks, blk = item % A.blocks;   // blocks that start together walk the same rows
+  const int b = slab / a.Hk, hk = slab % a.Hk;
+  const Sight s = sight(a, b);
+  const int j0 = blk * 128 + w * 16, jt = j0 / kTile * kTile, j = j0 + l;   // masks are judged by whole tiles of keys
+  const bool valid = j < a.Tk;
+  const int doc = s.doc && valid ? s.doc[j] : -1;
+  TileInfo mine = A.ki[(int64_t)slab * A.ktiles + min(jt / kTile, A.ktiles - 1)];
+  if (jt >= a.Tk) {
+    mine.dmin = INT32_MAX;
+    mine.dmax = INT32_MIN;
+  }
+  const TileInfo* qi = A.qi + (int64_t)slab * A.qtiles;
+  const TileInfo* gi = A.gi + (int64_t)slab * A.qtiles;
+  int from, to;
+  if (!part_rows(A, s, blk * 128, split, from, to)) return;   // nothing, and the join knows
+  const Range range_ = tile_range(s, from, to, gi, qi, gi, mine.dmin, mine.dmax, range);
+  int t0 = range_.t0, t1 = range_.t1;
+  if (!document_part(A, s, split, slab, blk, t0, t1)) return;
+  if (__builtin_expect(range_.odd, 0)) {
+    plain_keys<WHAT, 16>(A, s, split, slab, b, hk, j0, t0 * kTile, t1 * kTile);
+    return;
+  }
+
+  half8 kh[N], kl[N], vh[DK ? N : 1], vl[DK ? N : 1];
+  const int ke = load_rows16<N>(a.k.p + b * a.k.b + hk * a.k.h + (int64_t)min(j, a.Tk - 1) * a.k.t, valid, a.D, A.wide, kh, kl);
+  int ve = 0;
+  if constexpr (DK) ve = load_rows16<N>(a.v.p + b * a.v.b + hk * a.v.h + (int64_t)min(j, a.Tk - 1) * a.v.t, valid, a.Dv, A.wide, vh, vl);
+  const int64_t tile0 = (int64_t)slab * A.qtiles + t0;
+  const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
+  const char* qr = (const char*)(A.qr + tile0 * (F * kFrag)) + w * 1024;
+  const char* gr = (const char*)(A.gr + tile0 * (F * kFrag)) + w * 1024;
+  const char* qc = (const char*)(A.qc + tile0 * (F * kFrag)) + w * 1024;
+  const char* gc = (const char*)(A.gc + tile0 * (F * kFrag)) + w * 1024;
+  const char* side_p = (const char*)(A.qside + tile0 * (kSide * kTile)) + w * 1024;
+  auto fetch = [&](int buf) {      // the next tile
+    const uint32_t to = base + buf * (NF * 1024);
+    frags_by_eight<F>(qr, to, lane16, w);
+    qr += F * 1024;
+    if (DK) {
+      frags_by_eight<F>(gr, to + F_GR * 1024, lane16, w);
+      frags_by_eight<F>(qc, to + F_QC * 1024, lane16, w);
+      gr += F * 1024;
+      qc += F * 1024;
+    }
+    if (DV) {
+      frags_by_eight<F>(gc, to + F_GC * 1024, lane16, w);
+      gc += F * 1024;
+    }
+    frags_by_eight<kSideFrags>(side_p, to + F_SIDE * 1024, lane16, w);
+    side_p += kSide * kTile * 4;
+  };
+
+  f32x4 dk[2 * N], dv[2 * N];
+#pragma unroll
+  for (int d = 0; d < 2 * N; ++d) dk[d] = dv[d] = f32x4{};
+  int ck = kUnset, cv = kUnset;
+  const float icap = RICH && a.cap > 0 ? 1.0f / a.cap : 0.0f;
+  if (t0 < t1) fetch(0);
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1, r0 = t * kTile;
+    loads_done();
+    __syncthreads();
+    if (t + 1 < t1) fetch(buf ^ 1);
+    const _Float16* L = lds + buf * (NF * kFrag);
+    const float* side = (const float*)(L + F_SIDE * kFrag);
+    const TileInfo qt = side_info(side, 0), gt = side_info(side, 1);
+    Span rows;
+    rows.pmin = s.first + (int)fastdiv((uint32_t)r0, A.group);
+    rows.pmax = s.first + (int)fastdiv((uint32_t)min(r0 + kTile - 1, A.M - 1), A.group);
+    rows.dmin = gt.dmin;
+    rows.dmax = gt.dmax;
+    rows.same = gt.same;
+    if (__builtin_expect(j0 >= a.Tk || !any_seen(s, rows, mine, jt), 0)) continue;
+    // element q: row r0 + 16 (q / 4) + 4 g + q % 4
+    float x[8], y[8] = {};
+    scores16<N>(L, 0, kh, kl, x);
+    if constexpr (DK) scores16<N>(L, F_GR, vh, vl, y);
+    if (__builtin_expect(qt.uneven, 0)) per_row16(x, side + QS_RELQ * kTile, g);
+    if (DK && __builtin_expect(gt.uneven, 0)) per_row16(y, side + QS_RELG * kTile, g);
+    const float unit = a.scale * pow2(-ke) * qt.inv, yunit = pow2(-ve) * gt.inv;
+    float f = unit * kLog2e;
+    if (RICH && a.cap > 0) {
+      const float u = unit * icap;
+      float most = 0;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        x[q] *= u;
+        most = fmaxf(most, fabsf(x[q]));
+      }
+      if (__any(most >= kFlat)) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[q] = tanh_of(x[q]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[q] = tanh_flat(x[q]);
+      }
+      f = a.cap * kLog2e;
+    }
+    const bool all = A.M - r0 >= kTile && all_seen(s, rows, mine, jt);
+#pragma unroll
+    for (int q4 = 0; q4 < 2; ++q4) {
+      const int at = 16 * q4 + 4 * g;
+      const f32x4 lse = *(const f32x4*)(side + QS_LSE * kTile + at), dot = *(const f32x4*)(side + QS_DOT * kTile + at);
+      f32x4 off = lse;
+      if (RICH && a.slopes) {
+        const f32x4 pos = *(const f32x4*)(side + QS_POS * kTile + at), slope = *(const f32x4*)(side + QS_SLOPE * kTile + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) off[e] = fmaf(slope[e], fabsf((float)(__float_as_int(pos[e]) - j)), lse[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int q = 4 * q4 + e;
+        const float p = __builtin_amdgcn_exp2f(fmaf(x[q], f, -off[e]));
+        if (DK) {
+          y[q] = p * fmaf(y[q], yunit, -dot[e]);
+          if (RICH && a.cap > 0) y[q] *= fmaf(-x[q], x[q], 1.0f);   // 1 - tanh^2
+        }
+        x[q] = p;
+      }
+      if (__builtin_expect(!all, 0)) {
+        const f32x4 below = *(const f32x4*)(side + QS_BELOW * kTile + at), rdoc = *(const f32x4*)(side + QS_DOC * kTile + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool ok = j < __float_as_int(below[e]) && (!s.doc || (doc >= 0 && __float_as_int(rdoc[e]) == doc));
+          x[4 * q4 + e] = ok ? x[4 * q4 + e] : 0.0f;
+          y[4 * q4 + e] = ok ? y[4 * q4 + e] : 0.0f;
+        }
+      }
+    }
+    if (DV) {
+      if (__builtin_expect(gt.uneven, 0)) per_row16(x, side + QS_RELG * kTile, g);
+      float change = 1;
+      const int e = fit_unit(cv, largest16(x), exponent(gt.scale), &change);
+      rescale16(dv, change);
+      accumulate16(dv, x, pow2(e), L, F_GC);
+    }
+    if (DK) {
+      if (__builtin_expect(qt.uneven, 0)) per_row16(y, side + QS_RELQ * kTile, g);
+      float change = 1;
+      const int e = fit_unit(ck, largest16(y), exponent(qt.scale), &change);
+      rescale16(dk, change);
+      accumulate16(dk, y, pow2(e), L, F_QC);
+    }
+  }
+
+  if (!valid) return;
+  float* ok = dk_row(A, split, slab, b, hk, j);
+  float* ov = dv_row(A, split, slab, b, hk, j);
+  if (DK && ok) store_row16(ok, dk, ck, a.scale, a.D, A.splits > 1 ? a.D % 4 == 0 : A.wide, g);
+  if (DV && ov) store_row16(ov, dv, cv, 1.0f, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide, g);
 }
 
 // The parts of dk, dv and dq in order: a block takes 32 keys of the 128 that the parts were split for, or 32 query rows.
@@ -538,13 +826,14 @@ template <int DP, bool RICH>
 void run_grad(const GradArgs& A, int slabs, hipStream_t st) {
   const AttendGradDesc& g = A.g;
   const dim3 keys(place_grid(slabs, (int64_t)A.blocks * A.splits));
-  if constexpr (DP <= 96) {
+  if constexpr (DP <= 64) {
     if (g.dk.p && g.dv.p) klaunch(attend_grad_kv<DP, RICH, 3>, keys, dim3(256), 0, st, A);
     else if (g.dk.p) klaunch(attend_grad_kv<DP, RICH, 1>, keys, dim3(256), 0, st, A);
     else if (g.dv.p) klaunch(attend_grad_kv<DP, RICH, 2>, keys, dim3(256), 0, st, A);
   } else {
-    if (g.dk.p) klaunch(attend_grad_kv<DP, RICH, 1>, keys, dim3(256), 0, st, A);
-    if (g.dv.p) klaunch(attend_grad_kv<DP, RICH, 2>, keys, dim3(256), 0, st, A);
+    if (g.dk.p && g.dv.p) klaunch(attend_grad_kv16<DP, RICH, 3>, keys, dim3(512), 0, st, A);
+    else if (g.dk.p) klaunch(attend_grad_kv16<DP, RICH, 1>, keys, dim3(512), 0, st, A);
+    else if (g.dv.p) klaunch(attend_grad_kv16<DP, RICH, 2>, keys, dim3(512), 0, st, A);
   }
   if (g.dq.p)
     klaunch(attend_grad_q<DP, RICH>, dim3(place_grid(slabs, (int64_t)((A.M + 127) / 128) * A.qsplits)), dim3(256), 0, st, A);
@@ -572,6 +861,7 @@ void attend_grad(const AttendGradDesc& g, void* work, hipStream_t st) {
   k.n = 4;
   k.Hk = a.Hk;
   k.wide = wide;
+  k.narrow = p.DP > 64;
   k.a = a;
   float *qs = (float*)(w + p.qside), *ks = (float*)(w + p.kside);
   k.job[0] = {a.q, a.D, p.G, p.M, p.qtiles, half(p.qr), half(p.qc), info(p.qi), true, qs, QS_RELQ, false, false, {}};
