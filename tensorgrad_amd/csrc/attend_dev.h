@@ -321,40 +321,6 @@ __device__ __forceinline__ void scores_woven(f32x16& x, const _Float16* L, int f
     __builtin_amdgcn_sched_barrier(0);
   }
 }
-// Both products of a gradient's pair, step by step in turn: four accumulators, and twice the products between a fragment's
-// read and its use. For head sizes above 64, where a SIMD has one wavefront to keep it busy.
-template <int KC>
-__device__ __forceinline__ void scores2(const _Float16* L, int f0, const half8 (&bh)[KC], const half8 (&bl)[KC], f32x16& x, int f1,
-                                        const half8 (&ch)[KC], const half8 (&cl)[KC], f32x16& y) {
-  f32x16 x0 = {}, x1 = {}, y0 = {}, y1 = {};
-  half8 a[2][4];
-  auto read = [&](int c) {
-    a[c & 1][0] = frag(L, f0 + 2 * c);
-    a[c & 1][1] = frag(L, f0 + 2 * c + 1);
-    a[c & 1][2] = frag(L, f1 + 2 * c);
-    a[c & 1][3] = frag(L, f1 + 2 * c + 1);
-  };
-  read(0);
-  __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-  for (int c = 0; c < KC; ++c) {
-    if (c + 1 < KC) read(c + 1);
-    const half8* f = a[c & 1];
-    x1 = mfma(f[1], bh[c], x1);
-    y1 = mfma(f[3], ch[c], y1);
-    x0 = mfma(f[0], bh[c], x0);
-    y0 = mfma(f[2], ch[c], y0);
-    x1 = mfma(f[0], bl[c], x1);
-    y1 = mfma(f[2], cl[c], y1);
-    if (c + 1 < KC) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);   // the next step's reads, then this step's products
-    __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
-  }
-#pragma unroll
-  for (int q = 0; q < 16; ++q) {
-    x[q] = x0[q] + x1[q];
-    y[q] = y0[q] + y1[q];
-  }
-}
 // x[q] *= rel of the tile's row 8 (q / 4) + 4 h + q % 4
 __device__ __forceinline__ void per_row(f32x16& x, const float* rel) {
   const int h = (threadIdx.x >> 5) & 1;
@@ -511,7 +477,7 @@ struct Packs {
   int n;
   int Hk, tiles;                   // tiles: the most of any job
   bool wide;                       // every operand's rows are 16-byte aligned and whole 16-byte pieces
-  bool narrow;                     // queries are packed for products of 16 columns
+  bool narrow;                     // packed for products of 16 columns
   PackJob job[4];
   AttendDesc a;
 };

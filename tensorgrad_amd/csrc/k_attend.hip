@@ -107,7 +107,7 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
   }
   if (bad) return;
   __syncthreads();
-  const bool narrow = p.narrow && j.query;
+  const bool narrow = p.narrow;
   const int g16 = lane >> 4, l16 = lane & 15;
   if (j.rowf)
     for (int c = w; c < KC; c += 4) {
