@@ -313,44 +313,54 @@ __device__ __forceinline__ void frags_by_eight(const char* src, uint32_t lds, ui
   for (int f = 0; f < N / 8; ++f) frags_to_lds<4>(src + f * 8192, lds + f * 8192, lane16);
   if (N % 8 && w < N % 8) frags_to_lds<4>(src + N / 8 * 8192, lds + N / 8 * 8192, lane16);
 }
-// x = A fragments (N chunks of 32 features, two blocks of 16 rows each, from fragment f0) times B fragments.
+// x = A fragments (N chunks of 32 features, two blocks of 16 rows each, from fragment f0) times B fragments; a chunk's
+// fragments are read while the chunk before is multiplied.
 template <int N>
 __device__ __forceinline__ void scores16(const _Float16* L, int f0, const half8 (&bh)[N], const half8 (&bl)[N], float (&x)[8]) {
   f32x4 z[2] = {};
+  half8 a[2][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[0][i] = frag(L, f0 + i);
 #pragma unroll
   for (int c = 0; c < N; ++c) {
-    half8 a[4];
+    const half8* u = a[c & 1];
+    if (c + 1 < N)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = frag(L, f0 + 4 * c + i);
-    z[0] = mfma16(a[1], bh[c], z[0]);
-    z[1] = mfma16(a[3], bh[c], z[1]);
-    z[0] = mfma16(a[0], bl[c], z[0]);
-    z[1] = mfma16(a[2], bl[c], z[1]);
-    z[0] = mfma16(a[0], bh[c], z[0]);
-    z[1] = mfma16(a[2], bh[c], z[1]);
+      for (int i = 0; i < 4; ++i) a[(c + 1) & 1][i] = frag(L, f0 + 4 * c + 4 + i);
+    z[0] = mfma16(u[1], bh[c], z[0]);
+    z[1] = mfma16(u[3], bh[c], z[1]);
+    z[0] = mfma16(u[0], bl[c], z[0]);
+    z[1] = mfma16(u[2], bl[c], z[1]);
+    z[0] = mfma16(u[0], bh[c], z[0]);
+    z[1] = mfma16(u[2], bh[c], z[1]);
+    __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
   for (int q = 0; q < 8; ++q) x[q] = z[q / 4][q % 4];
 }
-// acc += A fragments (N blocks of 16 features, from fragment f0) times the split of x * scale.
+// acc += A fragments (N blocks of 16 features, from fragment f0) times the split of x * scale, read as above.
 template <int N>
 __device__ __forceinline__ void accumulate16(f32x4 (&acc)[N], const float (&x)[8], float scale, const _Float16* L, int f0) {
-  half8 bh, bl;
+  half8 a[2][4], bh, bl;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[0][i] = frag(L, f0 + i);
   float z[8];
 #pragma unroll
   for (int q = 0; q < 8; ++q) z[q] = x[q] * scale;
   split8(z, bh, bl);
 #pragma unroll
   for (int d = 0; d < N; d += 2) {
-    half8 a[4];
+    const half8* u = a[d / 2 & 1];
+    if (d + 2 < N)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = frag(L, f0 + 2 * d + i);
-    acc[d] = mfma16(a[1], bh, acc[d]);
-    acc[d + 1] = mfma16(a[3], bh, acc[d + 1]);
-    acc[d] = mfma16(a[0], bl, acc[d]);
-    acc[d + 1] = mfma16(a[2], bl, acc[d + 1]);
-    acc[d] = mfma16(a[0], bh, acc[d]);
-    acc[d + 1] = mfma16(a[2], bh, acc[d + 1]);
+      for (int i = 0; i < 4; ++i) a[(d / 2 + 1) & 1][i] = frag(L, f0 + 2 * d + 4 + i);
+    acc[d] = mfma16(u[1], bh, acc[d]);
+    acc[d + 1] = mfma16(u[3], bh, acc[d + 1]);
+    acc[d] = mfma16(u[0], bl, acc[d]);
+    acc[d + 1] = mfma16(u[2], bl, acc[d + 1]);
+    acc[d] = mfma16(u[0], bh, acc[d]);
+    acc[d + 1] = mfma16(u[2], bh, acc[d + 1]);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 template <int N>
