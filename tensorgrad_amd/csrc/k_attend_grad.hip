@@ -338,6 +338,44 @@ __device__ __forceinline__ void scores16(const _Float16* L, int f0, const half8 
 #pragma unroll
   for (int q = 0; q < 8; ++q) x[q] = z[q / 4][q % 4];
 }
+// Both products of a pair, step by step in turn.
+template <int N>
+__device__ __forceinline__ void pair16(const _Float16* L, int f0, const half8 (&bh)[N], const half8 (&bl)[N], float (&x)[8], int f1,
+                                       const half8 (&ch)[N], const half8 (&cl)[N], float (&y)[8]) {
+  f32x4 z[4] = {};
+  half8 a[2][8];
+  auto read = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[c & 1][i] = frag(L, f0 + 4 * c + i);
+      a[c & 1][4 + i] = frag(L, f1 + 4 * c + i);
+    }
+  };
+  read(0);
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    const half8* u = a[c & 1];
+    if (c + 1 < N) read(c + 1);
+    z[0] = mfma16(u[1], bh[c], z[0]);
+    z[1] = mfma16(u[3], bh[c], z[1]);
+    z[2] = mfma16(u[5], ch[c], z[2]);
+    z[3] = mfma16(u[7], ch[c], z[3]);
+    z[0] = mfma16(u[0], bl[c], z[0]);
+    z[1] = mfma16(u[2], bl[c], z[1]);
+    z[2] = mfma16(u[4], cl[c], z[2]);
+    z[3] = mfma16(u[6], cl[c], z[3]);
+    z[0] = mfma16(u[0], bh[c], z[0]);
+    z[1] = mfma16(u[2], bh[c], z[1]);
+    z[2] = mfma16(u[4], ch[c], z[2]);
+    z[3] = mfma16(u[6], ch[c], z[3]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    x[q] = z[q / 4][q % 4];
+    y[q] = z[2 + q / 4][q % 4];
+  }
+}
 // acc += A fragments (N blocks of 16 features, from fragment f0) times the split of x * scale, read as above.
 template <int N>
 __device__ __forceinline__ void accumulate16(f32x4 (&acc)[N], const float (&x)[8], float scale, const _Float16* L, int f0) {
@@ -501,8 +539,8 @@ __global__ __launch_bounds__(512) void attend_grad_kv16(GradArgs A) {
     if (__builtin_expect(j0 >= a.Tk || !any_seen(s, rows, mine, jt), 0)) continue;
     // element q: row r0 + 16 (q / 4) + 4 g + q % 4
     float x[8], y[8] = {};
-    scores16<N>(L, 0, kh, kl, x);
-    if constexpr (DK) scores16<N>(L, F_GR, vh, vl, y);
+    if constexpr (DK) pair16<N>(L, 0, kh, kl, x, F_GR, vh, vl, y);
+    else scores16<N>(L, 0, kh, kl, x);
     if (__builtin_expect(qt.uneven, 0)) per_row16(x, side + QS_RELQ * kTile, g);
     if (DK && __builtin_expect(gt.uneven, 0)) per_row16(y, side + QS_RELG * kTile, g);
     const float unit = a.scale * pow2(-ke) * qt.inv, yunit = pow2(-ve) * gt.inv;
@@ -870,8 +908,7 @@ __global__ __launch_bounds__(512) void attend_grad_q16(GradArgs A) {
     if (__builtin_expect(!any_seen(s, me, kt, j0), 0)) continue;
     // element q: key j0 + 16 (q / 4) + 4 g4 + q % 4
     float x[8], y[8];
-    scores16<N>(L, 0, qh, ql, x);
-    scores16<N>(L, F_V, gh, gl, y);
+    pair16<N>(L, 0, qh, ql, x, F_V, gh, gl, y);
     if (__builtin_expect(kt.uneven, 0)) per_row16(x, side + KS_RELK * kTile, g4);
     if (__builtin_expect(vt.uneven, 0)) per_row16(y, side + KS_RELV * kTile, g4);
     const float unit = a.scale * pow2(-qe) * kt.inv, yunit = pow2(-ge) * vt.inv;
