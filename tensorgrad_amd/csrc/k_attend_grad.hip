@@ -2,9 +2,9 @@
 //   ds = P (dP - D) (1 - tanh^2),  dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i P_ij dy_i
 // (sums over i run over the query heads that share the key head). Two kernels, each with the whole of its own sums, so that
 // nothing is added by atomics and results repeat bit for bit; scores and dP are computed in both (7 products instead of 5):
-//  * attend_grad_kv: a wavefront keeps 32 keys, k and v in registers, and walks the query rows; scores are computed as
+//  * attend_grad_kv: a wavefront keeps 16 keys, k and v in registers, and walks the query rows; scores are computed as
 //    queries x keys, so that P and ds are the B fragments of dv and dk as they stand;
-//  * attend_grad_q: a wavefront keeps 32 query rows and walks the keys, scores transposed as in the forward pass.
+//  * attend_grad_q: a wavefront keeps 16 query rows and walks the keys, scores transposed as in the forward pass.
 // The walked operands are packed once (attend_pack, k_attend.hip); lse and D come with them.
 #include "attend_dev.h"
 
@@ -67,15 +67,15 @@ __device__ __forceinline__ float* dv_row(const GradArgs& A, int split, int slab,
   return A.g.dv.p + b * A.g.dv.b + hk * A.g.dv.h + (int64_t)j * A.g.dv.t;
 }
 
-// A wavefront's keys [j0, j0 + KEYS) over query rows [r0, r1) in plain f32.
-template <int WHAT, int KEYS>
+// A wavefront's keys [j0, j0 + 16) over query rows [r0, r1) in plain f32.
+template <int WHAT>
 __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, int split, int slab, int b, int hk, int j0, int r0, int r1) {
   const AttendDesc& a = A.g.a;
   const int lane = threadIdx.x & 63, G = (int)A.group.d;
   r1 = min(r1, A.M);
   auto row = [&](const Rows& x, int r) { return x.p + b * x.b + (hk * G + r % G) * x.h + (int64_t)(r / G) * x.t; };
 #pragma unroll 1
-  for (int j = j0; j < min(j0 + KEYS, a.Tk); ++j) {
+  for (int j = j0; j < min(j0 + 16, a.Tk); ++j) {
     const float* k = a.k.p + b * a.k.b + hk * a.k.h + (int64_t)j * a.k.t;
     const float* v = a.v.p + b * a.v.b + hk * a.v.h + (int64_t)j * a.v.t;
     const int doc = s.doc ? s.doc[j] : 0;
@@ -105,167 +105,12 @@ __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, in
   }
 }
 
-// WHAT: 1 for dk, 2 for dv, 3 for both in one walk. For head sizes up to 64.
-template <int DP, bool RICH, int WHAT>
-__global__ __launch_bounds__(256, 2) void attend_grad_kv(GradArgs A) {
-  constexpr int KC = DP / 16, DB = DP / 32;
-  constexpr bool DK = WHAT & 1, DV = WHAT & 2;
-  constexpr int F_GR = 2 * KC, F_QC = F_GR + (DK ? 2 * KC : 0), F_GC = F_QC + (DK ? 4 * DB : 0), F_SIDE = F_GC + (DV ? 4 * DB : 0),
-                NF = F_SIDE + kSideFrags;
-  __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
-  __shared__ int range[5];
-  const AttendDesc& a = A.g.a;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
-  int slab, item;
-  place(blockIdx.x, a.B * a.Hk, slab, item);
-  if (item >= A.blocks * A.splits) return;
-  const int split = A.splits - 1 - item / A.blocks, blk = item % A.blocks;   // blocks that start together walk the same rows
-  const int b = slab / a.Hk, hk = slab % a.Hk;
-  const Sight s = sight(a, b);
-  const int j0 = blk * 128 + w * kTile, j = j0 + l;
-  const bool valid = j < a.Tk;
-  const int doc = s.doc && valid ? s.doc[j] : -1;
-  TileInfo mine = A.ki[(int64_t)slab * A.ktiles + min(j0 / kTile, A.ktiles - 1)];
-  if (j0 >= a.Tk) {
-    mine.dmin = INT32_MAX;
-    mine.dmax = INT32_MIN;
-  }
+// ---- products of 16 columns ------------------------------------------------------------------------
+//
+// A wavefront's own rows (keys, or query rows) are the columns of 16 x 16 x 32 products: at head size 128 their operands and
+// gradients then leave room for two wavefronts a SIMD, where 32 columns took the registers of one, which waited for every
+// product. Fragments are read from LDS twice as often for it.
 
-  // the query tiles that see any of the block's keys: from its first key's position on, unless a prefix shows it to all
-  const TileInfo* qi = A.qi + (int64_t)slab * A.qtiles;
-  const TileInfo* gi = A.gi + (int64_t)slab * A.qtiles;
-  const int k0 = blk * 128;
-  int from, to;
-  if (!part_rows(A, s, k0, split, from, to)) return;   // nothing, and the join knows
-  const Range range_ = tile_range(s, from, to, gi, qi, gi, mine.dmin, mine.dmax, range);
-  int t0 = range_.t0, t1 = range_.t1;
-  if (!document_part(A, s, split, slab, blk, t0, t1)) return;
-  if (__builtin_expect(range_.odd, 0)) {
-    plain_keys<WHAT, kTile>(A, s, split, slab, b, hk, j0, t0 * kTile, t1 * kTile);
-    return;
-  }
-
-  half8 kh[KC], kl[KC], vh[DK ? KC : 1], vl[DK ? KC : 1];
-  const int ke = load_rows<KC>(a.k.p + b * a.k.b + hk * a.k.h + (int64_t)min(j, a.Tk - 1) * a.k.t, valid, a.D, A.wide, kh, kl);
-  int ve = 0;
-  if constexpr (DK) ve = load_rows<KC>(a.v.p + b * a.v.b + hk * a.v.h + (int64_t)min(j, a.Tk - 1) * a.v.t, valid, a.Dv, A.wide, vh, vl);
-  const int64_t tile0 = (int64_t)slab * A.qtiles;
-  const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
-  const char* qr = (const char*)(A.qr + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
-  const char* gr = (const char*)(A.gr + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
-  const char* qc = (const char*)(A.qc + (tile0 + t0) * (4 * DB * kFrag)) + w * 1024;
-  const char* gc = (const char*)(A.gc + (tile0 + t0) * (4 * DB * kFrag)) + w * 1024;
-  const char* side_p = (const char*)(A.qside + (tile0 + t0) * (kSide * kTile)) + w * 1024;
-  auto fetch = [&](int buf) {    // the next tile
-    const uint32_t to = base + buf * (NF * 1024);
-    frags_to_lds<2 * KC>(qr, to, lane16);
-    qr += 2 * KC * 1024;
-    if (DK) {
-      frags_to_lds<2 * KC>(gr, to + F_GR * 1024, lane16);
-      frags_to_lds<4 * DB>(qc, to + F_QC * 1024, lane16);
-      gr += 2 * KC * 1024;
-      qc += 4 * DB * 1024;
-    }
-    if (DV) {
-      frags_to_lds<4 * DB>(gc, to + F_GC * 1024, lane16);
-      gc += 4 * DB * 1024;
-    }
-    if (w < kSideFrags) frags_to_lds<4>(side_p, to + F_SIDE * 1024, lane16);
-    side_p += kSide * kTile * 4;
-  };
-
-  f32x16 dk[DB], dv[DB];
-#pragma unroll
-  for (int d = 0; d < DB; ++d) dk[d] = dv[d] = f32x16{};
-  int ck = kUnset, cv = kUnset;
-  const float icap = RICH && a.cap > 0 ? 1.0f / a.cap : 0.0f;
-  if (t0 < t1) fetch(0);
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1, r0 = t * kTile;
-    loads_done();
-    __syncthreads();
-    if (t + 1 < t1) fetch(buf ^ 1);
-    const _Float16* L = lds + buf * (NF * kFrag);
-    const float* side = (const float*)(L + F_SIDE * kFrag);
-    const TileInfo qt = side_info(side, 0), gt = side_info(side, 1);
-    Span rows;
-    rows.pmin = s.first + (int)fastdiv((uint32_t)r0, A.group);
-    rows.pmax = s.first + (int)fastdiv((uint32_t)min(r0 + kTile - 1, A.M - 1), A.group);
-    rows.dmin = gt.dmin;
-    rows.dmax = gt.dmax;
-    rows.same = gt.same;
-    if (__builtin_expect(j0 >= a.Tk || !any_seen(s, rows, mine, j0), 0)) continue;
-    // register r: row r0 + 8 (r / 4) + 4 h + r % 4
-    f32x16 x, y = {};
-    x = scores<KC>(L, 0, kh, kl);
-    if constexpr (DK) y = scores<KC>(L, F_GR, vh, vl);
-    if (__builtin_expect(qt.uneven, 0)) per_row(x, side + QS_RELQ * kTile);
-    if (DK && __builtin_expect(gt.uneven, 0)) per_row(y, side + QS_RELG * kTile);
-    const float unit = a.scale * pow2(-ke) * qt.inv, yunit = pow2(-ve) * gt.inv;
-    float f = unit * kLog2e;
-    if (RICH && a.cap > 0) {
-      tanh_all(x, unit * icap);
-      f = a.cap * kLog2e;
-    }
-    const bool all = A.M - r0 >= kTile && all_seen(s, rows, mine, j0);
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
-      const int at = 8 * q4 + 4 * h;
-      const f32x4 lse = *(const f32x4*)(side + QS_LSE * kTile + at), dot = *(const f32x4*)(side + QS_DOT * kTile + at);
-      f32x4 off = lse;
-      if (RICH && a.slopes) {
-        const f32x4 pos = *(const f32x4*)(side + QS_POS * kTile + at), slope = *(const f32x4*)(side + QS_SLOPE * kTile + at);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) off[e] = fmaf(slope[e], fabsf((float)(__float_as_int(pos[e]) - j)), lse[e]);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int q = 4 * q4 + e;
-        const float p = __builtin_amdgcn_exp2f(fmaf(x[q], f, -off[e]));
-        if (DK) {
-          y[q] = p * fmaf(y[q], yunit, -dot[e]);
-          if (RICH && a.cap > 0) y[q] *= fmaf(-x[q], x[q], 1.0f);   // 1 - tanh^2
-        }
-        x[q] = p;
-      }
-      if (__builtin_expect(!all, 0)) {
-        const f32x4 below = *(const f32x4*)(side + QS_BELOW * kTile + at), rdoc = *(const f32x4*)(side + QS_DOC * kTile + at);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool ok = j < __float_as_int(below[e]) && (!s.doc || (doc >= 0 && __float_as_int(rdoc[e]) == doc));
-          x[4 * q4 + e] = ok ? x[4 * q4 + e] : 0.0f;
-          y[4 * q4 + e] = ok ? y[4 * q4 + e] : 0.0f;
-        }
-      }
-    }
-    if (DV) {
-      if (__builtin_expect(gt.uneven, 0)) per_row(x, side + QS_RELG * kTile);
-      float change = 1;
-      const int e = fit_unit(cv, largest(x), exponent(gt.scale), &change);
-      rescale<DB>(dv, change);
-      accumulate<DB>(dv, x, pow2(e), L, F_GC);
-    }
-    if (DK) {
-      if (__builtin_expect(qt.uneven, 0)) per_row(y, side + QS_RELQ * kTile);
-      float change = 1;
-      const int e = fit_unit(ck, largest(y), exponent(qt.scale), &change);
-      rescale<DB>(dk, change);
-      accumulate<DB>(dk, y, pow2(e), L, F_QC);
-    }
-  }
-
-  if (!valid) return;
-  float* ok = dk_row(A, split, slab, b, hk, j);
-  float* ov = dv_row(A, split, slab, b, hk, j);
-  if (DK && ok) store_row<DB>(ok, dk, ck, a.scale, a.D, A.splits > 1 ? a.D % 4 == 0 : A.wide);
-  if (DV && ov) store_row<DB>(ov, dv, cv, 1.0f, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide);
-}
-
-// The same for head sizes above 64, where 32 keys with their k, v, dk and dv take all registers of a SIMD and its one wavefront
-// waits for every product: a wavefront keeps 16 keys and multiplies 16 x 16 x 32, two wavefronts a SIMD, 8 a block. The
-// fragments are read from LDS twice as often for it. Both gradients of
-// 4096 causal rows of 16 heads of 128: 690 us, where dk and dv by 32 keys took 638 and 350 in walks of their own; 32 slabs of
-// 777 rows, head size 96: 72 us instead of 88.
 __device__ __forceinline__ float groups_max(float x) {   // over lanes l % 16 + 0, 16, 32, 48
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
@@ -452,8 +297,11 @@ __device__ __forceinline__ void store_row16(float* row, const f32x4 (&acc)[N], i
   }
 }
 
+// Eight wavefronts of 16 keys. WHAT: 1 for dk, 2 for dv, 3 for both in one walk. Up to head size 64 two blocks share a CU. Both
+// gradients of 4096 causal rows of 16 heads of 128: 664 us (by 32 keys 990, in walks of their own); of 8 heads of 64: 193 us
+// (205); of 8 x 1000 rows of 8 heads of 32: 76 us (66), in documents of 50: 38 us (44).
 template <int DP, bool RICH, int WHAT>
-__global__ __launch_bounds__(512) void attend_grad_kv16(GradArgs A) {
+__global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs A) {
   constexpr int N = DP / 32, F = 4 * N;                      // chunks of 32 features; fragments of an operand
   constexpr bool DK = WHAT & 1, DV = WHAT & 2;
   constexpr int F_GR = F, F_QC = F_GR + (DK ? F : 0), F_GC = F_QC + (DK ? F : 0), F_SIDE = F_GC + (DV ? F : 0), NF = F_SIDE + kSideFrags;
@@ -483,7 +331,7 @@ __global__ __launch_bounds__(512) void attend_grad_kv16(GradArgs A) {
   int t0 = range_.t0, t1 = range_.t1;
   if (!document_part(A, s, split, slab, blk, t0, t1)) return;
   if (__builtin_expect(range_.odd, 0)) {
-    plain_keys<WHAT, 16>(A, s, split, slab, b, hk, j0, t0 * kTile, t1 * kTile);
+    plain_keys<WHAT>(A, s, split, slab, b, hk, j0, t0 * kTile, t1 * kTile);
     return;
   }
 
@@ -539,8 +387,13 @@ __global__ __launch_bounds__(512) void attend_grad_kv16(GradArgs A) {
     if (__builtin_expect(j0 >= a.Tk || !any_seen(s, rows, mine, jt), 0)) continue;
     // element q: row r0 + 16 (q / 4) + 4 g + q % 4
     float x[8], y[8] = {};
-    if constexpr (DK) pair16<N>(L, 0, kh, kl, x, F_GR, vh, vl, y);
-    else scores16<N>(L, 0, kh, kl, x);
+    if constexpr (DK && N == 2) {  // the pair in turn would spill registers here
+      scores16<N>(L, 0, kh, kl, x);
+      scores16<N>(L, F_GR, vh, vl, y);
+    } else if constexpr (DK) pair16<N>(L, 0, kh, kl, x, F_GR, vh, vl, y);
+    else {
+      scores16<N>(L, 0, kh, kl, x);
+    }
     if (__builtin_expect(qt.uneven, 0)) per_row16(x, side + QS_RELQ * kTile, g);
     if (DK && __builtin_expect(gt.uneven, 0)) per_row16(y, side + QS_RELG * kTile, g);
     const float unit = a.scale * pow2(-ke) * qt.inv, yunit = pow2(-ve) * gt.inv;
@@ -663,15 +516,14 @@ __device__ __forceinline__ float* dq_row(const GradArgs& A, int split, int slab,
   if (A.qsplits > 1) return A.pq + (((int64_t)split * A.g.a.B * A.g.a.Hk + slab) * A.M + r) * A.g.a.D;
   return A.g.dq.p + b * A.g.dq.b + head * A.g.dq.h + (int64_t)i * A.g.dq.t;
 }
-// A wavefront's rows [row0, row0 + ROWS) over keys [j0, j1) in plain f32.
-template <int ROWS>
+// A wavefront's rows [row0, row0 + 16) over keys [j0, j1) in plain f32.
 __device__ __forceinline__ void plain_dq(const GradArgs& A, const Sight& s, int split, int slab, int b, int hk, int row0, int j0, int j1) {
   const AttendDesc& a = A.g.a;
   const int lane = threadIdx.x & 63, G = (int)A.group.d;
   const float* k = a.k.p + b * a.k.b + hk * a.k.h;
   const float* v = a.v.p + b * a.v.b + hk * a.v.h;
 #pragma unroll 1
-  for (int r = row0; r < min(row0 + ROWS, A.M); ++r) {
+  for (int r = row0; r < min(row0 + 16, A.M); ++r) {
     const int i = r / G, head = hk * G + r % G;
     const float* q = a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t;
     const float* dy = A.g.dy.p + b * A.g.dy.b + head * A.g.dy.h + (int64_t)i * A.g.dy.t;
@@ -695,134 +547,10 @@ __device__ __forceinline__ void plain_dq(const GradArgs& A, const Sight& s, int 
   }
 }
 
-// For head sizes up to 64.
+// Eight wavefronts of 16 query rows. 4096 causal rows of 16 heads of 128: 371 us (470 by 32 rows); 8 x 1000 rows of 8 heads
+// of 64 in documents of 170: 49 us (57).
 template <int DP, bool RICH>
-__global__ __launch_bounds__(256, 2) void attend_grad_q(GradArgs A) {
-  constexpr int KC = DP / 16, DB = DP / 32;
-  constexpr int F_V = 2 * KC, F_KC = 4 * KC, F_SIDE = F_KC + 4 * DB, NF = F_SIDE + kSideFrags;
-  __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
-  __shared__ int range[5];
-  const AttendDesc& a = A.g.a;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
-  const int rblocks = (A.M + 127) / 128;
-  int slab, item;
-  place(blockIdx.x, a.B * a.Hk, slab, item);
-  if (item >= rblocks * A.qsplits) return;
-  const int split = item % A.qsplits, blk = rblocks - 1 - item / A.qsplits;
-  const int b = slab / a.Hk, hk = slab % a.Hk, G = (int)A.group.d;
-  const Sight s = sight(a, b);
-  const int row0 = blk * 128 + w * kTile, r = row0 + l, rr = min(r, A.M - 1);
-  const bool valid = r < A.M;
-  const int i = (int)fastdiv((uint32_t)rr, A.group), g = rr - i * G, head = hk * G + g;
-  const int p = s.first + i, doc = doc_at(s, p), below = sees_below(s, p);
-  const int qt = min(row0 / kTile, A.qtiles - 1);
-  const float* mine = A.qside + ((int64_t)slab * A.qtiles + qt) * (kSide * kTile) + l;
-  const float lse = mine[QS_LSE * kTile], dot = mine[QS_DOT * kTile];
-  const TileInfo gt = A.gi[(int64_t)slab * A.qtiles + qt];
-  Span me;
-  me.pmin = s.first + (int)fastdiv((uint32_t)min(row0, A.M - 1), A.group);
-  me.pmax = s.first + (int)fastdiv((uint32_t)min(row0 + kTile - 1, A.M - 1), A.group);
-  me.dmin = row0 < A.M ? gt.dmin : INT32_MAX;
-  me.dmax = row0 < A.M ? gt.dmax : INT32_MIN;
-  me.same = gt.same;
-
-  const TileInfo* ki = A.ki + (int64_t)slab * A.ktiles;
-  const TileInfo* vi = A.vi + (int64_t)slab * A.ktiles;
-  const int last = s.first + (int)fastdiv((uint32_t)min(blk * 128 + 127, A.M - 1), A.group);
-  int end = s.n;
-  if (s.causal) end = min(end, max(last + 1, s.prefix));
-  if (s.positional && last < 0) end = 0;
-  const Range range_ = tile_range(s, 0, (end + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax, range);
-  int t0 = range_.t0, t1 = range_.t1;
-  if (A.qsplits > 1) {
-    const int each = (t1 - t0 + A.qsplits - 1) / A.qsplits;
-    t0 = min(t0 + split * each, t1);
-    t1 = min(t0 + each, t1);
-  }
-  if (__builtin_expect(range_.odd, 0)) {
-    plain_dq<kTile>(A, s, split, slab, b, hk, row0, t0 * kTile, t1 * kTile);
-    return;
-  }
-
-  half8 qh[KC], ql[KC], gh[KC], gl[KC];
-  const int qe = load_rows<KC>(a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t, valid, a.D, A.wide, qh, ql);
-  const int ge = load_rows<KC>(A.g.dy.p + b * A.g.dy.b + head * A.g.dy.h + (int64_t)i * A.g.dy.t, valid, a.Dv, A.wide, gh, gl);
-  const float slope = RICH && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
-  const int64_t tile0 = (int64_t)slab * A.ktiles;
-  const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
-  const char* kr = (const char*)(A.kr + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
-  const char* vr = (const char*)(A.vr + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
-  const char* kc = (const char*)(A.kc + (tile0 + t0) * (4 * DB * kFrag)) + w * 1024;
-  const char* side_p = (const char*)(A.kside + (tile0 + t0) * (kSide * kTile)) + w * 1024;
-  auto fetch = [&](int buf) {    // the next tile
-    const uint32_t to = base + buf * (NF * 1024);
-    frags_to_lds<2 * KC>(kr, to, lane16);
-    kr += 2 * KC * 1024;
-    frags_to_lds<2 * KC>(vr, to + F_V * 1024, lane16);
-    vr += 2 * KC * 1024;
-    frags_to_lds<4 * DB>(kc, to + F_KC * 1024, lane16);
-    kc += 4 * DB * 1024;
-    if (w < kSideFrags) frags_to_lds<4>(side_p, to + F_SIDE * 1024, lane16);
-    side_p += kSide * kTile * 4;
-  };
-
-  f32x16 dq[DB];
-#pragma unroll
-  for (int d = 0; d < DB; ++d) dq[d] = f32x16{};
-  int cq = kUnset;
-  const float icap = RICH && a.cap > 0 ? 1.0f / a.cap : 0.0f;
-  if (t0 < t1) fetch(0);
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1, j0 = t * kTile;
-    loads_done();
-    __syncthreads();
-    if (t + 1 < t1) fetch(buf ^ 1);
-    const _Float16* L = lds + buf * (NF * kFrag);
-    const float* side = (const float*)(L + F_SIDE * kFrag);
-    const TileInfo kt = side_info(side, 0), vt = side_info(side, 1);
-    if (__builtin_expect(!any_seen(s, me, kt, j0), 0)) continue;
-    f32x16 x, y;
-    x = scores<KC>(L, 0, qh, ql);
-    y = scores<KC>(L, F_V, gh, gl);
-    if (__builtin_expect(kt.uneven, 0)) per_row(x, side + KS_RELK * kTile);
-    if (__builtin_expect(vt.uneven, 0)) per_row(y, side + KS_RELV * kTile);
-    const float unit = a.scale * pow2(-qe) * kt.inv, yunit = pow2(-ge) * vt.inv;
-    const bool cap = RICH && a.cap > 0;
-    if (cap) tanh_all(x, unit * icap);
-    const float f = (cap ? a.cap : unit) * kLog2e;
-#pragma unroll
-    for (int q = 0; q < 16; ++q) {
-      float off = lse;
-      if (RICH && a.slopes) off = fmaf(slope, fabsf((float)(p - (j0 + 8 * (q / 4) + 4 * h + q % 4))), lse);
-      y[q] = __builtin_amdgcn_exp2f(fmaf(x[q], f, -off)) * fmaf(y[q], yunit, -dot);
-      if (cap) y[q] *= fmaf(-x[q], x[q], 1.0f);
-    }
-    if (__builtin_expect(!all_seen(s, me, kt, j0), 0)) {
-      if (s.doc) {
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const f32x4 dj = *(const f32x4*)(side + KS_DOC * kTile + 8 * q4 + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[4 * q4 + e] = __float_as_int(dj[e]) == doc && doc >= 0 ? y[4 * q4 + e] : 0.0f;
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < 16; ++q) y[q] = j0 + 8 * (q / 4) + 4 * h + q % 4 < below ? y[q] : 0.0f;
-    }
-    if (__builtin_expect(kt.uneven, 0)) per_row(y, side + KS_RELK * kTile);
-    float change = 1;
-    const int e = fit_unit(cq, largest(y), exponent(kt.scale), &change);
-    rescale<DB>(dq, change);
-    accumulate<DB>(dq, y, pow2(e), L, F_KC);
-  }
-  if (valid)
-    store_row<DB>(dq_row(A, split, slab, b, head, r, i), dq, cq, a.scale, a.D, A.qsplits > 1 ? a.D % 4 == 0 : A.wide);
-}
-
-// The same by 16 rows a wavefront, 8 wavefronts a block, for head sizes above 64 (see attend_grad_kv16): 4096 causal
-// rows of 16 heads of 128 in 390 us instead of 470, 32 slabs of 777 rows of 96 in 54 us instead of 64.
-template <int DP, bool RICH>
-__global__ __launch_bounds__(512) void attend_grad_q16(GradArgs A) {
+__global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   constexpr int N = DP / 32, F = 4 * N, F_V = F, F_KC = 2 * F, F_SIDE = 3 * F, NF = F_SIDE + kSideFrags;
   __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
   __shared__ int range[5];
@@ -864,7 +592,7 @@ __global__ __launch_bounds__(512) void attend_grad_q16(GradArgs A) {
     t1 = min(t0 + each, t1);
   }
   if (__builtin_expect(range_.odd, 0)) {
-    plain_dq<16>(A, s, split, slab, b, hk, row0, t0 * kTile, t1 * kTile);
+    plain_dq(A, s, split, slab, b, hk, row0, t0 * kTile, t1 * kTile);
     return;
   }
 
@@ -995,19 +723,10 @@ template <int DP, bool RICH>
 void run_grad(const GradArgs& A, int slabs, hipStream_t st) {
   const AttendGradDesc& g = A.g;
   const dim3 keys(place_grid(slabs, (int64_t)A.blocks * A.splits));
-  if constexpr (DP <= 64) {
-    if (g.dk.p && g.dv.p) klaunch(attend_grad_kv<DP, RICH, 3>, keys, dim3(256), 0, st, A);
-    else if (g.dk.p) klaunch(attend_grad_kv<DP, RICH, 1>, keys, dim3(256), 0, st, A);
-    else if (g.dv.p) klaunch(attend_grad_kv<DP, RICH, 2>, keys, dim3(256), 0, st, A);
-  } else {
-    if (g.dk.p && g.dv.p) klaunch(attend_grad_kv16<DP, RICH, 3>, keys, dim3(512), 0, st, A);
-    else if (g.dk.p) klaunch(attend_grad_kv16<DP, RICH, 1>, keys, dim3(512), 0, st, A);
-    else if (g.dv.p) klaunch(attend_grad_kv16<DP, RICH, 2>, keys, dim3(512), 0, st, A);
-  }
-  if (!g.dq.p) return;
-  const dim3 rows(place_grid(slabs, (int64_t)((A.M + 127) / 128) * A.qsplits));
-  if constexpr (DP <= 64) klaunch(attend_grad_q<DP, RICH>, rows, dim3(256), 0, st, A);
-  else klaunch(attend_grad_q16<DP, RICH>, rows, dim3(512), 0, st, A);
+  if (g.dk.p && g.dv.p) klaunch(attend_grad_kv<DP, RICH, 3>, keys, dim3(512), 0, st, A);
+  else if (g.dk.p) klaunch(attend_grad_kv<DP, RICH, 1>, keys, dim3(512), 0, st, A);
+  else if (g.dv.p) klaunch(attend_grad_kv<DP, RICH, 2>, keys, dim3(512), 0, st, A);
+  if (g.dq.p) klaunch(attend_grad_q<DP, RICH>, dim3(place_grid(slabs, (int64_t)((A.M + 127) / 128) * A.qsplits)), dim3(512), 0, st, A);
 }
 template <int DP>
 void run_grad(const GradArgs& A, int slabs, hipStream_t st) {
@@ -1032,7 +751,7 @@ void attend_grad(const AttendGradDesc& g, void* work, hipStream_t st) {
   k.n = 4;
   k.Hk = a.Hk;
   k.wide = wide;
-  k.narrow = p.DP > 64;
+  k.narrow = true;
   k.a = a;
   float *qs = (float*)(w + p.qside), *ks = (float*)(w + p.kside);
   k.job[0] = {a.q, a.D, p.G, p.M, p.qtiles, half(p.qr), half(p.qc), info(p.qi), true, qs, QS_RELQ, false, false, {}};
