@@ -165,14 +165,14 @@ __device__ __forceinline__ float* result_row(const TilesArgs& A, int split, int 
   return a.y.p ? a.y.p + b * a.y.b + head * a.y.h + (int64_t)i * a.y.t : nullptr;
 }
 
-// A wavefront's rows [row0, row0 + 32) over keys [j0, j1) in plain f32.
+// A wavefront's rows [row0, row0 + 16) over keys [j0, j1) in plain f32.
 __device__ __forceinline__ void plain_rows(const TilesArgs& A, const Sight& s, int split, int slab, int b, int hk, int row0, int j0, int j1) {
   const AttendDesc& a = A.a;
   const int lane = threadIdx.x & 63, G = (int)A.group.d;
   const float* k = a.k.p + b * a.k.b + hk * a.k.h;
   const float* v = a.v.p + b * a.v.b + hk * a.v.h;
 #pragma unroll 1
-  for (int r = row0; r < min(row0 + kTile, A.M); ++r) {
+  for (int r = row0; r < min(row0 + 16, A.M); ++r) {
     const int i = r / G, head = hk * G + r % G, p = s.first + i, doc = doc_at(s, p), end = min(j1, sees_below(s, p));
     const float* q = a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t;
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
@@ -207,12 +207,12 @@ __device__ __forceinline__ void plain_rows(const TilesArgs& A, const Sight& s, i
 }
 
 template <int DP, bool CAP, bool SLOPES>
-__global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
-  constexpr int KC = DP / 16, DB = DP / 32, NV = 4 * DB + kSideFrags;   // LDS: k, k, v and side, v and side
-  __shared__ __align__(16) _Float16 lds[(4 * KC + 2 * NV) * kFrag];
+__global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
+  constexpr int N = DP / 32, F = 4 * N, F_V = F, F_SIDE = 2 * F, NF = F_SIDE + kSideFrags;
+  __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
   __shared__ int range[5];
   const AttendDesc& a = A.a;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g4 = lane >> 4, l = lane & 15;
   int slab, item;
   place(blockIdx.x, a.B * a.Hk, slab, item);
   if (item >= A.blocks * A.splits) return;
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   const int tiles = (a.Tk + kTile - 1) / kTile;
 
   // this lane's query
-  const int row0 = blk * 128 + w * kTile, r = row0 + l;
+  const int row0 = blk * 128 + w * 16, r = row0 + l;
   const bool valid = r < A.M;
   const int i = (int)fastdiv((uint32_t)min(r, A.M - 1), A.group), g = min(r, A.M - 1) - i * G, head = hk * G + g;
   const int p = s.first + i, doc = doc_at(s, p), below = sees_below(s, p);
@@ -230,12 +230,12 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
   // the wavefront's rows, and the block's key tiles
   Span me;
   me.pmin = s.first + (int)fastdiv((uint32_t)min(row0, A.M - 1), A.group);
-  me.pmax = s.first + (int)fastdiv((uint32_t)min(row0 + kTile - 1, A.M - 1), A.group);
+  me.pmax = s.first + (int)fastdiv((uint32_t)min(row0 + 15, A.M - 1), A.group);
   me.dmin = valid && doc >= 0 ? doc : INT32_MAX;
   me.dmax = valid && doc >= 0 ? doc : INT32_MIN;
   if (s.doc) {
 #pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
+    for (int o = 1; o < 16; o *= 2) {
       me.dmin = min(me.dmin, __shfl_xor(me.dmin, o));
       me.dmax = max(me.dmax, __shfl_xor(me.dmax, o));
     }
@@ -262,150 +262,98 @@ __global__ __launch_bounds__(256, 2) void attend_tiles(TilesArgs A) {
     return;
   }
 
-  const float* qrow = a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t;
-  half8 qh[KC], ql[KC];
-  const int qe = load_rows<KC>(qrow, valid, a.D, A.wide, qh, ql);
+  half8 qh[N], ql[N];
+  const int qe = load_rows16<N>(a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t, valid, a.D, A.wide, qh, ql);
   const float slope = SLOPES ? a.slopes[head] * kLog2e : 0.0f;
-  const int64_t tile0 = (int64_t)slab * tiles;
+  const int64_t tile0 = (int64_t)slab * tiles + t0;
   const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
-  const char* kf = (const char*)(A.kf + (tile0 + t0) * (2 * KC * kFrag)) + w * 1024;
-  const char* vf = (const char*)(A.vf + (tile0 + t0) * (4 * DB * kFrag)) + w * 1024;
-  const char* side_p = (const char*)(A.side + (tile0 + t0) * (kSide * kTile)) + w * 1024;
-  auto fetch_k = [&](int buf) {    // the next tile of each
-    frags_to_lds<2 * KC>(kf, base + buf * (2 * KC * 1024), lane16);
-    kf += 2 * KC * 1024;
-  };
-  auto fetch_v = [&](int buf) {
-    const uint32_t to = base + (4 * KC + buf * NV) * 1024;
-    frags_to_lds<4 * DB>(vf, to, lane16);
-    vf += 4 * DB * 1024;
-    if (w < kSideFrags) frags_to_lds<4>(side_p, to + 4 * DB * 1024, lane16);
+  const char* kf = (const char*)(A.kf + tile0 * (F * kFrag)) + w * 1024;
+  const char* vf = (const char*)(A.vf + tile0 * (F * kFrag)) + w * 1024;
+  const char* side_p = (const char*)(A.side + tile0 * (kSide * kTile)) + w * 1024;
+  auto fetch = [&](int buf) {      // the next tile
+    const uint32_t to = base + buf * (NF * 1024);
+    frags_by_eight<F>(kf, to, lane16, w);
+    frags_by_eight<F>(vf, to + F_V * 1024, lane16, w);
+    frags_by_eight<kSideFrags>(side_p, to + F_SIDE * 1024, lane16, w);
+    kf += F * 1024;
+    vf += F * 1024;
     side_p += kSide * kTile * 4;
   };
 
-  f32x16 acc[DB];
+  f32x4 acc[2 * N];
 #pragma unroll
-  for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
-  float m = kNone, sum = 0;        // running maximum (log2) and this lane half's sum
+  for (int d = 0; d < 2 * N; ++d) acc[d] = f32x4{};
+  float m = kNone, sum = 0;        // running maximum (log2) and this lane's part of the sum
   int ce = kUnset;                 // acc is in units of 2^-ce
   const float icap = CAP ? 1.0f / a.cap : 0.0f;
-  // A tile's scores are computed a tile ahead, while the weights of the tile before are: k runs a tile ahead of v.
-  f32x16 next = {};
-  if (t0 < t1) {
-    fetch_k(0);
-    fetch_v(0);
-    if (t0 + 1 < t1) fetch_k(1);
-    loads_done();
-    __syncthreads();
-    next = scores<KC>(lds, 0, qh, ql);
-  }
-  const float capped = CAP ? a.cap * kLog2e : 0.0f;
+  if (t0 < t1) fetch(0);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, j0 = t * kTile;
     loads_done();
     __syncthreads();
-    if (t + 1 < t1) fetch_v(buf ^ 1);
-    if (t + 2 < t1) fetch_k(buf);
-    const _Float16 *K = lds + (buf ^ 1) * (2 * KC * kFrag), *V = lds + (4 * KC + buf * NV) * kFrag;
-    const float* side = (const float*)(V + 4 * DB * kFrag);
+    if (t + 1 < t1) fetch(buf ^ 1);
+    const _Float16* L = lds + buf * (NF * kFrag);
+    const float* side = (const float*)(L + F_SIDE * kFrag);
     const TileInfo kt = side_info(side, 0), vt = side_info(side, 1);
-    f32x16 x = next;               // transposed: register r of this lane is key j0 + 8 (r / 4) + 4 h + r % 4
-    if (__builtin_expect(!any_seen(s, me, kt, j0), 0)) {
-      next = scores<KC>(K, 0, qh, ql);
-      continue;
-    }
+    if (__builtin_expect(!any_seen(s, me, kt, j0), 0)) continue;
+    float x[8];                    // transposed: element q of this lane is key j0 + 16 (q / 4) + 4 g4 + q % 4
+    scores16<N>(L, 0, qh, ql, x);
     const float unit = a.scale * pow2(-qe) * kt.inv;
-    float top = kNone, most = 0;
-    if (CAP)
+    if (__builtin_expect(kt.uneven, 0)) per_row16(x, side + KS_RELK * kTile, g4);
+    float f = unit * kLog2e;       // the score is f x, in log2
+    if (CAP) {
+      tanh_all16(x, unit * icap);
+      f = a.cap * kLog2e;
+    }
+    if (SLOPES) {
 #pragma unroll
-      for (int q = 0; q < 16; ++q) most = fmaxf(most, fabsf(x[q]));
-    const float u = CAP ? unit * icap : unit * kLog2e;
-    float change = 1, big;
-    auto grow = [&](float top) {   // the running maximum, and what acc and sum take for it
-      // It moves only when it grows by more than 2^8 (or from nothing), so that most tiles leave acc alone: weights then
-      // reach 2^8 instead of 1.
-      const bool up = top > m + 8 || (m == kNone && top > kNone);
-      const float to = up ? top : m, keep = up ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
-      m = to;
-      sum *= keep;
-      // what acc held has shrunk: so may its unit
-      const int shrunk = up && keep > 0 && ce != kUnset ? min(-exponent(keep) - 1, 100) : 0;
-      change = keep * pow2(shrunk);
-      ce += shrunk;
-    };
-    if (__builtin_expect(all_seen(s, me, kt, j0) && !kt.uneven && !vt.uneven && (!CAP || !__any(most * u >= kFlat)), 1)) {
-      // the common tile, without a branch: the next scores' products between the vector work
-      const float f = SLOPES ? 1.0f : CAP ? capped : u;
-      float part = 0;
-      scores_woven<KC, 32>(next, K, 0, qh, ql, [&](int i) {
-        const int q = i % 16;
-        if (i < 16) {              // scores, and their maximum
-          if (CAP) x[q] = tanh_flat(x[q] * u);
-          if (SLOPES) x[q] = x[q] * (CAP ? capped : u) - slope * fabsf((float)(p - (j0 + 8 * (q / 4) + 4 * h + q % 4)));
-          top = fmaxf(top, x[q]);
-        } else {
-          if (i == 16) {
-            top = halves_max(top) * f;
-            grow(top);
-          }
-          x[q] = __builtin_amdgcn_exp2f(fmaf(x[q], f, -m));
-          part += x[q];
-        }
-      });
-      sum += part;
-      big = __builtin_amdgcn_exp2f(top - m);
-    } else {
-      next = scores<KC>(K, 0, qh, ql);
-      if (kt.uneven) per_row(x, side + KS_RELK * kTile);
-      float f = u;                 // the score is f x, in log2
-      if (CAP) {
-        tanh_all(x, u);
-        f = capped;
+      for (int q = 0; q < 8; ++q) x[q] = x[q] * f - slope * fabsf((float)(p - (j0 + 16 * (q / 4) + 4 * g4 + q % 4)));
+      f = 1;
+    }
+    if (__builtin_expect(!all_seen(s, me, kt, j0), 0)) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const int z = 16 * (q / 4) + 4 * g4 + q % 4;
+        const bool ok = j0 + z < below && (!s.doc || (doc >= 0 && __float_as_int(side[KS_DOC * kTile + z]) == doc));
+        x[q] = ok ? x[q] : kNone;
       }
-      if (SLOPES) {
+    }
+    float top = x[0];
 #pragma unroll
-        for (int q = 0; q < 16; ++q) x[q] = x[q] * f - slope * fabsf((float)(p - (j0 + 8 * (q / 4) + 4 * h + q % 4)));
-        f = 1;
-      }
-      if (s.doc) {
+    for (int q = 1; q < 8; ++q) top = fmaxf(top, x[q]);
+    top = groups_max(top) * f;
+    // The running maximum moves only when it grows by more than 2^8 (or from nothing), so that most tiles leave acc alone:
+    // weights then reach 2^8 instead of 1.
+    const bool up = top > m + 8 || (m == kNone && top > kNone);
+    const float to = up ? top : m, keep = up ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
+    m = to;
+    // what acc held has shrunk: so may its unit
+    const int shrunk = up && keep > 0 && ce != kUnset ? min(-exponent(keep) - 1, 100) : 0;
+    float change = keep * pow2(shrunk), part = 0;
+    ce += shrunk;
+    const float off = m == kNone ? 0.0f : m;
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const f32x4 dj = *(const f32x4*)(side + KS_DOC * kTile + 8 * q4 + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[4 * q4 + e] = __float_as_int(dj[e]) == doc && doc >= 0 ? x[4 * q4 + e] : kNone;
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < 16; ++q) x[q] = j0 + 8 * (q / 4) + 4 * h + q % 4 < below ? x[q] : kNone;
-      top = x[0];
-#pragma unroll
-      for (int q = 1; q < 16; ++q) top = fmaxf(top, x[q]);
-      top = halves_max(top) * f;
-      grow(top);
-      const float off = m == kNone ? 0.0f : m;
-#pragma unroll
-      for (int q = 0; q < 16; ++q) x[q] = __builtin_amdgcn_exp2f(fmaf(x[q], f, -off));
-      float part = 0;
-#pragma unroll
-      for (int q = 0; q < 16; ++q) part += x[q];
-      sum += part;
-      big = __builtin_amdgcn_exp2f(top - off);
-      if (vt.uneven) {
-        per_row(x, side + KS_RELV * kTile);
-        big = largest(x);
-      }
+    for (int q = 0; q < 8; ++q) {
+      x[q] = __builtin_amdgcn_exp2f(fmaf(x[q], f, -off));
+      part += x[q];
+    }
+    sum = fmaf(sum, keep, part);
+    float big = __builtin_amdgcn_exp2f(top - off);
+    if (__builtin_expect(vt.uneven, 0)) {
+      per_row16(x, side + KS_RELV * kTile, g4);
+      big = largest16(x);
     }
     const int e = fit_unit(ce, big, exponent(vt.scale), &change);
-    rescale<DB>(acc, change);
-    accumulate<DB>(acc, x, pow2(e), V, 0);
+    rescale16(acc, change);
+    accumulate16(acc, x, pow2(e), L, F_V);
   }
 
-  sum = halves_sum(sum);
+  sum = groups_sum(sum);
   if (!valid) return;
   const bool none = sum == 0;      // not m: a visible NaN leaves no maximum
   const float out = none ? 0.0f : 1.0f / sum;
-  float* y = result_row(A, split, slab, b, head, r, i, m + __builtin_amdgcn_logf(sum), none, h == 0);
-  if (y) store_row<DB>(y, acc, ce, out, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide);
+  float* y = result_row(A, split, slab, b, head, r, i, m + __builtin_amdgcn_logf(sum), none, g4 == 0);
+  if (y) store_row16(y, acc, ce, out, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide, g4);
 }
 
 // ---- few rows --------------------------------------------------------------------------------------
@@ -679,10 +627,10 @@ Plan plan(const AttendDesc& a) {
 
 template <int DP>
 void run_tiles(const TilesArgs& t, unsigned grid, hipStream_t st) {
-  if (t.a.cap > 0 && t.a.slopes) klaunch(attend_tiles<DP, true, true>, dim3(grid), dim3(256), 0, st, t);
-  else if (t.a.cap > 0) klaunch(attend_tiles<DP, true, false>, dim3(grid), dim3(256), 0, st, t);
-  else if (t.a.slopes) klaunch(attend_tiles<DP, false, true>, dim3(grid), dim3(256), 0, st, t);
-  else klaunch(attend_tiles<DP, false, false>, dim3(grid), dim3(256), 0, st, t);
+  if (t.a.cap > 0 && t.a.slopes) klaunch(attend_tiles<DP, true, true>, dim3(grid), dim3(512), 0, st, t);
+  else if (t.a.cap > 0) klaunch(attend_tiles<DP, true, false>, dim3(grid), dim3(512), 0, st, t);
+  else if (t.a.slopes) klaunch(attend_tiles<DP, false, true>, dim3(grid), dim3(512), 0, st, t);
+  else klaunch(attend_tiles<DP, false, false>, dim3(grid), dim3(512), 0, st, t);
 }
 template <int E, int R>
 void run_few(const FewArgs& f, bool wide, int slabs, hipStream_t st) {
@@ -732,6 +680,7 @@ void attend(const AttendDesc& a, void* work, hipStream_t st) {
     k.n = 2;
     k.Hk = a.Hk;
     k.wide = wide;
+    k.narrow = true;
     k.a = a;
     float* side = (float*)(w + p.side);
     k.job[0] = {a.k, a.D, 1, a.Tk, p.tiles, (_Float16*)(w + p.kf), nullptr, (TileInfo*)(w + p.ki), false, side, KS_RELK, false, true, {}};

@@ -105,198 +105,6 @@ __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, in
   }
 }
 
-// ---- products of 16 columns ------------------------------------------------------------------------
-//
-// A wavefront's own rows (keys, or query rows) are the columns of 16 x 16 x 32 products: at head size 128 their operands and
-// gradients then leave room for two wavefronts a SIMD, where 32 columns took the registers of one, which waited for every
-// product. Fragments are read from LDS twice as often for it.
-
-__device__ __forceinline__ float groups_max(float x) {   // over lanes l % 16 + 0, 16, 32, 48
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-}
-// B fragments of 16 rows (lane l: row l % 16), each row with its own power of two; returns its exponent.
-template <int N>
-__device__ __forceinline__ int load_rows16(const float* row, bool valid, int n, bool wide, half8 (&hi)[N], half8 (&lo)[N]) {
-  const int g = (threadIdx.x >> 4) & 3;
-  float x[N][8], m = 0;
-#pragma unroll
-  for (int c = 0; c < N; ++c) {
-    const int d = 32 * c + 8 * g;
-    if (wide) {
-      f32x4 u = {}, w = {};
-      if (valid && d < n) {
-        u = *(const f32x4*)(row + d);
-        w = *(const f32x4*)(row + d + 4);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { x[c][i] = u[i]; x[c][4 + i] = w[i]; }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[c][i] = valid && d + i < n ? row[d + i] : 0.0f;
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < N; ++c)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(x[c][i]));
-  m = groups_max(m);
-  const int e = m > 0 ? min(14 - exponent(m), 126) : 0;
-  const float s = pow2(e);
-#pragma unroll
-  for (int c = 0; c < N; ++c) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[c][i] *= s;
-    split8(x[c], hi[c], lo[c]);
-  }
-  return e;
-}
-// N fragments by eight wavefronts, wavefront w's at src and lds + 1024 w.
-template <int N>
-__device__ __forceinline__ void frags_by_eight(const char* src, uint32_t lds, uint32_t lane16, int w) {
-#pragma unroll
-  for (int f = 0; f < N / 8; ++f) frags_to_lds<4>(src + f * 8192, lds + f * 8192, lane16);
-  if (N % 8 && w < N % 8) frags_to_lds<4>(src + N / 8 * 8192, lds + N / 8 * 8192, lane16);
-}
-// x = A fragments (N chunks of 32 features, two blocks of 16 rows each, from fragment f0) times B fragments; a chunk's
-// fragments are read while the chunk before is multiplied.
-template <int N>
-__device__ __forceinline__ void scores16(const _Float16* L, int f0, const half8 (&bh)[N], const half8 (&bl)[N], float (&x)[8]) {
-  f32x4 z[2] = {};
-  half8 a[2][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) a[0][i] = frag(L, f0 + i);
-#pragma unroll
-  for (int c = 0; c < N; ++c) {
-    const half8* u = a[c & 1];
-    if (c + 1 < N)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[(c + 1) & 1][i] = frag(L, f0 + 4 * c + 4 + i);
-    z[0] = mfma16(u[1], bh[c], z[0]);
-    z[1] = mfma16(u[3], bh[c], z[1]);
-    z[0] = mfma16(u[0], bl[c], z[0]);
-    z[1] = mfma16(u[2], bl[c], z[1]);
-    z[0] = mfma16(u[0], bh[c], z[0]);
-    z[1] = mfma16(u[2], bh[c], z[1]);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-#pragma unroll
-  for (int q = 0; q < 8; ++q) x[q] = z[q / 4][q % 4];
-}
-// Both products of a pair, step by step in turn.
-template <int N>
-__device__ __forceinline__ void pair16(const _Float16* L, int f0, const half8 (&bh)[N], const half8 (&bl)[N], float (&x)[8], int f1,
-                                       const half8 (&ch)[N], const half8 (&cl)[N], float (&y)[8]) {
-  f32x4 z[4] = {};
-  half8 a[2][8];
-  auto read = [&](int c) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[c & 1][i] = frag(L, f0 + 4 * c + i);
-      a[c & 1][4 + i] = frag(L, f1 + 4 * c + i);
-    }
-  };
-  read(0);
-#pragma unroll
-  for (int c = 0; c < N; ++c) {
-    const half8* u = a[c & 1];
-    if (c + 1 < N) read(c + 1);
-    z[0] = mfma16(u[1], bh[c], z[0]);
-    z[1] = mfma16(u[3], bh[c], z[1]);
-    z[2] = mfma16(u[5], ch[c], z[2]);
-    z[3] = mfma16(u[7], ch[c], z[3]);
-    z[0] = mfma16(u[0], bl[c], z[0]);
-    z[1] = mfma16(u[2], bl[c], z[1]);
-    z[2] = mfma16(u[4], cl[c], z[2]);
-    z[3] = mfma16(u[6], cl[c], z[3]);
-    z[0] = mfma16(u[0], bh[c], z[0]);
-    z[1] = mfma16(u[2], bh[c], z[1]);
-    z[2] = mfma16(u[4], ch[c], z[2]);
-    z[3] = mfma16(u[6], ch[c], z[3]);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-#pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    x[q] = z[q / 4][q % 4];
-    y[q] = z[2 + q / 4][q % 4];
-  }
-}
-// acc += A fragments (N blocks of 16 features, from fragment f0) times the split of x * scale, read as above.
-template <int N>
-__device__ __forceinline__ void accumulate16(f32x4 (&acc)[N], const float (&x)[8], float scale, const _Float16* L, int f0) {
-  half8 a[2][4], bh, bl;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) a[0][i] = frag(L, f0 + i);
-  float z[8];
-#pragma unroll
-  for (int q = 0; q < 8; ++q) z[q] = x[q] * scale;
-  split8(z, bh, bl);
-#pragma unroll
-  for (int d = 0; d < N; d += 2) {
-    const half8* u = a[d / 2 & 1];
-    if (d + 2 < N)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[(d / 2 + 1) & 1][i] = frag(L, f0 + 2 * d + 4 + i);
-    acc[d] = mfma16(u[1], bh, acc[d]);
-    acc[d + 1] = mfma16(u[3], bh, acc[d + 1]);
-    acc[d] = mfma16(u[0], bl, acc[d]);
-    acc[d + 1] = mfma16(u[2], bl, acc[d + 1]);
-    acc[d] = mfma16(u[0], bh, acc[d]);
-    acc[d + 1] = mfma16(u[2], bh, acc[d + 1]);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-}
-template <int N>
-__device__ __forceinline__ void rescale16(f32x4 (&acc)[N], float change) {
-  if (__builtin_expect(!__any(change != 1), 1)) return;
-#pragma unroll
-  for (int d = 0; d < N; ++d)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) acc[d][q] *= change;
-}
-__device__ __forceinline__ void per_row16(float (&x)[8], const float* rel, int g) {
-#pragma unroll
-  for (int q = 0; q < 8; ++q) x[q] *= rel[16 * (q / 4) + 4 * g + q % 4];
-}
-__device__ __forceinline__ float largest16(const float (&x)[8]) {
-  float m = 0;
-#pragma unroll
-  for (int q = 0; q < 8; ++q) m = fmaxf(m, fabsf(x[q]));
-  return groups_max(m);
-}
-// x = tanh(x u), all 8; the polynomial alone where no lane needs more
-__device__ __forceinline__ void tanh_all16(float (&x)[8], float u) {
-  float m = 0;
-#pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    x[q] *= u;
-    m = fmaxf(m, fabsf(x[q]));
-  }
-  if (__any(m >= kFlat)) {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) x[q] = tanh_of(x[q]);
-  } else {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) x[q] = tanh_flat(x[q]);
-  }
-}
-template <int N>
-__device__ __forceinline__ void store_row16(float* row, const f32x4 (&acc)[N], int c, float scale, int n, bool wide, int g) {
-#pragma unroll
-  for (int d = 0; d < N; ++d) {
-    const int at = 16 * d + 4 * g;
-    f32x4 v;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_ldexpf(acc[d][e], -c) * scale;
-    if (wide) {
-      if (at < n) *(f32x4*)(row + at) = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) if (at + e < n) row[at + e] = v[e];
-    }
-  }
-}
-
 // Eight wavefronts of 16 keys. WHAT: 1 for dk, 2 for dv, 3 for both in one walk. Up to head size 64 two blocks share a CU. Both
 // gradients of 4096 causal rows of 16 heads of 128: 664 us (by 32 keys 990, in walks of their own); of 8 heads of 64: 193 us
 // (205); of 8 x 1000 rows of 8 heads of 32: 76 us (66), in documents of 50: 38 us (44).
