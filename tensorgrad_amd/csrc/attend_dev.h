@@ -6,14 +6,15 @@
 // lo part, an error of 2^-40 of the largest. Three products at the f16 rate stand for one f32 product: 443 TFLOP/s of a
 // measured 1329, where the f32 matrix instruction reaches 154.
 //
-// Fragments of a 32 x 32 x 16 product: lane l holds row (A) or column (B) l % 32 and k = 8 (l / 32) + 0..7; a result's
-// register r holds row 8 (r / 4) + 4 (l / 32) + r % 4 of column l % 32. One fragment of a wavefront is 1 KiB. The scores'
-// registers 8 s .. 8 s + 7 are the B fragment of the next product's k step s as they stand, if that product's A fragments
-// take their k in the same order: rows 16 s + 4 h + 0..3 and 16 s + 8 + 4 h + 0..3 for lane half h.
+// Fragments of a 16 x 16 x 32 product: lane l holds row (A) or column (B) l % 16 and k = 8 g + 0..7, g = l / 16; a result's
+// register r holds row 4 g + r of column l % 16. One fragment of a wavefront is 1 KiB. A wavefront's own 16 rows (queries, or
+// keys) are the columns, so that a lane's results belong to ONE of them: running maxima and sums are lane arithmetic and two
+// exchanges. Two blocks of scores, tile rows 0..15 and 16..31, are the next product's B fragment as they stand, if its A
+// fragments take their k in the same order: rows 4 g + 0..3, then 16 + 4 g + 0..3.
 //
-// Of a 16 x 16 x 32 product: lane l holds row or column l % 16 and k = 8 g + 0..7, g = l / 16; result register r holds row
-// 4 g + r of column l % 16. Two such blocks of scores, rows 0..15 and 16..31, are the B fragment of one k step: rows
-// 4 g + 0..3 and 16 + 4 g + 0..3.
+// 32 columns a wavefront (32 x 32 x 16) would read fragments from LDS half as often, but their operands and results took the
+// registers of a SIMD's only wavefront, or of two, which then waited for every product: slower in every case but one
+// (gradients of head size 32 without documents, by 4 %), twice as slow for the gradients of head size 128.
 #pragma once
 #include "kernels.h"
 #include "sequence.h"
@@ -25,12 +26,11 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 32;          // rows of a tile
 constexpr int kFrag = 512;         // halves of a fragment (1 KiB)
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNone = -INFINITY;
 
 // What the kernels need to know of a packed tile. One power of two serves all its rows, that of the largest, unless they
@@ -78,19 +78,7 @@ __device__ __forceinline__ void split8(const float* x, half8& hi, half8& lo) {
   lo = __builtin_bit_cast(half8, b);
 }
 
-__device__ __forceinline__ f32x16 mfma(half8 a, half8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-
-__device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-
-// Over lanes l and l ^ 32, which hold the two halves of a row.
-__device__ __forceinline__ float halves_max(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float halves_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
+__device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 // tanh. Up to kFlat by an odd polynomial (least squares in the relative error: 0.16 * 2^-24 off, 1.4 with f32's roundings);
 // above by 1 - e^-2x, which does not cancel there.
@@ -105,23 +93,6 @@ __device__ __forceinline__ float tanh_of(float x) {
   const float far = copysignf((1 - e) * __builtin_amdgcn_rcpf(1 + e), x);
   return z < kFlat ? tanh_flat(x) : far;
 }
-// x = tanh(x u), all 16; the polynomial alone where no lane needs more
-__device__ __forceinline__ void tanh_all(f32x16& x, float u) {
-  float m = 0;
-#pragma unroll
-  for (int q = 0; q < 16; ++q) {
-    x[q] *= u;
-    m = fmaxf(m, fabsf(x[q]));
-  }
-  if (__any(m >= kFlat)) {
-#pragma unroll
-    for (int q = 0; q < 16; ++q) x[q] = tanh_of(x[q]);
-  } else {
-#pragma unroll
-    for (int q = 0; q < 16; ++q) x[q] = tanh_flat(x[q]);
-  }
-}
-
 // What the queries of one batch entry see, wave-uniform.
 struct Sight {
   int n, first, prefix;            // keys that are there; position of query 0; keys every query sees
@@ -161,15 +132,17 @@ __device__ __forceinline__ bool all_seen(const Sight& s, const Span& q, const Ti
   return !s.doc || (k.same && q.same && k.dmin == q.dmin);
 }
 
-// Fragments from memory straight into LDS (lane l's 16 bytes land at base + 16 l), N of 1 KiB by four wavefronts, wavefront
-// w's at src and lds + 1024 w; N is a multiple of 4. In inline assembly, so that the compiler does not drain every load
-// before the next LDS read; the kernels wait (vmcnt) and meet (barrier) themselves.
+// N fragments from memory straight into LDS (lane l's 16 bytes land at base + 16 l) by eight wavefronts, wavefront w's at src
+// and lds + 1024 w. In inline assembly, so that the compiler does not drain every load before the next LDS read; the kernels
+// wait (vmcnt) and meet (barrier) themselves.
+__device__ __forceinline__ void frag_to_lds(const char* src, uint32_t lds, uint32_t lane16) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane16), "s"(src), "{m0}"(lds));
+}
 template <int N>
-__device__ __forceinline__ void frags_to_lds(const char* src, uint32_t lds, uint32_t lane16) {
-  static_assert(N % 4 == 0, "whole rounds of four wavefronts");
+__device__ __forceinline__ void frags_to_lds(const char* src, uint32_t lds, uint32_t lane16, int w) {
 #pragma unroll
-  for (int f = 0; f < N / 4; ++f)
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane16), "s"(src + f * 4096), "{m0}"(lds + f * 4096));
+  for (int f = 0; f < N / 8; ++f) frag_to_lds(src + f * 8192, lds + f * 8192, lane16);
+  if (N % 8 && w < N % 8) frag_to_lds(src + N / 8 * 8192, lds + N / 8 * 8192, lane16);
 }
 __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
@@ -179,45 +152,6 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 __device__ __forceinline__ float finite_abs(float x) {
   x = fabsf(x);
   return x < INFINITY ? x : 0.0f;
-}
-
-// B fragments of 32 rows (lane l: row l % 32), each row with its own power of two; returns its exponent. wide: rows are
-// 16-byte aligned and n a multiple of 8.
-template <int KC>
-__device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bool wide, half8 (&hi)[KC], half8 (&lo)[KC]) {
-  const int h = (threadIdx.x >> 5) & 1;
-  float x[KC][8];
-#pragma unroll
-  for (int c = 0; c < KC; ++c) {
-    const int d = 16 * c + 8 * h;
-    if (wide) {
-      f32x4 u = {}, w = {};
-      if (valid && d < n) {
-        u = *(const f32x4*)(row + d);
-        w = *(const f32x4*)(row + d + 4);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { x[c][i] = u[i]; x[c][4 + i] = w[i]; }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[c][i] = valid && d + i < n ? row[d + i] : 0.0f;
-    }
-  }
-  float m = 0;
-#pragma unroll
-  for (int c = 0; c < KC; ++c)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(x[c][i]));   // the others stay what they are
-  m = halves_max(m);
-  const int e = m > 0 ? min(14 - exponent(m), 126) : 0;
-  const float s = pow2(e);
-#pragma unroll
-  for (int c = 0; c < KC; ++c) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[c][i] *= s;
-    split8(x[c], hi[c], lo[c]);
-  }
-  return e;
 }
 
 // Sums over several tiles in one accumulator: the weights (f16 parts of x 2^e) times a tile packed at 2^t are in units of
@@ -234,148 +168,23 @@ __device__ __forceinline__ int fit_unit(int& c, float big, int t, float* change)
   }
   return e;
 }
-template <int DB>
-__device__ __forceinline__ void rescale(f32x16 (&acc)[DB], float change) {
-  if (__builtin_expect(!__any(change != 1), 1)) return;   // the hint keeps the moves for it out of the common path
-#pragma unroll
-  for (int d = 0; d < DB; ++d)
-#pragma unroll
-    for (int q = 0; q < 16; ++q) acc[d][q] *= change;
-}
 __device__ __forceinline__ half8 frag(const _Float16* L, int f) { return *(const half8*)(L + f * kFrag + (threadIdx.x & 63) * 8); }
-// acc += A fragments (feature blocks x two k steps, from fragment f0 of L) times the split of x * scale, two of them a step;
-// a step's fragments are read while the step before is multiplied.
-template <int DB>
-__device__ __forceinline__ void accumulate(f32x16 (&acc)[DB], const f32x16& x, float scale, const _Float16* L, int f0) {
-  half8 a[2][4];
-  auto read = [&](int i) {         // of fragments 2 i and 2 i + 1: feature block u % DB, k step u / DB
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int u = 2 * i + e, f = f0 + u % DB * 4 + u / DB * 2;
-      a[i & 1][2 * e] = frag(L, f);
-      a[i & 1][2 * e + 1] = frag(L, f + 1);
-    }
-  };
-  read(0);
-  half8 bh[2], bl[2];
-#pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
-    float z[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) z[q] = x[8 * ks + q] * scale;
-    split8(z, bh[ks], bl[ks]);
-  }
-#pragma unroll
-  for (int i = 0; i < DB; ++i) {
-    if (i + 1 < DB) read(i + 1);
-    const int d0 = 2 * i % DB, k0 = 2 * i / DB, d1 = (2 * i + 1) % DB, k1 = (2 * i + 1) / DB;
-    const half8* f = a[i & 1];
-    acc[d0] = mfma(f[1], bh[k0], acc[d0]);
-    acc[d1] = mfma(f[3], bh[k1], acc[d1]);
-    acc[d0] = mfma(f[0], bl[k0], acc[d0]);
-    acc[d1] = mfma(f[2], bl[k1], acc[d1]);
-    acc[d0] = mfma(f[0], bh[k0], acc[d0]);
-    acc[d1] = mfma(f[2], bh[k1], acc[d1]);
-  }
-}
-// A fragments (KC k steps, from fragment f0 of L) times B fragments; two accumulators take turns.
-template <int KC>
-__device__ __forceinline__ f32x16 scores(const _Float16* L, int f0, const half8 (&bh)[KC], const half8 (&bl)[KC]) {
-  f32x16 x = {}, y = {};
-  half8 ah[2], al[2];
-  ah[0] = frag(L, f0);
-  al[0] = frag(L, f0 + 1);
-#pragma unroll
-  for (int c = 0; c < KC; ++c) {
-    if (c + 1 < KC) {
-      ah[(c + 1) & 1] = frag(L, f0 + 2 * c + 2);
-      al[(c + 1) & 1] = frag(L, f0 + 2 * c + 3);
-    }
-    y = mfma(al[c & 1], bh[c], y);
-    x = mfma(ah[c & 1], bh[c], x);
-    y = mfma(ah[c & 1], bl[c], y);
-  }
-#pragma unroll
-  for (int q = 0; q < 16; ++q) x[q] += y[q];
-  return x;
-}
-// x = A fragments times B fragments, woven with work(0), .. work(N - 1), vector work of other data. A wavefront issues in
-// order: a product issued right behind another waits for the matrix unit, and everything after it waits too. With vector work
-// between the products both units run. The scheduler is held to the written order, step by step.
-template <int KC, int N, class Work>
-__device__ __forceinline__ void scores_woven(f32x16& x, const _Float16* L, int f0, const half8 (&bh)[KC], const half8 (&bl)[KC], Work work) {
-  half8 ah[2], al[2];
-  ah[0] = frag(L, f0);
-  al[0] = frag(L, f0 + 1);
-  x = f32x16{};
-#pragma unroll
-  for (int m = 0; m < 3 * KC; ++m) {
-    const int c = m / 3, k = m % 3;
-    if (k == 0 && c + 1 < KC) {
-      ah[(c + 1) & 1] = frag(L, f0 + 2 * c + 2);
-      al[(c + 1) & 1] = frag(L, f0 + 2 * c + 3);
-    }
-    x = mfma(k == 0 ? al[c & 1] : ah[c & 1], k == 1 ? bl[c] : bh[c], x);
-#pragma unroll
-    for (int i = N * m / (3 * KC); i < N * (m + 1) / (3 * KC); ++i) work(i);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-}
-// x[q] *= rel of the tile's row 8 (q / 4) + 4 h + q % 4
-__device__ __forceinline__ void per_row(f32x16& x, const float* rel) {
-  const int h = (threadIdx.x >> 5) & 1;
-#pragma unroll
-  for (int q4 = 0; q4 < 4; ++q4) {
-    const f32x4 r = *(const f32x4*)(rel + 8 * q4 + 4 * h);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[4 * q4 + e] *= r[e];
-  }
-}
-__device__ __forceinline__ float largest(const f32x16& x) {   // magnitude, over a row's two lane halves
-  float m = 0;
-#pragma unroll
-  for (int q = 0; q < 16; ++q) m = fmaxf(m, fabsf(x[q]));
-  return halves_max(m);
-}
-
-// This lane's column of acc (features), in units of 2^-c, to a row in memory.
-template <int DB>
-__device__ __forceinline__ void store_row(float* row, const f32x16 (&acc)[DB], int c, float scale, int n, bool wide) {
-  const int h = (threadIdx.x >> 5) & 1;
-#pragma unroll
-  for (int d = 0; d < DB; ++d)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int at = 32 * d + 8 * q + 4 * h;
-      f32x4 v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_ldexpf(acc[d][4 * q + e], -c) * scale;
-      if (wide) {
-        if (at < n) *(f32x4*)(row + at) = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) if (at + e < n) row[at + e] = v[e];
-      }
-    }
-}
-
-// ---- products of 16 columns ------------------------------------------------------------------------
-//
-// A wavefront's own rows (keys, or query rows) are the columns of 16 x 16 x 32 products: at head size 128 their operands and
-// gradients then leave room for two wavefronts a SIMD, where 32 columns took the registers of one, which waited for every
-// product. Fragments are read from LDS twice as often for it.
-
-__device__ __forceinline__ float groups_max(float x) {   // over lanes l % 16 + 0, 16, 32, 48
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+// Over the four lanes l % 16 + 0, 16, 32, 48 of a column.
+__device__ __forceinline__ float groups_max(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float groups_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return halves_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 // B fragments of 16 rows (lane l: row l % 16), each row with its own power of two; returns its exponent.
 template <int N>
-__device__ __forceinline__ int load_rows16(const float* row, bool valid, int n, bool wide, half8 (&hi)[N], half8 (&lo)[N]) {
+__device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bool wide, half8 (&hi)[N], half8 (&lo)[N]) {
   const int g = (threadIdx.x >> 4) & 3;
   float x[N][8], m = 0;
 #pragma unroll
@@ -409,17 +218,10 @@ __device__ __forceinline__ int load_rows16(const float* row, bool valid, int n, 
   }
   return e;
 }
-// N fragments by eight wavefronts, wavefront w's at src and lds + 1024 w.
-template <int N>
-__device__ __forceinline__ void frags_by_eight(const char* src, uint32_t lds, uint32_t lane16, int w) {
-#pragma unroll
-  for (int f = 0; f < N / 8; ++f) frags_to_lds<4>(src + f * 8192, lds + f * 8192, lane16);
-  if (N % 8 && w < N % 8) frags_to_lds<4>(src + N / 8 * 8192, lds + N / 8 * 8192, lane16);
-}
 // x = A fragments (N chunks of 32 features, two blocks of 16 rows each, from fragment f0) times B fragments; a chunk's
 // fragments are read while the chunk before is multiplied.
 template <int N>
-__device__ __forceinline__ void scores16(const _Float16* L, int f0, const half8 (&bh)[N], const half8 (&bl)[N], float (&x)[8]) {
+__device__ __forceinline__ void scores(const _Float16* L, int f0, const half8 (&bh)[N], const half8 (&bl)[N], float (&x)[8]) {
   f32x4 z[2] = {};
   half8 a[2][4];
 #pragma unroll
@@ -430,12 +232,12 @@ __device__ __forceinline__ void scores16(const _Float16* L, int f0, const half8 
     if (c + 1 < N)
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[(c + 1) & 1][i] = frag(L, f0 + 4 * c + 4 + i);
-    z[0] = mfma16(u[1], bh[c], z[0]);
-    z[1] = mfma16(u[3], bh[c], z[1]);
-    z[0] = mfma16(u[0], bl[c], z[0]);
-    z[1] = mfma16(u[2], bl[c], z[1]);
-    z[0] = mfma16(u[0], bh[c], z[0]);
-    z[1] = mfma16(u[2], bh[c], z[1]);
+    z[0] = mfma(u[1], bh[c], z[0]);
+    z[1] = mfma(u[3], bh[c], z[1]);
+    z[0] = mfma(u[0], bl[c], z[0]);
+    z[1] = mfma(u[2], bl[c], z[1]);
+    z[0] = mfma(u[0], bh[c], z[0]);
+    z[1] = mfma(u[2], bh[c], z[1]);
     __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
@@ -443,7 +245,7 @@ __device__ __forceinline__ void scores16(const _Float16* L, int f0, const half8 
 }
 // Both products of a pair, step by step in turn.
 template <int N>
-__device__ __forceinline__ void pair16(const _Float16* L, int f0, const half8 (&bh)[N], const half8 (&bl)[N], float (&x)[8], int f1,
+__device__ __forceinline__ void pair(const _Float16* L, int f0, const half8 (&bh)[N], const half8 (&bl)[N], float (&x)[8], int f1,
                                        const half8 (&ch)[N], const half8 (&cl)[N], float (&y)[8]) {
   f32x4 z[4] = {};
   half8 a[2][8];
@@ -459,18 +261,18 @@ __device__ __forceinline__ void pair16(const _Float16* L, int f0, const half8 (&
   for (int c = 0; c < N; ++c) {
     const half8* u = a[c & 1];
     if (c + 1 < N) read(c + 1);
-    z[0] = mfma16(u[1], bh[c], z[0]);
-    z[1] = mfma16(u[3], bh[c], z[1]);
-    z[2] = mfma16(u[5], ch[c], z[2]);
-    z[3] = mfma16(u[7], ch[c], z[3]);
-    z[0] = mfma16(u[0], bl[c], z[0]);
-    z[1] = mfma16(u[2], bl[c], z[1]);
-    z[2] = mfma16(u[4], cl[c], z[2]);
-    z[3] = mfma16(u[6], cl[c], z[3]);
-    z[0] = mfma16(u[0], bh[c], z[0]);
-    z[1] = mfma16(u[2], bh[c], z[1]);
-    z[2] = mfma16(u[4], ch[c], z[2]);
-    z[3] = mfma16(u[6], ch[c], z[3]);
+    z[0] = mfma(u[1], bh[c], z[0]);
+    z[1] = mfma(u[3], bh[c], z[1]);
+    z[2] = mfma(u[5], ch[c], z[2]);
+    z[3] = mfma(u[7], ch[c], z[3]);
+    z[0] = mfma(u[0], bl[c], z[0]);
+    z[1] = mfma(u[2], bl[c], z[1]);
+    z[2] = mfma(u[4], cl[c], z[2]);
+    z[3] = mfma(u[6], cl[c], z[3]);
+    z[0] = mfma(u[0], bh[c], z[0]);
+    z[1] = mfma(u[2], bh[c], z[1]);
+    z[2] = mfma(u[4], ch[c], z[2]);
+    z[3] = mfma(u[6], ch[c], z[3]);
     __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
@@ -481,7 +283,7 @@ __device__ __forceinline__ void pair16(const _Float16* L, int f0, const half8 (&
 }
 // acc += A fragments (N blocks of 16 features, from fragment f0) times the split of x * scale, read as above.
 template <int N>
-__device__ __forceinline__ void accumulate16(f32x4 (&acc)[N], const float (&x)[8], float scale, const _Float16* L, int f0) {
+__device__ __forceinline__ void accumulate(f32x4 (&acc)[N], const float (&x)[8], float scale, const _Float16* L, int f0) {
   half8 a[2][4], bh, bl;
 #pragma unroll
   for (int i = 0; i < 4; ++i) a[0][i] = frag(L, f0 + i);
@@ -495,35 +297,35 @@ __device__ __forceinline__ void accumulate16(f32x4 (&acc)[N], const float (&x)[8
     if (d + 2 < N)
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[(d / 2 + 1) & 1][i] = frag(L, f0 + 2 * d + 4 + i);
-    acc[d] = mfma16(u[1], bh, acc[d]);
-    acc[d + 1] = mfma16(u[3], bh, acc[d + 1]);
-    acc[d] = mfma16(u[0], bl, acc[d]);
-    acc[d + 1] = mfma16(u[2], bl, acc[d + 1]);
-    acc[d] = mfma16(u[0], bh, acc[d]);
-    acc[d + 1] = mfma16(u[2], bh, acc[d + 1]);
+    acc[d] = mfma(u[1], bh, acc[d]);
+    acc[d + 1] = mfma(u[3], bh, acc[d + 1]);
+    acc[d] = mfma(u[0], bl, acc[d]);
+    acc[d + 1] = mfma(u[2], bl, acc[d + 1]);
+    acc[d] = mfma(u[0], bh, acc[d]);
+    acc[d + 1] = mfma(u[2], bh, acc[d + 1]);
     __builtin_amdgcn_sched_barrier(0);
   }
 }
 template <int N>
-__device__ __forceinline__ void rescale16(f32x4 (&acc)[N], float change) {
-  if (__builtin_expect(!__any(change != 1), 1)) return;
+__device__ __forceinline__ void rescale(f32x4 (&acc)[N], float change) {
+  if (__builtin_expect(!__any(change != 1), 1)) return;   // the hint keeps the moves for it out of the common path
 #pragma unroll
   for (int d = 0; d < N; ++d)
 #pragma unroll
     for (int q = 0; q < 4; ++q) acc[d][q] *= change;
 }
-__device__ __forceinline__ void per_row16(float (&x)[8], const float* rel, int g) {
+__device__ __forceinline__ void per_row(float (&x)[8], const float* rel, int g) {
 #pragma unroll
   for (int q = 0; q < 8; ++q) x[q] *= rel[16 * (q / 4) + 4 * g + q % 4];
 }
-__device__ __forceinline__ float largest16(const float (&x)[8]) {
+__device__ __forceinline__ float largest(const float (&x)[8]) {
   float m = 0;
 #pragma unroll
   for (int q = 0; q < 8; ++q) m = fmaxf(m, fabsf(x[q]));
   return groups_max(m);
 }
 // x = tanh(x u), all 8; the polynomial alone where no lane needs more
-__device__ __forceinline__ void tanh_all16(float (&x)[8], float u) {
+__device__ __forceinline__ void tanh_all(float (&x)[8], float u) {
   float m = 0;
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
@@ -539,7 +341,7 @@ __device__ __forceinline__ void tanh_all16(float (&x)[8], float u) {
   }
 }
 template <int N>
-__device__ __forceinline__ void store_row16(float* row, const f32x4 (&acc)[N], int c, float scale, int n, bool wide, int g) {
+__device__ __forceinline__ void store_row(float* row, const f32x4 (&acc)[N], int c, float scale, int n, bool wide, int g) {
 #pragma unroll
   for (int d = 0; d < N; ++d) {
     const int at = 16 * d + 4 * g;
@@ -560,6 +362,12 @@ __device__ __forceinline__ TileInfo side_info(const float* side, int x) {
   const int* p = (const int*)(side + S_INFO * kTile + 8 * x);
   auto u = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
   return {__int_as_float(u(p[0])), __int_as_float(u(p[1])), u(p[2]), u(p[3]), u(p[4]), u(p[5]), u(p[6]), 0};
+}
+// Does a query with these bounds see key z of the tile at j0. Without branches: with the document read behind the other
+// conditions the compiler has lost the value chosen (capped scores and documents: gradients of 0).
+__device__ __forceinline__ bool key_seen(const Sight& s, const float* side, int j0, int z, int below, int doc) {
+  const int id = __float_as_int(side[KS_DOC * kTile + z]);
+  return (j0 + z < below) & (!s.doc | ((doc >= 0) & (id == doc)));
 }
 // First and one past the last of the tiles [t0, t1) whose documents meet [lo, hi] (all of them without documents); odd: one
 // of those is. By the whole block.
@@ -659,7 +467,7 @@ __device__ __forceinline__ void place(uint32_t id, uint32_t slabs, int& slab, in
 struct PackJob {
   Rows x;
   int n, G, rows, tiles;           // features; heads that share a key head; rows = positions * G; tiles
-  _Float16 *rowf, *colf;           // [slab][tile][2 KC][512], [slab][tile][4 DB][512], or null
+  _Float16 *rowf, *colf;           // [slab][tile][D padded / 8][512], or null
   TileInfo* info;                  // [slab][tile]
   bool query;                      // rows are queries, else keys
   float* side;                     // [slab][tile][kSide][32]: what a block needs of each row of the tile, see below
@@ -673,7 +481,6 @@ struct Packs {
   int n;
   int Hk, tiles;                   // tiles: the most of any job
   bool wide;                       // every operand's rows are 16-byte aligned and whole 16-byte pieces
-  bool narrow;                     // packed for products of 16 columns
   PackJob job[4];
   AttendDesc a;
 };

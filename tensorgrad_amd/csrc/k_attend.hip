@@ -1,9 +1,8 @@
 // Masked attention for gfx950: y = softmax(scores) v, one pass over the keys with a running maximum and sum, so that no
 // score reaches memory. Two ways, by the number of query rows that share a key head (G query heads times Tq):
-//  * many rows: k and v are packed once into f16 hi / lo fragments (pack_tiles), then blocks of 4 wavefronts with 32 rows
-//    each walk the visible key tiles (attend_tiles). Scores are computed transposed (keys x queries), so that a lane holds
-//    half the keys of ONE query: maximum and sum are lane arithmetic and one exchange between lane halves, and the
-//    probabilities are the next product's B fragment as they stand;
+//  * many rows: k and v are packed once into f16 hi / lo fragments (pack_tiles), then blocks of 8 wavefronts with 16 rows
+//    each walk the visible key tiles (attend_tiles), four wavefronts a SIMD, so that one's products run beside the others'
+//    vector work. Scores are computed transposed (keys x queries);
 //  * few rows (one new token against a cache): the keys are read once, in f32, by all heads that share them (attend_few);
 //    bound by memory, so split over the keys until the card is full.
 // Both split a long key axis when there are few rows (attend_join). A few dozen positions in all: k_attend_small.hip.
@@ -18,7 +17,7 @@ namespace {
 // are seen by nothing are packed as zeros, whatever they hold.
 template <int DP>
 __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
-  constexpr int KC = DP / 16, DB = DP / 32, LD = DP + 4;
+  constexpr int DB = DP / 32, LD = DP + 4;
   __shared__ float x[kTile * LD];
   __shared__ float top[kTile], own[kTile];
   __shared__ int doc[kTile];
@@ -80,7 +79,7 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
     }
   }
   __syncthreads();
-  const int lane = tid & 63, w = tid >> 6, h = lane >> 5, l = lane & 31;
+  const int lane = tid & 63, w = tid >> 6, l = lane & 31;
   const float mine = top[l];
   float hi = mine, lo = mine > 0 ? mine : INFINITY;
   int dmin = doc[l] >= 0 ? doc[l] : INT32_MAX, dmax = doc[l] >= 0 ? doc[l] : INT32_MIN;
@@ -107,29 +106,26 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
   }
   if (bad) return;
   __syncthreads();
-  const bool narrow = p.narrow;
-  const int g16 = lane >> 4, l16 = lane & 15;
+  const int g4 = lane >> 4, l16 = lane & 15;
   if (j.rowf)
-    for (int c = w; c < KC; c += 4) {
-      // 16 features c of 32 rows; narrow: 32 features c / 2 of 16 rows
-      const int r = narrow ? 16 * (c % 2) + l16 : l, d = narrow ? 32 * (c / 2) + 8 * g16 : 16 * c + 8 * h;
+    for (int c = w; c < 2 * DB; c += 4) {   // 32 features c / 2 of 16 rows c % 2
+      const int r = 16 * (c % 2) + l16;
       float z[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) z[q] = x[r * LD + d + q] * own[r];
+      for (int q = 0; q < 8; ++q) z[q] = x[r * LD + 32 * (c / 2) + 8 * g4 + q] * own[r];
       half8 a, f;
       split8(z, a, f);
-      half8* o = (half8*)(j.rowf + (slot * KC + c) * 2 * kFrag) + lane;
+      half8* o = (half8*)(j.rowf + (slot * 2 * DB + c) * 2 * kFrag) + lane;
       o[0] = a;
       o[kFrag / 8] = f;
     }
   if (j.colf)
-    for (int c = w; c < 2 * DB; c += 4) {   // feature block c / 2, k step c % 2; narrow: feature block c of 16
-      const int d = narrow ? 16 * c + l16 : 32 * (c / 2) + l;
+    for (int c = w; c < 2 * DB; c += 4) {   // 16 features c of all rows
       float z[8];
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        const int k = narrow ? 16 * (q / 4) + 4 * g16 + q % 4 : 16 * (c % 2) + 8 * (q / 4) + 4 * h + q % 4;
-        z[q] = x[k * LD + d] * own[k];
+        const int k = 16 * (q / 4) + 4 * g4 + q % 4;
+        z[q] = x[k * LD + 16 * c + l16] * own[k];
       }
       half8 a, f;
       split8(z, a, f);
@@ -263,7 +259,7 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   }
 
   half8 qh[N], ql[N];
-  const int qe = load_rows16<N>(a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t, valid, a.D, A.wide, qh, ql);
+  const int qe = load_rows<N>(a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t, valid, a.D, A.wide, qh, ql);
   const float slope = SLOPES ? a.slopes[head] * kLog2e : 0.0f;
   const int64_t tile0 = (int64_t)slab * tiles + t0;
   const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
@@ -272,9 +268,9 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   const char* side_p = (const char*)(A.side + tile0 * (kSide * kTile)) + w * 1024;
   auto fetch = [&](int buf) {      // the next tile
     const uint32_t to = base + buf * (NF * 1024);
-    frags_by_eight<F>(kf, to, lane16, w);
-    frags_by_eight<F>(vf, to + F_V * 1024, lane16, w);
-    frags_by_eight<kSideFrags>(side_p, to + F_SIDE * 1024, lane16, w);
+    frags_to_lds<F>(kf, to, lane16, w);
+    frags_to_lds<F>(vf, to + F_V * 1024, lane16, w);
+    frags_to_lds<kSideFrags>(side_p, to + F_SIDE * 1024, lane16, w);
     kf += F * 1024;
     vf += F * 1024;
     side_p += kSide * kTile * 4;
@@ -297,12 +293,12 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
     const TileInfo kt = side_info(side, 0), vt = side_info(side, 1);
     if (__builtin_expect(!any_seen(s, me, kt, j0), 0)) continue;
     float x[8];                    // transposed: element q of this lane is key j0 + 16 (q / 4) + 4 g4 + q % 4
-    scores16<N>(L, 0, qh, ql, x);
+    scores<N>(L, 0, qh, ql, x);
     const float unit = a.scale * pow2(-qe) * kt.inv;
-    if (__builtin_expect(kt.uneven, 0)) per_row16(x, side + KS_RELK * kTile, g4);
+    if (__builtin_expect(kt.uneven, 0)) per_row(x, side + KS_RELK * kTile, g4);
     float f = unit * kLog2e;       // the score is f x, in log2
     if (CAP) {
-      tanh_all16(x, unit * icap);
+      tanh_all(x, unit * icap);
       f = a.cap * kLog2e;
     }
     if (SLOPES) {
@@ -312,11 +308,7 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
     }
     if (__builtin_expect(!all_seen(s, me, kt, j0), 0)) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const int z = 16 * (q / 4) + 4 * g4 + q % 4;
-        const bool ok = j0 + z < below && (!s.doc || (doc >= 0 && __float_as_int(side[KS_DOC * kTile + z]) == doc));
-        x[q] = ok ? x[q] : kNone;
-      }
+      for (int q = 0; q < 8; ++q) x[q] = key_seen(s, side, j0, 16 * (q / 4) + 4 * g4 + q % 4, below, doc) ? x[q] : kNone;
     }
     float top = x[0];
 #pragma unroll
@@ -340,12 +332,12 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
     sum = fmaf(sum, keep, part);
     float big = __builtin_amdgcn_exp2f(top - off);
     if (__builtin_expect(vt.uneven, 0)) {
-      per_row16(x, side + KS_RELV * kTile, g4);
-      big = largest16(x);
+      per_row(x, side + KS_RELV * kTile, g4);
+      big = largest(x);
     }
     const int e = fit_unit(ce, big, exponent(vt.scale), &change);
-    rescale16(acc, change);
-    accumulate16(acc, x, pow2(e), L, F_V);
+    rescale(acc, change);
+    accumulate(acc, x, pow2(e), L, F_V);
   }
 
   sum = groups_sum(sum);
@@ -353,7 +345,7 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   const bool none = sum == 0;      // not m: a visible NaN leaves no maximum
   const float out = none ? 0.0f : 1.0f / sum;
   float* y = result_row(A, split, slab, b, head, r, i, m + __builtin_amdgcn_logf(sum), none, g4 == 0);
-  if (y) store_row16(y, acc, ce, out, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide, g4);
+  if (y) store_row(y, acc, ce, out, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide, g4);
 }
 
 // ---- few rows --------------------------------------------------------------------------------------
@@ -680,7 +672,6 @@ void attend(const AttendDesc& a, void* work, hipStream_t st) {
     k.n = 2;
     k.Hk = a.Hk;
     k.wide = wide;
-    k.narrow = true;
     k.a = a;
     float* side = (float*)(w + p.side);
     k.job[0] = {a.k, a.D, 1, a.Tk, p.tiles, (_Float16*)(w + p.kf), nullptr, (TileInfo*)(w + p.ki), false, side, KS_RELK, false, true, {}};

@@ -144,9 +144,9 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
   }
 
   half8 kh[N], kl[N], vh[DK ? N : 1], vl[DK ? N : 1];
-  const int ke = load_rows16<N>(a.k.p + b * a.k.b + hk * a.k.h + (int64_t)min(j, a.Tk - 1) * a.k.t, valid, a.D, A.wide, kh, kl);
+  const int ke = load_rows<N>(a.k.p + b * a.k.b + hk * a.k.h + (int64_t)min(j, a.Tk - 1) * a.k.t, valid, a.D, A.wide, kh, kl);
   int ve = 0;
-  if constexpr (DK) ve = load_rows16<N>(a.v.p + b * a.v.b + hk * a.v.h + (int64_t)min(j, a.Tk - 1) * a.v.t, valid, a.Dv, A.wide, vh, vl);
+  if constexpr (DK) ve = load_rows<N>(a.v.p + b * a.v.b + hk * a.v.h + (int64_t)min(j, a.Tk - 1) * a.v.t, valid, a.Dv, A.wide, vh, vl);
   const int64_t tile0 = (int64_t)slab * A.qtiles + t0;
   const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
   const char* qr = (const char*)(A.qr + tile0 * (F * kFrag)) + w * 1024;
@@ -156,19 +156,19 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
   const char* side_p = (const char*)(A.qside + tile0 * (kSide * kTile)) + w * 1024;
   auto fetch = [&](int buf) {      // the next tile
     const uint32_t to = base + buf * (NF * 1024);
-    frags_by_eight<F>(qr, to, lane16, w);
+    frags_to_lds<F>(qr, to, lane16, w);
     qr += F * 1024;
     if (DK) {
-      frags_by_eight<F>(gr, to + F_GR * 1024, lane16, w);
-      frags_by_eight<F>(qc, to + F_QC * 1024, lane16, w);
+      frags_to_lds<F>(gr, to + F_GR * 1024, lane16, w);
+      frags_to_lds<F>(qc, to + F_QC * 1024, lane16, w);
       gr += F * 1024;
       qc += F * 1024;
     }
     if (DV) {
-      frags_by_eight<F>(gc, to + F_GC * 1024, lane16, w);
+      frags_to_lds<F>(gc, to + F_GC * 1024, lane16, w);
       gc += F * 1024;
     }
-    frags_by_eight<kSideFrags>(side_p, to + F_SIDE * 1024, lane16, w);
+    frags_to_lds<kSideFrags>(side_p, to + F_SIDE * 1024, lane16, w);
     side_p += kSide * kTile * 4;
   };
 
@@ -196,18 +196,18 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
     // element q: row r0 + 16 (q / 4) + 4 g + q % 4
     float x[8], y[8] = {};
     if constexpr (DK && N == 2) {  // the pair in turn would spill registers here
-      scores16<N>(L, 0, kh, kl, x);
-      scores16<N>(L, F_GR, vh, vl, y);
-    } else if constexpr (DK) pair16<N>(L, 0, kh, kl, x, F_GR, vh, vl, y);
+      scores<N>(L, 0, kh, kl, x);
+      scores<N>(L, F_GR, vh, vl, y);
+    } else if constexpr (DK) pair<N>(L, 0, kh, kl, x, F_GR, vh, vl, y);
     else {
-      scores16<N>(L, 0, kh, kl, x);
+      scores<N>(L, 0, kh, kl, x);
     }
-    if (__builtin_expect(qt.uneven, 0)) per_row16(x, side + QS_RELQ * kTile, g);
-    if (DK && __builtin_expect(gt.uneven, 0)) per_row16(y, side + QS_RELG * kTile, g);
+    if (__builtin_expect(qt.uneven, 0)) per_row(x, side + QS_RELQ * kTile, g);
+    if (DK && __builtin_expect(gt.uneven, 0)) per_row(y, side + QS_RELG * kTile, g);
     const float unit = a.scale * pow2(-ke) * qt.inv, yunit = pow2(-ve) * gt.inv;
     float f = unit * kLog2e;
     if (RICH && a.cap > 0) {
-      tanh_all16(x, unit * icap);
+      tanh_all(x, unit * icap);
       f = a.cap * kLog2e;
     }
     const bool all = A.M - r0 >= kTile && all_seen(s, rows, mine, jt);
@@ -235,33 +235,33 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
         const f32x4 below = *(const f32x4*)(side + QS_BELOW * kTile + at), rdoc = *(const f32x4*)(side + QS_DOC * kTile + at);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool ok = j < __float_as_int(below[e]) && (!s.doc || (doc >= 0 && __float_as_int(rdoc[e]) == doc));
+          const bool ok = (j < __float_as_int(below[e])) & (!s.doc | ((doc >= 0) & (__float_as_int(rdoc[e]) == doc)));
           x[4 * q4 + e] = ok ? x[4 * q4 + e] : 0.0f;
           y[4 * q4 + e] = ok ? y[4 * q4 + e] : 0.0f;
         }
       }
     }
     if (DV) {
-      if (__builtin_expect(gt.uneven, 0)) per_row16(x, side + QS_RELG * kTile, g);
+      if (__builtin_expect(gt.uneven, 0)) per_row(x, side + QS_RELG * kTile, g);
       float change = 1;
-      const int e = fit_unit(cv, largest16(x), exponent(gt.scale), &change);
-      rescale16(dv, change);
-      accumulate16(dv, x, pow2(e), L, F_GC);
+      const int e = fit_unit(cv, largest(x), exponent(gt.scale), &change);
+      rescale(dv, change);
+      accumulate(dv, x, pow2(e), L, F_GC);
     }
     if (DK) {
-      if (__builtin_expect(qt.uneven, 0)) per_row16(y, side + QS_RELQ * kTile, g);
+      if (__builtin_expect(qt.uneven, 0)) per_row(y, side + QS_RELQ * kTile, g);
       float change = 1;
-      const int e = fit_unit(ck, largest16(y), exponent(qt.scale), &change);
-      rescale16(dk, change);
-      accumulate16(dk, y, pow2(e), L, F_QC);
+      const int e = fit_unit(ck, largest(y), exponent(qt.scale), &change);
+      rescale(dk, change);
+      accumulate(dk, y, pow2(e), L, F_QC);
     }
   }
 
   if (!valid) return;
   float* ok = dk_row(A, split, slab, b, hk, j);
   float* ov = dv_row(A, split, slab, b, hk, j);
-  if (DK && ok) store_row16(ok, dk, ck, a.scale, a.D, A.splits > 1 ? a.D % 4 == 0 : A.wide, g);
-  if (DV && ov) store_row16(ov, dv, cv, 1.0f, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide, g);
+  if (DK && ok) store_row(ok, dk, ck, a.scale, a.D, A.splits > 1 ? a.D % 4 == 0 : A.wide, g);
+  if (DV && ov) store_row(ov, dv, cv, 1.0f, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide, g);
 }
 
 // The parts of dk, dv and dq in order: a block takes 32 keys of the 128 that the parts were split for, or 32 query rows.
@@ -405,8 +405,8 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   }
 
   half8 qh[N], ql[N], gh[N], gl[N];
-  const int qe = load_rows16<N>(a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t, valid, a.D, A.wide, qh, ql);
-  const int ge = load_rows16<N>(A.g.dy.p + b * A.g.dy.b + head * A.g.dy.h + (int64_t)i * A.g.dy.t, valid, a.Dv, A.wide, gh, gl);
+  const int qe = load_rows<N>(a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t, valid, a.D, A.wide, qh, ql);
+  const int ge = load_rows<N>(A.g.dy.p + b * A.g.dy.b + head * A.g.dy.h + (int64_t)i * A.g.dy.t, valid, a.Dv, A.wide, gh, gl);
   const float slope = RICH && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
   const int64_t tile0 = (int64_t)slab * A.ktiles + t0;
   const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
@@ -416,10 +416,10 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   const char* side_p = (const char*)(A.kside + tile0 * (kSide * kTile)) + w * 1024;
   auto fetch = [&](int buf) {      // the next tile
     const uint32_t to = base + buf * (NF * 1024);
-    frags_by_eight<F>(kr, to, lane16, w);
-    frags_by_eight<F>(vr, to + F_V * 1024, lane16, w);
-    frags_by_eight<F>(kc, to + F_KC * 1024, lane16, w);
-    frags_by_eight<kSideFrags>(side_p, to + F_SIDE * 1024, lane16, w);
+    frags_to_lds<F>(kr, to, lane16, w);
+    frags_to_lds<F>(vr, to + F_V * 1024, lane16, w);
+    frags_to_lds<F>(kc, to + F_KC * 1024, lane16, w);
+    frags_to_lds<kSideFrags>(side_p, to + F_SIDE * 1024, lane16, w);
     kr += F * 1024;
     vr += F * 1024;
     kc += F * 1024;
@@ -444,11 +444,11 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
     if (__builtin_expect(!any_seen(s, me, kt, j0), 0)) continue;
     // element q: key j0 + 16 (q / 4) + 4 g4 + q % 4
     float x[8], y[8];
-    pair16<N>(L, 0, qh, ql, x, F_V, gh, gl, y);
-    if (__builtin_expect(kt.uneven, 0)) per_row16(x, side + KS_RELK * kTile, g4);
-    if (__builtin_expect(vt.uneven, 0)) per_row16(y, side + KS_RELV * kTile, g4);
+    pair<N>(L, 0, qh, ql, x, F_V, gh, gl, y);
+    if (__builtin_expect(kt.uneven, 0)) per_row(x, side + KS_RELK * kTile, g4);
+    if (__builtin_expect(vt.uneven, 0)) per_row(y, side + KS_RELV * kTile, g4);
     const float unit = a.scale * pow2(-qe) * kt.inv, yunit = pow2(-ge) * vt.inv;
-    if (cap) tanh_all16(x, unit * icap);
+    if (cap) tanh_all(x, unit * icap);
     const float f = (cap ? a.cap : unit) * kLog2e;
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
@@ -459,20 +459,16 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
     }
     if (__builtin_expect(!all_seen(s, me, kt, j0), 0)) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const int z = 16 * (q / 4) + 4 * g4 + q % 4;
-        const bool ok = j0 + z < below && (!s.doc || (doc >= 0 && __float_as_int(side[KS_DOC * kTile + z]) == doc));
-        y[q] = ok ? y[q] : 0.0f;
-      }
+      for (int q = 0; q < 8; ++q) y[q] = key_seen(s, side, j0, 16 * (q / 4) + 4 * g4 + q % 4, below, doc) ? y[q] : 0.0f;
     }
-    if (__builtin_expect(kt.uneven, 0)) per_row16(y, side + KS_RELK * kTile, g4);
+    if (__builtin_expect(kt.uneven, 0)) per_row(y, side + KS_RELK * kTile, g4);
     float change = 1;
-    const int e = fit_unit(cq, largest16(y), exponent(kt.scale), &change);
-    rescale16(dq, change);
-    accumulate16(dq, y, pow2(e), L, F_KC);
+    const int e = fit_unit(cq, largest(y), exponent(kt.scale), &change);
+    rescale(dq, change);
+    accumulate(dq, y, pow2(e), L, F_KC);
   }
   if (valid)
-    store_row16(dq_row(A, split, slab, b, head, r, i), dq, cq, a.scale, a.D, A.qsplits > 1 ? a.D % 4 == 0 : A.wide, g4);
+    store_row(dq_row(A, split, slab, b, head, r, i), dq, cq, a.scale, a.D, A.qsplits > 1 ? a.D % 4 == 0 : A.wide, g4);
 }
 
 // ---- plan --------------------------------------------------------------------------------------------
@@ -559,7 +555,6 @@ void attend_grad(const AttendGradDesc& g, void* work, hipStream_t st) {
   k.n = 4;
   k.Hk = a.Hk;
   k.wide = wide;
-  k.narrow = true;
   k.a = a;
   float *qs = (float*)(w + p.qside), *ks = (float*)(w + p.kside);
   k.job[0] = {a.q, a.D, p.G, p.M, p.qtiles, half(p.qr), half(p.qc), info(p.qi), true, qs, QS_RELQ, false, false, {}};

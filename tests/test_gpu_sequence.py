@@ -110,6 +110,23 @@ def test_attention_masks(shape, kind):
         assert not any(np.any(x) for x in got.values())
 
 
+@pytest.mark.parametrize('D', [16, 40, 64, 96, 128])
+@pytest.mark.parametrize('scores', [dict(softcap=30.0), dict(softcap=0.5), dict(slopes=[0.5, -0.1]), dict(softcap=5.0, slopes=[0.5, 0.02])],
+                         ids=['cap', 'low cap', 'slopes', 'both'])
+@pytest.mark.parametrize('T,kind', [(20, 'all'), (90, 'documents'), (150, 'prefix'), (260, 'all'), (130, 'lengths')])
+def test_attention_scores_with_masks(T, kind, scores, D):
+    """Every variant of the kernels under every kind of mask."""
+    q, k, v, dy = qkv(2, 2, 1, T, T, D, D, 27)
+    r, masks = rng(T, D, 28), {}
+    if kind in ('documents', 'all'):
+        masks['documents'] = np.sort(r.integers(-1, 4, (2, T), dtype=np.int32), 1)
+    if kind in ('prefix', 'all'):
+        masks['prefix'] = np.array([T // 2, 3], np.int32)
+    if kind in ('lengths', 'all'):
+        masks['lengths'] = np.array([T - 1, T // 2], np.int32)
+    check_attention(q, k, v, dy, scores, masks, kind)
+
+
 @pytest.mark.parametrize('Tq,Tk', [(1, 1), (1, 31), (1, 700), (5, 700), (33, 700), (128, 1000)])
 @pytest.mark.parametrize('causal', [True, False])
 def test_attention_over_a_part_filled_cache(Tq, Tk, causal):
@@ -120,6 +137,19 @@ def test_attention_over_a_part_filled_cache(Tq, Tk, causal):
         k[b, :, min(n[b], Tk):], v[b, :, min(n[b], Tk):] = np.nan, np.inf
     check_attention(q, k, v, dy, dict(causal=causal), dict(lengths=n), f'{Tq}x{Tk}')
     check_attention(q, k, v, None, dict(causal=causal), dict(lengths=n), f'{Tq}x{Tk} forward')
+
+
+@pytest.mark.parametrize('Tq,H,D', [(1, 1, 64), (1, 4, 128), (2, 2, 96), (4, 4, 32), (3, 1, 17)])
+@pytest.mark.parametrize('scores', [{}, dict(softcap=4.0), dict(softcap=30.0, slopes=True)], ids=['plain', 'cap', 'both'])
+def test_few_rows_with_masks(Tq, H, D, scores):
+    """The last tokens against a long cache with documents, a prefix and lengths."""
+    q, k, v, _ = qkv(3, H, 1, Tq, 900, D, D, 29)
+    r = rng(Tq, D, 30)
+    doc = np.sort(r.integers(0, 3, (3, 900), dtype=np.int32), 1)
+    doc[1, 870:] = -1
+    masks = dict(documents=doc, prefix=np.array([0, 5, 900], np.int32), lengths=np.array([900, 900, 555], np.int32))
+    how = dict(scores, slopes=[0.3 / (n + 1) for n in range(H)]) if 'slopes' in scores else scores
+    check_attention(q, k, v, None, how, masks)
 
 
 @pytest.mark.parametrize('bad', [np.nan, np.inf, -np.inf, 3.4e38])
