@@ -12,9 +12,9 @@
 // exchanges. Two blocks of scores, tile rows 0..15 and 16..31, are the next product's B fragment as they stand, if its A
 // fragments take their k in the same order: rows 4 g + 0..3, then 16 + 4 g + 0..3.
 //
-// 32 columns a wavefront (32 x 32 x 16) would read fragments from LDS half as often, but their operands and results took the
-// registers of a SIMD's only wavefront, or of two, which then waited for every product: slower in every case but one
-// (gradients of head size 32 without documents, by 4 %), twice as slow for the gradients of head size 128.
+// 32 columns a wavefront (32 x 32 x 16) would read fragments from LDS half as often, but their operands and results take the
+// registers of a SIMD's one or two wavefronts, which then wait for every product: measured slower in every case but the
+// gradients of head size 32 without documents (4 %); those of head size 128 took half as long again.
 #pragma once
 #include "kernels.h"
 #include "sequence.h"

@@ -14,7 +14,8 @@ namespace {
 // ---- packing -------------------------------------------------------------------------------------
 
 // A block packs one tile of 32 rows: reads them once, finds their scales, writes its fragments. Rows that see nothing and
-// are seen by nothing are packed as zeros, whatever they hold.
+// are seen by nothing are packed as zeros, whatever they hold. Bound by memory: the seven operands of a gradient over 4096
+// rows of 16 query and 4 key heads of 128 are 50 us (117 MB read, 159 MB written: 5.5 TB/s).
 template <int DP>
 __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
   constexpr int DB = DP / 32, LD = DP + 4;
@@ -202,6 +203,9 @@ __device__ __forceinline__ void plain_rows(const TilesArgs& A, const Sight& s, i
   }
 }
 
+// Bound by the issue of products and vector work together, which overlap only between wavefronts: 4096 x 4096 pairs without
+// masks, 8 heads of 128: 208 us, 330 TFLOP/s of the 443 that three f16 products for one allow; capped and causal: 158 us. k and
+// v come two tiles in turn: the next one travels while this one is multiplied.
 template <int DP, bool CAP, bool SLOPES>
 __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   constexpr int N = DP / 32, F = 4 * N, F_V = F, F_SIDE = 2 * F, NF = F_SIDE + kSideFrags;
@@ -358,7 +362,9 @@ struct FewArgs {
 
 // Eight lanes share a key row: each reads E of its features as 16-byte pieces (8 rows of 128 bytes a load instruction) and
 // multiplies them with the same features of all R query rows, which it keeps. Every group of eight lanes carries a running
-// maximum, sum and result of its own; the 32 groups of a block are joined once at its end.
+// maximum, sum and result of its own; the 32 groups of a block are joined once at its end. A part is the same number of keys
+// for every batch entry, so that blocks past a short one end at once and those that work are alike. 8 caches of up to 16000
+// keys, 4 key heads of 128, 16 query heads: 66 us, 6.0 TB/s.
 template <int E, int R, bool WIDE>
 __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
   const AttendDesc& a = A.a;
@@ -511,8 +517,9 @@ struct JoinArgs {
   int M, splits;
   const float *part, *plse;
 };
-// L threads join a row: its weights first, then every 32 threads an L / 32nd of the parts. 32 threads take a row with few
-// parts and a block one with many (a long cache read by one token).
+// Bound by memory (24864 rows of 2 parts of 96: 10 us). L threads join a row: its weights first, then every 32 threads an
+// L / 32nd of the parts. 32 threads take a row with few parts and a block one with many (a long cache read by one token: 16
+// parts by 32 threads or 64 by a block, 8 or 7 us; one thread a feature took 33).
 template <int L>
 __global__ __launch_bounds__(256) void attend_join(JoinArgs A) {
   constexpr int W = L < 64 ? L : 64, P = L / 32, PER = 256 / L;
