@@ -35,8 +35,8 @@ __device__ __forceinline__ void seeing_tiles(const GradArgs& A, const Sight& s, 
 }
 // Those of part `split`, equal stretches of all rows, so that blocks that run together walk the same ones. False: none, which
 // the join finds again and does not read. With documents the stretch that a key block's own see is short: there its tiles are
-// cut into equal parts, of 8 at least, when they are known (8 x 1000 positions, 2 key heads of 64, documents of 50: 53 us
-// instead of 81, of 170: 82 instead of 87; one document: 130 instead of 123).
+// cut into equal parts, of 8 at least, when they are known (8 x 1000 positions, 2 key heads of 64, with 32 keys a wavefront:
+// documents of 50 took 53 us instead of 81, of 170 82 instead of 87; one document 130 instead of 123).
 __device__ __forceinline__ bool part_rows(const GradArgs& A, const Sight& s, int k0, int split, int& from, int& to) {
   seeing_tiles(A, s, k0, from, to);
   if (A.splits == 1 || s.doc) return true;
@@ -107,7 +107,7 @@ __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, in
 
 // Eight wavefronts of 16 keys. WHAT: 1 for dk, 2 for dv, 3 for both in one walk. Up to head size 64 two blocks share a CU. Both
 // gradients of 4096 causal rows of 16 heads of 128: 664 us (by 32 keys 990, in walks of their own); of 8 heads of 64: 193 us
-// (205); of 8 x 1000 rows of 8 heads of 32: 76 us (66), in documents of 50: 38 us (44).
+// (205); of 8 x 1000 rows of 8 heads of 64 in documents of 170: 66 us (81); of 32 without documents: 76 us (66).
 template <int DP, bool RICH, int WHAT>
 __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs A) {
   constexpr int N = DP / 32, F = 4 * N;                      // chunks of 32 features; fragments of an operand
@@ -356,7 +356,7 @@ __device__ __forceinline__ void plain_dq(const GradArgs& A, const Sight& s, int 
 }
 
 // Eight wavefronts of 16 query rows. 4096 causal rows of 16 heads of 128: 371 us (470 by 32 rows); 8 x 1000 rows of 8 heads
-// of 64 in documents of 170: 49 us (57).
+// of 64 in documents of 170: 43 us (57).
 template <int DP, bool RICH>
 __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   constexpr int N = DP / 32, F = 4 * N, F_V = F, F_KC = 2 * F, F_SIDE = 3 * F, NF = F_SIDE + kSideFrags;
@@ -488,11 +488,12 @@ GradPlan grad_plan(const AttendGradDesc& g) {
   p.ktiles = (a.Tk + kTile - 1) / kTile;
   p.blocks = (a.Tk + 127) / 128;
   const int64_t have = (int64_t)p.slabs * p.blocks;
-  // About 1024 blocks, two to four rounds of the card: 512 leave it to the longest (4096 causal rows of 4 slabs: 1.30 ms
-  // instead of 1.03), 2048 write and join twice the parts (58 us instead of 38).
+  // About 1024 blocks, two to four rounds of the card: 512 leave it to the longest (4096 causal rows of 4 slabs, head size 128:
+  // 832 us and 21 to join, instead of 677 and 31), 2048 write and join twice the parts (624 and 58).
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((1024 + have - 1) / have, p.qtiles / 8));
-  // dq: one round of the card (32 slabs of 777 rows, head size 96: 64 us and 4 more to join, instead of 73; in two rounds 73)
-  p.qsplits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / ((int64_t)p.slabs * ((p.M + 127) / 128)), p.ktiles / 8));
+  // dq in parts only where its blocks leave compute units idle: 224 of them (32 slabs of 777 rows, head size 96) take 55 us, in
+  // two parts 52 and 6 to join.
+  p.qsplits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / ((int64_t)p.slabs * ((p.M + 127) / 128)), p.ktiles / 8));
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t b = at;
