@@ -306,6 +306,44 @@ def test_one_tensor_in_every_place_and_gradients_asked_twice(T, D):
         R.check(g, want[n], tol[n], n)
 
 
+@pytest.mark.parametrize('T,D', [(20, 24), (150, 32), (700, 64), (200, 96), (800, 128)])
+@pytest.mark.parametrize('which', [0, 1, 2, (0, 1), (2, 0), (1, 2)])
+@pytest.mark.parametrize('how', [{}, dict(softcap=10.0)], ids=['plain', 'cap'])
+def test_some_of_the_gradients(T, D, which, how):
+    """What is not asked for is not computed; what is, is the same."""
+    q, k, v, dy = qkv(1, 2, 1, T, T, D, D, 31)
+    doc = np.sort(rng(T, 32).integers(0, 3, (1, T), dtype=np.int32), 1)
+    which = (which,) if isinstance(which, int) else which
+
+    def fn(i):
+        m = dict(how, documents=i['documents'])
+        g = O.attention_grad(i['q'], i['k'], i['v'], O.attention(i['q'], i['k'], i['v'], **m), i['dy'], **m)
+        return [g[n] for n in which]
+    got = forward(fn, dict(q=q, k=k, v=v, dy=dy, documents=doc))
+    want, tol = R.attention(q, k, v, dy, documents=doc, **how)
+    for n, g in zip(which, got):
+        name = ('dq', 'dk', 'dv')[n]
+        R.check(g, want[name], tol[name], name)
+
+
+def test_strided_heads_and_gradients():
+    """q, k and v as views of one projection, heads of 40 in rows of 200: read in place, whatever their alignment."""
+    B, T, D = 2, 90, 40
+    r = rng(33)
+    x, dy = f32(r.standard_normal((B, T, 5 * D))), f32(r.standard_normal((B, 3, T, D)))
+
+    def fn(i):
+        a, b, c = O.split(i['x'], [3 * D, D, D], -1)
+        q, k, v = O.split_heads(a, 3), O.split_heads(b, 1), O.split_heads(c, 1)
+        y = O.attention(q, k, v)
+        return [y, *O.attention_grad(q, k, v, y, i['dy'])]
+    got = forward(fn, dict(x=x, dy=dy))
+    heads = lambda z: f32(z.reshape(B, T, -1, D).transpose(0, 2, 1, 3))  # noqa: E731
+    want, tol = R.attention(heads(x[..., :3 * D]), heads(x[..., 3 * D:4 * D]), heads(x[..., 4 * D:]), dy)
+    for n, g in zip(('y', 'dq', 'dk', 'dv'), got):
+        R.check(g, want[n], tol[n], n)
+
+
 @pytest.mark.parametrize('T', [3, 70])
 def test_more_key_heads_than_a_grid_axis_holds(T):
     """70000 key heads, forward: of a few positions, and one token against a longer cache."""
