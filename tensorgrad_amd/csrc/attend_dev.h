@@ -54,6 +54,13 @@ constexpr int kSideFrags = kSide * kTile * 4 / 1024;
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 __device__ __forceinline__ int exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 255) - 127; }   // floor(log2 |x|)
+// What a score's sum of products is multiplied by, c 2^e, c > 0. Rows of 1e-19, or of 1e25, take it out of f32's range: kept
+// within, it leaves such scores next to 0, or past f32's range, and a sum of 0 or a hidden key's minus infinity as they are.
+__device__ __forceinline__ float score_unit(float c, int e) {
+  return __builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(c, e), 0x1p-126f, 0x1p127f);
+}
+// The same of dP: a sum of 0 stays 0.
+__device__ __forceinline__ float dot_unit(int e) { return __builtin_amdgcn_ldexpf(1.0f, min(e, 127)); }
 
 // hi and lo of two values.
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {

@@ -298,11 +298,11 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
     if (__builtin_expect(!any_seen(s, me, kt, j0), 0)) continue;
     float x[8];                    // transposed: element q of this lane is key j0 + 16 (q / 4) + 4 g4 + q % 4
     scores<N>(L, 0, qh, ql, x);
-    const float unit = a.scale * pow2(-qe) * kt.inv;
+    const int unit = exponent(kt.inv) - qe;
     if (__builtin_expect(kt.uneven, 0)) per_row(x, side + KS_RELK * kTile, g4);
-    float f = unit * kLog2e;       // the score is f x, in log2
+    float f = score_unit(a.scale * kLog2e, unit);   // the score is f x, in log2
     if (CAP) {
-      tanh_all(x, unit * icap);
+      tanh_all(x, score_unit(a.scale * icap, unit));
       f = a.cap * kLog2e;
     }
     if (SLOPES) {

@@ -204,10 +204,11 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
     }
     if (__builtin_expect(qt.uneven, 0)) per_row(x, side + QS_RELQ * kTile, g);
     if (DK && __builtin_expect(gt.uneven, 0)) per_row(y, side + QS_RELG * kTile, g);
-    const float unit = a.scale * pow2(-ke) * qt.inv, yunit = pow2(-ve) * gt.inv;
-    float f = unit * kLog2e;
+    const int unit = exponent(qt.inv) - ke;
+    const float yunit = dot_unit(exponent(gt.inv) - ve);
+    float f = score_unit(a.scale * kLog2e, unit);
     if (RICH && a.cap > 0) {
-      tanh_all(x, unit * icap);
+      tanh_all(x, score_unit(a.scale * icap, unit));
       f = a.cap * kLog2e;
     }
     const bool all = A.M - r0 >= kTile && all_seen(s, rows, mine, jt);
@@ -447,9 +448,10 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
     pair<N>(L, 0, qh, ql, x, F_V, gh, gl, y);
     if (__builtin_expect(kt.uneven, 0)) per_row(x, side + KS_RELK * kTile, g4);
     if (__builtin_expect(vt.uneven, 0)) per_row(y, side + KS_RELV * kTile, g4);
-    const float unit = a.scale * pow2(-qe) * kt.inv, yunit = pow2(-ge) * vt.inv;
-    if (cap) tanh_all(x, unit * icap);
-    const float f = (cap ? a.cap : unit) * kLog2e;
+    const int unit = exponent(kt.inv) - qe;
+    const float yunit = dot_unit(exponent(vt.inv) - ge);
+    if (cap) tanh_all(x, score_unit(a.scale * icap, unit));
+    const float f = cap ? a.cap * kLog2e : score_unit(a.scale * kLog2e, unit);
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       float off = lse;

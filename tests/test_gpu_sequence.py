@@ -741,3 +741,52 @@ def test_parametric_length_and_host_run():
         torch.cuda.synchronize()
         assert np.array_equal(out.cpu().numpy(), host)
     ex.destroy()
+
+
+# ---- values at the ends of f32's range --------------------------------------------------------------------
+
+@pytest.mark.parametrize('T,D', [(20, 16), (90, 64), (150, 128), (700, 40)])
+@pytest.mark.parametrize('kind', ['causal', 'lengths', 'documents', 'prefix'])
+@pytest.mark.parametrize('sizes', [(1e-20, 1e-20, None), (1e-35, 1e-3, None), (1e-3, 1e-35, None), (1e-10, 1e-10, 2.0 ** -60)],
+                         ids=['both tiny', 'tiny q', 'tiny k', 'small scale'])
+def test_scores_too_small_to_tell_apart(T, D, kind, sizes):
+    """Products of q, k and the scale near or below f32's least: every key counts alike, hidden ones not at all."""
+    q, k, v, dy = qkv(2, 2, 1, T, T, D, D, 61)
+    r, how, masks = rng(T, 62), {}, {}
+    if kind == 'lengths':
+        how['causal'] = False
+        masks['lengths'] = np.array([T - 1, T // 2], np.int32)
+    if kind == 'documents':
+        masks['documents'] = np.sort(r.integers(-1, 3, (2, T), dtype=np.int32), 1)
+    if kind == 'prefix':
+        masks['prefix'] = np.array([T // 2, 3], np.int32)
+    if sizes[2]:
+        how['scale'] = sizes[2]
+    check_attention(f32(q * sizes[0]), f32(k * sizes[1]), v, dy, how, masks, kind)
+
+
+def test_one_tiny_query_row_among_others():
+    q, k, v, dy = qkv(1, 2, 1, 150, 150, 64, 64, 63)
+    q[0, :, 77] *= 1e-36
+    check_attention(q, f32(k * 1e-2), v, dy, {}, {})
+
+
+@pytest.mark.parametrize('T', [40, 150])
+@pytest.mark.parametrize('how', [{}, dict(softcap=5.0), dict(slopes=[0.0, 0.0])], ids=['plain', 'cap', 'slopes'])
+def test_large_rows_whose_products_vanish(T, how):
+    """q has only even features, k only odd ones, of 1e25: all scores are exactly 0, so y is the mean of the seen values, though
+    the sizes' product passes f32's range. v and dy likewise: dP is 0. A mean of n values in f32 from weights off by some 20
+    roundings: 64 (16 + 4 sqrt n) roundings of the mean absolute value are generous."""
+    q, k, v, dy = qkv(1, 2, 1, T, T, 64, 64, 64)
+    q, k = f32(q * 1e25), f32(k * 1e25)
+    q[..., 1::2], k[..., ::2] = 0, 0
+    n = np.arange(1, T + 1)[:, None]
+    got = attend(q, k, v, dy, how)
+    slack = 64 * (16 + 4 * np.sqrt(T)) * R.U
+    for h in range(2):
+        want = np.cumsum(v[0, 0].astype(np.float64), 0) / n
+        assert np.all(np.abs(got['y'][0, h] - want) <= slack * np.cumsum(np.abs(v[0, 0]), 0) / n)
+    P = np.tril(np.ones((T, T))) / n
+    G = dy[0].astype(np.float64)
+    assert np.all(np.abs(got['dv'][0, 0] - sum(P.T @ G[h] for h in range(2))) <= slack * sum(P.T @ np.abs(G[h]) for h in range(2)))
+    assert np.isfinite(got['dq']).all() and np.isfinite(got['dk']).all()
