@@ -122,6 +122,9 @@ __device__ __forceinline__ int sees_below(const Sight& s, int p) {
   return s.causal ? min(s.n, max(p + 1, s.prefix)) : s.n;
 }
 __device__ __forceinline__ int doc_at(const Sight& s, int p) { return s.doc && p >= 0 ? s.doc[p] : -1; }   // negative: sees nothing
+// Does it see any: then, where positions matter, the key at its own. From the masks, not from sums or maxima, which NaN and
+// minus infinities in what is seen empty as well.
+__device__ __forceinline__ bool sees_any(const Sight& s, int below, int doc) { return below > 0 && (!s.doc || doc >= 0); }
 
 // Rows [lo, hi] of positions against keys [j0, j0 + 32): does any pair see, do all.
 struct Span {

@@ -149,13 +149,13 @@ struct TilesArgs {
   float *part, *plse;              // parts: [split][slab][M][Dv], [split][slab][M]
 };
 
-// Where a row's result goes, and its lse.
+// Where a row's result goes, and its lse. A part whose weights are all 0 has an lse of minus infinity and a result of 0.
 __device__ __forceinline__ float* result_row(const TilesArgs& A, int split, int slab, int b, int head, int r, int i, float lse, bool none,
                                              bool writes) {
   const AttendDesc& a = A.a;
   if (A.splits > 1) {
     const int64_t at = ((int64_t)split * a.B * a.Hk + slab) * A.M + r;
-    if (writes) A.plse[at] = none ? kNone : lse;
+    if (writes) A.plse[at] = lse;
     return A.part + at * a.Dv;
   }
   if (writes && a.lse) a.lse[((int64_t)b * a.H + head) * a.Tq + i] = none ? INFINITY : lse;
@@ -176,17 +176,13 @@ __device__ __forceinline__ void plain_rows(const TilesArgs& A, const Sight& s, i
     auto shown = [&](int j) { return j < end && (!s.doc || (doc >= 0 && s.doc[j] == doc)); };
     auto score = [&](int j) { return plain_score(a, plain_dot(k + j * a.k.t, q, a.D), slope, p - j).score; };
     float m = kNone;
-    bool any = false;
 #pragma unroll 1
     for (int j = j0 + lane; j < end; j += 64)
-      if (shown(j)) {
-        m = fmaxf(m, score(j));
-        any = true;
-      }
+      if (shown(j)) m = fmaxf(m, score(j));
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
-    const bool none = !__any(any);
-    if (m == kNone) m = 0;         // NaN alone, or minus infinities
+    const bool none = !sees_any(s, sees_below(s, p), doc);
+    if (m == kNone) m = 0;         // nothing, NaN alone, or minus infinities
     float sum = 0, acc[2] = {0, 0};
 #pragma unroll 1
     for (int c = j0; c < end; c += 64) {
@@ -199,7 +195,8 @@ __device__ __forceinline__ void plain_rows(const TilesArgs& A, const Sight& s, i
     for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
     float* y = result_row(A, split, slab, b, head, r, i, m + __builtin_amdgcn_logf(sum), none, lane == 0);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) if (y && 64 * e + lane < a.Dv) y[64 * e + lane] = none ? 0.0f : acc[e] / sum;
+    for (int e = 0; e < 2; ++e)
+      if (y && 64 * e + lane < a.Dv) y[64 * e + lane] = (A.splits > 1 ? sum == 0 : none) ? 0.0f : acc[e] / sum;
   }
 }
 
@@ -346,8 +343,8 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
 
   sum = groups_sum(sum);
   if (!valid) return;
-  const bool none = sum == 0;      // not m: a visible NaN leaves no maximum
-  const float out = none ? 0.0f : 1.0f / sum;
+  const bool none = !sees_any(s, below, doc);
+  const float out = (A.splits > 1 ? sum == 0 : none) ? 0.0f : 1.0f / sum;
   float* y = result_row(A, split, slab, b, head, r, i, m + __builtin_amdgcn_logf(sum), none, g4 == 0);
   if (y) store_row(y, acc, ce, out, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide, g4);
 }
@@ -521,7 +518,8 @@ struct JoinArgs {
 };
 // Bound by memory (24864 rows of 2 parts of 96: 10 us). L threads join a row: its weights first, then every 32 threads an
 // L / 32nd of the parts. 32 threads take a row with few parts and a block one with many (a long cache read by one token: 16
-// parts by 32 threads or 64 by a block, 8 or 7 us; one thread a feature took 33).
+// parts by 32 threads or 64 by a block, 8 or 7 us; one thread a feature took 33). An lse of NaN makes the row NaN; fmaxf passes
+// over it, so that its row's largest may be minus infinity.
 template <int L>
 __global__ __launch_bounds__(256) void attend_join(JoinArgs A) {
   constexpr int W = L < 64 ? L : 64, P = L / 32, PER = 256 / L;
@@ -532,6 +530,8 @@ __global__ __launch_bounds__(256) void attend_join(JoinArgs A) {
   const int64_t rows = (int64_t)a.B * a.Hk * A.M, row = (int64_t)blockIdx.x * PER + own, at = min(row, rows - 1);
   const int r = (int)(at % A.M), slab = (int)(at / A.M), b = slab / a.Hk, hk = slab % a.Hk, G = a.H / a.Hk;
   const int i = r / G, head = hk * G + r % G;
+  const Sight s = sight(a, b);
+  const bool none = !sees_any(s, sees_below(s, s.first + i), doc_at(s, s.first + i));
   float top = kNone, all = 0;
   for (int z = t % W; z < A.splits; z += W) top = fmaxf(top, A.plse[at + z * rows]);
 #pragma unroll
@@ -570,9 +570,9 @@ __global__ __launch_bounds__(256) void attend_join(JoinArgs A) {
   if (a.y.p) {
     float* y = a.y.p + b * a.y.b + head * a.y.h + (int64_t)i * a.y.t + d;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) if (d + q < a.Dv) y[q] = top == kNone ? 0.0f : x[q] / all;
+    for (int q = 0; q < 4; ++q) if (d + q < a.Dv) y[q] = none ? 0.0f : x[q] / all;
   }
-  if (a.lse && t == 0) a.lse[((int64_t)b * a.H + head) * a.Tq + i] = top == kNone ? INFINITY : top + __builtin_amdgcn_logf(all);
+  if (a.lse && t == 0) a.lse[((int64_t)b * a.H + head) * a.Tq + i] = none ? INFINITY : top + __builtin_amdgcn_logf(all);
 }
 
 // ---- plans -----------------------------------------------------------------------------------------

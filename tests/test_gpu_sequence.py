@@ -790,3 +790,76 @@ def test_large_rows_whose_products_vanish(T, how):
     G = dy[0].astype(np.float64)
     assert np.all(np.abs(got['dv'][0, 0] - sum(P.T @ G[h] for h in range(2))) <= slack * sum(P.T @ np.abs(G[h]) for h in range(2)))
     assert np.isfinite(got['dq']).all() and np.isfinite(got['dk']).all()
+
+
+# ---- what is not finite and seen ----------------------------------------------------------------------------
+
+SPLIT = [  # B, H, Hk, Tq, Tk, D: keys in parts, by the kernel of few rows and by tiles, joined by 32 and by 256 threads a row
+    (8, 1, 1, 1, 1000, 64), (1, 4, 1, 1, 5000, 128), (1, 2, 2, 100, 600, 64), (1, 2, 1, 64, 5000, 32), (2, 2, 1, 300, 300, 64)]
+
+
+@pytest.mark.parametrize('shape', SPLIT)
+@pytest.mark.parametrize('bad', [np.nan, np.inf])
+def test_a_query_that_is_not_finite_shows(shape, bad):
+    """Its own row alone: an infinite query's scores are infinite (of either sign: NaN weights) or NaN."""
+    B, H, Hk, Tq, Tk, D = shape
+    q, k, v, _ = qkv(B, H, Hk, Tq, Tk, D, D, 71)
+    want, tol = R.attention(q, k, v)
+    q[0, 0, Tq // 2, 3] = bad
+    y = attend(q, k, v)['y']
+    assert np.isnan(y[0, 0, Tq // 2]).all()
+    rest = np.ones((B, H, Tq), bool)
+    rest[0, 0, Tq // 2] = False
+    R.check(y[rest], want['y'][rest], tol['y'][rest])
+
+
+@pytest.mark.parametrize('shape', SPLIT)
+@pytest.mark.parametrize('at', ['first', 'middle', 'last'])
+def test_a_key_that_is_not_a_number_shows_where_it_is_seen(shape, at):
+    B, H, Hk, Tq, Tk, D = shape
+    q, k, v, _ = qkv(B, H, Hk, Tq, Tk, D, D, 72)
+    want, tol = R.attention(q, k, v)
+    j = {'first': 0, 'middle': Tk - Tq // 2 - 1, 'last': Tk - 1}[at]
+    k[0, 0, j, 5] = np.nan
+    y = attend(q, k, v)['y']
+    hit = np.zeros((B, H, Tq), bool)
+    hit[0, :H // Hk, max(j - (Tk - Tq), 0):] = True
+    assert np.isnan(y[hit]).all()
+    R.check(y[~hit], want['y'][~hit], tol['y'][~hit])
+
+
+@pytest.mark.parametrize('T,D', [(20, 16), (90, 64), (600, 64)])
+def test_a_gradient_of_a_query_that_is_not_a_number(T, D):
+    """dq of its row, and dk and dv of the keys it sees."""
+    q, k, v, dy = qkv(1, 1, 1, T, T, D, D, 73)
+    want, tol = R.attention(q, k, v, dy)
+    at = T // 2
+    q[0, 0, at, 3] = np.nan
+    got = attend(q, k, v, dy)
+    rest = np.arange(T) != at
+    assert np.isnan(got['dq'][0, 0, at]).all() and np.isnan(got['y'][0, 0, at]).all()
+    R.check(got['dq'][0, 0, rest], want['dq'][0, 0, rest], tol['dq'][0, 0, rest])
+    for n in ('dk', 'dv'):
+        assert np.isnan(got[n][0, 0, :at + 1]).all()
+        R.check(got[n][0, 0, at + 1:], want[n][0, 0, at + 1:], tol[n][0, 0, at + 1:], n)
+
+
+def check_keys_of_minus_infinity(shape):
+    """A row that sees only scores of minus infinity has no softmax (NaN); beside others such a key counts for nothing."""
+    B, H, Hk, Tq, Tk, D = shape
+    q, k, v, _ = qkv(B, H, Hk, Tq, Tk, D, D, 74)
+    q = np.abs(q) + f32(0.1)
+    dead = Tk - Tq + 1                       # the first query sees these alone
+    k[0, 0, :dead] = -np.inf
+    y = attend(q, k, v)['y']
+    assert np.isnan(y[:, :, 0]).all()
+    if Tq > 1:
+        doc = np.zeros((B, Tk), np.int32)
+        doc[:, :dead] = -1
+        want, tol = R.attention(q, np.where(np.isfinite(k), k, f32(0)), v, documents=doc)
+        R.check(y[:, :, 1:], want['y'][:, :, 1:], tol['y'][:, :, 1:])
+
+
+@pytest.mark.parametrize('shape', [(1, 1, 1, 20, 20, 16), (1, 1, 1, 90, 90, 64), (1, 2, 1, 300, 600, 64)])
+def test_keys_of_minus_infinity_weigh_nothing(shape):
+    check_keys_of_minus_infinity(shape)
