@@ -4879,7 +4879,7 @@ void Runtime::allocate() {
     return;
   }
   hip_check(hipMalloc(&input_region_, input_region_bytes_), "hipMalloc(inputs)");
-  if (opt_cfg_) need_staging();   // a forward graph's calls may all stay within device memory: at its first host call
+  if (opt_cfg_) need_staging();   // a forward graph's calls may all stay within device memory: at its first replay or host call
   for (int t : input_roots) ptr_[t] = input_region_ + input_offset_[t];
   hip_check(hipHostMalloc(&loss_host_, 256, hipHostMallocDefault), "hipHostMalloc");
   if (workspace_bytes_) hip_check(hipMalloc(&workspace_, (workspace_bytes_ + 255) & ~(size_t)255), "hipMalloc(workspace)");
@@ -5019,6 +5019,7 @@ static constexpr size_t kFetchBytes = 1 << 20;
 // One execution of the step: a replay of the captured graph (one per way the inputs come, captured at its first use), or
 // (graphs disabled) the same launches issued directly on the stream.
 void Runtime::replay(bool host) {
+  need_staging();
   if (host && user_bytes_ > kFetchBytes) {
     hip_check(hipMemcpyAsync(input_region_, staging_, user_bytes_, hipMemcpyHostToDevice, stream_), "hipMemcpyAsync(H2D)");
     host = false;
@@ -5033,6 +5034,7 @@ void Runtime::replay(bool host) {
 
 void Runtime::ensure_graph(bool host) {
   if (graph_exec_[host]) return;
+  need_staging();   // the captured copy keeps its address
   hip_check(hipStreamBeginCapture(stream_, hipStreamCaptureModeThreadLocal), "hipStreamBeginCapture");
   try {
     launch_step(stream_, host);

@@ -863,3 +863,24 @@ def check_keys_of_minus_infinity(shape):
 @pytest.mark.parametrize('shape', [(1, 1, 1, 20, 20, 16), (1, 1, 1, 90, 90, 64), (1, 2, 1, 300, 600, 64)])
 def test_keys_of_minus_infinity_weigh_nothing(shape):
     check_keys_of_minus_infinity(shape)
+
+
+@pytest.mark.parametrize('graph', ['0', '1'])
+def test_replays_timed_before_the_first_call(graph, monkeypatch):
+    """A forward graph's host memory comes with its first replay, whoever asks for it: with dropout, with inputs that go by the
+    copy engine, and with none at all."""
+    monkeypatch.setenv('TG_GRAPH', graph)
+
+    class M(Module):
+        def __init__(self):
+            self.l = nn.Linear(8, 8)
+    x = f32(rng(61).standard_normal((40000, 8)))
+    for fwd, ins in ((lambda m, i: O.dropout(m.l.fwd(i['x']), 0.5), {'x': x}), (lambda m, i: m.l.fwd(i['x']), {'x': x[:4]}),
+                     (lambda m, i: O.mul(m.l.W, 2.0), {})):
+        a, b = (compile_forward(M(), fwd, {n: list(z.shape) for n, z in ins.items()}, seed=1) for _ in range(2))
+        assert a._owner[0].time_replays(3) > 0
+        for _ in range(3):
+            got, want = a.run(ins), b.run(ins)
+            assert got.error is None and np.array_equal(got.output, want.output)
+        a.destroy()
+        b.destroy()
