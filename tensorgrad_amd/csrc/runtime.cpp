@@ -32,6 +32,7 @@
 #include <memory>
 #include <mutex>
 #include <set>
+#include <shared_mutex>
 #include <sstream>
 #include <stdexcept>
 #include <string>
@@ -223,6 +224,10 @@ class Runtime {
   void run_device(int n, const char* const* names, const void* const* data, const int64_t* nbytes, int n_out,
                   void* const* out, const int64_t* out_bytes, hipStream_t st);
   void settle();
+  std::shared_lock<std::shared_mutex> host_call() const {
+    std::lock_guard<std::mutex> g(pending_->gate);
+    return std::shared_lock<std::shared_mutex>(pending_->order);
+  }
   void get_capture(const std::string& name, void* out, int64_t nbytes);
   void reset_optimizer();
   void set_lr(const char* json);
@@ -322,7 +327,11 @@ class Runtime {
   // Calls that return before their work is done (run_device): a family of runtimes, which share parameters, keeps the
   // stream of its last one. A later one on another stream waits for it there, every other entry point on the host. (An event
   // recorded after every call would say the same, for 4 us of the stream's time.)
+  // And host calls of several threads: those of a family run beside each other, a run_device beside none, as it reads what
+  // they write (parameters) and they have waited only for what was enqueued before. They return with their work done.
   struct Pending {
+    std::mutex gate;                 // taken before `order`, so that neither kind keeps the other waiting for ever
+    std::shared_mutex order;
     std::mutex mu;
     bool any = false;
     hipStream_t stream = nullptr;
@@ -5163,10 +5172,10 @@ void Runtime::run(int n, const char* const* names, const void* const* data, cons
     throw Error(TG_INVALID_ARGUMENT, "tensorgrad: missing input '" + opt_cfg_->at(f).str() + "'");
   }
   upload_inputs(n, names, data, nbytes, false);
-  replay(true);
   int o = outputs_.at(0);
   if (out_bytes != T_[o].numel * 4) throw Error(TG_INVALID_ARGUMENT, "run: output buffer has the wrong size");
   if (!view_[o].contiguous()) throw Error(TG_INTERNAL, "run: output is not contiguous");
+  replay(true);
   hip_check(hipMemcpyAsync(out, dptr(o), (size_t)out_bytes, hipMemcpyDeviceToHost, stream_), "hipMemcpyAsync(D2H)");
   hip_check(hipStreamSynchronize(stream_), "hipStreamSynchronize");
 }
@@ -5258,6 +5267,11 @@ void Runtime::run_device(int n, const char* const* names, const void* const* dat
   };
   // The family's earlier calls use the same buffers (this runtime's) or parameters: wait for them on the stream. The seed
   // goes through pinned memory that the last call may still read: wait on the host.
+  std::unique_lock<std::shared_mutex> order(pending_->order, std::defer_lock);
+  {
+    std::lock_guard<std::mutex> g(pending_->gate);
+    order.lock();
+  }
   std::unique_lock<std::mutex> lock(pending_->mu);
   if (pending_->any && (uses_prng_ || pending_->stream != st)) {
     if (!pending_->passed) hip_check(hipEventCreateWithFlags(&pending_->passed, hipEventDisableTiming), "hipEventCreate");
@@ -5778,13 +5792,15 @@ void tg_destroy(tg_runtime* h) {
   destroy_rec(h);
 }
 
-// Enters a call on h; the host first waits for work that an earlier tg_run_device of the family left running.
+// Enters a call on h; the host first waits for work that an earlier tg_run_device of the family left running, and a later one
+// waits for the call's end.
 #define TG_ENTER_RUNNING(h)                                               \
   if (!live(h)) { tg::g_error = "graph destroyed"; return TG_ABORTED; } \
   std::lock_guard<std::mutex> lk_((h)->mu);                               \
   if (!(h)->rt) { tg::g_error = "graph destroyed"; return TG_ABORTED; }
 #define TG_ENTER(h)                                                       \
   TG_ENTER_RUNNING(h)                                                     \
+  std::shared_lock<std::shared_mutex> order_ = (h)->rt->host_call();      \
   if (tg_status s_ = guarded([&] { (h)->rt->settle(); })) return s_;
 
 int tg_param_count(const tg_runtime* h) {

@@ -884,3 +884,37 @@ def test_replays_timed_before_the_first_call(graph, monkeypatch):
             assert got.error is None and np.array_equal(got.output, want.output)
         a.destroy()
         b.destroy()
+
+
+def test_run_device_beside_a_training_thread():
+    """Another thread trains while this one reads the weights, all equal before and after every step: no call sees half of one."""
+    import threading
+
+    class M(Module):
+        def __init__(self):
+            self.w = self.param([4096, 1024])
+    n = 4096 * 1024
+    t = tg_compile(M(), lambda p, i: O.mean(p.w), {}, {'kind': 'sgd', 'lr': float(n)}, seed=0)
+    t.upload_params({'w': np.zeros(n, np.float32)})
+    f = t.attach(lambda p, i: O.add(p.w, 0.5), {})
+    out = [torch.empty(4096, 1024, device='cuda') for _ in range(60)]
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    failed = []
+
+    def train():
+        for _ in range(150):
+            r = t.step({})
+            if r.kind != 'completed':
+                failed.append(r.error)
+    th = threading.Thread(target=train)
+    th.start()
+    for i, o in enumerate(out):
+        assert f.run_device({}, [o], s.cuda_stream if i % 2 else 0).error is None
+    th.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for o in out:
+        assert float(o.min()) == float(o.max())
+    assert np.all(f.run({}).output == np.float32(0.5 - 150))
+    t.destroy()
