@@ -228,6 +228,10 @@ class Runtime {
     std::lock_guard<std::mutex> g(pending_->gate);
     return std::shared_lock<std::shared_mutex>(pending_->order);
   }
+  std::unique_lock<std::shared_mutex> lone_call() const {
+    std::lock_guard<std::mutex> g(pending_->gate);
+    return std::unique_lock<std::shared_mutex>(pending_->order);
+  }
   void get_capture(const std::string& name, void* out, int64_t nbytes);
   void reset_optimizer();
   void set_lr(const char* json);
@@ -328,7 +332,9 @@ class Runtime {
   // stream of its last one. A later one on another stream waits for it there, every other entry point on the host. (An event
   // recorded after every call would say the same, for 4 us of the stream's time.)
   // And host calls of several threads: those of a family run beside each other, a run_device beside none, as it reads what
-  // they write (parameters) and they have waited only for what was enqueued before. They return with their work done.
+  // they write (parameters) and they have waited only for what was enqueued before. They return with their work done. Nor
+  // beside one that captures its step, or the creation of a sibling, which copies on the default stream: HIP refuses that
+  // stream's work while another is captured.
   struct Pending {
     std::mutex gate;                 // taken before `order`, so that neither kind keeps the other waiting for ever
     std::shared_mutex order;
@@ -5197,6 +5203,7 @@ void Runtime::settle() {
 void Runtime::run_device(int n, const char* const* names, const void* const* data, const int64_t* nbytes, int n_out,
                          void* const* out, const int64_t* out_bytes, hipStream_t st) {
   if (opt_cfg_) throw Error(TG_INVALID_ARGUMENT, "run_device: a training graph (use step)");
+  const std::unique_lock<std::shared_mutex> order = lone_call();
   int dev = 0;
   hip_check(hipGetDevice(&dev), "hipGetDevice");
   struct Current {   // the runtime's device for the call's duration
@@ -5267,11 +5274,6 @@ void Runtime::run_device(int n, const char* const* names, const void* const* dat
   };
   // The family's earlier calls use the same buffers (this runtime's) or parameters: wait for them on the stream. The seed
   // goes through pinned memory that the last call may still read: wait on the host.
-  std::unique_lock<std::shared_mutex> order(pending_->order, std::defer_lock);
-  {
-    std::lock_guard<std::mutex> g(pending_->gate);
-    order.lock();
-  }
   std::unique_lock<std::mutex> lock(pending_->mu);
   if (pending_->any && (uses_prng_ || pending_->stream != st)) {
     if (!pending_->passed) hip_check(hipEventCreateWithFlags(&pending_->passed, hipEventDisableTiming), "hipEventCreate");
@@ -5759,6 +5761,7 @@ tg_status tg_runtime_create_sibling(tg_runtime* parent, const char* ir_json, tg_
   return guarded([&] {
     auto* h = new tg_runtime();
     try {
+      const auto order = parent->rt->lone_call();
       h->rt.reset(new tg::Runtime(ir_json, parent->rt.get()));
     } catch (...) {
       delete h;

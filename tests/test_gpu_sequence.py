@@ -918,3 +918,38 @@ def test_run_device_beside_a_training_thread():
         assert float(o.min()) == float(o.max())
     assert np.all(f.run({}).output == np.float32(0.5 - 150))
     t.destroy()
+
+
+def test_siblings_made_while_another_thread_captures():
+    """Every new sibling's first host call captures its step; another thread makes siblings of the same parent meanwhile."""
+    import threading
+
+    class M(Module):
+        def __init__(self):
+            self.l = nn.Linear(16, 16)
+    t = tg_compile(M(), lambda p, i: O.mean(p.l.fwd(i['x'])), {'x': [4, 16]}, {'kind': 'sgd', 'lr': 0.0}, seed=0)
+    x = f32(rng(62).standard_normal((4, 16)))
+    xd, out = torch.from_numpy(x).cuda(), torch.empty(15, 4, 16, device='cuda')
+    want = t.attach(lambda p, i: O.relu(p.l.fwd(i['x'])), {'x': [4, 16]}).run({'x': x}).output
+    torch.cuda.synchronize()
+    failed = []
+
+    def host():
+        for _ in range(15):
+            f = t.attach(lambda p, i: O.relu(p.l.fwd(i['x'])), {'x': [4, 16]})
+            for _ in range(2):
+                r = f.run({'x': x})
+                if r.error is not None or not np.array_equal(r.output, want):
+                    failed.append(r.error or 'host output')
+            f.destroy()
+    th = threading.Thread(target=host)
+    th.start()
+    for n in range(15):
+        f = t.attach(lambda p, i: O.relu(p.l.fwd(i['x'])), {'x': [4, 16]})
+        r = f.run_device({'x': xd}, [out[n]])
+        if r.error is not None:
+            failed.append(r.error)
+        f.destroy()                                      # waits for the call
+    th.join()
+    assert not failed and all(np.array_equal(o, want) for o in out.cpu().numpy())
+    t.destroy()
