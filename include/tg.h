@@ -123,8 +123,9 @@ tg_status tg_run(tg_runtime* rt, int n, const char* const* names, const void* co
  * `stream` (a hipStream_t; NULL: the default stream) and the call returns without waiting:
  * inputs and outputs must stay as they are until the stream has passed it. Calls on one
  * runtime and its siblings run one after another, whatever their streams and threads; every
- * other entry point waits for them first, and they for its end. A stream must stay until a later call on another one, one that
- * waits, or tg_destroy. A stream under graph capture is refused (the runtime's
+ * other entry point waits for them first, and they for its end. A stream must stay until a
+ * later call on another one, one that waits, or tg_destroy. Refused: hipStreamPerThread (one
+ * handle for a stream of each thread) and a stream under graph capture (the runtime's
  * intermediate buffers would be shared with every later call). */
 tg_status tg_run_device(tg_runtime* rt, int n, const char* const* names, const void* const* dev_data,
                         const int64_t* nbytes, int n_out, void* const* dev_out, const int64_t* out_bytes,

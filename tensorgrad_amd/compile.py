@@ -189,8 +189,9 @@ class CompiledForward:
         """`run` within device memory, for tensors that stay on the GPU (no reference counterpart): reads `inputs` (tensors
         in device memory, by name) and writes the graph's outputs, all that the forward returned, into `outputs`; result
         `output` is `outputs`. The work is enqueued on `stream` (a hipStream_t as an int; 0: the default stream) and the call
-        returns without waiting for it. Calls on one executor run one after another, also from several streams; a stream must
-        stay until a later call on another one, a host call or `destroy`. A stream under graph capture is refused."""
+        returns without waiting for it. Calls on one executor run one after another, whatever their streams; a stream must
+        stay until a later call on another one, a host call or `destroy`. hipStreamPerThread and a stream under graph capture
+        are refused."""
         def body():
             if not self.parent._rt.alive:
                 raise AbortError('run aborted: graph destroyed')
@@ -396,8 +397,9 @@ class CompiledForwardExecutor:
         """`run` within device memory, for tensors that stay on the GPU (no reference counterpart): reads `inputs` (tensors
         in device memory, by name) and writes the graph's outputs, all that the forward returned, into `outputs`; result
         `output` is `outputs`. The work is enqueued on `stream` (a hipStream_t as an int; 0: the default stream) and the call
-        returns without waiting for it. Calls on one executor run one after another, also from several streams; a stream must
-        stay until a later call on another one, a host call or `destroy`. A stream under graph capture is refused."""
+        returns without waiting for it. Calls on one executor run one after another, whatever their streams; a stream must
+        stay until a later call on another one, a host call or `destroy`. hipStreamPerThread and a stream under graph capture
+        are refused."""
         def body():
             if self._destroyed:
                 raise AbortError('run aborted: executor destroyed')

@@ -5203,6 +5203,9 @@ void Runtime::settle() {
 void Runtime::run_device(int n, const char* const* names, const void* const* data, const int64_t* nbytes, int n_out,
                          void* const* out, const int64_t* out_bytes, hipStream_t st) {
   if (opt_cfg_) throw Error(TG_INVALID_ARGUMENT, "run_device: a training graph (use step)");
+  // One handle for a stream of each thread: a later call could not tell which of them to wait for.
+  if (st == hipStreamPerThread) throw Error(TG_INVALID_ARGUMENT, "run_device: hipStreamPerThread is another stream in each thread");
+  if (st == hipStreamLegacy) st = nullptr;
   const std::unique_lock<std::shared_mutex> order = lone_call();
   int dev = 0;
   hip_check(hipGetDevice(&dev), "hipGetDevice");

@@ -953,3 +953,14 @@ def test_siblings_made_while_another_thread_captures():
     th.join()
     assert not failed and all(np.array_equal(o, want) for o in out.cpu().numpy())
     t.destroy()
+
+
+def test_run_device_refuses_the_stream_of_each_thread():
+    ex, ins, outs = _scan_executor()
+    r = ex.run_device(ins, outs, 2)                      # hipStreamPerThread
+    assert r.kind == 'failed' and 'PerThread' in str(r.error)
+    want = ex.run({n: t.cpu().numpy() for n, t in ins.items()}).output
+    assert ex.run_device(ins, outs, 1).error is None     # hipStreamLegacy: the default stream
+    torch.cuda.synchronize()
+    assert np.array_equal(outs[0].cpu().numpy(), want)
+    ex.destroy()
