@@ -126,7 +126,8 @@ tg_status tg_run(tg_runtime* rt, int n, const char* const* names, const void* co
  * other entry point waits for them first, and they for its end. A stream must stay until a
  * later call on another one, one that waits, or tg_destroy. Refused: hipStreamPerThread (one
  * handle for a stream of each thread) and a stream under graph capture (the runtime's
- * intermediate buffers would be shared with every later call). */
+ * intermediate buffers would be shared with every later call). While a call's stream is
+ * captured after it, calls that would wait for it are refused too. */
 tg_status tg_run_device(tg_runtime* rt, int n, const char* const* names, const void* const* dev_data,
                         const int64_t* nbytes, int n_out, void* const* dev_out, const int64_t* out_bytes,
                         void* stream);

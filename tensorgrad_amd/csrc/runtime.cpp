@@ -224,6 +224,7 @@ class Runtime {
   void run_device(int n, const char* const* names, const void* const* data, const int64_t* nbytes, int n_out,
                   void* const* out, const int64_t* out_bytes, hipStream_t st);
   void settle();
+  void check_pending() const;
   std::shared_lock<std::shared_mutex> host_call() const {
     std::lock_guard<std::mutex> g(pending_->gate);
     return std::shared_lock<std::shared_mutex>(pending_->order);
@@ -5186,11 +5187,21 @@ void Runtime::run(int n, const char* const* names, const void* const* data, cons
   hip_check(hipStreamSynchronize(stream_), "hipStreamSynchronize");
 }
 
+// A wait for the family's last run_device would be recorded into a graph that its stream is being captured into since, with
+// the work that waits, and a wait on the host would end the capture.
+void Runtime::check_pending() const {
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(pending_->stream, &cap) != hipSuccess) (void)hipGetLastError();   // a stream that is gone
+  else if (cap != hipStreamCaptureStatusNone)
+    throw Error(TG_INVALID_ARGUMENT, "the stream of an earlier run_device is being captured into a graph: end that first");
+}
+
 // Waits on the host for the family's last run_device.
 void Runtime::settle() {
   if (!pending_) return;
   std::lock_guard<std::mutex> g(pending_->mu);
   if (!pending_->any) return;
+  check_pending();
   pending_->any = false;
   if (hipStreamSynchronize(pending_->stream) == hipSuccess) return;
   (void)hipGetLastError();   // a stream that is gone
@@ -5279,6 +5290,7 @@ void Runtime::run_device(int n, const char* const* names, const void* const* dat
   // goes through pinned memory that the last call may still read: wait on the host.
   std::unique_lock<std::mutex> lock(pending_->mu);
   if (pending_->any && (uses_prng_ || pending_->stream != st)) {
+    check_pending();
     if (!pending_->passed) hip_check(hipEventCreateWithFlags(&pending_->passed, hipEventDisableTiming), "hipEventCreate");
     if (uses_prng_ || hipEventRecord(pending_->passed, pending_->stream) != hipSuccess ||
         hipStreamWaitEvent(st, pending_->passed, 0) != hipSuccess) {

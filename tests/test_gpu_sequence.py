@@ -964,3 +964,32 @@ def test_run_device_refuses_the_stream_of_each_thread():
     torch.cuda.synchronize()
     assert np.array_equal(outs[0].cpu().numpy(), want)
     ex.destroy()
+
+
+def test_calls_are_refused_while_the_last_ones_stream_is_captured():
+    """They would wait for it, on their stream or on the host; after the capture they run."""
+    ex, ins, outs = _scan_executor()
+    host = {n: t.cpu().numpy() for n, t in ins.items()}
+    want = ex.run(host).output
+    s, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    assert ex.run_device(ins, outs, s.cuda_stream).error is None
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    y = torch.zeros(4, device='cuda')
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        graph.capture_begin(capture_error_mode='relaxed')
+        y.add_(1)
+        refused = [ex.run_device(ins, outs, other.cuda_stream), ex.run(host)]
+        graph.capture_end()
+    assert all(r.kind == 'failed' and 'captured' in str(r.error) for r in refused)
+    for turn in range(3):
+        graph.replay()
+        for o in outs:
+            o.fill_(float('nan'))
+        torch.cuda.synchronize()
+        assert ex.run_device(ins, outs, other.cuda_stream).error is None
+        assert np.array_equal(ex.run(host).output, want)
+        assert np.array_equal(outs[0].cpu().numpy(), want) and np.all(y.cpu().numpy() == turn + 1)
+    ex.destroy()
