@@ -31,7 +31,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kTile = 32;          // rows of a tile
 constexpr int kFrag = 512;         // halves of a fragment (1 KiB)
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kNone = -INFINITY;
+constexpr float kNone = -INFINITY, kLowest = -0x1.fffffep127f;
 
 // What the kernels need to know of a packed tile. One power of two serves all its rows, that of the largest, unless they
 // differ by more than 2^12 (uneven): then every row has its own, and what was multiplied by it takes the row's `rel`, the

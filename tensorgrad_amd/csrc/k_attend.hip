@@ -359,7 +359,8 @@ struct FewArgs {
 
 // Eight lanes share a key row: each reads E of its features as 16-byte pieces (8 rows of 128 bytes a load instruction) and
 // multiplies them with the same features of all R query rows, which it keeps. Every group of eight lanes carries a running
-// maximum, sum and result of its own; the 32 groups of a block are joined once at its end. A part is the same number of keys
+// maximum, sum and result of its own (the maximum from f32's lowest on, so that weights of scores of minus infinity are 0
+// whatever came before); the 32 groups of a block are joined once at its end. A part is the same number of keys
 // for every batch entry, so that blocks past a short one end at once and those that work are alike. 8 caches of up to 16000
 // keys, 4 key heads of 128, 16 query heads: 66 us, 6.0 TB/s.
 template <int E, int R, bool WIDE>
@@ -392,7 +393,7 @@ __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
     p[r] = s.first + i;
     doc[r] = doc_at(s, p[r]);
     below[r] = sees_below(s, p[r]);
-    m[r] = kNone;
+    m[r] = kLowest;
     sum[r] = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[r][e] = 0;
@@ -436,8 +437,8 @@ __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
       if (a.slopes) x -= a.slopes[hk * G + min(r, A.M - 1) % G] * fabsf((float)(p[r] - j));
       x *= kLog2e;
       if (!all && (j >= below[r] || (s.doc && (doc[r] < 0 || s.doc[j] != doc[r])))) continue;
-      if (x > m[r] + 8 || m[r] == kNone) {
-        const float top = __builtin_isfinite(x) ? x : m[r] == kNone ? 0.0f : m[r];   // an infinite score shows in the weight
+      if (x > m[r] + 8) {
+        const float top = x < INFINITY ? x : m[r] == kLowest ? 0.0f : m[r];   // an infinite score shows in the weight
         const float keep = __builtin_amdgcn_exp2f(m[r] - top);
         m[r] = top;
         sum[r] *= keep;
@@ -456,7 +457,7 @@ __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const float other = __shfl_xor(m[r], o), top = fmaxf(m[r], other);
-      const float here = top == kNone ? 0.0f : __builtin_amdgcn_exp2f(m[r] - top), there = top == kNone ? 0.0f : __builtin_amdgcn_exp2f(other - top);
+      const float here = __builtin_amdgcn_exp2f(m[r] - top), there = __builtin_amdgcn_exp2f(other - top);
       m[r] = top;
       sum[r] = fmaf(__shfl_xor(sum[r], o), there, sum[r] * here);
 #pragma unroll
@@ -477,27 +478,26 @@ __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
   __syncthreads();
   for (int z = tid; z < min(R, A.M) * (8 * E); z += 256) {
     const int r = z / (8 * E), d = z % (8 * E), i = r / G, head = hk * G + r % G;
-    float top = kNone, all = 0, o = 0;
+    float top = kLowest, all = 0, o = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) top = fmaxf(top, sm[u][r]);
-    if (top != kNone) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float f = __builtin_amdgcn_exp2f(sm[u][r] - top);
-        all = fmaf(ss[u][r], f, all);
-        o = fmaf(sa[u][r][d], f, o);
-      }
-      o /= all;
+    for (int u = 0; u < 4; ++u) {
+      const float f = __builtin_amdgcn_exp2f(sm[u][r] - top);
+      all = fmaf(ss[u][r], f, all);
+      o = fmaf(sa[u][r][d], f, o);
     }
+    const bool none = !sees_any(s, sees_below(s, s.first + i), doc_at(s, s.first + i));
+    o = (A.splits > 1 ? all == 0 : none) ? 0.0f : o / all;
     const int64_t at = ((int64_t)split * a.B * a.Hk + slab) * A.M + r;
     if (d < a.Dv) {
       if (A.splits > 1) A.part[at * a.Dv + d] = o;
       else if (a.y.p) a.y.p[b * a.y.b + head * a.y.h + i * a.y.t + d] = o;
     }
     if (d == 0) {
-      const float lse = top == kNone ? kNone : top + __builtin_amdgcn_logf(all);
+      const float lse = top + __builtin_amdgcn_logf(all);
       if (A.splits > 1) A.plse[at] = lse;
-      else if (a.lse) a.lse[((int64_t)b * a.H + head) * a.Tq + i] = top == kNone ? INFINITY : lse;
+      else if (a.lse) a.lse[((int64_t)b * a.H + head) * a.Tq + i] = none ? INFINITY : lse;
     }
   }
 }

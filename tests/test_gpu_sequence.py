@@ -850,9 +850,9 @@ def check_keys_of_minus_infinity(shape):
     q, k, v, _ = qkv(B, H, Hk, Tq, Tk, D, D, 74)
     q = np.abs(q) + f32(0.1)
     dead = Tk - Tq + 1                       # the first query sees these alone
-    k[0, 0, :dead] = -np.inf
+    k[0, 0, :dead] = -np.inf                 # of one key head
     y = attend(q, k, v)['y']
-    assert np.isnan(y[:, :, 0]).all()
+    assert np.isnan(y[0, :H // Hk, 0]).all() and np.isfinite(y[0, H // Hk:]).all() and np.isfinite(y[1:]).all()
     if Tq > 1:
         doc = np.zeros((B, Tk), np.int32)
         doc[:, :dead] = -1
@@ -993,3 +993,21 @@ def test_calls_are_refused_while_the_last_ones_stream_is_captured():
         assert np.array_equal(ex.run(host).output, want)
         assert np.array_equal(outs[0].cpu().numpy(), want) and np.all(y.cpu().numpy() == turn + 1)
     ex.destroy()
+
+
+@pytest.mark.parametrize('H,D,Tk', [(1, 64, 700), (4, 128, 900), (2, 96, 70), (8, 32, 5000)])
+def test_far_negative_scores_after_one_of_minus_infinity(H, D, Tk):
+    """Keys 0, 1, 2, .. of every group of lanes are minus infinity, all other scores some -300: the weights are theirs alone."""
+    q, k, v, _ = qkv(2, H, 1, 1, Tk, D, D, 81)
+    q, k = f32(np.full_like(q, 4)), f32(k / 16 - 300 / 4 / D)
+    doc = np.zeros((2, Tk), np.int32)
+    doc[:, :60] = -1
+    want, tol = R.attention(q, k, v, scale=1.0, documents=doc)
+    k[:, :, :60] = -np.inf
+    y = attend(q, k, v, None, dict(scale=1.0))['y']
+    R.check(y, want['y'], tol['y'])
+
+
+@pytest.mark.parametrize('shape', [(1, 1, 1, 1, 3000, 64), (1, 1, 1, 4, 900, 128), (8, 4, 4, 1, 70, 96)])
+def test_keys_of_minus_infinity_weigh_nothing_for_few_rows(shape):
+    check_keys_of_minus_infinity(shape)
