@@ -36,7 +36,7 @@ constexpr float kNone = -INFINITY, kLowest = -0x1.fffffep127f;
 // What the kernels need to know of a packed tile. One power of two serves all its rows, that of the largest, unless they
 // differ by more than 2^12 (uneven): then every row has its own, and what was multiplied by it takes the row's `rel`, the
 // tile's over the row's, afterwards. So a row keeps its precision whatever its neighbours are. odd: infinities, NaN or rows
-// 2^90 apart: blocks that walk such a tile run in plain f32.
+// 2^90 apart: blocks that walk such a tile, or have such rows of their own, run in plain f32.
 struct TileInfo {
   float scale, inv;                // power of two on the largest row's values, and its inverse
   int uneven, odd;
@@ -192,9 +192,11 @@ __device__ __forceinline__ float groups_sum(float x) {
   r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// B fragments of 16 rows (lane l: row l % 16), each row with its own power of two; returns its exponent.
+// B fragments of 16 rows (lane l: row l % 16), each row with its own power of two; returns its exponent. *infinite: the row holds
+// an infinity, which has no hi and lo parts.
 template <int N>
-__device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bool wide, half8 (&hi)[N], half8 (&lo)[N]) {
+__device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bool wide, half8 (&hi)[N], half8 (&lo)[N],
+                                         bool* infinite = nullptr) {
   const int g = (threadIdx.x >> 4) & 3;
   float x[N][8], m = 0;
 #pragma unroll
@@ -216,8 +218,9 @@ __device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bo
 #pragma unroll
   for (int c = 0; c < N; ++c)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(x[c][i]));
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[c][i]));
   m = groups_max(m);
+  if (infinite) *infinite = m == INFINITY;
   const int e = m > 0 ? min(14 - exponent(m), 126) : 0;
   const float s = pow2(e);
 #pragma unroll
@@ -380,13 +383,13 @@ __device__ __forceinline__ bool key_seen(const Sight& s, const float* side, int 
   return (j0 + z < below) & (!s.doc | ((doc >= 0) & (id == doc)));
 }
 // First and one past the last of the tiles [t0, t1) whose documents meet [lo, hi] (all of them without documents); odd: one
-// of those is. By the whole block.
+// of those is, or the block's own rows are (`own`, of each lane). By the whole block.
 struct Range {
   int t0, t1;
   bool odd;
 };
 __device__ __forceinline__ Range tile_range(const Sight& s, int t0, int t1, const TileInfo* docs, const TileInfo* x, const TileInfo* y,
-                                            int dmin, int dmax, int (&buf)[5]) {
+                                            int dmin, int dmax, bool own, int (&buf)[5]) {
   const int tid = threadIdx.x;
   if (tid < 5) buf[tid] = tid == 0 || tid == 2 ? INT32_MAX : tid == 4 ? 0 : INT32_MIN;
   __syncthreads();
@@ -394,6 +397,7 @@ __device__ __forceinline__ Range tile_range(const Sight& s, int t0, int t1, cons
     atomicMin(&buf[0], dmin);
     atomicMax(&buf[1], dmax);
   }
+  if (own) atomicOr(&buf[4], 1);
   __syncthreads();
   const int lo = buf[0], hi = buf[1];
   int first = INT32_MAX, end = INT32_MIN, odd = 0;

@@ -243,10 +243,14 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   const TileInfo* ki = A.ki + (int64_t)slab * tiles;
   const TileInfo* vi = A.vi + (int64_t)slab * tiles;
   const int last = s.first + (int)fastdiv((uint32_t)min(blk * 128 + 127, A.M - 1), A.group);   // of the block
+  half8 qh[N], ql[N];
+  bool infinite;
+  const int qe = load_rows<N>(a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t, valid, a.D, A.wide, qh, ql, &infinite);
   int t0 = 0, t1 = s.n;
   if (s.causal) t1 = min(t1, max(last + 1, s.prefix));
   if (s.positional && last < 0) t1 = 0;
-  const Range range_ = tile_range(s, 0, (t1 + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax, range);
+  const Range range_ = tile_range(s, 0, (t1 + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax,
+                                  infinite && sees_any(s, below, doc), range);
   t0 = range_.t0;
   t1 = range_.t1;
   if (A.splits > 1) {
@@ -259,8 +263,6 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
     return;
   }
 
-  half8 qh[N], ql[N];
-  const int qe = load_rows<N>(a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t, valid, a.D, A.wide, qh, ql);
   const float slope = SLOPES ? a.slopes[head] * kLog2e : 0.0f;
   const int64_t tile0 = (int64_t)slab * tiles + t0;
   const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;

@@ -126,7 +126,9 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
   const int j0 = blk * 128 + w * 16, jt = j0 / kTile * kTile, j = j0 + l;   // masks are judged by whole tiles of keys
   const bool valid = j < a.Tk;
   const int doc = s.doc && valid ? s.doc[j] : -1;
-  TileInfo mine = A.ki[(int64_t)slab * A.ktiles + min(jt / kTile, A.ktiles - 1)];
+  const int64_t kt = (int64_t)slab * A.ktiles + min(jt / kTile, A.ktiles - 1);
+  TileInfo mine = A.ki[kt];
+  const bool own = jt < a.Tk && (mine.odd || (DK && A.vi[kt].odd));
   if (jt >= a.Tk) {
     mine.dmin = INT32_MAX;
     mine.dmax = INT32_MIN;
@@ -135,7 +137,7 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
   const TileInfo* gi = A.gi + (int64_t)slab * A.qtiles;
   int from, to;
   if (!part_rows(A, s, blk * 128, split, from, to)) return;   // nothing, and the join knows
-  const Range range_ = tile_range(s, from, to, gi, qi, gi, mine.dmin, mine.dmax, range);
+  const Range range_ = tile_range(s, from, to, gi, qi, gi, mine.dmin, mine.dmax, own, range);
   int t0 = range_.t0, t1 = range_.t1;
   if (!document_part(A, s, split, slab, blk, t0, t1)) return;
   if (__builtin_expect(range_.odd, 0)) {
@@ -380,6 +382,7 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   const float* mine = A.qside + ((int64_t)slab * A.qtiles + qt) * (kSide * kTile) + row0 % kTile + l;
   const float lse = mine[QS_LSE * kTile], dot = mine[QS_DOT * kTile];
   const TileInfo gt = A.gi[(int64_t)slab * A.qtiles + qt];
+  const bool own = rt < A.M && (gt.odd || A.qi[(int64_t)slab * A.qtiles + qt].odd);
   Span me;
   me.pmin = s.first + (int)fastdiv((uint32_t)min(rt, A.M - 1), A.group);
   me.pmax = s.first + (int)fastdiv((uint32_t)min(rt + kTile - 1, A.M - 1), A.group);
@@ -393,7 +396,7 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   int end = s.n;
   if (s.causal) end = min(end, max(last + 1, s.prefix));
   if (s.positional && last < 0) end = 0;
-  const Range range_ = tile_range(s, 0, (end + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax, range);
+  const Range range_ = tile_range(s, 0, (end + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax, own, range);
   int t0 = range_.t0, t1 = range_.t1;
   if (A.qsplits > 1) {
     const int each = (t1 - t0 + A.qsplits - 1) / A.qsplits;

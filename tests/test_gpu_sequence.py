@@ -1011,3 +1011,27 @@ def test_far_negative_scores_after_one_of_minus_infinity(H, D, Tk):
 @pytest.mark.parametrize('shape', [(1, 1, 1, 1, 3000, 64), (1, 1, 1, 4, 900, 128), (8, 4, 4, 1, 70, 96)])
 def test_keys_of_minus_infinity_weigh_nothing_for_few_rows(shape):
     check_keys_of_minus_infinity(shape)
+
+
+@pytest.mark.parametrize('T,D', [(24, 16), (90, 64), (300, 128), (600, 40)])
+@pytest.mark.parametrize('sign', [1, -1])
+@pytest.mark.parametrize('what', ['q', 'k'])
+def test_infinite_rows_under_a_cap(T, D, sign, what):
+    """One infinite feature of a query, or of a key: its scores are plus or minus the cap by the other's sign, with a slope of
+    0. As with a feature of 1e6, whose tanh is +-1 to the last bit; that reference's bounds are those of its own size, so the
+    bounds here are of the rows before. Gradients of y by the row itself are 0 (the cap is flat there)."""
+    q, k, v, dy = qkv(1, 2, 1, T, T, D, D, 91)
+    how = dict(softcap=5.0)
+    x = dict(q=q, k=k)[what]
+    tol = R.attention(q, k, v, dy, **how)[1]
+    at = T // 3
+    x[0, 0, at, 2] = sign * 1e6
+    want, _ = R.attention(q, k, v, dy, **how)
+    x[0, 0, at, 2] = sign * np.inf
+    got = attend(q, k, v, dy, how)
+    for n in ('y', 'dv'):
+        R.check(got[n], want[n], 4 * tol[n].max() + 0 * tol[n], n)
+    own = 'd' + what
+    assert np.all(got[own][0, 0, at] == 0)
+    rest = np.arange(T) != at
+    R.check(got[own][0, 0, rest], want[own][0, 0, rest], 4 * tol[own].max() + 0 * tol[own][0, 0, rest], own)
