@@ -166,13 +166,14 @@ __device__ __forceinline__ float finite_abs(float x) {
 
 // Sums over several tiles in one accumulator: the weights (f16 parts of x 2^e) times a tile packed at 2^t are in units of
 // 2^-(e + t), which must be the accumulator's 2^-c. A lane's c only falls, when a tile's largest weight `big` would pass
-// 2^14: what comes later and is smaller is rounded like the largest of the sum (2^-37 of it), what was hidden has weight 0
-// and counts for nothing. c starts at kUnset, the accumulator at 0. Returns e; *change: the accumulator's factor.
+// 2^14, or e f32's exponents (weights below 2^-113 of large rows): what comes later and is smaller is rounded like the largest
+// of the sum (2^-37 of it), what was hidden has weight 0 and counts for nothing. c starts at kUnset, the accumulator at 0.
+// Returns e; *change: the accumulator's factor.
 constexpr int kUnset = 1000;
 __device__ __forceinline__ int fit_unit(int& c, float big, int t, float* change) {
   int e = c - t;
-  if (big > 0 && e > 14 - exponent(big)) {
-    e = min(12 - exponent(big), 110);
+  if (big > 0 && e > min(14 - exponent(big), 127)) {
+    e = min(12 - exponent(big), 125);
     *change *= __builtin_amdgcn_ldexpf(1.0f, e + t - c);   // 0 where acc no longer counts
     c = e + t;
   }

@@ -1035,3 +1035,16 @@ def test_infinite_rows_under_a_cap(T, D, sign, what):
     assert np.all(got[own][0, 0, at] == 0)
     rest = np.arange(T) != at
     R.check(got[own][0, 0, rest], want[own][0, 0, rest], 4 * tol[own].max() + 0 * tol[own][0, 0, rest], own)
+
+
+def test_tiny_weights_of_large_gradients():
+    """A key that every query weighs at 2^-100 (the first tile of rows) or 2^-120 (the second), with dy of 2^94 and 2^114: its dv
+    is a sum of ordinary size from both."""
+    q, k, v, dy = (np.zeros((1, 1, 64, 64), np.float32) for _ in range(4))
+    k[0, 0, 5, 0] = 1
+    q[0, 0, :32, 0], q[0, 0, 32:, 0] = -94 * np.log(2), -114 * np.log(2)
+    dy += f32(rng(95).uniform(1, 2, dy.shape))
+    dy[0, 0, :32] *= 2.0 ** 94
+    dy[0, 0, 32:] *= 2.0 ** 114
+    how = dict(causal=False, scale=1.0)
+    check_attention(q, k, v, dy, how, {})
