@@ -82,10 +82,11 @@ __global__ __launch_bounds__(256) void rope_pairs(RopeArgs R) {
 //    those of its own group;
 //  * then the steps are run again from registers, now with the true state, and stored.
 // 4 x 8192 x 1024: forward 403 MB in 87 us (4.6 TB/s), backward 671 MB in 131 us (5.1 TB/s); a large copy reaches 5.0.
-// Gates above 1 in magnitude can take a product A out of f32's range while no state is (h_in = 0, or a small gate later). A
-// block whose products leave [2^-100, 2^100] that way waits for the true state, runs its steps in order and publishes
-// (0, its state); a group whose product does, likewise. Where all gates are at most 1, A only shrinks, and what is lost below
-// 2^-126 is that part of h_in.
+// A state of 1e30 may fall to an ordinary value by a product of gates that f32 does not hold, so products are held as
+// s = A 2^100: A is exact to f32's roundings down to 2^-226, and what is lost below is at most 2^-250 of h_in, under 2^-122.
+// Gates above 1 in magnitude can take a product out of the range upwards (from 2^28 on) while no state is (h_in = 0, or a small
+// gate later), or bring back what fell out of it. A block with such products waits for the true state, runs its steps in order
+// and publishes (0, its state); a group with one, likewise.
 // A pair is one 64-bit word, stored and loaded whole at device scope; all ones mean "not there yet". A block takes its place
 // from a counter as it starts, and waits only for blocks of lower places: those are running, and publish their own pair
 // after waiting for lower places at most, a group's pair too. So every wait ends.
@@ -102,16 +103,26 @@ __device__ __forceinline__ void publish(word* at, float A, float H) {
   if (v == kEmpty) v = kEmpty - 1;             // a NaN either way
   __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-// Whether a product of gates, seen factor by factor, can be used: it must not have left the range upwards, nor downwards
-// where a factor above 1 may have brought it back.
+constexpr float kOne = 0x1p100f, kPerOne = 0x1p-100f;   // s of A = 1
+// A state through a product of gates, A state + H: the smaller factor takes the power of two, where nothing of it is lost that
+// the product would keep.
+__device__ __forceinline__ float through(float s, float state, float H) {
+  const bool large = fabsf(s) >= 1;
+  return fmaf(large ? s * kPerOne : s, large ? state : state * kPerOne, H);
+}
+__device__ __forceinline__ float product(float s, float z) {
+  const bool large = fabsf(s) >= fabsf(z);
+  return (large ? s : z) * kPerOne * (large ? z : s);
+}
+// Whether a product of gates, seen factor by factor, can be used: it must not have left the range upwards (then s is infinite,
+// or NaN), nor downwards where a factor above 1 may have brought it back.
 struct Reach {
-  float most = 1, least = 1, gate = 0;
-  __device__ __forceinline__ void see(float A, float g) {
-    most = fmaxf(most, fabsf(A));
-    least = fminf(least, fabsf(A));
+  float least = kOne, gate = 0;
+  __device__ __forceinline__ void see(float s, float g) {
+    least = fminf(least, fabsf(s));
     gate = fmaxf(gate, fabsf(g));
   }
-  __device__ __forceinline__ bool out(float A) const { return A != A || (gate > 1 && (most > 0x1p100f || least < 0x1p-100f)); }
+  __device__ __forceinline__ bool out(float s) const { return !(fabsf(s) < INFINITY) || (gate > 1 && least < 0x1p-126f); }
 };
 // (A, H) followed by n pairs, `step` words apart, in order. Loads go out together; what is not there yet is asked for again.
 __device__ __forceinline__ void follow(float& A, float& H, Reach& reach, const word* at, int64_t step, int n) {
@@ -126,9 +137,9 @@ __device__ __forceinline__ void follow(float& A, float& H, Reach& reach, const w
         __builtin_amdgcn_s_sleep(2);
         v[k] = look(at + (k0 + k) * step);
       }
-      H = fmaf(gates(v[k]), H, value(v[k]));
-      A *= gates(v[k]);
-      reach.see(A, gates(v[k]));
+      H = through(gates(v[k]), H, value(v[k]));
+      A = product(A, gates(v[k]));
+      reach.see(A, gates(v[k]) * kPerOne);
     }
   }
 }
@@ -196,7 +207,7 @@ __global__ __launch_bounds__(256) void scan_chunks(ScanArgs s) {
       g[k] = 1;
     }
   }
-  float A = 1, H = 0;
+  float A = kOne, H = 0;
   Reach own;
 #pragma unroll
   for (int k = 0; k < S; ++k) {
@@ -211,34 +222,35 @@ __global__ __launch_bounds__(256) void scan_chunks(ScanArgs s) {
   word* groups = pairs + s.chunks * row;
   const int group = chunk / kGroup, in_group = chunk % kGroup;
   const bool closes = in_group == kGroup - 1;
-  float state = BACK ? 0.0f : h0, skip = 1;
+  float state = BACK ? 0.0f : h0, skip = kOne;
   Reach none;
   if (!apart) {
     if (s.chunks > 1) {
       if (w == 0) {
-        float a4 = 1, h4 = 0;
+        float a4 = kOne, h4 = 0;
         Reach reach;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float f = fold[k][0][lane];
-          h4 = fmaf(f, h4, fold[k][1][lane]);
-          a4 *= f;
-          reach.see(a4, f);
+          h4 = through(f, h4, fold[k][1][lane]);
+          a4 = product(a4, f);
+          reach.see(a4, f * kPerOne);
         }
         const bool serial = __any(reach.out(a4));     // nor their product
         if (!serial) publish(pairs + chunk * row, a4, h4);
-        float ga = 1, gh = 0;
+        float ga = kOne, gh = 0;
         follow(ga, gh, reach, pairs + (int64_t)group * kGroup * row, row, in_group);   // the group's chunks before this one
-        reach.see(ga * a4, a4);
-        const bool whole = !__any(reach.out(ga * a4));     // the group's product
-        if (whole && closes) publish(groups + group * row, ga * a4, fmaf(a4, gh, h4));
+        const float all = product(ga, a4);                // the group's product
+        reach.see(all, a4 * kPerOne);
+        const bool whole = !__any(reach.out(all));
+        if (whole && closes) publish(groups + group * row, all, through(a4, gh, h4));
         follow(skip, state, none, groups, row, group);
-        if (whole) state = fmaf(ga, state, gh);
+        if (whole) state = through(ga, state, gh);
         else follow(skip, state, none, pairs + (int64_t)group * kGroup * row, row, in_group);
         came[lane] = state;
         if (!whole) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) state = fmaf(fold[k][0][lane], state, fold[k][1][lane]);
+          for (int k = 0; k < 4; ++k) state = through(fold[k][0][lane], state, fold[k][1][lane]);
           if (serial) publish(pairs + chunk * row, 0, state);
           if (closes) publish(groups + group * row, 0, state);
         }
@@ -246,7 +258,7 @@ __global__ __launch_bounds__(256) void scan_chunks(ScanArgs s) {
       __syncthreads();
       state = came[lane];
     }
-    for (int k = 0; k < w; ++k) state = fmaf(fold[k][0][lane], state, fold[k][1][lane]);
+    for (int k = 0; k < w; ++k) state = through(fold[k][0][lane], state, fold[k][1][lane]);
   } else {
     if (w == 0) {
       if (s.chunks > 1) {

@@ -1048,3 +1048,37 @@ def test_tiny_weights_of_large_gradients():
     dy[0, 0, 32:] *= 2.0 ** 114
     how = dict(causal=False, scale=1.0)
     check_attention(q, k, v, dy, how, {})
+
+
+@pytest.mark.parametrize('B,T,C', [(1, 60, 3), (1, 700, 5), (2, 2048, 70), (4, 4096, 256)])
+@pytest.mark.parametrize('back', [1.0, 2.0], ids=['stays', 'returns'])
+def test_recurrence_of_large_states_that_fade(B, T, C, back):
+    """A state of 1e30 falls by 1e-48 (1e-40), in steps of 0.1 side by side, to an ordinary value that nothing else covers (and
+    then grows again, from far below): the product of the gates alone is below f32's range. In the gradient's direction, dh is
+    1e30 at the end."""
+    r = rng(43, T)
+    a = f32(np.ones((B, T, C)))
+    lo, n = (T // 4, 40) if T < 100 else (T // 3, 48)
+    a[:, lo:lo + n] = 0.1
+    a[:, lo + n:lo + n + 20, ::2] = back
+    dh = np.zeros_like(a)
+    dh[:, -1] = 1e30 * r.uniform(1, 2, (B, C))
+    h0 = f32(1e30 * r.uniform(1, 2, (B, C)))
+    x = np.zeros_like(a)
+    got = scan_and_gradients(a, x, dh, h0)
+    want, tol = R.recurrence(a, x, h0, dh)
+    for n in want:
+        R.check(got[n], want[n], tol[n], n)
+
+
+@pytest.mark.parametrize('gate', [0.02, 0.3])
+def test_recurrence_that_forgets_at_once(gate):
+    """Products of gates far below f32's range in every span, over ordinary values and none."""
+    r = rng(44)
+    a = f32(gate * r.uniform(0.5, 1.5, (2, 1500, 70)))
+    x, dh, h0 = f32(r.standard_normal(a.shape)), f32(r.standard_normal(a.shape)), f32(1e25 * r.standard_normal((2, 70)))
+    x[:, 300:800] = 0
+    got = scan_and_gradients(a, x, dh, h0)
+    want, tol = R.recurrence(a, x, h0, dh)
+    for n in want:
+        R.check(got[n], want[n], tol[n], n)
