@@ -86,7 +86,8 @@ __global__ __launch_bounds__(256) void rope_pairs(RopeArgs R) {
 // s = A 2^100: A is exact to f32's roundings down to 2^-226, and what is lost below is at most 2^-250 of h_in, under 2^-122.
 // Gates above 1 in magnitude can take a product out of the range upwards (from 2^28 on) while no state is (h_in = 0, or a small
 // gate later), or bring back what fell out of it. A block with such products waits for the true state, runs its steps in order
-// and publishes (0, its state); a group with one, likewise.
+// and publishes (NaN, its state), which replaces any state; a group with one, likewise. s is 0 only after a gate of 0: a state
+// that is infinite stays so through smaller products.
 // A pair is one 64-bit word, stored and loaded whole at device scope; all ones mean "not there yet". A block takes its place
 // from a counter as it starts, and waits only for blocks of lower places: those are running, and publish their own pair
 // after waiting for lower places at most, a group's pair too. So every wait ends.
@@ -94,6 +95,7 @@ __global__ __launch_bounds__(256) void rope_pairs(RopeArgs R) {
 typedef unsigned long long word;
 constexpr int kGroup = 8;
 constexpr word kEmpty = ~0ull;
+constexpr float kSet = __builtin_nanf("");   // a product that replaces the state
 
 __device__ __forceinline__ word look(const word* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ float gates(word v) { return __uint_as_float((uint32_t)v); }
@@ -104,15 +106,18 @@ __device__ __forceinline__ void publish(word* at, float A, float H) {
   __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 constexpr float kOne = 0x1p100f, kPerOne = 0x1p-100f;   // s of A = 1
+__device__ __forceinline__ float not_zero(float s) { return s == 0 ? copysignf(0x1p-149f, s) : s; }
 // A state through a product of gates, A state + H: the smaller factor takes the power of two, where nothing of it is lost that
 // the product would keep.
 __device__ __forceinline__ float through(float s, float state, float H) {
   const bool large = fabsf(s) >= 1;
-  return fmaf(large ? s * kPerOne : s, large ? state : state * kPerOne, H);
+  const float h = fmaf(large ? s * kPerOne : s, large ? state : state * kPerOne, H);
+  return s != s ? H : h;
 }
 __device__ __forceinline__ float product(float s, float z) {
   const bool large = fabsf(s) >= fabsf(z);
-  return (large ? s : z) * kPerOne * (large ? z : s);
+  const float p = (large ? s : z) * kPerOne * (large ? z : s);
+  return s == 0 || z == 0 ? p : not_zero(p);
 }
 // Whether a product of gates, seen factor by factor, can be used: it must not have left the range upwards (then s is infinite,
 // or NaN), nor downwards where a factor above 1 may have brought it back.
@@ -207,14 +212,16 @@ __global__ __launch_bounds__(256) void scan_chunks(ScanArgs s) {
       g[k] = 1;
     }
   }
-  float A = kOne, H = 0;
+  float A = kOne, H = 0, gate = 1;   // gate: the smallest
   Reach own;
 #pragma unroll
   for (int k = 0; k < S; ++k) {
     H = fmaf(g[k], H, x[k]);
     A *= g[k];
     own.see(A, g[k]);
+    gate = fminf(gate, fabsf(g[k]));
   }
+  if (gate > 0) A = not_zero(A);
   fold[w][0][lane] = A;
   fold[w][1][lane] = H;
   const bool apart = __syncthreads_or(own.out(A));   // the wavefronts' products cannot be used
@@ -251,8 +258,8 @@ __global__ __launch_bounds__(256) void scan_chunks(ScanArgs s) {
         if (!whole) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) state = through(fold[k][0][lane], state, fold[k][1][lane]);
-          if (serial) publish(pairs + chunk * row, 0, state);
-          if (closes) publish(groups + group * row, 0, state);
+          if (serial) publish(pairs + chunk * row, kSet, state);
+          if (closes) publish(groups + group * row, kSet, state);
         }
       }
       __syncthreads();
@@ -279,8 +286,8 @@ __global__ __launch_bounds__(256) void scan_chunks(ScanArgs s) {
     }
     __syncthreads();
     if (s.chunks > 1 && w == 0) {
-      publish(pairs + chunk * row, 0, came[lane]);
-      if (closes) publish(groups + group * row, 0, came[lane]);
+      publish(pairs + chunk * row, kSet, came[lane]);
+      if (closes) publish(groups + group * row, kSet, came[lane]);
     }
     state = mine;
   }

@@ -1082,3 +1082,23 @@ def test_recurrence_that_forgets_at_once(gate):
     want, tol = R.recurrence(a, x, h0, dh)
     for n in want:
         R.check(got[n], want[n], tol[n], n)
+
+
+def test_recurrence_of_infinite_states():
+    """A state that has left f32's range stays infinite while its gates are positive, also past spans whose gates' products
+    leave the range in other channels or vanish."""
+    r = rng(45)
+    a, x = f32(r.uniform(0.5, 1, (1, 3000, 70))), f32(r.standard_normal((1, 3000, 70)))
+    a[0, 333, 3], a[0, 1500, 5] = np.inf, np.inf
+    a[0, 700:900] = 1e-3
+    a[0, 2000:2060, 9] = 1e30
+    a[0, 2200, 11] = np.nan
+    got = forward(lambda i: [O.linear_recurrence(i['a'], i['x'])], dict(a=a, x=x))[0]
+    h = np.zeros((3000, 70), np.float32)
+    with np.errstate(all='ignore'):
+        s = np.zeros(70, np.float32)
+        for t in range(3000):
+            s = a[0, t] * s + x[0, t]
+            h[t] = s
+    assert np.array_equal(np.isnan(got[0]), np.isnan(h))
+    assert np.array_equal(np.isposinf(got[0]), np.isposinf(h)) and np.array_equal(np.isneginf(got[0]), np.isneginf(h))
