@@ -15,7 +15,8 @@ namespace {
 // 5.5 TB/s.
 
 // cos and sin of position * freq. The product is taken in 64 bits and brought to r in [-pi/4, pi/4] by the nearest multiple
-// of pi/2 (in two parts, 2^-106 in all), where the Taylor series to r^9 and r^10 are off by less than 2^-28.
+// of pi/2 (in two parts, 2^-106 in all), where the Taylor series to r^9 and r^10 are off by less than 2^-28. Up to some 2^50: the
+// multiple must come out right to a half (bases below 2^-16 are refused).
 __device__ __forceinline__ void angle(int position, double freq, float& c, float& s) {
   const double x = (double)position * freq, n = rint(x * 0.63661977236758134308);
   const float r = (float)fma(-n, 6.123233995736766e-17, fma(-n, 1.5707963267948966, x));

@@ -3905,7 +3905,7 @@ void Runtime::lower_rope(int i) {
     expect(sizes.back() > 0, i, "sections must be positive");
     half += sizes.back();
   }
-  expect(half > 0 && 2 * half <= xs[3] && base > 0 && std::isfinite(base), i, "bad sections or base");
+  expect(half > 0 && 2 * half <= xs[3] && base >= 0x1p-16 && std::isfinite(base), i, "bad sections or base");
   expect(T_[pos].dt == I32 && T_[pos].shape == Dims({(int64_t)sizes.size(), xs[0], xs[2]}) && view_[pos].contiguous(), i,
          "positions must be i32 [axes, B, T]");
   expect(xs[0] * xs[2] * xs[3] < (int64_t(1) << 31), i, "too large");

@@ -546,6 +546,7 @@ def rope(q: Tensor, k: Tensor, base: float = 10000) -> Tuple[Tensor, Tensor]:
 
 ATTENTION_MAX_HEAD = 128   # the kernels' tiles hold whole heads
 ATTENTION_RANGE = 2.0 ** 60   # of constants that the kernels multiply in f32
+ROPE_LEAST_BASE = 2.0 ** -16   # angles below 2^47, which 64 bits reduce to a quarter turn
 
 
 def _finite(x) -> bool:
@@ -646,8 +647,8 @@ def rope_axes(q: Tensor, k: Tensor, positions: Tensor, sections: Sequence[int], 
     if positions.dtype != 'i32' or positions.shape != (len(sections), B, T):
         raise ShapeError(f'{site}: positions must be i32 {S.show((len(sections), B, T))}, got {positions.dtype} '
                          f'{S.show(positions.shape)}', site)
-    if not _finite(base) or base <= 0:
-        raise ShapeError(f'{site}: base must be positive, got {base}', site)
+    if not _finite(base) or base < ROPE_LEAST_BASE:
+        raise ShapeError(f'{site}: base must be positive, at least 2^-16, got {base}', site)
     return tuple(_rope_axes(x, positions, sections, base, bool(per_axis), bool(inverse)) for x in (q, k))
 
 

@@ -1102,3 +1102,15 @@ def test_recurrence_of_infinite_states():
             h[t] = s
     assert np.array_equal(np.isnan(got[0]), np.isnan(h))
     assert np.array_equal(np.isposinf(got[0]), np.isposinf(h)) and np.array_equal(np.isneginf(got[0]), np.isneginf(h))
+
+
+def test_rope_axes_of_the_least_base():
+    """Angles of up to 2^46: the product of position and frequency, rounded in 64 bits, is the angle; 2^-53 of 2^46 is more than
+    any bound on cosines, so the positions here are powers of two and the frequencies too, and their product exact."""
+    r = rng(27)
+    q = f32(r.standard_normal((1, 2, 24, 8)))
+    pos = (2 ** (np.arange(24) % 31)).astype(np.int32).reshape(1, 1, 24)
+    got = forward(lambda i: list(O.rope_axes(i['q'], i['q'], i['p'], [4], 2.0 ** -16)), dict(q=q, p=pos))
+    want, tol = R.rope_axes(q, pos, [4], 2.0 ** -16)
+    for g in got:
+        R.check(g, want, tol)

@@ -176,3 +176,18 @@ def test_the_64_bit_forms_agree_with_differences():
             p[name] = z + s * 1e-6 * u
             side.append((R.recurrence(p['da'], p['dx'], p['dh0'])[0]['h'] * dh).sum())
         assert abs((side[0] - side[1]) / 2e-6 - (got[name] * u).sum()) < 1e-6
+
+
+def test_rope_axes_refuses_a_base_whose_angles_cannot_be_reduced():
+    def turn(base):
+        return O.rope_axes(t('q', 2, 4, 3, 8), t('k', 2, 2, 3, 8), t('p', 2, 2, 3, dtype='i32'), [2, 2], base)
+    for base in (1e-5, 1e-9, 1e-300):
+        refuses(lambda: turn(base), 'base')
+    g = trace_fn(lambda: turn(2.0 ** -16))
+    doc = {'graph': IR.graph_to_wire(g), 'paramGrads': {}, 'writebacks': [], 'optimizer': None}
+    backend.plan(IR.dumps(doc))
+    for op in doc['graph']['ops']:
+        if op['kind'] == 'rope_axes':
+            op['base'] = 1e-9
+    with pytest.raises(backend.BackendError, match='base'):
+        backend.plan(IR.dumps(doc))
