@@ -48,17 +48,37 @@ struct TileInfo {
 // What a block needs of each row of a tile it walks, 32 values each (integers as bits), 2 KiB that come with the fragments
 // into LDS: of queries and of keys. Row S_INFO: the TileInfo of the first operand (q, k) and eight words on the second's (dy,
 // v). From LDS, because a load from memory inside the loop would wait for the next tile's fragments, which are ahead of it.
-enum { QS_LSE, QS_DOT, QS_POS, QS_SLOPE, QS_BELOW, QS_DOC, QS_RELQ, QS_RELG, S_INFO, kSide = 16 };   // dot(dy, y); sees keys below
+enum { QS_TOP, QS_SHARE, QS_DOT, QS_POS, QS_SLOPE, QS_BELOW, QS_DOC, QS_RELQ, QS_RELG, S_INFO, kSide = 16 };   // dot(dy, y) share;
+                                                                                                               // sees keys below
 enum { KS_DOC, KS_RELK, KS_RELV };
 constexpr int kSideFrags = kSide * kTile * 4 / 1024;
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 __device__ __forceinline__ int exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 255) - 127; }   // floor(log2 |x|)
-// What a score's sum of products is multiplied by, c 2^e, c > 0. Rows of 1e-19, or of 1e25, take it out of f32's range: kept
-// within, it leaves such scores next to 0, or past f32's range, and a sum of 0 or a hidden key's minus infinity as they are.
-__device__ __forceinline__ float score_unit(float c, int e) {
-  return __builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(c, e), 0x1p-126f, 0x1p127f);
+// A product that is rounded before it is added to.
+__device__ __forceinline__ float rounded_mul(float x, float y) {
+#pragma clang fp contract(off)
+  return x * y;
 }
+// What a score is made of: the queries' values take the factor `part` (0.5 to 1, rounded once, wherever they are split), so that
+// the sum of products times 2^exp is q.k scale log2(e), or q.k scale / cap, without a rounding. That makes a score the same
+// number in every walk, forward and backward, and its distance to the row's largest exact: with a rounded factor inside a
+// fused multiply-add that distance was off by half a step of the largest, a factor of 2^128 for scores of 2^32.
+struct Score {
+  float part;
+  int exp;
+};
+__device__ __forceinline__ Score score_parts(const AttendDesc& a) {
+  const float c = a.cap > 0 ? a.scale / a.cap : a.scale * kLog2e;
+  return {__builtin_amdgcn_frexp_mantf(c), __builtin_amdgcn_frexp_expf(c)};
+}
+// The score of x (sum of products, or its tanh) for f, in log2.
+__device__ __forceinline__ float score_of(bool slopes, float x, float f, float slope, int far) {
+  return slopes ? fmaf(x, f, -rounded_mul(slope, fabsf((float)far))) : rounded_mul(x, f);
+}
+// 2^e of a sum of products. Rows of 1e-19, or of 1e25, take it out of f32's range: kept within (pow2), it leaves such scores next
+// to 0, or past f32's range, and a sum of 0 or a hidden key's minus infinity as they are.
+__device__ __forceinline__ float score_unit(const Score& s, int e) { return pow2(s.exp + e); }
 // The same of dP: a sum of 0 stays 0.
 __device__ __forceinline__ float dot_unit(int e) { return __builtin_amdgcn_ldexpf(1.0f, min(e, 127)); }
 
@@ -125,6 +145,15 @@ __device__ __forceinline__ int doc_at(const Sight& s, int p) { return s.doc && p
 // Does it see any: then, where positions matter, the key at its own. From the masks, not from sums or maxima, which NaN and
 // minus infinities in what is seen empty as well.
 __device__ __forceinline__ bool sees_any(const Sight& s, int below, int doc) { return below > 0 && (!s.doc || doc >= 0); }
+// A row's softmax for its gradients, two values: P = exp2(score - top) share. top is the logarithm of the sum, and share what its
+// rounding leaves (close to 1), up to 2^24, where its steps reach 2; above, top is the largest score itself and share 1 / sum. A row
+// that sees nothing: exp2(score - inf) = 0.
+__device__ __forceinline__ void write_stats(const AttendDesc& a, int64_t row, bool none, float m, float sum) {
+  const float l = __builtin_amdgcn_logf(sum), lse = m + l;
+  const bool far = fabsf(m) >= 0x1p24f;
+  a.stats[2 * row] = none ? INFINITY : far ? m : lse;
+  a.stats[2 * row + 1] = none ? 1.0f : far ? 1.0f / sum : __builtin_amdgcn_exp2f((lse - m) - l);
+}
 
 // Rows [lo, hi] of positions against keys [j0, j0 + 32): does any pair see, do all.
 struct Span {
@@ -193,10 +222,10 @@ __device__ __forceinline__ float groups_sum(float x) {
   r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// B fragments of 16 rows (lane l: row l % 16), each row with its own power of two; returns its exponent. *infinite: the row holds
-// an infinity, which has no hi and lo parts.
+// B fragments of 16 rows times `mul` (lane l: row l % 16), each row with its own power of two; returns its exponent. *infinite:
+// the row holds an infinity, which has no hi and lo parts.
 template <int N>
-__device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bool wide, half8 (&hi)[N], half8 (&lo)[N],
+__device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bool wide, float mul, half8 (&hi)[N], half8 (&lo)[N],
                                          bool* infinite = nullptr) {
   const int g = (threadIdx.x >> 4) & 3;
   float x[N][8], m = 0;
@@ -219,7 +248,7 @@ __device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bo
 #pragma unroll
   for (int c = 0; c < N; ++c)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[c][i]));
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[c][i] * mul));
   m = groups_max(m);
   if (infinite) *infinite = m == INFINITY;
   const int e = m > 0 ? min(14 - exponent(m), 126) : 0;
@@ -227,14 +256,15 @@ __device__ __forceinline__ int load_rows(const float* row, bool valid, int n, bo
 #pragma unroll
   for (int c = 0; c < N; ++c) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[c][i] *= s;
+    for (int i = 0; i < 8; ++i) x[c][i] = x[c][i] * mul * s;
     split8(x[c], hi[c], lo[c]);
   }
   return e;
 }
 // x = A fragments (N chunks of 32 features, two blocks of 16 rows each, from fragment f0) times B fragments; a chunk's
-// fragments are read while the chunk before is multiplied.
-template <int N>
+// fragments are read while the chunk before is multiplied. Queries against keys or keys against queries (KQ), the products are
+// added in the same order: k lo q hi, k hi q lo, k hi q hi.
+template <bool KQ, int N>
 __device__ __forceinline__ void scores(const _Float16* L, int f0, const half8 (&bh)[N], const half8 (&bl)[N], float (&x)[8]) {
   f32x4 z[2] = {};
   half8 a[2][4];
@@ -246,10 +276,10 @@ __device__ __forceinline__ void scores(const _Float16* L, int f0, const half8 (&
     if (c + 1 < N)
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[(c + 1) & 1][i] = frag(L, f0 + 4 * c + 4 + i);
-    z[0] = mfma(u[1], bh[c], z[0]);
-    z[1] = mfma(u[3], bh[c], z[1]);
-    z[0] = mfma(u[0], bl[c], z[0]);
-    z[1] = mfma(u[2], bl[c], z[1]);
+    z[0] = KQ ? mfma(u[1], bh[c], z[0]) : mfma(u[0], bl[c], z[0]);
+    z[1] = KQ ? mfma(u[3], bh[c], z[1]) : mfma(u[2], bl[c], z[1]);
+    z[0] = KQ ? mfma(u[0], bl[c], z[0]) : mfma(u[1], bh[c], z[0]);
+    z[1] = KQ ? mfma(u[2], bl[c], z[1]) : mfma(u[3], bh[c], z[1]);
     z[0] = mfma(u[0], bh[c], z[0]);
     z[1] = mfma(u[2], bh[c], z[1]);
     __builtin_amdgcn_sched_barrier(0);
@@ -258,7 +288,7 @@ __device__ __forceinline__ void scores(const _Float16* L, int f0, const half8 (&
   for (int q = 0; q < 8; ++q) x[q] = z[q / 4][q % 4];
 }
 // Both products of a pair, step by step in turn.
-template <int N>
+template <bool KQ, int N>
 __device__ __forceinline__ void pair(const _Float16* L, int f0, const half8 (&bh)[N], const half8 (&bl)[N], float (&x)[8], int f1,
                                        const half8 (&ch)[N], const half8 (&cl)[N], float (&y)[8]) {
   f32x4 z[4] = {};
@@ -275,12 +305,12 @@ __device__ __forceinline__ void pair(const _Float16* L, int f0, const half8 (&bh
   for (int c = 0; c < N; ++c) {
     const half8* u = a[c & 1];
     if (c + 1 < N) read(c + 1);
-    z[0] = mfma(u[1], bh[c], z[0]);
-    z[1] = mfma(u[3], bh[c], z[1]);
+    z[0] = KQ ? mfma(u[1], bh[c], z[0]) : mfma(u[0], bl[c], z[0]);
+    z[1] = KQ ? mfma(u[3], bh[c], z[1]) : mfma(u[2], bl[c], z[1]);
     z[2] = mfma(u[5], ch[c], z[2]);
     z[3] = mfma(u[7], ch[c], z[3]);
-    z[0] = mfma(u[0], bl[c], z[0]);
-    z[1] = mfma(u[2], bl[c], z[1]);
+    z[0] = KQ ? mfma(u[0], bl[c], z[0]) : mfma(u[1], bh[c], z[0]);
+    z[1] = KQ ? mfma(u[2], bl[c], z[1]) : mfma(u[3], bh[c], z[1]);
     z[2] = mfma(u[4], cl[c], z[2]);
     z[3] = mfma(u[6], cl[c], z[3]);
     z[0] = mfma(u[0], bh[c], z[0]);
@@ -440,7 +470,7 @@ __device__ __forceinline__ PlainPair plain_score(const AttendDesc& a, float dot,
     t = tanh_of(x / a.cap);
     x = a.cap * t;
   }
-  r.score = (x * kLog2e) - slope * fabsf((float)far);
+  r.score = fmaf(-slope, fabsf((float)far), x * kLog2e);
   r.slack = fmaf(-t, t, 1.0f);
   return r;
 }
@@ -489,7 +519,8 @@ struct PackJob {
   int rel;                         // where this operand's rel goes
   bool second;                     // and its info
   bool ids;                        // this job also writes the rows' documents and the rest
-  Rows y;                          // of the gradient dy (ids of queries): y's rows for its dot products
+  bool score;                      // queries: the row fragments take their factor (score_parts)
+  Rows y;                          // of the gradient dy (ids of queries, times their share): y's rows for its dot products
 };
 // The attention's operands as packed for one pass, in the workspace.
 struct Packs {

@@ -4,7 +4,8 @@
 //    each walk the visible key tiles (attend_tiles), four wavefronts a SIMD, so that one's products run beside the others'
 //    vector work. Scores are computed transposed (keys x queries);
 //  * few rows (one new token against a cache): the keys are read once, in f32, by all heads that share them (attend_few);
-//    bound by memory, so split over the keys until the card is full.
+//    bound by memory, so split over the keys until the card is full. Without a gradient: the gradients compute scores as the
+//    tiles do.
 // Both split a long key axis when there are few rows (attend_join). A few dozen positions in all: k_attend_small.hip.
 #include "attend_dev.h"
 
@@ -32,6 +33,8 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
   const bool in = r < j.rows && (!s.doc || id >= 0) && (j.query ? !s.positional || pos >= 0 : pos < s.n);
   const int64_t at = b * j.x.b + (int64_t)(hk * j.G + g) * j.x.h + (int64_t)i * j.x.t;
   const bool dots = j.ids && j.query;
+  const int64_t stat = 2 * (((int64_t)b * p.a.H + hk * j.G + g) * p.a.Tq + i);
+  const float mul = dots && in ? p.a.stats[stat + 1] : 1.0f;
   float m = 0, dot = 0;
   bool odd = false;
 #pragma unroll
@@ -46,6 +49,7 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
+      u[q] *= mul;
       odd |= !(fabsf(u[q]) < INFINITY);
       m = fmaxf(m, finite_abs(u[q]));
     }
@@ -69,7 +73,8 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
     if (dots) {
       const AttendDesc& a = p.a;
       const int h = hk * j.G + g;
-      side[QS_LSE * kTile + row] = in ? a.lse[((int64_t)b * a.H + h) * a.Tq + i] : INFINITY;
+      side[QS_TOP * kTile + row] = in ? a.stats[stat] : INFINITY;
+      side[QS_SHARE * kTile + row] = mul;
       side[QS_DOT * kTile + row] = in ? dot : 0.0f;
       side[QS_POS * kTile + row] = __int_as_float(pos);
       side[QS_SLOPE * kTile + row] = in && a.slopes ? a.slopes[h] * kLog2e : 0.0f;
@@ -108,12 +113,13 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
   if (bad) return;
   __syncthreads();
   const int g4 = lane >> 4, l16 = lane & 15;
+  const float part = j.score ? score_parts(p.a).part : 1.0f;
   if (j.rowf)
     for (int c = w; c < 2 * DB; c += 4) {   // 32 features c / 2 of 16 rows c % 2
       const int r = 16 * (c % 2) + l16;
       float z[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) z[q] = x[r * LD + 32 * (c / 2) + 8 * g4 + q] * own[r];
+      for (int q = 0; q < 8; ++q) z[q] = x[r * LD + 32 * (c / 2) + 8 * g4 + q] * part * own[r];
       half8 a, f;
       split8(z, a, f);
       half8* o = (half8*)(j.rowf + (slot * 2 * DB + c) * 2 * kFrag) + lane;
@@ -146,19 +152,21 @@ struct TilesArgs {
   FastDiv group;                   // G
   int M, blocks, splits;           // rows of a slab, row blocks, parts of the key axis
   bool wide;
-  float *part, *plse;              // parts: [split][slab][M][Dv], [split][slab][M]
+  float* part;                     // parts: [split][slab][M][Dv], of sums of weights 1
+  f32x2* psum;                     // their largest scores and sums: [split][slab][M]
 };
 
-// Where a row's result goes, and its lse. A part whose weights are all 0 has an lse of minus infinity and a result of 0.
-__device__ __forceinline__ float* result_row(const TilesArgs& A, int split, int slab, int b, int head, int r, int i, float lse, bool none,
+// Where a row's result goes, and its largest score and sum. A part that has no such score says f32's lowest, and a part whose
+// weights are all 0 has a sum and a result of 0.
+__device__ __forceinline__ float* result_row(const TilesArgs& A, int split, int slab, int b, int head, int r, int i, float m, float sum, bool none,
                                              bool writes) {
   const AttendDesc& a = A.a;
   if (A.splits > 1) {
     const int64_t at = ((int64_t)split * a.B * a.Hk + slab) * A.M + r;
-    if (writes) A.plse[at] = lse;
+    if (writes) A.psum[at] = f32x2{fmaxf(m, kLowest), sum};
     return A.part + at * a.Dv;
   }
-  if (writes && a.lse) a.lse[((int64_t)b * a.H + head) * a.Tq + i] = none ? INFINITY : lse;
+  if (writes && a.stats) write_stats(a, ((int64_t)b * a.H + head) * a.Tq + i, none, m, sum);
   return a.y.p ? a.y.p + b * a.y.b + head * a.y.h + (int64_t)i * a.y.t : nullptr;
 }
 
@@ -193,7 +201,7 @@ __device__ __forceinline__ void plain_rows(const TilesArgs& A, const Sight& s, i
     }
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
-    float* y = result_row(A, split, slab, b, head, r, i, m + __builtin_amdgcn_logf(sum), none, lane == 0);
+    float* y = result_row(A, split, slab, b, head, r, i, m, sum, none, lane == 0);
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       if (y && 64 * e + lane < a.Dv) y[64 * e + lane] = (A.splits > 1 ? sum == 0 : none) ? 0.0f : acc[e] / sum;
@@ -245,7 +253,8 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   const int last = s.first + (int)fastdiv((uint32_t)min(blk * 128 + 127, A.M - 1), A.group);   // of the block
   half8 qh[N], ql[N];
   bool infinite;
-  const int qe = load_rows<N>(a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t, valid, a.D, A.wide, qh, ql, &infinite);
+  const Score sc = score_parts(a);
+  const int qe = load_rows<N>(a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t, valid, a.D, A.wide, sc.part, qh, ql, &infinite);
   int t0 = 0, t1 = s.n;
   if (s.causal) t1 = min(t1, max(last + 1, s.prefix));
   if (s.positional && last < 0) t1 = 0;
@@ -284,7 +293,6 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   for (int d = 0; d < 2 * N; ++d) acc[d] = f32x4{};
   float m = kNone, sum = 0;        // running maximum (log2) and this lane's part of the sum
   int ce = kUnset;                 // acc is in units of 2^-ce
-  const float icap = CAP ? 1.0f / a.cap : 0.0f;
   if (t0 < t1) fetch(0);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, j0 = t * kTile;
@@ -296,17 +304,16 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
     const TileInfo kt = side_info(side, 0), vt = side_info(side, 1);
     if (__builtin_expect(!any_seen(s, me, kt, j0), 0)) continue;
     float x[8];                    // transposed: element q of this lane is key j0 + 16 (q / 4) + 4 g4 + q % 4
-    scores<N>(L, 0, qh, ql, x);
-    const int unit = exponent(kt.inv) - qe;
+    scores<true, N>(L, 0, qh, ql, x);
     if (__builtin_expect(kt.uneven, 0)) per_row(x, side + KS_RELK * kTile, g4);
-    float f = score_unit(a.scale * kLog2e, unit);   // the score is f x, in log2
+    float f = score_unit(sc, exponent(kt.inv) - qe);   // the score is f x, in log2
     if (CAP) {
-      tanh_all(x, score_unit(a.scale * icap, unit));
+      tanh_all(x, f);
       f = a.cap * kLog2e;
     }
-    if (SLOPES) {
+    if (CAP || SLOPES) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) x[q] = x[q] * f - slope * fabsf((float)(p - (j0 + 16 * (q / 4) + 4 * g4 + q % 4)));
+      for (int q = 0; q < 8; ++q) x[q] = score_of(SLOPES, x[q], f, slope, p - (j0 + 16 * (q / 4) + 4 * g4 + q % 4));
       f = 1;
     }
     if (__builtin_expect(!all_seen(s, me, kt, j0), 0)) {
@@ -347,7 +354,7 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   if (!valid) return;
   const bool none = !sees_any(s, below, doc);
   const float out = (A.splits > 1 ? sum == 0 : none) ? 0.0f : 1.0f / sum;
-  float* y = result_row(A, split, slab, b, head, r, i, m + __builtin_amdgcn_logf(sum), none, g4 == 0);
+  float* y = result_row(A, split, slab, b, head, r, i, m, sum, none, g4 == 0);
   if (y) store_row(y, acc, ce, out, a.Dv, A.splits > 1 ? a.Dv % 4 == 0 : A.wide, g4);
 }
 
@@ -356,7 +363,8 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
 struct FewArgs {
   AttendDesc a;
   int M, splits, each;             // keys of a part
-  float *part, *plse;
+  float* part;
+  f32x2* psum;
 };
 
 // Eight lanes share a key row: each reads E of its features as 16-byte pieces (8 rows of 128 bytes a load instruction) and
@@ -437,7 +445,7 @@ __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
       x *= a.scale;
       if (a.cap > 0) x = a.cap * tanh_of(x / a.cap);
       if (a.slopes) x -= a.slopes[hk * G + min(r, A.M - 1) % G] * fabsf((float)(p[r] - j));
-      x *= kLog2e;
+      x = rounded_mul(x, kLog2e);
       if (!all && (j >= below[r] || (s.doc && (doc[r] < 0 || s.doc[j] != doc[r])))) continue;
       if (x > m[r] + 8) {
         const float top = x < INFINITY ? x : m[r] == kLowest ? 0.0f : m[r];   // an infinite score shows in the weight
@@ -496,11 +504,7 @@ __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
       if (A.splits > 1) A.part[at * a.Dv + d] = o;
       else if (a.y.p) a.y.p[b * a.y.b + head * a.y.h + i * a.y.t + d] = o;
     }
-    if (d == 0) {
-      const float lse = top + __builtin_amdgcn_logf(all);
-      if (A.splits > 1) A.plse[at] = lse;
-      else if (a.lse) a.lse[((int64_t)b * a.H + head) * a.Tq + i] = none ? INFINITY : lse;
-    }
+    if (d == 0 && A.splits > 1) A.psum[at] = f32x2{top, all};
   }
 }
 
@@ -516,12 +520,12 @@ constexpr int kJoinFew = 16;       // parts of a row that 32 threads join
 struct JoinArgs {
   AttendDesc a;
   int M, splits;
-  const float *part, *plse;
+  const float* part;
+  const f32x2* psum;
 };
 // Bound by memory (24864 rows of 2 parts of 96: 10 us). L threads join a row: its weights first, then every 32 threads an
 // L / 32nd of the parts. 32 threads take a row with few parts and a block one with many (a long cache read by one token: 16
-// parts by 32 threads or 64 by a block, 8 or 7 us; one thread a feature took 33). An lse of NaN makes the row NaN; fmaxf passes
-// over it, so that its row's largest may be minus infinity.
+// parts by 32 threads or 64 by a block, 8 or 7 us; one thread a feature took 33). A sum of NaN makes the row NaN.
 template <int L>
 __global__ __launch_bounds__(256) void attend_join(JoinArgs A) {
   constexpr int W = L < 64 ? L : 64, P = L / 32, PER = 256 / L;
@@ -534,12 +538,13 @@ __global__ __launch_bounds__(256) void attend_join(JoinArgs A) {
   const int i = r / G, head = hk * G + r % G;
   const Sight s = sight(a, b);
   const bool none = !sees_any(s, sees_below(s, s.first + i), doc_at(s, s.first + i));
-  float top = kNone, all = 0;
-  for (int z = t % W; z < A.splits; z += W) top = fmaxf(top, A.plse[at + z * rows]);
+  float top = kLowest, all = 0;
+  for (int z = t % W; z < A.splits; z += W) top = fmaxf(top, A.psum[at + z * rows].x);
 #pragma unroll
   for (int o = 1; o < W; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
   for (int z = t % W; z < A.splits; z += W) {
-    const float e = A.plse[at + z * rows], w = e == kNone ? 0.0f : __builtin_amdgcn_exp2f(e - top);
+    const f32x2 e = A.psum[at + z * rows];
+    const float w = __builtin_amdgcn_exp2f(e.x - top) * e.y;
     if (t < W) weight[own * A.splits + z] = w;
     all += w;
   }
@@ -574,7 +579,7 @@ __global__ __launch_bounds__(256) void attend_join(JoinArgs A) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) if (d + q < a.Dv) y[q] = none ? 0.0f : x[q] / all;
   }
-  if (a.lse && t == 0) a.lse[((int64_t)b * a.H + head) * a.Tq + i] = none ? INFINITY : top + __builtin_amdgcn_logf(all);
+  if (a.stats && t == 0) write_stats(a, ((int64_t)b * a.H + head) * a.Tq + i, none, top, all);
 }
 
 // ---- plans -----------------------------------------------------------------------------------------
@@ -582,7 +587,7 @@ __global__ __launch_bounds__(256) void attend_join(JoinArgs A) {
 struct Plan {
   int DP, M, G, tiles, blocks, splits, slabs, each;
   bool few;
-  int64_t kf, vf, ki, vi, side, part, plse, bytes;   // byte offsets into the workspace
+  int64_t kf, vf, ki, vi, side, part, psum, bytes;   // byte offsets into the workspace
 };
 constexpr int64_t kAlign = 256;
 inline int64_t take(int64_t& at, int64_t bytes) {
@@ -600,7 +605,7 @@ Plan plan(const AttendDesc& a) {
   p.M = p.G * a.Tq;
   p.slabs = a.B * a.Hk;
   p.tiles = (a.Tk + kTile - 1) / kTile;
-  p.few = p.M <= few_rows(p.DP) && (p.M <= 2 || a.Tk >= 32 * p.M);
+  p.few = !a.stats && p.M <= few_rows(p.DP) && (p.M <= 2 || a.Tk >= 32 * p.M);
   if (p.few) {
     p.blocks = 1;
     const int64_t want = std::max<int64_t>(1, kMostParts / p.slabs);
@@ -622,7 +627,7 @@ Plan plan(const AttendDesc& a) {
   }
   if (p.splits > 1) {
     p.part = take(at, (int64_t)p.splits * p.slabs * p.M * a.Dv * 4);
-    p.plse = take(at, (int64_t)p.splits * p.slabs * p.M * 4);
+    p.psum = take(at, (int64_t)p.splits * p.slabs * p.M * 8);
   }
   p.bytes = at;
   return p;
@@ -670,10 +675,10 @@ void attend(const AttendDesc& a, void* work, hipStream_t st) {
   const Plan p = plan(a);
   char* w = (char*)work;
   float* part = p.splits > 1 ? (float*)(w + p.part) : nullptr;
-  float* plse = p.splits > 1 ? (float*)(w + p.plse) : nullptr;
+  f32x2* psum = p.splits > 1 ? (f32x2*)(w + p.psum) : nullptr;
   const bool wide = attend_wide(a.q, a.D) && attend_wide(a.k, a.D) && attend_wide(a.v, a.Dv) && (!a.y.p || attend_wide(a.y, a.Dv));
   if (p.few) {
-    const FewArgs f{a, p.M, p.splits, p.each, part, plse};
+    const FewArgs f{a, p.M, p.splits, p.each, part, psum};
     if (p.DP == 32) run_few_rows<4>(f, wide, p.slabs, st);
     else if (p.DP == 64) run_few_rows<8>(f, wide, p.slabs, st);
     else if (p.DP == 96) run_few_rows<12>(f, wide, p.slabs, st);
@@ -685,11 +690,11 @@ void attend(const AttendDesc& a, void* work, hipStream_t st) {
     k.wide = wide;
     k.a = a;
     float* side = (float*)(w + p.side);
-    k.job[0] = {a.k, a.D, 1, a.Tk, p.tiles, (_Float16*)(w + p.kf), nullptr, (TileInfo*)(w + p.ki), false, side, KS_RELK, false, true, {}};
-    k.job[1] = {a.v, a.Dv, 1, a.Tk, p.tiles, nullptr, (_Float16*)(w + p.vf), (TileInfo*)(w + p.vi), false, side, KS_RELV, true, false, {}};
+    k.job[0] = {a.k, a.D, 1, a.Tk, p.tiles, (_Float16*)(w + p.kf), nullptr, (TileInfo*)(w + p.ki), false, side, KS_RELK, false, true, false, {}};
+    k.job[1] = {a.v, a.Dv, 1, a.Tk, p.tiles, nullptr, (_Float16*)(w + p.vf), (TileInfo*)(w + p.vi), false, side, KS_RELV, true, false, false, {}};
     attend_pack(k, p.DP, st);
     const TilesArgs t{a, (_Float16*)(w + p.kf), (_Float16*)(w + p.vf), (TileInfo*)(w + p.ki), (TileInfo*)(w + p.vi), side,
-                      make_fastdiv(p.G), p.M, p.blocks, p.splits, wide, part, plse};
+                      make_fastdiv(p.G), p.M, p.blocks, p.splits, wide, part, psum};
     const unsigned grid = place_grid(p.slabs, (int64_t)p.blocks * p.splits);
     if (p.DP == 32) run_tiles<32>(t, grid, st);
     else if (p.DP == 64) run_tiles<64>(t, grid, st);
@@ -697,7 +702,7 @@ void attend(const AttendDesc& a, void* work, hipStream_t st) {
     else run_tiles<128>(t, grid, st);
   }
   if (p.splits > 1) {
-    const JoinArgs j{a, p.M, p.splits, part, plse};
+    const JoinArgs j{a, p.M, p.splits, part, psum};
     const int64_t rows = (int64_t)p.slabs * p.M;
     if (p.splits <= kJoinFew) klaunch(attend_join<32>, dim3((rows + 7) / 8), dim3(256), 0, st, j);
     else klaunch(attend_join<256>, dim3(rows), dim3(256), 0, st, j);

@@ -1,11 +1,12 @@
-// Gradients of masked attention for gfx950. With P = exp(score - lse), D_i = dy_i . y_i, dP_ij = dy_i . v_j,
+// Gradients of masked attention for gfx950. With P = exp(score - top) share, D_i = dy_i . y_i, dP_ij = dy_i . v_j,
 //   ds = P (dP - D) (1 - tanh^2),  dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i P_ij dy_i
 // (sums over i run over the query heads that share the key head). Two kernels, each with the whole of its own sums, so that
 // nothing is added by atomics and results repeat bit for bit; scores and dP are computed in both (7 products instead of 5):
 //  * attend_grad_kv: a wavefront keeps 16 keys, k and v in registers, and walks the query rows; scores are computed as
 //    queries x keys, so that P and ds are the B fragments of dv and dk as they stand;
 //  * attend_grad_q: a wavefront keeps 16 query rows and walks the keys, scores transposed as in the forward pass.
-// The walked operands are packed once (attend_pack, k_attend.hip); lse and D come with them.
+// The walked operands are packed once (attend_pack, k_attend.hip); top and D come with them. A row's share is a factor of all
+// that is linear in its dy: dy is packed, and D made, with it.
 #include "attend_dev.h"
 
 namespace tgk {
@@ -88,8 +89,9 @@ __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, in
         const float* side = A.qside + ((int64_t)slab * A.qtiles + r / kTile) * (kSide * kTile) + r % kTile;
         if (j < __float_as_int(side[QS_BELOW * kTile]) && (!s.doc || (doc >= 0 && __float_as_int(side[QS_DOC * kTile]) == doc))) {
           const PlainPair z = plain_score(a, plain_dot(row(a.q, r), k, a.D), side[QS_SLOPE * kTile], __float_as_int(side[QS_POS * kTile]) - j);
-          p = __builtin_amdgcn_exp2f(z.score - side[QS_LSE * kTile]);
-          ds = p * (plain_dot(row(A.g.dy, r), v, a.Dv) - side[QS_DOT * kTile]) * z.slack;
+          const float share = side[QS_SHARE * kTile], w = __builtin_amdgcn_exp2f(z.score - side[QS_TOP * kTile]);
+          p = w * share;
+          ds = w * fmaf(plain_dot(row(A.g.dy, r), v, a.Dv), share, -side[QS_DOT * kTile]) * z.slack;
         }
       }
       if (WHAT & 2) plain_add(dv, p, [&](int z) { return row(A.g.dy, min(c + z, A.M - 1)); }, a.Dv);
@@ -146,9 +148,9 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
   }
 
   half8 kh[N], kl[N], vh[DK ? N : 1], vl[DK ? N : 1];
-  const int ke = load_rows<N>(a.k.p + b * a.k.b + hk * a.k.h + (int64_t)min(j, a.Tk - 1) * a.k.t, valid, a.D, A.wide, kh, kl);
+  const int ke = load_rows<N>(a.k.p + b * a.k.b + hk * a.k.h + (int64_t)min(j, a.Tk - 1) * a.k.t, valid, a.D, A.wide, 1.0f, kh, kl);
   int ve = 0;
-  if constexpr (DK) ve = load_rows<N>(a.v.p + b * a.v.b + hk * a.v.h + (int64_t)min(j, a.Tk - 1) * a.v.t, valid, a.Dv, A.wide, vh, vl);
+  if constexpr (DK) ve = load_rows<N>(a.v.p + b * a.v.b + hk * a.v.h + (int64_t)min(j, a.Tk - 1) * a.v.t, valid, a.Dv, A.wide, 1.0f, vh, vl);
   const int64_t tile0 = (int64_t)slab * A.qtiles + t0;
   const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
   const char* qr = (const char*)(A.qr + tile0 * (F * kFrag)) + w * 1024;
@@ -178,7 +180,7 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
 #pragma unroll
   for (int d = 0; d < 2 * N; ++d) dk[d] = dv[d] = f32x4{};
   int ck = kUnset, cv = kUnset;
-  const float icap = RICH && a.cap > 0 ? 1.0f / a.cap : 0.0f;
+  const Score sc = score_parts(a);
   if (t0 < t1) fetch(0);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, r0 = t * kTile;
@@ -198,36 +200,35 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
     // element q: row r0 + 16 (q / 4) + 4 g + q % 4
     float x[8], y[8] = {};
     if constexpr (DK && N == 2) {  // the pair in turn would spill registers here
-      scores<N>(L, 0, kh, kl, x);
-      scores<N>(L, F_GR, vh, vl, y);
-    } else if constexpr (DK) pair<N>(L, 0, kh, kl, x, F_GR, vh, vl, y);
+      scores<false, N>(L, 0, kh, kl, x);
+      scores<false, N>(L, F_GR, vh, vl, y);
+    } else if constexpr (DK) pair<false, N>(L, 0, kh, kl, x, F_GR, vh, vl, y);
     else {
-      scores<N>(L, 0, kh, kl, x);
+      scores<false, N>(L, 0, kh, kl, x);
     }
     if (__builtin_expect(qt.uneven, 0)) per_row(x, side + QS_RELQ * kTile, g);
     if (DK && __builtin_expect(gt.uneven, 0)) per_row(y, side + QS_RELG * kTile, g);
-    const int unit = exponent(qt.inv) - ke;
     const float yunit = dot_unit(exponent(gt.inv) - ve);
-    float f = score_unit(a.scale * kLog2e, unit);
+    float f = score_unit(sc, exponent(qt.inv) - ke);
     if (RICH && a.cap > 0) {
-      tanh_all(x, score_unit(a.scale * icap, unit));
+      tanh_all(x, f);
       f = a.cap * kLog2e;
     }
     const bool all = A.M - r0 >= kTile && all_seen(s, rows, mine, jt);
 #pragma unroll
     for (int q4 = 0; q4 < 2; ++q4) {
       const int at = 16 * q4 + 4 * g;
-      const f32x4 lse = *(const f32x4*)(side + QS_LSE * kTile + at), dot = *(const f32x4*)(side + QS_DOT * kTile + at);
-      f32x4 off = lse;
+      const f32x4 top = *(const f32x4*)(side + QS_TOP * kTile + at), dot = *(const f32x4*)(side + QS_DOT * kTile + at);
+      f32x4 pos = {}, slope = {};
       if (RICH && a.slopes) {
-        const f32x4 pos = *(const f32x4*)(side + QS_POS * kTile + at), slope = *(const f32x4*)(side + QS_SLOPE * kTile + at);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) off[e] = fmaf(slope[e], fabsf((float)(__float_as_int(pos[e]) - j)), lse[e]);
+        pos = *(const f32x4*)(side + QS_POS * kTile + at);
+        slope = *(const f32x4*)(side + QS_SLOPE * kTile + at);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int q = 4 * q4 + e;
-        const float p = __builtin_amdgcn_exp2f(fmaf(x[q], f, -off[e]));
+        const float far = RICH ? score_of(a.slopes, x[q], f, slope[e], __float_as_int(pos[e]) - j) - top[e] : fmaf(x[q], f, -top[e]);
+        const float p = __builtin_amdgcn_exp2f(far);
         if (DK) {
           y[q] = p * fmaf(y[q], yunit, -dot[e]);
           if (RICH && a.cap > 0) y[q] *= fmaf(-x[q], x[q], 1.0f);   // 1 - tanh^2
@@ -348,7 +349,8 @@ __device__ __forceinline__ void plain_dq(const GradArgs& A, const Sight& s, int 
       float ds = 0;
       if (j < end && (!s.doc || (doc >= 0 && s.doc[j] == doc))) {
         const PlainPair z = plain_score(a, plain_dot(k + j * a.k.t, q, a.D), side[QS_SLOPE * kTile], p - j);
-        ds = __builtin_amdgcn_exp2f(z.score - side[QS_LSE * kTile]) * (plain_dot(v + j * a.v.t, dy, a.Dv) - side[QS_DOT * kTile]) * z.slack;
+        ds = __builtin_amdgcn_exp2f(z.score - side[QS_TOP * kTile]) *
+             fmaf(plain_dot(v + j * a.v.t, dy, a.Dv), side[QS_SHARE * kTile], -side[QS_DOT * kTile]) * z.slack;
       }
       plain_add(dq, ds, [&](int z) { return k + min(c + z, a.Tk - 1) * a.k.t; }, a.D);
     }
@@ -380,7 +382,7 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   const int p = s.first + i, doc = doc_at(s, p), below = sees_below(s, p);
   const int qt = min(row0 / kTile, A.qtiles - 1), rt = row0 / kTile * kTile;   // masks are judged by whole tiles of rows
   const float* mine = A.qside + ((int64_t)slab * A.qtiles + qt) * (kSide * kTile) + row0 % kTile + l;
-  const float lse = mine[QS_LSE * kTile], dot = mine[QS_DOT * kTile];
+  const float top = mine[QS_TOP * kTile], share = mine[QS_SHARE * kTile], dot = mine[QS_DOT * kTile];
   const TileInfo gt = A.gi[(int64_t)slab * A.qtiles + qt];
   const bool own = rt < A.M && (gt.odd || A.qi[(int64_t)slab * A.qtiles + qt].odd);
   Span me;
@@ -409,8 +411,9 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   }
 
   half8 qh[N], ql[N], gh[N], gl[N];
-  const int qe = load_rows<N>(a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t, valid, a.D, A.wide, qh, ql);
-  const int ge = load_rows<N>(A.g.dy.p + b * A.g.dy.b + head * A.g.dy.h + (int64_t)i * A.g.dy.t, valid, a.Dv, A.wide, gh, gl);
+  const Score sc = score_parts(a);
+  const int qe = load_rows<N>(a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t, valid, a.D, A.wide, sc.part, qh, ql);
+  const int ge = load_rows<N>(A.g.dy.p + b * A.g.dy.b + head * A.g.dy.h + (int64_t)i * A.g.dy.t, valid, a.Dv, A.wide, share, gh, gl);
   const float slope = RICH && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
   const int64_t tile0 = (int64_t)slab * A.ktiles + t0;
   const uint32_t base = lds_address(lds) + w * 1024, lane16 = lane * 16;
@@ -435,7 +438,6 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   for (int d = 0; d < 2 * N; ++d) dq[d] = f32x4{};
   int cq = kUnset;
   const bool cap = RICH && a.cap > 0;
-  const float icap = cap ? 1.0f / a.cap : 0.0f;
   if (t0 < t1) fetch(0);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, j0 = t * kTile;
@@ -448,18 +450,20 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
     if (__builtin_expect(!any_seen(s, me, kt, j0), 0)) continue;
     // element q: key j0 + 16 (q / 4) + 4 g4 + q % 4
     float x[8], y[8];
-    pair<N>(L, 0, qh, ql, x, F_V, gh, gl, y);
+    pair<true, N>(L, 0, qh, ql, x, F_V, gh, gl, y);
     if (__builtin_expect(kt.uneven, 0)) per_row(x, side + KS_RELK * kTile, g4);
     if (__builtin_expect(vt.uneven, 0)) per_row(y, side + KS_RELV * kTile, g4);
-    const int unit = exponent(kt.inv) - qe;
     const float yunit = dot_unit(exponent(vt.inv) - ge);
-    if (cap) tanh_all(x, score_unit(a.scale * icap, unit));
-    const float f = cap ? a.cap * kLog2e : score_unit(a.scale * kLog2e, unit);
+    float f = score_unit(sc, exponent(kt.inv) - qe);
+    if (cap) {
+      tanh_all(x, f);
+      f = a.cap * kLog2e;
+    }
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      float off = lse;
-      if (RICH && a.slopes) off = fmaf(slope, fabsf((float)(p - (j0 + 16 * (q / 4) + 4 * g4 + q % 4))), lse);
-      y[q] = __builtin_amdgcn_exp2f(fmaf(x[q], f, -off)) * fmaf(y[q], yunit, -dot);
+      const int far = p - (j0 + 16 * (q / 4) + 4 * g4 + q % 4);
+      const float less = RICH ? score_of(a.slopes, x[q], f, slope, far) - top : fmaf(x[q], f, -top);
+      y[q] = __builtin_amdgcn_exp2f(less) * fmaf(y[q], yunit, -dot);
       if (cap) y[q] *= fmaf(-x[q], x[q], 1.0f);
     }
     if (__builtin_expect(!all_seen(s, me, kt, j0), 0)) {
@@ -563,10 +567,10 @@ void attend_grad(const AttendGradDesc& g, void* work, hipStream_t st) {
   k.wide = wide;
   k.a = a;
   float *qs = (float*)(w + p.qside), *ks = (float*)(w + p.kside);
-  k.job[0] = {a.q, a.D, p.G, p.M, p.qtiles, half(p.qr), half(p.qc), info(p.qi), true, qs, QS_RELQ, false, false, {}};
-  k.job[1] = {g.dy, a.Dv, p.G, p.M, p.qtiles, half(p.gr), half(p.gc), info(p.gi), true, qs, QS_RELG, true, true, a.y};
-  k.job[2] = {a.k, a.D, 1, a.Tk, p.ktiles, half(p.kr), half(p.kc), info(p.ki), false, ks, KS_RELK, false, true, {}};
-  k.job[3] = {a.v, a.Dv, 1, a.Tk, p.ktiles, half(p.vr), nullptr, info(p.vi), false, ks, KS_RELV, true, false, {}};
+  k.job[0] = {a.q, a.D, p.G, p.M, p.qtiles, half(p.qr), half(p.qc), info(p.qi), true, qs, QS_RELQ, false, false, true, {}};
+  k.job[1] = {g.dy, a.Dv, p.G, p.M, p.qtiles, half(p.gr), half(p.gc), info(p.gi), true, qs, QS_RELG, true, true, false, a.y};
+  k.job[2] = {a.k, a.D, 1, a.Tk, p.ktiles, half(p.kr), half(p.kc), info(p.ki), false, ks, KS_RELK, false, true, false, {}};
+  k.job[3] = {a.v, a.Dv, 1, a.Tk, p.ktiles, half(p.vr), nullptr, info(p.vi), false, ks, KS_RELV, true, false, false, {}};
   attend_pack(k, p.DP, st);
   const GradArgs A{g, half(p.qr), half(p.qc), half(p.gr), half(p.gc), half(p.kr), half(p.kc), half(p.vr),
                    info(p.qi), info(p.gi), info(p.ki), info(p.vi), qs, ks, make_fastdiv(p.G), p.M, p.qtiles,

@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256) void attend_small(AttendDesc a) {
     for (int o = 1; o < Z::T; o *= 2) sum += __shfl_xor(sum, o);
     if (sub == 0) {
       total[r] = any ? sum : INFINITY;             // a row that sees nothing is 0
-      if (a.lse) a.lse[((int64_t)b * a.H + w.head) * a.Tq + w.i] = any ? m + __builtin_amdgcn_logf(sum) : INFINITY;
+      if (a.stats) write_stats(a, ((int64_t)b * a.H + w.head) * a.Tq + w.i, !any, m, sum);
     }
   }
   if (!a.y.p) return;
@@ -184,13 +184,15 @@ __global__ __launch_bounds__(256) void attend_grad_small(AttendGradDesc g) {
     const int r = ti + 16 * i;
     if (r >= M) break;
     const Row w = row_at(a, s, hk, G, r);
-    const float slope = a.slopes ? a.slopes[w.head] * kLog2e : 0.0f, lse = a.lse[((int64_t)b * a.H + w.head) * a.Tq + w.i];
+    const float slope = a.slopes ? a.slopes[w.head] * kLog2e : 0.0f;
+    const float* stats = a.stats + 2 * (((int64_t)b * a.H + w.head) * a.Tq + w.i);
+    const float top = stats[0], share = stats[1];
 #pragma unroll
     for (int e = 0; e < Z::I; ++e) {
       const int j = tj + 16 * e;
       const PlainPair c = plain_score(a, x[i][e], slope, w.p - j);
       const bool shown = sees(s, w, j);
-      const float weight = shown ? __builtin_amdgcn_exp2f(c.score - lse) : 0.0f;
+      const float weight = shown ? __builtin_amdgcn_exp2f(c.score - top) * share : 0.0f;
       p[r * Z::LP + j] = weight;
       ds[r * Z::LP + j] = shown ? weight * (z[i][e] - dots[r]) * c.slack : 0.0f;
     }

@@ -750,10 +750,10 @@ static std::vector<int> op_inputs(const tgj::Value& op) {
       {"conv2d_weight_grad", {"input", "dy"}}, {"max_pool_2d", {"input"}},
       {"max_pool_2d_grad", {"input", "dy"}},
       {"attention", {"q", "k", "v", "documents", "prefix", "lengths"}},
-      {"attention_lse", {"q", "k", "v", "documents", "prefix", "lengths"}},
-      {"attention_grad_q", {"q", "k", "v", "y", "lse", "dy", "documents", "prefix", "lengths"}},
-      {"attention_grad_k", {"q", "k", "v", "y", "lse", "dy", "documents", "prefix", "lengths"}},
-      {"attention_grad_v", {"q", "k", "v", "y", "lse", "dy", "documents", "prefix", "lengths"}},
+      {"attention_stats", {"q", "k", "v", "documents", "prefix", "lengths"}},
+      {"attention_grad_q", {"q", "k", "v", "y", "stats", "dy", "documents", "prefix", "lengths"}},
+      {"attention_grad_k", {"q", "k", "v", "y", "stats", "dy", "documents", "prefix", "lengths"}},
+      {"attention_grad_v", {"q", "k", "v", "y", "stats", "dy", "documents", "prefix", "lengths"}},
       {"rope_axes", {"a", "positions"}}, {"linear_recurrence", {"a", "x", "h0"}},
       {"linear_recurrence_grad_a", {"a", "h", "dh", "h0"}}, {"linear_recurrence_grad_x", {"a", "h", "dh", "h0"}},
       {"linear_recurrence_grad_h0", {"a", "h", "dh", "h0"}},
@@ -3792,7 +3792,7 @@ std::function<tgk::AttendDesc()> Runtime::attend_binder(int i, const tgk::Attend
 
 #define TG_MASKED "q", "k", "v", "documents", "prefix", "lengths", "causal", "scale", "softcap", "slopes"
 
-// attention and attention_lse of the same inputs: one node, whichever comes first in the graph.
+// attention and attention_stats of the same inputs: one node, whichever comes first in the graph.
 void Runtime::lower_attend(int i) {
   Node n;
   n.kind = "attend";
@@ -3801,11 +3801,11 @@ void Runtime::lower_attend(int i) {
   n.detail = kinds_[i];
   tgk::AttendDesc d{};
   mask_fields(i, n, d);
-  int y = -1, lse = -1;
-  auto take = [&](int j) { (kinds_[j] == "attention" ? y : lse) = O(j).at("out").i32(); };
+  int y = -1, stats = -1;
+  auto take = [&](int j) { (kinds_[j] == "attention" ? y : stats) = O(j).at("out").i32(); };
   take(i);
   for (int j = i + 1; j < (int)ops_.size(); ++j)
-    if ((kinds_[j] == "attention" ? y : kinds_[j] == "attention_lse" ? lse : 0) < 0 && !gemm_done_[j] &&
+    if ((kinds_[j] == "attention" ? y : kinds_[j] == "attention_stats" ? stats : 0) < 0 && !gemm_done_[j] &&
         same_fields(i, j, {TG_MASKED})) {
       take(j);
       gemm_done_[j] = 1;
@@ -3815,13 +3815,14 @@ void Runtime::lower_attend(int i) {
     expect(T_[y].shape == Dims({d.B, d.H, d.Tq, d.Dv}) && T_[y].dt == F32, i, "bad output shape");
     n.writes.push_back(root(y));
   }
-  if (lse >= 0) {
-    expect(T_[lse].shape == Dims({d.B, d.H, d.Tq}) && T_[lse].dt == F32, i, "bad output shape");
-    n.writes.push_back(root(lse));
+  if (stats >= 0) {
+    expect(T_[stats].shape == Dims({d.B, d.H, d.Tq, 2}) && T_[stats].dt == F32, i, "bad output shape");
+    n.writes.push_back(root(stats));
   }
   n.shape = shape_str(T_[fld(i, "q")].shape) + "x" + shape_str(T_[fld(i, "k")].shape);
   n.flops = 2.0 * d.B * d.H * (double)d.Tq * d.Tk * (d.D + d.Dv);
   n.bytes = 4.0 * (T_[fld(i, "q")].numel + T_[fld(i, "k")].numel + T_[fld(i, "v")].numel + (y >= 0 ? T_[y].numel : 0));
+  d.stats = stats >= 0 ? (float*)16 : nullptr;   // presence decides the kernels; the address follows at bind
   const int64_t ws = tgk::attend_workspace_bytes(d);
   workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
   n.ws = ws > 0;
@@ -3829,7 +3830,7 @@ void Runtime::lower_attend(int i) {
   n.bind = [=]() -> std::function<void(hipStream_t)> {
     tgk::AttendDesc a = desc();
     if (y >= 0) a.y = rows_of(y, "attention y");
-    a.lse = lse >= 0 ? (float*)dptr(lse) : nullptr;
+    a.stats = stats >= 0 ? (float*)dptr(stats) : nullptr;
     void* w = cur_ws_;
     return [=](hipStream_t st) { tgk::attend(a, w, st); };
   };
@@ -3845,15 +3846,15 @@ void Runtime::lower_attend_grad(int i) {
   tgk::AttendGradDesc g{};
   mask_fields(i, n, g.a);
   const tgk::AttendDesc& d = g.a;
-  const int y = fld(i, "y"), lse = fld(i, "lse"), dy = fld(i, "dy");
+  const int y = fld(i, "y"), stats = fld(i, "stats"), dy = fld(i, "dy");
   const Dims ys = {d.B, d.H, d.Tq, d.Dv};
-  expect(T_[y].shape == ys && T_[dy].shape == ys && T_[lse].shape == Dims({d.B, d.H, d.Tq}) && T_[y].dt == F32 &&
-             T_[dy].dt == F32 && T_[lse].dt == F32 && view_[lse].contiguous(), i, "y, dy or lse do not fit");
-  for (int t : {y, lse, dy}) n.reads.push_back(root(t));
+  expect(T_[y].shape == ys && T_[dy].shape == ys && T_[stats].shape == Dims({d.B, d.H, d.Tq, 2}) && T_[y].dt == F32 &&
+             T_[dy].dt == F32 && T_[stats].dt == F32 && view_[stats].contiguous(), i, "y, dy or stats do not fit");
+  for (int t : {y, stats, dy}) n.reads.push_back(root(t));
   int out[3] = {-1, -1, -1};
   for (int j = i; j < (int)ops_.size(); ++j) {
     if (kinds_[j].compare(0, 15, "attention_grad_") != 0 || gemm_done_[j]) continue;
-    if (j != i && !same_fields(i, j, {TG_MASKED, "y", "lse", "dy"})) continue;
+    if (j != i && !same_fields(i, j, {TG_MASKED, "y", "stats", "dy"})) continue;
     const int which = kinds_[j].back() == 'q' ? 0 : kinds_[j].back() == 'k' ? 1 : 2;
     if (out[which] >= 0) continue;
     out[which] = O(j).at("out").i32();
@@ -3879,7 +3880,7 @@ void Runtime::lower_attend_grad(int i) {
     tgk::AttendGradDesc b{};
     b.a = desc();
     b.a.y = rows_of(y, "attention y");
-    b.a.lse = (float*)dptr(lse);
+    b.a.stats = (float*)dptr(stats);
     b.dy = rows_of(dy, "attention dy");
     if (dq >= 0) b.dq = rows_of(dq, "attention dq");
     if (dk >= 0) b.dk = rows_of(dk, "attention dk");
@@ -4710,7 +4711,7 @@ void Runtime::lower_op(int i) {
       const float* pd = (const float*)dptr(dy);
       return [=](hipStream_t st) { tgk::max_pool_grad(px, pd, po, p, st, relu); };
     };
-  } else if (k == "attention" || k == "attention_lse") {
+  } else if (k == "attention" || k == "attention_stats") {
     lower_attend(i);
     return;
   } else if (k.compare(0, 15, "attention_grad_") == 0) {

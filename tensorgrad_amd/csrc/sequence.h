@@ -13,11 +13,11 @@ struct Rows {
 };
 
 // y = attention(q, k, v), see ops.py: score = cap tanh(scale q.k / cap) - slope |p - j| (cap 0: scale q.k), p = n - Tq + i
-// for the n keys of a batch entry. y or lse may be absent (null).
+// for the n keys of a batch entry. y or stats may be absent (null).
 struct AttendDesc {
   int B, H, Hk, Tq, Tk, D, Dv;
   Rows q, k, v, y;
-  float* lse;                // [B, H, Tq]: log2 of the sum of exp(score); +inf for a row that sees nothing (its exp2(s - lse) is 0)
+  float* stats;              // [B, H, Tq, 2], for the gradients: P = exp2(score log2(e) - stats[0]) stats[1]
   const int32_t* documents;  // [B, Tk] or null
   const int32_t* prefix;     // [B] or null
   const int32_t* lengths;    // [B] or null
@@ -26,7 +26,7 @@ struct AttendDesc {
   bool causal, positional;   // positional: a query before position 0 sees nothing
 };
 struct AttendGradDesc {
-  AttendDesc a;              // a.y and a.lse: the forward's results, read
+  AttendDesc a;              // a.y and a.stats: the forward's results, read
   Rows dy, dq, dk, dv;       // dq, dk, dv may be absent (null)
 };
 constexpr int kAttendMaxHead = 128;

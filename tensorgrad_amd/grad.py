@@ -266,7 +266,7 @@ def _adjoint(op: dict, oc: Tensor, graph: Graph, cot: Dict[int, Tensor]) -> None
         grads = O.linear_recurrence_grad(T(op['a']), T(op['out']), oc, h0)
         for n, c in zip(('a', 'x', 'h0'), grads):
             acc(op[n], c)
-    elif k == 'attention_lse' or k.startswith(('attention_grad_', 'linear_recurrence_grad_')):
+    elif k == 'attention_stats' or k.startswith(('attention_grad_', 'linear_recurrence_grad_')):
         raise ValueError(f"autograd: cannot differentiate through {k} (it's a backward op)")
     elif k in ('conv2d_input_grad', 'conv2d_weight_grad', 'max_pool_2d_grad', 'scatter_axis'):
         raise ValueError(f"autograd: cannot differentiate through {k} (it's a backward op)")

@@ -105,10 +105,10 @@ OP_KINDS = tuple(_INPUT_FIELDS.keys())
 _MASKS = ('documents', 'prefix', 'lengths')
 _EXTENSIONS: Dict[str, Tuple[str, ...]] = {
     'attention': ('q', 'k', 'v') + _MASKS,
-    'attention_lse': ('q', 'k', 'v') + _MASKS,
-    'attention_grad_q': ('q', 'k', 'v', 'y', 'lse', 'dy') + _MASKS,
-    'attention_grad_k': ('q', 'k', 'v', 'y', 'lse', 'dy') + _MASKS,
-    'attention_grad_v': ('q', 'k', 'v', 'y', 'lse', 'dy') + _MASKS,
+    'attention_stats': ('q', 'k', 'v') + _MASKS,
+    'attention_grad_q': ('q', 'k', 'v', 'y', 'stats', 'dy') + _MASKS,
+    'attention_grad_k': ('q', 'k', 'v', 'y', 'stats', 'dy') + _MASKS,
+    'attention_grad_v': ('q', 'k', 'v', 'y', 'stats', 'dy') + _MASKS,
     'rope_axes': ('a', 'positions'),
     'linear_recurrence': ('a', 'x', 'h0'),
     'linear_recurrence_grad_a': ('a', 'h', 'dh', 'h0'),

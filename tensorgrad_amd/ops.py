@@ -622,8 +622,8 @@ def attention_grad(q: Tensor, k: Tensor, v: Tensor, y: Tensor, dy: Tensor, causa
         if t.dtype != 'f32' or t.shape != shape:
             raise ShapeError(f'{site}: {name} must be f32 {S.show(shape)}, got {t.dtype} {S.show(t.shape)}', site)
     g = current_graph()
-    lse = add_op(g, 'attention_lse', q.shape[:3], 'f32', site, f)
-    f = dict(f, y=y.id, lse=lse.id, dy=dy.id)
+    stats = add_op(g, 'attention_stats', (*q.shape[:3], 2), 'f32', site, f)
+    f = dict(f, y=y.id, stats=stats.id, dy=dy.id)
     return tuple(add_op(g, f'attention_grad_{n}', t.shape, 'f32', site, f) for n, t in (('q', q), ('k', k), ('v', v)))
 
 

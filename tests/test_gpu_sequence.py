@@ -1114,3 +1114,47 @@ def test_rope_axes_of_the_least_base():
     want, tol = R.rope_axes(q, pos, [4], 2.0 ** -16)
     for g in got:
         R.check(g, want, tol)
+
+
+@pytest.mark.parametrize('B,H,Hk,Tq,Tk,D', [(2, 2, 1, 20, 20, 16), (1, 2, 1, 90, 90, 64), (1, 2, 1, 300, 300, 128), (1, 1, 1, 64, 3000, 40),
+                                            (2, 4, 2, 1, 700, 64)])
+@pytest.mark.parametrize('how', [{}, dict(softcap=2.0 ** 50), dict(slopes=1e-3), dict(softcap=2.0 ** 50, slopes=1e-3)],
+                         ids=['plain', 'cap', 'slopes', 'both'])
+@pytest.mark.parametrize('size', [1e4, 1e6, 1e8, 1e10, 1e14, 1e30])
+def test_scores_of_any_size_choose_their_key(B, H, Hk, Tq, Tk, D, how, size):
+    """Keys are words of +-1.37 and a query is `size` times the word of one key that it sees: its score leads by `size` / D and
+    more, which is hundreds, though f32 holds it to `size` / 2^24 alone. So y is that key's value, dv the sum of dy over the
+    queries of a key, and dq and dk are what rounding leaves of dP - D, which cancel: dP and D are each off by (12 + 8 sqrt D)
+    roundings of |dy| |v| (the split of both operands, their sums, y's own roundings), in rows that the scale and |k| or |q|
+    multiply."""
+    if size > 1e14 and 'softcap' in how:
+        return                                           # the cap is reached
+    r = rng(B, H, Tq, Tk, D, 101)
+    how = dict(how, slopes=[how['slopes']] * H) if 'slopes' in how else how
+    _, _, v, dy = qkv(B, H, Hk, Tq, Tk, D, D, 102)
+    k = f32(1.37 * r.choice([-1, 1], (B, Hk, Tk, D)))
+    chosen = (r.random((B, H, Tq)) * (np.arange(Tq) + 1 + Tk - Tq)).astype(int)
+    word = np.stack([[k[b, h * Hk // H][chosen[b, h]] for h in range(H)] for b in range(B)])
+    q = f32(word * f32(size / 1.7))
+    s = np.einsum('bhqd,bhkd->bhqk', q.astype(np.float64), np.repeat(k, H // Hk, 1).astype(np.float64)) / np.sqrt(D)
+    np.put_along_axis(s, chosen[..., None], -np.inf, 3)
+    lead = size / 1.7 * 1.37 ** 2 * np.sqrt(D) - s.max(3)
+    assert lead.min() > 100                              # words are apart
+    got = attend(q, k, v, dy, how)
+    y = np.stack([[v[b, h * Hk // H][chosen[b, h]] for h in range(H)] for b in range(B)])
+    R.check(got['y'], y.astype(np.float64), 16 * R.U * np.abs(y), 'y')
+    dv, dva, n = np.zeros(v.shape), np.zeros(v.shape), np.zeros(v.shape[:3] + (1,))
+    for b in range(B):
+        for h in range(H):
+            np.add.at(dv[b, h * Hk // H], chosen[b, h], dy[b, h].astype(np.float64))
+            np.add.at(dva[b, h * Hk // H], chosen[b, h], np.abs(dy[b, h]))
+            np.add.at(n[b, h * Hk // H], chosen[b, h], 1)
+    R.check(got['dv'], dv, (16 + 4 * np.sqrt(n)) * R.U * dva + 1e-30, 'dv')
+    norm = lambda z: np.linalg.norm(z, axis=-1, keepdims=True)  # noqa: E731
+    noise = 2 * (12 + 8 * np.sqrt(D)) * R.U * norm(dy) * norm(y) / np.sqrt(D)
+    R.check(got['dq'], np.zeros(q.shape), noise * 1.37 + 0 * q, 'dq')
+    worst = np.zeros(v.shape[:3] + (1,))
+    for b in range(B):
+        for h in range(H):
+            np.add.at(worst[b, h * Hk // H], chosen[b, h], noise[b, h] * np.abs(q).max())
+    R.check(got['dk'], np.zeros(k.shape), worst + 1e-30 * size + 0 * k, 'dk')
