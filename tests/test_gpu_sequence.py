@@ -1158,3 +1158,43 @@ def test_scores_of_any_size_choose_their_key(B, H, Hk, Tq, Tk, D, how, size):
         for h in range(H):
             np.add.at(worst[b, h * Hk // H], chosen[b, h], noise[b, h] * np.abs(q).max())
     R.check(got['dk'], np.zeros(k.shape), worst + 1e-30 * size + 0 * k, 'dk')
+
+
+@pytest.mark.parametrize('H,Tq,Tk,D', [(1, 1, 1000, 64), (4, 1, 3000, 128), (2, 2, 700, 96), (16, 1, 5000, 32), (1, 3, 129, 17)])
+@pytest.mark.parametrize('how', [{}, dict(softcap=2.0 ** 50), dict(slopes=1e-3)], ids=['plain', 'cap', 'slopes'])
+@pytest.mark.parametrize('size', [1e4, 1e8, 1e14])
+def test_few_rows_of_scores_of_any_size(H, Tq, Tk, D, how, size):
+    """As above, without gradients: the keys are read as they are. 17 features: words that differ in one alone are 2 / 17 apart."""
+    r = rng(H, Tq, Tk, D, 103)
+    how = dict(how, slopes=[how['slopes']] * H) if 'slopes' in how else how
+    v = f32(r.standard_normal((2, 1, Tk, D)))
+    words = np.unique(r.choice([-1, 1], (4 * Tk, D)), axis=0)
+    k = f32(1.37 * np.stack([r.permutation(words)[:Tk] for _ in range(2)])[:, None])
+    chosen = (r.random((2, H, Tq)) * (np.arange(Tq) + 1 + Tk - Tq)).astype(int)
+    q = f32(np.stack([k[b, 0][chosen[b]] for b in range(2)]) * f32(size / 1.7))
+    y = attend(q, k, v, None, how)['y']
+    want = np.stack([v[b, 0][chosen[b]] for b in range(2)])
+    R.check(y, want.astype(np.float64), 16 * R.U * np.abs(want))
+
+
+@pytest.mark.parametrize('ratio', [2.0 ** 14, 2.0 ** 18, 2.0 ** 22])
+def test_features_of_very_different_size(ratio):
+    """One feature of k, and of v, `ratio` times the others, q's smaller by as much. A value is held to 2^-22 of itself or 2^-39 of
+    its row's (its tile's) largest, whichever is more: f16 parts of values scaled to 2^14 .. 2^15, whose steps end at 2^-24. The
+    second part of the bound counts that for the scores and for y; the rest is as everywhere."""
+    q, k, v, _ = qkv(1, 2, 1, 150, 150, 64, 64, 104)
+    q[..., 3] /= ratio
+    k[..., 3] *= ratio
+    v[..., 7] *= ratio
+    y = attend(q, k, v)['y']
+    tri, eps = np.tril(np.ones((150, 150), bool)), 2.0 ** -39
+    for h in range(2):
+        Q, K, V = (x.astype(np.float64) for x in (q[0, h], k[0, 0], v[0, 0]))
+        s = np.where(tri, Q @ K.T / 8, -np.inf)
+        P = np.exp(s - s.max(1, keepdims=True))
+        P /= P.sum(1, keepdims=True)
+        a = np.abs
+        e = (17 + 4 * 8) * R.U * a(Q) @ a(K).T + eps * (a(Q).max(1)[:, None] * a(K).sum(1)[None] + a(Q).sum(1)[:, None] * a(K).max())
+        E = np.where(tri, e / 8, 0).max(1)[:, None]
+        tol = (2 * E + (20 + 8 * np.sqrt(150)) * R.U) * (P @ a(V)) + eps * a(V).max()
+        R.check(y[0, h], P @ V, tol, str(ratio))
