@@ -334,8 +334,8 @@ class Runtime {
   // recorded after every call would say the same, for 4 us of the stream's time.)
   // And host calls of several threads: those of a family run beside each other, a run_device beside none, as it reads what
   // they write (parameters) and they have waited only for what was enqueued before. They return with their work done. Nor
-  // beside one that captures its step, or the creation of a sibling, which copies on the default stream: HIP refuses that
-  // stream's work while another is captured.
+  // beside one that captures its step, nor does the part of a sibling's creation that copies on the default stream: HIP refuses
+  // that stream's work while another is captured.
   struct Pending {
     std::mutex gate;                 // taken before `order`, so that neither kind keeps the other waiting for ever
     std::shared_mutex order;
@@ -680,10 +680,17 @@ Runtime::Runtime(const char* json, Runtime* par, bool plan_only) : parent(par) {
   if (!plan_only) hip_check(hipGetDevice(&device_), "hipGetDevice");
   pending_ = par ? par->pending_ : std::make_shared<Pending>();
   split_init_nodes();
-  allocate();
-  bind_all();   // in plan-only mode this still runs every launch's host-side bounds proof
+  auto alone = [&] { return par ? lone_call() : std::unique_lock<std::shared_mutex>(); };
+  {
+    const auto order = alone();   // copies on the default stream
+    allocate();
+    bind_all();   // in plan-only mode this still runs every launch's host-side bounds proof
+  }
   jit_finish();
-  if (!plan_only) prepare_noalloc();
+  if (!plan_only) {
+    const auto order = alone();
+    prepare_noalloc();
+  }
   if (!plan_only && !init_nodes_.empty()) {
     for (auto& n : init_nodes_) n.launch(stream_);
     hip_check(hipStreamSynchronize(stream_), "hipStreamSynchronize(constants)");
@@ -5777,7 +5784,6 @@ tg_status tg_runtime_create_sibling(tg_runtime* parent, const char* ir_json, tg_
   return guarded([&] {
     auto* h = new tg_runtime();
     try {
-      const auto order = parent->rt->lone_call();
       h->rt.reset(new tg::Runtime(ir_json, parent->rt.get()));
     } catch (...) {
       delete h;
