@@ -48,8 +48,8 @@ struct TileInfo {
 // What a block needs of each row of a tile it walks, 32 values each (integers as bits), 2 KiB that come with the fragments
 // into LDS: of queries and of keys. Row S_INFO: the TileInfo of the first operand (q, k) and eight words on the second's (dy,
 // v). From LDS, because a load from memory inside the loop would wait for the next tile's fragments, which are ahead of it.
-enum { QS_TOP, QS_SHARE, QS_DOT, QS_POS, QS_SLOPE, QS_BELOW, QS_DOC, QS_RELQ, QS_RELG, S_INFO, kSide = 16 };   // dot(dy, y) share;
-                                                                                                               // sees keys below
+// QS_DOT: dot(dy, y) share; QS_BELOW: sees keys below.
+enum { QS_TOP, QS_SHARE, QS_DOT, QS_POS, QS_SLOPE, QS_BELOW, QS_DOC, QS_RELQ, QS_RELG, S_INFO, kSide = 16 };
 enum { KS_DOC, KS_RELK, KS_RELV };
 constexpr int kSideFrags = kSide * kTile * 4 / 1024;
 
@@ -408,7 +408,8 @@ __device__ __forceinline__ TileInfo side_info(const float* side, int x) {
   return {__int_as_float(u(p[0])), __int_as_float(u(p[1])), u(p[2]), u(p[3]), u(p[4]), u(p[5]), u(p[6]), 0};
 }
 // Does a query with these bounds see key z of the tile at j0. Without branches: with the document read behind the other
-// conditions the compiler has lost the value chosen (capped scores and documents: gradients of 0).
+// conditions, `if (!seen) x[q] = 0` comes out of the compiler wrong (right in its IR; in the machine code the block for keys of
+// other documents is empty, their 0 written before a copy of the whole vector undoes it), and hidden keys keep their values.
 __device__ __forceinline__ bool key_seen(const Sight& s, const float* side, int j0, int z, int below, int doc) {
   const int id = __float_as_int(side[KS_DOC * kTile + z]);
   return (j0 + z < below) & (!s.doc | ((doc >= 0) & (id == doc)));

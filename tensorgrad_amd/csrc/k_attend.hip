@@ -16,7 +16,7 @@ namespace {
 
 // A block packs one tile of 32 rows: reads them once, finds their scales, writes its fragments. Rows that see nothing and
 // are seen by nothing are packed as zeros, whatever they hold. Bound by memory: the seven operands of a gradient over 4096
-// rows of 16 query and 4 key heads of 128 are 50 us (117 MB read, 159 MB written: 5.5 TB/s).
+// rows of 16 query and 4 key heads of 128 are 51 us (117 MB read, 159 MB written: 5.4 TB/s).
 template <int DP>
 __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
   constexpr int DB = DP / 32, LD = DP + 4;
@@ -209,7 +209,7 @@ __device__ __forceinline__ void plain_rows(const TilesArgs& A, const Sight& s, i
 }
 
 // Bound by the issue of products and vector work together, which overlap only between wavefronts: 4096 x 4096 pairs without
-// masks, 8 heads of 128: 208 us, 330 TFLOP/s of the 443 that three f16 products for one allow; capped and causal: 158 us. k and
+// masks, 8 heads of 128: 204 us, 337 TFLOP/s of the 443 that three f16 products for one allow; capped and causal: 156 us. k and
 // v come two tiles in turn: the next one travels while this one is multiplied.
 template <int DP, bool CAP, bool SLOPES>
 __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
@@ -372,7 +372,7 @@ struct FewArgs {
 // maximum, sum and result of its own (the maximum from f32's lowest on, so that weights of scores of minus infinity are 0
 // whatever came before); the 32 groups of a block are joined once at its end. A part is the same number of keys
 // for every batch entry, so that blocks past a short one end at once and those that work are alike. 8 caches of up to 16000
-// keys, 4 key heads of 128, 16 query heads: 66 us, 6.0 TB/s.
+// keys, 4 key heads of 128, 16 query heads: 67 to 68 us, 5.8 TB/s.
 template <int E, int R, bool WIDE>
 __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
   const AttendDesc& a = A.a;
@@ -523,7 +523,7 @@ struct JoinArgs {
   const float* part;
   const f32x2* psum;
 };
-// Bound by memory (24864 rows of 2 parts of 96: 10 us). L threads join a row: its weights first, then every 32 threads an
+// Bound by memory (24864 rows of 2 parts of 96: 11 us). L threads join a row: its weights first, then every 32 threads an
 // L / 32nd of the parts. 32 threads take a row with few parts and a block one with many (a long cache read by one token: 16
 // parts by 32 threads or 64 by a block, 8 or 7 us; one thread a feature took 33). A sum of NaN makes the row NaN.
 template <int L>

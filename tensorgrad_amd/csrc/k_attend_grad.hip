@@ -36,8 +36,8 @@ __device__ __forceinline__ void seeing_tiles(const GradArgs& A, const Sight& s, 
 }
 // Those of part `split`, equal stretches of all rows, so that blocks that run together walk the same ones. False: none, which
 // the join finds again and does not read. With documents the stretch that a key block's own see is short: there its tiles are
-// cut into equal parts, of 8 at least, when they are known (8 x 1000 positions, 2 key heads of 64, with 32 keys a wavefront:
-// documents of 50 took 53 us instead of 81, of 170 82 instead of 87; one document 130 instead of 123).
+// cut into equal parts, of 8 at least, when they are known (8 x 1000 positions, 2 key heads of 64: documents of 50 take 47 us and
+// 10 to join instead of 121 uncut, of 170 66 and 11 instead of 165, one document 120 and 13 instead of 282).
 __device__ __forceinline__ bool part_rows(const GradArgs& A, const Sight& s, int k0, int split, int& from, int& to) {
   seeing_tiles(A, s, k0, from, to);
   if (A.splits == 1 || s.doc) return true;
@@ -108,8 +108,8 @@ __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, in
 }
 
 // Eight wavefronts of 16 keys. WHAT: 1 for dk, 2 for dv, 3 for both in one walk. Up to head size 64 two blocks share a CU. Both
-// gradients of 4096 causal rows of 16 heads of 128: 664 us (by 32 keys 990, in walks of their own); of 8 heads of 64: 193 us
-// (205); of 8 x 1000 rows of 8 heads of 64 in documents of 170: 66 us (81); of 32 without documents: 76 us (66).
+// gradients of 4096 capped causal rows of 16 heads of 128: 679 us (by 32 keys 990, in walks of their own); of 8 heads of 64:
+// 194 us (205); of 8 x 1000 rows of 8 heads of 64 in documents of 170: 66 us (81); of 32 without documents: 87 us.
 template <int DP, bool RICH, int WHAT>
 __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs A) {
   constexpr int N = DP / 32, F = 4 * N;                      // chunks of 32 features; fragments of an operand
@@ -219,16 +219,19 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
     for (int q4 = 0; q4 < 2; ++q4) {
       const int at = 16 * q4 + 4 * g;
       const f32x4 top = *(const f32x4*)(side + QS_TOP * kTile + at), dot = *(const f32x4*)(side + QS_DOT * kTile + at);
-      f32x4 pos = {}, slope = {};
+      f32x4 less;                  // score less top
       if (RICH && a.slopes) {
-        pos = *(const f32x4*)(side + QS_POS * kTile + at);
-        slope = *(const f32x4*)(side + QS_SLOPE * kTile + at);
+        const f32x4 pos = *(const f32x4*)(side + QS_POS * kTile + at), slope = *(const f32x4*)(side + QS_SLOPE * kTile + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) less[e] = score_of(true, x[4 * q4 + e], f, slope[e], __float_as_int(pos[e]) - j) - top[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) less[e] = RICH ? rounded_mul(x[4 * q4 + e], f) - top[e] : fmaf(x[4 * q4 + e], f, -top[e]);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int q = 4 * q4 + e;
-        const float far = RICH ? score_of(a.slopes, x[q], f, slope[e], __float_as_int(pos[e]) - j) - top[e] : fmaf(x[q], f, -top[e]);
-        const float p = __builtin_amdgcn_exp2f(far);
+        const float p = __builtin_amdgcn_exp2f(less[e]);
         if (DK) {
           y[q] = p * fmaf(y[q], yunit, -dot[e]);
           if (RICH && a.cap > 0) y[q] *= fmaf(-x[q], x[q], 1.0f);   // 1 - tanh^2
@@ -360,8 +363,8 @@ __device__ __forceinline__ void plain_dq(const GradArgs& A, const Sight& s, int 
   }
 }
 
-// Eight wavefronts of 16 query rows. 4096 causal rows of 16 heads of 128: 371 us (470 by 32 rows); 8 x 1000 rows of 8 heads
-// of 64 in documents of 170: 43 us (57).
+// Eight wavefronts of 16 query rows. 4096 capped causal rows of 16 heads of 128: 374 us (470 by 32 rows); 8 x 1000 rows of 8
+// heads of 64 in documents of 170: 42 us (57).
 template <int DP, bool RICH>
 __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   constexpr int N = DP / 32, F = 4 * N, F_V = F, F_KC = 2 * F, F_SIDE = 3 * F, NF = F_SIDE + kSideFrags;
@@ -459,11 +462,17 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
       tanh_all(x, f);
       f = a.cap * kLog2e;
     }
+    float less[8];                 // score less top
+    if (RICH && a.slopes) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) less[q] = score_of(true, x[q], f, slope, p - (j0 + 16 * (q / 4) + 4 * g4 + q % 4)) - top;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) less[q] = RICH ? rounded_mul(x[q], f) - top : fmaf(x[q], f, -top);
+    }
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      const int far = p - (j0 + 16 * (q / 4) + 4 * g4 + q % 4);
-      const float less = RICH ? score_of(a.slopes, x[q], f, slope, far) - top : fmaf(x[q], f, -top);
-      y[q] = __builtin_amdgcn_exp2f(less) * fmaf(y[q], yunit, -dot);
+      y[q] = __builtin_amdgcn_exp2f(less[q]) * fmaf(y[q], yunit, -dot);
       if (cap) y[q] *= fmaf(-x[q], x[q], 1.0f);
     }
     if (__builtin_expect(!all_seen(s, me, kt, j0), 0)) {

@@ -1,7 +1,7 @@
 // Attention over a few dozen positions (sample-sized models), forward and gradients, in plain f32: a block takes a key head
 // and its G Tq query rows whole, in LDS, one launch a direction. Bound by launches and by the latency of a block's phases
-// (loads, products, softmax): for 256 key heads of 16 positions and head size 16 a training step is 6.4 + 8.2 us of kernels,
-// 20 us as called; packing, tiles and the two gradient walks were five launches and 32. 64 positions, head size 32: 39 us
+// (loads, products, softmax): for 256 key heads of 16 positions and head size 16 a training step is 6.4 + 8.3 us of kernels,
+// 19 us as called; packing, tiles and the two gradient walks were five launches and 32. 64 positions, head size 32: 39 us
 // instead of 49, and the same (38) for 8 key heads, which is where longer ones are left to the tiles.
 #include "attend_dev.h"
 

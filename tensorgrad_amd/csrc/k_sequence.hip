@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void rope_pairs(RopeArgs R) {
 //    for bit): first those of whole groups of kGroup chunks, which the last block of each group joins and publishes, then
 //    those of its own group;
 //  * then the steps are run again from registers, now with the true state, and stored.
-// 4 x 8192 x 1024: forward 403 MB in 87 us (4.6 TB/s), backward 671 MB in 131 us (5.1 TB/s); a large copy reaches 5.0.
+// 4 x 8192 x 1024: forward 403 MB in 87 us (4.6 TB/s), backward 671 MB in 132 us (5.1 TB/s); a large copy reaches 5.0.
 // A state of 1e30 may fall to an ordinary value by a product of gates that f32 does not hold, so products are held as
 // s = A 2^100: A is exact to f32's roundings down to 2^-226, and what is lost below is at most 2^-250 of h_in, under 2^-122.
 // Gates above 1 in magnitude can take a product out of the range upwards (from 2^28 on) while no state is (h_in = 0, or a small
