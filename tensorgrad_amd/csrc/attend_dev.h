@@ -62,8 +62,9 @@ __device__ __forceinline__ float rounded_mul(float x, float y) {
 }
 // What a score is made of: the queries' values take the factor `part` (0.5 to 1, rounded once, wherever they are split), so that
 // the sum of products times 2^exp is q.k scale log2(e), or q.k scale / cap, without a rounding. That makes a score the same
-// number in every walk, forward and backward, and its distance to the row's largest exact: with a rounded factor inside a
-// fused multiply-add that distance was off by half a step of the largest, a factor of 2^128 for scores of 2^32.
+// number in every walk, forward and backward (but for low parts below f16's steps, 2^-27 of a row's largest), and its distance
+// to the row's largest exact: with a rounded factor inside a fused multiply-add that distance would be off by half a step of the
+// largest, a factor of 2^128 for scores of 2^32.
 struct Score {
   float part;
   int exp;
