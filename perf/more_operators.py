@@ -229,7 +229,8 @@ def _compiled(c, t):
         return [O.sample(i['logits'], i['u'], **how)]
 
     decl = {n: {'shape': list(x.shape), 'dtype': 'i32' if x.dtype == torch.int32 else 'f32'} for n, x in t.items()}
-    return compile_forward(Module(), {'window': window, 'linear': linear, 'sample': sample}[c['op']], decl, seed=0)
+    return compile_forward(Module(), {'window': window, 'linear': linear, 'sample': sample}[c['op']], decl,
+                           output='i32' if c['op'] == 'sample' else 'f32', seed=0)
 
 
 def _outputs(c):
