@@ -124,6 +124,7 @@ __device__ __forceinline__ float tanh_of(float x) {
 // What the queries of one batch entry see, wave-uniform.
 struct Sight {
   int n, first, prefix;            // keys that are there; position of query 0; keys every query sees
+  int window, stay;                // last keys that a query sees (0: all), beside the first `stay` (sinks and prefix)
   const int32_t* doc;
   bool causal, positional;
 };
@@ -132,6 +133,8 @@ __device__ __forceinline__ Sight sight(const AttendDesc& a, int b) {
   s.n = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
   s.first = s.n - a.Tq;
   s.prefix = a.prefix ? a.prefix[b] : 0;
+  s.window = a.window;
+  s.stay = max(a.sinks, s.prefix);
   s.doc = a.documents ? a.documents + (int64_t)b * a.Tk : nullptr;
   s.causal = a.causal;
   s.positional = a.positional;
@@ -141,6 +144,17 @@ __device__ __forceinline__ Sight sight(const AttendDesc& a, int b) {
 __device__ __forceinline__ int sees_below(const Sight& s, int p) {
   if (s.positional && p < 0) return 0;
   return s.causal ? min(s.n, max(p + 1, s.prefix)) : s.n;
+}
+// And of those from `sees_from` on, but for the first s.stay.
+__device__ __forceinline__ int sees_from(const Sight& s, int p) { return s.window ? p - s.window + 1 : INT32_MIN; }
+// Key tiles [g0, g1) of which no query from position p on sees anything: behind the first keys that stay, before its window.
+struct Gap {
+  int g0, g1;
+};
+__device__ __forceinline__ Gap gap_before(const Sight& s, int p) {
+  if (!s.window) return {0, 0};
+  const int g0 = (int)(((int64_t)max(s.stay, 0) + kTile - 1) / kTile);
+  return {g0, max(g0, max(p - s.window + 1, 0) / kTile)};
 }
 __device__ __forceinline__ int doc_at(const Sight& s, int p) { return s.doc && p >= 0 ? s.doc[p] : -1; }   // negative: sees nothing
 // Does it see any: then, where positions matter, the key at its own. From the masks, not from sums or maxima, which NaN and
@@ -164,11 +178,13 @@ struct Span {
 __device__ __forceinline__ bool any_seen(const Sight& s, const Span& q, const TileInfo& k, int j0) {
   if (j0 >= s.n || (s.positional && q.pmax < 0)) return false;
   if (s.causal && j0 > q.pmax && j0 >= s.prefix) return false;
+  if (s.window && j0 + kTile <= sees_from(s, q.pmin) && j0 >= s.stay) return false;
   return !s.doc || (k.dmin <= q.dmax && q.dmin <= k.dmax);
 }
 __device__ __forceinline__ bool all_seen(const Sight& s, const Span& q, const TileInfo& k, int j0) {
   if (j0 + kTile > s.n || (s.positional && q.pmin < 0)) return false;
   if (s.causal && j0 + kTile - 1 > q.pmin && j0 + kTile > s.prefix) return false;
+  if (s.window && j0 < sees_from(s, q.pmax) && j0 + kTile > s.stay) return false;
   return !s.doc || (k.same && q.same && k.dmin == q.dmin);
 }
 
@@ -408,21 +424,21 @@ __device__ __forceinline__ TileInfo side_info(const float* side, int x) {
   auto u = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
   return {__int_as_float(u(p[0])), __int_as_float(u(p[1])), u(p[2]), u(p[3]), u(p[4]), u(p[5]), u(p[6]), 0};
 }
-// Does a query with these bounds see key z of the tile at j0. Without branches: with the document read behind the other
+// Does a query with these bounds see key z of the tile at j0 (below: and from `from` on, or one that stays). Without branches: with the document read behind the other
 // conditions, `if (!seen) x[q] = 0` comes out of the compiler wrong (right in its IR; in the machine code the block for keys of
 // other documents is empty, their 0 written before a copy of the whole vector undoes it), and hidden keys keep their values.
-__device__ __forceinline__ bool key_seen(const Sight& s, const float* side, int j0, int z, int below, int doc) {
+__device__ __forceinline__ bool key_seen(const Sight& s, const float* side, int j0, int z, int below, int from, int doc) {
   const int id = __float_as_int(side[KS_DOC * kTile + z]);
-  return (j0 + z < below) & (!s.doc | ((doc >= 0) & (id == doc)));
+  return (j0 + z < below) & ((j0 + z >= from) | (j0 + z < s.stay)) & (!s.doc | ((doc >= 0) & (id == doc)));
 }
-// First and one past the last of the tiles [t0, t1) whose documents meet [lo, hi] (all of them without documents); odd: one
-// of those is, or the block's own rows are (`own`, of each lane). By the whole block.
+// First and one past the last of the tiles [t0, t1), but for those of the gap, whose documents meet [lo, hi] (all of them without
+// documents); odd: one of those is, or the block's own rows are (`own`, of each lane). By the whole block.
 struct Range {
   int t0, t1;
   bool odd;
 };
 __device__ __forceinline__ Range tile_range(const Sight& s, int t0, int t1, const TileInfo* docs, const TileInfo* x, const TileInfo* y,
-                                            int dmin, int dmax, bool own, int (&buf)[5]) {
+                                            int dmin, int dmax, bool own, int (&buf)[5], Gap gap = {0, 0}) {
   const int tid = threadIdx.x;
   if (tid < 5) buf[tid] = tid == 0 || tid == 2 ? INT32_MAX : tid == 4 ? 0 : INT32_MIN;
   __syncthreads();
@@ -435,6 +451,7 @@ __device__ __forceinline__ Range tile_range(const Sight& s, int t0, int t1, cons
   const int lo = buf[0], hi = buf[1];
   int first = INT32_MAX, end = INT32_MIN, odd = 0;
   for (int t = t0 + tid; t < t1; t += 256) {
+    if (t >= gap.g0 && t < gap.g1) continue;
     if (s.doc && !(docs[t].dmin <= hi && lo <= docs[t].dmax)) continue;
     first = min(first, t);
     end = max(end, t + 1);
@@ -452,6 +469,26 @@ __device__ __forceinline__ Range tile_range(const Sight& s, int t0, int t1, cons
   r.odd = __builtin_amdgcn_readfirstlane(buf[4]) != 0;
   if (r.t0 >= r.t1) r.t0 = r.t1 = 0;
   return r;
+}
+
+// A walk over the tiles [t0, t1) but for a gap: part `split` of `splits`. The gap comes out within [t0, t1].
+struct Walk {
+  int t0, t1, g0, g1;
+  __device__ __forceinline__ int after(int t) const { return t + 1 == g0 ? g1 : t + 1; }
+};
+__device__ __forceinline__ Walk walk_part(int t0, int t1, Gap gap, int split, int splits) {
+  int g0 = min(max(gap.g0, t0), t1), g1 = min(max(gap.g1, g0), t1);
+  if (g0 == t0) t0 = g1;
+  if (t0 >= g0) g0 = g1 = t0;      // no gap inside
+  if (splits > 1) {
+    const int skip = g1 - g0, n = t1 - t0 - skip, each = (n + splits - 1) / splits;
+    const int u0 = min(split * each, n), u1 = min(u0 + each, n), start = t0;
+    auto at = [&](int u) { return start + u + (start + u >= g0 ? skip : 0); };
+    t0 = at(u0);
+    t1 = u1 > u0 ? at(u1 - 1) + 1 : t0;
+    if (!(t0 < g0 && g1 < t1)) g0 = g1 = t0;
+  }
+  return {t0, t1, g0, g1};
 }
 
 // ---- plain f32, for blocks that walk an odd tile: a wavefront takes one row at a time, a lane a pair ----

@@ -30,7 +30,9 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
   const int tid = threadIdx.x, row = tid / 8, sub = tid % 8, r = tile * kTile + row;
   const int i = r / j.G, g = r - i * j.G, pos = j.query ? s.first + i : r;
   const int id = r < j.rows ? doc_at(s, pos) : -1;
-  const bool in = r < j.rows && (!s.doc || id >= 0) && (j.query ? !s.positional || pos >= 0 : pos < s.n);
+  const Gap gap = j.query ? Gap{0, 0} : gap_before(s, max(s.first, 0));   // keys that no query sees
+  const bool skipped = tile >= gap.g0 && tile < gap.g1;
+  const bool in = !skipped && r < j.rows && (!s.doc || id >= 0) && (j.query ? !s.positional || pos >= 0 : pos < s.n);
   const int64_t at = b * j.x.b + (int64_t)(hk * j.G + g) * j.x.h + (int64_t)i * j.x.t;
   const bool dots = j.ids && j.query;
   const int64_t stat = 2 * (((int64_t)b * p.a.H + hk * j.G + g) * p.a.Tq + i);
@@ -110,7 +112,7 @@ __global__ __launch_bounds__(256) void pack_tiles(Packs p) {
     own[l] = pow2(mye);
     side[j.rel * kTile + l] = pow2(e - mye);
   }
-  if (bad) return;
+  if (bad || skipped) return;
   __syncthreads();
   const int g4 = lane >> 4, l16 = lane & 15;
   const float part = j.score ? score_parts(p.a).part : 1.0f;
@@ -178,10 +180,10 @@ __device__ __forceinline__ void plain_rows(const TilesArgs& A, const Sight& s, i
   const float* v = a.v.p + b * a.v.b + hk * a.v.h;
 #pragma unroll 1
   for (int r = row0; r < min(row0 + 16, A.M); ++r) {
-    const int i = r / G, head = hk * G + r % G, p = s.first + i, doc = doc_at(s, p), end = min(j1, sees_below(s, p));
+    const int i = r / G, head = hk * G + r % G, p = s.first + i, doc = doc_at(s, p), end = min(j1, sees_below(s, p)), from = sees_from(s, p);
     const float* q = a.q.p + b * a.q.b + head * a.q.h + (int64_t)i * a.q.t;
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
-    auto shown = [&](int j) { return j < end && (!s.doc || (doc >= 0 && s.doc[j] == doc)); };
+    auto shown = [&](int j) { return j < end && (j >= from || j < s.stay) && (!s.doc || (doc >= 0 && s.doc[j] == doc)); };
     auto score = [&](int j) { return plain_score(a, plain_dot(k + j * a.k.t, q, a.D), slope, p - j).score; };
     float m = kNone;
 #pragma unroll 1
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   const int row0 = blk * 128 + w * 16, r = row0 + l;
   const bool valid = r < A.M;
   const int i = (int)fastdiv((uint32_t)min(r, A.M - 1), A.group), g = min(r, A.M - 1) - i * G, head = hk * G + g;
-  const int p = s.first + i, doc = doc_at(s, p), below = sees_below(s, p);
+  const int p = s.first + i, doc = doc_at(s, p), below = sees_below(s, p), from = sees_from(s, p);
 
   // the wavefront's rows, and the block's key tiles
   Span me;
@@ -258,15 +260,12 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   int t0 = 0, t1 = s.n;
   if (s.causal) t1 = min(t1, max(last + 1, s.prefix));
   if (s.positional && last < 0) t1 = 0;
+  const Gap gap = gap_before(s, max(s.first + (int)fastdiv((uint32_t)(blk * 128), A.group), 0));
   const Range range_ = tile_range(s, 0, (t1 + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax,
-                                  infinite && sees_any(s, below, doc), range);
-  t0 = range_.t0;
-  t1 = range_.t1;
-  if (A.splits > 1) {
-    const int n = t1 - t0, each = (n + A.splits - 1) / A.splits;
-    t0 = min(t0 + split * each, t1);
-    t1 = min(t0 + each, t1);
-  }
+                                  infinite && sees_any(s, below, doc), range, gap);
+  const Walk walk = walk_part(range_.t0, range_.t1, gap, split, A.splits);
+  t0 = walk.t0;
+  t1 = walk.t1;
   if (__builtin_expect(range_.odd, 0)) {
     plain_rows(A, s, split, slab, b, hk, row0, t0 * kTile, t1 * kTile);
     return;
@@ -278,14 +277,14 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   const char* kf = (const char*)(A.kf + tile0 * (F * kFrag)) + w * 1024;
   const char* vf = (const char*)(A.vf + tile0 * (F * kFrag)) + w * 1024;
   const char* side_p = (const char*)(A.side + tile0 * (kSide * kTile)) + w * 1024;
-  auto fetch = [&](int buf) {      // the next tile
+  auto fetch = [&](int buf, int step) {   // the tile `step` ahead of the last
     const uint32_t to = base + buf * (NF * 1024);
+    kf += (int64_t)step * (F * 1024);
+    vf += (int64_t)step * (F * 1024);
+    side_p += (int64_t)step * (kSide * kTile * 4);
     frags_to_lds<F>(kf, to, lane16, w);
     frags_to_lds<F>(vf, to + F_V * 1024, lane16, w);
     frags_to_lds<kSideFrags>(side_p, to + F_SIDE * 1024, lane16, w);
-    kf += F * 1024;
-    vf += F * 1024;
-    side_p += kSide * kTile * 4;
   };
 
   f32x4 acc[2 * N];
@@ -293,12 +292,13 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   for (int d = 0; d < 2 * N; ++d) acc[d] = f32x4{};
   float m = kNone, sum = 0;        // running maximum (log2) and this lane's part of the sum
   int ce = kUnset;                 // acc is in units of 2^-ce
-  if (t0 < t1) fetch(0);
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1, j0 = t * kTile;
+  if (t0 < t1) fetch(0, 0);
+  for (int t = t0, next, buf = 0; t < t1; t = next, buf ^= 1) {
+    const int j0 = t * kTile;
+    next = walk.after(t);
     loads_done();
     __syncthreads();
-    if (t + 1 < t1) fetch(buf ^ 1);
+    if (next < t1) fetch(buf ^ 1, next - t);
     const _Float16* L = lds + buf * (NF * kFrag);
     const float* side = (const float*)(L + F_SIDE * kFrag);
     const TileInfo kt = side_info(side, 0), vt = side_info(side, 1);
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
     }
     if (__builtin_expect(!all_seen(s, me, kt, j0), 0)) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) x[q] = key_seen(s, side, j0, 16 * (q / 4) + 4 * g4 + q % 4, below, doc) ? x[q] : kNone;
+      for (int q = 0; q < 8; ++q) x[q] = key_seen(s, side, j0, 16 * (q / 4) + 4 * g4 + q % 4, below, from, doc) ? x[q] : kNone;
     }
     float top = x[0];
 #pragma unroll
@@ -412,28 +412,32 @@ __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
   int n = s.n;
   if (s.causal) n = min(n, max(pmax + 1, s.prefix));
   if (s.positional && pmax < 0) n = 0;
+  // keys that some row sees, counted through: the first `head`, then those from head + skip on
+  const int head = s.window ? min(max(s.stay, 0), n) : n, skip = s.window ? max(min(max(sees_from(s, max(pmin, 0)), 0), n) - head, 0) : 0;
+  n -= skip;
   const int begin = min((int64_t)split * A.each, (int64_t)n), end = min((int64_t)begin + A.each, (int64_t)n);
+  auto key = [&](int i) { return i < head ? i : i + skip; };
   const float* k = a.k.p + b * a.k.b + hk * a.k.h;
   const float* v = a.v.p + b * a.v.b + hk * a.v.h;
   float kn[E], vn[E];
   bool on = begin + grp < end;
   if (on) {
-    load(k + (begin + grp) * a.k.t, a.D, kn);
-    load(v + (begin + grp) * a.v.t, a.Dv, vn);
+    load(k + key(begin + grp) * a.k.t, a.D, kn);
+    load(v + key(begin + grp) * a.v.t, a.Dv, vn);
   }
   for (int j0 = begin; j0 < end; j0 += 32) {
-    const int j = j0 + grp;
+    const int j = key(j0 + grp);
     float kx[E], vx[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) { kx[e] = kn[e]; vx[e] = vn[e]; }
     const bool here = on;
-    on = j + 32 < end;
+    on = j0 + grp + 32 < end;
     if (on) {                      // the next rows travel while these are multiplied
-      load(k + (j + 32) * a.k.t, a.D, kn);
-      load(v + (j + 32) * a.v.t, a.Dv, vn);
+      load(k + key(j0 + grp + 32) * a.k.t, a.D, kn);
+      load(v + key(j0 + grp + 32) * a.v.t, a.Dv, vn);
     }
     if (!here) continue;
-    const bool all = !s.doc && (!s.causal || j <= pmin) && !(s.positional && pmin < 0);
+    const bool all = !s.doc && (!s.causal || j <= pmin) && !(s.positional && pmin < 0) && (!s.window || j >= sees_from(s, pmax));
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float x = 0;
@@ -446,7 +450,7 @@ __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
       if (a.cap > 0) x = a.cap * tanh_of(x / a.cap);
       if (a.slopes) x -= a.slopes[hk * G + min(r, A.M - 1) % G] * fabsf((float)(p[r] - j));
       x = rounded_mul(x, kLog2e);
-      if (!all && (j >= below[r] || (s.doc && (doc[r] < 0 || s.doc[j] != doc[r])))) continue;
+      if (!all && (j >= below[r] || (j < sees_from(s, p[r]) && j >= s.stay) || (s.doc && (doc[r] < 0 || s.doc[j] != doc[r])))) continue;
       if (x > m[r] + 8) {
         const float top = x < INFINITY ? x : m[r] == kLowest ? 0.0f : m[r];   // an infinite score shows in the weight
         const float keep = __builtin_amdgcn_exp2f(m[r] - top);
@@ -598,6 +602,10 @@ inline int64_t take(int64_t& at, int64_t bytes) {
 // Rows that attend_few keeps in registers: 16 E floats a lane of queries and results.
 inline int few_rows(int DP) { return DP <= 32 ? 16 : DP <= 64 ? 8 : 4; }
 
+// Keys that `span` neighbouring positions see at most: with a window, it and what stays.
+inline int64_t seen_keys(const AttendDesc& a, int64_t span) {
+  return a.window && !a.prefix ? std::min<int64_t>(a.Tk, (int64_t)a.window + a.sinks + span) : a.Tk;
+}
 Plan plan(const AttendDesc& a) {
   Plan p{};
   p.DP = attend_dp(a);
@@ -608,13 +616,13 @@ Plan plan(const AttendDesc& a) {
   p.few = !a.stats && p.M <= few_rows(p.DP) && (p.M <= 2 || a.Tk >= 32 * p.M);
   if (p.few) {
     p.blocks = 1;
-    const int64_t want = std::max<int64_t>(1, kMostParts / p.slabs);
-    p.each = (int)std::max<int64_t>(128, ((a.Tk + want - 1) / want + 31) / 32 * 32);
-    p.splits = std::max(1, (a.Tk - 1) / p.each + 1);
+    const int64_t want = std::max<int64_t>(1, kMostParts / p.slabs), keys = seen_keys(a, a.Tq);
+    p.each = (int)std::max<int64_t>(128, ((keys + want - 1) / want + 31) / 32 * 32);
+    p.splits = (int)std::max<int64_t>(1, (keys - 1) / p.each + 1);
   } else {
     p.blocks = (p.M + 127) / 128;
-    const int64_t have = (int64_t)p.slabs * p.blocks;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kMostParts / have, p.tiles / 8));
+    const int64_t have = (int64_t)p.slabs * p.blocks, walked = seen_keys(a, 127 / p.G + 1) / kTile + 1;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kMostParts / have, std::min<int64_t>(p.tiles, walked) / 8));
   }
   int64_t at = 0;
   if (!p.few) {

@@ -33,6 +33,10 @@ __device__ __forceinline__ void seeing_tiles(const GradArgs& A, const Sight& s, 
   if (s.positional) i0 = max(i0, (int64_t)-s.first);
   from = (int)min(max(i0, (int64_t)0) * A.group.d / kTile, (int64_t)A.qtiles);
   to = k0 < s.n ? A.qtiles : 0;
+  if (s.window && k0 >= s.stay) {  // the last of the keys leaves the window
+    const int64_t i1 = (int64_t)k0 + 127 + s.window - s.first;
+    to = (int)min((int64_t)to, (max(i1, (int64_t)0) * A.group.d + kTile - 1) / kTile);
+  }
 }
 // Those of part `split`, equal stretches of all rows, so that blocks that run together walk the same ones. False: none, which
 // the join finds again and does not read. With documents the stretch that a key block's own see is short: there its tiles are
@@ -87,7 +91,7 @@ __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, in
       float p = 0, ds = 0;
       if (r < r1) {
         const float* side = A.qside + ((int64_t)slab * A.qtiles + r / kTile) * (kSide * kTile) + r % kTile;
-        if (j < __float_as_int(side[QS_BELOW * kTile]) && (!s.doc || (doc >= 0 && __float_as_int(side[QS_DOC * kTile]) == doc))) {
+        if (j < __float_as_int(side[QS_BELOW * kTile]) && (j >= sees_from(s, __float_as_int(side[QS_POS * kTile])) || j < s.stay) && (!s.doc || (doc >= 0 && __float_as_int(side[QS_DOC * kTile]) == doc))) {
           const PlainPair z = plain_score(a, plain_dot(row(a.q, r), k, a.D), side[QS_SLOPE * kTile], __float_as_int(side[QS_POS * kTile]) - j);
           const float share = side[QS_SHARE * kTile], w = __builtin_amdgcn_exp2f(z.score - side[QS_TOP * kTile]);
           p = w * share;
@@ -240,9 +244,10 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
       }
       if (__builtin_expect(!all, 0)) {
         const f32x4 below = *(const f32x4*)(side + QS_BELOW * kTile + at), rdoc = *(const f32x4*)(side + QS_DOC * kTile + at);
+        const f32x4 pos = *(const f32x4*)(side + QS_POS * kTile + at);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool ok = (j < __float_as_int(below[e])) & (!s.doc | ((doc >= 0) & (__float_as_int(rdoc[e]) == doc)));
+          const bool ok = (j < __float_as_int(below[e])) & ((j >= sees_from(s, __float_as_int(pos[e]))) | (j < s.stay)) & (!s.doc | ((doc >= 0) & (__float_as_int(rdoc[e]) == doc)));
           x[4 * q4 + e] = ok ? x[4 * q4 + e] : 0.0f;
           y[4 * q4 + e] = ok ? y[4 * q4 + e] : 0.0f;
         }
@@ -344,13 +349,13 @@ __device__ __forceinline__ void plain_dq(const GradArgs& A, const Sight& s, int 
     const float* dy = A.g.dy.p + b * A.g.dy.b + head * A.g.dy.h + (int64_t)i * A.g.dy.t;
     const float* side = A.qside + ((int64_t)slab * A.qtiles + r / kTile) * (kSide * kTile) + r % kTile;
     const int p = __float_as_int(side[QS_POS * kTile]), doc = __float_as_int(side[QS_DOC * kTile]);
-    const int end = min(j1, __float_as_int(side[QS_BELOW * kTile]));
+    const int end = min(j1, __float_as_int(side[QS_BELOW * kTile])), from = sees_from(s, p);
     float dq[2] = {0, 0};
 #pragma unroll 1
     for (int c = j0; c < end; c += 64) {
       const int j = c + lane;
       float ds = 0;
-      if (j < end && (!s.doc || (doc >= 0 && s.doc[j] == doc))) {
+      if (j < end && (j >= from || j < s.stay) && (!s.doc || (doc >= 0 && s.doc[j] == doc))) {
         const PlainPair z = plain_score(a, plain_dot(k + j * a.k.t, q, a.D), side[QS_SLOPE * kTile], p - j);
         ds = __builtin_amdgcn_exp2f(z.score - side[QS_TOP * kTile]) *
              fmaf(plain_dot(v + j * a.v.t, dy, a.Dv), side[QS_SHARE * kTile], -side[QS_DOT * kTile]) * z.slack;
@@ -382,7 +387,7 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   const int row0 = blk * 128 + w * 16, r = row0 + l, rr = min(r, A.M - 1);
   const bool valid = r < A.M;
   const int i = (int)fastdiv((uint32_t)rr, A.group), g = rr - i * G, head = hk * G + g;
-  const int p = s.first + i, doc = doc_at(s, p), below = sees_below(s, p);
+  const int p = s.first + i, doc = doc_at(s, p), below = sees_below(s, p), from = sees_from(s, p);
   const int qt = min(row0 / kTile, A.qtiles - 1), rt = row0 / kTile * kTile;   // masks are judged by whole tiles of rows
   const float* mine = A.qside + ((int64_t)slab * A.qtiles + qt) * (kSide * kTile) + row0 % kTile + l;
   const float top = mine[QS_TOP * kTile], share = mine[QS_SHARE * kTile], dot = mine[QS_DOT * kTile];
@@ -401,13 +406,10 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   int end = s.n;
   if (s.causal) end = min(end, max(last + 1, s.prefix));
   if (s.positional && last < 0) end = 0;
-  const Range range_ = tile_range(s, 0, (end + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax, own, range);
-  int t0 = range_.t0, t1 = range_.t1;
-  if (A.qsplits > 1) {
-    const int each = (t1 - t0 + A.qsplits - 1) / A.qsplits;
-    t0 = min(t0 + split * each, t1);
-    t1 = min(t0 + each, t1);
-  }
+  const Gap gap = gap_before(s, max(s.first + (int)fastdiv((uint32_t)(blk * 128), A.group), 0));
+  const Range range_ = tile_range(s, 0, (end + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax, own, range, gap);
+  const Walk walk = walk_part(range_.t0, range_.t1, gap, split, A.qsplits);
+  const int t0 = walk.t0, t1 = walk.t1;
   if (__builtin_expect(range_.odd, 0)) {
     plain_dq(A, s, split, slab, b, hk, row0, t0 * kTile, t1 * kTile);
     return;
@@ -424,16 +426,16 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   const char* vr = (const char*)(A.vr + tile0 * (F * kFrag)) + w * 1024;
   const char* kc = (const char*)(A.kc + tile0 * (F * kFrag)) + w * 1024;
   const char* side_p = (const char*)(A.kside + tile0 * (kSide * kTile)) + w * 1024;
-  auto fetch = [&](int buf) {      // the next tile
+  auto fetch = [&](int buf, int step) {   // the tile `step` ahead of the last
     const uint32_t to = base + buf * (NF * 1024);
+    kr += (int64_t)step * (F * 1024);
+    vr += (int64_t)step * (F * 1024);
+    kc += (int64_t)step * (F * 1024);
+    side_p += (int64_t)step * (kSide * kTile * 4);
     frags_to_lds<F>(kr, to, lane16, w);
     frags_to_lds<F>(vr, to + F_V * 1024, lane16, w);
     frags_to_lds<F>(kc, to + F_KC * 1024, lane16, w);
     frags_to_lds<kSideFrags>(side_p, to + F_SIDE * 1024, lane16, w);
-    kr += F * 1024;
-    vr += F * 1024;
-    kc += F * 1024;
-    side_p += kSide * kTile * 4;
   };
 
   f32x4 dq[2 * N];
@@ -441,12 +443,13 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   for (int d = 0; d < 2 * N; ++d) dq[d] = f32x4{};
   int cq = kUnset;
   const bool cap = RICH && a.cap > 0;
-  if (t0 < t1) fetch(0);
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1, j0 = t * kTile;
+  if (t0 < t1) fetch(0, 0);
+  for (int t = t0, next, buf = 0; t < t1; t = next, buf ^= 1) {
+    const int j0 = t * kTile;
+    next = walk.after(t);
     loads_done();
     __syncthreads();
-    if (t + 1 < t1) fetch(buf ^ 1);
+    if (next < t1) fetch(buf ^ 1, next - t);
     const _Float16* L = lds + buf * (NF * kFrag);
     const float* side = (const float*)(L + F_SIDE * kFrag);
     const TileInfo kt = side_info(side, 0), vt = side_info(side, 1);
@@ -477,7 +480,7 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
     }
     if (__builtin_expect(!all_seen(s, me, kt, j0), 0)) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) y[q] = key_seen(s, side, j0, 16 * (q / 4) + 4 * g4 + q % 4, below, doc) ? y[q] : 0.0f;
+      for (int q = 0; q < 8; ++q) y[q] = key_seen(s, side, j0, 16 * (q / 4) + 4 * g4 + q % 4, below, from, doc) ? y[q] : 0.0f;
     }
     if (__builtin_expect(kt.uneven, 0)) per_row(y, side + KS_RELK * kTile, g4);
     float change = 1;

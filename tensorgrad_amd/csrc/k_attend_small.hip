@@ -63,7 +63,7 @@ __device__ __forceinline__ void product(float (&o)[A][B], int n, FA fa, FB fb) {
 
 // Row r of a slab: its query index, head, position, and what it sees.
 struct Row {
-  int i, head, p, doc, below;
+  int i, head, p, doc, below, from;
 };
 __device__ __forceinline__ Row row_at(const AttendDesc& a, const Sight& s, int hk, int G, int r) {
   Row x;
@@ -72,10 +72,11 @@ __device__ __forceinline__ Row row_at(const AttendDesc& a, const Sight& s, int h
   x.p = s.first + x.i;
   x.doc = doc_at(s, x.p);
   x.below = sees_below(s, x.p);
+  x.from = sees_from(s, x.p);
   return x;
 }
 __device__ __forceinline__ bool sees(const Sight& s, const Row& x, int j) {
-  return j < x.below && (!s.doc || (x.doc >= 0 && s.doc[j] == x.doc));
+  return j < x.below && (j >= x.from || j < s.stay) && (!s.doc || (x.doc >= 0 && s.doc[j] == x.doc));
 }
 __device__ __forceinline__ float* at(const Rows& x, int b, int head, int t) { return x.p + b * x.b + head * x.h + (int64_t)t * x.t; }
 

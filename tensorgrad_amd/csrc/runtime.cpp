@@ -540,6 +540,11 @@ class Runtime {
   void lower_rope(int i);
   void lower_scan(int i);
   void lower_scan_grad(int i);
+  tgk::LinearDesc linear_fields(int i, Node& n) const;
+  std::function<tgk::LinearDesc()> linear_binder(int i, const tgk::LinearDesc& d);
+  void lower_linear(int i);
+  void lower_linear_grad(int i);
+  void lower_sample(int i);
 
   // GEMMs whose results only the fused optimizer reads (weight gradients) and that would
   // split K run together just before it: one grouped launch per operand-layout kind, with
@@ -764,6 +769,13 @@ static std::vector<int> op_inputs(const tgj::Value& op) {
       {"rope_axes", {"a", "positions"}}, {"linear_recurrence", {"a", "x", "h0"}},
       {"linear_recurrence_grad_a", {"a", "h", "dh", "h0"}}, {"linear_recurrence_grad_x", {"a", "h", "dh", "h0"}},
       {"linear_recurrence_grad_h0", {"a", "h", "dh", "h0"}},
+      {"linear_attention", {"q", "k", "v", "state", "documents", "lengths"}},
+      {"linear_attention_state", {"q", "k", "v", "state", "documents", "lengths"}},
+      {"linear_attention_grad_q", {"q", "k", "v", "state", "documents", "lengths", "dy", "dstate"}},
+      {"linear_attention_grad_k", {"q", "k", "v", "state", "documents", "lengths", "dy", "dstate"}},
+      {"linear_attention_grad_v", {"q", "k", "v", "state", "documents", "lengths", "dy", "dstate"}},
+      {"linear_attention_grad_state", {"q", "k", "v", "state", "documents", "lengths", "dy", "dstate"}},
+      {"sample", {"logits", "u", "temperature", "topK", "topP", "minP"}},
       {"param_input", {}}, {"tensor_input", {}}, {"state_input", {}}, {"arange", {}},
       {"const_scalar", {}}, {"const_fill", {}},
   };
@@ -962,6 +974,9 @@ void Runtime::compute_views() {
         continue;   // strided element-wise kernels
       if ((k.compare(0, 9, "attention") == 0 || k == "rope_axes") && v.dims.size() == 4 && v.strides[3] == 1)
         continue;   // [B, heads, T, D] rows through strides
+      if (k.compare(0, 16, "linear_attention") == 0 && v.dims.size() == 4 && v.strides[3] == 1 && opt_fld(c, "state") != t &&
+          (k.compare(0, 21, "linear_attention_grad") != 0 || opt_fld(c, "dstate") != t))
+        continue;
       return true;
     }
     for (int o : outputs_) if (o == t) return true;
@@ -3722,7 +3737,11 @@ static bool same_value(const tgj::Value& x, const tgj::Value& y) {
 }
 
 bool Runtime::same_fields(int i, int j, std::initializer_list<const char*> names) const {
-  for (const char* f : names) if (!same_value(O(i).at(f), O(j).at(f))) return false;
+  static const tgj::Value none;
+  for (const char* f : names) {
+    const tgj::Value *x = O(i).get(f), *y = O(j).get(f);
+    if (!same_value(x ? *x : none, y ? *y : none)) return false;
+  }
   return true;
 }
 
@@ -3767,6 +3786,19 @@ void Runtime::mask_fields(int i, Node& n, tgk::AttendDesc& a) const {
   expect(op.at("slopes").null() || (int64_t)op.at("slopes").items.size() == a.H, i, "one slope per query head");
   if (!op.at("slopes").null())
     for (const auto& x : op.at("slopes").items) expect(std::fabs(x.num()) <= 0x1p60, i, "slopes must be finite, of 2^60 at most");
+  auto count = [&](const char* f) -> int {     // absent or null: 0
+    const tgj::Value* x = op.get(f);
+    if (!x || x->null()) return 0;
+    expect(x->num() >= 0 && x->num() < 0x1p31 && x->num() == std::floor(x->num()), i, "window and sinks must be whole numbers");
+    return (int)x->num();
+  };
+  a.window = count("window");
+  a.sinks = count("sinks");
+  const tgj::Value* window = op.get("window");
+  expect(!window || window->null() || (a.window > 0 && a.causal), i, "a window has 1 position at least and needs a causal mask");
+  expect(a.sinks == 0 || (a.window > 0 && doc < 0), i, "sinks need a window and no documents");
+  if (a.window >= a.Tk) a.window = 0;          // every query sees all keys before it
+  a.sinks = std::min(a.sinks, a.Tk);
   const std::pair<int, Dims> masks[] = {{doc, {a.B, a.Tk}}, {pre, {a.B}}, {len, {a.B}}};
   for (const auto& m : masks)
     if (m.first >= 0) {
@@ -3797,7 +3829,7 @@ std::function<tgk::AttendDesc()> Runtime::attend_binder(int i, const tgk::Attend
   };
 }
 
-#define TG_MASKED "q", "k", "v", "documents", "prefix", "lengths", "causal", "scale", "softcap", "slopes"
+#define TG_MASKED "q", "k", "v", "documents", "prefix", "lengths", "causal", "scale", "softcap", "slopes", "window", "sinks"
 
 // attention and attention_stats of the same inputs: one node, whichever comes first in the graph.
 void Runtime::lower_attend(int i) {
@@ -4036,6 +4068,222 @@ void Runtime::lower_scan_grad(int i) {
     tgk::ScanGradDesc d{s[0], s[1], s[2], in(a), in(h), in(dh), in(h0), to(da), to(dx), to(dh0)};
     void* w = cur_ws_;
     return [=](hipStream_t st) { tgk::scan_grad(d, w, st); };
+  };
+  add_node(std::move(n));
+}
+
+// Shapes, masks and constants of a linear attention, checked; reads q, k, v, the state and the masks.
+tgk::LinearDesc Runtime::linear_fields(int i, Node& n) const {
+  const tgj::Value& op = O(i);
+  const int q = fld(i, "q"), k = fld(i, "k"), v = fld(i, "v"), s = opt_fld(i, "state");
+  for (int t : {q, k, v}) {
+    expect(T_[t].dt == F32 && T_[t].shape.size() == 4 && T_[t].numel > 0, i, "q, k and v must be f32 of rank 4");
+    n.reads.push_back(root(t));
+  }
+  const Dims &qs = T_[q].shape, &ks = T_[k].shape, &vs = T_[v].shape;
+  expect(ks[0] == qs[0] && vs[0] == qs[0] && ks[2] == qs[2] && vs[2] == qs[2] && ks[3] == qs[3] && ks[1] == vs[1] && qs[1] % ks[1] == 0, i,
+         "q, k and v do not fit each other");
+  expect(qs[3] <= tgk::kLinearMaxHead && vs[3] <= tgk::kLinearMaxHead, i, "head size above 128");
+  // a launch has fewer than 2^32 threads, 256 of them for 32 positions of a head, and for 256 values of a state
+  expect(qs[2] < (int64_t(1) << 30) && qs[0] * qs[1] * std::max((qs[2] + 31) / 32, (qs[3] * vs[3] + 255) / 256) < (int64_t(1) << 24), i,
+         "too many rows");
+  tgk::LinearDesc a{};
+  a.B = (int)qs[0]; a.H = (int)qs[1]; a.T = (int)qs[2]; a.D = (int)qs[3];
+  a.Hk = (int)ks[1]; a.Dv = (int)vs[3];
+  const double scale = op.at("scale").num();
+  expect(scale >= 0x1p-60 && scale <= 0x1p60, i, "scale must be positive, between 2^-60 and 2^60");
+  a.scale = (float)scale;
+  expect((int64_t)op.at("decay").items.size() == a.H, i, "one decay per query head");
+  for (const auto& x : op.at("decay").items) expect(x.num() > 0 && x.num() <= 1, i, "decay must be above 0, 1 at most");
+  const Dims ss = {a.B, a.H, a.D, a.Dv};
+  const std::pair<int, Dims> masks[] = {{opt_fld(i, "documents"), {a.B, a.T}}, {opt_fld(i, "lengths"), {a.B}}};
+  for (const auto& m : masks)
+    if (m.first >= 0) {
+      expect(T_[m.first].dt == I32 && T_[m.first].shape == m.second && view_[m.first].contiguous(), i,
+             "documents must be i32 [B, T], lengths i32 [B]");
+      n.reads.push_back(root(m.first));
+    }
+  if (s >= 0) {
+    expect(T_[s].dt == F32 && T_[s].shape == ss && view_[s].contiguous(), i, "state must be f32 [B, H, D, Dv]");
+    n.reads.push_back(root(s));
+  }
+  return a;
+}
+
+// The descriptor with the addresses of the moment it is called (at bind).
+std::function<tgk::LinearDesc()> Runtime::linear_binder(int i, const tgk::LinearDesc& d) {
+  const int q = fld(i, "q"), k = fld(i, "k"), v = fld(i, "v"), s = opt_fld(i, "state");
+  const int doc = opt_fld(i, "documents"), len = opt_fld(i, "lengths");
+  std::vector<float> rate;
+  for (const auto& x : O(i).at("decay").items) rate.push_back((float)std::log2(x.num()));
+  return [=]() {
+    tgk::LinearDesc a = d;
+    a.q = rows_of(q, "linear attention q");
+    a.k = rows_of(k, "linear attention k");
+    a.v = rows_of(v, "linear attention v");
+    a.state = s >= 0 ? (const float*)dptr(s) : nullptr;
+    a.documents = doc >= 0 ? (const int32_t*)dptr(doc) : nullptr;
+    a.lengths = len >= 0 ? (const int32_t*)dptr(len) : nullptr;
+    if (!plan_only_) a.rate = (const float*)dev_table("decay " + std::to_string(i), rate.data(), rate.size() * sizeof(float));
+    return a;
+  };
+}
+
+#define TG_LINEAR "q", "k", "v", "state", "documents", "lengths", "decay", "scale"
+
+// The results and the last state of one linear attention: one node, whichever comes first in the graph.
+void Runtime::lower_linear(int i) {
+  Node n;
+  n.kind = "linear";
+  n.op = i;
+  n.direct = true;
+  tgk::LinearDesc d = linear_fields(i, n);
+  int y = -1, last = -1;
+  for (int j = i; j < (int)ops_.size(); ++j) {
+    if (kinds_[j] != "linear_attention" && kinds_[j] != "linear_attention_state") continue;
+    int& out = kinds_[j] == "linear_attention" ? y : last;
+    if (out >= 0 || gemm_done_[j] || (j != i && !same_fields(i, j, {TG_LINEAR}))) continue;
+    out = O(j).at("out").i32();
+    gemm_done_[j] = 1;
+    n.writes.push_back(root(out));
+    n.detail += (n.detail.empty() ? "" : ",") + kinds_[j];
+  }
+  expect(y < 0 || (T_[y].shape == Dims({d.B, d.H, d.T, d.Dv}) && T_[y].dt == F32), i, "bad output shape");
+  expect(last < 0 || (T_[last].shape == Dims({d.B, d.H, d.D, d.Dv}) && T_[last].dt == F32 && view_[last].contiguous()), i, "bad state shape");
+  n.shape = shape_str(T_[fld(i, "q")].shape) + "x" + shape_str(T_[fld(i, "v")].shape);
+  n.flops = 4.0 * d.B * d.H * (double)d.T * d.D * d.Dv;
+  n.bytes = 4.0 * (T_[fld(i, "q")].numel + T_[fld(i, "k")].numel + T_[fld(i, "v")].numel + (y >= 0 ? T_[y].numel : 0) +
+                   (last >= 0 ? T_[last].numel : 0) + (opt_fld(i, "state") >= 0 ? (double)d.B * d.H * d.D * d.Dv : 0.0));
+  // presence decides the kernels; the addresses follow at bind
+  d.y.p = y >= 0 ? (float*)16 : nullptr;
+  d.last = last >= 0 ? (float*)16 : nullptr;
+  const int64_t ws = tgk::linear_workspace_bytes(d);
+  workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
+  n.ws = ws > 0;
+  auto desc = linear_binder(i, d);
+  n.bind = [=]() -> std::function<void(hipStream_t)> {
+    tgk::LinearDesc a = desc();
+    if (y >= 0) a.y = rows_of(y, "linear attention y");
+    a.last = last >= 0 ? (float*)dptr(last) : nullptr;
+    void* w = cur_ws_;
+    return [=](hipStream_t st) { tgk::linear(a, w, st); };
+  };
+  add_node(std::move(n));
+}
+
+// The gradients of one linear attention: one node for those that the graph has.
+void Runtime::lower_linear_grad(int i) {
+  Node n;
+  n.kind = "linear_grad";
+  n.op = i;
+  n.direct = true;
+  tgk::LinearGradDesc g{};
+  g.a = linear_fields(i, n);
+  const tgk::LinearDesc& d = g.a;
+  const int dy = opt_fld(i, "dy"), ds = opt_fld(i, "dstate");
+  const Dims ys = {d.B, d.H, d.T, d.Dv}, ss = {d.B, d.H, d.D, d.Dv};
+  expect((dy >= 0 || ds >= 0) && (dy < 0 || (T_[dy].shape == ys && T_[dy].dt == F32)) &&
+             (ds < 0 || (T_[ds].shape == ss && T_[ds].dt == F32 && view_[ds].contiguous())), i, "dy or dstate does not fit");
+  for (int t : {dy, ds}) if (t >= 0) n.reads.push_back(root(t));
+  int out[4] = {-1, -1, -1, -1};
+  for (int j = i; j < (int)ops_.size(); ++j) {
+    if (kinds_[j].compare(0, 22, "linear_attention_grad_") != 0 || gemm_done_[j]) continue;
+    if (j != i && !same_fields(i, j, {TG_LINEAR, "dy", "dstate"})) continue;
+    const std::string of = kinds_[j].substr(22);
+    const int which = of == "q" ? 0 : of == "k" ? 1 : of == "v" ? 2 : 3;
+    if (out[which] >= 0) continue;
+    out[which] = O(j).at("out").i32();
+    expect(which < 3 || of == "state", j, "unknown gradient");
+    expect(T_[out[which]].shape == (which == 3 ? ss : T_[fld(j, which == 0 ? "q" : which == 1 ? "k" : "v")].shape) &&
+               T_[out[which]].dt == F32, j, "bad output shape");
+    gemm_done_[j] = 1;
+    n.writes.push_back(root(out[which]));
+    n.detail += (n.detail.empty() ? "" : ",") + kinds_[j];
+  }
+  const int dq = out[0], dk = out[1], dv = out[2], df = out[3];
+  expect(df < 0 || view_[df].contiguous(), i, "bad state shape");
+  n.shape = shape_str(T_[fld(i, "q")].shape) + "x" + shape_str(T_[fld(i, "v")].shape);
+  n.flops = 8.0 * d.B * d.H * (double)d.T * d.D * d.Dv;
+  n.bytes = 4.0 * (2.0 * T_[fld(i, "q")].numel + 2.0 * T_[fld(i, "k")].numel + 2.0 * T_[fld(i, "v")].numel + prod(ys));
+  // presence decides the kernels; the addresses follow at bind
+  g.dy.p = dy >= 0 ? (float*)16 : nullptr;
+  g.dq.p = dq >= 0 ? (float*)16 : nullptr;
+  g.dk.p = dk >= 0 ? (float*)16 : nullptr;
+  g.dv.p = dv >= 0 ? (float*)16 : nullptr;
+  g.dfirst = df >= 0 ? (float*)16 : nullptr;
+  const int64_t ws = tgk::linear_grad_workspace_bytes(g);
+  workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
+  n.ws = ws > 0;
+  auto desc = linear_binder(i, g.a);
+  n.bind = [=]() -> std::function<void(hipStream_t)> {
+    tgk::LinearGradDesc b{};
+    b.a = desc();
+    if (dy >= 0) b.dy = rows_of(dy, "linear attention dy");
+    if (dq >= 0) b.dq = rows_of(dq, "linear attention dq");
+    if (dk >= 0) b.dk = rows_of(dk, "linear attention dk");
+    if (dv >= 0) b.dv = rows_of(dv, "linear attention dv");
+    b.dstate = ds >= 0 ? (const float*)dptr(ds) : nullptr;
+    b.dfirst = df >= 0 ? (float*)dptr(df) : nullptr;
+    void* w = cur_ws_;
+    return [=](hipStream_t st) { tgk::linear_grad(b, w, st); };
+  };
+  add_node(std::move(n));
+}
+
+void Runtime::lower_sample(int i) {
+  const tgj::Value& op = O(i);
+  const int x = fld(i, "logits"), u = fld(i, "u"), out = op.at("out").i32();
+  const Dims& xs = T_[x].shape;
+  expect(T_[x].dt == F32 && !xs.empty() && T_[x].numel > 0 && xs.back() <= tgk::kSampleMaxVocab, i, "logits must be f32 [..., vocabulary]");
+  const Dims rows(xs.begin(), xs.end() - 1);
+  const int64_t n_rows = T_[x].numel / xs.back();
+  expect(T_[u].dt == F32 && T_[u].shape == rows && T_[out].dt == I32 && T_[out].shape == rows, i, "u and the tokens must have the logits' rows");
+  expect(n_rows < (int64_t(1) << 22), i, "too many rows");
+  Node n;
+  n.kind = "sample";
+  n.op = i;
+  n.direct = true;
+  n.shape = shape_str(xs);
+  n.writes.push_back(root(out));
+  const char* names[] = {"temperature", "topK", "topP", "minP"};
+  int limit[4];
+  double value[4];
+  expect(op.at("values").items.size() == 4, i, "four values");
+  for (int l = 0; l < 4; ++l) {
+    limit[l] = opt_fld(i, names[l]);
+    value[l] = op.at("values").items[l].num();
+    expect(limit[l] < 0 || (T_[limit[l]].dt == (l == 1 ? I32 : F32) && T_[limit[l]].shape == rows), i, "a limit has one number for each row");
+  }
+  expect(value[0] >= 0 && value[1] >= 0 && value[1] < 0x1p31 && value[2] > 0 && value[3] >= 0 && value[3] <= 1, i, "limit out of range");
+  for (int t : {x, u, limit[0], limit[1], limit[2], limit[3]}) if (t >= 0) {
+    if (!view_[t].contiguous()) throw Error(TG_INTERNAL, "sample needs contiguous operands");
+    n.reads.push_back(root(t));
+  }
+  n.flops = 3.0 * T_[x].numel;
+  n.bytes = 4.0 * T_[x].numel + 8.0 * n_rows;
+  tgk::SampleDesc d{};
+  d.rows = n_rows;
+  d.V = (int)xs.back();
+  d.temperature1 = value[0];
+  d.top_k1 = (int32_t)value[1];
+  d.top_p1 = value[2];
+  d.min_p1 = value[3];
+  const int64_t ws = tgk::sample_workspace_bytes(d);
+  workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
+  n.ws = ws > 0;
+  const int heat = limit[0], top_k = limit[1], top_p = limit[2], min_p = limit[3];
+  n.bind = [=]() -> std::function<void(hipStream_t)> {
+    tgk::SampleDesc s = d;
+    auto at = [&](int t) { return t >= 0 ? (const float*)dptr(t) : nullptr; };
+    s.logits = at(x);
+    s.u = at(u);
+    s.temperature = at(heat);
+    s.top_k = (const int32_t*)at(top_k);
+    s.top_p = at(top_p);
+    s.min_p = at(min_p);
+    s.token = (int32_t*)dptr(out);
+    void* w = cur_ws_;
+    return [=](hipStream_t st) { tgk::sample(s, w, st); };
   };
   add_node(std::move(n));
 }
@@ -4726,6 +4974,15 @@ void Runtime::lower_op(int i) {
     return;
   } else if (k == "rope_axes") {
     lower_rope(i);
+    return;
+  } else if (k == "linear_attention" || k == "linear_attention_state") {
+    lower_linear(i);
+    return;
+  } else if (k.compare(0, 22, "linear_attention_grad_") == 0) {
+    lower_linear_grad(i);
+    return;
+  } else if (k == "sample") {
+    lower_sample(i);
     return;
   } else if (k == "linear_recurrence") {
     lower_scan(i);

@@ -1,5 +1,5 @@
 // Host-side launch wrappers of the sequence operators: masked attention (k_attend.hip), rotary positions of several axes
-// and the gated linear recurrence (k_sequence.hip). Values are f32, indices i32; strides count elements.
+// and the gated linear recurrence (k_sequence.hip), linear attention (k_linear.hip), and of the choice of a token (k_sample.hip). Values are f32, indices i32; strides count elements.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <cstdint>
@@ -24,6 +24,7 @@ struct AttendDesc {
   const float* slopes;       // [H] or null
   float scale, cap;
   bool causal, positional;   // positional: a query before position 0 sees nothing
+  int window, sinks;         // a causal query sees its last `window` keys (0: all before it) and the first `sinks`
 };
 struct AttendGradDesc {
   AttendDesc a;              // a.y and a.stats: the forward's results, read
@@ -65,5 +66,43 @@ struct ScanGradDesc {
 int64_t scan_workspace_bytes(int64_t B, int64_t T, int64_t C);
 void scan(const ScanDesc& s, void* work, hipStream_t st);
 void scan_grad(const ScanGradDesc& s, void* work, hipStream_t st);
+
+// Linear attention, see ops.py: S[t] = decay S[t-1] + k[t] v[t]^T, y[t] = scale S[t]^T q[t].
+struct LinearDesc {
+  int B, H, Hk, T, D, Dv;
+  Rows q, k, v, y;           // y may be absent (null)
+  const float* state;        // [B, H, D, Dv] or null (zeros)
+  float* last;               // the last state, or null
+  const int32_t* documents;  // [B, T] or null
+  const int32_t* lengths;    // [B] or null
+  const float* rate;         // [H], log2(decay)
+  float scale;
+};
+struct LinearGradDesc {
+  LinearDesc a;              // a.y and a.last are not read
+  Rows dy, dq, dk, dv;       // each may be absent (null)
+  const float* dstate;       // of the last state, or null
+  float* dfirst;             // of `state`, or null
+};
+constexpr int kLinearMaxHead = 128;
+int64_t linear_workspace_bytes(const LinearDesc& a);
+void linear(const LinearDesc& a, void* work, hipStream_t st);
+int64_t linear_grad_workspace_bytes(const LinearGradDesc& g);
+void linear_grad(const LinearGradDesc& g, void* work, hipStream_t st);
+
+// The next token of each row, see ops.py. A limit is an array [rows], or its number where that is null.
+struct SampleDesc {
+  int64_t rows;
+  int V;
+  const float *logits, *u;   // [rows, V], [rows]
+  const float *temperature, *top_p, *min_p;
+  const int32_t* top_k;
+  double temperature1, top_p1, min_p1;
+  int32_t top_k1;
+  int32_t* token;
+};
+constexpr int kSampleMaxVocab = 1 << 24;
+int64_t sample_workspace_bytes(const SampleDesc& s);
+void sample(const SampleDesc& s, void* work, hipStream_t st);
 
 }  // namespace tgk

@@ -231,7 +231,7 @@ def _adjoint(op: dict, oc: Tensor, graph: Graph, cot: Dict[int, Tensor]) -> None
         s_keep = O.sum_(dcxc, -1, keep_dims=True)
         inner = O.sub(oc, O.broadcast_to(s_keep, c.shape))
         acc(op['a'], O.mul(inner, c))
-    elif k in ('less', 'greater', 'argmax_last', 'categorical_last'):
+    elif k in ('less', 'greater', 'argmax_last', 'categorical_last', 'sample'):
         return
     elif k == 'where':
         a, b = T(op['a']), T(op['b'])
@@ -256,7 +256,8 @@ def _adjoint(op: dict, oc: Tensor, graph: Graph, cot: Dict[int, Tensor]) -> None
     elif k == 'attention':
         opt = lambda n: None if op[n] is None else T(op[n])  # noqa: E731
         grads = O.attention_grad(T(op['q']), T(op['k']), T(op['v']), T(op['out']), oc, op['causal'], op['scale'],
-                                 op['softcap'], op['slopes'], opt('documents'), opt('prefix'), opt('lengths'))
+                                 op['softcap'], op['slopes'], opt('documents'), opt('prefix'), opt('lengths'),
+                                 op['window'], op['sinks'])
         for n, c in zip('qkv', grads):
             acc(op[n], c)
     elif k == 'rope_axes':
@@ -266,7 +267,18 @@ def _adjoint(op: dict, oc: Tensor, graph: Graph, cot: Dict[int, Tensor]) -> None
         grads = O.linear_recurrence_grad(T(op['a']), T(op['out']), oc, h0)
         for n, c in zip(('a', 'x', 'h0'), grads):
             acc(op[n], c)
-    elif k == 'attention_stats' or k.startswith(('attention_grad_', 'linear_recurrence_grad_')):
+    elif k in ('linear_attention', 'linear_attention_state'):
+        opt = lambda n: None if op[n] is None else T(op[n])  # noqa: E731
+        dy, dstate = (oc, None) if k == 'linear_attention' else (None, oc)
+        if dstate is not None:                           # y's op stands right before: both gradients in one pass
+            before = graph.ops[next(i for i, o in enumerate(graph.ops) if o is op) - 1]
+            if before['kind'] == 'linear_attention' and all(before[n] == op[n] for n in op if n not in ('kind', 'out')):
+                dy = cot.pop(before['out'], None)
+        grads = O.linear_attention_grad(T(op['q']), T(op['k']), T(op['v']), dy, op['decay'], op['scale'], opt('state'),
+                                        opt('documents'), opt('lengths'), dstate)
+        for n, c in zip(('q', 'k', 'v', 'state'), grads):
+            acc(op[n], c)
+    elif k == 'attention_stats' or k.startswith(('attention_grad_', 'linear_recurrence_grad_', 'linear_attention_grad_')):
         raise ValueError(f"autograd: cannot differentiate through {k} (it's a backward op)")
     elif k in ('conv2d_input_grad', 'conv2d_weight_grad', 'max_pool_2d_grad', 'scatter_axis'):
         raise ValueError(f"autograd: cannot differentiate through {k} (it's a backward op)")

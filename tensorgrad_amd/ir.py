@@ -101,8 +101,10 @@ _INPUT_FIELDS.update({
 OP_KINDS = tuple(_INPUT_FIELDS.keys())
 
 # Kinds of this framework that the reference's union does not have: sequence operators with
-# their gradients. Masks and initial states are optional inputs (None where absent).
+# their gradients, and the choice of a token. Masks, initial states and limits are optional
+# inputs (None where absent).
 _MASKS = ('documents', 'prefix', 'lengths')
+_LINEAR = ('q', 'k', 'v', 'state', 'documents', 'lengths')
 _EXTENSIONS: Dict[str, Tuple[str, ...]] = {
     'attention': ('q', 'k', 'v') + _MASKS,
     'attention_stats': ('q', 'k', 'v') + _MASKS,
@@ -114,6 +116,13 @@ _EXTENSIONS: Dict[str, Tuple[str, ...]] = {
     'linear_recurrence_grad_a': ('a', 'h', 'dh', 'h0'),
     'linear_recurrence_grad_x': ('a', 'h', 'dh', 'h0'),
     'linear_recurrence_grad_h0': ('a', 'h', 'dh', 'h0'),
+    'linear_attention': _LINEAR,
+    'linear_attention_state': _LINEAR,
+    'linear_attention_grad_q': _LINEAR + ('dy', 'dstate'),
+    'linear_attention_grad_k': _LINEAR + ('dy', 'dstate'),
+    'linear_attention_grad_v': _LINEAR + ('dy', 'dstate'),
+    'linear_attention_grad_state': _LINEAR + ('dy', 'dstate'),
+    'sample': ('logits', 'u', 'temperature', 'topK', 'topP', 'minP'),
 }
 _INPUT_FIELDS.update(_EXTENSIONS)
 EXTENSION_KINDS = tuple(_EXTENSIONS)

@@ -553,8 +553,12 @@ def _finite(x) -> bool:
     return _num(x) and math.isfinite(x)
 
 
+def _count(x) -> bool:
+    return isinstance(x, int) and not isinstance(x, bool)
+
+
 def _attention_fields(site: str, q: Tensor, k: Tensor, v: Tensor, causal, scale, softcap, slopes, documents, prefix,
-                      lengths) -> dict:
+                      lengths, window, sinks) -> dict:
     for name, t in (('q', q), ('k', k), ('v', v)):
         if t.dtype != 'f32':
             raise ShapeError(f'{site}: {name} must be f32, got {t.dtype}', site)
@@ -585,16 +589,28 @@ def _attention_fields(site: str, q: Tensor, k: Tensor, v: Tensor, causal, scale,
             raise ShapeError(f'{site}: slopes must be {H} finite numbers, one per query head, of 2^60 at most', site)
     if prefix is not None and not causal:
         raise ShapeError(f'{site}: a prefix needs a causal mask', site)
+    if window is not None and (not _count(window) or not 1 <= window < 2 ** 31):
+        raise ShapeError(f'{site}: window must be a whole number of positions, 1 at least, got {window}', site)
+    if not _count(sinks) or not 0 <= sinks < 2 ** 31:
+        raise ShapeError(f'{site}: sinks must be a whole number of positions, got {sinks}', site)
+    if window is not None and not causal:
+        raise ShapeError(f'{site}: a window needs a causal mask', site)
+    if sinks and window is None:
+        raise ShapeError(f'{site}: sinks need a window', site)
+    if sinks and documents is not None:
+        raise ShapeError(f'{site}: sinks are the first positions of a sequence, which documents end', site)
     for name, t, shape in (('documents', documents, (B, Tk)), ('prefix', prefix, (B,)), ('lengths', lengths, (B,))):
         if t is not None and (t.dtype != 'i32' or t.shape != shape):
             raise ShapeError(f'{site}: {name} must be i32 {S.show(shape)}, got {t.dtype} {S.show(t.shape)}', site)
     ids = {n: None if t is None else t.id for n, t in (('documents', documents), ('prefix', prefix), ('lengths', lengths))}
-    return {'q': q.id, 'k': k.id, 'v': v.id, **ids, 'causal': bool(causal), 'scale': scale, 'softcap': softcap, 'slopes': slopes}
+    return {'q': q.id, 'k': k.id, 'v': v.id, **ids, 'causal': bool(causal), 'scale': scale, 'softcap': softcap, 'slopes': slopes,
+            'window': window, 'sinks': sinks}
 
 
 def attention(q: Tensor, k: Tensor, v: Tensor, causal: bool = True, scale: Optional[float] = None,
               softcap: Optional[float] = None, slopes: Optional[Sequence[float]] = None, documents: Optional[Tensor] = None,
-              prefix: Optional[Tensor] = None, lengths: Optional[Tensor] = None) -> Tensor:
+              prefix: Optional[Tensor] = None, lengths: Optional[Tensor] = None, window: Optional[int] = None,
+              sinks: int = 0) -> Tensor:
     """Attention of q [B, H, Tq, D] over k [B, Hk, Tk, D], v [B, Hk, Tk, Dv] -> [B, H, Tq, Dv]. Query head h reads key head
     h // (H / Hk). With x = scale q.k (scale: 1 / sqrt(D)), the score of key j for a query at position p is
 
@@ -602,21 +618,22 @@ def attention(q: Tensor, k: Tensor, v: Tensor, causal: bool = True, scale: Optio
 
     `lengths` i32 [B]: only the first lengths[b] keys are there (clamped to 0..Tk; without it all Tk). The queries are the
     last Tq of those positions, so one new token against a filled cache is Tq = 1. `causal` hides keys after p, except those
-    below `prefix` i32 [B], which every query sees. `documents` i32 [B, Tk]: a query sees the keys of its own document (that
+    below `prefix` i32 [B], which every query sees. `window` leaves a query the last `window` keys up to its own, p - window < j,
+    beside the first `sinks` positions (not with documents) and those of a prefix; both need the causal mask. `documents` i32 [B, Tk]: a query sees the keys of its own document (that
     at its position); negative ids are padding, which sees and is seen by nothing. A query that sees no key (or, where
     positions matter, lies before position 0) gives zeros and takes and gives no gradient. What a mask hides has no
     influence, whatever its values (infinities and NaN included)."""
-    f = _attention_fields('attention', q, k, v, causal, scale, softcap, slopes, documents, prefix, lengths)
+    f = _attention_fields('attention', q, k, v, causal, scale, softcap, slopes, documents, prefix, lengths, window, sinks)
     return add_op(current_graph(), 'attention', (*q.shape[:3], v.shape[3]), 'f32', 'attention', f)
 
 
 def attention_grad(q: Tensor, k: Tensor, v: Tensor, y: Tensor, dy: Tensor, causal: bool = True, scale: Optional[float] = None,
                    softcap: Optional[float] = None, slopes: Optional[Sequence[float]] = None,
                    documents: Optional[Tensor] = None, prefix: Optional[Tensor] = None,
-                   lengths: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+                   lengths: Optional[Tensor] = None, window: Optional[int] = None, sinks: int = 0) -> Tuple[Tensor, Tensor, Tensor]:
     """(dq, dk, dv) of y = attention(q, k, v, ...) for the gradient dy of y; the other arguments as given there."""
     site = 'attentionGrad'
-    f = _attention_fields(site, q, k, v, causal, scale, softcap, slopes, documents, prefix, lengths)
+    f = _attention_fields(site, q, k, v, causal, scale, softcap, slopes, documents, prefix, lengths, window, sinks)
     shape = (*q.shape[:3], v.shape[3])
     for name, t in (('y', y), ('dy', dy)):
         if t.dtype != 'f32' or t.shape != shape:
@@ -681,6 +698,119 @@ def linear_recurrence_grad(a: Tensor, h: Tensor, dh: Tensor, h0: Optional[Tensor
     f = {'a': a.id, 'h': h.id, 'dh': dh.id, 'h0': None if h0 is None else h0.id}
     outs = (('a', a.shape), ('x', a.shape)) + ((('h0', h0.shape),) if h0 is not None else ())
     return tuple(add_op(current_graph(), f'linear_recurrence_grad_{n}', s, 'f32', site, f) for n, s in outs)
+
+
+LINEAR_MAX_HEAD = 128      # the kernels' tiles hold whole heads
+
+
+def _linear_fields(site: str, q: Tensor, k: Tensor, v: Tensor, decay, scale, state, documents, lengths) -> dict:
+    for name, t in (('q', q), ('k', k), ('v', v)):
+        if t.dtype != 'f32' or len(t.shape) != 4 or min(t.shape) < 1:
+            raise ShapeError(f'{site}: {name} must be f32 [batch, heads, length, head size], got {t.dtype} {S.show(t.shape)}', site)
+    B, H, T, D = q.shape
+    Hk, Dv = v.shape[1], v.shape[3]
+    if k.shape != (B, Hk, T, D) or v.shape != (B, Hk, T, Dv):
+        raise ShapeError(f'{site}: q {S.show(q.shape)}, k {S.show(k.shape)} and v {S.show(v.shape)} must agree in batch and length, '
+                         'q and k in head size, k and v in heads', site)
+    if H % Hk != 0:
+        raise ShapeError(f'{site}: {H} query heads cannot share {Hk} key heads evenly', site)
+    if max(D, Dv) > LINEAR_MAX_HEAD:
+        raise ShapeError(f'{site}: head sizes above {LINEAR_MAX_HEAD} are not supported, got {D} and {Dv}', site)
+    decay = [float(x) for x in decay] if all(_finite(x) and 0 < x <= 1 for x in decay) else None
+    if decay is None or len(decay) != H:
+        raise ShapeError(f'{site}: decay must be {H} numbers above 0, of 1 at most, one per query head', site)
+    if scale is None:
+        scale = 1 / math.sqrt(D)
+    if not _finite(scale) or not 1 / ATTENTION_RANGE <= scale <= ATTENTION_RANGE:
+        raise ShapeError(f'{site}: scale must be positive, between 2^-60 and 2^60, got {scale}', site)
+    if state is not None and (state.dtype != 'f32' or state.shape != (B, H, D, Dv)):
+        raise ShapeError(f'{site}: state must be f32 {S.show((B, H, D, Dv))}, got {state.dtype} {S.show(state.shape)}', site)
+    for name, t, shape in (('documents', documents, (B, T)), ('lengths', lengths, (B,))):
+        if t is not None and (t.dtype != 'i32' or t.shape != shape):
+            raise ShapeError(f'{site}: {name} must be i32 {S.show(shape)}, got {t.dtype} {S.show(t.shape)}', site)
+    ids = {n: None if t is None else t.id for n, t in (('state', state), ('documents', documents), ('lengths', lengths))}
+    return {'q': q.id, 'k': k.id, 'v': v.id, **ids, 'decay': decay, 'scale': scale}
+
+
+def linear_attention(q: Tensor, k: Tensor, v: Tensor, decay: Sequence[float], scale: Optional[float] = None,
+                     state: Optional[Tensor] = None, documents: Optional[Tensor] = None,
+                     lengths: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """Linear attention with a decay for each head: (y, last state) of q [B, H, T, D], k [B, Hk, T, D], v [B, Hk, T, Dv]. Query
+    head h reads key head h // (H / Hk) and has the state S [D, Dv], from `state` [B, H, D, Dv] (zeros without it):
+
+        S[t] = decay[h] S[t-1] + k[t] v[t]^T,   y[t] = scale S[t]^T q[t]        (scale: 1 / sqrt(D))
+
+    which is y[t] = scale sum over s <= t of decay^(t - s) (q[t].k[s]) v[s] beside what `state` adds. The last state [B, H, D, Dv]
+    is what the next positions start from: a prompt is read in one call, or in pieces, and answered with T = 1. `lengths` i32 [B]:
+    only the first lengths[b] positions are there (clamped to 0..T), y is 0 behind them and the last state that after them.
+    `documents` i32 [B, T]: the state starts from zeros where an id differs from the one before (position 0 goes on from `state`);
+    negative ids are padding, where y and the state are 0. What is not there has no influence, whatever its values."""
+    f = _linear_fields('linearAttention', q, k, v, decay, scale, state, documents, lengths)
+    B, H, T, D = q.shape
+    g = current_graph()
+    return (add_op(g, 'linear_attention', (B, H, T, v.shape[3]), 'f32', 'linearAttention', f),
+            add_op(g, 'linear_attention_state', (B, H, D, v.shape[3]), 'f32', 'linearAttention', f))
+
+
+def linear_attention_grad(q: Tensor, k: Tensor, v: Tensor, dy: Optional[Tensor], decay: Sequence[float],
+                          scale: Optional[float] = None, state: Optional[Tensor] = None, documents: Optional[Tensor] = None,
+                          lengths: Optional[Tensor] = None, dstate: Optional[Tensor] = None) -> Tuple[Tensor, ...]:
+    """(dq, dk, dv), with `state` (dq, dk, dv, its gradient), of linear_attention(q, k, v, decay, ...) for the gradients dy of y
+    and dstate of the last state, one of which may be absent (None)."""
+    site = 'linearAttentionGrad'
+    f = _linear_fields(site, q, k, v, decay, scale, state, documents, lengths)
+    B, H, T, D = q.shape
+    if dy is None and dstate is None:
+        raise ShapeError(f'{site}: needs the gradient of y or of the last state', site)
+    for name, t, shape in (('dy', dy, (B, H, T, v.shape[3])), ('dstate', dstate, (B, H, D, v.shape[3]))):
+        if t is not None and (t.dtype != 'f32' or t.shape != shape):
+            raise ShapeError(f'{site}: {name} must be f32 {S.show(shape)}, got {t.dtype} {S.show(t.shape)}', site)
+    f = dict(f, dy=None if dy is None else dy.id, dstate=None if dstate is None else dstate.id)
+    outs = (('q', q), ('k', k), ('v', v)) + ((('state', state),) if state is not None else ())
+    return tuple(add_op(current_graph(), f'linear_attention_grad_{n}', t.shape, 'f32', site, f) for n, t in outs)
+
+
+# ---- Choice of the next token (no reference counterpart) ---------------------------------------------
+
+SAMPLE_MAX_VOCAB = 1 << 24   # weights are whole numbers of 62 bits in all
+
+
+def sample(logits: Tensor, u: Tensor, temperature=1.0, top_k=None, top_p=None, min_p=None) -> Tensor:
+    """The next token of each row: i32 [...] for logits f32 [..., V] and random numbers u f32 [...] from [0, 1).
+
+    Tokens are ordered by falling logit, equal ones by rising index, and weigh exp((logit - largest) / temperature). Each limit
+    keeps a first part of that order: `top_k` tokens; of those the fewest whose weights reach `top_p` of their sum; and of those
+    the ones of at least `min_p` times the largest weight. The token is the first kept one, in the vocabulary's order, where the
+    kept weights' running sum passes u of them all.
+
+    A limit is one number for all rows, or a tensor of u's shape with a number for each (f32, `top_k` i32); None, a top_k below 1
+    or a top_p from 1 on do not limit, and a temperature of 0 takes the largest logit. Minus infinity and NaN are never chosen; a
+    row without any other logit gives -1. Weights below 2^-38 of the largest may count as 0 (2^-62 V, whatever V is)."""
+    site = 'sample'
+    if logits.dtype != 'f32' or len(logits.shape) < 1 or min(logits.shape) < 1:
+        raise ShapeError(f'{site}: logits must be f32 [..., vocabulary], got {logits.dtype} {S.show(logits.shape)}', site)
+    rows = logits.shape[:-1]
+    if logits.shape[-1] > SAMPLE_MAX_VOCAB:
+        raise ShapeError(f'{site}: vocabularies above {SAMPLE_MAX_VOCAB} are not supported, got {logits.shape[-1]}', site)
+    if u.dtype != 'f32' or u.shape != rows:
+        raise ShapeError(f'{site}: u must be f32 {S.show(rows)}, got {u.dtype} {S.show(u.shape)}', site)
+    f = {'logits': logits.id, 'u': u.id}
+    values = []
+    for name, x, none, ok in (('temperature', temperature, 1.0, lambda x: x >= 0), ('topK', top_k, 0, lambda x: _count(x) and 0 <= x < 2 ** 31),
+                              ('topP', top_p, 1.0, lambda x: x > 0), ('minP', min_p, 0.0, lambda x: 0 <= x <= 1)):
+        dtype = 'i32' if name == 'topK' else 'f32'
+        f[name] = None
+        if isinstance(x, Tensor):
+            if x.dtype != dtype or x.shape != rows:
+                raise ShapeError(f'{site}: {name} must be a number or {dtype} {S.show(rows)}, got {x.dtype} {S.show(x.shape)}', site)
+            f[name] = x.id
+            x = none
+        elif x is None:
+            x = none
+        elif not _finite(x) or not ok(x):
+            raise ShapeError(f'{site}: {name} out of range, got {x}', site)
+        values.append(x)
+    return add_op(current_graph(), 'sample', rows, 'i32', site, dict(f, values=values))
 
 
 # ---- Broadcast / constants / comparisons (ops.ts:943-1008) -----------------------------------------

@@ -1,0 +1,229 @@
+"""Windowed attention, linear attention and the choice of a token without a GPU: refusals, gradients' IR, the lowered schedule,
+and the tests' own 64-bit forms."""
+import numpy as np
+import pytest
+
+import _decoders as D
+from tensorgrad_amd import backend
+from tensorgrad_amd import ir as IR
+from tensorgrad_amd import ops as O
+from tensorgrad_amd.build_ir import build_forward_ir, build_training_ir
+from tensorgrad_amd.module import Module
+from tensorgrad_amd.shape import ShapeError
+from tensorgrad_amd.trace import tensor_input, trace_fn
+
+
+def t(name, *shape, dtype='f32'):
+    return tensor_input(name, list(shape), dtype)
+
+
+def refuses(fn, match):
+    with pytest.raises(ShapeError, match=match):
+        trace_fn(fn)
+
+
+def qkv(D_=8, T=4, H=4, Hk=2, Dv=8):
+    return t('q', 2, H, T, D_), t('k', 2, Hk, T, D_), t('v', 2, Hk, T, Dv)
+
+
+def test_window_refusals():
+    for window in (0, -1, 2.0, True, 2 ** 31, float('nan'), '3'):
+        refuses(lambda: O.attention(*qkv(), window=window), 'window')
+    for sinks in (-1, 1.0, None, True, 2 ** 31):
+        refuses(lambda: O.attention(*qkv(), window=2, sinks=sinks), 'sinks')
+    refuses(lambda: O.attention(*qkv(), causal=False, window=2), 'causal')
+    refuses(lambda: O.attention(*qkv(), sinks=2), 'sinks need')
+    refuses(lambda: O.attention(*qkv(), window=2, sinks=1, documents=t('d', 2, 4, dtype='i32')), 'documents')
+    refuses(lambda: O.attention_grad(*qkv(), t('y', 2, 4, 4, 8), t('g', 2, 4, 4, 8), window=0), 'window')
+    trace_fn(lambda: O.attention(*qkv(), window=2, documents=t('d', 2, 4, dtype='i32')))
+    trace_fn(lambda: O.attention(*qkv(), window=2 ** 31 - 1, sinks=2 ** 31 - 1))
+
+
+def test_linear_refusals():
+    ok = [0.5, 0.9, 1.0, 1e-300]
+    trace_fn(lambda: O.linear_attention(*qkv(), ok))
+    refuses(lambda: O.linear_attention(t('z', 2, 4, 8), *qkv()[1:], ok), 'q must be')
+    refuses(lambda: O.linear_attention(*qkv()[:2], t('w', 2, 2, 5, 8), ok), 'agree')
+    refuses(lambda: O.linear_attention(*qkv()[:2], t('w', 2, 4, 4, 8), ok), 'agree')
+    refuses(lambda: O.linear_attention(*qkv(H=3), ok[:3]), 'share')
+    refuses(lambda: O.linear_attention(*qkv(D_=129), ok), 'above 128')
+    refuses(lambda: O.linear_attention(*qkv(Dv=129), ok), 'above 128')
+    refuses(lambda: O.linear_attention(t('z', 2, 4, 0, 8), *qkv()[1:], ok), 'q must be')
+    for decay in ([0.5] * 3, [0.5] * 5, [0.5, 0.5, 0.5, 0], [0.5, 0.5, 0.5, 1.01], [0.5, 0.5, 0.5, -0.1], [0.5, 0.5, 0.5, float('nan')],
+                  [0.5, 0.5, 0.5, True]):
+        refuses(lambda: O.linear_attention(*qkv(), decay), 'decay')
+    for scale in (0, -1, float('nan'), float('inf'), 1e-300, True):
+        refuses(lambda: O.linear_attention(*qkv(), ok, scale=scale), 'scale')
+    refuses(lambda: O.linear_attention(*qkv(), ok, state=t('s', 2, 2, 8, 8)), 'state')
+    refuses(lambda: O.linear_attention(*qkv(), ok, state=t('s', 2, 4, 8, 8, dtype='i32')), 'state')
+    refuses(lambda: O.linear_attention(*qkv(), ok, documents=t('d', 2, 5, dtype='i32')), 'documents')
+    refuses(lambda: O.linear_attention(*qkv(), ok, lengths=t('n', 2)), 'lengths')
+    refuses(lambda: O.linear_attention_grad(*qkv(), None, ok), 'needs')
+    refuses(lambda: O.linear_attention_grad(*qkv(), t('g', 2, 4, 4, 9), ok), 'dy')
+    refuses(lambda: O.linear_attention_grad(*qkv(), None, ok, dstate=t('g', 2, 4, 8, 9)), 'dstate')
+
+
+def test_sample_refusals():
+    x, u = (lambda *s: t('x', *(s or (3, 7)))), (lambda *s: t('u', *(s or (3,))))
+    trace_fn(lambda: O.sample(x(), u(), 0, 0, 2, 0))
+    trace_fn(lambda: O.sample(x(5), tensor_input('u', [], 'f32')))
+    refuses(lambda: O.sample(t('x', 3, 7, dtype='i32'), u()), 'logits')
+    refuses(lambda: O.sample(tensor_input('x', [], 'f32'), u()), 'logits')
+    refuses(lambda: O.sample(x(3, 0), u()), 'logits')
+    refuses(lambda: O.sample(x(1, 2 ** 24 + 1), u(1)), 'above')
+    refuses(lambda: O.sample(x(), u(4)), 'u must')
+    refuses(lambda: O.sample(x(), t('u', 3, dtype='i32')), 'u must')
+    for bad in (dict(temperature=-0.1), dict(temperature=float('nan')), dict(top_k=-1), dict(top_k=2.0), dict(top_k=2 ** 31), dict(top_p=0),
+                dict(top_p=-1.0), dict(top_p=float('inf')), dict(min_p=-0.1), dict(min_p=1.1), dict(min_p='a'), dict(top_k=True)):
+        refuses(lambda: O.sample(x(), u(), **bad), 'out of range')
+    for name, dtype in (('temperature', 'i32'), ('top_k', 'f32'), ('top_p', 'i32'), ('min_p', 'i32')):
+        refuses(lambda: O.sample(x(), u(), **{name: t('l', 3, dtype=dtype)}), 'a number or')
+        refuses(lambda: O.sample(x(), u(), **{name: t('l', 4, dtype='i32' if name == 'top_k' else 'f32')}), 'a number or')
+
+
+class Params(Module):
+    def __init__(self, **shapes):
+        for n, s in shapes.items():
+            setattr(self, n, self.param(list(s)))
+
+
+def nodes_of(ir):
+    return backend.plan(ir.wire_json())['nodes']
+
+
+def test_gradients_reach_every_operand_and_lower_to_one_node_each():
+    m = Params(q=(2, 4, 6, 8), k=(2, 2, 6, 8), v=(2, 2, 6, 5), s=(2, 4, 8, 5))
+
+    def loss(p, i):
+        y, s = O.linear_attention(p.q, p.k, p.v, [0.9] * 4, state=p.s, documents=i['doc'])
+        z, _ = O.linear_attention(p.q, p.k, p.v, [0.5] * 4, state=s)
+        return O.mean(O.square(O.add(y, z)))
+    ir = build_training_ir(m, loss, {'doc': {'shape': [2, 6], 'dtype': 'i32'}}, {'kind': 'sgd', 'lr': 0.1})
+    assert {n: g.shape for n, g in ir.param_grads.items()} == {n: tuple(x) for n, x in (
+        ('q', (2, 4, 6, 8)), ('k', (2, 2, 6, 8)), ('v', (2, 2, 6, 5)), ('s', (2, 4, 8, 5)))}
+    kinds = [n['kind'] for n in nodes_of(ir)]
+    assert [kinds.count(k) for k in ('linear', 'linear_grad')] == [2, 2]
+
+    def loss(p, i):
+        return O.mean(O.square(O.attention(p.q, p.k, p.v, window=3, sinks=1)))
+    ir = build_training_ir(Params(q=(2, 4, 6, 8), k=(2, 2, 6, 8), v=(2, 2, 6, 5)), loss, {}, {'kind': 'sgd', 'lr': 0.1})
+    kinds = [n['kind'] for n in nodes_of(ir)]
+    assert [kinds.count(k) for k in ('attend', 'attend_grad')] == [1, 1]
+    grads = [o for o in ir.graph.ops if o['kind'].startswith('attention_grad_')]
+    assert len(grads) == 3 and all((o['window'], o['sinks']) == (3, 1) for o in grads)
+
+
+def test_only_what_is_needed_is_made():
+    def fwd(m, i):
+        return O.linear_attention(i['q'], i['k'], i['v'], [0.9] * 2)[0]
+    ir = build_forward_ir(Module(), fwd, {'q': [1, 2, 6, 8], 'k': [1, 1, 6, 8], 'v': [1, 1, 6, 8]})
+    assert [n['ops'] for n in nodes_of(ir) if n['kind'] == 'linear'] == ['linear_attention']
+    ir = build_training_ir(Params(k=(1, 1, 6, 8)), lambda p, i: O.mean(O.linear_attention(i['q'], p.k, i['v'], [0.9] * 2)[0]),
+                           {'q': [1, 2, 6, 8], 'v': [1, 1, 6, 8]}, {'kind': 'sgd', 'lr': 0.1})
+    assert [n['ops'] for n in nodes_of(ir) if n['kind'] == 'linear_grad'] == ['linear_attention_grad_k']
+
+
+def test_a_chosen_token_has_no_gradient_and_backward_ops_refuse_one():
+    ir = build_training_ir(Params(x=(3, 7)), lambda p, i: O.add(O.mean(O.square(p.x)), O.mean(O.one_hot(O.sample(p.x, i['u']), 7))),
+                           {'u': [3]}, {'kind': 'sgd', 'lr': 0.1})
+    assert not [o for o in ir.graph.ops if o['kind'] == 'categorical_last'] and list(ir.param_grads) == ['x']
+
+    def twice(p, i):
+        return O.mean(O.linear_attention_grad(p.q, i['k'], i['v'], i['dy'], [0.9])[0])
+    s = [1, 1, 6, 8]
+    with pytest.raises(ValueError, match='backward op'):
+        build_training_ir(Params(q=s), twice, {'k': s, 'v': s, 'dy': s}, {'kind': 'sgd', 'lr': 0.1})
+
+
+def test_heads_are_read_in_place():
+    def fwd(m, i):
+        q, k, v = (O.split_heads(O.matmul(i['x'], i[n]), 2) for n in ('wq', 'wk', 'wv'))
+        return O.linear_attention(q, k, v, [0.9, 0.8])[0]
+    ir = build_forward_ir(Module(), fwd, {'x': [2, 5, 16], 'wq': [16, 16], 'wk': [16, 16], 'wv': [16, 16]})
+    kinds = [n['kind'] for n in nodes_of(ir)]
+    assert 'copy' not in kinds and kinds.count('linear') == 1
+
+
+def wire(build, kind, **change):
+    g = trace_fn(build)
+    doc = {'graph': IR.graph_to_wire(g), 'paramGrads': {}, 'writebacks': [], 'optimizer': None}
+    for op in doc['graph']['ops']:
+        if op['kind'] == kind:
+            op.update(change)
+            for n in [n for n, x in change.items() if x == 'gone']:
+                del op[n]
+    return IR.dumps(doc)
+
+
+@pytest.mark.parametrize('change', [dict(scale=-1.0), dict(decay=[0.5]), dict(decay=[0.5, 0.5, 0.5, 2.0]), dict(decay=[0.5, 0.5, 0.5, 0.0]),
+                                    dict(k=0), dict(documents=0), dict(lengths=0), dict(state=0)])
+def test_bad_linear_documents_are_refused_by_the_runtime(change):
+    build = lambda: O.linear_attention(*qkv(D_=7), [0.5] * 4)[0]  # noqa: E731
+    backend.plan(wire(build, 'linear_attention'))
+    with pytest.raises(backend.BackendError) as e:
+        backend.plan(wire(build, 'linear_attention', **change))
+    assert e.value.status == backend.TG_INVALID_ARGUMENT
+
+
+def test_bad_window_and_sample_documents_are_refused_by_the_runtime():
+    attend = lambda: O.attention(*qkv(T=6), window=3, sinks=1)  # noqa: E731
+    backend.plan(wire(attend, 'attention'))
+    backend.plan(wire(attend, 'attention', window='gone', sinks='gone'))       # a document from before there were windows
+    draw = lambda: O.sample(t('x', 3, 7), t('u', 3))  # noqa: E731
+    backend.plan(wire(draw, 'sample'))
+    for build, kind, change in (
+            (attend, 'attention', dict(window=0)), (attend, 'attention', dict(window=1.5)), (attend, 'attention', dict(causal=False)),
+            (attend, 'attention', dict(window=None)), (attend, 'attention', dict(sinks=-1)), (attend, 'attention', dict(window=2 ** 31)),
+            (draw, 'sample', dict(u=0)), (draw, 'sample', dict(topK=1)), (draw, 'sample', dict(values=[1.0])),
+            (draw, 'sample', dict(values=[-1.0, 0, 1.0, 0.0])), (draw, 'sample', dict(values=[1.0, 0, 0.0, 0.0])), (draw, 'sample', dict(temperature=0))):
+        with pytest.raises(backend.BackendError) as e:
+            backend.plan(wire(build, kind, **change))
+        assert e.value.status == backend.TG_INVALID_ARGUMENT, (kind, change)
+
+
+# ---- the tests' own forms -----------------------------------------------------------------------------
+
+def inputs(seed, T=9):
+    r = np.random.default_rng(seed)
+    a = {n: r.standard_normal(s) for n, s in (('q', (1, 2, T, 4)), ('k', (1, 1, T, 4)), ('v', (1, 1, T, 3)), ('state', (1, 2, 4, 3)),
+                                              ('dy', (1, 2, T, 3)), ('dstate', (1, 2, 4, 3)))}
+    return a, dict(decay=[0.9, 0.4], scale=0.7, documents=np.array([[0, 0, 0, 2, 2, -1, -1, 1, 1]]), lengths=np.array([8]))
+
+
+@pytest.mark.parametrize('masks', [(), ('documents',), ('lengths',), ('documents', 'lengths')])
+def test_the_pair_form_agrees_with_the_recurrence(masks):
+    a, how = inputs(1)
+    how = {n: x for n, x in how.items() if n in ('decay', 'scale') + masks}
+    got, _ = D.linear(a['q'], a['k'], a['v'], state=a['state'], **how)
+    for h in range(2):
+        y, s = D.recurrence(a['q'][0, h], a['k'][0, 0], a['v'][0, 0], how['decay'][h], 0.7, a['state'][0, h],
+                            how['documents'][0] if 'documents' in masks else None, how['lengths'][0] if 'lengths' in masks else None)
+        assert np.allclose(got['y'][0, h], y, rtol=0, atol=1e-12) and np.allclose(got['state'][0, h], s, rtol=0, atol=1e-12)
+
+
+@pytest.mark.parametrize('masks', [(), ('documents',), ('lengths',)])
+def test_the_64_bit_gradients_agree_with_differences(masks):
+    a, how = inputs(2)
+    how = {n: x for n, x in how.items() if n in ('decay', 'scale') + masks}
+    got, _ = D.linear(**a, **how)
+    r = np.random.default_rng(3)
+    for name, grad in (('q', 'dq'), ('k', 'dk'), ('v', 'dv'), ('state', 'dstate')):
+        step, side = r.standard_normal(a[name].shape), []
+        for s in (1, -1):
+            b = dict(a, **{name: a[name] + s * 1e-5 * step})
+            out, _ = D.linear(b['q'], b['k'], b['v'], state=b['state'], **how)
+            side.append((out['y'] * a['dy']).sum() + (out['state'] * a['dstate']).sum())
+        assert abs((side[0] - side[1]) / 2e-5 - (got[grad] * step).sum()) < 1e-7
+
+
+def test_the_64_bit_choice_of_small_rows():
+    x = np.log(np.array([0.1, 0.4, 0.2, 0.3]))
+    at = lambda **how: [D.sample(x, u, **how) for u in (0.0, 0.05, 0.15, 0.45, 0.55, 0.65, 0.75, 0.999)]  # noqa: E731
+    assert at() == [0, 0, 1, 1, 2, 2, 3, 3]
+    assert at(top_k=2) == [1, 1, 1, 1, 1, 3, 3, 3]           # 4 / 7 and 3 / 7
+    assert at(top_p=0.69) == [1, 1, 1, 1, 1, 3, 3, 3]        # 0.4 + 0.3 reach it
+    assert at(top_p=0.71) == [1, 1, 1, 2, 2, 2, 3, 3]        # 4 / 9, 2 / 9, 3 / 9
+    assert at(min_p=0.6) == [1, 1, 1, 1, 1, 3, 3, 3]
+    assert at(temperature=0) == [1] * 8
+    assert at(top_k=3, top_p=0.5, min_p=0.9) == [1] * 8
+    assert D.sample(np.array([-np.inf, np.nan]), 0.5) == -1
