@@ -8,9 +8,19 @@
 //   dv_j = sum_{i >= j} scale w_ij (k_j.q_i) dy_i + e_j G_out^T k_j
 //   S_out = f S_in + sum_j e_j k_j v_j^T,    G_in = f G_out + sum_i scale c_i q_i dy_i^T,    f = lam^(rows of the segment) or 0
 //
-// G: the gradient of the state. All four results have one form, out_r = sum_s w (row_r.X_s) Z_s + coef_r M row_r, and both
-// states another, so there are three kernels: sums over a segment (linear_sums), states from sums (linear_join), results from
-// pairs and states (linear_pairs). Nothing is added by atomics.
+// G: the gradient of the state. y, dq, dk and dv have one form, out_r = sum_s w (row_r.X_s) Z_s + coef_r M row_r, and both states
+// another, so there are three kernels: sums over a segment (linear_sums), states from sums (linear_join), results from pairs and
+// states (linear_tiles; linear_pairs for rows that are not whole 16-byte pieces). A few positions are walked one after another
+// (linear_steps). Nothing is added by atomics.
+//
+// Products run on the f32 matrix instructions: no scales for operands of any size, and the work is bound by memory about as much.
+// Fragments of a 16 x 16 x 4 product: lane l holds row (A) or column (B) l % 16 and k = g = l / 16; a result's register q holds row
+// 4 g + q of column l % 16. A wavefront's own 16 rows are the columns of every product. A tile of 32 rows lies in LDS in f32: read
+// by 16 bytes, four steps of a product over features (k of step q is feature 4 g + q of 16), or by columns, a product over rows
+// whose k of step q is row 4 g + q, which is where the weights stand as they come out of the first product.
+//
+// What a row does not see has weight 0, and 0 times an infinity or NaN is NaN: rows whose result is not finite are computed again
+// pair by pair, from what they see alone.
 #include <algorithm>
 
 #include "kernels.h"
@@ -21,15 +31,14 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kSeg = 256;          // positions of a segment
-constexpr int kRows = 64;          // rows of a block
+constexpr int kSeg = 128;          // positions of a segment
 constexpr int kTile = 32;          // rows of a tile in LDS
 constexpr int kNever = INT32_MAX;
 
 __device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ float power(float rate, int n) { return __builtin_amdgcn_exp2f(rate * (float)n); }
+__device__ __forceinline__ float scalar(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
 
-// What the positions of one batch entry are, and those of one segment.
 struct Marks {
   const int32_t *documents, *lengths;
   int T;
@@ -37,27 +46,29 @@ struct Marks {
 __device__ __forceinline__ int count_of(const Marks& m, int b) { return m.lengths ? min(max(m.lengths[b], 0), m.T) : m.T; }
 
 // since[t - s0] for the positions of the segment at s0: the first one, in the segment, of the document they belong to; -1 where
-// that began before (or the state that came in counts); kNever for positions that are not there. By 256 threads; ends at a barrier.
-__device__ __forceinline__ void mark(const Marks& m, int b, int s0, int n, int* since, int* waves) {
-  const int tid = threadIdx.x, t = s0 + tid, lane = tid & 63, w = tid >> 6;
+// that began before (or the state that came in counts); kNever for positions that are not there. Ends at a barrier.
+__device__ __forceinline__ void mark(const Marks& m, int b, int s0, int n, int* since) {
+  const int tid = threadIdx.x;
   if (!m.documents) {
-    if (tid < kSeg) since[tid] = t < n ? -1 : kNever;
-    __syncthreads();
-    return;
-  }
-  const int32_t* doc = m.documents + (int64_t)b * m.T;
-  const bool here = tid < kSeg && t < n;
-  const int id = here ? doc[t] : -1;
-  int first = here && t > 0 && doc[t - 1] != id ? t : -1;
+    for (int i = tid; i < kSeg; i += blockDim.x) since[i] = s0 + i < n ? -1 : kNever;
+  } else if (tid < 64) {
+    const int32_t* doc = m.documents + (int64_t)b * m.T;
+    int before = -1;
+    for (int i = tid; i < kSeg; i += 64) {
+      const int t = s0 + i;
+      const bool here = t < n;
+      const int id = here ? doc[t] : -1;
+      int first = here && t > 0 && doc[t - 1] != id ? t : -1;
 #pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const int z = __shfl_up(first, o);
-    if (lane >= o) first = max(first, z);
+      for (int o = 1; o < 64; o *= 2) {
+        const int z = __shfl_up(first, o);
+        if (tid >= o) first = max(first, z);
+      }
+      first = max(first, before);
+      before = __shfl(first, 63);
+      since[i] = here && id >= 0 ? first : kNever;
+    }
   }
-  if (lane == 63) waves[w] = first;
-  __syncthreads();
-  for (int k = 0; k < w; ++k) first = max(first, waves[k]);
-  if (tid < kSeg) since[tid] = here && id >= 0 ? first : kNever;
   __syncthreads();
 }
 // The segment's last position that is there; what a position leaves of itself there, and of what came in.
@@ -78,29 +89,70 @@ __device__ __forceinline__ float stays(const Ends& e, int s0, float rate) {
   return e.last < s0 ? 1.0f : e.since == -1 ? power(rate, e.last - s0 + 1) : 0.0f;
 }
 
-// Rows [r0, r0 + 32) of x as a tile of LD floats a row, zero where keep(t) says that a row does not count and past its n
-// features. Returns whether this thread met infinities or NaN.
-template <int DP, class Keep>
-__device__ __forceinline__ bool stage(float* tile, const float* x, int64_t stride, int r0, int T, int n, bool wide, Keep keep) {
-  constexpr int LD = DP + 4, Q = DP / 4;
-  bool odd = false;
-  for (int e = threadIdx.x; e < kTile * Q; e += 256) {
-    const int r = e / Q, d = e % Q * 4, t = r0 + r;
-    f32x4 u = {};
-    if (t < T && keep(t)) {
-      const float* p = x + (int64_t)t * stride + d;
-      if (wide) {
-        if (d < n) u = *(const f32x4*)p;
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) if (d + q < n) u[q] = p[q];
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) odd |= !(fabsf(u[q]) < INFINITY);
-    *(f32x4*)(tile + r * LD + d) = u;
+// ---- tiles in LDS --------------------------------------------------------------------------------------
+//
+// A row has PITCH floats, in pieces of 16 bytes; piece c of row r lies at place c ^ swizzle(r), so that 16 rows' same piece, and 4
+// rows' 4 pieces, lie in different banks.
+
+template <int DP>
+struct Tile {
+  static constexpr int PITCH = DP == 96 ? 128 : DP, PIECES = PITCH / 4, FLOATS = kTile * PITCH, C = DP / 16;
+  static __device__ __forceinline__ int swizzle(int r) { return DP == 32 ? (r >> 1) & 7 : r & 15; }
+  static __device__ __forceinline__ int place(int r, int piece) { return r * PITCH + 4 * (piece ^ swizzle(r)); }
+  // Fragments. An opaque lane keeps the compiler from holding every place's address through a loop over tiles (230 registers
+  // instead of 124); where pieces are told apart by 4 c ^ .., what c's upper bits add is a constant of the instruction.
+  static __device__ __forceinline__ int opaque(int lane) {
+    asm volatile("" : "+v"(lane));
+    return lane;
   }
-  return odd;
+  // at[c % 4] + far(c): piece 4 c + g of row l
+  static __device__ __forceinline__ void by_piece(int (&at)[4], int lane) {
+    const int l = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) at[c] = place(l, (4 * c + g) % PIECES);
+  }
+  // row[q] + column[c % 4] + far(c): feature 16 c + l of row 4 g + q
+  static __device__ __forceinline__ void by_column(int (&row)[4], int (&column)[4], int lane) {
+    static_assert(DP > 32);
+    const int l = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      row[q] = (4 * g + q) * PITCH + 4 * ((l >> 2) ^ q) + (l & 3);
+      column[q] = 16 * (q ^ g);
+    }
+  }
+  static __device__ __forceinline__ constexpr int far(int c) { return c / 4 * 64; }
+};
+
+// Rows [r0, r0 + 32) of x from memory straight into LDS, by WAVES wavefronts, 1 KiB an instruction. Nothing is masked: rows past the
+// last and features past the n-th are others that are there. In inline assembly, so that the compiler does not drain every load
+// before the next LDS read; the kernels wait (vmcnt) and meet (barrier) themselves.
+template <int DP, int WAVES>
+__device__ __forceinline__ void tile_to_lds(const float* x, int64_t stride, int r0, int rows, int n, uint32_t lds, int w) {
+  constexpr int PIECES = Tile<DP>::PIECES, ROWS = 64 / PIECES, N = kTile / ROWS;
+  const int lane = Tile<DP>::opaque(threadIdx.x & 63), left = rows - 1 - r0;
+  const char* base = (const char*)(x + (int64_t)r0 * stride);
+#pragma unroll
+  for (int i = 0; i < (N + WAVES - 1) / WAVES; ++i) {
+    const int k = w + i * WAVES;
+    if (N % WAVES && k >= N) break;
+    const int r = k * ROWS + lane / PIECES, c = (lane % PIECES) ^ Tile<DP>::swizzle(r);
+    const uint32_t off = (uint32_t)min(r, left) * (uint32_t)(4 * stride) + (4 * c < n ? 16 * c : 0);
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds + k * 1024));
+  }
+}
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+// The same through registers, for rows that are not whole 16-byte pieces; zero past the end.
+template <int DP, int THREADS>
+__device__ __forceinline__ void tile_by_hand(float* tile, const float* x, int64_t stride, int r0, int rows, int n) {
+  for (int e = threadIdx.x; e < kTile * DP; e += THREADS) {
+    const int r = e / DP, d = e % DP;
+    const float u = x[(int64_t)min(r0 + r, rows - 1) * stride + min(d, n - 1)];
+    tile[Tile<DP>::place(r, d / 4) + d % 4] = r0 + r < rows && d < n ? u : 0.0f;
+  }
 }
 
 // ---- sums over a segment -----------------------------------------------------------------------------
@@ -109,54 +161,82 @@ struct SumsArgs {
   Marks m;
   Rows x, y;                       // x: k or q, y: v or dy
   int H, share, segs, n, ny;       // query heads, those that share a row of x and y (1: none); features
-  bool back, wide;                 // back: of q and dy, weights c, else of k and v, weights e
+  bool back;                       // back: of q and dy, weights c, else of k and v, weights e
   float scale;
   const float* rate;
   float *sums, *stay;              // [segs][B * H][n][ny], [segs][B * H]
 };
-template <int DP>
+template <int DP, bool WIDE>
 __global__ __launch_bounds__(256) void linear_sums(SumsArgs A) {
-  constexpr int LD = DP + 4, NB = DP / 16, PER = NB * NB / 4;
-  __shared__ __align__(16) float xs[kTile * LD], ys[kTile * LD];
-  __shared__ int since[kSeg], waves[4];
+  using L = Tile<DP>;
+  constexpr int HB = DP / 32;      // a wavefront takes a quarter of the sums
+  __shared__ __align__(16) float xs[2][L::FLOATS], ys[2][L::FLOATS];
+  __shared__ int since[kSeg];
   __shared__ float weight[kSeg];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, l = lane & 15;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15;
   const int seg = blockIdx.x % A.segs, bh = blockIdx.x / A.segs, b = bh / A.H, h = bh % A.H, s0 = seg * kSeg;
   const int n = count_of(A.m, b);
-  mark(A.m, b, s0, n, since, waves);
-  const Ends e = ends(since, s0, n);
-  const float rate = A.rate[h];
-  weight[tid] = s0 + tid > e.last ? 0.0f : A.back ? A.scale * comes(since, s0, s0 + tid, rate) : leaves(e, since, s0, s0 + tid, rate);
   const float* x = A.x.p + b * A.x.b + (h / A.share) * A.x.h;
   const float* y = A.y.p + b * A.y.b + (h / A.share) * A.y.h;
-  auto counts = [&](int t) { return weight[t - s0] != 0; };
-  f32x4 acc[PER];
+  const int stop = A.y.p ? min(s0 + kSeg, n) : s0;
+  auto fetch = [&](int t0, int buf) {
+    if (WIDE) {
+      tile_to_lds<DP, 4>(x, A.x.t, t0, A.m.T, A.n, lds_address(xs[buf]), w);
+      tile_to_lds<DP, 4>(y, A.y.t, t0, A.m.T, A.ny, lds_address(ys[buf]), w);
+    } else {
+      tile_by_hand<DP, 256>(xs[buf], x, A.x.t, t0, A.m.T, A.n);
+      tile_by_hand<DP, 256>(ys[buf], y, A.y.t, t0, A.m.T, A.ny);
+    }
+  };
+  const float rate = scalar(A.rate[h]);
+  mark(A.m, b, s0, n, since);
+  const Ends e = ends(since, s0, n);
+  if (s0 < stop) fetch(s0, 0);
+  if (tid < kSeg)
+    weight[tid] = s0 + tid > e.last ? 0.0f : A.back ? A.scale * comes(since, s0, s0 + tid, rate) : leaves(e, since, s0, s0 + tid, rate);
+  const int dx = (w >> 1) * HB, dy = (w & 1) * HB;
+  f32x4 acc[HB][HB];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) acc[i] = f32x4{};
-  const int stop = A.y.p ? e.last : s0 - 1;
-  for (int t0 = s0; t0 <= stop; t0 += kTile) {
+  for (int i = 0; i < HB; ++i)
+#pragma unroll
+    for (int j = 0; j < HB; ++j) acc[i][j] = f32x4{};
+  for (int t0 = s0, buf = 0; t0 < stop; t0 += kTile, buf ^= 1) {
+    if (WIDE) loads_done();
     __syncthreads();
-    stage<DP>(xs, x, A.x.t, t0, A.m.T, A.n, A.wide, counts);
-    stage<DP>(ys, y, A.y.t, t0, A.m.T, A.ny, A.wide, counts);
-    __syncthreads();
+    if (t0 + kTile < stop) fetch(t0 + kTile, buf ^ 1);
+    const float *X = xs[buf], *Y = ys[buf];
+    float u[2][HB], v[2][HB];
+    auto read = [&](int k) {       // positions t0 + 4 k + g, ahead of their use by one step; weight 0: whatever they hold
+      const int r = 4 * k + g;
+      const float c = weight[t0 - s0 + r];
 #pragma unroll
-    for (int k = 0; k < kTile; k += 4) {       // positions t0 + k + g
-      const float c = weight[t0 - s0 + k + g];
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int id = w * PER + i, dx = id / NB, dy = id % NB;
-        acc[i] = mfma(xs[(k + g) * LD + 16 * dx + l] * c, ys[(k + g) * LD + 16 * dy + l], acc[i]);
+      for (int i = 0; i < HB; ++i) {
+        const float a = X[L::place(r, 4 * (dx + i) + l / 4) + l % 4], z = Y[L::place(r, 4 * (dy + i) + l / 4) + l % 4];
+        u[k & 1][i] = c == 0 ? 0.0f : a * c;
+        v[k & 1][i] = c == 0 ? 0.0f : z;
       }
+    };
+    read(0);
+#pragma unroll
+    for (int k = 0; k < kTile / 4; ++k) {
+      if (k + 1 < kTile / 4) read(k + 1);
+#pragma unroll
+      for (int i = 0; i < HB; ++i)
+#pragma unroll
+        for (int j = 0; j < HB; ++j) acc[i][j] = mfma(u[k & 1][i], v[k & 1][j], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   const int64_t at = (int64_t)seg * (gridDim.x / A.segs) + bh;
   float* out = A.sums + at * A.n * A.ny;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int id = w * PER + i, d = 16 * (id / NB) + 4 * g, c = 16 * (id % NB) + l;
+  for (int i = 0; i < HB; ++i)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) if (d + q < A.n && c < A.ny) out[(d + q) * A.ny + c] = acc[i][q];
-  }
+    for (int j = 0; j < HB; ++j) {
+      const int d = 16 * (dx + i) + 4 * g, c = 16 * (dy + j) + l;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) if (d + q < A.n && c < A.ny) out[(d + q) * A.ny + c] = acc[i][j][q];
+    }
   if (tid == 0) A.stay[at] = stays(e, s0, rate);
 }
 
@@ -188,176 +268,478 @@ __global__ __launch_bounds__(256) void linear_join(JoinArgs A) {
 
 // ---- results from pairs and states -----------------------------------------------------------------------
 
-struct Pairs {
-  Rows rows, x, z, out;            // row r with x_s, weights on z_s
-  int heads, group, share;         // heads of `rows`; those of x and z that a row meets in turn; rows' heads that share one of x
-  int n, nz;                       // features of rows and x; of z and out
-  bool back, transposed;           // back: pairs with later positions; transposed: m is [nz][n], else [n][nz]
-  const float *m, *edge;           // states [segs][B * H][.], or null; at the first segment (back: last) this one, or null
-  float pairs, states;             // factors of both parts
+// One sum of the form above.
+struct Sum {
+  Rows rows, out, x, z;            // rows, x and z may be absent (null): zeros, no pairs
+  int n, nz;                       // features of rows and x; of out and z
+  bool across;                     // M's rows are out's features, else rows' features
 };
 struct PairsArgs {
   Marks m;
-  int B, H, segs, blocks;
-  bool wide;
-  const float* rate;
-  Pairs p[3];
+  Sum sum[2];
+  int sums, B, H, segs, blocks;    // blocks: of a head
+  int heads, group, share;         // heads of `rows`; back: those of x and z that a row meets in turn; else rows' heads that share one of x
+  const float *states, *edge;      // [segs][B * H][D][Dv]; at the first segment (back: last) this one, or null
+  int D, Dv;
+  float by_pair, by_state;         // factors of both parts
+  const float *rate, *any;         // any: some address, for rows that are absent
 };
-template <int DP>
-__global__ __launch_bounds__(256) void linear_pairs(PairsArgs A) {
-  constexpr int LD = DP + 4, C = DP / 16;
-  __shared__ __align__(16) float xs[kTile * LD], zs[kTile * LD];
-  __shared__ int since[kSeg], waves[4];
-  const Pairs p = A.p[blockIdx.y];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, l = lane & 15;
-  const int blk = blockIdx.x % A.blocks, bh = blockIdx.x / A.blocks, b = bh / p.heads, head = bh % p.heads;
-  if (b >= A.B) return;
-  const int T = A.m.T, r0 = blk * kRows, seg = r0 / kSeg, s0 = seg * kSeg, n = count_of(A.m, b);
-  mark(A.m, b, s0, n, since, waves);
-  const Ends end = ends(since, s0, n);
-  const int r = r0 + 16 * w + l;
-  const bool here = p.rows.p && r < T && since[r - s0] != kNever;
-  auto there = [&](int t) { return since[t - s0] != kNever; };
+__device__ __forceinline__ const float* row_at(const Rows& x, int b, int head, int t) { return x.p + b * x.b + head * x.h + (int64_t)t * x.t; }
+
+// What one block computes: rows [r0, ..) of a head.
+struct Place {
+  int b, head, r0, seg, s0, n;     // n: positions that are there
+  int h0, group;                   // the first head of x and z, and how many
+  const float* M;                  // state of h0, or null
+  int from, to;                    // positions of x and z
+};
+template <bool BACK>
+__device__ __forceinline__ Place place_of(const PairsArgs& p, const Sum& s, int unit, int rows) {
+  Place o;
+  const int blk = unit % p.blocks, bh = unit / p.blocks;
+  o.b = bh / p.heads;
+  o.head = bh % p.heads;
+  o.r0 = blk * rows;
+  o.seg = o.r0 / kSeg;
+  o.s0 = o.seg * kSeg;
+  o.n = count_of(p.m, o.b);
+  o.h0 = BACK ? o.head * p.group : o.head;
+  o.group = BACK ? p.group : 1;
+  const bool border = BACK ? o.seg == p.segs - 1 : o.seg == 0;
+  const int64_t each = (int64_t)p.D * p.Dv;
+  o.M = border ? p.edge : p.states + (int64_t)o.seg * p.B * p.H * each;
+  if (o.M) o.M += ((int64_t)o.b * p.H + o.h0) * each;
+  o.from = BACK ? o.r0 : o.s0;
+  o.to = s.x.p && s.z.p ? min(BACK ? o.s0 + kSeg : o.r0 + rows, o.n) : 0;
+  return o;
+}
+
+// A wavefront's rows [w0, w0 + 16) pair by pair, a lane a pair or one or two features of the result.
+template <bool BACK>
+__device__ __forceinline__ void plain_rows(const PairsArgs& p, const Sum& s, const Place& o, int w0, const int* since) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (int r = w0; r < min(w0 + 16, p.m.T); ++r) {
+    const int mine = since[r - o.s0];
+    if (mine == kNever || !s.rows.p) continue;
+    const float* row = row_at(s.rows, o.b, o.head, r);
+    float acc[2] = {0, 0};
+#pragma unroll 1
+    for (int gi = 0; gi < o.group; ++gi) {
+      const int h = o.h0 + gi, hx = BACK ? h : h / p.share;
+      const float rate = p.rate[h];
+      const float coef = p.by_state * (BACK ? leaves(ends(since, o.s0, o.n), since, o.s0, r, rate) : comes(since, o.s0, r, rate));
+      if (o.M && coef != 0) {
+        const float* M = o.M + (int64_t)gi * p.D * p.Dv;
+#pragma unroll 1
+        for (int e = 0; e < s.n; ++e)
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            const int d = 64 * a + lane;
+            if (d < s.nz) acc[a] = fmaf(row[e] * coef, s.across ? M[d * p.Dv + e] : M[e * p.Dv + d], acc[a]);
+          }
+      }
+#pragma unroll 1
+      for (int c = o.from; c < o.to; c += 64) {
+        const int t = c + lane, i = BACK ? t : r, j = BACK ? r : t;
+        float f = 0;
+        if (t < o.to && since[t - o.s0] != kNever && j <= i && j >= (BACK ? since[t - o.s0] : mine)) {
+          f = power(rate, i - j) * p.by_pair;
+          if (f != 0) {
+            const float* x = row_at(s.x, o.b, hx, t);
+            float dot = 0;
+#pragma unroll 1
+            for (int d = 0; d < s.n; ++d) dot = fmaf(x[d], row[d], dot);
+            f *= dot;
+          }
+        }
+#pragma unroll 1
+        for (int z = 0; z < min(64, o.to - c); ++z) {
+          const float x = __shfl(f, z);
+          if (x == 0) continue;
+          const float* Z = row_at(s.z, o.b, hx, c + z);
+#pragma unroll
+          for (int a = 0; a < 2; ++a) if (64 * a + lane < s.nz) acc[a] = fmaf(x, Z[64 * a + lane], acc[a]);
+        }
+      }
+    }
+    float* out = s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) if (64 * a + lane < s.nz) out[64 * a + lane] = acc[a];
+  }
+}
+
+// A wavefront's 16 rows: B fragments, and results. A fragment is read one step ahead of its use.
+template <int DP, bool WIDE>
+struct Own {
+  using L = Tile<DP>;
+  static constexpr int C = DP / 16;
   float row[C][4];
-  {
-    const float* at = p.rows.p + b * p.rows.b + head * p.rows.h + (int64_t)min(r, T - 1) * p.rows.t;
+  f32x4 acc[C];
+  __device__ __forceinline__ void load(const float* at, bool here, int n, int g) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int d = 16 * c + 4 * g;
-      f32x4 u = {};
-      if (here) {
-        if (A.wide) {
-          if (d < p.n) u = *(const f32x4*)(at + d);
-        } else {
+      f32x4 u;
+      if (WIDE) {
+        u = *(const f32x4*)(at + (d < n ? d : 0));
+      } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) if (d + q < p.n) u[q] = at[d + q];
-        }
+        for (int q = 0; q < 4; ++q) u[q] = at[min(d + q, n - 1)];
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) row[c][q] = u[q];
+      for (int q = 0; q < 4; ++q) row[c][q] = here && d + (WIDE ? 0 : q) < n ? u[q] : 0.0f;
+      acc[c] = f32x4{};
     }
   }
-  f32x4 acc[C];
+  // tile rows times own rows: x[q] of tile row 16 (q / 4) + 4 g + q % 4
+  __device__ __forceinline__ void dots(const float* tile, float (&x)[8], int g, int l) const {
+    f32x4 s[2] = {}, u[2][2];
+    int at[4];
+    L::by_piece(at, L::opaque(16 * g + l));
+    auto read = [&](int c) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) acc[c] = f32x4{};
-  // x[k][q]: weight of tile row 16 k + 4 g + q on this lane's row. odd: the tile has infinities or NaN, which must not reach the
-  // rows whose weight on them is 0.
-  auto add = [&](const float (&x)[2][4], bool odd) {
-    if (__builtin_expect(odd, 0)) {
+      for (int k = 0; k < 2; ++k) u[c & 1][k] = *(const f32x4*)(tile + at[c % 4] + (16 * k * L::PITCH + L::far(c)));
+    };
+    read(0);
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll 1
-          for (int o = 0; o < 4; ++o) {
-            const float f = __shfl(x[k][q], 16 * o + l);
-            if (f == 0) continue;
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[c][e] = fmaf(f, zs[(16 * k + 4 * o + q) * LD + 16 * c + 4 * g + e], acc[c][e]);
-          }
-      return;
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int c = 0; c < C; ++c) {
+      if (c + 1 < C) read(c + 1);
 #pragma unroll
       for (int q = 0; q < 4; ++q)
 #pragma unroll
-        for (int c = 0; c < C; ++c) acc[c] = mfma(zs[(16 * k + 4 * g + q) * LD + 16 * c + l], x[k][q], acc[c]);
-  };
-  for (int gi = 0; gi < p.group; ++gi) {
-    const int h = p.back ? head * p.group + gi : head, hx = h / p.share;
-    const float rate = A.rate[h];
-    const bool border = p.back ? seg == A.segs - 1 : seg == 0;
-    const float* m = border ? p.edge : p.m + ((int64_t)seg * A.B * A.H) * p.n * p.nz;
-    if (m) {
-      m += ((int64_t)b * A.H + h) * p.n * p.nz;
-      float coef = 0;
-      if (here) coef = p.states * (p.back ? leaves(end, since, s0, r, rate) : comes(since, s0, r, rate));
-      for (int e0 = 0; e0 < p.n; e0 += kTile) {
-        __syncthreads();
-        bool odd = false;
-        for (int e = tid; e < kTile * DP; e += 256) {
-          const int i = p.transposed ? e % kTile : e / DP, d = p.transposed ? e / kTile : e % DP;
-          float u = 0;
-          if (e0 + i < p.n && d < p.nz) u = p.transposed ? m[d * p.n + e0 + i] : m[(e0 + i) * p.nz + d];
-          odd |= !(fabsf(u) < INFINITY);
-          zs[i * LD + d] = u;
-        }
-        odd = __syncthreads_or(odd);
-        float x[2][4];
-#pragma unroll
-        for (int c = 0; c < C; c += 2) {
-          if (16 * c != e0) continue;
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) x[k][q] = coef == 0 ? 0.0f : row[c + k][q] * coef;
-        }
-        add(x, odd);
-      }
+        for (int k = 0; k < 2; ++k) s[k] = mfma(u[c & 1][k][q], row[c][q], s[k]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    const float* px = p.x.p + b * p.x.b + hx * p.x.h;
-    const float* pz = p.z.p + b * p.z.b + hx * p.z.h;
-    const int from = p.back ? r0 : s0, to = p.x.p && p.z.p ? min(p.back ? s0 + kSeg : r0 + kRows, n) : 0;
-    for (int t0 = from; t0 < to; t0 += kTile) {
-      __syncthreads();
-      stage<DP>(xs, px, p.x.t, t0, T, p.n, A.wide, there);
-      const bool odd = __syncthreads_or(stage<DP>(zs, pz, p.z.t, t0, T, p.nz, A.wide, there));
-      const int w0 = r0 + 16 * w;
-      if (p.back ? t0 + kTile <= w0 : t0 > w0 + 15) continue;
-      f32x4 s[2] = {};
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+    for (int q = 0; q < 8; ++q) x[q] = s[q / 4][q % 4];
+  }
+  // acc += weights x on the tile's rows
+  __device__ __forceinline__ void add(const float* tile, const float (&x)[8], int g, int l) {
+    constexpr int PART = C % 4 == 0 ? 4 : C % 3 == 0 ? 3 : C, PARTS = C / PART;   // MFMAs a step
+    float u[2][PART];
+    int row_[4], column[4];
+    if constexpr (DP > 32) L::by_column(row_, column, L::opaque(16 * g + l));
+    auto read = [&](int step) {
+      const int i = step / PARTS;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const f32x4 u = *(const f32x4*)(xs + (16 * k + l) * LD + 16 * c + 4 * g);
+      for (int e = 0; e < PART; ++e) {
+        const int c = step % PARTS * PART + e;
+        if constexpr (DP > 32) u[step & 1][e] = tile[row_[i % 4] + column[c % 4] + (16 * (i / 4) * L::PITCH + L::far(c))];
+        else u[step & 1][e] = tile[16 * (i / 4) * L::PITCH + L::place(4 * g + i % 4, 4 * c + l / 4) + l % 4];
+      }
+    };
+    read(0);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) s[k] = mfma(u[q], row[c][q], s[k]);
-        }
-      float x[2][4];
+    for (int step = 0; step < 8 * PARTS; ++step) {
+      if (step + 1 < 8 * PARTS) read(step + 1);
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int t = t0 + 16 * k + 4 * g + q, i = p.back ? t : r, j = p.back ? r : t;
-          const bool seen = here && t < n && j <= i && j >= since[i - s0];
-          x[k][q] = seen ? s[k][q] * power(rate, i - j) * p.pairs : 0.0f;
-        }
-      add(x, odd);
+      for (int e = 0; e < PART; ++e) {
+        const int c = step % PARTS * PART + e;
+        acc[c] = mfma(u[step & 1][e], x[step / PARTS], acc[c]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
-  if (r >= T) return;
-  float* out = p.out.p + b * p.out.b + head * p.out.h + (int64_t)r * p.out.t;
+  // acc += what the rows [m0, m0 + 32) of M in the tile give: `across`, features m0.. of the result, else weights of features m0..
+  template <bool ACROSS>
+  __device__ __forceinline__ void state(const float* tile, int m0, float coef, int g, int l) {
+    float x[8] = {};
+    if constexpr (ACROSS) {
+      dots(tile, x, g, l);
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int d = 16 * c + 4 * g;
-    const f32x4 u = here ? acc[c] : f32x4{};
-    if (A.wide) {
-      if (d < p.nz) *(f32x4*)(out + d) = u;
+      for (int c = 0; c < C; c += 2)
+        if (16 * c == m0)
+#pragma unroll
+          for (int q = 0; q < 8; ++q) acc[c + q / 4][q % 4] = fmaf(coef, x[q], acc[c + q / 4][q % 4]);
     } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) if (d + q < p.nz) out[d + q] = u[q];
+      for (int c = 0; c < C; c += 2)
+        if (16 * c == m0)
+#pragma unroll
+          for (int q = 0; q < 8; ++q) x[q] = row[c + q / 4][q % 4] * coef;
+      add(tile, x, g, l);
     }
+  }
+  // Waits for the rows here: left to the compiler, the wait stands in the loop, and there it waits for the next tile too.
+  __device__ __forceinline__ void arrived() {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(row[c][q]));
+  }
+  // Stores the rows; whether they are all finite.
+  __device__ __forceinline__ bool store(float* out, bool in, bool here, int n, int g) const {
+    float bad = 0;                 // NaN for infinities and NaN
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int d = 16 * c + 4 * g;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) bad = fmaf(acc[c][q], 0.0f, bad);
+      const f32x4 u = here ? acc[c] : f32x4{};
+      if (!in) continue;
+      if (WIDE) {
+        if (d < n) *(f32x4*)(out + d) = u;
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) if (d + q < n) out[d + q] = u[q];
+      }
+    }
+    return !__any(bad != bad);
+  }
+};
+// Weights of the pairs of row r and tile rows t0 + 16 (q / 4) + 4 g + q % 4; mine: r's mark.
+template <bool BACK>
+__device__ __forceinline__ void weights(float (&x)[8], const PairsArgs& p, const Place& o, float rate, int w0, int r, int t0, int mine,
+                                        const int* since, int g) {
+  const int far = BACK ? t0 + 4 * g - r : r - t0 - 4 * g;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) x[q] = power(rate, BACK ? far + 16 * (q / 4) + q % 4 : far - 16 * (q / 4) - q % 4) * p.by_pair;
+  // all pairs count where there are no documents and the tile is on one side of the rows
+  if (p.m.documents || (BACK ? t0 < w0 + 15 || t0 + kTile > o.n : t0 + kTile - 1 > w0) || w0 + 16 > o.n) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int t = t0 + 16 * (q / 4) + 4 * g + q % 4, i = BACK ? t : r, j = BACK ? r : t;
+      const int from = since[t - o.s0];
+      const bool seen = (from != kNever) & (j <= i) & (j >= (BACK ? from : mine));
+      x[q] = seen ? x[q] : 0.0f;
+    }
+  }
+}
+
+// W wavefronts of 16 rows. The tiles of M, then those of the pairs, one after another; the next one travels to the other half of LDS
+// while this one is multiplied, so that a tile costs one barrier. Four wavefronts a SIMD: their products, weights and waits overlap.
+template <int DP, int W, bool BACK, bool ACROSS>
+__device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int unit, float (&lds)[2][2][Tile<DP>::FLOATS], int (&since)[kSeg]) {
+  using L = Tile<DP>;
+  const Place o = place_of<BACK>(p, s, unit, 16 * W);
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15;
+  const int T = p.m.T, w0 = o.r0 + 16 * w, r = w0 + l;
+  const int mtiles = o.M ? (p.D + kTile - 1) / kTile : 0, count = mtiles + (o.from < o.to ? (o.to - o.from + kTile - 1) / kTile : 0);
+  const int hx = BACK ? o.h0 : o.h0 / p.share;
+  const float *M = o.M, *X = row_at(s.x, o.b, hx, 0), *Z = row_at(s.z, o.b, hx, 0);
+  const uint32_t base = lds_address(lds);
+  auto fetch = [&](int k, int buf) {   // a head's tile k: of its M, then of its pairs
+    const uint32_t to = base + buf * (8 * L::FLOATS);
+    if (k < mtiles) {
+      tile_to_lds<DP, W>(M, p.Dv, k * kTile, p.D, p.Dv, to, w);
+    } else {
+      const int t0 = o.from + (k - mtiles) * kTile;
+      tile_to_lds<DP, W>(Z, s.z.t, t0, T, s.nz, to, w);
+      tile_to_lds<DP, W>(X, s.x.t, t0, T, s.n, to + 4 * L::FLOATS, w);
+    }
+  };
+  if (count) fetch(0, 0);
+  Own<DP, true> own;
+  mark(p.m, o.b, o.s0, o.n, since);
+  const Ends end = ends(since, o.s0, o.n);
+  const int mine = r < T ? since[r - o.s0] : kNever;
+  const bool here = mine != kNever;
+  own.load(s.rows.p ? row_at(s.rows, o.b, o.head, min(r, T - 1)) : p.any, here && s.rows.p, s.n, g);
+  own.arrived();
+  const int steps = count * o.group;
+  float rate = 0, coef = 0;
+  for (int step = 0, k = 0, h = o.h0, buf = 0; step < steps; ++step, buf ^= 1) {
+    if (k == 0) {
+      rate = scalar(p.rate[h]);
+      coef = here ? p.by_state * (BACK ? leaves(end, since, o.s0, r, rate) : comes(since, o.s0, r, rate)) : 0.0f;
+    }
+    loads_done();
+    __syncthreads();
+    const int k1 = k + 1 < count ? k + 1 : 0;
+    if (BACK && k1 == 0) {
+      M += (int64_t)p.D * p.Dv;
+      X += s.x.h;
+      Z += s.z.h;
+      ++h;
+    }
+    if (step + 1 < steps) fetch(k1, buf ^ 1);
+    const float *z_tile = lds[buf][0], *x_tile = lds[buf][1];
+    if (k < mtiles) {
+      own.template state<ACROSS>(z_tile, k * kTile, coef, g, l);
+    } else {
+      const int t0 = o.from + (k - mtiles) * kTile;
+      if (BACK ? t0 + kTile > w0 : t0 <= w0 + 15) {
+        float x[8], f[8];
+        own.dots(x_tile, x, g, l);
+        weights<BACK>(f, p, o, rate, w0, r, t0, mine, since, g);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[q] = f[q] == 0 ? 0.0f : x[q] * f[q];
+        own.add(z_tile, x, g, l);
+      }
+    }
+    k = k1;
+  }
+  const bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here, s.nz, g);
+  if (__builtin_expect(!fine, 0)) plain_rows<BACK>(p, s, o, w0, since);
+}
+template <int DP, int W, bool BACK>
+__global__ __launch_bounds__(64 * W, 2) void linear_tiles(PairsArgs p) {
+  __shared__ __align__(16) float lds[2][2][Tile<DP>::FLOATS];
+  __shared__ int since[kSeg];
+  // both sums of a place run one after the other on one XCD (blocks go to the 8 XCDs in turn), whose L2 then has their tiles
+  const int id = blockIdx.x / 8, unit = (id / p.sums) * 8 + blockIdx.x % 8;
+  if (unit >= p.blocks * p.B * p.heads) return;
+  const Sum& s = p.sum[id % p.sums];
+  if (s.across) walk_tiles<DP, W, BACK, true>(p, s, unit, lds, since);
+  else walk_tiles<DP, W, BACK, false>(p, s, unit, lds, since);
+}
+
+// The same for any alignment and number of features, tile by tile.
+template <int DP, bool BACK>
+__global__ __launch_bounds__(256) void linear_pairs(PairsArgs p) {
+  using L = Tile<DP>;
+  __shared__ __align__(16) float x_tile[L::FLOATS], z_tile[L::FLOATS];
+  __shared__ int since[kSeg];
+  const Sum& s = p.sum[blockIdx.y];
+  const Place o = place_of<BACK>(p, s, blockIdx.x, 64);
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, l = lane & 15;
+  const int T = p.m.T, w0 = o.r0 + 16 * w, r = w0 + l;
+  mark(p.m, o.b, o.s0, o.n, since);
+  const Ends end = ends(since, o.s0, o.n);
+  const int mine = r < T ? since[r - o.s0] : kNever;
+  const bool here = mine != kNever;
+  Own<DP, false> own;
+  own.load(s.rows.p ? row_at(s.rows, o.b, o.head, min(r, T - 1)) : p.any, here && s.rows.p, s.n, g);
+  for (int gi = 0; gi < o.group; ++gi) {
+    const int h = o.h0 + gi, hx = BACK ? h : h / p.share;
+    const float rate = p.rate[h];
+    if (o.M) {
+      const float coef = here ? p.by_state * (BACK ? leaves(end, since, o.s0, r, rate) : comes(since, o.s0, r, rate)) : 0.0f;
+      for (int m0 = 0; m0 < p.D; m0 += kTile) {
+        __syncthreads();
+        tile_by_hand<DP, 256>(z_tile, o.M + (int64_t)gi * p.D * p.Dv, p.Dv, m0, p.D, p.Dv);
+        __syncthreads();
+        if (s.across) own.template state<true>(z_tile, m0, coef, g, l);
+        else own.template state<false>(z_tile, m0, coef, g, l);
+      }
+    }
+    for (int t0 = o.from; t0 < o.to; t0 += kTile) {
+      __syncthreads();
+      tile_by_hand<DP, 256>(x_tile, row_at(s.x, o.b, hx, 0), s.x.t, t0, T, s.n);
+      tile_by_hand<DP, 256>(z_tile, row_at(s.z, o.b, hx, 0), s.z.t, t0, T, s.nz);
+      __syncthreads();
+      if (BACK ? t0 + kTile <= w0 : t0 > w0 + 15) continue;
+      float x[8], f[8];
+      own.dots(x_tile, x, g, l);
+      weights<BACK>(f, p, o, rate, w0, r, t0, mine, since, g);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) x[q] = f[q] == 0 ? 0.0f : x[q] * f[q];
+      own.add(z_tile, x, g, l);
+    }
+  }
+  const bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here, s.nz, g);
+  if (!fine) plain_rows<BACK>(p, s, o, w0, since);
+}
+
+// ---- a few positions ---------------------------------------------------------------------------------------
+
+constexpr int kSteps = 8;          // at most
+
+// A block keeps one head's state: a thread four columns of every RG-th row. Bound by memory: the state is read and written once.
+struct StepsArgs {
+  LinearDesc a;
+  bool wide;                       // of the states
+};
+template <int DP>
+__global__ __launch_bounds__(256) void linear_steps(StepsArgs A) {
+  constexpr int CQ = DP <= 32 ? 8 : DP <= 64 ? 16 : 32, RG = 256 / CQ, R = (DP + RG - 1) / RG;
+  __shared__ float qs[kSteps][DP], ks[kSteps][DP], part[4][kSteps][4 * CQ];
+  __shared__ __align__(16) float vs[kSteps][4 * CQ];
+  const LinearDesc& a = A.a;
+  const int tid = threadIdx.x, cq = tid % CQ, rg = tid / CQ, w = tid >> 6, b = blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.Hk);
+  const int n = count_of({a.documents, a.lengths, a.T}, b);
+  const int64_t state = (int64_t)blockIdx.x * a.D * a.Dv;
+  f32x4 S[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int d = rg + RG * i;
+    S[i] = f32x4{};
+    if (!a.state || d >= a.D) continue;
+    const float* p = a.state + state + (int64_t)d * a.Dv + 4 * cq;
+    if (A.wide) {
+      if (4 * cq < a.Dv) S[i] = *(const f32x4*)p;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) if (4 * cq + q < a.Dv) S[i][q] = p[q];
+    }
+  }
+  const int32_t* doc = a.documents ? a.documents + (int64_t)b * a.T : nullptr;
+  for (int e = tid; e < a.T * DP; e += 256) {
+    const int t = e / DP, d = e % DP;
+    const bool here = t < n && (!doc || doc[t] >= 0);
+    qs[t][d] = here && d < a.D ? a.q.p[b * a.q.b + h * a.q.h + t * a.q.t + d] : 0.0f;
+    ks[t][d] = here && d < a.D ? a.k.p[b * a.k.b + hk * a.k.h + t * a.k.t + d] : 0.0f;
+  }
+  for (int e = tid; e < a.T * 4 * CQ; e += 256) {
+    const int t = e / (4 * CQ), c = e % (4 * CQ);
+    vs[t][c] = t < n && (!doc || doc[t] >= 0) && c < a.Dv ? a.v.p[b * a.v.b + hk * a.v.h + t * a.v.t + c] : 0.0f;
+  }
+  __syncthreads();
+  const float decay = __builtin_amdgcn_exp2f(a.rate[h]);
+  for (int t = 0; t < n; ++t) {
+    const bool fresh = doc && (doc[t] < 0 || (t > 0 && doc[t] != doc[t - 1]));
+    const f32x4 v = *(const f32x4*)&vs[t][4 * cq];
+    f32x4 y = {};
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int d = min(rg + RG * i, DP - 1);
+      const float kd = ks[t][d], qd = qs[t][d];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        S[i][q] = fmaf(kd, v[q], fresh ? 0.0f : decay * S[i][q]);
+        y[q] = fmaf(qd, rg + RG * i < a.D ? S[i][q] : 0.0f, y[q]);
+      }
+    }
+#pragma unroll
+    for (int o = CQ; o < 64; o *= 2)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) y[q] += __shfl_xor(y[q], o);
+    if ((tid & 63) < CQ) *(f32x4*)&part[w][t][4 * cq] = y;
+  }
+  if (a.last) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int d = rg + RG * i;
+      if (d >= a.D) continue;
+      float* p = a.last + state + (int64_t)d * a.Dv + 4 * cq;
+      if (A.wide) {
+        if (4 * cq < a.Dv) *(f32x4*)p = S[i];
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) if (4 * cq + q < a.Dv) p[q] = S[i][q];
+      }
+    }
+  }
+  if (!a.y.p) return;
+  __syncthreads();
+  for (int e = tid; e < a.T * a.Dv; e += 256) {
+    const int t = e / a.Dv, c = e % a.Dv;
+    const bool here = t < n && (!doc || doc[t] >= 0);
+    a.y.p[b * a.y.b + h * a.y.h + t * a.y.t + c] = here ? a.scale * ((part[0][t][c] + part[1][t][c]) + (part[2][t][c] + part[3][t][c])) : 0.0f;
   }
 }
 
 // ---- plans -------------------------------------------------------------------------------------------------
 
-inline bool wide_rows(const Rows& x, int n) { return ((uintptr_t)x.p & 15) == 0 && x.b % 4 == 0 && x.h % 4 == 0 && x.t % 4 == 0 && n % 4 == 0; }
+// Whole 16-byte pieces, and 32 rows within 32-bit offsets.
+inline bool wide_rows(const Rows& x) { return ((uintptr_t)x.p & 15) == 0 && x.b % 4 == 0 && x.h % 4 == 0 && x.t % 4 == 0 && x.t < (1 << 24); }
 inline int segments(const LinearDesc& a) { return (a.T + kSeg - 1) / kSeg; }
 inline int padded(const LinearDesc& a) { return (std::max(a.D, a.Dv) + 31) / 32 * 32; }
 inline int64_t sums_bytes(const LinearDesc& a) {
   const int64_t n = (int64_t)segments(a) * a.B * a.H;
-  return n * a.D * a.Dv * 4 + (n * 4 + 255) / 256 * 256;
+  return (n * a.D * a.Dv * 4 + 255) / 256 * 256 + (n * 4 + 255) / 256 * 256;
 }
-inline Marks marks(const LinearDesc& a) { return {a.documents, a.lengths, a.T}; }
 
+template <int DP>
+void sums(const SumsArgs& s, bool wide, const dim3& grid, hipStream_t st) {
+  if (wide) klaunch(linear_sums<DP, true>, grid, dim3(256), 0, st, s);
+  else klaunch(linear_sums<DP, false>, grid, dim3(256), 0, st, s);
+}
 // States at the borders of all segments (in place of the sums), and the one at the end.
-void states(const LinearDesc& a, const Rows& x, const Rows& y, bool back, const float* first, float* last, float* sums, hipStream_t st) {
+void states(const LinearDesc& a, const Rows& x, const Rows& y, bool back, const float* first, float* last, float* at, hipStream_t st) {
   SumsArgs s{};
-  s.m = marks(a);
+  s.m = {a.documents, a.lengths, a.T};
   s.x = x;
   s.y = y;
   s.H = a.H;
@@ -366,71 +748,103 @@ void states(const LinearDesc& a, const Rows& x, const Rows& y, bool back, const 
   s.n = a.D;
   s.ny = a.Dv;
   s.back = back;
-  s.wide = wide_rows(x, a.D) && wide_rows(y, a.Dv);
   s.scale = a.scale;
   s.rate = a.rate;
-  s.sums = sums;
+  s.sums = at;
   const int64_t rows = (int64_t)a.B * a.H, each = (int64_t)a.D * a.Dv;
-  s.stay = sums + s.segs * rows * each;
+  s.stay = at + (s.segs * rows * each + 63) / 64 * 64;
+  const bool wide = a.D % 4 == 0 && a.Dv % 4 == 0 && wide_rows(x) && wide_rows(y);
   const dim3 grid((unsigned)(rows * s.segs));
   switch (padded(a)) {
-    case 32: klaunch(linear_sums<32>, grid, dim3(256), 0, st, s); break;
-    case 64: klaunch(linear_sums<64>, grid, dim3(256), 0, st, s); break;
-    case 96: klaunch(linear_sums<96>, grid, dim3(256), 0, st, s); break;
-    default: klaunch(linear_sums<128>, grid, dim3(256), 0, st, s);
+    case 32: sums<32>(s, wide, grid, st); break;
+    case 64: sums<64>(s, wide, grid, st); break;
+    case 96: sums<96>(s, wide, grid, st); break;
+    default: sums<128>(s, wide, grid, st);
   }
-  const JoinArgs j{sums, s.stay, first, last, s.segs, rows, each, back};
+  const JoinArgs j{at, s.stay, first, last, s.segs, rows, each, back};
   klaunch(linear_join, dim3((unsigned)((rows * each + 255) / 256)), dim3(256), 0, st, j);
 }
-void pairs(PairsArgs& p, const LinearDesc& a, int jobs, hipStream_t st) {
-  p.m = marks(a);
+
+template <int DP, bool BACK>
+void pairs(PairsArgs& p, bool wide, hipStream_t st) {
+  // 64 rows a block where 128 would leave the card half empty
+  const int rows = wide && (int64_t)((p.m.T + 127) / 128) * p.B * p.heads * p.sums >= 512 ? 128 : 64;
+  p.blocks = (p.m.T + rows - 1) / rows;
+  const int64_t units = (int64_t)p.blocks * p.B * p.heads, grid = (units + 7) / 8 * 8 * p.sums;
+  if (!wide) klaunch(linear_pairs<DP, BACK>, dim3((unsigned)units, p.sums), dim3(256), 0, st, p);
+  else if (rows == 64) klaunch(linear_tiles<DP, 4, BACK>, dim3((unsigned)grid), dim3(256), 0, st, p);
+  else klaunch(linear_tiles<DP, 8, BACK>, dim3((unsigned)grid), dim3(512), 0, st, p);
+}
+template <bool BACK>
+void pairs(PairsArgs p, const LinearDesc& a, const float* at, const float* edge, hipStream_t st) {
+  p.m = {a.documents, a.lengths, a.T};
   p.B = a.B;
   p.H = a.H;
   p.segs = segments(a);
-  p.blocks = (a.T + kRows - 1) / kRows;
+  p.heads = BACK ? a.Hk : a.H;
+  p.group = p.share = a.H / a.Hk;
+  p.states = at;
+  p.edge = edge;
+  p.D = a.D;
+  p.Dv = a.Dv;
+  p.by_pair = a.scale;
+  p.by_state = BACK ? 1.0f : a.scale;
   p.rate = a.rate;
-  p.wide = true;
-  for (int i = 0; i < jobs; ++i)
-    p.wide = p.wide && wide_rows(p.p[i].rows, p.p[i].n) && wide_rows(p.p[i].x, p.p[i].n) && wide_rows(p.p[i].z, p.p[i].nz) &&
-             wide_rows(p.p[i].out, p.p[i].nz);
-  const dim3 grid((unsigned)((int64_t)p.blocks * a.B * a.H), jobs);
+  p.any = a.q.p;
+  bool wide = a.D % 4 == 0 && a.Dv % 4 == 0 && wide_rows(a.q) && (((uintptr_t)at | (uintptr_t)edge) & 15) == 0;
+  for (int i = 0; i < p.sums; ++i) {
+    const Sum& s = p.sum[i];
+    wide = wide && wide_rows(s.rows) && wide_rows(s.out) && wide_rows(s.x) && wide_rows(s.z);
+  }
   switch (padded(a)) {
-    case 32: klaunch(linear_pairs<32>, grid, dim3(256), 0, st, p); break;
-    case 64: klaunch(linear_pairs<64>, grid, dim3(256), 0, st, p); break;
-    case 96: klaunch(linear_pairs<96>, grid, dim3(256), 0, st, p); break;
-    default: klaunch(linear_pairs<128>, grid, dim3(256), 0, st, p);
+    case 32: pairs<32, BACK>(p, wide, st); break;
+    case 64: pairs<64, BACK>(p, wide, st); break;
+    case 96: pairs<96, BACK>(p, wide, st); break;
+    default: pairs<128, BACK>(p, wide, st);
   }
 }
+template <int DP>
+void steps(const StepsArgs& s, hipStream_t st) { klaunch(linear_steps<DP>, dim3((unsigned)(s.a.B * s.a.H)), dim3(256), 0, st, s); }
 
 }  // namespace
 
-int64_t linear_workspace_bytes(const LinearDesc& a) { return sums_bytes(a); }
+int64_t linear_workspace_bytes(const LinearDesc& a) { return a.T <= kSteps ? 0 : sums_bytes(a); }
 
 void linear(const LinearDesc& a, void* work, hipStream_t st) {
-  float* sums = (float*)work;
-  const int G = a.H / a.Hk;
-  if (a.last || (a.y.p && segments(a) > 1)) states(a, a.k, a.v, false, a.state, a.last, sums, st);
+  if (a.T <= kSteps) {
+    const StepsArgs s{a, a.Dv % 4 == 0 && ((uintptr_t)a.state & 15) == 0 && ((uintptr_t)a.last & 15) == 0};
+    switch (padded(a)) {
+      case 32: return steps<32>(s, st);
+      case 64: return steps<64>(s, st);
+      case 96: return steps<96>(s, st);
+      default: return steps<128>(s, st);
+    }
+  }
+  float* at = (float*)work;
+  if (a.last || (a.y.p && segments(a) > 1)) states(a, a.k, a.v, false, a.state, a.last, at, st);
   if (!a.y.p) return;
   PairsArgs p{};
-  p.p[0] = {a.q, a.k, a.v, a.y, a.H, 1, G, a.D, a.Dv, false, false, sums, a.state, a.scale, a.scale};
-  pairs(p, a, 1, st);
+  p.sum[p.sums++] = {a.q, a.y, a.k, a.v, a.D, a.Dv, false};
+  pairs<false>(p, a, at, a.state, st);
 }
 
 int64_t linear_grad_workspace_bytes(const LinearGradDesc& g) { return 2 * sums_bytes(g.a); }
 
 void linear_grad(const LinearGradDesc& g, void* work, hipStream_t st) {
   const LinearDesc& a = g.a;
-  float *S = (float*)work, *Gs = (float*)((char*)work + sums_bytes(a));
+  float *S = (float*)work, *G = (float*)((char*)work + sums_bytes(a));
   const bool several = segments(a) > 1;
-  const int G = a.H / a.Hk;
   if (g.dq.p && several) states(a, a.k, a.v, false, a.state, nullptr, S, st);
-  if (g.dfirst || ((g.dk.p || g.dv.p) && several)) states(a, a.q, g.dy, true, g.dstate, g.dfirst, Gs, st);
+  if (g.dfirst || ((g.dk.p || g.dv.p) && several)) states(a, a.q, g.dy, true, g.dstate, g.dfirst, G, st);
   PairsArgs p{};
-  int jobs = 0;
-  if (g.dq.p) p.p[jobs++] = {g.dy, a.v, a.k, g.dq, a.H, 1, G, a.Dv, a.D, false, true, S, a.state, a.scale, a.scale};
-  if (g.dk.p) p.p[jobs++] = {a.v, g.dy, a.q, g.dk, a.Hk, G, 1, a.Dv, a.D, true, true, Gs, g.dstate, a.scale, 1.0f};
-  if (g.dv.p) p.p[jobs++] = {a.k, a.q, g.dy, g.dv, a.Hk, G, 1, a.D, a.Dv, true, false, Gs, g.dstate, a.scale, 1.0f};
-  if (jobs) pairs(p, a, jobs, st);
+  if (g.dq.p) {
+    p.sum[p.sums++] = {g.dy, g.dq, a.v, a.k, a.Dv, a.D, true};
+    pairs<false>(p, a, S, a.state, st);
+    p.sums = 0;
+  }
+  if (g.dk.p) p.sum[p.sums++] = {a.v, g.dk, g.dy, a.q, a.Dv, a.D, true};
+  if (g.dv.p) p.sum[p.sums++] = {a.k, g.dv, a.q, g.dy, a.D, a.Dv, false};
+  if (p.sums) pairs<true>(p, a, G, g.dstate, st);
 }
 
 }  // namespace tgk

@@ -1,9 +1,16 @@
 // Choice of the next token for gfx950: temperature, top-k, top-p and min-p from a given random number, see ops.py.
 //
-// Every limit keeps a first part of the tokens ordered by (falling logit, rising index), so no sort is needed: a border (key,
-// ties) is found by counting and weighing tokens in bins of their logit's bits. Weights are whole numbers, exp(z) times 2^unit
-// with z = (logit - largest) / temperature in 64 bits and 62 bits for the sum of all: sums do not depend on their order, so
-// counts, borders and the choice agree with each other and repeat, and a weight is off by 2^(-unit-1) of the largest at most.
+// Every limit keeps a first part of the tokens ordered by (falling logit, rising index), so the row is not sorted. Tokens are
+// counted and weighed in bins of their distance to the largest logit; the bin that a limit's border lies in is found by sums over
+// bins, its tokens alone are listed and sorted, and what is kept is told by one bound on (logit, index). Then the weights of what is
+// kept are summed in the vocabulary's order, and the stretch where the sum passes u of all is walked once more.
+//
+// Weights are whole numbers, exp(-z) times 2^unit with z = (largest - logit) / temperature in 64 bits and 62 bits for the sum of
+// all: sums do not depend on their order, so counts, borders and the choice agree with each other and repeat, and a weight is off by
+// 2^(-unit-1) of the largest at most. Beyond some 32 to 43 in z they are 0.
+//
+// A row is read three times, the first time from memory. Many rows: a block takes one, in one launch (sample_one). Few rows of many
+// tokens: several blocks a row, in four launches (sample_tops, sample_bins, sample_list, sample_pick).
 #include <algorithm>
 
 #include "kernels.h"
@@ -13,8 +20,10 @@ namespace tgk {
 namespace {
 
 typedef unsigned long long u64;
-constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 2048;
+constexpr int kBins = 2048;
+constexpr int kList = 2048;                // tokens that are sorted, at most
 constexpr uint32_t kNoKey = 0xffffffffu;   // minus infinity and NaN: never chosen
+constexpr u64 kAll = ~0ull;
 
 // Ascending in falling logits; -0 and 0 are equal.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -23,18 +32,60 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return b & 0x80000000u ? b : ~b & 0x7fffffffu;
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu); }
+__device__ __forceinline__ u64 order_of(uint32_t key, int i) { return (u64)key << 32 | (uint32_t)i; }
 
+// A row, its limits and its largest logit.
 struct Row {
+  const float* x;
+  int V, most, unit;
   float top;                       // largest logit
-  double per;                      // 1 / temperature
-  int unit;
+  double per, p, least, u;         // 1 / temperature; top_p, min_p; the random number
+  bool greedy, by_count, by_mass;  // what limits
 };
-__device__ __forceinline__ double weight(const Row& r, float x) {   // of the largest
-  if (x == r.top) return 1;
-  return exp(((double)x - (double)r.top) * r.per);
+__device__ __forceinline__ Row row_of(const SampleDesc& s, int64_t row, float top) {
+  Row r;
+  r.x = s.logits + row * s.V;
+  r.V = s.V;
+  r.top = top;
+  const double heat = s.temperature ? (double)s.temperature[row] : s.temperature1;
+  r.greedy = !(heat > 0);
+  r.per = r.greedy ? 1 : 1 / heat;
+  r.unit = 62 - (s.V > 1 ? 32 - __clz(s.V - 1) : 0);
+  r.most = s.top_k ? s.top_k[row] : s.top_k1;
+  r.p = s.top_p ? (double)s.top_p[row] : s.top_p1;
+  r.least = s.min_p ? (double)s.min_p[row] : s.min_p1;
+  r.u = s.u[row];
+  r.by_count = r.most > 0 && r.most < s.V;
+  r.by_mass = r.p < 1;
+  return r;
 }
-__device__ __forceinline__ u64 whole(const Row& r, double w) { return (u64)rint(ldexp(w, r.unit)); }
+// The distance to the largest logit in units of the temperature; infinite: no weight.
+__device__ __forceinline__ double distance(const Row& r, float x) {
+  return x == r.top ? 0 : x > -INFINITY ? ((double)r.top - (double)x) * r.per : (double)INFINITY;
+}
+// exp(-z), of z >= 0: 2^-n times the Taylor series of 2^-f for |f| <= 1 / 2, 2^-52 off at most.
+__device__ __forceinline__ double weight(double z) {
+  const double t = fmin(z * 1.44269504088896340736, 2000.0), n = rint(t), f = (n - t) * 0.693147180559945309417;
+  double e = 1.0 / 479001600;
+  const double c[] = {1.0 / 39916800, 1.0 / 3628800, 1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720, 1.0 / 120, 1.0 / 24, 1.0 / 6, 0.5, 1, 1};
+#pragma unroll
+  for (int i = 0; i < 12; ++i) e = fma(e, f, c[i]);
+  return __builtin_amdgcn_ldexp(e, -(int)n);
+}
+__device__ __forceinline__ u64 whole(const Row& r, double w) { return (u64)rint(__builtin_amdgcn_ldexp(w, r.unit)); }
+// Its bin: of equal width, up to where weights are 0; kBins: no weight.
+__device__ __forceinline__ int bin_of(const Row& r, double z, u64 w) {
+  return w == 0 ? kBins : min((int)(z * (kBins / (0.6931471805599454 * (r.unit + 1)))), kBins - 1);
+}
 
+__device__ __forceinline__ u64 wave_min(u64 x) {
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const u64 z = __shfl_xor(x, o);
+    x = z < x ? z : x;
+  }
+  return x;
+}
 __device__ __forceinline__ u64 wave_sum(u64 x) {
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) x += __shfl_xor(x, o);
@@ -49,199 +100,606 @@ __device__ __forceinline__ u64 wave_scan(u64 x) {   // inclusive
   return x;
 }
 
-// The first tokens of the order: those of a key below `key`, and the first `ties` of that key.
+struct Bins {
+  u64 mass[kBins];
+  uint32_t count[kBins];
+};
+// What a block shares while it finds a row's borders and its choice.
+struct Work {
+  u64 list[kList];
+  u64 sums[2][16];
+  u64 found[8];
+  uint32_t listed;
+};
+
+// The first 8 tokens of each kind that a thread asks for at once: f(i, x[i]) for its i of [from, to), `step` apart from `at`.
+template <class F>
+__device__ __forceinline__ void each_token(const float* x, int from, int to, int step, F f) {
+  constexpr int N = 8;
+  for (int i = from; i < to; i += N * step) {
+    float v[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = x[min(i + e * step, to - 1)];
+#pragma unroll
+    for (int e = 0; e < N; ++e) if (i + e * step < to) f(i + e * step, v[e]);
+  }
+}
+
+template <int THREADS>
+__device__ __forceinline__ u64 block_min(u64 x, Work& w) {
+  x = wave_min(x);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) w.sums[0][threadIdx.x >> 6] = x;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < THREADS / 64; ++k) x = w.sums[0][k] < x ? w.sums[0][k] : x;
+  return x;
+}
+// Sums over the bins before this thread's first (it has kBins / THREADS of them), and over all.
+template <int THREADS>
+__device__ __forceinline__ void bin_sums(const Bins& b, Work& w, u64& count, u64& mass, u64& all_count, u64& all_mass) {
+  constexpr int N = kBins / THREADS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  u64 c = 0, m = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    c += b.count[tid * N + i];
+    m += b.mass[tid * N + i];
+  }
+  const u64 cs = wave_scan(c), ms = wave_scan(m);
+  __syncthreads();
+  if (lane == 63) {
+    w.sums[0][wave] = cs;
+    w.sums[1][wave] = ms;
+  }
+  __syncthreads();
+  count = cs - c;
+  mass = ms - m;
+  all_count = all_mass = 0;
+#pragma unroll
+  for (int k = 0; k < THREADS / 64; ++k) {
+    if (k < wave) {
+      count += w.sums[0][k];
+      mass += w.sums[1][k];
+    }
+    all_count += w.sums[0][k];
+    all_mass += w.sums[1][k];
+  }
+}
+
+// What the bins say: the bins [b0, b1] hold every border, `count` and `mass` stand before b0, and `size` tokens are in them. all:
+// the mass that top_p is a part of, or 0 where that ends within these bins (top_k does).
+struct Borders {
+  int b0, b1;
+  u64 count, mass, size, all;
+};
+template <int THREADS>
+__device__ __forceinline__ Borders borders(const Row& r, const Bins& b, Work& w) {
+  constexpr int N = kBins / THREADS;
+  const int tid = threadIdx.x;
+  u64 c0, m0, all_c, all_m;
+  bin_sums<THREADS>(b, w, c0, m0, all_c, all_m);
+  if (tid < 8) w.found[tid] = 0;
+  __syncthreads();
+  const bool counted = r.by_count && all_c > (u64)r.most;
+  // calls f(bin, sums before it, sums with it) for this thread's bins
+  auto each = [&](auto f) {
+    u64 c = c0, m = m0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const u64 c1 = c + b.count[tid * N + i], m1 = m + b.mass[tid * N + i];
+      f(tid * N + i, c, m, c1, m1);
+      c = c1;
+      m = m1;
+    }
+  };
+  if (counted) {
+    each([&](int bin, u64 c, u64 m, u64 c1, u64 m1) {
+      if (c < (u64)r.most && (u64)r.most <= c1) {
+        w.found[0] = bin;
+        w.found[1] = m;
+        w.found[2] = c1;
+      }
+    });
+    __syncthreads();
+  }
+  Borders o = {0, -1, 0, 0, 0, counted ? 0 : all_m};
+  const int kbin = (int)w.found[0];
+  // the least that the total of top-k can be: its border bin is not resolved yet
+  const double target = r.p > 0 ? r.p * (double)(counted ? w.found[1] : all_m) : 0;
+  if (r.by_mass) {
+    each([&](int bin, u64 c, u64 m, u64 c1, u64 m1) {
+      if (((double)m < target || bin == 0) && !((double)m1 < target)) {
+        w.found[3] = bin;
+        w.found[4] = c;
+        w.found[5] = m;
+        w.found[6] = c1;
+      }
+    });
+  } else if (counted) {
+    each([&](int bin, u64 c, u64 m, u64 c1, u64 m1) {
+      if (bin == kbin) {
+        w.found[3] = bin;
+        w.found[4] = c;
+        w.found[5] = m;
+      }
+    });
+  }
+  __syncthreads();
+  if (!r.by_mass && !counted) return o;
+  o.b0 = (int)w.found[3];
+  o.b1 = counted ? kbin : o.b0;
+  o.count = w.found[4];
+  o.mass = w.found[5];
+  o.size = (counted ? w.found[2] : w.found[6]) - o.count;
+  return o;
+}
+
+// The bound of what is kept (an order, inclusive) from the sorted tokens of the border's bins. `n` of them, in w.list.
+template <int THREADS>
+__device__ __forceinline__ u64 bound_of_list(const Row& r, const Borders& o, int n, Work& w) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int n2 = 64;
+  while (n2 < n) n2 *= 2;
+  for (int i = n + tid; i < n2; i += THREADS) w.list[i] = kAll;
+  __syncthreads();
+  for (int size = 2; size <= n2; size *= 2)   // bitonic
+    for (int half = size / 2; half > 0; half /= 2) {
+      for (int t = tid; t < n2 / 2; t += THREADS) {
+        const int i = 2 * t - (t & (half - 1)), j = i + half;
+        const u64 a = w.list[i], b = w.list[j];
+        if ((a > b) == ((i & size) == 0)) {
+          w.list[i] = b;
+          w.list[j] = a;
+        }
+      }
+      __syncthreads();
+    }
+  // a thread has N neighbours; those that top-k keeps
+  constexpr int N = kList / THREADS;
+  const int kept = r.by_count ? (int)min((u64)n, (u64)r.most - min((u64)r.most, o.count)) : n;
+  u64 m[N], sum = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const int i = tid * N + e;
+    m[e] = i < kept ? whole(r, weight(distance(r, value_of((uint32_t)(w.list[i] >> 32))))) : 0;
+    sum += m[e];
+  }
+  const u64 scan = wave_scan(sum);
+  if (lane == 63) w.sums[0][wave] = scan;
+  __syncthreads();
+  u64 before = o.mass + scan - sum, total = o.mass;
+#pragma unroll
+  for (int k = 0; k < THREADS / 64; ++k) {
+    if (k < wave) before += w.sums[0][k];
+    total += w.sums[0][k];
+  }
+  if (o.all) total = o.all;
+  if (tid == 0) w.found[0] = 0;
+  __syncthreads();
+  const double target = r.by_mass ? (r.p > 0 ? r.p * (double)total : 1.0) : (double)INFINITY;
+  int last = 0;                    // one past this thread's last token that is kept
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const int i = tid * N + e;
+    if (i < kept && (double)before < target) last = i + 1;
+    before += m[e];
+  }
+  atomicMax(&w.found[0], (u64)last);
+  __syncthreads();
+  const int end = (int)w.found[0];
+  return end > 0 ? w.list[end - 1] : n > 0 ? w.list[0] - 1 : kAll;
+}
+
+// The same bound without a list, for more tokens than it holds in the border's bins: three levels of the key's bits, each a walk
+// over the row. `within`: of what stands up to this key, and the first `ties` of that key.
 struct Border {
   uint32_t key;
   u64 ties;
 };
-
-struct Bins {
-  u64 mass[kBins];
-  uint32_t count[kBins];
-  u64 sums[kWaves];
-  u64 found[4];
-};
-
-// A border of the order before the border `within`: where the count reaches `most`, or the mass `target` (a token is kept while
-// what stands before it weighs less). *total: the mass of what is kept. Three levels of bits of the key.
-template <bool COUNT>
-__device__ Border find_border(const float* x, int V, const Row& r, Border within, u64 most, double target, Bins& bins, u64* total) {
+template <int THREADS, bool COUNT>
+__device__ __forceinline__ Border find_border(const Row& r, Border within, double target, Bins& b, Work& w, u64* total) {
+  constexpr int N = kBins / THREADS;
   const int tid = threadIdx.x;
   uint32_t lo = 0;                 // keys of the bin that the border lies in: lo ...
   int shift = 32;                  // ... and its first 32 - shift bits
   u64 before = 0, mass_before = 0;
+#pragma unroll 1
   for (int level = 0; level < 3; ++level) {
     const int bits = level < 2 ? 11 : 10, next = shift - bits;
-    for (int i = tid; i < kBins; i += kThreads) {
-      bins.mass[i] = 0;
-      bins.count[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < kBins; i += THREADS) {
+      b.mass[i] = 0;
+      b.count[i] = 0;
     }
     __syncthreads();
-    for (int i = tid; i < V; i += kThreads) {
-      const uint32_t k = key_of(x[i]);
+    for (int i = tid; i < r.V; i += THREADS) {
+      const float v = r.x[i];
+      const uint32_t k = key_of(v);
       if (k == kNoKey || k > within.key || (shift < 32 && (k >> shift) != (lo >> shift))) continue;
       const uint32_t bin = (k >> next) & ((1u << bits) - 1);
-      atomicAdd(&bins.count[bin], 1u);
-      if (k < within.key) atomicAdd(&bins.mass[bin], whole(r, weight(r, x[i])));
+      atomicAdd(&b.count[bin], 1u);
+      if (k < within.key) atomicAdd(&b.mass[bin], whole(r, weight(distance(r, v))));
     }
     __syncthreads();
-    if (tid == 0) {                // the last key's ties that count
-      if (within.key != kNoKey && (shift == 32 || (within.key >> shift) == (lo >> shift))) {
-        const uint32_t bin = (within.key >> next) & ((1u << bits) - 1);
-        bins.mass[bin] += within.ties * whole(r, weight(r, value_of(within.key)));
+    // the last key's ties that count
+    if (tid == 0 && within.key != kNoKey && (shift == 32 || (within.key >> shift) == (lo >> shift)))
+      b.mass[(within.key >> next) & ((1u << bits) - 1)] += within.ties * whole(r, weight(distance(r, value_of(within.key))));
+    if (tid == 0) w.found[0] = kBins;
+    __syncthreads();
+    u64 c, m, all_c, all_m;
+    bin_sums<THREADS>(b, w, c, m, all_c, all_m);
+    u64 c1 = c, m1 = m;
+    int last = -1;                 // the last bin that holds any, and the first that reaches the border
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int bin = tid * N + i;
+      c1 += b.count[bin];
+      m1 += b.mass[bin];
+      if (!b.count[bin]) continue;
+      last = bin;
+      if (COUNT ? before + c1 >= (u64)r.most : !((double)(mass_before + m1) < target)) {
+        atomicMin(&w.found[0], (u64)bin);
+        break;
       }
-      u64 c = before, m = mass_before;
-      int at = 0, last = -1;
-      u64 lc = c, lm = m;
-      for (; at < 1 << bits; ++at) {
-        if (!bins.count[at]) continue;
-        last = at;
-        lc = c;
-        lm = m;
-        c += bins.count[at];
-        m += bins.mass[at];
-        if (COUNT ? c >= most : !((double)m < target)) break;
+    }
+    if (tid == 0) w.found[1] = 0;
+    __syncthreads();
+    if (last >= 0) atomicMax(&w.found[1], (u64)last);
+    __syncthreads();
+    const int border = w.found[0] < kBins ? (int)w.found[0] : (int)w.found[1];
+    __syncthreads();
+    if (border / N == tid) {
+      for (int i = 0; i < border % N; ++i) {
+        c += b.count[tid * N + i];
+        m += b.mass[tid * N + i];
       }
-      bins.found[0] = last;        // the bin of the border, or the last one that holds any
-      bins.found[1] = lc;
-      bins.found[2] = lm;
-      bins.found[3] = last >= 0 ? bins.count[last] : 0;
+      w.found[2] = c;
+      w.found[3] = m;
+      w.found[4] = b.count[border];
     }
     __syncthreads();
-    lo |= (uint32_t)bins.found[0] << next;
-    before = bins.found[1];
-    mass_before = bins.found[2];
+    lo |= (uint32_t)border << next;
+    before += w.found[2];
+    mass_before += w.found[3];
     shift = next;
-    __syncthreads();
   }
-  const u64 w = whole(r, weight(r, value_of(lo)));
-  u64 ties = bins.found[3];        // of key lo, all there are
+  const u64 one = whole(r, weight(distance(r, value_of(lo))));
+  u64 ties = w.found[4];           // of key lo, all there are
   if (lo == within.key) ties = min(ties, within.ties);
   if (COUNT) {
-    ties = min(ties, most - before);
-  } else {
-    u64 keep = 0;                  // those with mass before them below the target
-    if (w == 0) keep = (double)mass_before < target ? ties : 0;
+    ties = min(ties, (u64)r.most - before);
+  } else {                         // those with mass before them below the target
+    u64 keep = 0;
+    if (one == 0) keep = (double)mass_before < target ? ties : 0;
     else {
-      const double room = (target - (double)mass_before) / (double)w;
+      const double room = (target - (double)mass_before) / (double)one;
       keep = room > 0 ? (u64)fmin(ceil(room), (double)ties) : 0;
-      while (keep > 0 && !((double)(mass_before + (keep - 1) * w) < target)) --keep;
-      while (keep < ties && (double)(mass_before + keep * w) < target) ++keep;
+      while (keep > 0 && !((double)(mass_before + (keep - 1) * one) < target)) --keep;
+      while (keep < ties && (double)(mass_before + keep * one) < target) ++keep;
     }
     ties = keep;
   }
-  *total = mass_before + ties * w;
+  *total = mass_before + ties * one;
   return {lo, ties};
 }
-
-// One block a row, several passes over it.
-__global__ __launch_bounds__(kThreads) void sample_rows(SampleDesc s) {
-  __shared__ Bins bins;
-  __shared__ uint32_t tops[kWaves];
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const float* x = s.logits + row * s.V;
-  uint32_t top = kNoKey;
-  for (int i = tid; i < s.V; i += kThreads) top = min(top, key_of(x[i]));
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) top = min(top, (uint32_t)__shfl_xor((int)top, o));
-  if (lane == 0) tops[w] = top;
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kWaves; ++k) top = min(top, tops[k]);
-  if (top == kNoKey) {
-    if (tid == 0) s.token[row] = -1;
-    return;
-  }
-  Row r;
-  r.top = value_of(top);
-  const double heat = s.temperature ? (double)s.temperature[row] : s.temperature1;
-  const bool greedy = !(heat > 0);
-  r.per = greedy ? 1 : 1 / heat;
-  r.unit = 62 - (s.V > 1 ? 32 - __clz(s.V - 1) : 0);
-  const int32_t most = s.top_k ? s.top_k[row] : s.top_k1;
-  const double p = s.top_p ? (double)s.top_p[row] : s.top_p1, least = s.min_p ? (double)s.min_p[row] : s.min_p1, u = s.u[row];
+template <int THREADS>
+__device__ __forceinline__ u64 bound_by_walks(const Row& r, u64 all_mass, Bins& b, Work& w) {
   Border kept = {kNoKey, 0};
-  u64 total = 0;
-  if (greedy) kept = {top, 1};
-  else {
-    if (most > 0 && most < s.V) kept = find_border<true>(x, s.V, r, kept, most, 0, bins, &total);
-    if (p < 1) {
-      if (kept.key == kNoKey) {    // the mass of all
-        u64 m = 0;
-        for (int i = tid; i < s.V; i += kThreads) if (key_of(x[i]) != kNoKey) m += whole(r, weight(r, x[i]));
-        m = wave_sum(m);
-        __syncthreads();
-        if (lane == 0) bins.sums[w] = m;
-        __syncthreads();
-        for (int k = 0; k < kWaves; ++k) total += bins.sums[k];
-      }
-      kept = find_border<false>(x, s.V, r, kept, 0, p > 0 ? p * (double)total : 1.0, bins, &total);
+  u64 total = all_mass;
+  if (r.by_count) kept = find_border<THREADS, true>(r, kept, 0, b, w, &total);
+  if (r.by_mass) kept = find_border<THREADS, false>(r, kept, r.p > 0 ? r.p * (double)total : 1.0, b, w, &total);
+  if (kept.ties == 0) return order_of(kept.key, 0) - 1;
+  // the index of the last tie that is kept: a wavefront takes a stretch
+  constexpr int W = THREADS / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, each = ((r.V + W - 1) / W + 63) / 64 * 64;
+  const int from = min(wave * each, r.V), to = min(from + each, r.V);
+  u64 ties = 0;
+  for (int i = from + lane; i < to; i += 64) ties += key_of(r.x[i]) == kept.key;
+  ties = wave_sum(ties);
+  __syncthreads();
+  if (lane == 0) w.sums[0][wave] = ties;
+  if (tid == 0) w.found[0] = r.V;
+  __syncthreads();
+  u64 before = 0;
+  for (int k = 0; k < wave; ++k) before += w.sums[0][k];
+  if (before < kept.ties && kept.ties <= before + ties) {
+    for (int i0 = from; i0 < to; i0 += 64) {
+      const int i = i0 + lane;
+      const bool tie = i < to && key_of(r.x[i]) == kept.key;
+      const u64 mask = __ballot(tie);
+      if (tie && before + __popcll(mask & ((1ull << lane) - 1)) + 1 == kept.ties) w.found[0] = i;
+      before += __popcll(mask);
     }
   }
-  // each wavefront takes one stretch of the row, 64 tokens a step
-  const int each = ((s.V + kWaves - 1) / kWaves + 63) / 64 * 64, from = min(w * each, s.V), to = min(from + each, s.V);
-  int limit = INT32_MAX;           // tokens of the border's key count below this index
-  if (kept.key != kNoKey) {
-    u64 ties = 0;
-    for (int i = from + lane; i < to; i += 64) ties += key_of(x[i]) == kept.key;
-    ties = wave_sum(ties);
-    __syncthreads();
-    if (lane == 0) bins.sums[w] = ties;
-    if (tid == 0) bins.found[0] = s.V;
-    __syncthreads();
-    u64 before = 0;
-    for (int k = 0; k < w; ++k) before += bins.sums[k];
-    if (before <= kept.ties && kept.ties < before + ties) {
-      for (int i0 = from; i0 < to; i0 += 64) {
-        const int i = i0 + lane;
-        const bool tie = i < to && key_of(x[i]) == kept.key;
-        const u64 mask = __ballot(tie);
-        const u64 at = before + __popcll(mask & ((1ull << lane) - 1));
-        if (tie && at == kept.ties) bins.found[0] = i;
-        before += __popcll(mask);
-        if (before > kept.ties) break;
-      }
-    }
-    __syncthreads();
-    limit = (int)bins.found[0];
-  }
-  auto weigh = [&](int i) -> u64 {
-    if (i >= to) return 0;
-    const float v = x[i];
-    const uint32_t k = key_of(v);
-    if (k == kNoKey || k > kept.key || (k == kept.key && i >= limit)) return 0;
-    const double m = weight(r, v);
-    return m >= least || k == top ? whole(r, m) : 0;
-  };
-  u64 mine = 0;
-  for (int i = from + lane; i - lane < to; i += 64) mine += weigh(i);
-  mine = wave_sum(mine);
   __syncthreads();
-  if (lane == 0) bins.sums[w] = mine;
-  __syncthreads();
-  u64 before = 0, all = 0;
-  for (int k = 0; k < kWaves; ++k) {
-    if (k < w) before += bins.sums[k];
-    all += bins.sums[k];
-  }
-  // passed: sum > u all, as whole numbers; u in [0, 1) leaves the last token's sum, all, to pass
-  const u64 goal = min((u64)fmax(u * (double)all, 0.0), all - 1);
-  if (!(before <= goal && goal < before + mine)) return;
+  return order_of(kept.key, (int)w.found[0]);
+}
+
+// The weight that token i has in the choice.
+__device__ __forceinline__ u64 kept_weight(const Row& r, u64 bound, int i, float x) {
+  const uint32_t k = key_of(x);
+  if (k == kNoKey || order_of(k, i) > bound) return 0;
+  const double z = distance(r, x), w = weight(z);
+  return w >= r.least || z == 0 ? whole(r, w) : 0;
+}
+// Sum of the weights of [from, to), by a wavefront.
+__device__ __forceinline__ u64 stretch_sum(const Row& r, u64 bound, int from, int to) {
+  u64 sum = 0;
+  each_token(r.x, from + (int)(threadIdx.x & 63), to, 64, [&](int i, float x) { sum += kept_weight(r, bound, i, x); });
+  return wave_sum(sum);
+}
+// The token of [from, to) where the sum of weights passes `goal`, by a wavefront.
+__device__ __forceinline__ void choose(const Row& r, u64 bound, int from, int to, u64 goal, int32_t* token) {
+  const int lane = threadIdx.x & 63;
+  u64 before = 0;
   for (int i0 = from; i0 < to; i0 += 64) {
-    const u64 m = weigh(i0 + lane), sum = before + wave_scan(m);
+    const u64 m = i0 + lane < to ? kept_weight(r, bound, i0 + lane, r.x[i0 + lane]) : 0, sum = before + wave_scan(m);
     const u64 passed = __ballot(sum > goal);
     if (passed) {
-      if (lane == __ffsll(passed) - 1) s.token[row] = i0 + lane;
+      if (lane == __ffsll(passed) - 1) *token = i0 + lane;
+      return;
+    }
+    before = __shfl(sum, 63);
+  }
+}
+// Passed: sum > u all, as whole numbers; u in [0, 1) leaves the last token's sum, all, to pass.
+__device__ __forceinline__ u64 goal_of(const Row& r, u64 all) { return min((u64)fmax(r.u * (double)all, 0.0), all - 1); }
+
+// ---- a block a row -------------------------------------------------------------------------------------
+
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_one(SampleDesc s) {
+  constexpr int W = THREADS / 64;
+  __shared__ Bins bins;
+  __shared__ Work w;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  u64 first = kAll;
+  each_token(s.logits + row * s.V, tid, s.V, THREADS, [&](int i, float x) {
+    const u64 o = order_of(key_of(x), i);
+    first = o < first ? o : first;
+  });
+  first = block_min<THREADS>(first, w);
+  const Row r = row_of(s, row, value_of((uint32_t)(first >> 32)));
+  if ((uint32_t)(first >> 32) == kNoKey || r.greedy) {
+    if (tid == 0) s.token[row] = (uint32_t)(first >> 32) == kNoKey ? -1 : (int32_t)(uint32_t)first;
+    return;
+  }
+  u64 bound = kAll;
+  if (r.by_count || r.by_mass) {
+    Borders o = {0, kBins - 1, 0, 0, (u64)s.V, 0};
+    if (s.V > kList) {
+      for (int i = tid; i < kBins; i += THREADS) {
+        bins.mass[i] = 0;
+        bins.count[i] = 0;
+      }
+      __syncthreads();
+      each_token(r.x, tid, s.V, THREADS, [&](int, float x) {
+        const double z = distance(r, x);
+        const u64 m = whole(r, weight(z));
+        const int bin = bin_of(r, z, m);
+        if (bin == kBins) return;
+        atomicAdd(&bins.count[bin], 1u);
+        atomicAdd(&bins.mass[bin], m);
+      });
+      __syncthreads();
+      o = borders<THREADS>(r, bins, w);
+    }
+    if (o.b1 >= 0 && o.size <= kList) {
+      if (tid == 0) w.listed = 0;
+      __syncthreads();
+      each_token(r.x, tid, s.V, THREADS, [&](int i, float x) {
+        const double z = distance(r, x);
+        const int bin = bin_of(r, z, whole(r, weight(z)));
+        if (bin >= o.b0 && bin <= o.b1) w.list[atomicAdd(&w.listed, 1u)] = order_of(key_of(x), i);
+      });
+      __syncthreads();
+      bound = bound_of_list<THREADS>(r, o, (int)w.listed, w);
+    } else if (o.b1 >= 0) {
+      bound = bound_by_walks<THREADS>(r, o.all, bins, w);
+    }
+  }
+  const int each = ((s.V + W - 1) / W + 63) / 64 * 64, from = min(wave * each, s.V), to = min(from + each, s.V);
+  const u64 mine = stretch_sum(r, bound, from, to);
+  __syncthreads();
+  if (lane == 0) w.sums[0][wave] = mine;
+  __syncthreads();
+  u64 before = 0, all = 0;
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    if (k < wave) before += w.sums[0][k];
+    all += w.sums[0][k];
+  }
+  const u64 goal = goal_of(r, all);
+  if (before <= goal && goal < before + mine) choose(r, bound, from, to, goal - before, s.token + row);
+}
+
+// ---- several blocks a row ------------------------------------------------------------------------------
+
+constexpr int kPartThreads = 256, kPartWaves = kPartThreads / 64;
+struct RowSpace {                  // of a row in the workspace
+  Bins bins;
+  u64 list[kList];
+  u64 first, bound, listed, over;
+};
+struct PartArgs {
+  SampleDesc s;
+  int parts, each;                 // tokens of a part, a multiple of 64 a wavefront
+  RowSpace* rows;
+  u64 *tops, *sums;                // [rows][parts], [rows][parts * kPartWaves]
+};
+__device__ __forceinline__ u64 first_of(const PartArgs& a, int64_t row) {
+  u64 first = kAll;
+  for (int k = threadIdx.x & 63; k < a.parts; k += 64) first = min(first, a.tops[row * a.parts + k]);
+  return wave_min(first);
+}
+__global__ __launch_bounds__(kPartThreads) void sample_tops(PartArgs a) {
+  __shared__ Work w;
+  const int part = blockIdx.x;
+  const int64_t row = blockIdx.y;
+  const int tid = threadIdx.x, from = part * a.each, to = min(from + a.each, a.s.V);
+  u64 first = kAll;
+  each_token(a.s.logits + row * a.s.V, from + tid, to, kPartThreads, [&](int i, float x) {
+    const u64 o = order_of(key_of(x), i);
+    first = o < first ? o : first;
+  });
+  first = block_min<kPartThreads>(first, w);
+  if (tid == 0) a.tops[row * a.parts + part] = first;
+  RowSpace& sp = a.rows[row];
+  for (int i = part * kPartThreads + tid; i < kBins; i += a.parts * kPartThreads) {
+    sp.bins.mass[i] = 0;
+    sp.bins.count[i] = 0;
+  }
+  if (part == 0 && tid == 0) sp.listed = 0;
+}
+__global__ __launch_bounds__(kPartThreads) void sample_bins(PartArgs a) {
+  __shared__ Bins bins;
+  const int part = blockIdx.x, tid = threadIdx.x, from = part * a.each, to = min(from + a.each, a.s.V);
+  const int64_t row = blockIdx.y;
+  const u64 first = first_of(a, row);
+  const Row r = row_of(a.s, row, value_of((uint32_t)(first >> 32)));
+  if ((uint32_t)(first >> 32) == kNoKey || r.greedy || !(r.by_count || r.by_mass)) return;
+  for (int i = tid; i < kBins; i += kPartThreads) {
+    bins.mass[i] = 0;
+    bins.count[i] = 0;
+  }
+  __syncthreads();
+  each_token(r.x, from + tid, to, kPartThreads, [&](int, float x) {
+    const double z = distance(r, x);
+    const u64 m = whole(r, weight(z));
+    const int bin = bin_of(r, z, m);
+    if (bin == kBins) return;
+    atomicAdd(&bins.count[bin], 1u);
+    atomicAdd(&bins.mass[bin], m);
+  });
+  __syncthreads();
+  RowSpace& sp = a.rows[row];
+  for (int i = tid; i < kBins; i += kPartThreads)
+    if (bins.count[i]) {
+      atomicAdd(&sp.bins.count[i], bins.count[i]);
+      atomicAdd(&sp.bins.mass[i], bins.mass[i]);
+    }
+}
+// Lists the tokens of the border's bins.
+__global__ __launch_bounds__(kPartThreads) void sample_list(PartArgs a) {
+  __shared__ Work w;
+  const int part = blockIdx.x, tid = threadIdx.x, from = part * a.each, to = min(from + a.each, a.s.V);
+  const int64_t row = blockIdx.y;
+  const u64 first = first_of(a, row);
+  const Row r = row_of(a.s, row, value_of((uint32_t)(first >> 32)));
+  if ((uint32_t)(first >> 32) == kNoKey || r.greedy || !(r.by_count || r.by_mass)) return;
+  RowSpace& sp = a.rows[row];
+  const Borders o = borders<kPartThreads>(r, sp.bins, w);
+  if (o.b1 < 0 || o.size > kList) return;
+  each_token(r.x, from + tid, to, kPartThreads, [&](int i, float x) {
+    const double z = distance(r, x);
+    const int bin = bin_of(r, z, whole(r, weight(z)));
+    if (bin >= o.b0 && bin <= o.b1) sp.list[atomicAdd(&sp.listed, 1ull)] = order_of(key_of(x), i);
+  });
+}
+// The bound of what is kept, a block a row.
+__global__ __launch_bounds__(1024) void sample_bound(PartArgs a) {
+  __shared__ Work w;
+  __shared__ Bins bins;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const u64 first = first_of(a, row);
+  const Row r = row_of(a.s, row, value_of((uint32_t)(first >> 32)));
+  RowSpace& sp = a.rows[row];
+  u64 bound = kAll;
+  if ((uint32_t)(first >> 32) != kNoKey && !r.greedy && (r.by_count || r.by_mass)) {
+    const Borders o = borders<1024>(r, sp.bins, w);
+    if (o.b1 >= 0 && o.size <= kList) {
+      for (int i = tid; i < (int)sp.listed; i += 1024) w.list[i] = sp.list[i];
+      bound = bound_of_list<1024>(r, o, (int)sp.listed, w);
+    } else if (o.b1 >= 0) {
+      bound = bound_by_walks<1024>(r, o.all, bins, w);
+    }
+  }
+  if (tid == 0) sp.bound = bound;
+}
+__global__ __launch_bounds__(kPartThreads) void sample_sums(PartArgs a) {
+  const int part = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
+  const int64_t row = blockIdx.y;
+  const u64 first = first_of(a, row);
+  const Row r = row_of(a.s, row, value_of((uint32_t)(first >> 32)));
+  if ((uint32_t)(first >> 32) == kNoKey || r.greedy) return;
+  const int each = a.each / kPartWaves, from = min(part * a.each + wave * each, a.s.V), to = min(from + each, a.s.V);
+  const u64 sum = stretch_sum(r, a.rows[row].bound, from, to);
+  if ((tid & 63) == 0) a.sums[(row * a.parts + part) * kPartWaves + wave] = sum;
+}
+// The choice, a wavefront a row.
+__global__ __launch_bounds__(64) void sample_pick(PartArgs a) {
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  const u64 first = first_of(a, row);
+  const Row r = row_of(a.s, row, value_of((uint32_t)(first >> 32)));
+  if ((uint32_t)(first >> 32) == kNoKey || r.greedy) {
+    if (lane == 0) a.s.token[row] = (uint32_t)(first >> 32) == kNoKey ? -1 : (int32_t)(uint32_t)first;
+    return;
+  }
+  const int n = a.parts * kPartWaves, each = a.each / kPartWaves;
+  const u64* sums = a.sums + row * n;
+  u64 all = 0;
+  for (int k = lane; k < n; k += 64) all += sums[k];
+  all = wave_sum(all);
+  u64 goal = goal_of(r, all), before = 0;
+  for (int k0 = 0; k0 < n; k0 += 64) {
+    const u64 m = k0 + lane < n ? sums[k0 + lane] : 0, sum = before + wave_scan(m), passed = __ballot(sum > goal);
+    if (passed) {
+      const int l = __ffsll(passed) - 1, k = k0 + l;
+      goal -= __shfl(sum - m, l);
+      const int from = min(k * each, a.s.V);
+      choose(r, a.rows[row].bound, from, min(from + each, a.s.V), goal, a.s.token + row);
       return;
     }
     before = __shfl(sum, 63);
   }
 }
 
+struct SamplePlan {
+  int parts, each;                 // 1 part: a block a row
+  int64_t tops, sums, bytes;
+};
+SamplePlan sample_plan(const SampleDesc& s) {
+  SamplePlan p{};
+  p.parts = 1;
+  // Several blocks a row where rows alone leave most of the card idle and are long enough.
+  if (s.rows < 128 && s.V > 8192) p.parts = (int)std::min<int64_t>((s.V + 2047) / 2048, (1024 + s.rows - 1) / s.rows);
+  p.each = ((s.V + p.parts - 1) / p.parts + kPartThreads - 1) / kPartThreads * kPartThreads;
+  p.parts = (s.V + p.each - 1) / p.each;
+  if (p.parts > 1) {
+    p.tops = s.rows * (int64_t)sizeof(RowSpace);
+    p.sums = p.tops + s.rows * p.parts * 8;
+    p.bytes = p.sums + s.rows * p.parts * kPartWaves * 8;
+  }
+  return p;
+}
+
 }  // namespace
 
-int64_t sample_workspace_bytes(const SampleDesc&) { return 0; }
-void sample(const SampleDesc& s, void*, hipStream_t st) { klaunch(sample_rows, dim3((unsigned)s.rows), dim3(kThreads), 0, st, s); }
+int64_t sample_workspace_bytes(const SampleDesc& s) { return sample_plan(s).bytes; }
+
+void sample(const SampleDesc& s, void* work, hipStream_t st) {
+  const SamplePlan p = sample_plan(s);
+  const dim3 rows((unsigned)s.rows), grid((unsigned)p.parts, (unsigned)s.rows), block(kPartThreads);
+  if (p.parts == 1) {
+    if (s.V <= 4096) klaunch(sample_one<256>, rows, block, 0, st, s);
+    else klaunch(sample_one<1024>, rows, dim3(1024), 0, st, s);
+    return;
+  }
+  char* w = (char*)work;
+  const PartArgs a{s, p.parts, p.each, (RowSpace*)w, (u64*)(w + p.tops), (u64*)(w + p.sums)};
+  const bool limits = s.top_k || s.top_p || (s.top_k1 > 0 && s.top_k1 < s.V) || s.top_p1 < 1;
+  klaunch(sample_tops, grid, block, 0, st, a);
+  if (limits) {
+    klaunch(sample_bins, grid, block, 0, st, a);
+    klaunch(sample_list, grid, block, 0, st, a);
+  }
+  klaunch(sample_bound, rows, dim3(1024), 0, st, a);
+  klaunch(sample_sums, grid, block, 0, st, a);
+  klaunch(sample_pick, rows, dim3(64), 0, st, a);
+}
 
 }  // namespace tgk
