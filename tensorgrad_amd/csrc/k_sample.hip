@@ -9,8 +9,8 @@
 // all: sums do not depend on their order, so counts, borders and the choice agree with each other and repeat, and a weight is off by
 // 2^(-unit-1) of the largest at most. Beyond some 32 to 43 in z they are 0.
 //
-// A row is read three times, the first time from memory. Many rows: a block takes one, in one launch (sample_one). Few rows of many
-// tokens: several blocks a row, in four launches (sample_tops, sample_bins, sample_list, sample_pick).
+// A row is read four times, the first time from memory. Many rows: a block takes one, in one launch (sample_one; sample_short, which
+// sorts all). Few rows of many tokens: several blocks a row, in six launches (sample_tops, _bins, _list, _bound, _sums, _pick).
 #include <algorithm>
 
 #include "kernels.h"
@@ -40,6 +40,7 @@ struct Row {
   int V, most, unit;
   float top;                       // largest logit
   double per, p, least, u;         // 1 / temperature; top_p, min_p; the random number
+  double per_bin;                  // bins for a distance of 1
   bool greedy, by_count, by_mass;  // what limits
 };
 __device__ __forceinline__ Row row_of(const SampleDesc& s, int64_t row, float top) {
@@ -51,6 +52,7 @@ __device__ __forceinline__ Row row_of(const SampleDesc& s, int64_t row, float to
   r.greedy = !(heat > 0);
   r.per = r.greedy ? 1 : 1 / heat;
   r.unit = 62 - (s.V > 1 ? 32 - __clz(s.V - 1) : 0);
+  r.per_bin = kBins / (0.6931471805599454 * (r.unit + 1));
   r.most = s.top_k ? s.top_k[row] : s.top_k1;
   r.p = s.top_p ? (double)s.top_p[row] : s.top_p1;
   r.least = s.min_p ? (double)s.min_p[row] : s.min_p1;
@@ -73,10 +75,8 @@ __device__ __forceinline__ double weight(double z) {
   return __builtin_amdgcn_ldexp(e, -(int)n);
 }
 __device__ __forceinline__ u64 whole(const Row& r, double w) { return (u64)rint(__builtin_amdgcn_ldexp(w, r.unit)); }
-// Its bin: of equal width, up to where weights are 0; kBins: no weight.
-__device__ __forceinline__ int bin_of(const Row& r, double z, u64 w) {
-  return w == 0 ? kBins : min((int)(z * (kBins / (0.6931471805599454 * (r.unit + 1)))), kBins - 1);
-}
+// Its bin: of equal width, up to where weights are 0; kBins from there on.
+__device__ __forceinline__ int bin_of(const Row& r, double z) { return (int)fmin(z * r.per_bin, (double)kBins); }
 
 __device__ __forceinline__ u64 wave_min(u64 x) {
 #pragma unroll
@@ -105,8 +105,9 @@ struct Bins {
   uint32_t count[kBins];
 };
 // What a block shares while it finds a row's borders and its choice.
+template <int LIST>
 struct Work {
-  u64 list[kList];
+  u64 list[LIST];
   u64 sums[2][16];
   u64 found[8];
   uint32_t listed;
@@ -125,7 +126,7 @@ __device__ __forceinline__ void each_token(const float* x, int from, int to, int
   }
 }
 
-template <int THREADS>
+template <int THREADS, class Work>
 __device__ __forceinline__ u64 block_min(u64 x, Work& w) {
   x = wave_min(x);
   __syncthreads();
@@ -136,7 +137,7 @@ __device__ __forceinline__ u64 block_min(u64 x, Work& w) {
   return x;
 }
 // Sums over the bins before this thread's first (it has kBins / THREADS of them), and over all.
-template <int THREADS>
+template <int THREADS, class Work>
 __device__ __forceinline__ void bin_sums(const Bins& b, Work& w, u64& count, u64& mass, u64& all_count, u64& all_mass) {
   constexpr int N = kBins / THREADS;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -173,7 +174,7 @@ struct Borders {
   int b0, b1;
   u64 count, mass, size, all;
 };
-template <int THREADS>
+template <int THREADS, class Work>
 __device__ __forceinline__ Borders borders(const Row& r, const Bins& b, Work& w) {
   constexpr int N = kBins / THREADS;
   const int tid = threadIdx.x;
@@ -235,28 +236,60 @@ __device__ __forceinline__ Borders borders(const Row& r, const Bins& b, Work& w)
   return o;
 }
 
-// The bound of what is kept (an order, inclusive) from the sorted tokens of the border's bins. `n` of them, in w.list.
-template <int THREADS>
-__device__ __forceinline__ u64 bound_of_list(const Row& r, const Borders& o, int n, Work& w) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// Sorts the first n of w.list: bitonic, a thread having every THREADS-th token. Steps of 1 to 32 places are exchanges of lanes, those of
+// THREADS and more a thread's own; the rest go through LDS, 10 of 55 steps for 1024 tokens of 1024 threads.
+template <int THREADS, int LIST>
+__device__ __forceinline__ void sort_list(int n, Work<LIST>& w) {
+  constexpr int N = LIST / THREADS;
+  const int tid = threadIdx.x;
   int n2 = 64;
   while (n2 < n) n2 *= 2;
-  for (int i = n + tid; i < n2; i += THREADS) w.list[i] = kAll;
-  __syncthreads();
-  for (int size = 2; size <= n2; size *= 2)   // bitonic
+  u64 x[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) x[e] = e * THREADS + tid < n ? w.list[e * THREADS + tid] : kAll;
+  auto keep = [&](int e, u64 other, int size, int half) {
+    const int i = e * THREADS + tid;
+    const bool low = ((i & half) == 0) == ((i & size) == 0);   // takes the smaller
+    x[e] = (other < x[e]) == low ? other : x[e];
+  };
+  for (int size = 2; size <= n2; size *= 2)
     for (int half = size / 2; half > 0; half /= 2) {
-      for (int t = tid; t < n2 / 2; t += THREADS) {
-        const int i = 2 * t - (t & (half - 1)), j = i + half;
-        const u64 a = w.list[i], b = w.list[j];
-        if ((a > b) == ((i & size) == 0)) {
-          w.list[i] = b;
-          w.list[j] = a;
-        }
+      if (half >= THREADS) {
+#pragma unroll
+        for (int d = 1; d < N; d *= 2)
+          if (half == d * THREADS)
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+              if ((e & d) == 0) {
+                const u64 a = x[e], b = x[e + d];
+                keep(e, b, size, half);
+                keep(e + d, a, size, half);
+              }
+      } else if (half >= 64) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < N; ++e) if (e * THREADS < n2) w.list[e * THREADS + tid] = x[e];
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < N; ++e) if (e * THREADS < n2) keep(e, w.list[e * THREADS + (tid ^ half)], size, half);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) if (e * THREADS < n2) keep(e, __shfl_xor(x[e], half), size, half);
       }
-      __syncthreads();
     }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < N; ++e) if (e * THREADS < n2) w.list[e * THREADS + tid] = x[e];
+  __syncthreads();
+}
+
+// The bound of what is kept (an order, inclusive) from the tokens of the border's bins, `n` of them, in w.list.
+template <int THREADS, int LIST>
+__device__ __forceinline__ u64 bound_of_list(const Row& r, const Borders& o, int n, Work<LIST>& w) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  sort_list<THREADS, LIST>(n, w);
   // a thread has N neighbours; those that top-k keeps
-  constexpr int N = kList / THREADS;
+  constexpr int N = LIST / THREADS;
   const int kept = r.by_count ? (int)min((u64)n, (u64)r.most - min((u64)r.most, o.count)) : n;
   u64 m[N], sum = 0;
 #pragma unroll
@@ -297,7 +330,7 @@ struct Border {
   uint32_t key;
   u64 ties;
 };
-template <int THREADS, bool COUNT>
+template <int THREADS, bool COUNT, class Work>
 __device__ __forceinline__ Border find_border(const Row& r, Border within, double target, Bins& b, Work& w, u64* total) {
   constexpr int N = kBins / THREADS;
   const int tid = threadIdx.x;
@@ -383,7 +416,7 @@ __device__ __forceinline__ Border find_border(const Row& r, Border within, doubl
   *total = mass_before + ties * one;
   return {lo, ties};
 }
-template <int THREADS>
+template <int THREADS, class Work>
 __device__ __forceinline__ u64 bound_by_walks(const Row& r, u64 all_mass, Bins& b, Work& w) {
   Border kept = {kNoKey, 0};
   u64 total = all_mass;
@@ -429,18 +462,41 @@ __device__ __forceinline__ u64 stretch_sum(const Row& r, u64 bound, int from, in
   each_token(r.x, from + (int)(threadIdx.x & 63), to, 64, [&](int i, float x) { sum += kept_weight(r, bound, i, x); });
   return wave_sum(sum);
 }
-// The token of [from, to) where the sum of weights passes `goal`, by a wavefront.
-__device__ __forceinline__ void choose(const Row& r, u64 bound, int from, int to, u64 goal, int32_t* token) {
-  const int lane = threadIdx.x & 63;
-  u64 before = 0;
-  for (int i0 = from; i0 < to; i0 += 64) {
-    const u64 m = i0 + lane < to ? kept_weight(r, bound, i0 + lane, r.x[i0 + lane]) : 0, sum = before + wave_scan(m);
-    const u64 passed = __ballot(sum > goal);
-    if (passed) {
-      if (lane == __ffsll(passed) - 1) *token = i0 + lane;
+// The token of [from, to) where the sum of weights passes `goal`, by a block: a thread sums N neighbours.
+template <int THREADS, class Work>
+__device__ __forceinline__ void choose(const Row& r, u64 bound, int from, int to, u64 goal, Work& w, int32_t* token) {
+  constexpr int N = 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int i0 = from; i0 < to; i0 += N * THREADS) {
+    u64 m[N], sum = 0;
+    float v[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = r.x[min(i0 + N * tid + e, to - 1)];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int i = i0 + N * tid + e;
+      m[e] = i < to ? kept_weight(r, bound, i, v[e]) : 0;
+      sum += m[e];
+    }
+    const u64 scan = wave_scan(sum);
+    __syncthreads();
+    if (lane == 63) w.sums[0][wave] = scan;
+    __syncthreads();
+    u64 before = scan - sum, all = 0;
+#pragma unroll
+    for (int k = 0; k < THREADS / 64; ++k) {
+      if (k < wave) before += w.sums[0][k];
+      all += w.sums[0][k];
+    }
+    if (goal < all) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if (before <= goal && goal < before + m[e]) *token = i0 + N * tid + e;
+        before += m[e];
+      }
       return;
     }
-    before = __shfl(sum, 63);
+    goal -= all;
   }
 }
 // Passed: sum > u all, as whole numbers; u in [0, 1) leaves the last token's sum, all, to pass.
@@ -448,11 +504,50 @@ __device__ __forceinline__ u64 goal_of(const Row& r, u64 all) { return min((u64)
 
 // ---- a block a row -------------------------------------------------------------------------------------
 
+// At most LIST tokens, all of them sorted: no bins, and for 256 a single wavefront. Bound by latency: some 20 dependent steps.
+template <int THREADS, int LIST>
+__global__ __launch_bounds__(THREADS) void sample_short(SampleDesc s) {
+  constexpr int N = LIST / THREADS;
+  __shared__ Work<LIST> w;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float* x = s.logits + row * s.V;
+  u64 first = kAll;
+  float v[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = x[min(e * THREADS + tid, s.V - 1)];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const int i = e * THREADS + tid;
+    const u64 o = i < s.V ? order_of(key_of(v[e]), i) : kAll;
+    w.list[i] = o;
+    first = o < first ? o : first;
+  }
+  first = block_min<THREADS>(first, w);
+  const Row r = row_of(s, row, value_of((uint32_t)(first >> 32)));
+  if ((uint32_t)(first >> 32) == kNoKey || r.greedy) {
+    if (tid == 0) s.token[row] = (uint32_t)(first >> 32) == kNoKey ? -1 : (int32_t)(uint32_t)first;
+    return;
+  }
+  const u64 bound = r.by_count || r.by_mass ? bound_of_list<THREADS, LIST>(r, {0, 0, 0, 0, 0, 0}, s.V, w) : kAll;
+  u64 mine = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) if (e * THREADS + tid < s.V) mine += kept_weight(r, bound, e * THREADS + tid, v[e]);
+  mine = wave_sum(mine);
+  __syncthreads();
+  if (lane == 0) w.sums[1][wave] = mine;
+  __syncthreads();
+  u64 all = 0;
+#pragma unroll
+  for (int k = 0; k < THREADS / 64; ++k) all += w.sums[1][k];
+  choose<THREADS>(r, bound, 0, s.V, goal_of(r, all), w, s.token + row);
+}
+
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void sample_one(SampleDesc s) {
   constexpr int W = THREADS / 64;
   __shared__ Bins bins;
-  __shared__ Work w;
+  __shared__ Work<kList> w;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   u64 first = kAll;
@@ -460,6 +555,11 @@ __global__ __launch_bounds__(THREADS) void sample_one(SampleDesc s) {
     const u64 o = order_of(key_of(x), i);
     first = o < first ? o : first;
   });
+  for (int i = tid; i < kBins; i += THREADS) {
+    bins.mass[i] = 0;
+    bins.count[i] = 0;
+  }
+  if (tid == 0) w.listed = 0;
   first = block_min<THREADS>(first, w);
   const Row r = row_of(s, row, value_of((uint32_t)(first >> 32)));
   if ((uint32_t)(first >> 32) == kNoKey || r.greedy) {
@@ -468,51 +568,38 @@ __global__ __launch_bounds__(THREADS) void sample_one(SampleDesc s) {
   }
   u64 bound = kAll;
   if (r.by_count || r.by_mass) {
-    Borders o = {0, kBins - 1, 0, 0, (u64)s.V, 0};
-    if (s.V > kList) {
-      for (int i = tid; i < kBins; i += THREADS) {
-        bins.mass[i] = 0;
-        bins.count[i] = 0;
-      }
-      __syncthreads();
-      each_token(r.x, tid, s.V, THREADS, [&](int, float x) {
-        const double z = distance(r, x);
-        const u64 m = whole(r, weight(z));
-        const int bin = bin_of(r, z, m);
-        if (bin == kBins) return;
-        atomicAdd(&bins.count[bin], 1u);
-        atomicAdd(&bins.mass[bin], m);
-      });
-      __syncthreads();
-      o = borders<THREADS>(r, bins, w);
-    }
-    if (o.b1 >= 0 && o.size <= kList) {
-      if (tid == 0) w.listed = 0;
-      __syncthreads();
+    each_token(r.x, tid, s.V, THREADS, [&](int, float x) {
+      const double z = distance(r, x);
+      const int bin = bin_of(r, z);
+      if (bin == kBins) return;
+      atomicAdd(&bins.count[bin], 1u);
+      atomicAdd(&bins.mass[bin], whole(r, weight(z)));
+    });
+    __syncthreads();
+    const Borders o = borders<THREADS>(r, bins, w);
+    if (__builtin_expect(o.b1 >= 0 && o.size > kList, 0)) {
+      bound = bound_by_walks<THREADS>(r, o.all, bins, w);
+    } else if (o.b1 >= 0) {
       each_token(r.x, tid, s.V, THREADS, [&](int i, float x) {
-        const double z = distance(r, x);
-        const int bin = bin_of(r, z, whole(r, weight(z)));
+        const int bin = bin_of(r, distance(r, x));
         if (bin >= o.b0 && bin <= o.b1) w.list[atomicAdd(&w.listed, 1u)] = order_of(key_of(x), i);
       });
       __syncthreads();
-      bound = bound_of_list<THREADS>(r, o, (int)w.listed, w);
-    } else if (o.b1 >= 0) {
-      bound = bound_by_walks<THREADS>(r, o.all, bins, w);
+      bound = bound_of_list<THREADS, kList>(r, o, (int)w.listed, w);
     }
   }
   const int each = ((s.V + W - 1) / W + 63) / 64 * 64, from = min(wave * each, s.V), to = min(from + each, s.V);
   const u64 mine = stretch_sum(r, bound, from, to);
   __syncthreads();
-  if (lane == 0) w.sums[0][wave] = mine;
+  if (lane == 0) w.sums[1][wave] = mine;
   __syncthreads();
-  u64 before = 0, all = 0;
+  u64 all = 0;
 #pragma unroll
-  for (int k = 0; k < W; ++k) {
-    if (k < wave) before += w.sums[0][k];
-    all += w.sums[0][k];
-  }
-  const u64 goal = goal_of(r, all);
-  if (before <= goal && goal < before + mine) choose(r, bound, from, to, goal - before, s.token + row);
+  for (int k = 0; k < W; ++k) all += w.sums[1][k];
+  u64 goal = goal_of(r, all);
+  int k = 0;
+  while (k < W - 1 && goal >= w.sums[1][k]) goal -= w.sums[1][k++];
+  choose<THREADS>(r, bound, min(k * each, s.V), min((k + 1) * each, s.V), goal, w, s.token + row);
 }
 
 // ---- several blocks a row ------------------------------------------------------------------------------
@@ -521,7 +608,8 @@ constexpr int kPartThreads = 256, kPartWaves = kPartThreads / 64;
 struct RowSpace {                  // of a row in the workspace
   Bins bins;
   u64 list[kList];
-  u64 first, bound, listed, over;
+  u64 bound, listed;
+  Borders borders;
 };
 struct PartArgs {
   SampleDesc s;
@@ -535,7 +623,7 @@ __device__ __forceinline__ u64 first_of(const PartArgs& a, int64_t row) {
   return wave_min(first);
 }
 __global__ __launch_bounds__(kPartThreads) void sample_tops(PartArgs a) {
-  __shared__ Work w;
+  __shared__ Work<64> w;
   const int part = blockIdx.x;
   const int64_t row = blockIdx.y;
   const int tid = threadIdx.x, from = part * a.each, to = min(from + a.each, a.s.V);
@@ -567,11 +655,10 @@ __global__ __launch_bounds__(kPartThreads) void sample_bins(PartArgs a) {
   __syncthreads();
   each_token(r.x, from + tid, to, kPartThreads, [&](int, float x) {
     const double z = distance(r, x);
-    const u64 m = whole(r, weight(z));
-    const int bin = bin_of(r, z, m);
+    const int bin = bin_of(r, z);
     if (bin == kBins) return;
     atomicAdd(&bins.count[bin], 1u);
-    atomicAdd(&bins.mass[bin], m);
+    atomicAdd(&bins.mass[bin], whole(r, weight(z)));
   });
   __syncthreads();
   RowSpace& sp = a.rows[row];
@@ -583,7 +670,7 @@ __global__ __launch_bounds__(kPartThreads) void sample_bins(PartArgs a) {
 }
 // Lists the tokens of the border's bins.
 __global__ __launch_bounds__(kPartThreads) void sample_list(PartArgs a) {
-  __shared__ Work w;
+  __shared__ Work<64> w;
   const int part = blockIdx.x, tid = threadIdx.x, from = part * a.each, to = min(from + a.each, a.s.V);
   const int64_t row = blockIdx.y;
   const u64 first = first_of(a, row);
@@ -591,16 +678,16 @@ __global__ __launch_bounds__(kPartThreads) void sample_list(PartArgs a) {
   if ((uint32_t)(first >> 32) == kNoKey || r.greedy || !(r.by_count || r.by_mass)) return;
   RowSpace& sp = a.rows[row];
   const Borders o = borders<kPartThreads>(r, sp.bins, w);
+  if (part == 0 && tid == 0) sp.borders = o;
   if (o.b1 < 0 || o.size > kList) return;
   each_token(r.x, from + tid, to, kPartThreads, [&](int i, float x) {
-    const double z = distance(r, x);
-    const int bin = bin_of(r, z, whole(r, weight(z)));
+    const int bin = bin_of(r, distance(r, x));
     if (bin >= o.b0 && bin <= o.b1) sp.list[atomicAdd(&sp.listed, 1ull)] = order_of(key_of(x), i);
   });
 }
 // The bound of what is kept, a block a row.
 __global__ __launch_bounds__(1024) void sample_bound(PartArgs a) {
-  __shared__ Work w;
+  __shared__ Work<kList> w;
   __shared__ Bins bins;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
@@ -609,12 +696,13 @@ __global__ __launch_bounds__(1024) void sample_bound(PartArgs a) {
   RowSpace& sp = a.rows[row];
   u64 bound = kAll;
   if ((uint32_t)(first >> 32) != kNoKey && !r.greedy && (r.by_count || r.by_mass)) {
-    const Borders o = borders<1024>(r, sp.bins, w);
-    if (o.b1 >= 0 && o.size <= kList) {
-      for (int i = tid; i < (int)sp.listed; i += 1024) w.list[i] = sp.list[i];
-      bound = bound_of_list<1024>(r, o, (int)sp.listed, w);
-    } else if (o.b1 >= 0) {
+    const Borders o = sp.borders;
+    if (__builtin_expect(o.b1 >= 0 && o.size > kList, 0)) {
       bound = bound_by_walks<1024>(r, o.all, bins, w);
+    } else if (o.b1 >= 0) {
+      for (int i = tid; i < (int)o.size; i += 1024) w.list[i] = sp.list[i];
+      __syncthreads();
+      bound = bound_of_list<1024, kList>(r, o, (int)o.size, w);
     }
   }
   if (tid == 0) sp.bound = bound;
@@ -629,14 +717,15 @@ __global__ __launch_bounds__(kPartThreads) void sample_sums(PartArgs a) {
   const u64 sum = stretch_sum(r, a.rows[row].bound, from, to);
   if ((tid & 63) == 0) a.sums[(row * a.parts + part) * kPartWaves + wave] = sum;
 }
-// The choice, a wavefront a row.
-__global__ __launch_bounds__(64) void sample_pick(PartArgs a) {
+// The choice, a block a row; every wavefront finds the stretch.
+__global__ __launch_bounds__(kPartThreads) void sample_pick(PartArgs a) {
+  __shared__ Work<64> w;
   const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63;
   const u64 first = first_of(a, row);
   const Row r = row_of(a.s, row, value_of((uint32_t)(first >> 32)));
   if ((uint32_t)(first >> 32) == kNoKey || r.greedy) {
-    if (lane == 0) a.s.token[row] = (uint32_t)(first >> 32) == kNoKey ? -1 : (int32_t)(uint32_t)first;
+    if (threadIdx.x == 0) a.s.token[row] = (uint32_t)(first >> 32) == kNoKey ? -1 : (int32_t)(uint32_t)first;
     return;
   }
   const int n = a.parts * kPartWaves, each = a.each / kPartWaves;
@@ -651,7 +740,7 @@ __global__ __launch_bounds__(64) void sample_pick(PartArgs a) {
       const int l = __ffsll(passed) - 1, k = k0 + l;
       goal -= __shfl(sum - m, l);
       const int from = min(k * each, a.s.V);
-      choose(r, a.rows[row].bound, from, min(from + each, a.s.V), goal, a.s.token + row);
+      choose<kPartThreads>(r, a.rows[row].bound, from, min(from + each, a.s.V), goal, w, a.s.token + row);
       return;
     }
     before = __shfl(sum, 63);
@@ -685,7 +774,8 @@ void sample(const SampleDesc& s, void* work, hipStream_t st) {
   const SamplePlan p = sample_plan(s);
   const dim3 rows((unsigned)s.rows), grid((unsigned)p.parts, (unsigned)s.rows), block(kPartThreads);
   if (p.parts == 1) {
-    if (s.V <= 4096) klaunch(sample_one<256>, rows, block, 0, st, s);
+    if (s.V <= 256) klaunch(sample_short<64, 256>, rows, dim3(64), 0, st, s);
+    else if (s.V <= 2048) klaunch(sample_short<256, 2048>, rows, block, 0, st, s);
     else klaunch(sample_one<1024>, rows, dim3(1024), 0, st, s);
     return;
   }
@@ -699,7 +789,7 @@ void sample(const SampleDesc& s, void* work, hipStream_t st) {
   }
   klaunch(sample_bound, rows, dim3(1024), 0, st, a);
   klaunch(sample_sums, grid, block, 0, st, a);
-  klaunch(sample_pick, rows, dim3(64), 0, st, a);
+  klaunch(sample_pick, rows, block, 0, st, a);
 }
 
 }  // namespace tgk
