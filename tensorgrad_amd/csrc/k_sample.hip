@@ -7,7 +7,7 @@
 //
 // Weights are whole numbers, exp(-z) times 2^unit with z = (largest - logit) / temperature in 64 bits and 62 bits for the sum of
 // all: sums do not depend on their order, so counts, borders and the choice agree with each other and repeat, and a weight is off by
-// 2^(-unit-1) of the largest at most. Beyond some 32 to 43 in z they are 0.
+// 2^(-unit-1) of the largest at most. Beyond some 32 to 43 in z they are 0. A temperature of 0 is a top-k of 1.
 //
 // A row is read four times, the first time from memory. Many rows: a block takes one, in one launch (sample_one; sample_short, which
 // sorts all). Few rows of many tokens: several blocks a row, in six launches (sample_tops, _bins, _list, _bound, _sums, _pick).
@@ -38,52 +38,57 @@ __device__ __forceinline__ u64 order_of(uint32_t key, int i) { return (u64)key <
 struct Row {
   const float* x;
   int V, most, unit;
-  float top;                       // largest logit
-  double per, p, least, u;         // 1 / temperature; top_p, min_p; the random number
-  double per_bin;                  // bins for a distance of 1
-  bool greedy, by_count, by_mass;  // what limits
+  float top, per_bin;              // largest logit; bins for a logit of 1 less
+  double per, p, least, u;         // log2(e) / temperature; top_p; min_p times 2^unit; the random number
+  bool by_count, by_mass;          // what limits
 };
+constexpr double kLn2 = 0.693147180559945309417;
 __device__ __forceinline__ Row row_of(const SampleDesc& s, int64_t row, float top) {
   Row r;
   r.x = s.logits + row * s.V;
   r.V = s.V;
   r.top = top;
   const double heat = s.temperature ? (double)s.temperature[row] : s.temperature1;
-  r.greedy = !(heat > 0);
-  r.per = r.greedy ? 1 : 1 / heat;
+  const bool greedy = !(heat > 0);           // the first of the order
+  const double per = greedy ? 1 : 1 / heat;
   r.unit = 62 - (s.V > 1 ? 32 - __clz(s.V - 1) : 0);
-  r.per_bin = kBins / (0.6931471805599454 * (r.unit + 1));
-  r.most = s.top_k ? s.top_k[row] : s.top_k1;
+  r.per = per * (1 / kLn2);
+  r.per_bin = (float)(per * (kBins / (1.001 * kLn2 * (r.unit + 1))));
+  r.most = greedy ? 1 : s.top_k ? s.top_k[row] : s.top_k1;
   r.p = s.top_p ? (double)s.top_p[row] : s.top_p1;
-  r.least = s.min_p ? (double)s.min_p[row] : s.min_p1;
+  r.least = __builtin_amdgcn_ldexp(s.min_p ? (double)s.min_p[row] : s.min_p1, r.unit);
   r.u = s.u[row];
   r.by_count = r.most > 0 && r.most < s.V;
-  r.by_mass = r.p < 1;
+  r.by_mass = r.p < 1 && !greedy;
   return r;
 }
-// The distance to the largest logit in units of the temperature; infinite: no weight.
-__device__ __forceinline__ double distance(const Row& r, float x) {
-  return x == r.top ? 0 : x > -INFINITY ? ((double)r.top - (double)x) * r.per : (double)INFINITY;
-}
-// exp(-z), of z >= 0: 2^-n times the Taylor series of 2^-f for |f| <= 1 / 2, 2^-52 off at most.
-__device__ __forceinline__ double weight(double z) {
-  const double t = fmin(z * 1.44269504088896340736, 2000.0), n = rint(t), f = (n - t) * 0.693147180559945309417;
-  double e = 1.0 / 479001600;
-  const double c[] = {1.0 / 39916800, 1.0 / 3628800, 1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720, 1.0 / 120, 1.0 / 24, 1.0 / 6, 0.5, 1, 1};
-#pragma unroll
-  for (int i = 0; i < 12; ++i) e = fma(e, f, c[i]);
-  return __builtin_amdgcn_ldexp(e, -(int)n);
-}
-__device__ __forceinline__ u64 whole(const Row& r, double w) { return (u64)rint(__builtin_amdgcn_ldexp(w, r.unit)); }
-// Its bin: of equal width, up to where weights are 0; kBins from there on.
-__device__ __forceinline__ int bin_of(const Row& r, double z) { return (int)fmin(z * r.per_bin, (double)kBins); }
-
-__device__ __forceinline__ u64 wave_min(u64 x) {
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const u64 z = __shfl_xor(x, o);
-    x = z < x ? z : x;
+// A token's weight times 2^unit, 0 far from the top: 2^-t = 2^-n 2^f by the series of 2^f for |f| <= 1 / 2, 2^-52 off at most. Of
+// a logit that is there.
+struct Series {
+  double c[13];
+  constexpr Series() : c() {
+    c[0] = 1;
+    for (int k = 1; k < 13; ++k) c[k] = c[k - 1] * kLn2 / k;
   }
+};
+__device__ __forceinline__ double weight(const Row& r, float x) {
+  constexpr Series s;
+  const double t = x == r.top ? 0 : fmin(((double)r.top - (double)x) * r.per, 4000.0), n = rint(t), f = n - t;
+  double e = s.c[12];
+#pragma unroll
+  for (int k = 11; k >= 0; --k) e = fma(e, f, s.c[k]);
+  return __builtin_amdgcn_ldexp(e, r.unit - (int)n);
+}
+__device__ __forceinline__ u64 whole(double w) { return (u64)rint(w); }
+// A token's bin, rising with the distance to the top in equal steps; kBins: so far that its weight is 0, or not there.
+__device__ __forceinline__ int bin_of(const Row& r, float x) {
+  const float b = x == r.top ? 0.0f : (r.top - x) * r.per_bin;
+  return b < kBins ? (int)b : kBins;
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) x = fmaxf(x, __shfl_xor(x, o));
   return x;
 }
 __device__ __forceinline__ u64 wave_sum(u64 x) {
@@ -126,15 +131,38 @@ __device__ __forceinline__ void each_token(const float* x, int from, int to, int
   }
 }
 
+// The largest logit of [from, to); NaN is none.
 template <int THREADS, class Work>
-__device__ __forceinline__ u64 block_min(u64 x, Work& w) {
-  x = wave_min(x);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) w.sums[0][threadIdx.x >> 6] = x;
+__device__ __forceinline__ float block_top(const float* x, int from, int to, Work& w) {
+  float top = -INFINITY;
+  each_token(x, from + (int)threadIdx.x, to, THREADS, [&](int, float v) { top = fmaxf(top, v); });
+  top = wave_max(top);
+  if ((threadIdx.x & 63) == 0) w.sums[0][threadIdx.x >> 6] = __float_as_uint(top);
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < THREADS / 64; ++k) x = w.sums[0][k] < x ? w.sums[0][k] : x;
-  return x;
+  for (int k = 0; k < THREADS / 64; ++k) top = fmaxf(top, __uint_as_float((uint32_t)w.sums[0][k]));
+  return top;
+}
+// Counts and weighs [from, to) in bins. A few tokens at most are kept by their count alone: then no mass is needed, since all of them
+// are listed.
+constexpr int kFew = 1024;
+__device__ __forceinline__ bool few(const Row& r) { return r.by_count && r.most <= kFew; }
+template <int THREADS>
+__device__ __forceinline__ void clear_bins(Bins& b) {
+  for (int i = threadIdx.x; i < kBins; i += THREADS) {
+    b.mass[i] = 0;
+    b.count[i] = 0;
+  }
+}
+template <int THREADS>
+__device__ __forceinline__ void fill_bins(const Row& r, int from, int to, Bins& b) {
+  const bool count_only = few(r);
+  each_token(r.x, from + (int)threadIdx.x, to, THREADS, [&](int, float x) {
+    const int bin = bin_of(r, x);
+    if (bin == kBins) return;
+    atomicAdd(&b.count[bin], 1u);
+    if (!count_only) atomicAdd(&b.mass[bin], whole(weight(r, x)));
+  });
 }
 // Sums over the bins before this thread's first (it has kBins / THREADS of them), and over all.
 template <int THREADS, class Work>
@@ -206,6 +234,11 @@ __device__ __forceinline__ Borders borders(const Row& r, const Bins& b, Work& w)
   }
   Borders o = {0, -1, 0, 0, 0, counted ? 0 : all_m};
   const int kbin = (int)w.found[0];
+  if (few(r)) {                    // all that top-k keeps, or all there are; without masses
+    o.b1 = counted ? kbin : kBins - 1;
+    o.size = counted ? w.found[2] : all_c;
+    return o;
+  }
   // the least that the total of top-k can be: its border bin is not resolved yet
   const double target = r.p > 0 ? r.p * (double)(counted ? w.found[1] : all_m) : 0;
   if (r.by_mass) {
@@ -236,6 +269,11 @@ __device__ __forceinline__ Borders borders(const Row& r, const Bins& b, Work& w)
   return o;
 }
 
+// The weight of a token by its order.
+__device__ __forceinline__ u64 listed_weight(const Row& r, u64 order) {
+  const uint32_t key = (uint32_t)(order >> 32);
+  return key == kNoKey ? 0 : whole(weight(r, value_of(key)));
+}
 // Sorts the first n of w.list: bitonic, a thread having every THREADS-th token. Steps of 1 to 32 places are exchanges of lanes, those of
 // THREADS and more a thread's own; the rest go through LDS, 10 of 55 steps for 1024 tokens of 1024 threads.
 template <int THREADS, int LIST>
@@ -295,7 +333,7 @@ __device__ __forceinline__ u64 bound_of_list(const Row& r, const Borders& o, int
 #pragma unroll
   for (int e = 0; e < N; ++e) {
     const int i = tid * N + e;
-    m[e] = i < kept ? whole(r, weight(distance(r, value_of((uint32_t)(w.list[i] >> 32))))) : 0;
+    m[e] = i < kept ? listed_weight(r, w.list[i]) : 0;
     sum += m[e];
   }
   const u64 scan = wave_scan(sum);
@@ -352,12 +390,12 @@ __device__ __forceinline__ Border find_border(const Row& r, Border within, doubl
       if (k == kNoKey || k > within.key || (shift < 32 && (k >> shift) != (lo >> shift))) continue;
       const uint32_t bin = (k >> next) & ((1u << bits) - 1);
       atomicAdd(&b.count[bin], 1u);
-      if (k < within.key) atomicAdd(&b.mass[bin], whole(r, weight(distance(r, v))));
+      if (k < within.key) atomicAdd(&b.mass[bin], whole(weight(r, v)));
     }
     __syncthreads();
     // the last key's ties that count
     if (tid == 0 && within.key != kNoKey && (shift == 32 || (within.key >> shift) == (lo >> shift)))
-      b.mass[(within.key >> next) & ((1u << bits) - 1)] += within.ties * whole(r, weight(distance(r, value_of(within.key))));
+      b.mass[(within.key >> next) & ((1u << bits) - 1)] += within.ties * whole(weight(r, value_of(within.key)));
     if (tid == 0) w.found[0] = kBins;
     __syncthreads();
     u64 c, m, all_c, all_m;
@@ -397,7 +435,7 @@ __device__ __forceinline__ Border find_border(const Row& r, Border within, doubl
     mass_before += w.found[3];
     shift = next;
   }
-  const u64 one = whole(r, weight(distance(r, value_of(lo))));
+  const u64 one = whole(weight(r, value_of(lo)));
   u64 ties = w.found[4];           // of key lo, all there are
   if (lo == within.key) ties = min(ties, within.ties);
   if (COUNT) {
@@ -418,6 +456,18 @@ __device__ __forceinline__ Border find_border(const Row& r, Border within, doubl
 }
 template <int THREADS, class Work>
 __device__ __forceinline__ u64 bound_by_walks(const Row& r, u64 all_mass, Bins& b, Work& w) {
+  if (r.by_mass && few(r)) {       // the mass of all was not needed so far
+    u64 sum = 0;
+    for (int i = threadIdx.x; i < r.V; i += THREADS)
+      if (key_of(r.x[i]) != kNoKey) sum += whole(weight(r, r.x[i]));
+    sum = wave_sum(sum);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) w.sums[0][threadIdx.x >> 6] = sum;
+    __syncthreads();
+    all_mass = 0;
+    for (int k = 0; k < THREADS / 64; ++k) all_mass += w.sums[0][k];
+    __syncthreads();
+  }
   Border kept = {kNoKey, 0};
   u64 total = all_mass;
   if (r.by_count) kept = find_border<THREADS, true>(r, kept, 0, b, w, &total);
@@ -451,10 +501,9 @@ __device__ __forceinline__ u64 bound_by_walks(const Row& r, u64 all_mass, Bins& 
 
 // The weight that token i has in the choice.
 __device__ __forceinline__ u64 kept_weight(const Row& r, u64 bound, int i, float x) {
-  const uint32_t k = key_of(x);
-  if (k == kNoKey || order_of(k, i) > bound) return 0;
-  const double z = distance(r, x), w = weight(z);
-  return w >= r.least || z == 0 ? whole(r, w) : 0;
+  if (!(x > -INFINITY) || x < value_of((uint32_t)(bound >> 32)) || order_of(key_of(x), i) > bound) return 0;
+  const double w = weight(r, x);
+  return w >= r.least || x == r.top ? whole(w) : 0;
 }
 // Sum of the weights of [from, to), by a wavefront.
 __device__ __forceinline__ u64 stretch_sum(const Row& r, u64 bound, int from, int to) {
@@ -512,23 +561,20 @@ __global__ __launch_bounds__(THREADS) void sample_short(SampleDesc s) {
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* x = s.logits + row * s.V;
-  u64 first = kAll;
   float v[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) v[e] = x[min(e * THREADS + tid, s.V - 1)];
 #pragma unroll
   for (int e = 0; e < N; ++e) {
     const int i = e * THREADS + tid;
-    const u64 o = i < s.V ? order_of(key_of(v[e]), i) : kAll;
-    w.list[i] = o;
-    first = o < first ? o : first;
+    w.list[i] = i < s.V ? order_of(key_of(v[e]), i) : kAll;
   }
-  first = block_min<THREADS>(first, w);
-  const Row r = row_of(s, row, value_of((uint32_t)(first >> 32)));
-  if ((uint32_t)(first >> 32) == kNoKey || r.greedy) {
-    if (tid == 0) s.token[row] = (uint32_t)(first >> 32) == kNoKey ? -1 : (int32_t)(uint32_t)first;
+  const float top = block_top<THREADS>(x, 0, s.V, w);
+  if (top == -INFINITY) {
+    if (tid == 0) s.token[row] = -1;
     return;
   }
+  const Row r = row_of(s, row, top);
   const u64 bound = r.by_count || r.by_mass ? bound_of_list<THREADS, LIST>(r, {0, 0, 0, 0, 0, 0}, s.V, w) : kAll;
   u64 mine = 0;
 #pragma unroll
@@ -550,38 +596,24 @@ __global__ __launch_bounds__(THREADS) void sample_one(SampleDesc s) {
   __shared__ Work<kList> w;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  u64 first = kAll;
-  each_token(s.logits + row * s.V, tid, s.V, THREADS, [&](int i, float x) {
-    const u64 o = order_of(key_of(x), i);
-    first = o < first ? o : first;
-  });
-  for (int i = tid; i < kBins; i += THREADS) {
-    bins.mass[i] = 0;
-    bins.count[i] = 0;
-  }
+  clear_bins<THREADS>(bins);
   if (tid == 0) w.listed = 0;
-  first = block_min<THREADS>(first, w);
-  const Row r = row_of(s, row, value_of((uint32_t)(first >> 32)));
-  if ((uint32_t)(first >> 32) == kNoKey || r.greedy) {
-    if (tid == 0) s.token[row] = (uint32_t)(first >> 32) == kNoKey ? -1 : (int32_t)(uint32_t)first;
+  const float top = block_top<THREADS>(s.logits + row * s.V, 0, s.V, w);
+  if (top == -INFINITY) {
+    if (tid == 0) s.token[row] = -1;
     return;
   }
+  const Row r = row_of(s, row, top);
   u64 bound = kAll;
   if (r.by_count || r.by_mass) {
-    each_token(r.x, tid, s.V, THREADS, [&](int, float x) {
-      const double z = distance(r, x);
-      const int bin = bin_of(r, z);
-      if (bin == kBins) return;
-      atomicAdd(&bins.count[bin], 1u);
-      atomicAdd(&bins.mass[bin], whole(r, weight(z)));
-    });
+    fill_bins<THREADS>(r, 0, s.V, bins);
     __syncthreads();
     const Borders o = borders<THREADS>(r, bins, w);
-    if (__builtin_expect(o.b1 >= 0 && o.size > kList, 0)) {
+    if (__builtin_expect(o.size > kList, 0)) {
       bound = bound_by_walks<THREADS>(r, o.all, bins, w);
     } else if (o.b1 >= 0) {
       each_token(r.x, tid, s.V, THREADS, [&](int i, float x) {
-        const int bin = bin_of(r, distance(r, x));
+        const int bin = bin_of(r, x);
         if (bin >= o.b0 && bin <= o.b1) w.list[atomicAdd(&w.listed, 1u)] = order_of(key_of(x), i);
       });
       __syncthreads();
@@ -615,25 +647,22 @@ struct PartArgs {
   SampleDesc s;
   int parts, each;                 // tokens of a part, a multiple of 64 a wavefront
   RowSpace* rows;
-  u64 *tops, *sums;                // [rows][parts], [rows][parts * kPartWaves]
+  float* tops;                     // [rows][parts]
+  u64* sums;                       // [rows][parts * kPartWaves]
 };
-__device__ __forceinline__ u64 first_of(const PartArgs& a, int64_t row) {
-  u64 first = kAll;
-  for (int k = threadIdx.x & 63; k < a.parts; k += 64) first = min(first, a.tops[row * a.parts + k]);
-  return wave_min(first);
+// The row's largest logit; minus infinity: none.
+__device__ __forceinline__ float top_of(const PartArgs& a, int64_t row) {
+  float top = -INFINITY;
+  for (int k = threadIdx.x & 63; k < a.parts; k += 64) top = fmaxf(top, a.tops[row * a.parts + k]);
+  return wave_max(top);
 }
 __global__ __launch_bounds__(kPartThreads) void sample_tops(PartArgs a) {
   __shared__ Work<64> w;
   const int part = blockIdx.x;
   const int64_t row = blockIdx.y;
   const int tid = threadIdx.x, from = part * a.each, to = min(from + a.each, a.s.V);
-  u64 first = kAll;
-  each_token(a.s.logits + row * a.s.V, from + tid, to, kPartThreads, [&](int i, float x) {
-    const u64 o = order_of(key_of(x), i);
-    first = o < first ? o : first;
-  });
-  first = block_min<kPartThreads>(first, w);
-  if (tid == 0) a.tops[row * a.parts + part] = first;
+  const float top = block_top<kPartThreads>(a.s.logits + row * a.s.V, from, to, w);
+  if (tid == 0) a.tops[row * a.parts + part] = top;
   RowSpace& sp = a.rows[row];
   for (int i = part * kPartThreads + tid; i < kBins; i += a.parts * kPartThreads) {
     sp.bins.mass[i] = 0;
@@ -645,45 +674,43 @@ __global__ __launch_bounds__(kPartThreads) void sample_bins(PartArgs a) {
   __shared__ Bins bins;
   const int part = blockIdx.x, tid = threadIdx.x, from = part * a.each, to = min(from + a.each, a.s.V);
   const int64_t row = blockIdx.y;
-  const u64 first = first_of(a, row);
-  const Row r = row_of(a.s, row, value_of((uint32_t)(first >> 32)));
-  if ((uint32_t)(first >> 32) == kNoKey || r.greedy || !(r.by_count || r.by_mass)) return;
-  for (int i = tid; i < kBins; i += kPartThreads) {
-    bins.mass[i] = 0;
-    bins.count[i] = 0;
-  }
+  const float top = top_of(a, row);
+  const Row r = row_of(a.s, row, top);
+  if (top == -INFINITY || !(r.by_count || r.by_mass)) return;
+  clear_bins<kPartThreads>(bins);
   __syncthreads();
-  each_token(r.x, from + tid, to, kPartThreads, [&](int, float x) {
-    const double z = distance(r, x);
-    const int bin = bin_of(r, z);
-    if (bin == kBins) return;
-    atomicAdd(&bins.count[bin], 1u);
-    atomicAdd(&bins.mass[bin], whole(r, weight(z)));
-  });
+  fill_bins<kPartThreads>(r, from, to, bins);
   __syncthreads();
   RowSpace& sp = a.rows[row];
   for (int i = tid; i < kBins; i += kPartThreads)
     if (bins.count[i]) {
       atomicAdd(&sp.bins.count[i], bins.count[i]);
-      atomicAdd(&sp.bins.mass[i], bins.mass[i]);
+      if (bins.mass[i]) atomicAdd(&sp.bins.mass[i], bins.mass[i]);
     }
 }
-// Lists the tokens of the border's bins.
+// Lists the tokens of the border's bins: in LDS first, so that a block takes its places in the row's list at once.
 __global__ __launch_bounds__(kPartThreads) void sample_list(PartArgs a) {
-  __shared__ Work<64> w;
+  __shared__ Work<kList> w;
   const int part = blockIdx.x, tid = threadIdx.x, from = part * a.each, to = min(from + a.each, a.s.V);
   const int64_t row = blockIdx.y;
-  const u64 first = first_of(a, row);
-  const Row r = row_of(a.s, row, value_of((uint32_t)(first >> 32)));
-  if ((uint32_t)(first >> 32) == kNoKey || r.greedy || !(r.by_count || r.by_mass)) return;
+  const float top = top_of(a, row);
+  const Row r = row_of(a.s, row, top);
+  if (top == -INFINITY || !(r.by_count || r.by_mass)) return;
   RowSpace& sp = a.rows[row];
+  if (tid == 0) w.listed = 0;
   const Borders o = borders<kPartThreads>(r, sp.bins, w);
   if (part == 0 && tid == 0) sp.borders = o;
   if (o.b1 < 0 || o.size > kList) return;
   each_token(r.x, from + tid, to, kPartThreads, [&](int i, float x) {
-    const int bin = bin_of(r, distance(r, x));
-    if (bin >= o.b0 && bin <= o.b1) sp.list[atomicAdd(&sp.listed, 1ull)] = order_of(key_of(x), i);
+    const int bin = bin_of(r, x);
+    if (bin >= o.b0 && bin <= o.b1) w.list[atomicAdd(&w.listed, 1u)] = order_of(key_of(x), i);
   });
+  __syncthreads();
+  const int n = (int)w.listed;
+  if (n == 0) return;
+  if (tid == 0) w.found[7] = atomicAdd(&sp.listed, (u64)n);
+  __syncthreads();
+  for (int i = tid; i < n; i += kPartThreads) sp.list[w.found[7] + i] = w.list[i];
 }
 // The bound of what is kept, a block a row.
 __global__ __launch_bounds__(1024) void sample_bound(PartArgs a) {
@@ -691,13 +718,13 @@ __global__ __launch_bounds__(1024) void sample_bound(PartArgs a) {
   __shared__ Bins bins;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
-  const u64 first = first_of(a, row);
-  const Row r = row_of(a.s, row, value_of((uint32_t)(first >> 32)));
+  const float top = top_of(a, row);
+  const Row r = row_of(a.s, row, top);
   RowSpace& sp = a.rows[row];
   u64 bound = kAll;
-  if ((uint32_t)(first >> 32) != kNoKey && !r.greedy && (r.by_count || r.by_mass)) {
+  if (top > -INFINITY && (r.by_count || r.by_mass)) {
     const Borders o = sp.borders;
-    if (__builtin_expect(o.b1 >= 0 && o.size > kList, 0)) {
+    if (__builtin_expect(o.size > kList, 0)) {
       bound = bound_by_walks<1024>(r, o.all, bins, w);
     } else if (o.b1 >= 0) {
       for (int i = tid; i < (int)o.size; i += 1024) w.list[i] = sp.list[i];
@@ -710,9 +737,9 @@ __global__ __launch_bounds__(1024) void sample_bound(PartArgs a) {
 __global__ __launch_bounds__(kPartThreads) void sample_sums(PartArgs a) {
   const int part = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
   const int64_t row = blockIdx.y;
-  const u64 first = first_of(a, row);
-  const Row r = row_of(a.s, row, value_of((uint32_t)(first >> 32)));
-  if ((uint32_t)(first >> 32) == kNoKey || r.greedy) return;
+  const float top = top_of(a, row);
+  const Row r = row_of(a.s, row, top);
+  if (top == -INFINITY) return;
   const int each = a.each / kPartWaves, from = min(part * a.each + wave * each, a.s.V), to = min(from + each, a.s.V);
   const u64 sum = stretch_sum(r, a.rows[row].bound, from, to);
   if ((tid & 63) == 0) a.sums[(row * a.parts + part) * kPartWaves + wave] = sum;
@@ -722,10 +749,10 @@ __global__ __launch_bounds__(kPartThreads) void sample_pick(PartArgs a) {
   __shared__ Work<64> w;
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x & 63;
-  const u64 first = first_of(a, row);
-  const Row r = row_of(a.s, row, value_of((uint32_t)(first >> 32)));
-  if ((uint32_t)(first >> 32) == kNoKey || r.greedy) {
-    if (threadIdx.x == 0) a.s.token[row] = (uint32_t)(first >> 32) == kNoKey ? -1 : (int32_t)(uint32_t)first;
+  const float top = top_of(a, row);
+  const Row r = row_of(a.s, row, top);
+  if (top == -INFINITY) {
+    if (threadIdx.x == 0) a.s.token[row] = -1;
     return;
   }
   const int n = a.parts * kPartWaves, each = a.each / kPartWaves;
@@ -760,7 +787,7 @@ SamplePlan sample_plan(const SampleDesc& s) {
   p.parts = (s.V + p.each - 1) / p.each;
   if (p.parts > 1) {
     p.tops = s.rows * (int64_t)sizeof(RowSpace);
-    p.sums = p.tops + s.rows * p.parts * 8;
+    p.sums = p.tops + (s.rows * p.parts * 4 + 7) / 8 * 8;
     p.bytes = p.sums + s.rows * p.parts * kPartWaves * 8;
   }
   return p;
@@ -780,8 +807,8 @@ void sample(const SampleDesc& s, void* work, hipStream_t st) {
     return;
   }
   char* w = (char*)work;
-  const PartArgs a{s, p.parts, p.each, (RowSpace*)w, (u64*)(w + p.tops), (u64*)(w + p.sums)};
-  const bool limits = s.top_k || s.top_p || (s.top_k1 > 0 && s.top_k1 < s.V) || s.top_p1 < 1;
+  const PartArgs a{s, p.parts, p.each, (RowSpace*)w, (float*)(w + p.tops), (u64*)(w + p.sums)};
+  const bool limits = s.temperature || !(s.temperature1 > 0) || s.top_k || s.top_p || (s.top_k1 > 0 && s.top_k1 < s.V) || s.top_p1 < 1;
   klaunch(sample_tops, grid, block, 0, st, a);
   if (limits) {
     klaunch(sample_bins, grid, block, 0, st, a);
