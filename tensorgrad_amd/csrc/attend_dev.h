@@ -128,13 +128,15 @@ struct Sight {
   const int32_t* doc;
   bool causal, positional;
 };
+// WIN: false where there is no window, so that nothing is left of it in a kernel.
+template <bool WIN = true>
 __device__ __forceinline__ Sight sight(const AttendDesc& a, int b) {
   Sight s;
   s.n = a.lengths ? min(max(a.lengths[b], 0), a.Tk) : a.Tk;
   s.first = s.n - a.Tq;
   s.prefix = a.prefix ? a.prefix[b] : 0;
-  s.window = a.window;
-  s.stay = max(a.sinks, s.prefix);
+  s.window = WIN ? a.window : 0;
+  s.stay = WIN ? max(a.sinks, s.prefix) : 0;
   s.doc = a.documents ? a.documents + (int64_t)b * a.Tk : nullptr;
   s.causal = a.causal;
   s.positional = a.positional;
@@ -476,7 +478,16 @@ struct Walk {
   int t0, t1, g0, g1;
   __device__ __forceinline__ int after(int t) const { return t + 1 == g0 ? g1 : t + 1; }
 };
+template <bool WIN>
 __device__ __forceinline__ Walk walk_part(int t0, int t1, Gap gap, int split, int splits) {
+  if (!WIN) {                      // no gap
+    if (splits > 1) {
+      const int each = (t1 - t0 + splits - 1) / splits;
+      t0 = min(t0 + split * each, t1);
+      t1 = min(t0 + each, t1);
+    }
+    return {t0, t1, t0, t0};
+  }
   int g0 = min(max(gap.g0, t0), t1), g1 = min(max(gap.g1, g0), t1);
   if (g0 == t0) t0 = g1;
   if (t0 >= g0) g0 = g1 = t0;      // no gap inside

@@ -213,7 +213,7 @@ __device__ __forceinline__ void plain_rows(const TilesArgs& A, const Sight& s, i
 // Bound by the issue of products and vector work together, which overlap only between wavefronts: 4096 x 4096 pairs without
 // masks, 8 heads of 128: 204 us, 337 TFLOP/s of the 443 that three f16 products for one allow; capped and causal: 156 us. k and
 // v come two tiles in turn: the next one travels while this one is multiplied.
-template <int DP, bool CAP, bool SLOPES>
+template <int DP, bool CAP, bool SLOPES, bool WIN>
 __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   constexpr int N = DP / 32, F = 4 * N, F_V = F, F_SIDE = 2 * F, NF = F_SIDE + kSideFrags;
   __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   if (item >= A.blocks * A.splits) return;
   const int split = item % A.splits, blk = A.blocks - 1 - item / A.splits;   // the last rows see the most keys: first
   const int b = slab / a.Hk, hk = slab % a.Hk, G = (int)A.group.d;
-  const Sight s = sight(a, b);
+  const Sight s = sight<WIN>(a, b);
   const int tiles = (a.Tk + kTile - 1) / kTile;
 
   // this lane's query
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   const Gap gap = gap_before(s, max(s.first + (int)fastdiv((uint32_t)(blk * 128), A.group), 0));
   const Range range_ = tile_range(s, 0, (t1 + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax,
                                   infinite && sees_any(s, below, doc), range, gap);
-  const Walk walk = walk_part(range_.t0, range_.t1, gap, split, A.splits);
+  const Walk walk = walk_part<WIN>(range_.t0, range_.t1, gap, split, A.splits);
   t0 = walk.t0;
   t1 = walk.t1;
   if (__builtin_expect(range_.odd, 0)) {
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(512, 4) void attend_tiles(TilesArgs A) {
   if (t0 < t1) fetch(0, 0);
   for (int t = t0, next, buf = 0; t < t1; t = next, buf ^= 1) {
     const int j0 = t * kTile;
-    next = walk.after(t);
+    next = WIN ? walk.after(t) : t + 1;
     loads_done();
     __syncthreads();
     if (next < t1) fetch(buf ^ 1, next - t);
@@ -373,12 +373,12 @@ struct FewArgs {
 // whatever came before); the 32 groups of a block are joined once at its end. A part is the same number of keys
 // for every batch entry, so that blocks past a short one end at once and those that work are alike. 8 caches of up to 16000
 // keys, 4 key heads of 128, 16 query heads: 67 to 68 us, 5.8 TB/s.
-template <int E, int R, bool WIDE>
+template <int E, int R, bool WIDE, bool WIN>
 __global__ __launch_bounds__(256) void attend_few(FewArgs A) {
   const AttendDesc& a = A.a;
   const int tid = threadIdx.x, sub = tid & 7, grp = tid >> 3;
   const int split = blockIdx.x % A.splits, slab = blockIdx.x / A.splits, b = slab / a.Hk, hk = slab % a.Hk, G = a.H / a.Hk;
-  const Sight s = sight(a, b);
+  const Sight s = sight<WIN>(a, b);
   auto feature = [&](int e) { return WIDE ? 4 * (sub + 8 * (e / 4)) + e % 4 : sub + 8 * e; };
   auto load = [&](const float* row, int n, float (&x)[E]) {
     if (WIDE) {
@@ -641,17 +641,26 @@ Plan plan(const AttendDesc& a) {
   return p;
 }
 
+template <int DP, bool WIN>
+void run_tiles(const TilesArgs& t, unsigned grid, hipStream_t st) {
+  if (t.a.cap > 0 && t.a.slopes) klaunch(attend_tiles<DP, true, true, WIN>, dim3(grid), dim3(512), 0, st, t);
+  else if (t.a.cap > 0) klaunch(attend_tiles<DP, true, false, WIN>, dim3(grid), dim3(512), 0, st, t);
+  else if (t.a.slopes) klaunch(attend_tiles<DP, false, true, WIN>, dim3(grid), dim3(512), 0, st, t);
+  else klaunch(attend_tiles<DP, false, false, WIN>, dim3(grid), dim3(512), 0, st, t);
+}
+// A window has kernels of its own: in one, the others' walks took 3 to 7 % longer.
 template <int DP>
 void run_tiles(const TilesArgs& t, unsigned grid, hipStream_t st) {
-  if (t.a.cap > 0 && t.a.slopes) klaunch(attend_tiles<DP, true, true>, dim3(grid), dim3(512), 0, st, t);
-  else if (t.a.cap > 0) klaunch(attend_tiles<DP, true, false>, dim3(grid), dim3(512), 0, st, t);
-  else if (t.a.slopes) klaunch(attend_tiles<DP, false, true>, dim3(grid), dim3(512), 0, st, t);
-  else klaunch(attend_tiles<DP, false, false>, dim3(grid), dim3(512), 0, st, t);
+  if (t.a.window) run_tiles<DP, true>(t, grid, st);
+  else run_tiles<DP, false>(t, grid, st);
 }
 template <int E, int R>
 void run_few(const FewArgs& f, bool wide, int slabs, hipStream_t st) {
-  if (wide) klaunch(attend_few<E, R, true>, dim3(f.splits * slabs), dim3(256), 0, st, f);
-  else klaunch(attend_few<E, R, false>, dim3(f.splits * slabs), dim3(256), 0, st, f);
+  const dim3 grid(f.splits * slabs);
+  if (wide && f.a.window) klaunch(attend_few<E, R, true, true>, grid, dim3(256), 0, st, f);
+  else if (wide) klaunch(attend_few<E, R, true, false>, grid, dim3(256), 0, st, f);
+  else if (f.a.window) klaunch(attend_few<E, R, false, true>, grid, dim3(256), 0, st, f);
+  else klaunch(attend_few<E, R, false, false>, grid, dim3(256), 0, st, f);
 }
 template <int E>
 void run_few_rows(const FewArgs& f, bool wide, int slabs, hipStream_t st) {

@@ -114,7 +114,7 @@ __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, in
 // Eight wavefronts of 16 keys. WHAT: 1 for dk, 2 for dv, 3 for both in one walk. Up to head size 64 two blocks share a CU. Both
 // gradients of 4096 capped causal rows of 16 heads of 128: 679 us (by 32 keys 990, in walks of their own); of 8 heads of 64:
 // 194 us (205); of 8 x 1000 rows of 8 heads of 64 in documents of 170: 66 us (81); of 32 without documents: 87 us.
-template <int DP, bool RICH, int WHAT>
+template <int DP, bool RICH, int WHAT, bool WIN>
 __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs A) {
   constexpr int N = DP / 32, F = 4 * N;                      // chunks of 32 features; fragments of an operand
   constexpr bool DK = WHAT & 1, DV = WHAT & 2;
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
   if (item >= A.blocks * A.splits) return;
   const int split = A.splits - 1 - item / A.blocks, blk = item % A.blocks;   // blocks that start together walk the same rows
   const int b = slab / a.Hk, hk = slab % a.Hk;
-  const Sight s = sight(a, b);
+  const Sight s = sight<WIN>(a, b);
   const int j0 = blk * 128 + w * 16, jt = j0 / kTile * kTile, j = j0 + l;   // masks are judged by whole tiles of keys
   const bool valid = j < a.Tk;
   const int doc = s.doc && valid ? s.doc[j] : -1;
@@ -370,7 +370,7 @@ __device__ __forceinline__ void plain_dq(const GradArgs& A, const Sight& s, int 
 
 // Eight wavefronts of 16 query rows. 4096 capped causal rows of 16 heads of 128: 374 us (470 by 32 rows); 8 x 1000 rows of 8
 // heads of 64 in documents of 170: 42 us (57).
-template <int DP, bool RICH>
+template <int DP, bool RICH, bool WIN>
 __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   constexpr int N = DP / 32, F = 4 * N, F_V = F, F_KC = 2 * F, F_SIDE = 3 * F, NF = F_SIDE + kSideFrags;
   __shared__ __align__(16) _Float16 lds[2 * NF * kFrag];
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   if (item >= rblocks * A.qsplits) return;
   const int split = item % A.qsplits, blk = rblocks - 1 - item / A.qsplits;
   const int b = slab / a.Hk, hk = slab % a.Hk, G = (int)A.group.d;
-  const Sight s = sight(a, b);
+  const Sight s = sight<WIN>(a, b);
   const int row0 = blk * 128 + w * 16, r = row0 + l, rr = min(r, A.M - 1);
   const bool valid = r < A.M;
   const int i = (int)fastdiv((uint32_t)rr, A.group), g = rr - i * G, head = hk * G + g;
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   if (s.positional && last < 0) end = 0;
   const Gap gap = gap_before(s, max(s.first + (int)fastdiv((uint32_t)(blk * 128), A.group), 0));
   const Range range_ = tile_range(s, 0, (end + kTile - 1) / kTile, ki, ki, vi, me.dmin, me.dmax, own, range, gap);
-  const Walk walk = walk_part(range_.t0, range_.t1, gap, split, A.qsplits);
+  const Walk walk = walk_part<WIN>(range_.t0, range_.t1, gap, split, A.qsplits);
   const int t0 = walk.t0, t1 = walk.t1;
   if (__builtin_expect(range_.odd, 0)) {
     plain_dq(A, s, split, slab, b, hk, row0, t0 * kTile, t1 * kTile);
@@ -446,7 +446,7 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
   if (t0 < t1) fetch(0, 0);
   for (int t = t0, next, buf = 0; t < t1; t = next, buf ^= 1) {
     const int j0 = t * kTile;
-    next = walk.after(t);
+    next = WIN ? walk.after(t) : t + 1;
     loads_done();
     __syncthreads();
     if (next < t1) fetch(buf ^ 1, next - t);
@@ -545,19 +545,23 @@ GradPlan grad_plan(const AttendGradDesc& g) {
   return p;
 }
 
-template <int DP, bool RICH>
+template <int DP, bool RICH, bool WIN>
 void run_grad(const GradArgs& A, int slabs, hipStream_t st) {
   const AttendGradDesc& g = A.g;
   const dim3 keys(place_grid(slabs, (int64_t)A.blocks * A.splits));
-  if (g.dk.p && g.dv.p) klaunch(attend_grad_kv<DP, RICH, 3>, keys, dim3(512), 0, st, A);
-  else if (g.dk.p) klaunch(attend_grad_kv<DP, RICH, 1>, keys, dim3(512), 0, st, A);
-  else if (g.dv.p) klaunch(attend_grad_kv<DP, RICH, 2>, keys, dim3(512), 0, st, A);
-  if (g.dq.p) klaunch(attend_grad_q<DP, RICH>, dim3(place_grid(slabs, (int64_t)((A.M + 127) / 128) * A.qsplits)), dim3(512), 0, st, A);
+  if (g.dk.p && g.dv.p) klaunch(attend_grad_kv<DP, RICH, 3, WIN>, keys, dim3(512), 0, st, A);
+  else if (g.dk.p) klaunch(attend_grad_kv<DP, RICH, 1, WIN>, keys, dim3(512), 0, st, A);
+  else if (g.dv.p) klaunch(attend_grad_kv<DP, RICH, 2, WIN>, keys, dim3(512), 0, st, A);
+  if (g.dq.p)
+    klaunch(attend_grad_q<DP, RICH, WIN>, dim3(place_grid(slabs, (int64_t)((A.M + 127) / 128) * A.qsplits)), dim3(512), 0, st, A);
 }
 template <int DP>
 void run_grad(const GradArgs& A, int slabs, hipStream_t st) {
-  if (A.g.a.cap > 0 || A.g.a.slopes) run_grad<DP, true>(A, slabs, st);
-  else run_grad<DP, false>(A, slabs, st);
+  const bool rich = A.g.a.cap > 0 || A.g.a.slopes;
+  if (rich && A.g.a.window) run_grad<DP, true, true>(A, slabs, st);
+  else if (rich) run_grad<DP, true, false>(A, slabs, st);
+  else if (A.g.a.window) run_grad<DP, false, true>(A, slabs, st);
+  else run_grad<DP, false, false>(A, slabs, st);
 }
 
 }  // namespace
