@@ -21,7 +21,7 @@ struct GradArgs {
   int M, qtiles, ktiles, blocks, splits, qsplits;     // splits: parts of the query rows; qsplits: parts of the keys
   bool wide;
   float *pk, *pv, *pq;                                // parts: of dk, dv [split][slab][Tk][D or Dv], of dq [qsplit][slab][M][D]
-  int* parts;                                         // with documents: parts of dk and dv that were written, [slab][blocks]
+  int* parts;                                         // with documents or a window: parts of dk and dv that were written, [slab][blocks]
 };
 
 // ---- dk, dv --------------------------------------------------------------------------------------
@@ -39,21 +39,22 @@ __device__ __forceinline__ void seeing_tiles(const GradArgs& A, const Sight& s, 
   }
 }
 // Those of part `split`, equal stretches of all rows, so that blocks that run together walk the same ones. False: none, which
-// the join finds again and does not read. With documents the stretch that a key block's own see is short: there its tiles are
-// cut into equal parts, of 8 at least, when they are known (8 x 1000 positions, 2 key heads of 64: documents of 50 take 47 us and
+// the join finds again and does not read. With documents or a window the stretch that sees a key block is short: there its tiles are
+// cut into equal parts, of 8 at least (a window: of 20, and the long ones of keys that stay start first: 4096 rows of 4 slabs, head
+// size 128, a window of 512 and 4 sinks 373 us, by equal stretches of all rows 409), when they are known (8 x 1000 positions, 2 key heads of 64: documents of 50 take 47 us and
 // 10 to join instead of 121 uncut, of 170 66 and 11 instead of 165, one document 120 and 13 instead of 282).
 __device__ __forceinline__ bool part_rows(const GradArgs& A, const Sight& s, int k0, int split, int& from, int& to) {
   seeing_tiles(A, s, k0, from, to);
-  if (A.splits == 1 || s.doc) return true;
+  if (A.splits == 1 || s.doc || s.window) return true;
   const int each = (A.qtiles + A.splits - 1) / A.splits;
   from = max(from, split * each);
   to = min(to, (split + 1) * each);
   return from < to;
 }
 
-__device__ __forceinline__ bool document_part(const GradArgs& A, const Sight& s, int split, int slab, int blk, int& t0, int& t1) {
-  if (!s.doc || A.splits == 1) return true;
-  const int each = max((t1 - t0 + A.splits - 1) / A.splits, 8);
+__device__ __forceinline__ bool own_part(const GradArgs& A, const Sight& s, int split, int slab, int blk, int& t0, int& t1) {
+  if (!(s.doc || s.window) || A.splits == 1) return true;
+  const int each = max((t1 - t0 + A.splits - 1) / A.splits, s.doc ? 8 : 20);
   if (split == 0 && threadIdx.x == 0) A.parts[slab * A.blocks + blk] = (t1 - t0 + each - 1) / each;
   t0 += split * each;
   t1 = min(t0 + each, t1);
@@ -126,7 +127,8 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
   int slab, item;
   place(blockIdx.x, a.B * a.Hk, slab, item);
   if (item >= A.blocks * A.splits) return;
-  const int split = A.splits - 1 - item / A.blocks, blk = item % A.blocks;   // blocks that start together walk the same rows
+  // blocks that start together walk the same rows; with a window, those of the first keys start first
+  const int split = WIN ? item % A.splits : A.splits - 1 - item / A.blocks, blk = WIN ? item / A.splits : item % A.blocks;
   const int b = slab / a.Hk, hk = slab % a.Hk;
   const Sight s = sight<WIN>(a, b);
   const int j0 = blk * 128 + w * 16, jt = j0 / kTile * kTile, j = j0 + l;   // masks are judged by whole tiles of keys
@@ -145,7 +147,7 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
   if (!part_rows(A, s, blk * 128, split, from, to)) return;   // nothing, and the join knows
   const Range range_ = tile_range(s, from, to, gi, qi, gi, mine.dmin, mine.dmax, own, range);
   int t0 = range_.t0, t1 = range_.t1;
-  if (!document_part(A, s, split, slab, blk, t0, t1)) return;
+  if (!own_part(A, s, split, slab, blk, t0, t1)) return;
   if (__builtin_expect(range_.odd, 0)) {
     plain_keys<WHAT>(A, s, split, slab, b, hk, j0, t0 * kTile, t1 * kTile);
     return;
@@ -287,7 +289,7 @@ __global__ __launch_bounds__(256) void attend_grad_join(GradArgs A) {
   const int b = slab / a.Hk, hk = slab % a.Hk;
   const Sight s = sight(a, b);
   int first = 0, last = A.qsplits - 1;   // parts that were written
-  if (what < 2 && s.doc) {
+  if (what < 2 && (s.doc || s.window)) {
     last = A.parts[slab * A.blocks + r0 / 128] - 1;
   } else if (what < 2) {
     first = A.splits;

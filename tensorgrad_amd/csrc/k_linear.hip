@@ -376,39 +376,45 @@ struct Own {
   static constexpr int C = DP / 16;
   float row[C][4];
   f32x4 acc[C];
-  __device__ __forceinline__ void load(const float* at, bool here, int n, int g) {
+  __device__ __forceinline__ void load(const float* at, int n, int g) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int d = 16 * c + 4 * g;
-      f32x4 u;
       if (WIDE) {
-        u = *(const f32x4*)(at + (d < n ? d : 0));
+        const f32x4 u = *(const f32x4*)(at + (d < n ? d : 0));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) row[c][q] = u[q];
       } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) u[q] = at[min(d + q, n - 1)];
+        for (int q = 0; q < 4; ++q) row[c][q] = at[min(d + q, n - 1)];
       }
+    }
+  }
+  // Zero for rows that are not there and past the features. Waits for the rows here: left to the compiler, the wait stands in the
+  // loop over tiles, and there it waits for the next tiles too.
+  __device__ __forceinline__ void start(bool here, int n, int g) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) row[c][q] = here && d + (WIDE ? 0 : q) < n ? u[q] : 0.0f;
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        row[c][q] = here && 16 * c + 4 * g + (WIDE ? 0 : q) < n ? row[c][q] : 0.0f;
+        asm volatile("" : "+v"(row[c][q]));
+      }
       acc[c] = f32x4{};
     }
   }
   // tile rows times own rows: x[q] of tile row 16 (q / 4) + 4 g + q % 4
   __device__ __forceinline__ void dots(const float* tile, float (&x)[8], int g, int l) const {
-    f32x4 s[2] = {}, u[2][2];
+    f32x4 s[2] = {}, u[2];
     int at[4];
     L::by_piece(at, L::opaque(16 * g + l));
-    auto read = [&](int c) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) u[c & 1][k] = *(const f32x4*)(tile + at[c % 4] + (16 * k * L::PITCH + L::far(c)));
-    };
+    auto read = [&](int i) { u[i & 1] = *(const f32x4*)(tile + at[i / 2 % 4] + (16 * (i & 1) * L::PITCH + L::far(i / 2))); };
     read(0);
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      if (c + 1 < C) read(c + 1);
+    for (int i = 0; i < 2 * C; ++i) {
+      if (i + 1 < 2 * C) read(i + 1);
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) s[k] = mfma(u[c & 1][k][q], row[c][q], s[k]);
+      for (int q = 0; q < 4; ++q) s[i & 1] = mfma(u[i & 1][q], row[i / 2][q], s[i & 1]);
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
@@ -441,32 +447,19 @@ struct Own {
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  // acc += what the rows [m0, m0 + 32) of M in the tile give: `across`, features m0.. of the result, else weights of features m0..
+  // acc += what the rows [32 c, 32 c + 32) of M in the tile give: ACROSS, these features of the result, else these features' weights
   template <bool ACROSS>
-  __device__ __forceinline__ void state(const float* tile, int m0, float coef, int g, int l) {
-    float x[8] = {};
+  __device__ __forceinline__ void state(const float* tile, int c, float coef, int g, int l) {
+    float x[8];
     if constexpr (ACROSS) {
       dots(tile, x, g, l);
 #pragma unroll
-      for (int c = 0; c < C; c += 2)
-        if (16 * c == m0)
-#pragma unroll
-          for (int q = 0; q < 8; ++q) acc[c + q / 4][q % 4] = fmaf(coef, x[q], acc[c + q / 4][q % 4]);
+      for (int q = 0; q < 8; ++q) acc[2 * c + q / 4][q % 4] = fmaf(coef, x[q], acc[2 * c + q / 4][q % 4]);
     } else {
 #pragma unroll
-      for (int c = 0; c < C; c += 2)
-        if (16 * c == m0)
-#pragma unroll
-          for (int q = 0; q < 8; ++q) x[q] = row[c + q / 4][q % 4] * coef;
+      for (int q = 0; q < 8; ++q) x[q] = row[2 * c + q / 4][q % 4] * coef;
       add(tile, x, g, l);
     }
-  }
-  // Waits for the rows here: left to the compiler, the wait stands in the loop, and there it waits for the next tile too.
-  __device__ __forceinline__ void arrived() {
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(row[c][q]));
   }
   // Stores the rows; whether they are all finite.
   __device__ __forceinline__ bool store(float* out, bool in, bool here, int n, int g) const {
@@ -508,9 +501,15 @@ __device__ __forceinline__ void weights(float (&x)[8], const PairsArgs& p, const
 }
 
 // W wavefronts of 16 rows. The tiles of M, then those of the pairs, one after another; the next one travels to the other half of LDS
-// while this one is multiplied, so that a tile costs one barrier. Four wavefronts a SIMD: their products, weights and waits overlap.
+// while this one is multiplied, so that a tile costs one barrier. A wavefront walks the tiles that it has nothing to do with in
+// loops of their own: with a branch around the work the compiler copied all 32 registers of results for every tile, and had none
+// left for a second block on the CU.
+template <int DP>
+struct Ring {
+  float tile[2][2][Tile<DP>::FLOATS];
+};
 template <int DP, int W, bool BACK, bool ACROSS>
-__device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int unit, float (&lds)[2][2][Tile<DP>::FLOATS], int (&since)[kSeg]) {
+__device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int unit, Ring<DP>& ring, int (&since)[kSeg]) {
   using L = Tile<DP>;
   const Place o = place_of<BACK>(p, s, unit, 16 * W);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15;
@@ -518,71 +517,82 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
   const int mtiles = o.M ? (p.D + kTile - 1) / kTile : 0, count = mtiles + (o.from < o.to ? (o.to - o.from + kTile - 1) / kTile : 0);
   const int hx = BACK ? o.h0 : o.h0 / p.share;
   const float *M = o.M, *X = row_at(s.x, o.b, hx, 0), *Z = row_at(s.z, o.b, hx, 0);
-  const uint32_t base = lds_address(lds);
-  auto fetch = [&](int k, int buf) {   // a head's tile k: of its M, then of its pairs
-    const uint32_t to = base + buf * (8 * L::FLOATS);
-    if (k < mtiles) {
-      tile_to_lds<DP, W>(M, p.Dv, k * kTile, p.D, p.Dv, to, w);
+  const uint32_t base = lds_address(&ring);
+  int left = count * o.group, next = 0, into = 0;   // tiles to fetch; the next one of its head (of M, then of pairs), and where to
+  auto fetch = [&]() {
+    if (left == 0) return;
+    --left;
+    const uint32_t to = base + into * (8 * L::FLOATS);
+    if (next < mtiles) {
+      tile_to_lds<DP, W>(M, p.Dv, next * kTile, p.D, p.Dv, to, w);
     } else {
-      const int t0 = o.from + (k - mtiles) * kTile;
+      const int t0 = o.from + (next - mtiles) * kTile;
       tile_to_lds<DP, W>(Z, s.z.t, t0, T, s.nz, to, w);
       tile_to_lds<DP, W>(X, s.x.t, t0, T, s.n, to + 4 * L::FLOATS, w);
     }
+    into ^= 1;
+    if (++next == count) {
+      next = 0;
+      if (BACK) {
+        M += (int64_t)p.D * p.Dv;
+        X += s.x.h;
+        Z += s.z.h;
+      }
+    }
   };
-  if (count) fetch(0, 0);
+  fetch();
   Own<DP, true> own;
+  own.load(s.rows.p ? row_at(s.rows, o.b, o.head, min(r, T - 1)) : p.any, s.n, g);
   mark(p.m, o.b, o.s0, o.n, since);
   const Ends end = ends(since, o.s0, o.n);
   const int mine = r < T ? since[r - o.s0] : kNever;
   const bool here = mine != kNever;
-  own.load(s.rows.p ? row_at(s.rows, o.b, o.head, min(r, T - 1)) : p.any, here && s.rows.p, s.n, g);
-  own.arrived();
-  const int steps = count * o.group;
-  float rate = 0, coef = 0;
-  for (int step = 0, k = 0, h = o.h0, buf = 0; step < steps; ++step, buf ^= 1) {
-    if (k == 0) {
-      rate = scalar(p.rate[h]);
-      coef = here ? p.by_state * (BACK ? leaves(end, since, o.s0, r, rate) : comes(since, o.s0, r, rate)) : 0.0f;
-    }
+  own.start(here && s.rows.p, s.n, g);
+  int buf = 1;
+  auto arrive = [&]() {            // the next tile is there, in `buf`, and the one after it on its way
     loads_done();
     __syncthreads();
-    const int k1 = k + 1 < count ? k + 1 : 0;
-    if (BACK && k1 == 0) {
-      M += (int64_t)p.D * p.Dv;
-      X += s.x.h;
-      Z += s.z.h;
-      ++h;
-    }
-    if (step + 1 < steps) fetch(k1, buf ^ 1);
-    const float *z_tile = lds[buf][0], *x_tile = lds[buf][1];
-    if (k < mtiles) {
-      own.template state<ACROSS>(z_tile, k * kTile, coef, g, l);
-    } else {
-      const int t0 = o.from + (k - mtiles) * kTile;
-      if (BACK ? t0 + kTile > w0 : t0 <= w0 + 15) {
-        float x[8], f[8];
-        own.dots(x_tile, x, g, l);
-        weights<BACK>(f, p, o, rate, w0, r, t0, mine, since, g);
+    fetch();
+    buf ^= 1;
+  };
+  for (int gi = 0; gi < o.group; ++gi) {
+    const float rate = scalar(p.rate[o.h0 + gi]);
+    const float coef = here ? p.by_state * (BACK ? leaves(end, since, o.s0, r, rate) : comes(since, o.s0, r, rate)) : 0.0f;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) x[q] = f[q] == 0 ? 0.0f : x[q] * f[q];
-        own.add(z_tile, x, g, l);
+    for (int c = 0; c < DP / 32; ++c)
+      if (c < mtiles) {
+        arrive();
+        own.template state<ACROSS>(ring.tile[buf][0], c, coef, g, l);
       }
+    int t0 = o.from;
+    if (BACK)
+      for (; t0 < min(o.to, w0 - kTile + 1); t0 += kTile) arrive();
+    for (const int stop = BACK ? o.to : min(o.to, w0 + 16); t0 < stop; t0 += kTile) {
+      arrive();
+      float x[8], f[8];
+      own.dots(ring.tile[buf][1], x, g, l);
+      __builtin_amdgcn_sched_barrier(0);
+      weights<BACK>(f, p, o, rate, w0, r, t0, mine, since, g);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) x[q] = f[q] == 0 ? 0.0f : x[q] * f[q];
+      __builtin_amdgcn_sched_barrier(0);
+      own.add(ring.tile[buf][0], x, g, l);
     }
-    k = k1;
+    for (; t0 < o.to; t0 += kTile) arrive();
   }
   const bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here, s.nz, g);
   if (__builtin_expect(!fine, 0)) plain_rows<BACK>(p, s, o, w0, since);
 }
 template <int DP, int W, bool BACK>
-__global__ __launch_bounds__(64 * W, 2) void linear_tiles(PairsArgs p) {
-  __shared__ __align__(16) float lds[2][2][Tile<DP>::FLOATS];
+__global__ __launch_bounds__(64 * W, 4) void linear_tiles(PairsArgs p) {
+  __shared__ __align__(16) Ring<DP> ring;
   __shared__ int since[kSeg];
   // both sums of a place run one after the other on one XCD (blocks go to the 8 XCDs in turn), whose L2 then has their tiles
   const int id = blockIdx.x / 8, unit = (id / p.sums) * 8 + blockIdx.x % 8;
   if (unit >= p.blocks * p.B * p.heads) return;
   const Sum& s = p.sum[id % p.sums];
-  if (s.across) walk_tiles<DP, W, BACK, true>(p, s, unit, lds, since);
-  else walk_tiles<DP, W, BACK, false>(p, s, unit, lds, since);
+  if (s.across) walk_tiles<DP, W, BACK, true>(p, s, unit, ring, since);
+  else walk_tiles<DP, W, BACK, false>(p, s, unit, ring, since);
 }
 
 // The same for any alignment and number of features, tile by tile.
@@ -600,18 +610,21 @@ __global__ __launch_bounds__(256) void linear_pairs(PairsArgs p) {
   const int mine = r < T ? since[r - o.s0] : kNever;
   const bool here = mine != kNever;
   Own<DP, false> own;
-  own.load(s.rows.p ? row_at(s.rows, o.b, o.head, min(r, T - 1)) : p.any, here && s.rows.p, s.n, g);
+  own.load(s.rows.p ? row_at(s.rows, o.b, o.head, min(r, T - 1)) : p.any, s.n, g);
+  own.start(here && s.rows.p, s.n, g);
   for (int gi = 0; gi < o.group; ++gi) {
     const int h = o.h0 + gi, hx = BACK ? h : h / p.share;
     const float rate = p.rate[h];
     if (o.M) {
       const float coef = here ? p.by_state * (BACK ? leaves(end, since, o.s0, r, rate) : comes(since, o.s0, r, rate)) : 0.0f;
-      for (int m0 = 0; m0 < p.D; m0 += kTile) {
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) {
+        if (c * kTile >= p.D) break;
         __syncthreads();
-        tile_by_hand<DP, 256>(z_tile, o.M + (int64_t)gi * p.D * p.Dv, p.Dv, m0, p.D, p.Dv);
+        tile_by_hand<DP, 256>(z_tile, o.M + (int64_t)gi * p.D * p.Dv, p.Dv, c * kTile, p.D, p.Dv);
         __syncthreads();
-        if (s.across) own.template state<true>(z_tile, m0, coef, g, l);
-        else own.template state<false>(z_tile, m0, coef, g, l);
+        if (s.across) own.template state<true>(z_tile, c, coef, g, l);
+        else own.template state<false>(z_tile, c, coef, g, l);
       }
     }
     for (int t0 = o.from; t0 < o.to; t0 += kTile) {
