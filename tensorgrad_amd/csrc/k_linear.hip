@@ -31,7 +31,7 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kSeg = 128;          // positions of a segment
+constexpr int kSeg = kLinearSegment;   // positions of a segment
 constexpr int kTile = 32;          // rows of a tile in LDS
 constexpr int kNever = INT32_MAX;
 
@@ -282,7 +282,7 @@ struct PairsArgs {
   const float *states, *edge;      // [segs][B * H][D][Dv]; at the first segment (back: last) this one, or null
   int D, Dv;
   float by_pair, by_state;         // factors of both parts
-  const float *rate, *any;         // any: some address, for rows that are absent
+  const float *rate, *any;         // any: an address with a feature (wide: 4), for rows that are absent
 };
 __device__ __forceinline__ const float* row_at(const Rows& x, int b, int head, int t) { return x.p + b * x.b + head * x.h + (int64_t)t * x.t; }
 
@@ -542,7 +542,7 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
   };
   fetch();
   Own<DP, true> own;
-  own.load(s.rows.p ? row_at(s.rows, o.b, o.head, min(r, T - 1)) : p.any, s.n, g);
+  own.load(s.rows.p ? row_at(s.rows, o.b, o.head, min(r, T - 1)) : p.any, s.rows.p ? s.n : 1, g);
   mark(p.m, o.b, o.s0, o.n, since);
   const Ends end = ends(since, o.s0, o.n);
   const int mine = r < T ? since[r - o.s0] : kNever;
@@ -584,7 +584,7 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
   if (__builtin_expect(!fine, 0)) plain_rows<BACK>(p, s, o, w0, since);
 }
 template <int DP, int W, bool BACK>
-__global__ __launch_bounds__(64 * W, 4) void linear_tiles(PairsArgs p) {
+__global__ __launch_bounds__(64 * W, W == 8 || DP <= 64 ? 4 : 2) void linear_tiles(PairsArgs p) {
   __shared__ __align__(16) Ring<DP> ring;
   __shared__ int since[kSeg];
   // both sums of a place run one after the other on one XCD (blocks go to the 8 XCDs in turn), whose L2 then has their tiles
@@ -610,7 +610,7 @@ __global__ __launch_bounds__(256) void linear_pairs(PairsArgs p) {
   const int mine = r < T ? since[r - o.s0] : kNever;
   const bool here = mine != kNever;
   Own<DP, false> own;
-  own.load(s.rows.p ? row_at(s.rows, o.b, o.head, min(r, T - 1)) : p.any, s.n, g);
+  own.load(s.rows.p ? row_at(s.rows, o.b, o.head, min(r, T - 1)) : p.any, s.rows.p ? s.n : 1, g);
   own.start(here && s.rows.p, s.n, g);
   for (int gi = 0; gi < o.group; ++gi) {
     const int h = o.h0 + gi, hx = BACK ? h : h / p.share;
@@ -739,10 +739,8 @@ __global__ __launch_bounds__(256) void linear_steps(StepsArgs A) {
 inline bool wide_rows(const Rows& x) { return ((uintptr_t)x.p & 15) == 0 && x.b % 4 == 0 && x.h % 4 == 0 && x.t % 4 == 0 && x.t < (1 << 24); }
 inline int segments(const LinearDesc& a) { return (a.T + kSeg - 1) / kSeg; }
 inline int padded(const LinearDesc& a) { return (std::max(a.D, a.Dv) + 31) / 32 * 32; }
-inline int64_t sums_bytes(const LinearDesc& a) {
-  const int64_t n = (int64_t)segments(a) * a.B * a.H;
-  return (n * a.D * a.Dv * 4 + 255) / 256 * 256 + (n * 4 + 255) / 256 * 256;
-}
+inline int64_t states_bytes(const LinearDesc& a) { return ((int64_t)segments(a) * a.B * a.H * a.D * a.Dv * 4 + 255) / 256 * 256; }
+inline int64_t stay_bytes(const LinearDesc& a) { return ((int64_t)segments(a) * a.B * a.H * 4 + 255) / 256 * 256; }
 
 template <int DP>
 void sums(const SumsArgs& s, bool wide, const dim3& grid, hipStream_t st) {
@@ -750,7 +748,7 @@ void sums(const SumsArgs& s, bool wide, const dim3& grid, hipStream_t st) {
   else klaunch(linear_sums<DP, false>, grid, dim3(256), 0, st, s);
 }
 // States at the borders of all segments (in place of the sums), and the one at the end.
-void states(const LinearDesc& a, const Rows& x, const Rows& y, bool back, const float* first, float* last, float* at, hipStream_t st) {
+void states(const LinearDesc& a, const Rows& x, const Rows& y, bool back, const float* first, float* last, float* at, float* stay, hipStream_t st) {
   SumsArgs s{};
   s.m = {a.documents, a.lengths, a.T};
   s.x = x;
@@ -765,7 +763,7 @@ void states(const LinearDesc& a, const Rows& x, const Rows& y, bool back, const 
   s.rate = a.rate;
   s.sums = at;
   const int64_t rows = (int64_t)a.B * a.H, each = (int64_t)a.D * a.Dv;
-  s.stay = at + (s.segs * rows * each + 63) / 64 * 64;
+  s.stay = stay;
   const bool wide = a.D % 4 == 0 && a.Dv % 4 == 0 && wide_rows(x) && wide_rows(y);
   const dim3 grid((unsigned)(rows * s.segs));
   switch (padded(a)) {
@@ -821,7 +819,10 @@ void steps(const StepsArgs& s, hipStream_t st) { klaunch(linear_steps<DP>, dim3(
 
 }  // namespace
 
-int64_t linear_workspace_bytes(const LinearDesc& a) { return a.T <= kSteps ? 0 : sums_bytes(a); }
+int64_t linear_workspace_bytes(const LinearDesc& a) {
+  if (a.T <= kSteps) return 0;
+  return stay_bytes(a) + (a.borders ? 0 : states_bytes(a));
+}
 
 void linear(const LinearDesc& a, void* work, hipStream_t st) {
   if (a.T <= kSteps) {
@@ -833,26 +834,26 @@ void linear(const LinearDesc& a, void* work, hipStream_t st) {
       default: return steps<128>(s, st);
     }
   }
-  float* at = (float*)work;
-  if (a.last || (a.y.p && segments(a) > 1)) states(a, a.k, a.v, false, a.state, a.last, at, st);
+  float *stay = (float*)work, *at = a.borders ? a.borders : (float*)((char*)work + stay_bytes(a));
+  if (a.last || a.borders || (a.y.p && segments(a) > 1)) states(a, a.k, a.v, false, a.state, a.last, at, stay, st);
   if (!a.y.p) return;
   PairsArgs p{};
   p.sum[p.sums++] = {a.q, a.y, a.k, a.v, a.D, a.Dv, false};
   pairs<false>(p, a, at, a.state, st);
 }
 
-int64_t linear_grad_workspace_bytes(const LinearGradDesc& g) { return 2 * sums_bytes(g.a); }
+int64_t linear_grad_workspace_bytes(const LinearGradDesc& g) { return stay_bytes(g.a) + (g.borders ? 1 : 2) * states_bytes(g.a); }
 
 void linear_grad(const LinearGradDesc& g, void* work, hipStream_t st) {
   const LinearDesc& a = g.a;
-  float *S = (float*)work, *G = (float*)((char*)work + sums_bytes(a));
+  float *stay = (float*)work, *G = (float*)((char*)work + stay_bytes(a)), *S = (float*)((char*)G + states_bytes(a));
   const bool several = segments(a) > 1;
-  if (g.dq.p && several) states(a, a.k, a.v, false, a.state, nullptr, S, st);
-  if (g.dfirst || ((g.dk.p || g.dv.p) && several)) states(a, a.q, g.dy, true, g.dstate, g.dfirst, G, st);
+  if (g.dq.p && several && !g.borders) states(a, a.k, a.v, false, a.state, nullptr, S, stay, st);
+  if (g.dfirst || ((g.dk.p || g.dv.p) && several)) states(a, a.q, g.dy, true, g.dstate, g.dfirst, G, stay, st);
   PairsArgs p{};
   if (g.dq.p) {
     p.sum[p.sums++] = {g.dy, g.dq, a.v, a.k, a.Dv, a.D, true};
-    pairs<false>(p, a, S, a.state, st);
+    pairs<false>(p, a, g.borders ? g.borders : S, a.state, st);
     p.sums = 0;
   }
   if (g.dk.p) p.sum[p.sums++] = {a.v, g.dk, g.dy, a.q, a.Dv, a.D, true};

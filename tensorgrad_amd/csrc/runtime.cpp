@@ -771,7 +771,8 @@ static std::vector<int> op_inputs(const tgj::Value& op) {
       {"linear_recurrence_grad_h0", {"a", "h", "dh", "h0"}},
       {"linear_attention", {"q", "k", "v", "state", "documents", "lengths"}},
       {"linear_attention_state", {"q", "k", "v", "state", "documents", "lengths"}},
-      {"linear_attention_grad_q", {"q", "k", "v", "state", "documents", "lengths", "dy", "dstate"}},
+      {"linear_attention_borders", {"q", "k", "v", "state", "documents", "lengths"}},
+      {"linear_attention_grad_q", {"q", "k", "v", "state", "documents", "lengths", "dy", "dstate", "borders"}},
       {"linear_attention_grad_k", {"q", "k", "v", "state", "documents", "lengths", "dy", "dstate"}},
       {"linear_attention_grad_v", {"q", "k", "v", "state", "documents", "lengths", "dy", "dstate"}},
       {"linear_attention_grad_state", {"q", "k", "v", "state", "documents", "lengths", "dy", "dstate"}},
@@ -4131,17 +4132,18 @@ std::function<tgk::LinearDesc()> Runtime::linear_binder(int i, const tgk::Linear
 
 #define TG_LINEAR "q", "k", "v", "state", "documents", "lengths", "decay", "scale"
 
-// The results and the last state of one linear attention: one node, whichever comes first in the graph.
+// The results, the last state and the states at the segments' borders of one linear attention: one node, whichever comes first in
+// the graph.
 void Runtime::lower_linear(int i) {
   Node n;
   n.kind = "linear";
   n.op = i;
   n.direct = true;
   tgk::LinearDesc d = linear_fields(i, n);
-  int y = -1, last = -1;
+  int y = -1, last = -1, borders = -1;
   for (int j = i; j < (int)ops_.size(); ++j) {
-    if (kinds_[j] != "linear_attention" && kinds_[j] != "linear_attention_state") continue;
-    int& out = kinds_[j] == "linear_attention" ? y : last;
+    if (kinds_[j] != "linear_attention" && kinds_[j] != "linear_attention_state" && kinds_[j] != "linear_attention_borders") continue;
+    int& out = kinds_[j] == "linear_attention" ? y : kinds_[j] == "linear_attention_state" ? last : borders;
     if (out >= 0 || gemm_done_[j] || (j != i && !same_fields(i, j, {TG_LINEAR}))) continue;
     out = O(j).at("out").i32();
     gemm_done_[j] = 1;
@@ -4150,6 +4152,8 @@ void Runtime::lower_linear(int i) {
   }
   expect(y < 0 || (T_[y].shape == Dims({d.B, d.H, d.T, d.Dv}) && T_[y].dt == F32), i, "bad output shape");
   expect(last < 0 || (T_[last].shape == Dims({d.B, d.H, d.D, d.Dv}) && T_[last].dt == F32 && view_[last].contiguous()), i, "bad state shape");
+  expect(borders < 0 || (T_[borders].shape == Dims({(d.T + tgk::kLinearSegment - 1) / tgk::kLinearSegment, d.B, d.H, d.D, d.Dv}) &&
+                         T_[borders].dt == F32 && view_[borders].contiguous()), i, "bad borders' shape");
   n.shape = shape_str(T_[fld(i, "q")].shape) + "x" + shape_str(T_[fld(i, "v")].shape);
   n.flops = 4.0 * d.B * d.H * (double)d.T * d.D * d.Dv;
   n.bytes = 4.0 * (T_[fld(i, "q")].numel + T_[fld(i, "k")].numel + T_[fld(i, "v")].numel + (y >= 0 ? T_[y].numel : 0) +
@@ -4157,6 +4161,7 @@ void Runtime::lower_linear(int i) {
   // presence decides the kernels; the addresses follow at bind
   d.y.p = y >= 0 ? (float*)16 : nullptr;
   d.last = last >= 0 ? (float*)16 : nullptr;
+  d.borders = borders >= 0 ? (float*)16 : nullptr;
   const int64_t ws = tgk::linear_workspace_bytes(d);
   workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
   n.ws = ws > 0;
@@ -4165,6 +4170,7 @@ void Runtime::lower_linear(int i) {
     tgk::LinearDesc a = desc();
     if (y >= 0) a.y = rows_of(y, "linear attention y");
     a.last = last >= 0 ? (float*)dptr(last) : nullptr;
+    a.borders = borders >= 0 ? (float*)dptr(borders) : nullptr;
     void* w = cur_ws_;
     return [=](hipStream_t st) { tgk::linear(a, w, st); };
   };
@@ -4185,7 +4191,7 @@ void Runtime::lower_linear_grad(int i) {
   expect((dy >= 0 || ds >= 0) && (dy < 0 || (T_[dy].shape == ys && T_[dy].dt == F32)) &&
              (ds < 0 || (T_[ds].shape == ss && T_[ds].dt == F32 && view_[ds].contiguous())), i, "dy or dstate does not fit");
   for (int t : {dy, ds}) if (t >= 0) n.reads.push_back(root(t));
-  int out[4] = {-1, -1, -1, -1};
+  int out[4] = {-1, -1, -1, -1}, borders = -1;
   for (int j = i; j < (int)ops_.size(); ++j) {
     if (kinds_[j].compare(0, 22, "linear_attention_grad_") != 0 || gemm_done_[j]) continue;
     if (j != i && !same_fields(i, j, {TG_LINEAR, "dy", "dstate"})) continue;
@@ -4194,6 +4200,11 @@ void Runtime::lower_linear_grad(int i) {
     if (out[which] >= 0) continue;
     out[which] = O(j).at("out").i32();
     expect(which < 3 || of == "state", j, "unknown gradient");
+    if (which == 0 && (borders = opt_fld(j, "borders")) >= 0) {
+      const Dims bs = {(d.T + tgk::kLinearSegment - 1) / tgk::kLinearSegment, d.B, d.H, d.D, d.Dv};
+      expect(T_[borders].shape == bs && T_[borders].dt == F32 && view_[borders].contiguous(), j, "bad borders' shape");
+      n.reads.push_back(root(borders));
+    }
     expect(T_[out[which]].shape == (which == 3 ? ss : T_[fld(j, which == 0 ? "q" : which == 1 ? "k" : "v")].shape) &&
                T_[out[which]].dt == F32, j, "bad output shape");
     gemm_done_[j] = 1;
@@ -4211,6 +4222,7 @@ void Runtime::lower_linear_grad(int i) {
   g.dk.p = dk >= 0 ? (float*)16 : nullptr;
   g.dv.p = dv >= 0 ? (float*)16 : nullptr;
   g.dfirst = df >= 0 ? (float*)16 : nullptr;
+  g.borders = borders >= 0 ? (const float*)16 : nullptr;
   const int64_t ws = tgk::linear_grad_workspace_bytes(g);
   workspace_bytes_ = std::max(workspace_bytes_, (size_t)ws);
   n.ws = ws > 0;
@@ -4224,6 +4236,7 @@ void Runtime::lower_linear_grad(int i) {
     if (dv >= 0) b.dv = rows_of(dv, "linear attention dv");
     b.dstate = ds >= 0 ? (const float*)dptr(ds) : nullptr;
     b.dfirst = df >= 0 ? (float*)dptr(df) : nullptr;
+    b.borders = borders >= 0 ? (const float*)dptr(borders) : nullptr;
     void* w = cur_ws_;
     return [=](hipStream_t st) { tgk::linear_grad(b, w, st); };
   };
@@ -4975,7 +4988,7 @@ void Runtime::lower_op(int i) {
   } else if (k == "rope_axes") {
     lower_rope(i);
     return;
-  } else if (k == "linear_attention" || k == "linear_attention_state") {
+  } else if (k == "linear_attention" || k == "linear_attention_state" || k == "linear_attention_borders") {
     lower_linear(i);
     return;
   } else if (k.compare(0, 22, "linear_attention_grad_") == 0) {

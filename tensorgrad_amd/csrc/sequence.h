@@ -73,18 +73,20 @@ struct LinearDesc {
   Rows q, k, v, y;           // y may be absent (null)
   const float* state;        // [B, H, D, Dv] or null (zeros)
   float* last;               // the last state, or null
+  float* borders;            // [ceil(T / kLinearSegment)][B, H, D, Dv]: the states before each segment, for the gradients; or null
   const int32_t* documents;  // [B, T] or null
   const int32_t* lengths;    // [B] or null
   const float* rate;         // [H], log2(decay)
   float scale;
 };
 struct LinearGradDesc {
-  LinearDesc a;              // a.y and a.last are not read
+  LinearDesc a;              // a.y, a.last and a.borders are not read
   Rows dy, dq, dk, dv;       // each may be absent (null)
+  const float* borders;      // the forward's, or null
   const float* dstate;       // of the last state, or null
   float* dfirst;             // of `state`, or null
 };
-constexpr int kLinearMaxHead = 128;
+constexpr int kLinearMaxHead = 128, kLinearSegment = 128;
 int64_t linear_workspace_bytes(const LinearDesc& a);
 void linear(const LinearDesc& a, void* work, hipStream_t st);
 int64_t linear_grad_workspace_bytes(const LinearGradDesc& g);

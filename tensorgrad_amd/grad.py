@@ -278,7 +278,7 @@ def _adjoint(op: dict, oc: Tensor, graph: Graph, cot: Dict[int, Tensor]) -> None
                                         opt('documents'), opt('lengths'), dstate)
         for n, c in zip(('q', 'k', 'v', 'state'), grads):
             acc(op[n], c)
-    elif k == 'attention_stats' or k.startswith(('attention_grad_', 'linear_recurrence_grad_', 'linear_attention_grad_')):
+    elif k in ('attention_stats', 'linear_attention_borders') or k.startswith(('attention_grad_', 'linear_recurrence_grad_', 'linear_attention_grad_')):
         raise ValueError(f"autograd: cannot differentiate through {k} (it's a backward op)")
     elif k in ('conv2d_input_grad', 'conv2d_weight_grad', 'max_pool_2d_grad', 'scatter_axis'):
         raise ValueError(f"autograd: cannot differentiate through {k} (it's a backward op)")

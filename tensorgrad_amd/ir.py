@@ -118,7 +118,8 @@ _EXTENSIONS: Dict[str, Tuple[str, ...]] = {
     'linear_recurrence_grad_h0': ('a', 'h', 'dh', 'h0'),
     'linear_attention': _LINEAR,
     'linear_attention_state': _LINEAR,
-    'linear_attention_grad_q': _LINEAR + ('dy', 'dstate'),
+    'linear_attention_borders': _LINEAR,
+    'linear_attention_grad_q': _LINEAR + ('dy', 'dstate', 'borders'),
     'linear_attention_grad_k': _LINEAR + ('dy', 'dstate'),
     'linear_attention_grad_v': _LINEAR + ('dy', 'dstate'),
     'linear_attention_grad_state': _LINEAR + ('dy', 'dstate'),

@@ -701,6 +701,7 @@ def linear_recurrence_grad(a: Tensor, h: Tensor, dh: Tensor, h0: Optional[Tensor
 
 
 LINEAR_MAX_HEAD = 128      # the kernels' tiles hold whole heads
+LINEAR_SEGMENT = 128       # positions between the states that the gradients take from the forward pass
 
 
 def _linear_fields(site: str, q: Tensor, k: Tensor, v: Tensor, decay, scale, state, documents, lengths) -> dict:
@@ -765,9 +766,13 @@ def linear_attention_grad(q: Tensor, k: Tensor, v: Tensor, dy: Optional[Tensor],
     for name, t, shape in (('dy', dy, (B, H, T, v.shape[3])), ('dstate', dstate, (B, H, D, v.shape[3]))):
         if t is not None and (t.dtype != 'f32' or t.shape != shape):
             raise ShapeError(f'{site}: {name} must be f32 {S.show(shape)}, got {t.dtype} {S.show(t.shape)}', site)
+    g = current_graph()
+    segments = -(-T // LINEAR_SEGMENT)
+    borders = None if segments == 1 else add_op(g, 'linear_attention_borders', (segments, B, H, D, v.shape[3]), 'f32', site, f)
     f = dict(f, dy=None if dy is None else dy.id, dstate=None if dstate is None else dstate.id)
     outs = (('q', q), ('k', k), ('v', v)) + ((('state', state),) if state is not None else ())
-    return tuple(add_op(current_graph(), f'linear_attention_grad_{n}', t.shape, 'f32', site, f) for n, t in outs)
+    more = {'q': {'borders': None if borders is None else borders.id}}
+    return tuple(add_op(g, f'linear_attention_grad_{n}', t.shape, 'f32', site, dict(f, **more.get(n, {}))) for n, t in outs)
 
 
 # ---- Choice of the next token (no reference counterpart) ---------------------------------------------
