@@ -38,7 +38,7 @@ __device__ __forceinline__ u64 order_of(uint32_t key, int i) { return (u64)key <
 struct Row {
   const float* x;
   int V, most, unit;
-  float top, per_bin;              // largest logit; bins for a logit of 1 less
+  float top, per_bin, per1;        // largest logit; bins for a logit of 1 less; per in 32 bits
   double per, p, least, u;         // log2(e) / temperature; top_p; min_p times 2^unit; the random number
   bool by_count, by_mass;          // what limits
 };
@@ -53,6 +53,7 @@ __device__ __forceinline__ Row row_of(const SampleDesc& s, int64_t row, float to
   const double per = greedy ? 1 : 1 / heat;
   r.unit = 62 - (s.V > 1 ? 32 - __clz(s.V - 1) : 0);
   r.per = per * (1 / kLn2);
+  r.per1 = (float)r.per;
   r.per_bin = (float)(per * (kBins / (1.001 * kLn2 * (r.unit + 1))));
   r.most = greedy ? 1 : s.top_k ? s.top_k[row] : s.top_k1;
   r.p = s.top_p ? (double)s.top_p[row] : s.top_p1;
@@ -86,27 +87,55 @@ __device__ __forceinline__ int bin_of(const Row& r, float x) {
   return b < kBins ? (int)b : kBins;
 }
 
+// The same from 32 bits, 2^-17 of it off at most (and 1): what finds where a border is to be looked for.
+constexpr double kSlack = 0x1p-16;         // of a part of the sum: both sums off
+__device__ __forceinline__ u64 about(const Row& r, float x) {
+  return (u64)__builtin_amdgcn_exp2f((float)r.unit - (x == r.top ? 0.0f : (r.top - x) * r.per1));
+}
+
+// Lanes' values without LDS: of a 64-bit number, by rows of 16 lanes (0 where there is none).
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ u64 moved(u64 x) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
+  return (u64)hi << 32 | lo;
+}
+// Lane ^ half's value.
+template <int HALF>
+__device__ __forceinline__ u64 other_lane(u64 x) {
+  if constexpr (HALF == 1) return moved<0xB1>(x);                 // [1, 0, 3, 2] of 4
+  else if constexpr (HALF == 2) return moved<0x4E>(x);            // [2, 3, 0, 1]
+  else if constexpr (HALF == 4) return moved<0x1B>(moved<0x141>(x));   // 8 mirrored, then 4
+  else if constexpr (HALF == 8) return moved<0x128>(x);           // 16 turned by 8
+  else {
+    const uint32_t lo = (uint32_t)x, hi = (uint32_t)(x >> 32);
+    const auto l = HALF == 16 ? __builtin_amdgcn_permlane16_swap(lo, lo, false, false) : __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+    const auto h = HALF == 16 ? __builtin_amdgcn_permlane16_swap(hi, hi, false, false) : __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+    const int k = threadIdx.x & HALF ? 0 : 1;
+    return (u64)h[k] << 32 | l[k];
+  }
+}
+__device__ __forceinline__ u64 wave_scan(u64 x) {   // inclusive
+  x += moved<0x111>(x);
+  x += moved<0x112>(x);
+  x += moved<0x114>(x);
+  x += moved<0x118>(x);
+  x += moved<0x142, 0xa>(x);       // a row's last to the next, for rows 1 and 3; then lane 31's to rows 2 and 3
+  x += moved<0x143, 0xc>(x);
+  return x;
+}
+__device__ __forceinline__ u64 lane_value(u64 x, int lane) {
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
+__device__ __forceinline__ u64 wave_sum(u64 x) { return lane_value(wave_scan(x), 63); }
 __device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) x = fmaxf(x, __shfl_xor(x, o));
   return x;
 }
-__device__ __forceinline__ u64 wave_sum(u64 x) {
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) x += __shfl_xor(x, o);
-  return x;
-}
-__device__ __forceinline__ u64 wave_scan(u64 x) {   // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const u64 z = __shfl_up(x, o);
-    if ((int)(threadIdx.x & 63) >= o) x += z;
-  }
-  return x;
-}
 
 struct Bins {
-  u64 mass[kBins];
+  u64 mass[kBins];                         // about
   uint32_t count[kBins];
 };
 // What a block shares while it finds a row's borders and its choice.
@@ -143,8 +172,7 @@ __device__ __forceinline__ float block_top(const float* x, int from, int to, Wor
   for (int k = 0; k < THREADS / 64; ++k) top = fmaxf(top, __uint_as_float((uint32_t)w.sums[0][k]));
   return top;
 }
-// Counts and weighs [from, to) in bins. A few tokens at most are kept by their count alone: then no mass is needed, since all of them
-// are listed.
+// Counts and weighs [from, to) in bins. A few tokens at most are kept by their count alone: then all of them are listed.
 constexpr int kFew = 1024;
 __device__ __forceinline__ bool few(const Row& r) { return r.by_count && r.most <= kFew; }
 template <int THREADS>
@@ -156,12 +184,12 @@ __device__ __forceinline__ void clear_bins(Bins& b) {
 }
 template <int THREADS>
 __device__ __forceinline__ void fill_bins(const Row& r, int from, int to, Bins& b) {
-  const bool count_only = few(r);
+  const bool weigh = r.by_mass && !few(r);
   each_token(r.x, from + (int)threadIdx.x, to, THREADS, [&](int, float x) {
     const int bin = bin_of(r, x);
     if (bin == kBins) return;
     atomicAdd(&b.count[bin], 1u);
-    if (!count_only) atomicAdd(&b.mass[bin], whole(weight(r, x)));
+    if (weigh) atomicAdd(&b.mass[bin], about(r, x));
   });
 }
 // Sums over the bins before this thread's first (it has kBins / THREADS of them), and over all.
@@ -196,12 +224,14 @@ __device__ __forceinline__ void bin_sums(const Bins& b, Work& w, u64& count, u64
   }
 }
 
-// What the bins say: the bins [b0, b1] hold every border, `count` and `mass` stand before b0, and `size` tokens are in them. all:
-// the mass that top_p is a part of, or 0 where that ends within these bins (top_k does).
+// What the bins say: the bins [b0, b1] hold every border, `count` tokens stand before b0 and `size` are in them. whole: top_p is a
+// part of the mass of all tokens, else of those up to b1 that top_k keeps.
 struct Borders {
   int b0, b1;
-  u64 count, mass, size, all;
+  u64 count, size;
+  bool whole;
 };
+constexpr Borders kNoBorder = {kBins, kBins - 1, 0, 0, false};
 template <int THREADS, class Work>
 __device__ __forceinline__ Borders borders(const Row& r, const Bins& b, Work& w) {
   constexpr int N = kBins / THREADS;
@@ -228,52 +258,59 @@ __device__ __forceinline__ Borders borders(const Row& r, const Bins& b, Work& w)
         w.found[0] = bin;
         w.found[1] = m;
         w.found[2] = c1;
+        w.found[3] = c;
       }
     });
     __syncthreads();
   }
-  Borders o = {0, -1, 0, 0, 0, counted ? 0 : all_m};
   const int kbin = (int)w.found[0];
-  if (few(r)) {                    // all that top-k keeps, or all there are; without masses
-    o.b1 = counted ? kbin : kBins - 1;
-    o.size = counted ? w.found[2] : all_c;
-    return o;
-  }
-  // the least that the total of top-k can be: its border bin is not resolved yet
-  const double target = r.p > 0 ? r.p * (double)(counted ? w.found[1] : all_m) : 0;
-  if (r.by_mass) {
-    each([&](int bin, u64 c, u64 m, u64 c1, u64 m1) {
-      if (((double)m < target || bin == 0) && !((double)m1 < target)) {
-        w.found[3] = bin;
-        w.found[4] = c;
-        w.found[5] = m;
-        w.found[6] = c1;
-      }
-    });
-  } else if (counted) {
-    each([&](int bin, u64 c, u64 m, u64 c1, u64 m1) {
-      if (bin == kbin) {
-        w.found[3] = bin;
-        w.found[4] = c;
-        w.found[5] = m;
-      }
-    });
-  }
+  const u64 through = counted ? w.found[2] : all_c;
+  if (few(r)) return {0, counted ? kbin : kBins - 1, 0, through, false};   // all that top-k keeps, or all there are
+  if (!r.by_mass) return counted ? Borders{kbin, kbin, w.found[3], through - w.found[3], false} : kNoBorder;
+  // the sum that top_p is a part of: top-k's border bin is not resolved yet
+  const double least = r.p > 0 ? r.p * (1 - kSlack) * (double)(counted ? w.found[1] : all_m) : 0;
+  const double most = r.p > 0 ? r.p * (1 + kSlack) * (double)all_m : 0;
+  each([&](int bin, u64 c, u64 m, u64 c1, u64 m1) {
+    if (((double)m < least || bin == 0) && !((double)m1 < least)) {
+      w.found[4] = bin;
+      w.found[5] = c;
+    }
+    if (((double)m < most || bin == 0) && (!((double)m1 < most) || bin == kBins - 1)) {
+      w.found[6] = bin;
+      w.found[7] = c1;
+    }
+  });
   __syncthreads();
-  if (!r.by_mass && !counted) return o;
-  o.b0 = (int)w.found[3];
-  o.b1 = counted ? kbin : o.b0;
-  o.count = w.found[4];
-  o.mass = w.found[5];
-  o.size = (counted ? w.found[2] : w.found[6]) - o.count;
-  return o;
+  const int b0 = (int)w.found[4];
+  const u64 count = w.found[5];
+  if (counted) return {b0, kbin, count, through - count, false};
+  return {b0, (int)w.found[6], count, w.found[7] - count, true};
 }
 
-// The weight of a token by its order.
-__device__ __forceinline__ u64 listed_weight(const Row& r, u64 order) {
-  const uint32_t key = (uint32_t)(order >> 32);
-  return key == kNoKey ? 0 : whole(weight(r, value_of(key)));
+// Lists the tokens of a stretch in the border's bins, and sums weights of the others, by a wavefront.
+struct Sums {
+  u64 all, before, kept;           // of all (`whole`); of the bins before the border's; of those of them that min_p keeps
+};
+template <class Push>
+__device__ __forceinline__ Sums list_and_sum(const Row& r, const Borders& o, int from, int to, Push push) {
+  Sums s = {};
+  const int weigh = o.whole ? kBins : o.b0;
+  each_token(r.x, from + (int)(threadIdx.x & 63), to, 64, [&](int i, float x) {
+    const int bin = bin_of(r, x);
+    if (bin >= o.b0 && bin <= o.b1) push(order_of(key_of(x), i));
+    if (bin < weigh) {
+      const double w = weight(r, x);
+      const u64 m = whole(w);
+      s.all += m;
+      if (bin < o.b0) {
+        s.before += m;
+        s.kept += w >= r.least || x == r.top ? m : 0;
+      }
+    }
+  });
+  return {wave_sum(s.all), wave_sum(s.before), wave_sum(s.kept)};
 }
+
 // Sorts the first n of w.list: bitonic, a thread having every THREADS-th token. Steps of 1 to 32 places are exchanges of lanes, those of
 // THREADS and more a thread's own; the rest go through LDS, 10 of 55 steps for 1024 tokens of 1024 threads.
 template <int THREADS, int LIST>
@@ -312,7 +349,17 @@ __device__ __forceinline__ void sort_list(int n, Work<LIST>& w) {
         for (int e = 0; e < N; ++e) if (e * THREADS < n2) keep(e, w.list[e * THREADS + (tid ^ half)], size, half);
       } else {
 #pragma unroll
-        for (int e = 0; e < N; ++e) if (e * THREADS < n2) keep(e, __shfl_xor(x[e], half), size, half);
+        for (int e = 0; e < N; ++e) {
+          if (e * THREADS >= n2) break;
+          switch (half) {
+            case 1: keep(e, other_lane<1>(x[e]), size, half); break;
+            case 2: keep(e, other_lane<2>(x[e]), size, half); break;
+            case 4: keep(e, other_lane<4>(x[e]), size, half); break;
+            case 8: keep(e, other_lane<8>(x[e]), size, half); break;
+            case 16: keep(e, other_lane<16>(x[e]), size, half); break;
+            default: keep(e, other_lane<32>(x[e]), size, half);
+          }
+        }
       }
     }
   __syncthreads();
@@ -321,42 +368,50 @@ __device__ __forceinline__ void sort_list(int n, Work<LIST>& w) {
   __syncthreads();
 }
 
-// The bound of what is kept (an order, inclusive) from the tokens of the border's bins, `n` of them, in w.list.
-template <int THREADS, int LIST>
-__device__ __forceinline__ u64 bound_of_list(const Row& r, const Borders& o, int n, Work<LIST>& w) {
+// The bound of what is kept (an order, inclusive) from the n tokens of the border's bins in w.list and the mass of the others; calls
+// add(token, weight) for those of them that are kept, by min_p too. ok: the border does lie in these bins.
+template <int THREADS, int LIST, class Add>
+__device__ __forceinline__ u64 bound_of_list(const Row& r, const Borders& o, int n, u64 before_all, u64 all, Work<LIST>& w, bool& ok, Add add) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   sort_list<THREADS, LIST>(n, w);
   // a thread has N neighbours; those that top-k keeps
   constexpr int N = LIST / THREADS;
   const int kept = r.by_count ? (int)min((u64)n, (u64)r.most - min((u64)r.most, o.count)) : n;
-  u64 m[N], sum = 0;
+  double m[N];
+  u64 sum = 0;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
     const int i = tid * N + e;
-    m[e] = i < kept ? listed_weight(r, w.list[i]) : 0;
-    sum += m[e];
+    const uint32_t key = i < kept ? (uint32_t)(w.list[i] >> 32) : kNoKey;
+    m[e] = key == kNoKey ? 0 : weight(r, value_of(key));
+    sum += whole(m[e]);
   }
   const u64 scan = wave_scan(sum);
   if (lane == 63) w.sums[0][wave] = scan;
   __syncthreads();
-  u64 before = o.mass + scan - sum, total = o.mass;
+  u64 before = before_all + scan - sum, through = before_all;
 #pragma unroll
   for (int k = 0; k < THREADS / 64; ++k) {
     if (k < wave) before += w.sums[0][k];
-    total += w.sums[0][k];
+    through += w.sums[0][k];
   }
-  if (o.all) total = o.all;
   if (tid == 0) w.found[0] = 0;
   __syncthreads();
-  const double target = r.by_mass ? (r.p > 0 ? r.p * (double)total : 1.0) : (double)INFINITY;
-  int last = 0;                    // one past this thread's last token that is kept
+  const double target = r.by_mass ? (r.p > 0 ? r.p * (double)(o.whole ? all : through) : 1.0) : (double)INFINITY;
+  ok = (o.b0 == 0 || (double)before_all < target) && (!o.whole || o.b1 == kBins - 1 || !((double)through < target));
+  int mine = 0;                    // what a wavefront keeps: in all, a first part of the list
 #pragma unroll
   for (int e = 0; e < N; ++e) {
     const int i = tid * N + e;
-    if (i < kept && (double)before < target) last = i + 1;
-    before += m[e];
+    const u64 u = whole(m[e]);
+    const bool in = i < kept && (double)before < target;
+    mine += __popcll(__ballot(in));
+    if (in) {
+      if (m[e] >= r.least || value_of((uint32_t)(w.list[i] >> 32)) == r.top) add((int)(uint32_t)w.list[i], u);
+    }
+    before += u;
   }
-  atomicMax(&w.found[0], (u64)last);
+  if (lane == 0 && mine) atomicAdd(&w.found[0], (u64)mine);
   __syncthreads();
   const int end = (int)w.found[0];
   return end > 0 ? w.list[end - 1] : n > 0 ? w.list[0] - 1 : kAll;
@@ -455,8 +510,9 @@ __device__ __forceinline__ Border find_border(const Row& r, Border within, doubl
   return {lo, ties};
 }
 template <int THREADS, class Work>
-__device__ __forceinline__ u64 bound_by_walks(const Row& r, u64 all_mass, Bins& b, Work& w) {
-  if (r.by_mass && few(r)) {       // the mass of all was not needed so far
+__device__ __forceinline__ u64 bound_by_walks(const Row& r, Bins& b, Work& w) {
+  u64 all_mass = 0;
+  if (r.by_mass && !r.by_count) {
     u64 sum = 0;
     for (int i = threadIdx.x; i < r.V; i += THREADS)
       if (key_of(r.x[i]) != kNoKey) sum += whole(weight(r, r.x[i]));
@@ -464,7 +520,6 @@ __device__ __forceinline__ u64 bound_by_walks(const Row& r, u64 all_mass, Bins& 
     __syncthreads();
     if ((threadIdx.x & 63) == 0) w.sums[0][threadIdx.x >> 6] = sum;
     __syncthreads();
-    all_mass = 0;
     for (int k = 0; k < THREADS / 64; ++k) all_mass += w.sums[0][k];
     __syncthreads();
   }
@@ -575,7 +630,8 @@ __global__ __launch_bounds__(THREADS) void sample_short(SampleDesc s) {
     return;
   }
   const Row r = row_of(s, row, top);
-  const u64 bound = r.by_count || r.by_mass ? bound_of_list<THREADS, LIST>(r, {0, 0, 0, 0, 0, 0}, s.V, w) : kAll;
+  bool ok;
+  const u64 bound = r.by_count || r.by_mass ? bound_of_list<THREADS, LIST>(r, {0, kBins - 1, 0, 0, false}, s.V, 0, 0, w, ok, [](int, u64) {}) : kAll;
   u64 mine = 0;
 #pragma unroll
   for (int e = 0; e < N; ++e) if (e * THREADS + tid < s.V) mine += kept_weight(r, bound, e * THREADS + tid, v[e]);
@@ -594,53 +650,61 @@ __global__ __launch_bounds__(THREADS) void sample_one(SampleDesc s) {
   constexpr int W = THREADS / 64;
   __shared__ Bins bins;
   __shared__ Work<kList> w;
+  __shared__ u64 stretch[W], total[2];   // what is kept of a wavefront's stretch; mass of all, and before the border's bins
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   clear_bins<THREADS>(bins);
   if (tid == 0) w.listed = 0;
+  if (tid < 2) total[tid] = 0;
   const float top = block_top<THREADS>(s.logits + row * s.V, 0, s.V, w);
   if (top == -INFINITY) {
     if (tid == 0) s.token[row] = -1;
     return;
   }
   const Row r = row_of(s, row, top);
-  u64 bound = kAll;
+  Borders o = kNoBorder;
   if (r.by_count || r.by_mass) {
     fill_bins<THREADS>(r, 0, s.V, bins);
     __syncthreads();
-    const Borders o = borders<THREADS>(r, bins, w);
-    if (__builtin_expect(o.size > kList, 0)) {
-      bound = bound_by_walks<THREADS>(r, o.all, bins, w);
-    } else if (o.b1 >= 0) {
-      each_token(r.x, tid, s.V, THREADS, [&](int i, float x) {
-        const int bin = bin_of(r, x);
-        if (bin >= o.b0 && bin <= o.b1) w.list[atomicAdd(&w.listed, 1u)] = order_of(key_of(x), i);
-      });
-      __syncthreads();
-      bound = bound_of_list<THREADS, kList>(r, o, (int)w.listed, w);
-    }
+    o = borders<THREADS>(r, bins, w);
   }
   const int each = ((s.V + W - 1) / W + 63) / 64 * 64, from = min(wave * each, s.V), to = min(from + each, s.V);
-  const u64 mine = stretch_sum(r, bound, from, to);
-  __syncthreads();
-  if (lane == 0) w.sums[1][wave] = mine;
+  u64 bound = kAll;
+  bool ok = o.size <= kList;
+  if (ok) {
+    const Sums mine = list_and_sum(r, o, from, to, [&](u64 x) { w.list[atomicAdd(&w.listed, 1u)] = x; });
+    if (lane == 0) {
+      stretch[wave] = mine.kept;
+      atomicAdd(&total[0], mine.all);
+      atomicAdd(&total[1], mine.before);
+    }
+    __syncthreads();
+    if (o.b1 >= o.b0)
+      bound = bound_of_list<THREADS, kList>(r, o, (int)w.listed, total[1], total[0], w, ok, [&](int i, u64 m) { atomicAdd(&stretch[i / each], m); });
+  }
+  if (__builtin_expect(!ok, 0)) {
+    bound = bound_by_walks<THREADS>(r, bins, w);
+    const u64 mine = stretch_sum(r, bound, from, to);
+    __syncthreads();
+    if (lane == 0) stretch[wave] = mine;
+  }
   __syncthreads();
   u64 all = 0;
 #pragma unroll
-  for (int k = 0; k < W; ++k) all += w.sums[1][k];
+  for (int k = 0; k < W; ++k) all += stretch[k];
   u64 goal = goal_of(r, all);
   int k = 0;
-  while (k < W - 1 && goal >= w.sums[1][k]) goal -= w.sums[1][k++];
+  while (k < W - 1 && goal >= stretch[k]) goal -= stretch[k++];
   choose<THREADS>(r, bound, min(k * each, s.V), min((k + 1) * each, s.V), goal, w, s.token + row);
 }
 
 // ---- several blocks a row ------------------------------------------------------------------------------
 
-constexpr int kPartThreads = 256, kPartWaves = kPartThreads / 64;
+constexpr int kPartThreads = 256, kPartWaves = kPartThreads / 64, kParts = 1024;   // threads of a part; parts, at most
 struct RowSpace {                  // of a row in the workspace
   Bins bins;
   u64 list[kList];
-  u64 bound, listed;
+  u64 listed;
   Borders borders;
 };
 struct PartArgs {
@@ -648,7 +712,7 @@ struct PartArgs {
   int parts, each;                 // tokens of a part, a multiple of 64 a wavefront
   RowSpace* rows;
   float* tops;                     // [rows][parts]
-  u64* sums;                       // [rows][parts * kPartWaves]
+  Sums* sums;                      // [rows][parts]
 };
 // The row's largest logit; minus infinity: none.
 __device__ __forceinline__ float top_of(const PartArgs& a, int64_t row) {
@@ -688,89 +752,98 @@ __global__ __launch_bounds__(kPartThreads) void sample_bins(PartArgs a) {
       if (bins.mass[i]) atomicAdd(&sp.bins.mass[i], bins.mass[i]);
     }
 }
-// Lists the tokens of the border's bins: in LDS first, so that a block takes its places in the row's list at once.
+// Lists the tokens of the border's bins, in LDS first, so that a block takes its places in the row's list at once; sums the others.
 __global__ __launch_bounds__(kPartThreads) void sample_list(PartArgs a) {
   __shared__ Work<kList> w;
-  const int part = blockIdx.x, tid = threadIdx.x, from = part * a.each, to = min(from + a.each, a.s.V);
-  const int64_t row = blockIdx.y;
-  const float top = top_of(a, row);
-  const Row r = row_of(a.s, row, top);
-  if (top == -INFINITY || !(r.by_count || r.by_mass)) return;
-  RowSpace& sp = a.rows[row];
-  if (tid == 0) w.listed = 0;
-  const Borders o = borders<kPartThreads>(r, sp.bins, w);
-  if (part == 0 && tid == 0) sp.borders = o;
-  if (o.b1 < 0 || o.size > kList) return;
-  each_token(r.x, from + tid, to, kPartThreads, [&](int i, float x) {
-    const int bin = bin_of(r, x);
-    if (bin >= o.b0 && bin <= o.b1) w.list[atomicAdd(&w.listed, 1u)] = order_of(key_of(x), i);
-  });
-  __syncthreads();
-  const int n = (int)w.listed;
-  if (n == 0) return;
-  if (tid == 0) w.found[7] = atomicAdd(&sp.listed, (u64)n);
-  __syncthreads();
-  for (int i = tid; i < n; i += kPartThreads) sp.list[w.found[7] + i] = w.list[i];
-}
-// The bound of what is kept, a block a row.
-__global__ __launch_bounds__(1024) void sample_bound(PartArgs a) {
-  __shared__ Work<kList> w;
-  __shared__ Bins bins;
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const float top = top_of(a, row);
-  const Row r = row_of(a.s, row, top);
-  RowSpace& sp = a.rows[row];
-  u64 bound = kAll;
-  if (top > -INFINITY && (r.by_count || r.by_mass)) {
-    const Borders o = sp.borders;
-    if (__builtin_expect(o.size > kList, 0)) {
-      bound = bound_by_walks<1024>(r, o.all, bins, w);
-    } else if (o.b1 >= 0) {
-      for (int i = tid; i < (int)o.size; i += 1024) w.list[i] = sp.list[i];
-      __syncthreads();
-      bound = bound_of_list<1024, kList>(r, o, (int)o.size, w);
-    }
-  }
-  if (tid == 0) sp.bound = bound;
-}
-__global__ __launch_bounds__(kPartThreads) void sample_sums(PartArgs a) {
+  __shared__ Sums sums[kPartWaves];
   const int part = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
   const int64_t row = blockIdx.y;
   const float top = top_of(a, row);
   const Row r = row_of(a.s, row, top);
   if (top == -INFINITY) return;
+  RowSpace& sp = a.rows[row];
+  if (tid == 0) w.listed = 0;
+  Borders o = kNoBorder;
+  if (r.by_count || r.by_mass) o = borders<kPartThreads>(r, sp.bins, w);
+  if (part == 0 && tid == 0) sp.borders = o;
+  if (o.size > kList) return;
+  __syncthreads();
   const int each = a.each / kPartWaves, from = min(part * a.each + wave * each, a.s.V), to = min(from + each, a.s.V);
-  const u64 sum = stretch_sum(r, a.rows[row].bound, from, to);
-  if ((tid & 63) == 0) a.sums[(row * a.parts + part) * kPartWaves + wave] = sum;
+  const Sums mine = list_and_sum(r, o, from, to, [&](u64 x) { w.list[atomicAdd(&w.listed, 1u)] = x; });
+  if ((tid & 63) == 0) sums[wave] = mine;
+  __syncthreads();
+  const int n = (int)w.listed;
+  if (tid == 0) {
+    Sums all = {};
+#pragma unroll
+    for (int k = 0; k < kPartWaves; ++k) {
+      all.all += sums[k].all;
+      all.before += sums[k].before;
+      all.kept += sums[k].kept;
+    }
+    a.sums[row * a.parts + part] = all;
+    if (n > 0) w.found[0] = atomicAdd(&sp.listed, (u64)n);
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += kPartThreads) sp.list[w.found[0] + i] = w.list[i];
 }
-// The choice, a block a row; every wavefront finds the stretch.
-__global__ __launch_bounds__(kPartThreads) void sample_pick(PartArgs a) {
-  __shared__ Work<64> w;
+// The bound of what is kept, and the choice, a block a row.
+__global__ __launch_bounds__(1024) void sample_choice(PartArgs a) {
+  __shared__ Work<kList> w;
+  __shared__ Bins bins;
+  __shared__ u64 stretch[kParts], total[2];
   const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x & 63;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float top = top_of(a, row);
-  const Row r = row_of(a.s, row, top);
   if (top == -INFINITY) {
-    if (threadIdx.x == 0) a.s.token[row] = -1;
+    if (tid == 0) a.s.token[row] = -1;
     return;
   }
-  const int n = a.parts * kPartWaves, each = a.each / kPartWaves;
-  const u64* sums = a.sums + row * n;
+  const Row r = row_of(a.s, row, top);
+  RowSpace& sp = a.rows[row];
+  const Borders o = sp.borders;
+  u64 bound = kAll;
+  bool ok = o.size <= kList;
+  if (ok) {
+    if (tid < 2) total[tid] = 0;
+    for (int i = tid; i < (int)o.size; i += 1024) w.list[i] = sp.list[i];
+    __syncthreads();
+    const Sums s = tid < a.parts ? a.sums[row * a.parts + tid] : Sums{};
+    stretch[tid] = s.kept;
+    if (wave * 64 < a.parts) {
+      const u64 all = wave_sum(s.all), before = wave_sum(s.before);
+      if (lane == 0) {
+        atomicAdd(&total[0], all);
+        atomicAdd(&total[1], before);
+      }
+    }
+    __syncthreads();
+    if (o.b1 >= o.b0)
+      bound = bound_of_list<1024, kList>(r, o, (int)o.size, total[1], total[0], w, ok, [&](int i, u64 m) { atomicAdd(&stretch[i / a.each], m); });
+  }
+  if (__builtin_expect(!ok, 0)) {
+    bound = bound_by_walks<1024>(r, bins, w);
+    __syncthreads();
+    for (int k = wave; k < a.parts; k += 16) {
+      const u64 sum = stretch_sum(r, bound, min(k * a.each, a.s.V), min((k + 1) * a.each, a.s.V));
+      if (lane == 0) stretch[k] = sum;
+    }
+  }
+  __syncthreads();
+  // every wavefront finds the stretch
   u64 all = 0;
-  for (int k = lane; k < n; k += 64) all += sums[k];
+  for (int k = lane; k < a.parts; k += 64) all += stretch[k];
   all = wave_sum(all);
   u64 goal = goal_of(r, all), before = 0;
-  for (int k0 = 0; k0 < n; k0 += 64) {
-    const u64 m = k0 + lane < n ? sums[k0 + lane] : 0, sum = before + wave_scan(m), passed = __ballot(sum > goal);
+  for (int k0 = 0; k0 < a.parts; k0 += 64) {
+    const u64 m = k0 + lane < a.parts ? stretch[k0 + lane] : 0, sum = before + wave_scan(m), passed = __ballot(sum > goal);
     if (passed) {
-      const int l = __ffsll(passed) - 1, k = k0 + l;
-      goal -= __shfl(sum - m, l);
-      const int from = min(k * each, a.s.V);
-      choose<kPartThreads>(r, a.rows[row].bound, from, min(from + each, a.s.V), goal, w, a.s.token + row);
+      const int l = __ffsll(passed) - 1, from = min((k0 + l) * a.each, a.s.V);
+      goal -= lane_value(sum - m, l);
+      choose<1024>(r, bound, from, min(from + a.each, a.s.V), goal, w, a.s.token + row);
       return;
     }
-    before = __shfl(sum, 63);
+    before = lane_value(sum, 63);
   }
 }
 
@@ -782,13 +855,13 @@ SamplePlan sample_plan(const SampleDesc& s) {
   SamplePlan p{};
   p.parts = 1;
   // Several blocks a row where rows alone leave most of the card idle and are long enough.
-  if (s.rows < 128 && s.V > 8192) p.parts = (int)std::min<int64_t>((s.V + 2047) / 2048, (1024 + s.rows - 1) / s.rows);
+  if (s.rows < 128 && s.V > 8192) p.parts = (int)std::min<int64_t>((s.V + 2047) / 2048, std::max<int64_t>(kParts / s.rows, 1));
   p.each = ((s.V + p.parts - 1) / p.parts + kPartThreads - 1) / kPartThreads * kPartThreads;
   p.parts = (s.V + p.each - 1) / p.each;
   if (p.parts > 1) {
     p.tops = s.rows * (int64_t)sizeof(RowSpace);
     p.sums = p.tops + (s.rows * p.parts * 4 + 7) / 8 * 8;
-    p.bytes = p.sums + s.rows * p.parts * kPartWaves * 8;
+    p.bytes = p.sums + s.rows * p.parts * (int64_t)sizeof(Sums);
   }
   return p;
 }
@@ -807,16 +880,12 @@ void sample(const SampleDesc& s, void* work, hipStream_t st) {
     return;
   }
   char* w = (char*)work;
-  const PartArgs a{s, p.parts, p.each, (RowSpace*)w, (float*)(w + p.tops), (u64*)(w + p.sums)};
+  const PartArgs a{s, p.parts, p.each, (RowSpace*)w, (float*)(w + p.tops), (Sums*)(w + p.sums)};
   const bool limits = s.temperature || !(s.temperature1 > 0) || s.top_k || s.top_p || (s.top_k1 > 0 && s.top_k1 < s.V) || s.top_p1 < 1;
   klaunch(sample_tops, grid, block, 0, st, a);
-  if (limits) {
-    klaunch(sample_bins, grid, block, 0, st, a);
-    klaunch(sample_list, grid, block, 0, st, a);
-  }
-  klaunch(sample_bound, rows, dim3(1024), 0, st, a);
-  klaunch(sample_sums, grid, block, 0, st, a);
-  klaunch(sample_pick, rows, block, 0, st, a);
+  if (limits) klaunch(sample_bins, grid, block, 0, st, a);
+  klaunch(sample_list, grid, block, 0, st, a);
+  klaunch(sample_choice, rows, dim3(1024), 0, st, a);
 }
 
 }  // namespace tgk
