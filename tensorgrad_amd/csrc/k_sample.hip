@@ -311,24 +311,46 @@ __device__ __forceinline__ Sums list_and_sum(const Row& r, const Borders& o, int
   return {wave_sum(s.all), wave_sum(s.before), wave_sum(s.kept)};
 }
 
+// One step of a bitonic sort between lanes, straight: a branch a step cost 300 ns of latency instead of 40.
+template <int HALF>
+__device__ __forceinline__ void lane_step(u64& x, int i, int size) {
+  const u64 y = other_lane<HALF>(x);
+  const bool low = ((i & HALF) == 0) == ((i & size) == 0);   // takes the smaller
+  x = (y < x) == low ? y : x;
+}
+template <int HALF>
+__device__ __forceinline__ void lane_steps(u64& x, int i, int size) {
+  lane_step<HALF>(x, i, size);
+  if constexpr (HALF > 1) lane_steps<HALF / 2>(x, i, size);
+}
 // Sorts the first n of w.list: bitonic, a thread having every THREADS-th token. Steps of 1 to 32 places are exchanges of lanes, those of
 // THREADS and more a thread's own; the rest go through LDS, 10 of 55 steps for 1024 tokens of 1024 threads.
 template <int THREADS, int LIST>
 __device__ __forceinline__ void sort_list(int n, Work<LIST>& w) {
   constexpr int N = LIST / THREADS;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, uniform = __builtin_amdgcn_readfirstlane(n);
   int n2 = 64;
-  while (n2 < n) n2 *= 2;
+  while (n2 < uniform) n2 *= 2;
   u64 x[N];
 #pragma unroll
-  for (int e = 0; e < N; ++e) x[e] = e * THREADS + tid < n ? w.list[e * THREADS + tid] : kAll;
+  for (int e = 0; e < N; ++e) {
+    const int i = e * THREADS + tid;
+    x[e] = i < n ? w.list[i] : kAll;
+    if (e * THREADS >= n2) continue;
+    lane_steps<1>(x[e], i, 2);
+    lane_steps<2>(x[e], i, 4);
+    lane_steps<4>(x[e], i, 8);
+    lane_steps<8>(x[e], i, 16);
+    lane_steps<16>(x[e], i, 32);
+    lane_steps<32>(x[e], i, 64);
+  }
   auto keep = [&](int e, u64 other, int size, int half) {
     const int i = e * THREADS + tid;
-    const bool low = ((i & half) == 0) == ((i & size) == 0);   // takes the smaller
+    const bool low = ((i & half) == 0) == ((i & size) == 0);
     x[e] = (other < x[e]) == low ? other : x[e];
   };
-  for (int size = 2; size <= n2; size *= 2)
-    for (int half = size / 2; half > 0; half /= 2) {
+  for (int size = 128; size <= n2; size *= 2) {
+    for (int half = size / 2; half >= 64; half /= 2) {
       if (half >= THREADS) {
 #pragma unroll
         for (int d = 1; d < N; d *= 2)
@@ -340,28 +362,18 @@ __device__ __forceinline__ void sort_list(int n, Work<LIST>& w) {
                 keep(e, b, size, half);
                 keep(e + d, a, size, half);
               }
-      } else if (half >= 64) {
+      } else {
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < N; ++e) if (e * THREADS < n2) w.list[e * THREADS + tid] = x[e];
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < N; ++e) if (e * THREADS < n2) keep(e, w.list[e * THREADS + (tid ^ half)], size, half);
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          if (e * THREADS >= n2) break;
-          switch (half) {
-            case 1: keep(e, other_lane<1>(x[e]), size, half); break;
-            case 2: keep(e, other_lane<2>(x[e]), size, half); break;
-            case 4: keep(e, other_lane<4>(x[e]), size, half); break;
-            case 8: keep(e, other_lane<8>(x[e]), size, half); break;
-            case 16: keep(e, other_lane<16>(x[e]), size, half); break;
-            default: keep(e, other_lane<32>(x[e]), size, half);
-          }
-        }
       }
     }
+#pragma unroll
+    for (int e = 0; e < N; ++e) if (e * THREADS < n2) lane_steps<32>(x[e], e * THREADS + tid, size);
+  }
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < N; ++e) if (e * THREADS < n2) w.list[e * THREADS + tid] = x[e];
@@ -700,7 +712,7 @@ __global__ __launch_bounds__(THREADS) void sample_one(SampleDesc s) {
 
 // ---- several blocks a row ------------------------------------------------------------------------------
 
-constexpr int kPartThreads = 256, kPartWaves = kPartThreads / 64, kParts = 1024;   // threads of a part; parts, at most
+constexpr int kPartThreads = 1024, kPartWaves = kPartThreads / 64, kParts = 256;   // threads of a part; parts, at most
 struct RowSpace {                  // of a row in the workspace
   Bins bins;
   u64 list[kList];
@@ -791,7 +803,7 @@ __global__ __launch_bounds__(kPartThreads) void sample_list(PartArgs a) {
 __global__ __launch_bounds__(1024) void sample_choice(PartArgs a) {
   __shared__ Work<kList> w;
   __shared__ Bins bins;
-  __shared__ u64 stretch[kParts], total[2];
+  __shared__ u64 stretch[1024], total[2];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float top = top_of(a, row);
@@ -855,7 +867,7 @@ SamplePlan sample_plan(const SampleDesc& s) {
   SamplePlan p{};
   p.parts = 1;
   // Several blocks a row where rows alone leave most of the card idle and are long enough.
-  if (s.rows < 128 && s.V > 8192) p.parts = (int)std::min<int64_t>((s.V + 2047) / 2048, std::max<int64_t>(kParts / s.rows, 1));
+  if (s.rows < 128 && s.V > 8192) p.parts = (int)std::min<int64_t>((s.V + 4095) / 4096, std::max<int64_t>(kParts / s.rows, 1));
   p.each = ((s.V + p.parts - 1) / p.parts + kPartThreads - 1) / kPartThreads * kPartThreads;
   p.parts = (s.V + p.each - 1) / p.each;
   if (p.parts > 1) {
@@ -875,7 +887,7 @@ void sample(const SampleDesc& s, void* work, hipStream_t st) {
   const dim3 rows((unsigned)s.rows), grid((unsigned)p.parts, (unsigned)s.rows), block(kPartThreads);
   if (p.parts == 1) {
     if (s.V <= 256) klaunch(sample_short<64, 256>, rows, dim3(64), 0, st, s);
-    else if (s.V <= 2048) klaunch(sample_short<256, 2048>, rows, block, 0, st, s);
+    else if (s.V <= 2048) klaunch(sample_short<256, 2048>, rows, dim3(256), 0, st, s);
     else klaunch(sample_one<1024>, rows, dim3(1024), 0, st, s);
     return;
   }
