@@ -12,6 +12,7 @@
 // A row is read four times, the first time from memory. Many rows: a block takes one, in one launch (sample_one; sample_short, which
 // sorts all). Few rows of many tokens: several blocks a row, in six launches (sample_tops, _bins, _list, _bound, _sums, _pick).
 #include <algorithm>
+#include <cfloat>
 
 #include "kernels.h"
 #include "sequence.h"
@@ -48,7 +49,7 @@ __device__ __forceinline__ Row row_of(const SampleDesc& s, int64_t row, float to
   r.x = s.logits + row * s.V;
   r.V = s.V;
   r.top = top;
-  const double heat = s.temperature ? (double)s.temperature[row] : s.temperature1;
+  const double heat = fmin(s.temperature ? (double)s.temperature[row] : s.temperature1, FLT_MAX);
   const bool greedy = !(heat > 0);           // the first of the order
   const double per = greedy ? 1 : 1 / heat;
   r.unit = 62 - (s.V > 1 ? 32 - __clz(s.V - 1) : 0);
@@ -64,7 +65,8 @@ __device__ __forceinline__ Row row_of(const SampleDesc& s, int64_t row, float to
   return r;
 }
 // A token's weight times 2^unit, 0 far from the top: 2^-t = 2^-n 2^f by the series of 2^f for |f| <= 1 / 2, 2^-52 off at most. Of
-// a logit that is there.
+// a logit that is there. t is a number for infinite logits too. Three-operand instructions with the coefficient in scalar registers:
+// the compiler's own choice copies every coefficient first.
 struct Series {
   double c[13];
   constexpr Series() : c() {
@@ -74,11 +76,11 @@ struct Series {
 };
 __device__ __forceinline__ double weight(const Row& r, float x) {
   constexpr Series s;
-  const double t = x == r.top ? 0 : fmin(((double)r.top - (double)x) * r.per, 4000.0), n = rint(t), f = n - t;
+  const double t = fmin(fmax(((double)r.top - (double)x) * r.per, 0.0), 4000.0), n = rint(t), f = n - t;
   double e = s.c[12];
 #pragma unroll
-  for (int k = 11; k >= 0; --k) e = fma(e, f, s.c[k]);
-  return __builtin_amdgcn_ldexp(e, r.unit - (int)n);
+  for (int k = 11; k > 0; --k) asm("v_fma_f64 %0, %1, %2, %3" : "=v"(e) : "v"(e), "v"(f), "s"(s.c[k]));
+  return __builtin_amdgcn_ldexp(fma(e, f, 1.0), r.unit - (int)n);
 }
 __device__ __forceinline__ u64 whole(double w) { return (u64)rint(w); }
 // A token's bin, rising with the distance to the top in equal steps; kBins: so far that its weight is 0, or not there.
@@ -712,7 +714,8 @@ __global__ __launch_bounds__(THREADS) void sample_one(SampleDesc s) {
 
 // ---- several blocks a row ------------------------------------------------------------------------------
 
-constexpr int kPartThreads = 1024, kPartWaves = kPartThreads / 64, kParts = 256;   // threads of a part; parts, at most
+constexpr int kPartThreads = 1024, kPartWaves = kPartThreads / 64, kParts = 256;   // parts: at most
+constexpr int kStretches = 4;      // of a part: what is kept is summed for each
 struct RowSpace {                  // of a row in the workspace
   Bins bins;
   u64 list[kList];
@@ -724,7 +727,7 @@ struct PartArgs {
   int parts, each;                 // tokens of a part, a multiple of 64 a wavefront
   RowSpace* rows;
   float* tops;                     // [rows][parts]
-  Sums* sums;                      // [rows][parts]
+  Sums* sums;                      // [rows][parts * kStretches]
 };
 // The row's largest logit; minus infinity: none.
 __device__ __forceinline__ float top_of(const PartArgs& a, int64_t row) {
@@ -785,16 +788,17 @@ __global__ __launch_bounds__(kPartThreads) void sample_list(PartArgs a) {
   if ((tid & 63) == 0) sums[wave] = mine;
   __syncthreads();
   const int n = (int)w.listed;
-  if (tid == 0) {
+  if (tid < kStretches) {
+    constexpr int W = kPartWaves / kStretches;
     Sums all = {};
 #pragma unroll
-    for (int k = 0; k < kPartWaves; ++k) {
-      all.all += sums[k].all;
-      all.before += sums[k].before;
-      all.kept += sums[k].kept;
+    for (int k = 0; k < W; ++k) {
+      all.all += sums[tid * W + k].all;
+      all.before += sums[tid * W + k].before;
+      all.kept += sums[tid * W + k].kept;
     }
-    a.sums[row * a.parts + part] = all;
-    if (n > 0) w.found[0] = atomicAdd(&sp.listed, (u64)n);
+    a.sums[(row * a.parts + part) * kStretches + tid] = all;
+    if (tid == 0 && n > 0) w.found[0] = atomicAdd(&sp.listed, (u64)n);
   }
   __syncthreads();
   for (int i = tid; i < n; i += kPartThreads) sp.list[w.found[0] + i] = w.list[i];
@@ -803,7 +807,8 @@ __global__ __launch_bounds__(kPartThreads) void sample_list(PartArgs a) {
 __global__ __launch_bounds__(1024) void sample_choice(PartArgs a) {
   __shared__ Work<kList> w;
   __shared__ Bins bins;
-  __shared__ u64 stretch[1024], total[2];
+  __shared__ u64 stretch[kParts * kStretches], total[2];
+  static_assert(kParts * kStretches == 1024);
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float top = top_of(a, row);
@@ -814,15 +819,16 @@ __global__ __launch_bounds__(1024) void sample_choice(PartArgs a) {
   const Row r = row_of(a.s, row, top);
   RowSpace& sp = a.rows[row];
   const Borders o = sp.borders;
+  const int n = a.parts * kStretches, each = a.each / kStretches;
   u64 bound = kAll;
   bool ok = o.size <= kList;
   if (ok) {
     if (tid < 2) total[tid] = 0;
     for (int i = tid; i < (int)o.size; i += 1024) w.list[i] = sp.list[i];
     __syncthreads();
-    const Sums s = tid < a.parts ? a.sums[row * a.parts + tid] : Sums{};
+    const Sums s = tid < n ? a.sums[row * n + tid] : Sums{};
     stretch[tid] = s.kept;
-    if (wave * 64 < a.parts) {
+    if (wave * 64 < n) {
       const u64 all = wave_sum(s.all), before = wave_sum(s.before);
       if (lane == 0) {
         atomicAdd(&total[0], all);
@@ -831,28 +837,28 @@ __global__ __launch_bounds__(1024) void sample_choice(PartArgs a) {
     }
     __syncthreads();
     if (o.b1 >= o.b0)
-      bound = bound_of_list<1024, kList>(r, o, (int)o.size, total[1], total[0], w, ok, [&](int i, u64 m) { atomicAdd(&stretch[i / a.each], m); });
+      bound = bound_of_list<1024, kList>(r, o, (int)o.size, total[1], total[0], w, ok, [&](int i, u64 m) { atomicAdd(&stretch[i / each], m); });
   }
   if (__builtin_expect(!ok, 0)) {
     bound = bound_by_walks<1024>(r, bins, w);
     __syncthreads();
-    for (int k = wave; k < a.parts; k += 16) {
-      const u64 sum = stretch_sum(r, bound, min(k * a.each, a.s.V), min((k + 1) * a.each, a.s.V));
+    for (int k = wave; k < n; k += 16) {
+      const u64 sum = stretch_sum(r, bound, min(k * each, a.s.V), min((k + 1) * each, a.s.V));
       if (lane == 0) stretch[k] = sum;
     }
   }
   __syncthreads();
   // every wavefront finds the stretch
   u64 all = 0;
-  for (int k = lane; k < a.parts; k += 64) all += stretch[k];
+  for (int k = lane; k < n; k += 64) all += stretch[k];
   all = wave_sum(all);
   u64 goal = goal_of(r, all), before = 0;
-  for (int k0 = 0; k0 < a.parts; k0 += 64) {
-    const u64 m = k0 + lane < a.parts ? stretch[k0 + lane] : 0, sum = before + wave_scan(m), passed = __ballot(sum > goal);
+  for (int k0 = 0; k0 < n; k0 += 64) {
+    const u64 m = k0 + lane < n ? stretch[k0 + lane] : 0, sum = before + wave_scan(m), passed = __ballot(sum > goal);
     if (passed) {
-      const int l = __ffsll(passed) - 1, from = min((k0 + l) * a.each, a.s.V);
+      const int l = __ffsll(passed) - 1, from = min((k0 + l) * each, a.s.V);
       goal -= lane_value(sum - m, l);
-      choose<1024>(r, bound, from, min(from + a.each, a.s.V), goal, w, a.s.token + row);
+      choose<1024>(r, bound, from, min(from + each, a.s.V), goal, w, a.s.token + row);
       return;
     }
     before = lane_value(sum, 63);
@@ -873,7 +879,7 @@ SamplePlan sample_plan(const SampleDesc& s) {
   if (p.parts > 1) {
     p.tops = s.rows * (int64_t)sizeof(RowSpace);
     p.sums = p.tops + (s.rows * p.parts * 4 + 7) / 8 * 8;
-    p.bytes = p.sums + s.rows * p.parts * (int64_t)sizeof(Sums);
+    p.bytes = p.sums + s.rows * p.parts * kStretches * (int64_t)sizeof(Sums);
   }
   return p;
 }
