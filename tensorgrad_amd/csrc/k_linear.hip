@@ -278,7 +278,8 @@ struct PairsArgs {
   Marks m;
   Sum sum[2];
   int sums, B, H, segs, blocks;    // blocks: of a head
-  int heads, group, share;         // heads of `rows`; back: those of x and z that a row meets in turn; else rows' heads that share one of x
+  int heads, group, share;         // heads of `out`; back: those of x and z that a row meets in turn; else rows' heads that share one of x
+  int keys;                        // heads of `out` that share one of `rows`
   const float *states, *edge;      // [segs][B * H][D][Dv]; at the first segment (back: last) this one, or null
   int D, Dv;
   float by_pair, by_state;         // factors of both parts
@@ -322,7 +323,7 @@ __device__ __forceinline__ void plain_rows(const PairsArgs& p, const Sum& s, con
   for (int r = w0; r < min(w0 + 16, p.m.T); ++r) {
     const int mine = since[r - o.s0];
     if (mine == kNever || !s.rows.p) continue;
-    const float* row = row_at(s.rows, o.b, o.head, r);
+    const float* row = row_at(s.rows, o.b, o.head / p.keys, r);
     float acc[2] = {0, 0};
 #pragma unroll 1
     for (int gi = 0; gi < o.group; ++gi) {
@@ -542,7 +543,7 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
   };
   fetch();
   Own<DP, true> own;
-  own.load(s.rows.p ? row_at(s.rows, o.b, o.head, min(r, T - 1)) : p.any, s.rows.p ? s.n : 1, g);
+  own.load(s.rows.p ? row_at(s.rows, o.b, o.head / p.keys, min(r, T - 1)) : p.any, s.rows.p ? s.n : 1, g);
   mark(p.m, o.b, o.s0, o.n, since);
   const Ends end = ends(since, o.s0, o.n);
   const int mine = r < T ? since[r - o.s0] : kNever;
@@ -610,7 +611,7 @@ __global__ __launch_bounds__(256) void linear_pairs(PairsArgs p) {
   const int mine = r < T ? since[r - o.s0] : kNever;
   const bool here = mine != kNever;
   Own<DP, false> own;
-  own.load(s.rows.p ? row_at(s.rows, o.b, o.head, min(r, T - 1)) : p.any, s.rows.p ? s.n : 1, g);
+  own.load(s.rows.p ? row_at(s.rows, o.b, o.head / p.keys, min(r, T - 1)) : p.any, s.rows.p ? s.n : 1, g);
   own.start(here && s.rows.p, s.n, g);
   for (int gi = 0; gi < o.group; ++gi) {
     const int h = o.h0 + gi, hx = BACK ? h : h / p.share;
@@ -643,6 +644,27 @@ __global__ __launch_bounds__(256) void linear_pairs(PairsArgs p) {
   }
   const bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here, s.nz, g);
   if (!fine) plain_rows<BACK>(p, s, o, w0, since);
+}
+
+// Sums of what each query head gave a key head's rows, in the heads' order.
+struct FoldArgs {
+  const float* parts[2];           // [B][Hk * group][T][n]
+  Rows out[2];
+  int n[2];
+  int Hk, group, T;
+  int64_t rows;                    // B * Hk * T
+};
+__global__ __launch_bounds__(256) void linear_fold(FoldArgs A) {
+  const int n = A.n[blockIdx.y];
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / n;
+  if (row >= A.rows) return;
+  const int d = (int)(id % n), t = (int)(row % A.T), h = (int)(row / A.T % A.Hk);
+  const int64_t b = row / A.T / A.Hk, head = (int64_t)A.T * n;
+  const float* part = A.parts[blockIdx.y] + ((b * A.Hk + h) * A.group) * head + (int64_t)t * n + d;
+  float s = part[0];
+  for (int i = 1; i < A.group; ++i) s += part[i * head];
+  const Rows& out = A.out[blockIdx.y];
+  out.p[b * out.b + h * out.h + t * out.t + d] = s;
 }
 
 // ---- a few positions ---------------------------------------------------------------------------------------
@@ -792,8 +814,12 @@ void pairs(PairsArgs p, const LinearDesc& a, const float* at, const float* edge,
   p.B = a.B;
   p.H = a.H;
   p.segs = segments(a);
-  p.heads = BACK ? a.Hk : a.H;
-  p.group = p.share = a.H / a.Hk;
+  p.share = a.H / a.Hk;
+  if (!p.heads) {
+    p.heads = BACK ? a.Hk : a.H;
+    p.group = p.share;
+    p.keys = 1;
+  }
   p.states = at;
   p.edge = edge;
   p.D = a.D;
@@ -842,7 +868,19 @@ void linear(const LinearDesc& a, void* work, hipStream_t st) {
   pairs<false>(p, a, at, a.state, st);
 }
 
-int64_t linear_grad_workspace_bytes(const LinearGradDesc& g) { return stay_bytes(g.a) + (g.borders ? 1 : 2) * states_bytes(g.a); }
+// Key heads that several query heads share: a block takes all of those in turn, or one where all of them would leave the card half
+// empty, and what they give is summed after (3 sequences of 1777, 8 heads on 2 of 96 and
+// 80 features: 96 us in turn, 64 + 11 apart).
+static bool split_heads(const LinearGradDesc& g) {
+  const LinearDesc& a = g.a;
+  const int sums = (g.dk.p != nullptr) + (g.dv.p != nullptr);
+  return a.H > a.Hk && (int64_t)((a.T + 63) / 64) * a.B * a.Hk * sums < 512;
+}
+static int64_t part_bytes(const LinearDesc& a, int n) { return ((int64_t)a.B * a.H * a.T * n * 4 + 255) / 256 * 256; }
+int64_t linear_grad_workspace_bytes(const LinearGradDesc& g) {
+  const int64_t parts = split_heads(g) ? (g.dk.p ? part_bytes(g.a, g.a.D) : 0) + (g.dv.p ? part_bytes(g.a, g.a.Dv) : 0) : 0;
+  return stay_bytes(g.a) + (g.borders ? 1 : 2) * states_bytes(g.a) + parts;
+}
 
 void linear_grad(const LinearGradDesc& g, void* work, hipStream_t st) {
   const LinearDesc& a = g.a;
@@ -850,15 +888,35 @@ void linear_grad(const LinearGradDesc& g, void* work, hipStream_t st) {
   const bool several = segments(a) > 1;
   if (g.dq.p && several && !g.borders) states(a, a.k, a.v, false, a.state, nullptr, S, stay, st);
   if (g.dfirst || ((g.dk.p || g.dv.p) && several)) states(a, a.q, g.dy, true, g.dstate, g.dfirst, G, stay, st);
-  PairsArgs p{};
   if (g.dq.p) {
+    PairsArgs p{};
     p.sum[p.sums++] = {g.dy, g.dq, a.v, a.k, a.Dv, a.D, true};
     pairs<false>(p, a, g.borders ? g.borders : S, a.state, st);
-    p.sums = 0;
   }
+  PairsArgs p{};
   if (g.dk.p) p.sum[p.sums++] = {a.v, g.dk, g.dy, a.q, a.Dv, a.D, true};
   if (g.dv.p) p.sum[p.sums++] = {a.k, g.dv, a.q, g.dy, a.D, a.Dv, false};
-  if (p.sums) pairs<true>(p, a, G, g.dstate, st);
+  if (!p.sums) return;
+  if (!split_heads(g)) return pairs<true>(p, a, G, g.dstate, st);
+  FoldArgs f{};
+  char* part = (char*)S + (g.borders ? 0 : states_bytes(a));
+  f.Hk = a.Hk;
+  f.group = a.H / a.Hk;
+  f.T = a.T;
+  f.rows = (int64_t)a.B * a.Hk * a.T;
+  for (int i = 0; i < p.sums; ++i) {
+    const int n = p.sum[i].nz;
+    f.parts[i] = (const float*)part;
+    f.out[i] = p.sum[i].out;
+    f.n[i] = n;
+    p.sum[i].out = {(float*)part, (int64_t)a.H * a.T * n, (int64_t)a.T * n, n};
+    part += part_bytes(a, n);
+  }
+  p.heads = a.H;
+  p.group = 1;
+  p.keys = f.group;
+  pairs<true>(p, a, G, g.dstate, st);
+  klaunch(linear_fold, dim3((unsigned)((f.rows * std::max(f.n[0], f.n[1]) + 255) / 256), p.sums), dim3(256), 0, st, f);
 }
 
 }  // namespace tgk
