@@ -227,3 +227,15 @@ def test_the_64_bit_choice_of_small_rows():
     assert at(temperature=0) == [1] * 8
     assert at(top_k=3, top_p=0.5, min_p=0.9) == [1] * 8
     assert D.sample(np.array([-np.inf, np.nan]), 0.5) == -1
+
+
+@pytest.mark.parametrize('T,ops', [(128, []), (129, ['linear_attention_borders'])])
+def test_states_between_segments_are_kept_for_the_gradients_that_read_them(T, ops):
+    """One node makes them beside the results; none does for a sequence of one segment, or for gradients of keys and values."""
+    def made(names):
+        m = Params(**{n: (1, 1, T, 8) for n in names})
+        loss = lambda p, i: O.mean(O.linear_attention(*(getattr(p, n) if n in names else i[n] for n in 'qkv'), [0.9])[0])  # noqa: E731
+        ir = build_training_ir(m, loss, {n: [1, 1, T, 8] for n in 'qkv' if n not in names}, {'kind': 'sgd', 'lr': 0.1})
+        return [n['ops'].split(',') for n in nodes_of(ir) if n['kind'] == 'linear']
+    assert made('qkv') == [['linear_attention', *ops]] and made('q') == [['linear_attention', *ops]]
+    assert made('kv') == [['linear_attention']]
