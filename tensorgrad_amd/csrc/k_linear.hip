@@ -148,10 +148,17 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 // The same through registers, for rows that are not whole 16-byte pieces; zero past the end.
 template <int DP, int THREADS>
 __device__ __forceinline__ void tile_by_hand(float* tile, const float* x, int64_t stride, int r0, int rows, int n) {
-  for (int e = threadIdx.x; e < kTile * DP; e += THREADS) {
-    const int r = e / DP, d = e % DP;
-    const float u = x[(int64_t)min(r0 + r, rows - 1) * stride + min(d, n - 1)];
-    tile[Tile<DP>::place(r, d / 4) + d % 4] = r0 + r < rows && d < n ? u : 0.0f;
+  constexpr int N = kTile * DP / THREADS;
+  float u[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = threadIdx.x + i * THREADS, r = e / DP, d = e % DP;
+    u[i] = x[(int64_t)min(r0 + r, rows - 1) * stride + min(d, n - 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = threadIdx.x + i * THREADS, r = e / DP, d = e % DP;
+    tile[Tile<DP>::place(r, d / 4) + d % 4] = r0 + r < rows && d < n ? u[i] : 0.0f;
   }
 }
 
@@ -166,11 +173,12 @@ struct SumsArgs {
   const float* rate;
   float *sums, *stay;              // [segs][B * H][n][ny], [segs][B * H]
 };
-template <int DP, bool WIDE>
+template <int DX, int DY, bool WIDE>
 __global__ __launch_bounds__(256) void linear_sums(SumsArgs A) {
-  using L = Tile<DP>;
-  constexpr int HB = DP / 32;      // a wavefront takes a quarter of the sums
-  __shared__ __align__(16) float xs[2][L::FLOATS], ys[2][L::FLOATS];
+  using LX = Tile<DX>;
+  using LY = Tile<DY>;
+  constexpr int BX = DX / 32, BY = DY / 32;   // a wavefront takes a quarter of the sums
+  __shared__ __align__(16) float xs[2][LX::FLOATS], ys[2][LY::FLOATS];
   __shared__ int since[kSeg];
   __shared__ float weight[kSeg];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15;
@@ -181,11 +189,11 @@ __global__ __launch_bounds__(256) void linear_sums(SumsArgs A) {
   const int stop = A.y.p ? min(s0 + kSeg, n) : s0;
   auto fetch = [&](int t0, int buf) {
     if (WIDE) {
-      tile_to_lds<DP, 4>(x, A.x.t, t0, A.m.T, A.n, lds_address(xs[buf]), w);
-      tile_to_lds<DP, 4>(y, A.y.t, t0, A.m.T, A.ny, lds_address(ys[buf]), w);
+      tile_to_lds<DX, 4>(x, A.x.t, t0, A.m.T, A.n, lds_address(xs[buf]), w);
+      tile_to_lds<DY, 4>(y, A.y.t, t0, A.m.T, A.ny, lds_address(ys[buf]), w);
     } else {
-      tile_by_hand<DP, 256>(xs[buf], x, A.x.t, t0, A.m.T, A.n);
-      tile_by_hand<DP, 256>(ys[buf], y, A.y.t, t0, A.m.T, A.ny);
+      tile_by_hand<DX, 256>(xs[buf], x, A.x.t, t0, A.m.T, A.n);
+      tile_by_hand<DY, 256>(ys[buf], y, A.y.t, t0, A.m.T, A.ny);
     }
   };
   const float rate = scalar(A.rate[h]);
@@ -194,26 +202,30 @@ __global__ __launch_bounds__(256) void linear_sums(SumsArgs A) {
   if (s0 < stop) fetch(s0, 0);
   if (tid < kSeg)
     weight[tid] = s0 + tid > e.last ? 0.0f : A.back ? A.scale * comes(since, s0, s0 + tid, rate) : leaves(e, since, s0, s0 + tid, rate);
-  const int dx = (w >> 1) * HB, dy = (w & 1) * HB;
-  f32x4 acc[HB][HB];
+  const int dx = (w >> 1) * BX, dy = (w & 1) * BY;
+  f32x4 acc[BX][BY];
 #pragma unroll
-  for (int i = 0; i < HB; ++i)
+  for (int i = 0; i < BX; ++i)
 #pragma unroll
-    for (int j = 0; j < HB; ++j) acc[i][j] = f32x4{};
+    for (int j = 0; j < BY; ++j) acc[i][j] = f32x4{};
   for (int t0 = s0, buf = 0; t0 < stop; t0 += kTile, buf ^= 1) {
     if (WIDE) loads_done();
     __syncthreads();
     if (t0 + kTile < stop) fetch(t0 + kTile, buf ^ 1);
     const float *X = xs[buf], *Y = ys[buf];
-    float u[2][HB], v[2][HB];
+    float u[2][BX], v[2][BY];
     auto read = [&](int k) {       // positions t0 + 4 k + g, ahead of their use by one step; weight 0: whatever they hold
       const int r = 4 * k + g;
       const float c = weight[t0 - s0 + r];
 #pragma unroll
-      for (int i = 0; i < HB; ++i) {
-        const float a = X[L::place(r, 4 * (dx + i) + l / 4) + l % 4], z = Y[L::place(r, 4 * (dy + i) + l / 4) + l % 4];
+      for (int i = 0; i < BX; ++i) {
+        const float a = X[LX::place(r, 4 * (dx + i) + l / 4) + l % 4];
         u[k & 1][i] = c == 0 ? 0.0f : a * c;
-        v[k & 1][i] = c == 0 ? 0.0f : z;
+      }
+#pragma unroll
+      for (int j = 0; j < BY; ++j) {
+        const float z = Y[LY::place(r, 4 * (dy + j) + l / 4) + l % 4];
+        v[k & 1][j] = c == 0 ? 0.0f : z;
       }
     };
     read(0);
@@ -221,18 +233,18 @@ __global__ __launch_bounds__(256) void linear_sums(SumsArgs A) {
     for (int k = 0; k < kTile / 4; ++k) {
       if (k + 1 < kTile / 4) read(k + 1);
 #pragma unroll
-      for (int i = 0; i < HB; ++i)
+      for (int i = 0; i < BX; ++i)
 #pragma unroll
-        for (int j = 0; j < HB; ++j) acc[i][j] = mfma(u[k & 1][i], v[k & 1][j], acc[i][j]);
+        for (int j = 0; j < BY; ++j) acc[i][j] = mfma(u[k & 1][i], v[k & 1][j], acc[i][j]);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
   const int64_t at = (int64_t)seg * (gridDim.x / A.segs) + bh;
   float* out = A.sums + at * A.n * A.ny;
 #pragma unroll
-  for (int i = 0; i < HB; ++i)
+  for (int i = 0; i < BX; ++i)
 #pragma unroll
-    for (int j = 0; j < HB; ++j) {
+    for (int j = 0; j < BY; ++j) {
       const int d = 16 * (dx + i) + 4 * g, c = 16 * (dy + j) + l;
 #pragma unroll
       for (int q = 0; q < 4; ++q) if (d + q < A.n && c < A.ny) out[(d + q) * A.ny + c] = acc[i][j][q];
@@ -371,15 +383,16 @@ __device__ __forceinline__ void plain_rows(const PairsArgs& p, const Sum& s, con
 }
 
 // A wavefront's 16 rows: B fragments, and results. A fragment is read one step ahead of its use.
-template <int DP, bool WIDE>
+template <int DN, int DZ, bool WIDE>   // features, padded: of the rows, of the results
 struct Own {
-  using L = Tile<DP>;
-  static constexpr int C = DP / 16;
-  float row[C][4];
-  f32x4 acc[C];
+  using LN = Tile<DN>;
+  using LZ = Tile<DZ>;
+  static constexpr int CN = DN / 16, CZ = DZ / 16;
+  float row[CN][4];
+  f32x4 acc[CZ];
   __device__ __forceinline__ void load(const float* at, int n, int g) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
+    for (int c = 0; c < CN; ++c) {
       const int d = 16 * c + 4 * g;
       if (WIDE) {
         const f32x4 u = *(const f32x4*)(at + (d < n ? d : 0));
@@ -395,25 +408,25 @@ struct Own {
   // loop over tiles, and there it waits for the next tiles too.
   __device__ __forceinline__ void start(bool here, int n, int g) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
+    for (int c = 0; c < CN; ++c)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         row[c][q] = here && 16 * c + 4 * g + (WIDE ? 0 : q) < n ? row[c][q] : 0.0f;
         asm volatile("" : "+v"(row[c][q]));
       }
-      acc[c] = f32x4{};
-    }
+#pragma unroll
+    for (int c = 0; c < CZ; ++c) acc[c] = f32x4{};
   }
   // tile rows times own rows: x[q] of tile row 16 (q / 4) + 4 g + q % 4
   __device__ __forceinline__ void dots(const float* tile, float (&x)[8], int g, int l) const {
     f32x4 s[2] = {}, u[2];
     int at[4];
-    L::by_piece(at, L::opaque(16 * g + l));
-    auto read = [&](int i) { u[i & 1] = *(const f32x4*)(tile + at[i / 2 % 4] + (16 * (i & 1) * L::PITCH + L::far(i / 2))); };
+    LN::by_piece(at, LN::opaque(16 * g + l));
+    auto read = [&](int i) { u[i & 1] = *(const f32x4*)(tile + at[i / 2 % 4] + (16 * (i & 1) * LN::PITCH + LN::far(i / 2))); };
     read(0);
 #pragma unroll
-    for (int i = 0; i < 2 * C; ++i) {
-      if (i + 1 < 2 * C) read(i + 1);
+    for (int i = 0; i < 2 * CN; ++i) {
+      if (i + 1 < 2 * CN) read(i + 1);
 #pragma unroll
       for (int q = 0; q < 4; ++q) s[i & 1] = mfma(u[i & 1][q], row[i / 2][q], s[i & 1]);
       __builtin_amdgcn_sched_barrier(0);
@@ -423,17 +436,17 @@ struct Own {
   }
   // acc += weights x on the tile's rows
   __device__ __forceinline__ void add(const float* tile, const float (&x)[8], int g, int l) {
-    constexpr int PART = C % 4 == 0 ? 4 : C % 3 == 0 ? 3 : C, PARTS = C / PART;   // MFMAs a step
+    constexpr int PART = CZ % 4 == 0 ? 4 : CZ % 3 == 0 ? 3 : CZ, PARTS = CZ / PART;   // MFMAs a step
     float u[2][PART];
     int row_[4], column[4];
-    if constexpr (DP > 32) L::by_column(row_, column, L::opaque(16 * g + l));
+    if constexpr (DZ > 32) LZ::by_column(row_, column, LZ::opaque(16 * g + l));
     auto read = [&](int step) {
       const int i = step / PARTS;
 #pragma unroll
       for (int e = 0; e < PART; ++e) {
         const int c = step % PARTS * PART + e;
-        if constexpr (DP > 32) u[step & 1][e] = tile[row_[i % 4] + column[c % 4] + (16 * (i / 4) * L::PITCH + L::far(c))];
-        else u[step & 1][e] = tile[16 * (i / 4) * L::PITCH + L::place(4 * g + i % 4, 4 * c + l / 4) + l % 4];
+        if constexpr (DZ > 32) u[step & 1][e] = tile[row_[i % 4] + column[c % 4] + (16 * (i / 4) * LZ::PITCH + LZ::far(c))];
+        else u[step & 1][e] = tile[16 * (i / 4) * LZ::PITCH + LZ::place(4 * g + i % 4, 4 * c + l / 4) + l % 4];
       }
     };
     read(0);
@@ -466,7 +479,7 @@ struct Own {
   __device__ __forceinline__ bool store(float* out, bool in, bool here, int n, int g) const {
     float bad = 0;                 // NaN for infinities and NaN
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
+    for (int c = 0; c < CZ; ++c) {
       const int d = 16 * c + 4 * g;
 #pragma unroll
       for (int q = 0; q < 4; ++q) bad = fmaf(acc[c][q], 0.0f, bad);
@@ -505,31 +518,31 @@ __device__ __forceinline__ void weights(float (&x)[8], const PairsArgs& p, const
 // while this one is multiplied, so that a tile costs one barrier. A wavefront walks the tiles that it has nothing to do with in
 // loops of their own: with a branch around the work the compiler copied all 32 registers of results for every tile, and had none
 // left for a second block on the CU.
-template <int DP>
+template <int DA, int DB>
 struct Ring {
-  float tile[2][2][Tile<DP>::FLOATS];
+  float tile[2][Tile<DA>::FLOATS + Tile<DB>::FLOATS];
 };
-template <int DP, int W, bool BACK, bool ACROSS>
-__device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int unit, Ring<DP>& ring, int (&since)[kSeg]) {
-  using L = Tile<DP>;
+template <int DN, int DZ, int W, bool BACK, bool ACROSS>
+__device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int unit, float* ring, int (&since)[kSeg]) {
+  constexpr int FZ = Tile<DZ>::FLOATS, HALF = FZ + Tile<DN>::FLOATS, FM = ACROSS ? FZ : 0;   // M's tile: as wide as its rows are
   const Place o = place_of<BACK>(p, s, unit, 16 * W);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15;
   const int T = p.m.T, w0 = o.r0 + 16 * w, r = w0 + l;
   const int mtiles = o.M ? (p.D + kTile - 1) / kTile : 0, count = mtiles + (o.from < o.to ? (o.to - o.from + kTile - 1) / kTile : 0);
   const int hx = BACK ? o.h0 : o.h0 / p.share;
   const float *M = o.M, *X = row_at(s.x, o.b, hx, 0), *Z = row_at(s.z, o.b, hx, 0);
-  const uint32_t base = lds_address(&ring);
+  const uint32_t base = lds_address(ring);
   int left = count * o.group, next = 0, into = 0;   // tiles to fetch; the next one of its head (of M, then of pairs), and where to
   auto fetch = [&]() {
     if (left == 0) return;
     --left;
-    const uint32_t to = base + into * (8 * L::FLOATS);
+    const uint32_t to = base + into * (4 * HALF);
     if (next < mtiles) {
-      tile_to_lds<DP, W>(M, p.Dv, next * kTile, p.D, p.Dv, to, w);
+      tile_to_lds<ACROSS ? DN : DZ, W>(M, p.Dv, next * kTile, p.D, p.Dv, to + 4 * FM, w);
     } else {
       const int t0 = o.from + (next - mtiles) * kTile;
-      tile_to_lds<DP, W>(Z, s.z.t, t0, T, s.nz, to, w);
-      tile_to_lds<DP, W>(X, s.x.t, t0, T, s.n, to + 4 * L::FLOATS, w);
+      tile_to_lds<DZ, W>(Z, s.z.t, t0, T, s.nz, to, w);
+      tile_to_lds<DN, W>(X, s.x.t, t0, T, s.n, to + 4 * FZ, w);
     }
     into ^= 1;
     if (++next == count) {
@@ -542,7 +555,7 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
     }
   };
   fetch();
-  Own<DP, true> own;
+  Own<DN, DZ, true> own;
   own.load(s.rows.p ? row_at(s.rows, o.b, o.head / p.keys, min(r, T - 1)) : p.any, s.rows.p ? s.n : 1, g);
   mark(p.m, o.b, o.s0, o.n, since);
   const Ends end = ends(since, o.s0, o.n);
@@ -560,10 +573,10 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
     const float rate = scalar(p.rate[o.h0 + gi]);
     const float coef = here ? p.by_state * (BACK ? leaves(end, since, o.s0, r, rate) : comes(since, o.s0, r, rate)) : 0.0f;
 #pragma unroll
-    for (int c = 0; c < DP / 32; ++c)
+    for (int c = 0; c < (ACROSS ? DZ : DN) / 32; ++c)
       if (c < mtiles) {
         arrive();
-        own.template state<ACROSS>(ring.tile[buf][0], c, coef, g, l);
+        own.template state<ACROSS>(ring + buf * HALF + FM, c, coef, g, l);
       }
     int t0 = o.from;
     if (BACK)
@@ -571,29 +584,29 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
     for (const int stop = BACK ? o.to : min(o.to, w0 + 16); t0 < stop; t0 += kTile) {
       arrive();
       float x[8], f[8];
-      own.dots(ring.tile[buf][1], x, g, l);
+      own.dots(ring + buf * HALF + FZ, x, g, l);
       __builtin_amdgcn_sched_barrier(0);
       weights<BACK>(f, p, o, rate, w0, r, t0, mine, since, g);
 #pragma unroll
       for (int q = 0; q < 8; ++q) x[q] = f[q] == 0 ? 0.0f : x[q] * f[q];
       __builtin_amdgcn_sched_barrier(0);
-      own.add(ring.tile[buf][0], x, g, l);
+      own.add(ring + buf * HALF, x, g, l);
     }
     for (; t0 < o.to; t0 += kTile) arrive();
   }
   const bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here, s.nz, g);
   if (__builtin_expect(!fine, 0)) plain_rows<BACK>(p, s, o, w0, since);
 }
-template <int DP, int W, bool BACK>
-__global__ __launch_bounds__(64 * W, W == 8 || DP <= 64 ? 4 : 2) void linear_tiles(PairsArgs p) {
-  __shared__ __align__(16) Ring<DP> ring;
+template <int DK, int DV, int W, bool BACK>   // features of keys and of values, padded
+__global__ __launch_bounds__(64 * W, W == 8 || DK + DV <= 128 ? 4 : 2) void linear_tiles(PairsArgs p) {
+  __shared__ __align__(16) Ring<DK, DV> ring;
   __shared__ int since[kSeg];
   // both sums of a place run one after the other on one XCD (blocks go to the 8 XCDs in turn), whose L2 then has their tiles
   const int id = blockIdx.x / 8, unit = (id / p.sums) * 8 + blockIdx.x % 8;
   if (unit >= p.blocks * p.B * p.heads) return;
   const Sum& s = p.sum[id % p.sums];
-  if (s.across) walk_tiles<DP, W, BACK, true>(p, s, unit, ring, since);
-  else walk_tiles<DP, W, BACK, false>(p, s, unit, ring, since);
+  if (s.across) walk_tiles<DV, DK, W, BACK, true>(p, s, unit, ring.tile[0], since);
+  else walk_tiles<DK, DV, W, BACK, false>(p, s, unit, ring.tile[0], since);
 }
 
 // The same for any alignment and number of features, tile by tile.
@@ -610,7 +623,7 @@ __global__ __launch_bounds__(256) void linear_pairs(PairsArgs p) {
   const Ends end = ends(since, o.s0, o.n);
   const int mine = r < T ? since[r - o.s0] : kNever;
   const bool here = mine != kNever;
-  Own<DP, false> own;
+  Own<DP, DP, false> own;
   own.load(s.rows.p ? row_at(s.rows, o.b, o.head / p.keys, min(r, T - 1)) : p.any, s.rows.p ? s.n : 1, g);
   own.start(here && s.rows.p, s.n, g);
   for (int gi = 0; gi < o.group; ++gi) {
@@ -764,10 +777,31 @@ inline int padded(const LinearDesc& a) { return (std::max(a.D, a.Dv) + 31) / 32 
 inline int64_t states_bytes(const LinearDesc& a) { return ((int64_t)segments(a) * a.B * a.H * a.D * a.Dv * 4 + 255) / 256 * 256; }
 inline int64_t stay_bytes(const LinearDesc& a) { return ((int64_t)segments(a) * a.B * a.H * 4 + 255) / 256 * 256; }
 
-template <int DP>
-void sums(const SumsArgs& s, bool wide, const dim3& grid, hipStream_t st) {
-  if (wide) klaunch(linear_sums<DP, true>, grid, dim3(256), 0, st, s);
-  else klaunch(linear_sums<DP, false>, grid, dim3(256), 0, st, s);
+// f(keys' features, values' features), padded, as constants. Values of another size than keys have kernels of their own (8 heads of
+// 128 and 16 features, 14 sequences of 617: forward @@); 96 features go with 96, or count as 128.
+template <class F>
+void by_sizes(const LinearDesc& a, F f) {
+  int k = (a.D + 31) / 32 * 32, v = (a.Dv + 31) / 32 * 32;
+  if (k == 96 || v == 96) k = v = std::max(k, v);
+  auto values = [&](auto K) {
+    if (v == 32) f(K, std::integral_constant<int, 32>());
+    else if (v == 64) f(K, std::integral_constant<int, 64>());
+    else f(K, std::integral_constant<int, 128>());
+  };
+  if (v == 96) f(std::integral_constant<int, 96>(), std::integral_constant<int, 96>());
+  else if (k == 32) values(std::integral_constant<int, 32>());
+  else if (k == 64) values(std::integral_constant<int, 64>());
+  else values(std::integral_constant<int, 128>());
+}
+// f(the larger of both, padded).
+template <class F>
+void by_larger(const LinearDesc& a, F f) {
+  switch (padded(a)) {
+    case 32: return f(std::integral_constant<int, 32>());
+    case 64: return f(std::integral_constant<int, 64>());
+    case 96: return f(std::integral_constant<int, 96>());
+    default: return f(std::integral_constant<int, 128>());
+  }
 }
 // States at the borders of all segments (in place of the sums), and the one at the end.
 void states(const LinearDesc& a, const Rows& x, const Rows& y, bool back, const float* first, float* last, float* at, float* stay, hipStream_t st) {
@@ -788,26 +822,12 @@ void states(const LinearDesc& a, const Rows& x, const Rows& y, bool back, const 
   s.stay = stay;
   const bool wide = a.D % 4 == 0 && a.Dv % 4 == 0 && wide_rows(x) && wide_rows(y);
   const dim3 grid((unsigned)(rows * s.segs));
-  switch (padded(a)) {
-    case 32: sums<32>(s, wide, grid, st); break;
-    case 64: sums<64>(s, wide, grid, st); break;
-    case 96: sums<96>(s, wide, grid, st); break;
-    default: sums<128>(s, wide, grid, st);
-  }
+  if (wide) by_sizes(a, [&](auto K, auto V) { klaunch(linear_sums<K.value, V.value, true>, grid, dim3(256), 0, st, s); });
+  else by_larger(a, [&](auto P) { klaunch(linear_sums<P.value, P.value, false>, grid, dim3(256), 0, st, s); });
   const JoinArgs j{at, s.stay, first, last, s.segs, rows, each, back};
   klaunch(linear_join, dim3((unsigned)((rows * each + 255) / 256)), dim3(256), 0, st, j);
 }
 
-template <int DP, bool BACK>
-void pairs(PairsArgs& p, bool wide, hipStream_t st) {
-  // 64 rows a block where 128 would leave the card half empty
-  const int rows = wide && (int64_t)((p.m.T + 127) / 128) * p.B * p.heads * p.sums >= 512 ? 128 : 64;
-  p.blocks = (p.m.T + rows - 1) / rows;
-  const int64_t units = (int64_t)p.blocks * p.B * p.heads, grid = (units + 7) / 8 * 8 * p.sums;
-  if (!wide) klaunch(linear_pairs<DP, BACK>, dim3((unsigned)units, p.sums), dim3(256), 0, st, p);
-  else if (rows == 64) klaunch(linear_tiles<DP, 4, BACK>, dim3((unsigned)grid), dim3(256), 0, st, p);
-  else klaunch(linear_tiles<DP, 8, BACK>, dim3((unsigned)grid), dim3(512), 0, st, p);
-}
 template <bool BACK>
 void pairs(PairsArgs p, const LinearDesc& a, const float* at, const float* edge, hipStream_t st) {
   p.m = {a.documents, a.lengths, a.T};
@@ -833,15 +853,19 @@ void pairs(PairsArgs p, const LinearDesc& a, const float* at, const float* edge,
     const Sum& s = p.sum[i];
     wide = wide && wide_rows(s.rows) && wide_rows(s.out) && wide_rows(s.x) && wide_rows(s.z);
   }
-  switch (padded(a)) {
-    case 32: pairs<32, BACK>(p, wide, st); break;
-    case 64: pairs<64, BACK>(p, wide, st); break;
-    case 96: pairs<96, BACK>(p, wide, st); break;
-    default: pairs<128, BACK>(p, wide, st);
+  // 64 rows a block where 128 would leave the card half empty
+  const int rows = wide && (int64_t)((a.T + 127) / 128) * p.B * p.heads * p.sums >= 512 ? 128 : 64;
+  p.blocks = (a.T + rows - 1) / rows;
+  const int64_t units = (int64_t)p.blocks * p.B * p.heads;
+  const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.sums));
+  if (!wide) {
+    by_larger(a, [&](auto P) { klaunch(linear_pairs<P.value, BACK>, dim3((unsigned)units, p.sums), dim3(256), 0, st, p); });
+  } else if (rows == 64) {
+    by_sizes(a, [&](auto K, auto V) { klaunch(linear_tiles<K.value, V.value, 4, BACK>, grid, dim3(256), 0, st, p); });
+  } else {
+    by_sizes(a, [&](auto K, auto V) { klaunch(linear_tiles<K.value, V.value, 8, BACK>, grid, dim3(512), 0, st, p); });
   }
 }
-template <int DP>
-void steps(const StepsArgs& s, hipStream_t st) { klaunch(linear_steps<DP>, dim3((unsigned)(s.a.B * s.a.H)), dim3(256), 0, st, s); }
 
 }  // namespace
 
@@ -853,12 +877,7 @@ int64_t linear_workspace_bytes(const LinearDesc& a) {
 void linear(const LinearDesc& a, void* work, hipStream_t st) {
   if (a.T <= kSteps) {
     const StepsArgs s{a, a.Dv % 4 == 0 && ((uintptr_t)a.state & 15) == 0 && ((uintptr_t)a.last & 15) == 0};
-    switch (padded(a)) {
-      case 32: return steps<32>(s, st);
-      case 64: return steps<64>(s, st);
-      case 96: return steps<96>(s, st);
-      default: return steps<128>(s, st);
-    }
+    return by_larger(a, [&](auto P) { klaunch(linear_steps<P.value>, dim3((unsigned)(a.B * a.H)), dim3(256), 0, st, s); });
   }
   float *stay = (float*)work, *at = a.borders ? a.borders : (float*)((char*)work + stay_bytes(a));
   if (a.last || a.borders || (a.y.p && segments(a) > 1)) states(a, a.k, a.v, false, a.state, a.last, at, stay, st);
