@@ -10,8 +10,7 @@
 //
 // G: the gradient of the state. y, dq, dk and dv have one form, out_r = sum_s w (row_r.X_s) Z_s + coef_r M row_r, and both states
 // another, so there are three kernels: sums over a segment (linear_sums), states from sums (linear_join), results from pairs and
-// states (linear_tiles; linear_pairs for rows that are not whole 16-byte pieces). A few positions are walked one after another
-// (linear_steps). Nothing is added by atomics.
+// states (linear_tiles). A few positions are walked one after another (linear_steps). Nothing is added by atomics.
 //
 // Products run on the f32 matrix instructions: no scales for operands of any size, and the work is bound by memory about as much.
 // Fragments of a 16 x 16 x 4 product: lane l holds row (A) or column (B) l % 16 and k = g = l / 16; a result's register q holds row
@@ -124,44 +123,34 @@ struct Tile {
   static __device__ __forceinline__ constexpr int far(int c) { return c / 4 * 64; }
 };
 
-// Rows [r0, r0 + 32) of x from memory straight into LDS, by WAVES wavefronts, 1 KiB an instruction. Nothing is masked: rows past the
-// last and features past the n-th are others that are there. In inline assembly, so that the compiler does not drain every load
-// before the next LDS read; the kernels wait (vmcnt) and meet (barrier) themselves.
-template <int DP, int WAVES>
+// Rows [r0, r0 + 32) of x from memory straight into LDS, by WAVES wavefronts: 16 bytes a lane, or (not WIDE: rows that are not whole
+// 16-byte pieces) 4, with addresses of 64 bits. Nothing is masked: rows past the last and features past the n-th are others that are
+// there. In inline assembly, so that the compiler does not drain every load before the next LDS read; the kernels wait (vmcnt) and
+// meet (barrier) themselves.
+template <int DP, int WAVES, bool WIDE>
 __device__ __forceinline__ void tile_to_lds(const float* x, int64_t stride, int r0, int rows, int n, uint32_t lds, int w) {
-  constexpr int PIECES = Tile<DP>::PIECES, ROWS = 64 / PIECES, N = kTile / ROWS;
+  constexpr int PIECES = Tile<DP>::PIECES, PITCH = Tile<DP>::PITCH, N = kTile * PITCH / (WIDE ? 256 : 64);
   const int lane = Tile<DP>::opaque(threadIdx.x & 63), left = rows - 1 - r0;
-  const char* base = (const char*)(x + (int64_t)r0 * stride);
+  const float* base = x + (int64_t)r0 * stride;
 #pragma unroll
   for (int i = 0; i < (N + WAVES - 1) / WAVES; ++i) {
     const int k = w + i * WAVES;
     if (N % WAVES && k >= N) break;
-    const int r = k * ROWS + lane / PIECES, c = (lane % PIECES) ^ Tile<DP>::swizzle(r);
-    const uint32_t off = (uint32_t)min(r, left) * (uint32_t)(4 * stride) + (4 * c < n ? 16 * c : 0);
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds + k * 1024));
+    if constexpr (WIDE) {
+      const int r = k * (64 / PIECES) + lane / PIECES, c = (lane % PIECES) ^ Tile<DP>::swizzle(r);
+      const uint32_t off = (uint32_t)min(r, left) * (uint32_t)(4 * stride) + (4 * c < n ? 16 * c : 0);
+      asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds + k * 1024));
+    } else {
+      const int e = k * 64 + lane, r = e / PITCH, c = (e % PITCH / 4) ^ Tile<DP>::swizzle(r);
+      const float* at = base + min(r, left) * stride + min(4 * c + e % 4, n - 1);
+      asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(at), "{m0}"(lds + k * 256));
+    }
   }
 }
 __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
-// The same through registers, for rows that are not whole 16-byte pieces; zero past the end.
-template <int DP, int THREADS>
-__device__ __forceinline__ void tile_by_hand(float* tile, const float* x, int64_t stride, int r0, int rows, int n) {
-  constexpr int N = kTile * DP / THREADS;
-  float u[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = threadIdx.x + i * THREADS, r = e / DP, d = e % DP;
-    u[i] = x[(int64_t)min(r0 + r, rows - 1) * stride + min(d, n - 1)];
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = threadIdx.x + i * THREADS, r = e / DP, d = e % DP;
-    tile[Tile<DP>::place(r, d / 4) + d % 4] = r0 + r < rows && d < n ? u[i] : 0.0f;
-  }
-}
-
 // ---- sums over a segment -----------------------------------------------------------------------------
 
 struct SumsArgs {
@@ -188,13 +177,8 @@ __global__ __launch_bounds__(256) void linear_sums(SumsArgs A) {
   const float* y = A.y.p + b * A.y.b + (h / A.share) * A.y.h;
   const int stop = A.y.p ? min(s0 + kSeg, n) : s0;
   auto fetch = [&](int t0, int buf) {
-    if (WIDE) {
-      tile_to_lds<DX, 4>(x, A.x.t, t0, A.m.T, A.n, lds_address(xs[buf]), w);
-      tile_to_lds<DY, 4>(y, A.y.t, t0, A.m.T, A.ny, lds_address(ys[buf]), w);
-    } else {
-      tile_by_hand<DX, 256>(xs[buf], x, A.x.t, t0, A.m.T, A.n);
-      tile_by_hand<DY, 256>(ys[buf], y, A.y.t, t0, A.m.T, A.ny);
-    }
+    tile_to_lds<DX, 4, WIDE>(x, A.x.t, t0, A.m.T, A.n, lds_address(xs[buf]), w);
+    tile_to_lds<DY, 4, WIDE>(y, A.y.t, t0, A.m.T, A.ny, lds_address(ys[buf]), w);
   };
   const float rate = scalar(A.rate[h]);
   mark(A.m, b, s0, n, since);
@@ -209,7 +193,7 @@ __global__ __launch_bounds__(256) void linear_sums(SumsArgs A) {
 #pragma unroll
     for (int j = 0; j < BY; ++j) acc[i][j] = f32x4{};
   for (int t0 = s0, buf = 0; t0 < stop; t0 += kTile, buf ^= 1) {
-    if (WIDE) loads_done();
+    loads_done();
     __syncthreads();
     if (t0 + kTile < stop) fetch(t0 + kTile, buf ^ 1);
     const float *X = xs[buf], *Y = ys[buf];
@@ -522,7 +506,7 @@ template <int DA, int DB>
 struct Ring {
   float tile[2][Tile<DA>::FLOATS + Tile<DB>::FLOATS];
 };
-template <int DN, int DZ, int W, bool BACK, bool ACROSS>
+template <int DN, int DZ, int W, bool BACK, bool WIDE, bool ACROSS>
 __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int unit, float* ring, int (&since)[kSeg]) {
   constexpr int FZ = Tile<DZ>::FLOATS, HALF = FZ + Tile<DN>::FLOATS, FM = ACROSS ? FZ : 0;   // M's tile: as wide as its rows are
   const Place o = place_of<BACK>(p, s, unit, 16 * W);
@@ -538,11 +522,11 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
     --left;
     const uint32_t to = base + into * (4 * HALF);
     if (next < mtiles) {
-      tile_to_lds<ACROSS ? DN : DZ, W>(M, p.Dv, next * kTile, p.D, p.Dv, to + 4 * FM, w);
+      tile_to_lds<ACROSS ? DN : DZ, W, WIDE>(M, p.Dv, next * kTile, p.D, p.Dv, to + 4 * FM, w);
     } else {
       const int t0 = o.from + (next - mtiles) * kTile;
-      tile_to_lds<DZ, W>(Z, s.z.t, t0, T, s.nz, to, w);
-      tile_to_lds<DN, W>(X, s.x.t, t0, T, s.n, to + 4 * FZ, w);
+      tile_to_lds<DZ, W, WIDE>(Z, s.z.t, t0, T, s.nz, to, w);
+      tile_to_lds<DN, W, WIDE>(X, s.x.t, t0, T, s.n, to + 4 * FZ, w);
     }
     into ^= 1;
     if (++next == count) {
@@ -555,7 +539,7 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
     }
   };
   fetch();
-  Own<DN, DZ, true> own;
+  Own<DN, DZ, WIDE> own;
   own.load(s.rows.p ? row_at(s.rows, o.b, o.head / p.keys, min(r, T - 1)) : p.any, s.rows.p ? s.n : 1, g);
   mark(p.m, o.b, o.s0, o.n, since);
   const Ends end = ends(since, o.s0, o.n);
@@ -597,7 +581,7 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
   const bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here, s.nz, g);
   if (__builtin_expect(!fine, 0)) plain_rows<BACK>(p, s, o, w0, since);
 }
-template <int DK, int DV, int W, bool BACK>   // features of keys and of values, padded
+template <int DK, int DV, int W, bool BACK, bool WIDE>   // features of keys and of values, padded
 __global__ __launch_bounds__(64 * W, W == 8 || DK + DV <= 128 ? 4 : 2) void linear_tiles(PairsArgs p) {
   __shared__ __align__(16) Ring<DK, DV> ring;
   __shared__ int since[kSeg];
@@ -605,58 +589,8 @@ __global__ __launch_bounds__(64 * W, W == 8 || DK + DV <= 128 ? 4 : 2) void line
   const int id = blockIdx.x / 8, unit = (id / p.sums) * 8 + blockIdx.x % 8;
   if (unit >= p.blocks * p.B * p.heads) return;
   const Sum& s = p.sum[id % p.sums];
-  if (s.across) walk_tiles<DV, DK, W, BACK, true>(p, s, unit, ring.tile[0], since);
-  else walk_tiles<DK, DV, W, BACK, false>(p, s, unit, ring.tile[0], since);
-}
-
-// The same for any alignment and number of features, tile by tile.
-template <int DP, bool BACK>
-__global__ __launch_bounds__(256) void linear_pairs(PairsArgs p) {
-  using L = Tile<DP>;
-  __shared__ __align__(16) float x_tile[L::FLOATS], z_tile[L::FLOATS];
-  __shared__ int since[kSeg];
-  const Sum& s = p.sum[blockIdx.y];
-  const Place o = place_of<BACK>(p, s, blockIdx.x, 64);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, l = lane & 15;
-  const int T = p.m.T, w0 = o.r0 + 16 * w, r = w0 + l;
-  mark(p.m, o.b, o.s0, o.n, since);
-  const Ends end = ends(since, o.s0, o.n);
-  const int mine = r < T ? since[r - o.s0] : kNever;
-  const bool here = mine != kNever;
-  Own<DP, DP, false> own;
-  own.load(s.rows.p ? row_at(s.rows, o.b, o.head / p.keys, min(r, T - 1)) : p.any, s.rows.p ? s.n : 1, g);
-  own.start(here && s.rows.p, s.n, g);
-  for (int gi = 0; gi < o.group; ++gi) {
-    const int h = o.h0 + gi, hx = BACK ? h : h / p.share;
-    const float rate = p.rate[h];
-    if (o.M) {
-      const float coef = here ? p.by_state * (BACK ? leaves(end, since, o.s0, r, rate) : comes(since, o.s0, r, rate)) : 0.0f;
-#pragma unroll
-      for (int c = 0; c < DP / 32; ++c) {
-        if (c * kTile >= p.D) break;
-        __syncthreads();
-        tile_by_hand<DP, 256>(z_tile, o.M + (int64_t)gi * p.D * p.Dv, p.Dv, c * kTile, p.D, p.Dv);
-        __syncthreads();
-        if (s.across) own.template state<true>(z_tile, c, coef, g, l);
-        else own.template state<false>(z_tile, c, coef, g, l);
-      }
-    }
-    for (int t0 = o.from; t0 < o.to; t0 += kTile) {
-      __syncthreads();
-      tile_by_hand<DP, 256>(x_tile, row_at(s.x, o.b, hx, 0), s.x.t, t0, T, s.n);
-      tile_by_hand<DP, 256>(z_tile, row_at(s.z, o.b, hx, 0), s.z.t, t0, T, s.nz);
-      __syncthreads();
-      if (BACK ? t0 + kTile <= w0 : t0 > w0 + 15) continue;
-      float x[8], f[8];
-      own.dots(x_tile, x, g, l);
-      weights<BACK>(f, p, o, rate, w0, r, t0, mine, since, g);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) x[q] = f[q] == 0 ? 0.0f : x[q] * f[q];
-      own.add(z_tile, x, g, l);
-    }
-  }
-  const bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here, s.nz, g);
-  if (!fine) plain_rows<BACK>(p, s, o, w0, since);
+  if (s.across) walk_tiles<DV, DK, W, BACK, WIDE, true>(p, s, unit, ring.tile[0], since);
+  else walk_tiles<DK, DV, W, BACK, WIDE, false>(p, s, unit, ring.tile[0], since);
 }
 
 // Sums of what each query head gave a key head's rows, in the heads' order.
@@ -854,17 +788,16 @@ void pairs(PairsArgs p, const LinearDesc& a, const float* at, const float* edge,
     wide = wide && wide_rows(s.rows) && wide_rows(s.out) && wide_rows(s.x) && wide_rows(s.z);
   }
   // 64 rows a block where 128 would leave the card half empty
-  const int rows = wide && (int64_t)((a.T + 127) / 128) * p.B * p.heads * p.sums >= 512 ? 128 : 64;
+  const int rows = (int64_t)((a.T + 127) / 128) * p.B * p.heads * p.sums >= 512 ? 128 : 64;
   p.blocks = (a.T + rows - 1) / rows;
   const int64_t units = (int64_t)p.blocks * p.B * p.heads;
   const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.sums));
-  if (!wide) {
-    by_larger(a, [&](auto P) { klaunch(linear_pairs<P.value, BACK>, dim3((unsigned)units, p.sums), dim3(256), 0, st, p); });
-  } else if (rows == 64) {
-    by_sizes(a, [&](auto K, auto V) { klaunch(linear_tiles<K.value, V.value, 4, BACK>, grid, dim3(256), 0, st, p); });
-  } else {
-    by_sizes(a, [&](auto K, auto V) { klaunch(linear_tiles<K.value, V.value, 8, BACK>, grid, dim3(512), 0, st, p); });
-  }
+  auto launch = [&](auto K, auto V, auto wide) {
+    if (rows == 64) klaunch(linear_tiles<K.value, V.value, 4, BACK, wide.value>, grid, dim3(256), 0, st, p);
+    else klaunch(linear_tiles<K.value, V.value, 8, BACK, wide.value>, grid, dim3(512), 0, st, p);
+  };
+  if (wide) by_sizes(a, [&](auto K, auto V) { launch(K, V, std::true_type()); });
+  else by_larger(a, [&](auto P) { launch(P, P, std::false_type()); });
 }
 
 }  // namespace
