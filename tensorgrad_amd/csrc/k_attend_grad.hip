@@ -40,9 +40,10 @@ __device__ __forceinline__ void seeing_tiles(const GradArgs& A, const Sight& s, 
 }
 // Those of part `split`, equal stretches of all rows, so that blocks that run together walk the same ones. False: none, which
 // the join finds again and does not read. With documents or a window the stretch that sees a key block is short: there its tiles are
-// cut into equal parts, of 8 at least (a window: of 20, and the long ones of keys that stay start first: 4096 rows of 4 slabs, head
-// size 128, a window of 512 and 4 sinks 373 us, by equal stretches of all rows 409), when they are known (8 x 1000 positions, 2 key heads of 64: documents of 50 take 47 us and
-// 10 to join instead of 121 uncut, of 170 66 and 11 instead of 165, one document 120 and 13 instead of 282).
+// cut into equal parts, of 8 at least, when they are known (8 x 1000 positions, 2 key heads of 64: documents of 50 take 47 us and 10
+// to join instead of 121 uncut, of 170 66 and 11 instead of 165, one document 120 and 13 instead of 282; 4096 rows of 4 slabs, head
+// size 128, a window of 512 and 4 sinks, 80 tiles a block: 257 and 36, in parts of 20 at least 369 and 28, by equal stretches of all
+// rows 409). With a window the long walks, of keys that stay, start first.
 __device__ __forceinline__ bool part_rows(const GradArgs& A, const Sight& s, int k0, int split, int& from, int& to) {
   seeing_tiles(A, s, k0, from, to);
   if (A.splits == 1 || s.doc || s.window) return true;
@@ -54,7 +55,7 @@ __device__ __forceinline__ bool part_rows(const GradArgs& A, const Sight& s, int
 
 __device__ __forceinline__ bool own_part(const GradArgs& A, const Sight& s, int split, int slab, int blk, int& t0, int& t1) {
   if (!(s.doc || s.window) || A.splits == 1) return true;
-  const int each = max((t1 - t0 + A.splits - 1) / A.splits, s.doc ? 8 : 20);
+  const int each = max((t1 - t0 + A.splits - 1) / A.splits, 8);
   if (split == 0 && threadIdx.x == 0) A.parts[slab * A.blocks + blk] = (t1 - t0 + each - 1) / each;
   t0 += split * each;
   t1 = min(t0 + each, t1);
