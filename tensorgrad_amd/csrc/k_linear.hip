@@ -95,11 +95,11 @@ __device__ __forceinline__ float stays(const Ends& e, int s0, float rate) {
 
 template <int DP>
 struct Tile {
-  static constexpr int PITCH = DP == 96 ? 128 : DP, PIECES = PITCH / 4, FLOATS = kTile * PITCH, C = DP / 16;
+  static constexpr int PITCH = DP == 96 ? 128 : DP, PIECES = PITCH / 4, FLOATS = kTile * PITCH;
   static __device__ __forceinline__ int swizzle(int r) { return DP == 32 ? (r >> 1) & 7 : r & 15; }
   static __device__ __forceinline__ int place(int r, int piece) { return r * PITCH + 4 * (piece ^ swizzle(r)); }
-  // Fragments. An opaque lane keeps the compiler from holding every place's address through a loop over tiles (230 registers
-  // instead of 124); where pieces are told apart by 4 c ^ .., what c's upper bits add is a constant of the instruction.
+  // Fragments. An opaque lane keeps the compiler from holding every place's address through a loop over tiles (142 registers
+  // instead of 121 for 128 features); where pieces are told apart by 4 c ^ .., what c's upper bits add is a constant of the instruction.
   static __device__ __forceinline__ int opaque(int lane) {
     asm volatile("" : "+v"(lane));
     return lane;
@@ -152,6 +152,11 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
 // ---- sums over a segment -----------------------------------------------------------------------------
+//
+// A block sums k v^T of a segment, four wavefronts a quarter of the product each, over tiles of 32 positions of which the next one
+// is on its way. Bound by memory: 64 heads of 4096 positions, 128 x 128 features, read 268 MB and write 134 MB of states in 115 us
+// (3.5 TB/s). Segments of 128: a state of 128 features then weighs as much as a segment's keys do; in longer ones the states'
+// bytes fall and the pairs, bound by the matrix instructions, rise.
 
 struct SumsArgs {
   Marks m;
@@ -246,6 +251,8 @@ struct JoinArgs {
   int64_t rows, each;
   bool back;
 };
+// A thread walks one value of a state through all segments. Bound by memory (the same 134 MB read and written: 42 us, 6.4 TB/s, out
+// of the last-level cache).
 __global__ __launch_bounds__(256) void linear_join(JoinArgs A) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, all = A.rows * A.each;
   if (id >= all) return;
@@ -498,7 +505,9 @@ __device__ __forceinline__ void weights(float (&x)[8], const PairsArgs& p, const
   }
 }
 
-// W wavefronts of 16 rows. The tiles of M, then those of the pairs, one after another; the next one travels to the other half of LDS
+// W wavefronts of 16 rows. Bound by the f32 matrix instructions: 64 heads of 4096 positions, 128 x 128 features, keep them busy for
+// 66 % of the cycles (y or dq 217 us, dk and dv 427; 19 GFLOP a result with the masked halves of tiles); what is lost is wavefronts
+// of early rows, which wait for the tiles of late ones. LDS has no conflicts. The tiles of M, then those of the pairs, one after another; the next one travels to the other half of LDS
 // while this one is multiplied, so that a tile costs one barrier. A wavefront walks the tiles that it has nothing to do with in
 // loops of their own: with a branch around the work the compiler copied all 32 registers of results for every tile, and had none
 // left for a second block on the CU.
@@ -593,7 +602,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || DK + DV <= 128 ? 4 : 2) void line
   else walk_tiles<DK, DV, W, BACK, WIDE, false>(p, s, unit, ring.tile[0], since);
 }
 
-// Sums of what each query head gave a key head's rows, in the heads' order.
+// Sums of what each query head gave a key head's rows, in the heads' order. Bound by memory (38 MB in 10 us).
 struct FoldArgs {
   const float* parts[2];           // [B][Hk * group][T][n]
   Rows out[2];
@@ -618,7 +627,8 @@ __global__ __launch_bounds__(256) void linear_fold(FoldArgs A) {
 
 constexpr int kSteps = 8;          // at most
 
-// A block keeps one head's state: a thread four columns of every RG-th row. Bound by memory: the state is read and written once.
+// A block keeps one head's state: a thread four columns of every RG-th row. Bound by memory: the state is read and written once (1024
+// heads of 128 x 128: 136 MB in 23 us, 5.9 TB/s).
 struct StepsArgs {
   LinearDesc a;
   bool wide;                       // of the states
@@ -787,8 +797,9 @@ void pairs(PairsArgs p, const LinearDesc& a, const float* at, const float* edge,
     const Sum& s = p.sum[i];
     wide = wide && wide_rows(s.rows) && wide_rows(s.out) && wide_rows(s.x) && wide_rows(s.z);
   }
-  // 64 rows a block where 128 would leave the card half empty
-  const int rows = (int64_t)((a.T + 127) / 128) * p.B * p.heads * p.sums >= 512 ? 128 : 64;
+  // 64 rows a block where 128 would be fewer than the card has compute units (8 heads of 4000 positions, 256 blocks of 128: a training
+  // step 93 us, of 64 99)
+  const int rows = a.T > 64 && (int64_t)((a.T + 127) / 128) * p.B * p.heads * p.sums >= 256 ? 128 : 64;
   p.blocks = (a.T + rows - 1) / rows;
   const int64_t units = (int64_t)p.blocks * p.B * p.heads;
   const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.sums));

@@ -1,16 +1,18 @@
 // Choice of the next token for gfx950: temperature, top-k, top-p and min-p from a given random number, see ops.py.
 //
 // Every limit keeps a first part of the tokens ordered by (falling logit, rising index), so the row is not sorted. Tokens are
-// counted and weighed in bins of their distance to the largest logit; the bin that a limit's border lies in is found by sums over
-// bins, its tokens alone are listed and sorted, and what is kept is told by one bound on (logit, index). Then the weights of what is
-// kept are summed in the vocabulary's order, and the stretch where the sum passes u of all is walked once more.
+// counted and weighed in bins of their distance to the largest logit; the bins that a limit's border may lie in are found by sums
+// over bins, their tokens alone are listed and sorted, and what is kept is told by one bound on (logit, index). The weights of what
+// is kept are summed by stretches of the vocabulary, and the stretch where the sum passes u of all is walked once more.
 //
 // Weights are whole numbers, exp(-z) times 2^unit with z = (largest - logit) / temperature in 64 bits and 62 bits for the sum of
 // all: sums do not depend on their order, so counts, borders and the choice agree with each other and repeat, and a weight is off by
 // 2^(-unit-1) of the largest at most. Beyond some 32 to 43 in z they are 0. A temperature of 0 is a top-k of 1.
 //
-// A row is read four times, the first time from memory. Many rows: a block takes one, in one launch (sample_one; sample_short, which
-// sorts all). Few rows of many tokens: several blocks a row, in six launches (sample_tops, _bins, _list, _bound, _sums, _pick).
+// A row is read three times, the first time from memory, and a stretch of it once more: for its largest logit; into bins, with
+// weights of 32 bits that tell where top_p's border is to be looked for; for the list, with the weights of 64 bits that decide. Many
+// rows: a block takes one, in one launch (sample_one; sample_short, which sorts all). Few rows of many tokens: several blocks a row,
+// in four launches (sample_tops, _bins, _list, _choice).
 #include <algorithm>
 #include <cfloat>
 
@@ -149,7 +151,7 @@ struct Work {
   uint32_t listed;
 };
 
-// The first 8 tokens of each kind that a thread asks for at once: f(i, x[i]) for its i of [from, to), `step` apart from `at`.
+// f(i, x[i]) for a thread's i of [from, to), `step` apart; 8 loads at once.
 template <class F>
 __device__ __forceinline__ void each_token(const float* x, int from, int to, int step, F f) {
   constexpr int N = 8;
@@ -622,7 +624,8 @@ __device__ __forceinline__ u64 goal_of(const Row& r, u64 all) { return min((u64)
 
 // ---- a block a row -------------------------------------------------------------------------------------
 
-// At most LIST tokens, all of them sorted: no bins, and for 256 a single wavefront. Bound by latency: some 20 dependent steps.
+// At most LIST tokens, all of them sorted: no bins, and for 256 a single wavefront. Bound by latency: the sort's dependent steps (64
+// rows of 65 tokens 8 us).
 template <int THREADS, int LIST>
 __global__ __launch_bounds__(THREADS) void sample_short(SampleDesc s) {
   constexpr int N = LIST / THREADS;
@@ -659,6 +662,9 @@ __global__ __launch_bounds__(THREADS) void sample_short(SampleDesc s) {
   choose<THREADS>(r, bound, 0, s.V, goal_of(r, all), w, s.token + row);
 }
 
+// 1024 threads a row, so that 256 rows fill the card. Bound by the weights in 64 bits, some 60 instructions of 4 to 8 cycles a token,
+// which every token up to a border needs once (256 rows of 50001, 51 MB: no limit 38 us, top-k of 50 34, top_p 0.9 53; limits of
+// their own in each row 54, 0.95 TB/s).
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void sample_one(SampleDesc s) {
   constexpr int W = THREADS / 64;
@@ -713,6 +719,11 @@ __global__ __launch_bounds__(THREADS) void sample_one(SampleDesc s) {
 }
 
 // ---- several blocks a row ------------------------------------------------------------------------------
+//
+// Parts of 4096 tokens or more, 1024 threads each: with 256 threads the rows' bins, joined by atomics on whole numbers, took 16 us
+// instead of 11. 32 rows of 200000 tokens (25.6 MB), temperature 1.6, top_p 0.95: largest logits 6 us, bins 11, list and weights 20
+// (bound by the weights in 64 bits), choice 16 (a sort of some 800 tokens 5, the rest dependent steps). 4 rows of 128000, top-k of 50:
+// 3, 4, 8 and 9: latency.
 
 constexpr int kPartThreads = 1024, kPartWaves = kPartThreads / 64, kParts = 256;   // parts: at most
 constexpr int kStretches = 4;      // of a part: what is kept is summed for each
@@ -872,8 +883,9 @@ struct SamplePlan {
 SamplePlan sample_plan(const SampleDesc& s) {
   SamplePlan p{};
   p.parts = 1;
-  // Several blocks a row where rows alone leave most of the card idle and are long enough.
-  if (s.rows < 128 && s.V > 8192) p.parts = (int)std::min<int64_t>((s.V + 4095) / 4096, std::max<int64_t>(kParts / s.rows, 1));
+  // Several blocks a row where rows alone leave half of the card idle and are long enough for four launches (top_p 0.9: a row of
+  // 20000 tokens 24 us, in one block 26; of 9000 24 and 19; 64 rows of 50001 37 and 48, 127 of them 47 and 49).
+  if (s.rows <= 128 && s.V > 24576) p.parts = (int)std::min<int64_t>((s.V + 4095) / 4096, std::max<int64_t>(kParts / s.rows, 1));
   p.each = ((s.V + p.parts - 1) / p.parts + kPartThreads - 1) / kPartThreads * kPartThreads;
   p.parts = (s.V + p.each - 1) / p.each;
   if (p.parts > 1) {

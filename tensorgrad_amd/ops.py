@@ -790,7 +790,8 @@ def sample(logits: Tensor, u: Tensor, temperature=1.0, top_k=None, top_p=None, m
 
     A limit is one number for all rows, or a tensor of u's shape with a number for each (f32, `top_k` i32); None, a top_k below 1
     or a top_p from 1 on do not limit, and a temperature of 0 takes the largest logit. Minus infinity and NaN are never chosen; a
-    row without any other logit gives -1. Weights below 2^-38 of the largest may count as 0 (2^-62 V, whatever V is)."""
+    row without any other logit gives -1. Weights are summed exactly, as whole multiples of 2^(b - 62) of the largest for a vocabulary
+    of b bits: what is smaller than half of that counts as 0."""
     site = 'sample'
     if logits.dtype != 'f32' or len(logits.shape) < 1 or min(logits.shape) < 1:
         raise ShapeError(f'{site}: logits must be f32 [..., vocabulary], got {logits.dtype} {S.show(logits.shape)}', site)

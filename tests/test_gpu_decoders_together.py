@@ -317,7 +317,7 @@ def test_windows_of_keys_shared_by_many_queries():
 @pytest.mark.parametrize('how', [dict(top_k=1024, top_p=0.97), dict(top_k=1025, top_p=0.97), dict(top_k=1025), dict(top_p=1e-30), dict(top_p=1 - 2.0 ** -40),
                                  dict(top_k=2, top_p=0.999999, min_p=1.0), dict(min_p=1e-12), dict(temperature=2.0 ** -149)],
                          ids=lambda h: '+'.join(f'{n}={x}' for n, x in h.items()))
-@pytest.mark.parametrize('rows,V', [(2, 2048), (3, 2049), (5, 8193), (130, 8193), (2, 30011)])
+@pytest.mark.parametrize('rows,V', [(2, 2048), (3, 2049), (5, 8193), (130, 8193), (2, 24576), (2, 24577), (129, 24577), (2, 30011)])
 def test_sample_limits_where_the_way_changes(rows, V, how):
     r = rng(rows, V, 66)
     check_sample(f32(2 * r.standard_normal((rows, V))), f32(r.random(rows)), **how)
