@@ -587,7 +587,7 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
     }
     for (; t0 < o.to; t0 += kTile) arrive();
   }
-  const bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here, s.nz, g);
+  const bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here && s.rows.p, s.nz, g);
   if (__builtin_expect(!fine, 0)) plain_rows<BACK>(p, s, o, w0, since);
 }
 template <int DK, int DV, int W, bool BACK, bool WIDE>   // features of keys and of values, padded

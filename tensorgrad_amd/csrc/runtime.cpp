@@ -4085,8 +4085,8 @@ tgk::LinearDesc Runtime::linear_fields(int i, Node& n) const {
   expect(ks[0] == qs[0] && vs[0] == qs[0] && ks[2] == qs[2] && vs[2] == qs[2] && ks[3] == qs[3] && ks[1] == vs[1] && qs[1] % ks[1] == 0, i,
          "q, k and v do not fit each other");
   expect(qs[3] <= tgk::kLinearMaxHead && vs[3] <= tgk::kLinearMaxHead, i, "head size above 128");
-  // a launch has fewer than 2^32 threads, 256 of them for 32 positions of a head, and for 256 values of a state
-  expect(qs[2] < (int64_t(1) << 30) && qs[0] * qs[1] * std::max((qs[2] + 31) / 32, (qs[3] * vs[3] + 255) / 256) < (int64_t(1) << 24), i,
+  // a launch has fewer than 2^32 threads: 256 for 64 positions of a head or 512 for 128, for two results, and 256 for 256 values of a state
+  expect(qs[2] < (int64_t(1) << 28) && qs[0] * qs[1] * std::max((qs[2] + 31) / 32, (qs[3] * vs[3] + 255) / 256) <= (int64_t(1) << 23) - 8, i,
          "too many rows");
   tgk::LinearDesc a{};
   a.B = (int)qs[0]; a.H = (int)qs[1]; a.T = (int)qs[2]; a.D = (int)qs[3];
@@ -4197,10 +4197,12 @@ void Runtime::lower_linear_grad(int i) {
     if (j != i && !same_fields(i, j, {TG_LINEAR, "dy", "dstate"})) continue;
     const std::string of = kinds_[j].substr(22);
     const int which = of == "q" ? 0 : of == "k" ? 1 : of == "v" ? 2 : 3;
-    if (out[which] >= 0) continue;
+    const int kept = which == 0 ? opt_fld(j, "borders") : -1;
+    if (out[which] >= 0 || (j != i && kept >= 0 && !ready_now(kept))) continue;
     out[which] = O(j).at("out").i32();
     expect(which < 3 || of == "state", j, "unknown gradient");
-    if (which == 0 && (borders = opt_fld(j, "borders")) >= 0) {
+    if (kept >= 0) {
+      borders = kept;
       const Dims bs = {(d.T + tgk::kLinearSegment - 1) / tgk::kLinearSegment, d.B, d.H, d.D, d.Dv};
       expect(T_[borders].shape == bs && T_[borders].dt == F32 && view_[borders].contiguous(), j, "bad borders' shape");
       n.reads.push_back(root(borders));

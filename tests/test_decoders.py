@@ -239,3 +239,41 @@ def test_states_between_segments_are_kept_for_the_gradients_that_read_them(T, op
         return [n['ops'].split(',') for n in nodes_of(ir) if n['kind'] == 'linear']
     assert made('qkv') == [['linear_attention', *ops]] and made('q') == [['linear_attention', *ops]]
     assert made('kv') == [['linear_attention']]
+
+
+def test_sizes_that_no_launch_can_hold_are_refused():
+    """Before anything is made: fewer than 2^32 threads a launch."""
+    def planned(B, T, D=1):
+        ir = build_forward_ir(Module(), lambda m, i: O.linear_attention(i['q'], i['q'], i['q'], [0.9] * 4)[0], {'q': [B, 4, T, D]})
+        return nodes_of(ir)
+    assert planned(2 ** 21 - 2, 32) and planned(1, 2 ** 26 - 256)
+    for bad in ((2 ** 21 - 1, 32), (2 ** 20, 65), (1, 2 ** 28), (2 ** 16, 1, 128)):
+        with pytest.raises(backend.BackendError, match='too many rows'):
+            planned(*bad)
+    draw = lambda rows: nodes_of(build_forward_ir(Module(), lambda m, i: O.sample(i['x'], i['u']), {'x': [rows, 2], 'u': [rows]}))  # noqa: E731
+    assert draw(2 ** 22 - 1)
+    with pytest.raises(backend.BackendError, match='too many rows'):
+        draw(2 ** 22)
+
+
+def test_bad_states_between_segments_are_refused_by_the_runtime():
+    build = lambda: O.linear_attention_grad(*qkv(T=200), t('dy', 2, 4, 200, 8), [0.5] * 4)[0]  # noqa: E731
+    backend.plan(wire(build, 'linear_attention_grad_q'))
+    backend.plan(wire(build, 'linear_attention_grad_q', borders=None))        # made again
+    for change in (dict(borders=0), dict(borders=10 ** 6), dict(dy=0, borders=1)):
+        with pytest.raises(backend.BackendError) as e:
+            backend.plan(wire(build, 'linear_attention_grad_q', **change))
+        assert e.value.status == backend.TG_INVALID_ARGUMENT, change
+
+
+def test_a_gradient_waits_for_the_states_it_reads():
+    """A document where those states are made after another gradient of the same attention: nodes in order."""
+    def build():
+        q, k, v = qkv(T=200)
+        dy = t('dy', 2, 4, 200, 8)
+        f = O._linear_fields('early', q, k, v, [0.5] * 4, None, None, None, None)
+        early = O.add_op(O.current_graph(), 'linear_attention_grad_k', k.shape, 'f32', 'early', dict(f, dy=dy.id, dstate=None))
+        return [early, *O.linear_attention_grad(q, k, v, dy, [0.5] * 4)]
+    doc = {'graph': IR.graph_to_wire(trace_fn(build)), 'paramGrads': {}, 'writebacks': [], 'optimizer': None}
+    assert [n['ops'] for n in backend.plan(IR.dumps(doc))['nodes'] if n['kind'].startswith('linear')] == [
+        'linear_attention_grad_k,linear_attention_grad_v', 'linear_attention_borders', 'linear_attention_grad_q,linear_attention_grad_k']

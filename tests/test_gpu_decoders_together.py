@@ -271,6 +271,18 @@ def test_linear_gradients_of_the_state_alone_with_wide_values(T):
     check_linear(a, [0.9])
 
 
+@pytest.mark.parametrize('T', [40, 300])
+def test_linear_queries_get_no_gradient_from_an_infinite_state_alone(T):
+    """Without a gradient of y nothing reaches the queries, whatever the state holds."""
+    a = linear_inputs(1, 2, 1, T, 32, 32, 68, True)
+    a['state'][0, 0, 3, 4], a['state'][0, 1, 5, 6] = np.inf, np.nan
+    a['v'][0, 0, T // 2, 7] = np.inf
+    def fn(i):
+        return list(O.linear_attention_grad(i['q'], i['k'], i['v'], None, decays(2), state=i['state'], dstate=i['dstate']))
+    dq, _, dv, _ = forward(fn, {n: x for n, x in a.items() if n != 'dy'})
+    assert not dq.any() and np.isfinite(dv).all()
+
+
 @pytest.mark.parametrize('shape', [(16, 4, 2, 512, 16, 16), (9, 6, 2, 900, 32, 20), (2, 4, 2, 140, 16, 19)])
 def test_linear_shared_heads_in_turn_and_apart(shape):
     """Enough blocks that one takes all query heads of a key head, and so few that each is taken alone."""
