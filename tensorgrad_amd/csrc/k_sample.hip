@@ -624,8 +624,8 @@ __device__ __forceinline__ u64 goal_of(const Row& r, u64 all) { return min((u64)
 
 // ---- a block a row -------------------------------------------------------------------------------------
 
-// At most LIST tokens, all of them sorted: no bins, and for 256 a single wavefront. Bound by latency: the sort's dependent steps (64
-// rows of 65 tokens 8 us).
+// At most LIST tokens, all of them sorted by a single wavefront: no bins. Bound by latency: the sort's dependent steps (64 rows of 65
+// tokens 8 us; 512 rows of 300, sorted by 256 threads, 16 where sample_one takes 14).
 template <int THREADS, int LIST>
 __global__ __launch_bounds__(THREADS) void sample_short(SampleDesc s) {
   constexpr int N = LIST / THREADS;
@@ -662,7 +662,7 @@ __global__ __launch_bounds__(THREADS) void sample_short(SampleDesc s) {
   choose<THREADS>(r, bound, 0, s.V, goal_of(r, all), w, s.token + row);
 }
 
-// 1024 threads a row, so that 256 rows fill the card. Bound by the weights in 64 bits, some 60 instructions of 4 to 8 cycles a token,
+// 1024 threads a row, so that 256 rows fill the card, or 256. Bound by the weights in 64 bits, some 60 instructions of 4 to 8 cycles a token,
 // which every token up to a border needs once (256 rows of 50001, 51 MB: no limit 38 us, top-k of 50 34, top_p 0.9 53; limits of
 // their own in each row 54, 0.95 TB/s).
 template <int THREADS>
@@ -904,8 +904,10 @@ void sample(const SampleDesc& s, void* work, hipStream_t st) {
   const SamplePlan p = sample_plan(s);
   const dim3 rows((unsigned)s.rows), grid((unsigned)p.parts, (unsigned)s.rows), block(kPartThreads);
   if (p.parts == 1) {
+    // 256 threads where a row is short, or more rows than compute units are not long: top-k of 50 of 512 rows of 4000 tokens 18 us, by
+    // 1024 threads 29, of 300 rows of 8000 22 and 28; of 4 rows of 8000 19 and 14, of 512 of 20000 41 and 38
     if (s.V <= 256) klaunch(sample_short<64, 256>, rows, dim3(64), 0, st, s);
-    else if (s.V <= 2048) klaunch(sample_short<256, 2048>, rows, dim3(256), 0, st, s);
+    else if (s.V <= 4096 || (s.rows > 256 && s.V <= 16384)) klaunch(sample_one<256>, rows, dim3(256), 0, st, s);
     else klaunch(sample_one<1024>, rows, dim3(1024), 0, st, s);
     return;
   }
