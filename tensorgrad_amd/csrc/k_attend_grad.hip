@@ -18,7 +18,7 @@ struct GradArgs {
   const TileInfo *qi, *gi, *ki, *vi;
   const float *qside, *kside;
   FastDiv group;
-  int M, qtiles, ktiles, blocks, splits, qsplits;     // splits: parts of the query rows; qsplits: parts of the keys
+  int M, qtiles, ktiles, blocks, splits, qsplits, least;   // splits: parts of the query rows, of `least` tiles; qsplits: of the keys
   bool wide;
   float *pk, *pv, *pq;                                // parts: of dk, dv [split][slab][Tk][D or Dv], of dq [qsplit][slab][M][D]
   int* parts;                                         // with documents or a window: parts of dk and dv that were written, [slab][blocks]
@@ -40,10 +40,10 @@ __device__ __forceinline__ void seeing_tiles(const GradArgs& A, const Sight& s, 
 }
 // Those of part `split`, equal stretches of all rows, so that blocks that run together walk the same ones. False: none, which
 // the join finds again and does not read. With documents or a window the stretch that sees a key block is short: there its tiles are
-// cut into equal parts, of 8 at least, when they are known (8 x 1000 positions, 2 key heads of 64: documents of 50 take 47 us and 10
-// to join instead of 121 uncut, of 170 66 and 11 instead of 165, one document 120 and 13 instead of 282; 4096 rows of 4 slabs, head
-// size 128, a window of 512 and 4 sinks, 80 tiles a block: 257 and 36, in parts of 20 at least 369 and 28, by equal stretches of all
-// rows 409). With a window the long walks, of keys that stay, start first.
+// cut into equal parts, of 8 at least (few rows with a window: 3), when they are known (8 x 1000 positions, 2 key heads of 64:
+// documents of 50 take 47 us and 10 to join instead of 121 uncut, of 170 66 and 11 instead of 165, one document 120 and 13 instead
+// of 282; 4096 rows of 4 slabs, head size 128, a window of 512 and 4 sinks, 80 tiles a block: 257 and 36, in parts of 20 at least
+// 369 and 28, by equal stretches of all rows 409). With a window the long walks, of keys that stay, start first.
 __device__ __forceinline__ bool part_rows(const GradArgs& A, const Sight& s, int k0, int split, int& from, int& to) {
   seeing_tiles(A, s, k0, from, to);
   if (A.splits == 1 || s.doc || s.window) return true;
@@ -55,7 +55,7 @@ __device__ __forceinline__ bool part_rows(const GradArgs& A, const Sight& s, int
 
 __device__ __forceinline__ bool own_part(const GradArgs& A, const Sight& s, int split, int slab, int blk, int& t0, int& t1) {
   if (!(s.doc || s.window) || A.splits == 1) return true;
-  const int each = max((t1 - t0 + A.splits - 1) / A.splits, 8);
+  const int each = max((t1 - t0 + A.splits - 1) / A.splits, A.least);
   if (split == 0 && threadIdx.x == 0) A.parts[slab * A.blocks + blk] = (t1 - t0 + each - 1) / each;
   t0 += split * each;
   t1 = min(t0 + each, t1);
@@ -498,7 +498,7 @@ __global__ __launch_bounds__(512) void attend_grad_q(GradArgs A) {
 // ---- plan --------------------------------------------------------------------------------------------
 
 struct GradPlan {
-  int DP, M, G, qtiles, ktiles, blocks, splits, qsplits, slabs;
+  int DP, M, G, qtiles, ktiles, blocks, splits, qsplits, least, slabs;
   int64_t qr, qc, gr, gc, kr, kc, vr, qi, gi, ki, vi, qside, kside, pk, pv, pq, parts, bytes;
 };
 GradPlan grad_plan(const AttendGradDesc& g) {
@@ -514,7 +514,9 @@ GradPlan grad_plan(const AttendGradDesc& g) {
   const int64_t have = (int64_t)p.slabs * p.blocks;
   // About 1024 blocks, two to four rounds of the card: 512 leave it to the longest (4096 causal rows of 4 slabs, head size 128:
   // 832 us and 21 to join, instead of 677 and 31), 2048 write and join twice the parts (624 and 58).
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((1024 + have - 1) / have, p.qtiles / 8));
+  // Of a window's few rows parts of 3 tiles: 19 slabs of 7 heads, 81 positions, head size 128, a training step 87 us instead of 98.
+  p.least = a.window && have * (p.qtiles / 8) < 256 ? 3 : 8;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((1024 + have - 1) / have, p.qtiles / p.least));
   // dq in parts only where its blocks leave compute units idle: 224 of them (32 slabs of 777 rows, head size 96) take 55 us, in
   // two parts 52 and 6 to join.
   p.qsplits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / ((int64_t)p.slabs * ((p.M + 127) / 128)), p.ktiles / 8));
@@ -593,7 +595,7 @@ void attend_grad(const AttendGradDesc& g, void* work, hipStream_t st) {
   attend_pack(k, p.DP, st);
   const GradArgs A{g, half(p.qr), half(p.qc), half(p.gr), half(p.gc), half(p.kr), half(p.kc), half(p.vr),
                    info(p.qi), info(p.gi), info(p.ki), info(p.vi), qs, ks, make_fastdiv(p.G), p.M, p.qtiles,
-                   p.ktiles, p.blocks, p.splits, p.qsplits, wide, (float*)(w + p.pk), (float*)(w + p.pv), (float*)(w + p.pq),
+                   p.ktiles, p.blocks, p.splits, p.qsplits, p.least, wide, (float*)(w + p.pk), (float*)(w + p.pv), (float*)(w + p.pq),
                    (int*)(w + p.parts)};
   if (p.DP == 32) run_grad<32>(A, p.slabs, st);
   else if (p.DP == 64) run_grad<64>(A, p.slabs, st);
