@@ -51,9 +51,9 @@ __device__ __forceinline__ Row row_of(const SampleDesc& s, int64_t row, float to
   r.x = s.logits + row * s.V;
   r.V = s.V;
   r.top = top;
-  const double heat = fmin(s.temperature ? (double)s.temperature[row] : s.temperature1, FLT_MAX);
-  const bool greedy = !(heat > 0);           // the first of the order
-  const double per = greedy ? 1 : 1 / heat;
+  const double heat = s.temperature ? (double)s.temperature[row] : s.temperature1;
+  const bool greedy = !(heat > 0);           // the first of the order; NaN too
+  const double per = greedy ? 1 : 1 / fmin(heat, FLT_MAX);
   r.unit = 62 - (s.V > 1 ? 32 - __clz(s.V - 1) : 0);
   r.per = per * (1 / kLn2);
   r.per1 = (float)r.per;
