@@ -41,7 +41,9 @@ __device__ __forceinline__ u64 order_of(uint32_t key, int i) { return (u64)key <
 struct Row {
   const float* x;
   int V, most, unit;
-  float top, per_bin, per1;        // largest logit; bins for a logit of 1 less; per in 32 bits
+  float top;                       // largest logit
+  float shrink, shrunk;            // 1 or, where differences of logits may pass f32, 1 / 2; top times it
+  float per_bin, per1;             // of differences times `shrink`: bins for 1; per in 32 bits
   double per, p, least, u;         // log2(e) / temperature; top_p; min_p times 2^unit; the random number
   bool by_count, by_mass;          // what limits
 };
@@ -56,8 +58,11 @@ __device__ __forceinline__ Row row_of(const SampleDesc& s, int64_t row, float to
   const double per = greedy ? 1 : 1 / fmin(heat, FLT_MAX);
   r.unit = 62 - (s.V > 1 ? 32 - __clz(s.V - 1) : 0);
   r.per = per * (1 / kLn2);
-  r.per1 = (float)r.per;
-  r.per_bin = (float)(per * (kBins / (1.001 * kLn2 * (r.unit + 1))));
+  const bool vast = top > 0x1p100f;          // up to there f32 holds the distance of any x
+  r.shrink = vast ? 0.5f : 1.0f;
+  r.shrunk = top * r.shrink;
+  r.per1 = (float)(vast ? 2 * r.per : r.per);
+  r.per_bin = (float)((vast ? 2 * per : per) * (kBins / (1.001 * kLn2 * (r.unit + 1))));
   r.most = greedy ? 1 : s.top_k ? s.top_k[row] : s.top_k1;
   r.p = s.top_p ? (double)s.top_p[row] : s.top_p1;
   r.least = __builtin_amdgcn_ldexp(s.min_p ? (double)s.min_p[row] : s.min_p1, r.unit);
@@ -85,16 +90,18 @@ __device__ __forceinline__ double weight(const Row& r, float x) {
   return __builtin_amdgcn_ldexp(fma(e, f, 1.0), r.unit - (int)n);
 }
 __device__ __forceinline__ u64 whole(double w) { return (u64)rint(w); }
+// per_bin or per1 times how far a logit is from the largest. None where it is the largest: the factor may be infinite, or both logits.
+__device__ __forceinline__ float distance(const Row& r, float x, float per) { return x == r.top ? 0.0f : fmaf(-x, r.shrink, r.shrunk) * per; }
 // A token's bin, rising with the distance to the top in equal steps; kBins: so far that its weight is 0, or not there.
 __device__ __forceinline__ int bin_of(const Row& r, float x) {
-  const float b = x == r.top ? 0.0f : (r.top - x) * r.per_bin;
+  const float b = distance(r, x, r.per_bin);
   return b < kBins ? (int)b : kBins;
 }
 
 // The same from 32 bits, 2^-17 of it off at most (and 1): what finds where a border is to be looked for.
 constexpr double kSlack = 0x1p-16;         // of a part of the sum: both sums off
 __device__ __forceinline__ u64 about(const Row& r, float x) {
-  return (u64)__builtin_amdgcn_exp2f((float)r.unit - (x == r.top ? 0.0f : (r.top - x) * r.per1));
+  return (u64)__builtin_amdgcn_exp2f((float)r.unit - distance(r, x, r.per1));
 }
 
 // Lanes' values without LDS: of a 64-bit number, by rows of 16 lanes (0 where there is none).

@@ -19,3 +19,15 @@ def test_sample_a_temperature_that_is_no_number_takes_the_largest_logit(V, how):
     heat = f32(np.where(np.arange(8) % 2, np.nan, 0.9))
     heat[6] = -1
     check_sample(f32(r.standard_normal((8, V))), f32(r.uniform(0.5, 1, 8)), temperature=heat, **how)
+
+
+@pytest.mark.parametrize('V', FORMS)
+@pytest.mark.parametrize('temperature', [1e38, 2.0 ** 127, 3e38])
+@pytest.mark.parametrize('how', [dict(), dict(top_k=50), dict(top_p=0.8), dict(min_p=0.1)], ids=['none', 'k', 'p', 'm'])
+def test_sample_logits_whose_difference_passes_f32(V, temperature, how):
+    """Each weighs by its distance to the largest, also where f32 cannot hold that."""
+    r = rng(V, 102)
+    logits, u = f32(3.4e38 * r.uniform(-1, 1, (8, V))), f32(r.random(8))
+    logits[4:6] = np.where(r.random((2, V)) < 0.1, np.float32(2e38), np.float32(-2e38)) * f32(r.uniform(0.9, 1, (2, V)))
+    logits[6, ::2] = -np.inf
+    check_sample(logits, u, temperature=temperature, **how)
