@@ -54,7 +54,8 @@ __device__ __forceinline__ Row row_of(const SampleDesc& s, int64_t row, float to
   r.V = s.V;
   r.top = top;
   const double heat = s.temperature ? (double)s.temperature[row] : s.temperature1;
-  const bool greedy = !(heat > 0);           // the first of the order; NaN too
+  const double share = s.min_p ? (double)s.min_p[row] : s.min_p1;
+  const bool greedy = !(heat > 0) || !(share <= 1);   // the first of the order alone; by NaN too
   const double per = greedy ? 1 : 1 / fmin(heat, FLT_MAX);
   r.unit = 62 - (s.V > 1 ? 32 - __clz(s.V - 1) : 0);
   r.per = per * (1 / kLn2);
@@ -65,7 +66,7 @@ __device__ __forceinline__ Row row_of(const SampleDesc& s, int64_t row, float to
   r.per_bin = (float)((vast ? 2 * per : per) * (kBins / (1.001 * kLn2 * (r.unit + 1))));
   r.most = greedy ? 1 : s.top_k ? s.top_k[row] : s.top_k1;
   r.p = s.top_p ? (double)s.top_p[row] : s.top_p1;
-  r.least = __builtin_amdgcn_ldexp(s.min_p ? (double)s.min_p[row] : s.min_p1, r.unit);
+  r.least = greedy ? 0 : __builtin_amdgcn_ldexp(share, r.unit);
   r.u = s.u[row];
   r.by_count = r.most > 0 && r.most < s.V;
   r.by_mass = r.p < 1 && !greedy;
@@ -315,7 +316,7 @@ __device__ __forceinline__ Sums list_and_sum(const Row& r, const Borders& o, int
       s.all += m;
       if (bin < o.b0) {
         s.before += m;
-        s.kept += w >= r.least || x == r.top ? m : 0;
+        s.kept += w >= r.least ? m : 0;
       }
     }
   });
@@ -429,9 +430,7 @@ __device__ __forceinline__ u64 bound_of_list(const Row& r, const Borders& o, int
     const u64 u = whole(m[e]);
     const bool in = i < kept && (double)before < target;
     mine += __popcll(__ballot(in));
-    if (in) {
-      if (m[e] >= r.least || value_of((uint32_t)(w.list[i] >> 32)) == r.top) add((int)(uint32_t)w.list[i], u);
-    }
+    if (in && m[e] >= r.least) add((int)(uint32_t)w.list[i], u);
     before += u;
   }
   if (lane == 0 && mine) atomicAdd(&w.found[0], (u64)mine);
@@ -581,7 +580,7 @@ __device__ __forceinline__ u64 bound_by_walks(const Row& r, Bins& b, Work& w) {
 __device__ __forceinline__ u64 kept_weight(const Row& r, u64 bound, int i, float x) {
   if (!(x > -INFINITY) || x < value_of((uint32_t)(bound >> 32)) || order_of(key_of(x), i) > bound) return 0;
   const double w = weight(r, x);
-  return w >= r.least || x == r.top ? whole(w) : 0;
+  return w >= r.least ? whole(w) : 0;
 }
 // Sum of the weights of [from, to), by a wavefront.
 __device__ __forceinline__ u64 stretch_sum(const Row& r, u64 bound, int from, int to) {
@@ -920,7 +919,7 @@ void sample(const SampleDesc& s, void* work, hipStream_t st) {
   }
   char* w = (char*)work;
   const PartArgs a{s, p.parts, p.each, (RowSpace*)w, (float*)(w + p.tops), (Sums*)(w + p.sums)};
-  const bool limits = s.temperature || !(s.temperature1 > 0) || s.top_k || s.top_p || (s.top_k1 > 0 && s.top_k1 < s.V) || s.top_p1 < 1;
+  const bool limits = s.temperature || s.min_p || !(s.temperature1 > 0) || s.top_k || s.top_p || (s.top_k1 > 0 && s.top_k1 < s.V) || s.top_p1 < 1;
   klaunch(sample_tops, grid, block, 0, st, a);
   if (limits) klaunch(sample_bins, grid, block, 0, st, a);
   klaunch(sample_list, grid, block, 0, st, a);

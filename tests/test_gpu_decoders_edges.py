@@ -31,3 +31,19 @@ def test_sample_logits_whose_difference_passes_f32(V, temperature, how):
     logits[4:6] = np.where(r.random((2, V)) < 0.1, np.float32(2e38), np.float32(-2e38)) * f32(r.uniform(0.9, 1, (2, V)))
     logits[6, ::2] = -np.inf
     check_sample(logits, u, temperature=temperature, **how)
+
+
+@pytest.mark.parametrize('V', FORMS)
+def test_sample_limits_out_of_range_keep_the_first_or_all(V):
+    """In tensors. The first of the order is always kept: alone by a min_p above 1 or not a number and by a top_p that is not above
+    0, equal logits behind it or not; a min_p below 0 and a top_p that is 1 at least or not a number do not limit."""
+    r = rng(V, 103)
+    logits = f32(np.round(r.standard_normal((24, V))))       # many equal ones at the top
+    p, m = np.ones(24, np.float32), np.zeros(24, np.float32)
+    m[:4], m[4:8], m[8:10], m[10:12] = 3.0, np.nan, np.inf, np.nextafter(np.float32(1), np.float32(2))
+    p[12:14], p[14:16], p[16:18], p[18:20], m[20:22], p[22:] = 0.0, -0.5, -np.inf, np.nan, -0.5, np.inf
+    k = np.where(np.arange(24) % 2, 30, 0).astype(np.int32)
+    got = check_sample(logits, f32(r.uniform(0.3, 1, 24)), top_p=p, min_p=m, top_k=k)
+    alone = np.arange(24) < 18
+    assert (got[alone] == logits[alone].argmax(1)).all() and (got[~alone] != logits[~alone].argmax(1)).any()
+    check_sample(logits, f32(r.uniform(0.3, 1, 24)), min_p=m)
