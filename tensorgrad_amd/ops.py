@@ -791,8 +791,10 @@ def sample(logits: Tensor, u: Tensor, temperature=1.0, top_k=None, top_p=None, m
     A limit is one number for all rows, or a tensor of u's shape with a number for each (f32, `top_k` i32); None, a top_k below 1
     or a top_p from 1 on do not limit, and a temperature of 0 takes the largest logit. In tensors, a temperature that is not above 0
     does so too (NaN with it); the first of the order is always kept, alone where top_p is not above 0, min_p above 1 or min_p NaN; a
-    top_p of NaN and a min_p below 0 do not limit. Minus infinity and NaN are never chosen; a row without any other logit gives -1. Weights are summed exactly, as whole multiples of 2^(b - 62) of the largest for a vocabulary
-    of b bits: what is smaller than half of that counts as 0."""
+    top_p of NaN and a min_p below 0 do not limit. Minus infinity and NaN are never chosen; a row without any other logit gives -1.
+
+    Weights are computed in 64 bits, 2^-50 of the largest off at most, and rounded to whole multiples of 2^(b - 62) of it for a
+    vocabulary of b bits (less than half of that counts as 0); sums of these are exact."""
     site = 'sample'
     if logits.dtype != 'f32' or len(logits.shape) < 1 or min(logits.shape) < 1:
         raise ShapeError(f'{site}: logits must be f32 [..., vocabulary], got {logits.dtype} {S.show(logits.shape)}', site)
