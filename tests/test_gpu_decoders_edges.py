@@ -2,7 +2,12 @@
 no numbers, logits and states near the ends of f32, infinities and NaN under decays that vanish."""
 import numpy as np
 import pytest
+import torch
 
+import _decoders as D
+from tensorgrad_amd import ops as O
+from tensorgrad_amd.compile import compile_forward
+from tensorgrad_amd.module import Module
 from test_gpu_decoders import check_sample, f32, rng
 
 pytestmark = pytest.mark.gpu
@@ -47,3 +52,53 @@ def test_sample_limits_out_of_range_keep_the_first_or_all(V):
     alone = np.arange(24) < 18
     assert (got[alone] == logits[alone].argmax(1)).all() and (got[~alone] != logits[~alone].argmax(1)).any()
     check_sample(logits, f32(r.uniform(0.3, 1, 24)), min_p=m)
+
+
+def mixed_rows(rows, V, seed):
+    """Rows without a limit, with each limit, all equal, rounded, flat, greedy, empty, masked, side by side."""
+    r = rng(rows, V, seed)
+    a = dict(logits=f32(2 * r.standard_normal((rows, V))), u=f32(r.random(rows)),
+             **{n: np.full(rows, x, t) for n, x, t in (('temperature', 1, np.float32), ('top_k', 0, np.int32), ('top_p', 1, np.float32), ('min_p', 0, np.float32))})
+    kinds = [dict(), dict(temperature=0), dict(top_k=40), dict(top_p=0.7), dict(), dict(top_k=5000), dict(top_p=0.9, top_k=3000), dict(min_p=0.2),
+             dict(temperature=np.finfo(np.float32).max), dict(top_k=2 ** 31 - 1), dict(top_p=0.99), dict(min_p=3.0), dict(temperature=np.nan),
+             dict(temperature=1e-30, top_p=0.5), dict(top_k=7, top_p=0.6, min_p=0.3)]
+    for i in range(rows):
+        for n, x in kinds[(i + seed) % len(kinds)].items():
+            a[n][i] = x
+    at = (np.arange(rows) + seed) % len(kinds)
+    a['logits'][at == 3] = 1.5
+    a['logits'][at == 4] = -np.inf
+    a['logits'][at == 5, ::3] = -np.inf
+    a['logits'][at == 6] = np.round(4 * a['logits'][at == 6]) / 4
+    a['logits'][at == 10] *= f32(0.01)
+    return a
+
+
+# sample_short; sample_one by 256 and by 1024 threads, twice for their two rules; several blocks a row
+@pytest.mark.parametrize('rows,V', [(20, 250), (20, 3001), (300, 9000), (30, 9000), (30, 20000), (16, 30011), (16, 70001), (128, 24577)])
+def test_sample_mixed_rows_one_batch_after_another(rows, V):
+    """Through one compiled graph: what one batch's rows left in the workspace reaches none of the next one's."""
+    batches = [mixed_rows(rows, V, s) for s in (0, 4, 9)]
+    decl = {n: {'shape': list(x.shape), 'dtype': 'i32' if x.dtype == np.int32 else 'f32'} for n, x in batches[0].items()}
+    ex = compile_forward(Module(), lambda m, i: O.sample(i['logits'], i['u'], i['temperature'], i['top_k'], i['top_p'], i['min_p']), decl,
+                         output='i32', seed=0)
+    want = [[D.sample(a['logits'][r], float(a['u'][r]), *(a[n][r].item() for n in ('temperature', 'top_k', 'top_p', 'min_p'))) for r in range(rows)]
+            for a in batches]
+    for turn in (0, 1, 2, 1, 0):
+        ins = {n: torch.from_numpy(x).cuda() for n, x in batches[turn].items()}
+        out = torch.full((rows,), -7, device='cuda', dtype=torch.int32)
+        torch.cuda.synchronize()
+        r = ex.run_device(ins, [out])
+        assert r.error is None, r.error
+        torch.cuda.synchronize()
+        assert out.tolist() == want[turn], turn
+    ex.destroy()
+
+
+@pytest.mark.parametrize('how', [dict(), dict(top_k=40, top_p=0.9), dict(temperature=1.5, top_p=0.97), dict(top_k=1025), dict(min_p=0.01)],
+                         ids=lambda h: '+'.join(f'{n}={x}' for n, x in h.items()) or 'none')
+@pytest.mark.parametrize('rows,V', [(5, 256), (5, 257), (5, 4096), (5, 4097), (256, 4097), (257, 4097), (256, 16384), (257, 16384), (257, 16385),
+                                    (128, 24576), (128, 24577), (129, 24577)])
+def test_sample_sizes_where_the_kernel_changes(rows, V, how):
+    r = rng(rows, V, 107)
+    check_sample(f32(2 * r.standard_normal((rows, V))), f32(r.random(rows)), **{n: min(x, V) if n == 'top_k' else x for n, x in how.items()})
