@@ -636,8 +636,8 @@ struct StepsArgs {
 template <int DP>
 __global__ __launch_bounds__(256) void linear_steps(StepsArgs A) {
   constexpr int CQ = DP <= 32 ? 8 : DP <= 64 ? 16 : 32, RG = 256 / CQ, R = (DP + RG - 1) / RG;
-  __shared__ float qs[kSteps][DP], ks[kSteps][DP], part[4][kSteps][4 * CQ];
-  __shared__ __align__(16) float vs[kSteps][4 * CQ];
+  __shared__ float qs[kSteps][DP], ks[kSteps][DP];
+  __shared__ __align__(16) float vs[kSteps][4 * CQ], part[4][kSteps][4 * CQ];   // by 16 bytes
   const LinearDesc& a = A.a;
   const int tid = threadIdx.x, cq = tid % CQ, rg = tid / CQ, w = tid >> 6, b = blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.Hk);
   const int n = count_of({a.documents, a.lengths, a.T}, b);
