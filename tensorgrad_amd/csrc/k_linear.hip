@@ -18,8 +18,8 @@
 // by 16 bytes, four steps of a product over features (k of step q is feature 4 g + q of 16), or by columns, a product over rows
 // whose k of step q is row 4 g + q, which is where the weights stand as they come out of the first product.
 //
-// What a row does not see has weight 0, and 0 times an infinity or NaN is NaN: rows whose result is not finite are computed again
-// pair by pair, from what they see alone.
+// What a row does not see has weight 0, and 0 times an infinity or NaN is NaN; a dot product may be infinite where no state is: rows
+// whose result is not finite are computed again pair by pair in 64 bits, from what they see alone.
 #include <algorithm>
 
 #include "kernels.h"
@@ -70,7 +70,8 @@ __device__ __forceinline__ void mark(const Marks& m, int b, int s0, int n, int* 
   }
   __syncthreads();
 }
-// The segment's last position that is there; what a position leaves of itself there, and of what came in.
+// The segment's last position that is there; and how often the decay applies, none (-1) where the weight is 0 by a mask: to what a
+// position leaves of itself there, to what came in at a position, and to what is left of it at the end.
 struct Ends {
   int last, since;                 // last < s0: none
 };
@@ -78,15 +79,12 @@ __device__ __forceinline__ Ends ends(const int* since, int s0, int n) {
   const int last = min(s0 + kSeg, n) - 1;
   return {last, last >= s0 ? since[last - s0] : kNever};
 }
-__device__ __forceinline__ float leaves(const Ends& e, const int* since, int s0, int j, float rate) {
-  return j <= e.last && since[j - s0] != kNever && j >= e.since ? power(rate, e.last - j) : 0.0f;
+__device__ __forceinline__ int leaves(const Ends& e, const int* since, int s0, int j) {
+  return j <= e.last && since[j - s0] != kNever && j >= e.since ? e.last - j : -1;
 }
-__device__ __forceinline__ float comes(const int* since, int s0, int i, float rate) {
-  return since[i - s0] == -1 ? power(rate, i - s0 + 1) : 0.0f;
-}
-__device__ __forceinline__ float stays(const Ends& e, int s0, float rate) {
-  return e.last < s0 ? 1.0f : e.since == -1 ? power(rate, e.last - s0 + 1) : 0.0f;
-}
+__device__ __forceinline__ int comes(const int* since, int s0, int i) { return since[i - s0] == -1 ? i - s0 + 1 : -1; }
+__device__ __forceinline__ int stays(const Ends& e, int s0) { return e.last < s0 ? 0 : e.since == -1 ? e.last - s0 + 1 : -1; }
+__device__ __forceinline__ float weight_of(float rate, int n) { return n < 0 ? 0.0f : power(rate, n); }
 
 // ---- tiles in LDS --------------------------------------------------------------------------------------
 //
@@ -190,7 +188,8 @@ __global__ __launch_bounds__(256) void linear_sums(SumsArgs A) {
   const Ends e = ends(since, s0, n);
   if (s0 < stop) fetch(s0, 0);
   if (tid < kSeg)
-    weight[tid] = s0 + tid > e.last ? 0.0f : A.back ? A.scale * comes(since, s0, s0 + tid, rate) : leaves(e, since, s0, s0 + tid, rate);
+    weight[tid] = s0 + tid > e.last ? 0.0f : A.back ? A.scale * weight_of(rate, comes(since, s0, s0 + tid))
+                                                                 : weight_of(rate, leaves(e, since, s0, s0 + tid));
   const int dx = (w >> 1) * BX, dy = (w & 1) * BY;
   f32x4 acc[BX][BY];
 #pragma unroll
@@ -238,7 +237,7 @@ __global__ __launch_bounds__(256) void linear_sums(SumsArgs A) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) if (d + q < A.n && c < A.ny) out[(d + q) * A.ny + c] = acc[i][j][q];
     }
-  if (tid == 0) A.stay[at] = stays(e, s0, rate);
+  if (tid == 0) A.stay[at] = weight_of(rate, stays(e, s0));
 }
 
 // ---- states at the segments' borders -------------------------------------------------------------------
@@ -318,7 +317,17 @@ __device__ __forceinline__ Place place_of(const PairsArgs& p, const Sum& s, int 
   return o;
 }
 
-// A wavefront's rows [w0, w0 + 16) pair by pair, a lane a pair or one or two features of the result.
+// Weights of 64 bits, for what is computed again: no operand or product of f32 values leaves their range, and an infinity times one of
+// them stays.
+__device__ __forceinline__ double power64(float rate, int n) {
+  const double e = (double)rate * n, k = floor(e);
+  return __builtin_amdgcn_ldexp((double)__builtin_amdgcn_exp2f((float)(e - k)), max((int)k, -1000));
+}
+__device__ __forceinline__ bool is_number(float x) { return fabsf(x) < INFINITY; }
+
+// A wavefront's rows [w0, w0 + 16) pair by pair in 64 bits, a lane a pair or one or two features of the result. What is not finite goes
+// where the states would carry it: a pair's X_e Z_d is a term of the state's entry (e, d), which row_e then multiplies. A row's own
+// infinities therefore meet whole entries; other features are taken through dot products.
 template <bool BACK>
 __device__ __forceinline__ void plain_rows(const PairsArgs& p, const Sum& s, const Place& o, int w0, const int* since) {
   const int lane = threadIdx.x & 63;
@@ -327,49 +336,70 @@ __device__ __forceinline__ void plain_rows(const PairsArgs& p, const Sum& s, con
     const int mine = since[r - o.s0];
     if (mine == kNever || !s.rows.p) continue;
     const float* row = row_at(s.rows, o.b, o.head / p.keys, r);
-    float acc[2] = {0, 0};
+    auto seen = [&](int t) {
+      const int from = since[t - o.s0], i = BACK ? t : r, j = BACK ? r : t;
+      return from != kNever && j <= i && j >= (BACK ? from : mine);
+    };
+    const int by = BACK ? leaves(ends(since, o.s0, o.n), since, o.s0, r) : comes(since, o.s0, r);
+    const int heads = (o.M && by >= 0) || o.from < o.to ? o.group : 0;   // none: it sees nothing at all
+    double acc[2] = {0, 0};
+    bool nan = false;              // then every feature is
 #pragma unroll 1
-    for (int gi = 0; gi < o.group; ++gi) {
+    for (int e = 0; e < s.n && heads > 0; ++e) nan |= row[e] != row[e];
+#pragma unroll 1
+    for (int gi = 0; gi < heads; ++gi) {
       const int h = o.h0 + gi, hx = BACK ? h : h / p.share;
       const float rate = p.rate[h];
-      const float coef = p.by_state * (BACK ? leaves(ends(since, o.s0, o.n), since, o.s0, r, rate) : comes(since, o.s0, r, rate));
-      if (o.M && coef != 0) {
-        const float* M = o.M + (int64_t)gi * p.D * p.Dv;
+      const double coef = by < 0 ? 0.0 : p.by_state * power64(rate, by);
+      const float* M = o.M && by >= 0 ? o.M + (int64_t)gi * p.D * p.Dv : nullptr;
+      auto state = [&](int e, int d) { return M ? coef * (s.across ? M[d * p.Dv + e] : M[e * p.Dv + d]) : 0.0; };
+      auto weight = [&](int t) { return power64(rate, BACK ? t - r : r - t) * p.by_pair; };
 #pragma unroll 1
-        for (int e = 0; e < s.n; ++e)
+      for (int e = 0; e < s.n; ++e)
 #pragma unroll
-          for (int a = 0; a < 2; ++a) {
-            const int d = 64 * a + lane;
-            if (d < s.nz) acc[a] = fmaf(row[e] * coef, s.across ? M[d * p.Dv + e] : M[e * p.Dv + d], acc[a]);
-          }
-      }
+        for (int a = 0; a < 2; ++a) {
+          const int d = 64 * a + lane;
+          if (d >= s.nz) continue;
+          double entry = state(e, d);
+          if (!is_number(row[e]) && !nan)
 #pragma unroll 1
-      for (int c = o.from; c < o.to; c += 64) {
-        const int t = c + lane, i = BACK ? t : r, j = BACK ? r : t;
-        float f = 0;
-        if (t < o.to && since[t - o.s0] != kNever && j <= i && j >= (BACK ? since[t - o.s0] : mine)) {
-          f = power(rate, i - j) * p.by_pair;
-          if (f != 0) {
-            const float* x = row_at(s.x, o.b, hx, t);
-            float dot = 0;
-#pragma unroll 1
-            for (int d = 0; d < s.n; ++d) dot = fmaf(x[d], row[d], dot);
-            f *= dot;
-          }
+            for (int t = o.from; t < o.to; ++t)
+              if (seen(t)) entry += weight(t) * row_at(s.x, o.b, hx, t)[e] * row_at(s.z, o.b, hx, t)[d];
+          acc[a] += row[e] * entry;
         }
 #pragma unroll 1
-        for (int z = 0; z < min(64, o.to - c); ++z) {
-          const float x = __shfl(f, z);
-          if (x == 0) continue;
-          const float* Z = row_at(s.z, o.b, hx, c + z);
+      for (int c = o.from; c < o.to; c += 64) {
+        const int t = c + lane;
+        const bool in = t < o.to && seen(t);
+        double f = 0;
+        if (in) {
+          const float* x = row_at(s.x, o.b, hx, t);
+#pragma unroll 1
+          for (int e = 0; e < s.n; ++e) if (is_number(row[e])) f += (double)x[e] * row[e];
+          f *= weight(t);
+        }
+        uint64_t left = __ballot(in);
+#pragma unroll 1
+        while (left) {
+          const int z = __ffsll((unsigned long long)left) - 1;
+          left &= left - 1;
+          const double w = __shfl(f, z);
+          const float *X = row_at(s.x, o.b, hx, c + z), *Z = row_at(s.z, o.b, hx, c + z);
 #pragma unroll
-          for (int a = 0; a < 2; ++a) if (64 * a + lane < s.nz) acc[a] = fmaf(x, Z[64 * a + lane], acc[a]);
+          for (int a = 0; a < 2; ++a) {
+            if (64 * a + lane >= s.nz) continue;
+            const float u = Z[64 * a + lane];
+            if (is_number(u)) acc[a] += w * u;
+            else
+#pragma unroll 1
+              for (int e = 0; e < s.n; ++e) if (is_number(row[e])) acc[a] += (double)X[e] * row[e] * u;
+          }
         }
       }
     }
     float* out = s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t;
 #pragma unroll
-    for (int a = 0; a < 2; ++a) if (64 * a + lane < s.nz) out[64 * a + lane] = acc[a];
+    for (int a = 0; a < 2; ++a) if (64 * a + lane < s.nz) out[64 * a + lane] = nan ? NAN : (float)acc[a];
   }
 }
 
@@ -564,7 +594,7 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
   };
   for (int gi = 0; gi < o.group; ++gi) {
     const float rate = scalar(p.rate[o.h0 + gi]);
-    const float coef = here ? p.by_state * (BACK ? leaves(end, since, o.s0, r, rate) : comes(since, o.s0, r, rate)) : 0.0f;
+    const float coef = here ? p.by_state * weight_of(rate, BACK ? leaves(end, since, o.s0, r) : comes(since, o.s0, r)) : 0.0f;
 #pragma unroll
     for (int c = 0; c < (ACROSS ? DZ : DN) / 32; ++c)
       if (c < mtiles) {
@@ -588,7 +618,10 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
     for (; t0 < o.to; t0 += kTile) arrive();
   }
   const bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here && s.rows.p, s.nz, g);
-  if (__builtin_expect(!fine, 0)) plain_rows<BACK>(p, s, o, w0, since);
+  if (__builtin_expect(!fine, 0)) {
+    loads_done();                  // the rows are written before they are written again
+    plain_rows<BACK>(p, s, o, w0, since);
+  }
 }
 template <int DK, int DV, int W, bool BACK, bool WIDE>   // features of keys and of values, padded
 __global__ __launch_bounds__(64 * W, W == 8 || DK + DV <= 128 ? 4 : 2) void linear_tiles(PairsArgs p) {

@@ -5,10 +5,11 @@ import pytest
 import torch
 
 import _decoders as D
+import _sequence as R
 from tensorgrad_amd import ops as O
 from tensorgrad_amd.compile import compile_forward
 from tensorgrad_amd.module import Module
-from test_gpu_decoders import check_sample, f32, rng
+from test_gpu_decoders import check_linear, check_sample, f32, linear_inputs, rng, run_linear
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +103,65 @@ def test_sample_mixed_rows_one_batch_after_another(rows, V):
 def test_sample_sizes_where_the_kernel_changes(rows, V, how):
     r = rng(rows, V, 107)
     check_sample(f32(2 * r.standard_normal((rows, V))), f32(r.random(rows)), **{n: min(x, V) if n == 'top_k' else x for n, x in how.items()})
+
+
+# ---- linear attention -------------------------------------------------------------------------------
+
+def by_positions(a, decay, scale):
+    """The definition position by position in 64 bits, forward and backward, so that what is not finite goes where it goes."""
+    q, k, v, dy = (a[n].astype(np.float64) for n in ('q', 'k', 'v', 'dy'))
+    B, H, T, _ = q.shape
+    G = H // k.shape[1]
+    out = dict(y=np.zeros(dy.shape), state=np.zeros(a['state'].shape), dq=np.zeros(q.shape), dk=np.zeros(k.shape), dv=np.zeros(v.shape),
+               dstate=np.zeros(a['state'].shape))
+    for b in range(B):
+        for h in range(H):
+            S, states = a['state'][b, h].astype(np.float64), []
+            for t in range(T):
+                S = decay[h] * S + np.outer(k[b, h // G, t], v[b, h // G, t])
+                states.append(S)
+                out['y'][b, h, t] = scale * (S * q[b, h, t][:, None]).sum(0)
+                out['dq'][b, h, t] = scale * (S * dy[b, h, t]).sum(1)
+            out['state'][b, h] = S
+            g = a['dstate'][b, h].astype(np.float64)
+            for t in reversed(range(T)):
+                g = g + scale * np.outer(q[b, h, t], dy[b, h, t])
+                out['dk'][b, h // G, t] += (g * v[b, h // G, t]).sum(1)
+                out['dv'][b, h // G, t] += (g * k[b, h // G, t][:, None]).sum(0)
+                g = decay[h] * g
+            out['dstate'][b, h] = g
+    return out
+
+
+@pytest.mark.parametrize('shape', [(2, 2, 1, 5, 32, 32), (1, 2, 2, 100, 64, 64), (1, 4, 2, 300, 64, 32), (1, 2, 1, 420, 15, 19), (1, 2, 1, 300, 128, 96)])
+@pytest.mark.parametrize('decay', [0.9])
+@pytest.mark.parametrize('where', ['q', 'k', 'v', 'state', 'dy', 'dstate'])
+def test_linear_infinities_go_where_states_carry_them(shape, decay, where):
+    """Infinities and NaN in any operand are in the states, results and gradients that they are in by the definition."""
+    a = linear_inputs(*shape, 104, True)
+    H, T = shape[1], shape[3]
+    lam = [decay] + [0.9] * (H - 1)
+    scale = shape[4] ** -0.5
+    for n, x in enumerate((np.inf, np.nan, -np.inf)):
+        clean = {m: z.copy() for m, z in a.items()}
+        bad = {m: z.copy() for m, z in a.items()}
+        at = (0, 0, {'q': T - 2, 'dy': T - 2}.get(where, 1), n) if where not in ('state', 'dstate') else (0, 0, n, 2)
+        bad[where][at], clean[where][at] = x, 0
+        with np.errstate(all='ignore'):
+            want = by_positions(bad, lam, scale)
+        _, tol = D.linear(**clean, decay=lam)
+        got = run_linear(bad, lam)
+        for m in want:
+            w, fine = want[m], np.isfinite(want[m])
+            assert (np.isfinite(got[m]) == fine).all(), (where, x, m)
+            assert (np.isnan(got[m]) == np.isnan(w)).all() and (got[m] == w)[np.isinf(w)].all(), (where, x, m)
+            R.check(np.where(fine, got[m], 0), np.where(fine, w, 0), np.where(fine, tol[m], 0), f'{where} {x} {m}')
+
+
+@pytest.mark.parametrize('decay', [1.0, 0.9, 0.4])
+def test_linear_products_that_pass_f32_on_the_way(decay):
+    """q.k is infinite in 32 bits where no state and no result is."""
+    a = linear_inputs(1, 2, 1, 200, 32, 32, 106, True)
+    for n, e in (('q', 70), ('k', 60), ('v', -40), ('dy', -50), ('state', 20), ('dstate', 20)):
+        a[n] *= f32(2.0 ** e)
+    check_linear(a, [decay] * 2)
