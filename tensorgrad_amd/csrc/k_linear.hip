@@ -84,7 +84,32 @@ __device__ __forceinline__ int leaves(const Ends& e, const int* since, int s0, i
 }
 __device__ __forceinline__ int comes(const int* since, int s0, int i) { return since[i - s0] == -1 ? i - s0 + 1 : -1; }
 __device__ __forceinline__ int stays(const Ends& e, int s0) { return e.last < s0 ? 0 : e.since == -1 ? e.last - s0 + 1 : -1; }
-__device__ __forceinline__ float weight_of(float rate, int n) { return n < 0 ? 0.0f : power(rate, n); }
+
+// 2^(rate n) as a product, so that a state counts where its weight alone is below f32's range: down to 2^-226 together, and exactly
+// `near` down to 2^-100. A negative `near` stands for a weight that a mask makes 0.
+struct Weight {
+  float near, far;
+};
+__device__ __forceinline__ Weight weight_of(float rate, int n) {
+  const float e = rate * (float)n;
+  return n < 0 ? Weight{-1.0f, 0.0f} : Weight{__builtin_amdgcn_exp2f(fmaxf(e, -100.0f)), __builtin_amdgcn_exp2f(fminf(e + 100.0f, 0.0f))};
+}
+// The same as a factor above 1 / 2 and a power of 2, by which a state is multiplied: no decay above 0 forgets an infinity or NaN.
+struct Decay {
+  float factor;
+  int shift;
+};
+__device__ __forceinline__ Decay decay_of(float e) {   // of 2^e
+  const float whole = ceilf(e);
+  return {__builtin_amdgcn_exp2f(e - whole), (int)whole};
+}
+__device__ __forceinline__ bool is_number(float x) { return fabsf(x) < INFINITY; }
+// Weights of 64 bits, for what is computed again: no operand or product of f32 values leaves their range, and an infinity times one of
+// them stays.
+__device__ __forceinline__ double power64(float rate, int n) {
+  const double e = (double)rate * n, k = floor(e);
+  return __builtin_amdgcn_ldexp((double)__builtin_amdgcn_exp2f((float)(e - k)), max((int)k, -1000));
+}
 
 // ---- tiles in LDS --------------------------------------------------------------------------------------
 //
@@ -163,7 +188,8 @@ struct SumsArgs {
   bool back;                       // back: of q and dy, weights c, else of k and v, weights e
   float scale;
   const float* rate;
-  float *sums, *stay;              // [segs][B * H][n][ny], [segs][B * H]
+  float* sums;                     // [segs][B * H][n][ny]
+  float* stay;                     // [segs][B * H]: log2 of what stays of the state that came in; 1: nothing
 };
 template <int DX, int DY, bool WIDE>
 __global__ __launch_bounds__(256) void linear_sums(SumsArgs A) {
@@ -172,7 +198,7 @@ __global__ __launch_bounds__(256) void linear_sums(SumsArgs A) {
   constexpr int BX = DX / 32, BY = DY / 32;   // a wavefront takes a quarter of the sums
   __shared__ __align__(16) float xs[2][LX::FLOATS], ys[2][LY::FLOATS];
   __shared__ int since[kSeg];
-  __shared__ float weight[kSeg];
+  __shared__ Weight weight[kSeg];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15;
   const int seg = blockIdx.x % A.segs, bh = blockIdx.x / A.segs, b = bh / A.H, h = bh % A.H, s0 = seg * kSeg;
   const int n = count_of(A.m, b);
@@ -187,64 +213,91 @@ __global__ __launch_bounds__(256) void linear_sums(SumsArgs A) {
   mark(A.m, b, s0, n, since);
   const Ends e = ends(since, s0, n);
   if (s0 < stop) fetch(s0, 0);
-  if (tid < kSeg)
-    weight[tid] = s0 + tid > e.last ? 0.0f : A.back ? A.scale * weight_of(rate, comes(since, s0, s0 + tid))
-                                                                 : weight_of(rate, leaves(e, since, s0, s0 + tid));
+  auto times = [&](int t) { return A.back ? comes(since, s0, t) : leaves(e, since, s0, t); };
+  if (tid < kSeg) {
+    Weight c = weight_of(rate, s0 + tid > e.last ? -1 : times(s0 + tid));
+    if (A.back && c.near > 0) (c.near * A.scale >= 0x1p-110f ? c.near : c.far) *= A.scale;   // where it keeps both in range
+    weight[tid] = c;
+  }
   const int dx = (w >> 1) * BX, dy = (w & 1) * BY;
   f32x4 acc[BX][BY];
 #pragma unroll
   for (int i = 0; i < BX; ++i)
 #pragma unroll
     for (int j = 0; j < BY; ++j) acc[i][j] = f32x4{};
-  for (int t0 = s0, buf = 0; t0 < stop; t0 += kTile, buf ^= 1) {
-    loads_done();
-    __syncthreads();
-    if (t0 + kTile < stop) fetch(t0 + kTile, buf ^ 1);
-    const float *X = xs[buf], *Y = ys[buf];
-    float u[2][BX], v[2][BY];
-    auto read = [&](int k) {       // positions t0 + 4 k + g, ahead of their use by one step; weight 0: whatever they hold
-      const int r = 4 * k + g;
-      const float c = weight[t0 - s0 + r];
+  // `far` is not 1 only where the decay is fast or the scale small; the loop with it takes 3 % longer
+  auto walk = [&](auto far) {
+    constexpr bool FAR = far.value;
+    for (int t0 = s0, buf = 0; t0 < stop; t0 += kTile, buf ^= 1) {
+      loads_done();
+      __syncthreads();
+      if (t0 + kTile < stop) fetch(t0 + kTile, buf ^ 1);
+      const float *X = xs[buf], *Y = ys[buf];
+      float u[2][BX], v[2][BY];
+      auto read = [&](int k) {       // positions t0 + 4 k + g, ahead of their use by one step; 0 where masked, whatever they hold
+        const int r = 4 * k + g;
+        const Weight c = weight[t0 - s0 + r];
 #pragma unroll
-      for (int i = 0; i < BX; ++i) {
-        const float a = X[LX::place(r, 4 * (dx + i) + l / 4) + l % 4];
-        u[k & 1][i] = c == 0 ? 0.0f : a * c;
+        for (int i = 0; i < BX; ++i) {
+          const float a = X[LX::place(r, 4 * (dx + i) + l / 4) + l % 4];
+          u[k & 1][i] = c.near < 0 ? 0.0f : a * c.near;
+        }
+#pragma unroll
+        for (int j = 0; j < BY; ++j) {
+          const float z = Y[LY::place(r, 4 * (dy + j) + l / 4) + l % 4];
+          v[k & 1][j] = c.near < 0 ? 0.0f : FAR ? z * c.far : z;
+        }
+      };
+      read(0);
+#pragma unroll
+      for (int k = 0; k < kTile / 4; ++k) {
+        if (k + 1 < kTile / 4) read(k + 1);
+#pragma unroll
+        for (int i = 0; i < BX; ++i)
+#pragma unroll
+          for (int j = 0; j < BY; ++j) acc[i][j] = mfma(u[k & 1][i], v[k & 1][j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int j = 0; j < BY; ++j) {
-        const float z = Y[LY::place(r, 4 * (dy + j) + l / 4) + l % 4];
-        v[k & 1][j] = c == 0 ? 0.0f : z;
-      }
-    };
-    read(0);
-#pragma unroll
-    for (int k = 0; k < kTile / 4; ++k) {
-      if (k + 1 < kTile / 4) read(k + 1);
-#pragma unroll
-      for (int i = 0; i < BX; ++i)
-#pragma unroll
-        for (int j = 0; j < BY; ++j) acc[i][j] = mfma(u[k & 1][i], v[k & 1][j], acc[i][j]);
-      __builtin_amdgcn_sched_barrier(0);
     }
-  }
+  };
+  if (rate * kSeg < -100.0f || (A.back && A.scale < 0x1p-10f)) walk(std::true_type());
+  else walk(std::false_type());
   const int64_t at = (int64_t)seg * (gridDim.x / A.segs) + bh;
   float* out = A.sums + at * A.n * A.ny;
+  float bad = 0;                   // NaN for infinities and NaN
 #pragma unroll
   for (int i = 0; i < BX; ++i)
 #pragma unroll
     for (int j = 0; j < BY; ++j) {
       const int d = 16 * (dx + i) + 4 * g, c = 16 * (dy + j) + l;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) if (d + q < A.n && c < A.ny) out[(d + q) * A.ny + c] = acc[i][j][q];
+      for (int q = 0; q < 4; ++q) {
+        bad = fmaf(acc[i][j][q], 0.0f, bad);
+        if (d + q < A.n && c < A.ny) out[(d + q) * A.ny + c] = acc[i][j][q];
+      }
     }
-  if (tid == 0) A.stay[at] = weight_of(rate, stays(e, s0));
+  if (tid == 0) A.stay[at] = stays(e, s0) < 0 ? 1.0f : rate * (float)stays(e, s0);
+  if (__builtin_expect(!__any(bad != bad), 1)) return;
+  // again in 64 bits, a lane its own entries: an infinity times a weight that is 0 in 32 bits is an infinity
+  loads_done();                    // they are written before they are written again
+#pragma unroll 1
+  for (int i = 0; i < 4 * BX * BY; ++i) {
+    const int d = 16 * (dx + i / (4 * BY)) + 4 * g + i % 4, c = 16 * (dy + i / 4 % BY) + l;
+    if (d >= A.n || c >= A.ny) continue;
+    double sum = 0;
+#pragma unroll 1
+    for (int t = s0; t < min(stop, e.last + 1); ++t)
+      if (times(t) >= 0) sum += (double)x[(int64_t)t * A.x.t + d] * y[(int64_t)t * A.y.t + c] * power64(rate, times(t));
+    out[d * A.ny + c] = (float)(A.back ? sum * A.scale : sum);
+  }
 }
 
 // ---- states at the segments' borders -------------------------------------------------------------------
 
 struct JoinArgs {
   float* sums;                     // [segs][rows][each]: replaced by the state that comes in (back: goes out)
-  const float *stay, *first;       // first: [rows][each] or null
+  const float* stay;               // [segs][rows]
+  const float* first;              // [rows][each] or null
   float* last;                     // or null
   int segs;
   int64_t rows, each;
@@ -261,9 +314,11 @@ __global__ __launch_bounds__(256) void linear_join(JoinArgs A) {
   for (int i = 0; i < A.segs; ++i) {
     const int64_t seg = A.back ? A.segs - 1 - i : i;
     float* at = A.sums + seg * all + id;
-    const float add = *at, f = A.stay[seg * A.rows + row];
+    const float add = *at;
+    const float e = A.stay[seg * A.rows + row];
+    const Decay f = decay_of(e);
     *at = s;
-    s = f == 0 ? add : fmaf(f, s, add);
+    s = e > 0 ? add : fmaf(f.factor, __builtin_amdgcn_ldexpf(s, f.shift), add);
   }
   if (A.last) A.last[id] = s;
 }
@@ -316,14 +371,6 @@ __device__ __forceinline__ Place place_of(const PairsArgs& p, const Sum& s, int 
   o.to = s.x.p && s.z.p ? min(BACK ? o.s0 + kSeg : o.r0 + rows, o.n) : 0;
   return o;
 }
-
-// Weights of 64 bits, for what is computed again: no operand or product of f32 values leaves their range, and an infinity times one of
-// them stays.
-__device__ __forceinline__ double power64(float rate, int n) {
-  const double e = (double)rate * n, k = floor(e);
-  return __builtin_amdgcn_ldexp((double)__builtin_amdgcn_exp2f((float)(e - k)), max((int)k, -1000));
-}
-__device__ __forceinline__ bool is_number(float x) { return fabsf(x) < INFINITY; }
 
 // A wavefront's rows [w0, w0 + 16) pair by pair in 64 bits, a lane a pair or one or two features of the result. What is not finite goes
 // where the states would carry it: a pair's X_e Z_d is a term of the state's entry (e, d), which row_e then multiplies. A row's own
@@ -516,7 +563,7 @@ struct Own {
     return !__any(bad != bad);
   }
 };
-// Weights of the pairs of row r and tile rows t0 + 16 (q / 4) + 4 g + q % 4; mine: r's mark.
+// Weights of the pairs of row r and tile rows t0 + 16 (q / 4) + 4 g + q % 4, -1 where masked; mine: r's mark.
 template <bool BACK>
 __device__ __forceinline__ void weights(float (&x)[8], const PairsArgs& p, const Place& o, float rate, int w0, int r, int t0, int mine,
                                         const int* since, int g) {
@@ -530,7 +577,7 @@ __device__ __forceinline__ void weights(float (&x)[8], const PairsArgs& p, const
       const int t = t0 + 16 * (q / 4) + 4 * g + q % 4, i = BACK ? t : r, j = BACK ? r : t;
       const int from = since[t - o.s0];
       const bool seen = (from != kNever) & (j <= i) & (j >= (BACK ? from : mine));
-      x[q] = seen ? x[q] : 0.0f;
+      x[q] = seen ? x[q] : -1.0f;
     }
   }
 }
@@ -594,7 +641,8 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
   };
   for (int gi = 0; gi < o.group; ++gi) {
     const float rate = scalar(p.rate[o.h0 + gi]);
-    const float coef = here ? p.by_state * weight_of(rate, BACK ? leaves(end, since, o.s0, r) : comes(since, o.s0, r)) : 0.0f;
+    const int by = here ? BACK ? leaves(end, since, o.s0, r) : comes(since, o.s0, r) : -1;
+    const float coef = by < 0 ? 0.0f : p.by_state * power(rate, by);
 #pragma unroll
     for (int c = 0; c < (ACROSS ? DZ : DN) / 32; ++c)
       if (c < mtiles) {
@@ -611,7 +659,7 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
       __builtin_amdgcn_sched_barrier(0);
       weights<BACK>(f, p, o, rate, w0, r, t0, mine, since, g);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) x[q] = f[q] == 0 ? 0.0f : x[q] * f[q];
+      for (int q = 0; q < 8; ++q) x[q] = f[q] < 0 ? 0.0f : x[q] * f[q];
       __builtin_amdgcn_sched_barrier(0);
       own.add(ring + buf * HALF, x, g, l);
     }
@@ -701,7 +749,7 @@ __global__ __launch_bounds__(256) void linear_steps(StepsArgs A) {
     vs[t][c] = t < n && (!doc || doc[t] >= 0) && c < a.Dv ? a.v.p[b * a.v.b + hk * a.v.h + t * a.v.t + c] : 0.0f;
   }
   __syncthreads();
-  const float decay = __builtin_amdgcn_exp2f(a.rate[h]);
+  const Decay decay = decay_of(a.rate[h]);
   for (int t = 0; t < n; ++t) {
     const bool fresh = doc && (doc[t] < 0 || (t > 0 && doc[t] != doc[t - 1]));
     const f32x4 v = *(const f32x4*)&vs[t][4 * cq];
@@ -712,7 +760,7 @@ __global__ __launch_bounds__(256) void linear_steps(StepsArgs A) {
       const float kd = ks[t][d], qd = qs[t][d];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        S[i][q] = fmaf(kd, v[q], fresh ? 0.0f : decay * S[i][q]);
+        S[i][q] = fmaf(kd, v[q], fresh ? 0.0f : __builtin_amdgcn_ldexpf(decay.factor * S[i][q], decay.shift));
         y[q] = fmaf(qd, rg + RG * i < a.D ? S[i][q] : 0.0f, y[q]);
       }
     }

@@ -134,10 +134,11 @@ def by_positions(a, decay, scale):
 
 
 @pytest.mark.parametrize('shape', [(2, 2, 1, 5, 32, 32), (1, 2, 2, 100, 64, 64), (1, 4, 2, 300, 64, 32), (1, 2, 1, 420, 15, 19), (1, 2, 1, 300, 128, 96)])
-@pytest.mark.parametrize('decay', [0.9])
+@pytest.mark.parametrize('decay', [0.9, 0.4, 0.003, 1e-30, 5e-324])
 @pytest.mark.parametrize('where', ['q', 'k', 'v', 'state', 'dy', 'dstate'])
 def test_linear_infinities_go_where_states_carry_them(shape, decay, where):
-    """Infinities and NaN in any operand are in the states, results and gradients that they are in by the definition."""
+    """Infinities and NaN in any operand are in the states, results and gradients that they are in by the definition. No
+    decay above 0 forgets them, however small its powers have become in 32 bits."""
     a = linear_inputs(*shape, 104, True)
     H, T = shape[1], shape[3]
     lam = [decay] + [0.9] * (H - 1)
