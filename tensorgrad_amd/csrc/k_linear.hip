@@ -19,8 +19,11 @@
 // whose k of step q is row 4 g + q, which is where the weights stand as they come out of the first product.
 //
 // What a row does not see has weight 0, and 0 times an infinity or NaN is NaN; a dot product may be infinite where no state is: rows
-// whose result is not finite are computed again pair by pair in 64 bits, from what they see alone.
+// whose result is not finite are computed again pair by pair in 64 bits, from what they see alone. So are all rows of a block whose
+// operands reach 2^16 (over the scale, if that is above 1) under a decay whose weights in a segment fall below 2^-100: what such a
+// weight leaves of them counts. What weights below 2^-126 leave of smaller ones, 2^-126 D 2^48 a pair at most, does not.
 #include <algorithm>
+#include <cmath>
 
 #include "kernels.h"
 #include "sequence.h"
@@ -340,6 +343,7 @@ struct PairsArgs {
   const float *states, *edge;      // [segs][B * H][D][Dv]; at the first segment (back: last) this one, or null
   int D, Dv;
   float by_pair, by_state;         // factors of both parts
+  float fast, limit;               // a decay's log2 below which operands are looked at, and from what size on they are large
   const float *rate, *any;         // any: an address with a feature (wide: 4), for rows that are absent
 };
 __device__ __forceinline__ const float* row_at(const Rows& x, int b, int head, int t) { return x.p + b * x.b + head * x.h + (int64_t)t * x.t; }
@@ -485,6 +489,14 @@ struct Own {
 #pragma unroll
     for (int c = 0; c < CZ; ++c) acc[c] = f32x4{};
   }
+  __device__ __forceinline__ float largest() const {
+    float top = 0;
+#pragma unroll
+    for (int c = 0; c < CN; ++c)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) top = fmaxf(top, fabsf(row[c][q]));
+    return top;
+  }
   // tile rows times own rows: x[q] of tile row 16 (q / 4) + 4 g + q % 4
   __device__ __forceinline__ void dots(const float* tile, float (&x)[8], int g, int l) const {
     f32x4 s[2] = {}, u[2];
@@ -593,7 +605,7 @@ struct Ring {
   float tile[2][Tile<DA>::FLOATS + Tile<DB>::FLOATS];
 };
 template <int DN, int DZ, int W, bool BACK, bool WIDE, bool ACROSS>
-__device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int unit, float* ring, int (&since)[kSeg]) {
+__device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int unit, float* ring, int (&since)[kSeg], int& large) {
   constexpr int FZ = Tile<DZ>::FLOATS, HALF = FZ + Tile<DN>::FLOATS, FM = ACROSS ? FZ : 0;   // M's tile: as wide as its rows are
   const Place o = place_of<BACK>(p, s, unit, 16 * W);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15;
@@ -627,33 +639,45 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
   fetch();
   Own<DN, DZ, WIDE> own;
   own.load(s.rows.p ? row_at(s.rows, o.b, o.head / p.keys, min(r, T - 1)) : p.any, s.rows.p ? s.n : 1, g);
+  if (tid == 0) large = 0;
   mark(p.m, o.b, o.s0, o.n, since);
   const Ends end = ends(since, o.s0, o.n);
   const int mine = r < T ? since[r - o.s0] : kNever;
   const bool here = mine != kNever;
   own.start(here && s.rows.p, s.n, g);
   int buf = 1;
-  auto arrive = [&]() {            // the next tile is there, in `buf`, and the one after it on its way
+  bool fast = false, looked = false;
+  float top = 0;                   // the largest operand under a fast decay, a thread a share of each tile
+  auto arrive = [&](int from, int to) {   // the next tile is there, [from, to) of `buf`, and the one after it on its way
     loads_done();
     __syncthreads();
     fetch();
     buf ^= 1;
+    if (!fast) return;
+#pragma unroll 1
+    for (int i = from + 4 * tid; i < to; i += 256 * W) {
+      const f32x4 u = *(const f32x4*)(ring + buf * HALF + i);
+      top = fmaxf(top, fmaxf(fmaxf(fabsf(u[0]), fabsf(u[1])), fmaxf(fabsf(u[2]), fabsf(u[3]))));
+    }
   };
   for (int gi = 0; gi < o.group; ++gi) {
     const float rate = scalar(p.rate[o.h0 + gi]);
+    fast = rate < p.fast;
+    looked |= fast;
+    if (fast) top = fmaxf(top, own.largest());
     const int by = here ? BACK ? leaves(end, since, o.s0, r) : comes(since, o.s0, r) : -1;
     const float coef = by < 0 ? 0.0f : p.by_state * power(rate, by);
 #pragma unroll
     for (int c = 0; c < (ACROSS ? DZ : DN) / 32; ++c)
       if (c < mtiles) {
-        arrive();
+        arrive(FM, FM + (ACROSS ? Tile<DN>::FLOATS : FZ));
         own.template state<ACROSS>(ring + buf * HALF + FM, c, coef, g, l);
       }
     int t0 = o.from;
     if (BACK)
-      for (; t0 < min(o.to, w0 - kTile + 1); t0 += kTile) arrive();
+      for (; t0 < min(o.to, w0 - kTile + 1); t0 += kTile) arrive(0, HALF);
     for (const int stop = BACK ? o.to : min(o.to, w0 + 16); t0 < stop; t0 += kTile) {
-      arrive();
+      arrive(0, HALF);
       float x[8], f[8];
       own.dots(ring + buf * HALF + FZ, x, g, l);
       __builtin_amdgcn_sched_barrier(0);
@@ -663,9 +687,14 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
       __builtin_amdgcn_sched_barrier(0);
       own.add(ring + buf * HALF, x, g, l);
     }
-    for (; t0 < o.to; t0 += kTile) arrive();
+    for (; t0 < o.to; t0 += kTile) arrive(0, HALF);
   }
-  const bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here && s.rows.p, s.nz, g);
+  bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here && s.rows.p, s.nz, g);
+  if (looked) {
+    if (top >= p.limit) large = 1;
+    __syncthreads();
+    fine = fine && !large;
+  }
   if (__builtin_expect(!fine, 0)) {
     loads_done();                  // the rows are written before they are written again
     plain_rows<BACK>(p, s, o, w0, since);
@@ -674,13 +703,13 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
 template <int DK, int DV, int W, bool BACK, bool WIDE>   // features of keys and of values, padded
 __global__ __launch_bounds__(64 * W, W == 8 || DK + DV <= 128 ? 4 : 2) void linear_tiles(PairsArgs p) {
   __shared__ __align__(16) Ring<DK, DV> ring;
-  __shared__ int since[kSeg];
+  __shared__ int since[kSeg], large;
   // both sums of a place run one after the other on one XCD (blocks go to the 8 XCDs in turn), whose L2 then has their tiles
   const int id = blockIdx.x / 8, unit = (id / p.sums) * 8 + blockIdx.x % 8;
   if (unit >= p.blocks * p.B * p.heads) return;
   const Sum& s = p.sum[id % p.sums];
-  if (s.across) walk_tiles<DV, DK, W, BACK, WIDE, true>(p, s, unit, ring.tile[0], since);
-  else walk_tiles<DK, DV, W, BACK, WIDE, false>(p, s, unit, ring.tile[0], since);
+  if (s.across) walk_tiles<DV, DK, W, BACK, WIDE, true>(p, s, unit, ring.tile[0], since, large);
+  else walk_tiles<DK, DV, W, BACK, WIDE, false>(p, s, unit, ring.tile[0], since, large);
 }
 
 // Sums of what each query head gave a key head's rows, in the heads' order. Bound by memory (38 MB in 10 us).
@@ -871,6 +900,8 @@ void pairs(PairsArgs p, const LinearDesc& a, const float* at, const float* edge,
   p.Dv = a.Dv;
   p.by_pair = a.scale;
   p.by_state = BACK ? 1.0f : a.scale;
+  p.fast = (-100 - std::min(0.0f, std::log2(a.scale))) / kSeg;
+  p.limit = 0x1p16f / std::max(1.0f, a.scale);
   p.rate = a.rate;
   p.any = a.q.p;
   bool wide = a.D % 4 == 0 && a.Dv % 4 == 0 && wide_rows(a.q) && (((uintptr_t)at | (uintptr_t)edge) & 15) == 0;

@@ -745,7 +745,8 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, decay: Sequence[float], sc
     is what the next positions start from: a prompt is read in one call, or in pieces, and answered with T = 1. `lengths` i32 [B]:
     only the first lengths[b] positions are there (clamped to 0..T), y is 0 behind them and the last state that after them.
     `documents` i32 [B, T]: the state starts from zeros where an id differs from the one before (position 0 goes on from `state`);
-    negative ids are padding, where y and the state are 0. What is not there has no influence, whatever its values."""
+    negative ids are padding, where y and the state are 0. What is not there has no influence, whatever its values; infinities and
+    NaN that are there stay in the state, whatever the decay."""
     f = _linear_fields('linearAttention', q, k, v, decay, scale, state, documents, lengths)
     B, H, T, D = q.shape
     g = current_graph()

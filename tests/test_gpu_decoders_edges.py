@@ -166,3 +166,19 @@ def test_linear_products_that_pass_f32_on_the_way(decay):
     for n, e in (('q', 70), ('k', 60), ('v', -40), ('dy', -50), ('state', 20), ('dstate', 20)):
         a[n] *= f32(2.0 ** e)
     check_linear(a, [decay] * 2)
+
+
+@pytest.mark.parametrize('shape', [(1, 2, 1, 8, 32, 32), (1, 2, 2, 100, 64, 64), (1, 4, 2, 300, 64, 32), (1, 2, 1, 420, 15, 19)])
+@pytest.mark.parametrize('where', ['q', 'k', 'v', 'state', 'dy', 'dstate', 'all states'])
+def test_linear_large_values_outlast_small_weights(shape, where):
+    """2^116 times a power of the decay below 2^-126 still counts."""
+    a = linear_inputs(*shape, 105, True)
+    T = shape[3]
+    lam = [0.4] + [0.45] * (shape[1] - 1)
+    if where == 'all states':
+        a['state'] *= f32(2.0 ** 116)
+    elif where in ('state', 'dstate'):
+        a[where][0, 0, 1] *= f32(2.0 ** 116)
+    else:
+        a[where][0, 0, T - 2 if where in ('q', 'dy') else 1] *= f32(2.0 ** 116)
+    check_linear(a, lam, what=where)
