@@ -94,7 +94,9 @@ __device__ __forceinline__ double weight(const Row& r, float x) {
 }
 __device__ __forceinline__ u64 whole(double w) { return (u64)rint(w); }
 // per_bin or per1 times how far a logit is from the largest. None where it is the largest: the factor may be infinite, or both logits.
-__device__ __forceinline__ float distance(const Row& r, float x, float per) { return x == r.top ? 0.0f : fmaf(-x, r.shrink, r.shrunk) * per; }
+__device__ __forceinline__ float distance(const Row& r, float x, float per) {
+  return x == r.top ? 0.0f : fmaf(-x, r.shrink, r.shrunk) * per;
+}
 // A token's bin, rising with the distance to the top in equal steps; kBins: so far that its weight is 0, or not there.
 __device__ __forceinline__ int bin_of(const Row& r, float x) {
   const float b = distance(r, x, r.per_bin);
@@ -632,14 +634,14 @@ __device__ __forceinline__ u64 goal_of(const Row& r, u64 all) { return min((u64)
 
 // ---- a block a row -------------------------------------------------------------------------------------
 
-// At most LIST tokens, all of them sorted by a single wavefront: no bins. Bound by latency: the sort's dependent steps (64 rows of 65
-// tokens 8 us; 512 rows of 300, sorted by 256 threads, 16 where sample_one takes 14).
-template <int THREADS, int LIST>
-__global__ __launch_bounds__(THREADS) void sample_short(SampleDesc s) {
-  constexpr int N = LIST / THREADS;
-  __shared__ Work<LIST> w;
+// At most 256 tokens, all of them sorted by a single wavefront: no bins. Bound by latency: the sort's dependent steps (64 rows of 65
+// tokens 8 us).
+constexpr int kShort = 256;
+__global__ __launch_bounds__(64) void sample_short(SampleDesc s) {
+  constexpr int THREADS = 64, N = kShort / THREADS;
+  __shared__ Work<kShort> w;
   const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x;
   const float* x = s.logits + row * s.V;
   float v[N];
 #pragma unroll
@@ -656,23 +658,19 @@ __global__ __launch_bounds__(THREADS) void sample_short(SampleDesc s) {
   }
   const Row r = row_of(s, row, top);
   bool ok;
-  const u64 bound = r.by_count || r.by_mass ? bound_of_list<THREADS, LIST>(r, {0, kBins - 1, 0, 0, false}, s.V, 0, 0, w, ok, [](int, u64) {}) : kAll;
+  const u64 bound =
+      r.by_count || r.by_mass ? bound_of_list<THREADS, kShort>(r, {0, kBins - 1, 0, 0, false}, s.V, 0, 0, w, ok, [](int, u64) {}) : kAll;
   u64 mine = 0;
 #pragma unroll
   for (int e = 0; e < N; ++e) if (e * THREADS + tid < s.V) mine += kept_weight(r, bound, e * THREADS + tid, v[e]);
-  mine = wave_sum(mine);
-  __syncthreads();
-  if (lane == 0) w.sums[1][wave] = mine;
-  __syncthreads();
-  u64 all = 0;
-#pragma unroll
-  for (int k = 0; k < THREADS / 64; ++k) all += w.sums[1][k];
-  choose<THREADS>(r, bound, 0, s.V, goal_of(r, all), w, s.token + row);
+  choose<THREADS>(r, bound, 0, s.V, goal_of(r, wave_sum(mine)), w, s.token + row);
 }
 
-// 1024 threads a row, so that 256 rows fill the card, or 256. Bound by the weights in 64 bits, some 60 instructions of 4 to 8 cycles a token,
-// which every token up to a border needs once (256 rows of 50001, 51 MB: no limit 38 us, top-k of 50 34, top_p 0.9 53; limits of
-// their own in each row 54, 0.95 TB/s).
+// 1024 threads a row, so that 256 rows fill the card, or 256. Bound by the weights in 64 bits, some 60 instructions of 4 to 8 cycles
+// a token, which every token up to a border needs once (256 rows of 50001, 51 MB: no limit 38 us, top-k of 50 34, top_p 0.9 53;
+// limits of their own in each row 54, 0.95 TB/s). More than 2048 tokens in the border's bins send a row to bound_by_walks: 256 rows of
+// 50001 equal logits 434 us; several blocks a row, 4 rows of 128000 rounded to quarters 312 (28 unrounded), 32 of 200000 as good as
+// flat 475.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void sample_one(SampleDesc s) {
   constexpr int W = THREADS / 64;
@@ -914,14 +912,15 @@ void sample(const SampleDesc& s, void* work, hipStream_t st) {
   if (p.parts == 1) {
     // 256 threads where a row is short, or more rows than compute units are not long: top-k of 50 of 512 rows of 4000 tokens 18 us, by
     // 1024 threads 29, of 300 rows of 8000 22 and 28; of 4 rows of 8000 19 and 14, of 512 of 20000 41 and 38
-    if (s.V <= 256) klaunch(sample_short<64, 256>, rows, dim3(64), 0, st, s);
+    if (s.V <= kShort) klaunch(sample_short, rows, dim3(64), 0, st, s);
     else if (s.V <= 4096 || (s.rows > 256 && s.V <= 16384)) klaunch(sample_one<256>, rows, dim3(256), 0, st, s);
     else klaunch(sample_one<1024>, rows, dim3(1024), 0, st, s);
     return;
   }
   char* w = (char*)work;
   const PartArgs a{s, p.parts, p.each, (RowSpace*)w, (float*)(w + p.tops), (Sums*)(w + p.sums)};
-  const bool limits = s.temperature || s.min_p || !(s.temperature1 > 0) || s.top_k || s.top_p || (s.top_k1 > 0 && s.top_k1 < s.V) || s.top_p1 < 1;
+  const bool limits = s.temperature || s.min_p || s.top_k || s.top_p || !(s.temperature1 > 0) || (s.top_k1 > 0 && s.top_k1 < s.V) ||
+                      s.top_p1 < 1;
   klaunch(sample_tops, grid, block, 0, st, a);
   if (limits) klaunch(sample_bins, grid, block, 0, st, a);
   klaunch(sample_list, grid, block, 0, st, a);
