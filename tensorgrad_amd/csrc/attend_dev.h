@@ -17,6 +17,7 @@
 // gradients of head size 32 without documents (4 %); those of head size 128 took half as long again.
 #pragma once
 #include "kernels.h"
+#include "lds_dev.h"
 #include "sequence.h"
 
 namespace tgk {
@@ -201,10 +202,6 @@ __device__ __forceinline__ void frags_to_lds(const char* src, uint32_t lds, uint
 #pragma unroll
   for (int f = 0; f < N / 8; ++f) frag_to_lds(src + f * 8192, lds + f * 8192, lane16);
   if (N % 8 && w < N % 8) frag_to_lds(src + N / 8 * 8192, lds + N / 8 * 8192, lane16);
-}
-__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-__device__ __forceinline__ uint32_t lds_address(const void* p) {
-  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
 
 __device__ __forceinline__ float finite_abs(float x) {
@@ -426,9 +423,10 @@ __device__ __forceinline__ TileInfo side_info(const float* side, int x) {
   auto u = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
   return {__int_as_float(u(p[0])), __int_as_float(u(p[1])), u(p[2]), u(p[3]), u(p[4]), u(p[5]), u(p[6]), 0};
 }
-// Does a query with these bounds see key z of the tile at j0 (below: and from `from` on, or one that stays). Without branches: with the document read behind the other
-// conditions, `if (!seen) x[q] = 0` comes out of the compiler wrong (right in its IR; in the machine code the block for keys of
-// other documents is empty, their 0 written before a copy of the whole vector undoes it), and hidden keys keep their values.
+// Does a query with these bounds see key z of the tile at j0 (below: and from `from` on, or one that stays). Without branches: with
+// the document read behind the other conditions, `if (!seen) x[q] = 0` comes out of the compiler wrong (right in its IR; in the
+// machine code the block for keys of other documents is empty, their 0 written before a copy of the whole vector undoes it), and
+// hidden keys keep their values.
 __device__ __forceinline__ bool key_seen(const Sight& s, const float* side, int j0, int z, int below, int from, int doc) {
   const int id = __float_as_int(side[KS_DOC * kTile + z]);
   return (j0 + z < below) & ((j0 + z >= from) | (j0 + z < s.stay)) & (!s.doc | ((doc >= 0) & (id == doc)));

@@ -26,6 +26,7 @@
 #include <cmath>
 
 #include "kernels.h"
+#include "lds_dev.h"
 #include "sequence.h"
 
 namespace tgk {
@@ -173,10 +174,7 @@ __device__ __forceinline__ void tile_to_lds(const float* x, int64_t stride, int 
     }
   }
 }
-__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-__device__ __forceinline__ uint32_t lds_address(const void* p) {
-  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
-}
+
 // ---- sums over a segment -----------------------------------------------------------------------------
 //
 // A block sums k v^T of a segment, four wavefronts a quarter of the product each, over tiles of 32 positions of which the next one
@@ -596,10 +594,10 @@ __device__ __forceinline__ void weights(float (&x)[8], const PairsArgs& p, const
 
 // W wavefronts of 16 rows. Bound by the f32 matrix instructions: 64 heads of 4096 positions, 128 x 128 features, keep them busy for
 // 66 % of the cycles (y or dq 217 us, dk and dv 427; 19 GFLOP a result with the masked halves of tiles); what is lost is wavefronts
-// of early rows, which wait for the tiles of late ones. LDS has no conflicts. The tiles of M, then those of the pairs, one after another; the next one travels to the other half of LDS
-// while this one is multiplied, so that a tile costs one barrier. A wavefront walks the tiles that it has nothing to do with in
-// loops of their own: with a branch around the work the compiler copied all 32 registers of results for every tile, and had none
-// left for a second block on the CU.
+// of early rows, which wait for the tiles of late ones. LDS has no conflicts. The tiles of M, then those of the pairs, one after
+// another; the next one travels to the other half of LDS while this one is multiplied, so that a tile costs one barrier. A wavefront
+// walks the tiles that it has nothing to do with in loops of their own: with a branch around the work the compiler copied all 32
+// registers of results for every tile, and had none left for a second block on the CU.
 template <int DA, int DB>
 struct Ring {
   float tile[2][Tile<DA>::FLOATS + Tile<DB>::FLOATS];
@@ -831,8 +829,9 @@ inline int padded(const LinearDesc& a) { return (std::max(a.D, a.Dv) + 31) / 32 
 inline int64_t states_bytes(const LinearDesc& a) { return ((int64_t)segments(a) * a.B * a.H * a.D * a.Dv * 4 + 255) / 256 * 256; }
 inline int64_t stay_bytes(const LinearDesc& a) { return ((int64_t)segments(a) * a.B * a.H * 4 + 255) / 256 * 256; }
 
-// f(keys' features, values' features), padded, as constants. Values of another size than keys have kernels of their own (8 heads of
-// 128 and 16 features, 14 sequences of 617: forward @@); 96 features go with 96, or count as 128.
+// f(keys' features, values' features), padded, as constants. Values of another size than keys have kernels of their own (14 sequences
+// of 617, 8 heads of 128 and 16 features: forward 64 us, a training step 190; padded to the larger size 114 and 341; of 64 and 32: 42
+// and 127 instead of 54 and 161); 96 features go with 96, or count as 128.
 template <class F>
 void by_sizes(const LinearDesc& a, F f) {
   int k = (a.D + 31) / 32 * 32, v = (a.Dv + 31) / 32 * 32;
@@ -944,8 +943,9 @@ void linear(const LinearDesc& a, void* work, hipStream_t st) {
 }
 
 // Key heads that several query heads share: a block takes all of those in turn, or one where all of them would leave the card half
-// empty, and what they give is summed after (3 sequences of 1777, 8 heads on 2 of 96 and
-// 80 features: 96 us in turn, 64 + 11 apart).
+// empty, and what they give is summed after (3 sequences of 1777, 8 heads on 2 of 96 and 80 features: 96 us in turn, 64 + 11 apart).
+// Training steps, apart and in turn: 336 blocks of 64 rows in turn 197 us and 218, 448 of them 221 and 223; 512, of 64 features, 148 and
+// 142, of 128 183 and 169; 1024 260 and 239. Seven query heads a key head lose by turns longer (540 blocks 251 and 295).
 static bool split_heads(const LinearGradDesc& g) {
   const LinearDesc& a = g.a;
   const int sums = (g.dk.p != nullptr) + (g.dv.p != nullptr);
