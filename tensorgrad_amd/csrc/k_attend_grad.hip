@@ -93,7 +93,8 @@ __device__ __forceinline__ void plain_keys(const GradArgs& A, const Sight& s, in
       float p = 0, ds = 0;
       if (r < r1) {
         const float* side = A.qside + ((int64_t)slab * A.qtiles + r / kTile) * (kSide * kTile) + r % kTile;
-        if (j < __float_as_int(side[QS_BELOW * kTile]) && (j >= sees_from(s, __float_as_int(side[QS_POS * kTile])) || j < s.stay) && (!s.doc || (doc >= 0 && __float_as_int(side[QS_DOC * kTile]) == doc))) {
+        if (j < __float_as_int(side[QS_BELOW * kTile]) && (j >= sees_from(s, __float_as_int(side[QS_POS * kTile])) || j < s.stay) &&
+            (!s.doc || (doc >= 0 && __float_as_int(side[QS_DOC * kTile]) == doc))) {
           const PlainPair z = plain_score(a, plain_dot(row(a.q, r), k, a.D), side[QS_SLOPE * kTile], __float_as_int(side[QS_POS * kTile]) - j);
           const float share = side[QS_SHARE * kTile], w = __builtin_amdgcn_exp2f(z.score - side[QS_TOP * kTile]);
           p = w * share;
@@ -250,7 +251,8 @@ __global__ __launch_bounds__(512, DP <= 64 ? 4 : 2) void attend_grad_kv(GradArgs
         const f32x4 pos = *(const f32x4*)(side + QS_POS * kTile + at);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool ok = (j < __float_as_int(below[e])) & ((j >= sees_from(s, __float_as_int(pos[e]))) | (j < s.stay)) & (!s.doc | ((doc >= 0) & (__float_as_int(rdoc[e]) == doc)));
+          const bool ok = (j < __float_as_int(below[e])) & ((j >= sees_from(s, __float_as_int(pos[e]))) | (j < s.stay)) &
+                          (!s.doc | ((doc >= 0) & (__float_as_int(rdoc[e]) == doc)));
           x[4 * q4 + e] = ok ? x[4 * q4 + e] : 0.0f;
           y[4 * q4 + e] = ok ? y[4 * q4 + e] : 0.0f;
         }
@@ -514,7 +516,9 @@ GradPlan grad_plan(const AttendGradDesc& g) {
   const int64_t have = (int64_t)p.slabs * p.blocks;
   // About 1024 blocks, two to four rounds of the card: 512 leave it to the longest (4096 causal rows of 4 slabs, head size 128:
   // 832 us and 21 to join, instead of 677 and 31), 2048 write and join twice the parts (624 and 58).
-  // Of a window's few rows parts of 3 tiles: 19 slabs of 7 heads, 81 positions, head size 128, a training step 87 us instead of 98.
+  // Of a window's few rows parts of 3 tiles; training steps by those and by 8: 19 slabs of 7 heads, 81 positions, head size 128 (38
+  // parts of 8) 85 us and 96, 16 of 4 heads, 300 x 64 (192) 80 and 88, 8 of 2, 700 x 128 (240) 112 and 111, 8 of 1, 1000 x 64 (256) 74
+  // and 80; from there on those of 8, but for the least work: 8 of 4, 600 x 96 (360) 155 and 123, 16 of 4, 512 x 64 (512) 114 and 107.
   p.least = a.window && have * (p.qtiles / 8) < 256 ? 3 : 8;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((1024 + have - 1) / have, p.qtiles / p.least));
   // dq in parts only where its blocks leave compute units idle: 224 of them (32 slabs of 777 rows, head size 96) take 55 us, in

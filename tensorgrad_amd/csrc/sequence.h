@@ -1,5 +1,6 @@
 // Host-side launch wrappers of the sequence operators: masked attention (k_attend.hip), rotary positions of several axes
-// and the gated linear recurrence (k_sequence.hip), linear attention (k_linear.hip), and of the choice of a token (k_sample.hip). Values are f32, indices i32; strides count elements.
+// and the gated linear recurrence (k_sequence.hip), linear attention (k_linear.hip), and of the choice of a token
+// (k_sample.hip). Values are f32, indices i32; strides count elements.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <cstdint>

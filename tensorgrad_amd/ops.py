@@ -619,8 +619,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, causal: bool = True, scale: Optio
     `lengths` i32 [B]: only the first lengths[b] keys are there (clamped to 0..Tk; without it all Tk). The queries are the
     last Tq of those positions, so one new token against a filled cache is Tq = 1. `causal` hides keys after p, except those
     below `prefix` i32 [B], which every query sees. `window` leaves a query the last `window` keys up to its own, p - window < j,
-    beside the first `sinks` positions (not with documents) and those of a prefix; both need the causal mask. `documents` i32 [B, Tk]: a query sees the keys of its own document (that
-    at its position); negative ids are padding, which sees and is seen by nothing. A query that sees no key (or, where
+    beside the first `sinks` positions (not with documents) and those of a prefix; both need the causal mask. `documents` i32
+    [B, Tk]: a query sees the keys of its own document (that at its position); negative ids are padding, which sees and is seen by nothing. A query that sees no key (or, where
     positions matter, lies before position 0) gives zeros and takes and gives no gradient. What a mask hides has no
     influence, whatever its values (infinities and NaN included)."""
     f = _attention_fields('attention', q, k, v, causal, scale, softcap, slopes, documents, prefix, lengths, window, sinks)
