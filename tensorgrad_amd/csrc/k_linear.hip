@@ -390,13 +390,13 @@ __device__ __forceinline__ void plain_rows(const PairsArgs& p, const Sum& s, con
       return from != kNever && j <= i && j >= (BACK ? from : mine);
     };
     const int by = BACK ? leaves(ends(since, o.s0, o.n), since, o.s0, r) : comes(since, o.s0, r);
-    const int heads = (o.M && by >= 0) || o.from < o.to ? o.group : 0;   // none: it sees nothing at all
+    const bool some = (o.M && by >= 0) || o.from < o.to;   // else it sees nothing at all
     double acc[2] = {0, 0};
     bool nan = false;              // then every feature is
 #pragma unroll 1
-    for (int e = 0; e < s.n && heads > 0; ++e) nan |= row[e] != row[e];
+    for (int e = 0; e < s.n; ++e) nan |= some && row[e] != row[e];
 #pragma unroll 1
-    for (int gi = 0; gi < heads; ++gi) {
+    for (int gi = 0; gi < (some && !nan ? o.group : 0); ++gi) {
       const int h = o.h0 + gi, hx = BACK ? h : h / p.share;
       const float rate = p.rate[h];
       const double coef = by < 0 ? 0.0 : p.by_state * power64(rate, by);
@@ -410,7 +410,7 @@ __device__ __forceinline__ void plain_rows(const PairsArgs& p, const Sum& s, con
           const int d = 64 * a + lane;
           if (d >= s.nz) continue;
           double entry = state(e, d);
-          if (!is_number(row[e]) && !nan)
+          if (!is_number(row[e]))
 #pragma unroll 1
             for (int t = o.from; t < o.to; ++t)
               if (seen(t)) entry += weight(t) * row_at(s.x, o.b, hx, t)[e] * row_at(s.z, o.b, hx, t)[d];

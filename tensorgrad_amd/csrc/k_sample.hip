@@ -629,8 +629,10 @@ __device__ __forceinline__ void choose(const Row& r, u64 bound, int from, int to
     goal -= all;
   }
 }
-// Passed: sum > u all, as whole numbers; u in [0, 1) leaves the last token's sum, all, to pass.
-__device__ __forceinline__ u64 goal_of(const Row& r, u64 all) { return min((u64)fmax(r.u * (double)all, 0.0), all - 1); }
+// Passed: sum > u all, as whole numbers; at most all - 1, which the last token's sum passes. Clamped before it is a whole number, too.
+__device__ __forceinline__ u64 goal_of(const Row& r, u64 all) {
+  return min((u64)fmin(fmax(r.u * (double)all, 0.0), (double)all), all - 1);
+}
 
 // ---- a block a row -------------------------------------------------------------------------------------
 

@@ -787,7 +787,7 @@ def sample(logits: Tensor, u: Tensor, temperature=1.0, top_k=None, top_p=None, m
     Tokens are ordered by falling logit, equal ones by rising index, and weigh exp((logit - largest) / temperature). Each limit
     keeps a first part of that order: `top_k` tokens; of those the fewest whose weights reach `top_p` of their sum; and of those
     the ones of at least `min_p` times the largest weight. The token is the first kept one, in the vocabulary's order, where the
-    kept weights' running sum passes u of them all.
+    kept weights' running sum passes u of them all; a u below 0 (or NaN) counts as 0, one from 1 on takes the last.
 
     A limit is one number for all rows, or a tensor of u's shape with a number for each (f32, `top_k` i32); None, a top_k below 1
     or a top_p from 1 on do not limit, and a temperature of 0 takes the largest logit. In tensors, a temperature that is not above 0

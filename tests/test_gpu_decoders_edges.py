@@ -55,6 +55,13 @@ def test_sample_limits_out_of_range_keep_the_first_or_all(V):
     check_sample(logits, f32(r.uniform(0.3, 1, 24)), min_p=m)
 
 
+@pytest.mark.parametrize('V', FORMS)
+def test_sample_random_numbers_out_of_range_take_an_end(V):
+    r = rng(V, 108)
+    u = f32([0, 1, 2, 3.9, 4.1, 1e30, np.inf, -0.5, -1e30, -np.inf, np.nan, 0.5])
+    check_sample(f32(r.standard_normal((len(u), V))), u, top_k=7)
+
+
 def mixed_rows(rows, V, seed):
     """Rows without a limit, with each limit, all equal, rounded, flat, greedy, empty, masked, side by side."""
     r = rng(rows, V, seed)
