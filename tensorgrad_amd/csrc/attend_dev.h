@@ -192,16 +192,12 @@ __device__ __forceinline__ bool all_seen(const Sight& s, const Span& q, const Ti
 }
 
 // N fragments from memory straight into LDS (lane l's 16 bytes land at base + 16 l) by eight wavefronts, wavefront w's at src
-// and lds + 1024 w. In inline assembly, so that the compiler does not drain every load before the next LDS read; the kernels
-// wait (vmcnt) and meet (barrier) themselves.
-__device__ __forceinline__ void frag_to_lds(const char* src, uint32_t lds, uint32_t lane16) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane16), "s"(src), "{m0}"(lds));
-}
+// and lds + 1024 w. The kernels wait (vmcnt) and meet (barrier) themselves.
 template <int N>
 __device__ __forceinline__ void frags_to_lds(const char* src, uint32_t lds, uint32_t lane16, int w) {
 #pragma unroll
-  for (int f = 0; f < N / 8; ++f) frag_to_lds(src + f * 8192, lds + f * 8192, lane16);
-  if (N % 8 && w < N % 8) frag_to_lds(src + N / 8 * 8192, lds + N / 8 * 8192, lane16);
+  for (int f = 0; f < N / 8; ++f) load16_to_lds(src + f * 8192, lane16, lds + f * 8192);
+  if (N % 8 && w < N % 8) load16_to_lds(src + N / 8 * 8192, lane16, lds + N / 8 * 8192);
 }
 
 __device__ __forceinline__ float finite_abs(float x) {

@@ -27,6 +27,23 @@ struct GemmDesc {
   float* C; int64_t sCz0, sCz1, sCm, sCn;
 };
 
+// One load of a wavefront from memory straight into LDS: lane l's 16 bytes at base + offset go to lds + 16 l, or 4 bytes to lds + 4 l.
+// Issued from inline assembly, so that the compiler does not treat it as an LDS write of unknown extent: for such writes it drains
+// every outstanding load before the next LDS read. The five wait states stand between a vector instruction that wrote the base (or
+// M0) and the load that reads it, v_readfirstlane, or v_readlane where a scalar register had been spilled to lanes: loads do not wait
+// for those by themselves, and the compiler adds none inside assembly. With one wait state (what a scalar write of M0 needs) a base that
+// came back from a spill right before the load was read half old, and the load faulted.
+__device__ __forceinline__ void load16_to_lds(const void* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "{m0}"(lds));
+}
+__device__ __forceinline__ void load4_to_lds(const void* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "{m0}"(lds));
+}
+// The same with a 64-bit address in each lane.
+__device__ __forceinline__ void load4_to_lds(const float* at, uint32_t lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" ::"v"(at), "{m0}"(lds));
+}
+
 namespace gd {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -135,22 +152,17 @@ struct DTile {
 
   // Issue this thread's chunks of one stage: global base `gb` (tile origin of the stage,
   // wave-uniform, in SGPRs) plus the 32-bit per-lane offsets; LDS byte address `lds` of the
-  // stage's slot and the wave index `wave`, both wave-uniform, so M0 is scalar arithmetic.
-  // Each global_load_lds_dwordx4 moves lane l's 16 bytes to M0 + 16 l (a dword load: 4
-  // bytes to M0 + 4 l). It is issued from inline assembly so the compiler does not treat it
-  // as an LDS write of unknown extent: for such writes it drains every outstanding load
-  // before the next LDS read, which would expose the full load latency at every pipeline
-  // stage. The kernel orders LDS reads itself (explicit vmcnt waits and barriers). One wait
-  // state separates the M0 write from the load.
+  // stage's slot and the wave index `wave`, both wave-uniform.
+  // The kernel orders LDS reads itself (explicit vmcnt waits and barriers).
   __device__ __forceinline__ static void dma(const float* gb, const uint32_t* off, uint32_t lds, int wave) {
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
       if (DW) {
         const uint32_t m0v = lds + (uint32_t)((e * (NT / 64) + wave) * 64 * 4);
-        asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off[e]), "s"(gb), "{m0}"(m0v));
+        load4_to_lds(gb, off[e], m0v);
       } else {
         const uint32_t m0v = lds + (uint32_t)((e * (NT / 64) + wave) * kLdsBlock * 4);
-        asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[e]), "s"(gb), "{m0}"(m0v));
+        load16_to_lds(gb, off[e], m0v);
       }
     }
   }

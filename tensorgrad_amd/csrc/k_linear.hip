@@ -152,8 +152,7 @@ struct Tile {
 
 // Rows [r0, r0 + 32) of x from memory straight into LDS, by WAVES wavefronts: 16 bytes a lane, or (not WIDE: rows that are not whole
 // 16-byte pieces) 4, with addresses of 64 bits. Nothing is masked: rows past the last and features past the n-th are others that are
-// there. In inline assembly, so that the compiler does not drain every load before the next LDS read; the kernels wait (vmcnt) and
-// meet (barrier) themselves.
+// there. The kernels wait (vmcnt) and meet (barrier) themselves.
 template <int DP, int WAVES, bool WIDE>
 __device__ __forceinline__ void tile_to_lds(const float* x, int64_t stride, int r0, int rows, int n, uint32_t lds, int w) {
   constexpr int PIECES = Tile<DP>::PIECES, PITCH = Tile<DP>::PITCH, N = kTile * PITCH / (WIDE ? 256 : 64);
@@ -166,11 +165,11 @@ __device__ __forceinline__ void tile_to_lds(const float* x, int64_t stride, int 
     if constexpr (WIDE) {
       const int r = k * (64 / PIECES) + lane / PIECES, c = (lane % PIECES) ^ Tile<DP>::swizzle(r);
       const uint32_t off = (uint32_t)min(r, left) * (uint32_t)(4 * stride) + (4 * c < n ? 16 * c : 0);
-      asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds + k * 1024));
+      load16_to_lds(base, off, lds + k * 1024);
     } else {
       const int e = k * 64 + lane, r = e / PITCH, c = (e % PITCH / 4) ^ Tile<DP>::swizzle(r);
       const float* at = base + min(r, left) * stride + min(4 * c + e % 4, n - 1);
-      asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(at), "{m0}"(lds + k * 256));
+      load4_to_lds(at, lds + k * 256);
     }
   }
 }

@@ -1,6 +1,6 @@
 // Loads from memory straight into LDS: their addresses and their wait. Shared by the attention kernels and k_linear.hip.
 #pragma once
-#include <cstdint>
+#include "gemm_dev.h"   // the loads
 
 namespace tgk {
 
