@@ -19,9 +19,9 @@
 // whose k of step q is row 4 g + q, which is where the weights stand as they come out of the first product.
 //
 // What a row does not see has weight 0, and 0 times an infinity or NaN is NaN; a dot product may be infinite where no state is: rows
-// whose result is not finite are computed again pair by pair in 64 bits, from what they see alone. So are all rows of a block whose
-// operands reach 2^16 (over the scale, if that is above 1) under a decay whose weights in a segment fall below 2^-100: what such a
-// weight leaves of them counts. What weights below 2^-126 leave of smaller ones, 2^-126 D 2^48 a pair at most, does not.
+// whose result is not finite are computed again pair by pair in 64 bits, from what they see alone. So are rows of
+// which weights below f32's range, 2^-126, may lose something that counts: under a decay whose weights in a segment fall below 2^-100,
+// where 2^-126 times the largest products that a block's operands allow is above 2^-60 and above 2^-30 of a result of theirs.
 #include <algorithm>
 #include <cmath>
 
@@ -340,7 +340,7 @@ struct PairsArgs {
   const float *states, *edge;      // [segs][B * H][D][Dv]; at the first segment (back: last) this one, or null
   int D, Dv;
   float by_pair, by_state;         // factors of both parts
-  float fast, limit;               // a decay's log2 below which operands are looked at, and from what size on they are large
+  float fast, large;               // a decay's log2 below which operands are looked at; the size below which they lose nothing that counts
   const float *rate, *any;         // any: an address with a feature (wide: 4), for rows that are absent
 };
 __device__ __forceinline__ const float* row_at(const Rows& x, int b, int head, int t) { return x.p + b * x.b + head * x.h + (int64_t)t * x.t; }
@@ -486,6 +486,7 @@ struct Own {
 #pragma unroll
     for (int c = 0; c < CZ; ++c) acc[c] = f32x4{};
   }
+  // Of a lane's part of a row's features, and of its results.
   __device__ __forceinline__ float largest() const {
     float top = 0;
 #pragma unroll
@@ -493,6 +494,14 @@ struct Own {
 #pragma unroll
       for (int q = 0; q < 4; ++q) top = fmaxf(top, fabsf(row[c][q]));
     return top;
+  }
+  __device__ __forceinline__ float smallest(int n, int g) const {
+    float least = INFINITY;
+#pragma unroll
+    for (int c = 0; c < CZ; ++c)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) if (16 * c + 4 * g + q < n) least = fminf(least, fabsf(acc[c][q]));
+    return least;
   }
   // tile rows times own rows: x[q] of tile row 16 (q / 4) + 4 g + q % 4
   __device__ __forceinline__ void dots(const float* tile, float (&x)[8], int g, int l) const {
@@ -601,8 +610,15 @@ template <int DA, int DB>
 struct Ring {
   float tile[2][Tile<DA>::FLOATS + Tile<DB>::FLOATS];
 };
-template <int DN, int DZ, int W, bool BACK, bool WIDE, bool ACROSS>
-__device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int unit, float* ring, int (&since)[kSeg], int& large) {
+// Where a wavefront has a size from `large` on: the larger of `most` (a size's bits, in LDS) and its sizes.
+__device__ __forceinline__ void join_max(uint32_t& most, float size, float large) {
+  if (!__any(size >= large)) return;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) size = fmaxf(size, __shfl_xor(size, o));
+  if ((threadIdx.x & 63) == 0) atomicMax(&most, __float_as_uint(size));
+}
+template <int DN, int DZ, int W, bool BACK, bool WIDE, bool LOOK, bool ACROSS>
+__device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int unit, float* ring, int (&since)[kSeg], uint32_t (&most)[2]) {
   constexpr int FZ = Tile<DZ>::FLOATS, HALF = FZ + Tile<DN>::FLOATS, FM = ACROSS ? FZ : 0;   // M's tile: as wide as its rows are
   const Place o = place_of<BACK>(p, s, unit, 16 * W);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15;
@@ -636,22 +652,23 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
   fetch();
   Own<DN, DZ, WIDE> own;
   own.load(s.rows.p ? row_at(s.rows, o.b, o.head / p.keys, min(r, T - 1)) : p.any, s.rows.p ? s.n : 1, g);
-  if (tid == 0) large = 0;
+  if (LOOK && tid < 2) most[tid] = 0;
   mark(p.m, o.b, o.s0, o.n, since);
   const Ends end = ends(since, o.s0, o.n);
   const int mine = r < T ? since[r - o.s0] : kNever;
   const bool here = mine != kNever;
   own.start(here && s.rows.p, s.n, g);
+  if (LOOK) join_max(most[1], own.largest(), p.large);
   int buf = 1;
-  bool fast = false, looked = false;
+  bool fast = false, looked = false;   // LOOK: this head's decay is, one was
   float top = 0;                   // the largest operand under a fast decay, a thread a share of each tile
   auto arrive = [&](int from, int to) {   // the next tile is there, [from, to) of `buf`, and the one after it on its way
     loads_done();
     __syncthreads();
     fetch();
     buf ^= 1;
-    if (!fast) return;
-#pragma unroll 1
+    if (!LOOK || !fast) return;
+#pragma unroll 2
     for (int i = from + 4 * tid; i < to; i += 256 * W) {
       const f32x4 u = *(const f32x4*)(ring + buf * HALF + i);
       top = fmaxf(top, fmaxf(fmaxf(fabsf(u[0]), fabsf(u[1])), fmaxf(fabsf(u[2]), fabsf(u[3]))));
@@ -659,9 +676,10 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
   };
   for (int gi = 0; gi < o.group; ++gi) {
     const float rate = scalar(p.rate[o.h0 + gi]);
-    fast = rate < p.fast;
-    looked |= fast;
-    if (fast) top = fmaxf(top, own.largest());
+    if (LOOK) {
+      fast = rate < p.fast;
+      looked |= fast;
+    }
     const int by = here ? BACK ? leaves(end, since, o.s0, r) : comes(since, o.s0, r) : -1;
     const float coef = by < 0 ? 0.0f : p.by_state * power(rate, by);
 #pragma unroll
@@ -686,27 +704,36 @@ __device__ __forceinline__ void walk_tiles(const PairsArgs& p, const Sum& s, int
     }
     for (; t0 < o.to; t0 += kTile) arrive(0, HALF);
   }
-  bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here && s.rows.p, s.nz, g);
+  bool lossy = false;
   if (looked) {
-    if (top >= p.limit) large = 1;
+    join_max(most[0], top, p.large);
     __syncthreads();
-    fine = fine && !large;
+    if (__builtin_expect((most[0] | most[1]) != 0, 0)) {
+      // of 128 pairs: a dot product times two more operands at most (the state's products are fewer and have one)
+      const double row = fmaxf(p.large, __uint_as_float(most[1])), x = fmaxf(fmaxf(p.large, 1.0f), __uint_as_float(most[0]));
+      const double lost = 0x1p-126 * kSeg * fmax(s.n * row, 1.0) * x * x * fmaxf(1.0f, p.by_pair);
+      lossy = __any(lost > 0x1p-60 && own.smallest(s.nz, g) < lost * 0x1p30);
+    }
   }
-  if (__builtin_expect(!fine, 0)) {
+  const bool fine = own.store(s.out.p + o.b * s.out.b + o.head * s.out.h + (int64_t)r * s.out.t, r < T, here && s.rows.p, s.nz, g);
+  if (__builtin_expect(!fine || lossy, 0)) {
     loads_done();                  // the rows are written before they are written again
     plain_rows<BACK>(p, s, o, w0, since);
   }
 }
-template <int DK, int DV, int W, bool BACK, bool WIDE>   // features of keys and of values, padded
+// Features of keys and of values, padded. LOOK: a head's decay is fast (kernels of their own: the look in all of them took 2 to 5 % of
+// layers of 32 and 64 features without fast decays).
+template <int DK, int DV, int W, bool BACK, bool WIDE, bool LOOK>
 __global__ __launch_bounds__(64 * W, W == 8 || DK + DV <= 128 ? 4 : 2) void linear_tiles(PairsArgs p) {
   __shared__ __align__(16) Ring<DK, DV> ring;
-  __shared__ int since[kSeg], large;
+  __shared__ int since[kSeg];
+  __shared__ uint32_t most[2];     // sizes of tiles' and of rows' operands
   // both sums of a place run one after the other on one XCD (blocks go to the 8 XCDs in turn), whose L2 then has their tiles
   const int id = blockIdx.x / 8, unit = (id / p.sums) * 8 + blockIdx.x % 8;
   if (unit >= p.blocks * p.B * p.heads) return;
   const Sum& s = p.sum[id % p.sums];
-  if (s.across) walk_tiles<DV, DK, W, BACK, WIDE, true>(p, s, unit, ring.tile[0], since, large);
-  else walk_tiles<DK, DV, W, BACK, WIDE, false>(p, s, unit, ring.tile[0], since, large);
+  if (s.across) walk_tiles<DV, DK, W, BACK, WIDE, LOOK, true>(p, s, unit, ring.tile[0], since, most);
+  else walk_tiles<DK, DV, W, BACK, WIDE, LOOK, false>(p, s, unit, ring.tile[0], since, most);
 }
 
 // Sums of what each query head gave a key head's rows, in the heads' order. Bound by memory (38 MB in 10 us).
@@ -899,7 +926,7 @@ void pairs(PairsArgs p, const LinearDesc& a, const float* at, const float* edge,
   p.by_pair = a.scale;
   p.by_state = BACK ? 1.0f : a.scale;
   p.fast = (-100 - std::min(0.0f, std::log2(a.scale))) / kSeg;
-  p.limit = 0x1p16f / std::max(1.0f, a.scale);
+  p.large = 0x1p17f / std::cbrt(std::max(1.0f, a.scale));   // 128 pairs of 128 products of three of them: 2^-60 lost at most
   p.rate = a.rate;
   p.any = a.q.p;
   bool wide = a.D % 4 == 0 && a.Dv % 4 == 0 && wide_rows(a.q) && (((uintptr_t)at | (uintptr_t)edge) & 15) == 0;
@@ -913,12 +940,16 @@ void pairs(PairsArgs p, const LinearDesc& a, const float* at, const float* edge,
   p.blocks = (a.T + rows - 1) / rows;
   const int64_t units = (int64_t)p.blocks * p.B * p.heads;
   const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.sums));
-  auto launch = [&](auto K, auto V, auto wide) {
-    if (rows == 64) klaunch(linear_tiles<K.value, V.value, 4, BACK, wide.value>, grid, dim3(256), 0, st, p);
-    else klaunch(linear_tiles<K.value, V.value, 8, BACK, wide.value>, grid, dim3(512), 0, st, p);
+  auto launch = [&](auto K, auto V, auto wide, auto look) {
+    if (rows == 64) klaunch(linear_tiles<K.value, V.value, 4, BACK, wide.value, look.value>, grid, dim3(256), 0, st, p);
+    else klaunch(linear_tiles<K.value, V.value, 8, BACK, wide.value, look.value>, grid, dim3(512), 0, st, p);
   };
-  if (wide) by_sizes(a, [&](auto K, auto V) { launch(K, V, std::true_type()); });
-  else by_larger(a, [&](auto P) { launch(P, P, std::false_type()); });
+  auto sized = [&](auto look) {
+    if (wide) by_sizes(a, [&](auto K, auto V) { launch(K, V, std::true_type(), look); });
+    else by_larger(a, [&](auto P) { launch(P, P, std::false_type(), look); });
+  };
+  if (a.least < p.fast) sized(std::true_type());
+  else sized(std::false_type());
 }
 
 }  // namespace

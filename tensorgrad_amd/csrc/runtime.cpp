@@ -4125,6 +4125,7 @@ std::function<tgk::LinearDesc()> Runtime::linear_binder(int i, const tgk::Linear
     a.state = s >= 0 ? (const float*)dptr(s) : nullptr;
     a.documents = doc >= 0 ? (const int32_t*)dptr(doc) : nullptr;
     a.lengths = len >= 0 ? (const int32_t*)dptr(len) : nullptr;
+    a.least = *std::min_element(rate.begin(), rate.end());
     if (!plan_only_) a.rate = (const float*)dev_table("decay " + std::to_string(i), rate.data(), rate.size() * sizeof(float));
     return a;
   };

@@ -78,6 +78,7 @@ struct LinearDesc {
   const int32_t* documents;  // [B, T] or null
   const int32_t* lengths;    // [B] or null
   const float* rate;         // [H], log2(decay)
+  float least;               // the least of them
   float scale;
 };
 struct LinearGradDesc {

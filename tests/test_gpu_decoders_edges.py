@@ -189,3 +189,27 @@ def test_linear_large_values_outlast_small_weights(shape, where):
     else:
         a[where][0, 0, T - 2 if where in ('q', 'dy') else 1] *= f32(2.0 ** 116)
     check_linear(a, lam, what=where)
+
+
+@pytest.mark.parametrize('size', [2.0 ** 20, 2.0 ** 40])
+@pytest.mark.parametrize('gone', [None, 'q', 'v'])
+def test_linear_large_values_of_one_size(size, gone):
+    """Also where rows or columns of zeros are among them."""
+    a = linear_inputs(1, 4, 2, 300, 64, 32, 109, True)
+    for n in a:
+        a[n] *= f32(size)
+    a['dy'] /= f32(size)
+    if gone == 'q':
+        a['q'][:, :, ::3] = 0
+    elif gone == 'v':
+        a['v'][..., ::3] = 0
+        a['state'][..., ::3] = 0
+    check_linear(a, [0.4, 0.1, 0.45, 0.9])
+
+
+def test_linear_one_column_of_early_values_is_large():
+    a = linear_inputs(1, 2, 1, 200, 32, 32, 110)
+    a['v'][0, 0, 3, 5] *= np.float32(2.0 ** 116)
+    a['v'][0, 0, 3, 6] = 2.0 ** 90
+    a['v'][0, 0, 4:, 6] *= np.float32(2.0 ** -30)
+    check_linear(a, [0.4, 0.45])
