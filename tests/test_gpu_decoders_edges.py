@@ -213,3 +213,46 @@ def test_linear_one_column_of_early_values_is_large():
     a['v'][0, 0, 3, 6] = 2.0 ** 90
     a['v'][0, 0, 4:, 6] *= np.float32(2.0 ** -30)
     check_linear(a, [0.4, 0.45])
+
+
+@pytest.mark.parametrize('T,Dk', [(6, 32), (100, 64), (300, 64), (420, 20), (300, 96)])
+@pytest.mark.parametrize('kind', ['documents', 'lengths', 'both'])
+@pytest.mark.parametrize('garbage', [np.inf, np.nan, 3e38])
+def test_linear_masks_under_fast_decays(T, Dk, kind, garbage):
+    """What is not there is garbage of any size, and no result shows it."""
+    a = linear_inputs(3, 4, 2, T, Dk, Dk, 111, True)
+    hidden = np.zeros((3, T), bool)
+    if kind != 'lengths':
+        a['documents'] = np.repeat(np.arange((T + 36) // 37, dtype=np.int32), 37)[:T][None].repeat(3, 0).copy()
+        a['documents'][0, T // 2:T // 2 + 5] = -1
+        a['documents'][2, :3] = -2
+        hidden |= a['documents'] < 0
+    if kind != 'documents':
+        a['lengths'] = np.array([T, T - T // 3, 0], np.int32)
+        hidden |= np.arange(T)[None] >= a['lengths'][:, None]
+    clean = {n: x.copy() for n, x in a.items()}
+    for b in range(3):
+        for n in ('q', 'k', 'v', 'dy'):
+            a[n][b, :, hidden[b]] = garbage
+            clean[n][b, :, hidden[b]] = 0
+    lam = [0.4, 0.003, 1e-30, 0.9]
+    want, tol = D.linear(**clean, decay=lam)
+    got = run_linear(a, lam)
+    for n in got:
+        R.check(got[n], want[n], tol[n], n)
+    assert not got['y'][np.broadcast_to(hidden[:, None], got['y'].shape[:3])].any()
+
+
+def test_linear_results_under_fast_decays_repeat():
+    """Also those that are computed again: a batch with an infinity, then without, then with it."""
+    a = linear_inputs(2, 4, 2, 300, 64, 64, 112, True)
+    lam = [0.4, 0.3, 0.9, 0.999]
+    bad = {n: x.copy() for n, x in a.items()}
+    bad['v'][0, 1, 17, 3] = np.inf
+    bad['k'][1, 0, 5] *= np.float32(2.0 ** 100)
+    first, clean = run_linear(bad, lam), run_linear(a, lam)
+    check_linear(a, lam)
+    for n, x in run_linear(bad, lam).items():
+        assert np.array_equal(x, first[n], equal_nan=True), n
+    for n, x in run_linear(a, lam).items():
+        assert np.array_equal(x, clean[n]), n
