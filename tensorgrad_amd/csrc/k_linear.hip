@@ -955,12 +955,12 @@ void pairs(PairsArgs p, const LinearDesc& a, const float* at, const float* edge,
 }  // namespace
 
 int64_t linear_workspace_bytes(const LinearDesc& a) {
-  if (a.T <= kSteps) return 0;
+  if (a.T <= kSteps && !a.borders) return 0;
   return stay_bytes(a) + (a.borders ? 0 : states_bytes(a));
 }
 
 void linear(const LinearDesc& a, void* work, hipStream_t st) {
-  if (a.T <= kSteps) {
+  if (a.T <= kSteps && !a.borders) {   // the steps make no states at borders
     const StepsArgs s{a, a.Dv % 4 == 0 && ((uintptr_t)a.state & 15) == 0 && ((uintptr_t)a.last & 15) == 0};
     return by_larger(a, [&](auto P) { klaunch(linear_steps<P.value>, dim3((unsigned)(a.B * a.H)), dim3(256), 0, st, s); });
   }

@@ -9,7 +9,7 @@ import _sequence as R
 from tensorgrad_amd import ops as O
 from tensorgrad_amd.compile import compile_forward
 from tensorgrad_amd.module import Module
-from test_gpu_decoders import check_linear, check_sample, f32, linear_inputs, rng, run_linear
+from test_gpu_decoders import check_linear, check_sample, f32, forward, linear_inputs, rng, run_linear
 
 pytestmark = pytest.mark.gpu
 
@@ -256,3 +256,51 @@ def test_linear_results_under_fast_decays_repeat():
         assert np.array_equal(x, first[n], equal_nan=True), n
     for n, x in run_linear(a, lam).items():
         assert np.array_equal(x, clean[n]), n
+
+
+@pytest.mark.parametrize('T', [1, 8, 9, 128])
+def test_linear_states_before_segments_of_one_segment(T):
+    """The op that keeps them for the gradients, in a document that asks for it where there is one segment: the first state."""
+    a = linear_inputs(2, 4, 2, T, 32, 16, 113, True, grad=False)
+
+    def fn(i):
+        out = O.linear_attention(i['q'], i['k'], i['v'], [0.9] * 4, state=i['state'])
+        f = O._linear_fields('borders', i['q'], i['k'], i['v'], [0.9] * 4, None, i['state'], None, None)
+        return [*out, O.add_op(O.current_graph(), 'linear_attention_borders', (1, 2, 4, 32, 16), 'f32', 'borders', f)]
+    y, state, borders = forward(fn, a)
+    want, tol = D.linear(**a, decay=[0.9] * 4)
+    R.check(y, want['y'], tol['y'], 'y')
+    R.check(state, want['state'], tol['state'], 'state')
+    assert np.array_equal(borders[0], a['state'])
+
+
+@pytest.mark.parametrize('start', [1, 4])
+@pytest.mark.parametrize('axis', [2, 3])
+def test_operands_that_are_parts_of_others(axis, start):
+    """Rows and features of larger tensors from an odd or an aligned place on, read where they lie."""
+    T, size = 150, 24
+    r = rng(axis, start, 114)
+    big = {n: f32(r.standard_normal((2, h, T + 7 * (axis == 2), size + 8 * (axis == 3)))) for n, h in (('q', 4), ('k', 2), ('v', 2), ('dy', 4))}
+    cut = lambda x: O.narrow(x, axis, start, T if axis == 2 else size)  # noqa: E731
+    part = {n: np.ascontiguousarray(x.take(np.arange(start, start + (T if axis == 2 else size)), axis)) for n, x in big.items()}
+
+    def linear(i):
+        q, k, v, dy = (cut(i[n]) for n in ('q', 'k', 'v', 'dy'))
+        return [*O.linear_attention(q, k, v, [0.9] * 4), *O.linear_attention_grad(q, k, v, dy, [0.9] * 4)]
+
+    def window(i):
+        q, k, v, dy = (cut(i[n]) for n in ('q', 'k', 'v', 'dy'))
+        y = O.attention(q, k, v, window=40, sinks=3)
+        return [y, *O.attention_grad(q, k, v, y, dy, window=40, sinks=3)]
+    for fn, (want, tol), names in ((linear, D.linear(part['q'], part['k'], part['v'], [0.9] * 4, dy=part['dy']), ('y', 'state', 'dq', 'dk', 'dv')),
+                                   (window, D.attention(part['q'], part['k'], part['v'], part['dy'], window=40, sinks=3), ('y', 'dq', 'dk', 'dv'))):
+        for n, x in zip(names, forward(fn, big)):
+            R.check(x, want[n], tol[n], n)
+
+
+@pytest.mark.parametrize('V', FORMS)
+def test_sample_of_a_part_of_the_vocabulary(V):
+    r = rng(V, 115)
+    x, u = f32(r.standard_normal((6, V + 3))), f32(r.random(6))
+    got = forward(lambda i: [O.sample(O.narrow(i['x'], 1, 3, V), i['u'], top_p=0.9)], dict(x=x, u=u))[0]
+    assert got.tolist() == [D.sample(x[b, 3:], float(u[b]), top_p=0.9) for b in range(6)]
