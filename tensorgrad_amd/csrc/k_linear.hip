@@ -19,9 +19,9 @@
 // whose k of step q is row 4 g + q, which is where the weights stand as they come out of the first product.
 //
 // What a row does not see has weight 0, and 0 times an infinity or NaN is NaN; a dot product may be infinite where no state is: rows
-// whose result is not finite are computed again pair by pair in 64 bits, from what they see alone. So are rows of
-// which weights below f32's range, 2^-126, may lose something that counts: under a decay whose weights in a segment fall below 2^-100,
-// where 2^-126 times the largest products that a block's operands allow is above 2^-60 and above 2^-30 of a result of theirs.
+// whose result is not finite are computed again pair by pair in 64 bits, from what they see alone. So are rows of which weights below
+// f32's range, 2^-126, may lose something that counts: under a decay whose weights in a segment fall below 2^-100, where 2^-126 times
+// the largest products that a block's operands allow is above 2^-60 and above 2^-30 of a result of theirs.
 #include <algorithm>
 #include <cmath>
 
